@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define SLK_ABI_VERSION 18
+#define SLK_ABI_VERSION 19
 
 #if defined(__GNUC__)
 #define SLK_API __attribute__((visibility("default")))
@@ -714,6 +714,82 @@ SLK_API int slk_rigl_mfma_probe(const uint16_t* A, const uint16_t* B, const floa
  * one fma.                                                                  */
 SLK_API int slk_dense_mfma_probe(const float* A, const float* B, const float* C, float* D,
                                  int64_t n, void* stream);
+
+/* ─────────── the training step around the sparse layers ────────────
+ * No counterpart in the reference (its users call torch's optimizer, norm
+ * and loss).                                                                */
+
+/* Element types of the entry points below that take more than one.         */
+enum slk_dtype { SLK_F32 = 0, SLK_BF16 = 1 };
+
+/* Elements that share one float32 scale of an 8-bit moment: element i of a
+ * tensor has scale i / SLK_Q8_BLOCK, the block's largest magnitude.         */
+#define SLK_Q8_BLOCK 256
+
+/* One tensor of slk_adamw: n elements of param and grad (the call's dtype),
+ * n of each moment: float32 (state_bits 32; the scales are not read), or
+ * 8-bit codes (int8 exp_avg, uint8 exp_avg_sq) with ceil(n / SLK_Q8_BLOCK)
+ * scales each. Any alignment that the element types allow; arrays that are
+ * 16-byte aligned (8 for bf16, 4 for codes) go four elements a load.        */
+typedef struct slk_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int64_t n;
+} slk_adamw_tensor;
+
+/* Scalars of slk_adamw. step is 1 at the first step. step_dev and lr_dev
+ * (device float32, may be NULL) replace step and lr where these live on the
+ * device, as in a captured graph.                                           */
+typedef struct slk_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay, step;
+    const float* step_dev;
+    const float* lr_dev;
+} slk_adamw_args;
+
+/* One AdamW step, in place, of n_tensors tensors in ceil(n_tensors / 56)
+ * launches (tensors_host and args_host are read before the call returns):
+ *   m = beta1·m + (1 - beta1)·g,  v = beta2·v + (1 - beta2)·g²,
+ *   p = (1 - lr·weight_decay)·p
+ *       - lr / (1 - beta1^step) · m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * All arithmetic in float32; a bf16 parameter is rounded once, and 8-bit
+ * moments are rounded to codes after the parameter took the unrounded ones.
+ * The arrays of one call must not overlap.                                  */
+SLK_API int slk_adamw(const slk_adamw_tensor* tensors_host, int64_t n_tensors, int dtype,
+                      int state_bits, const slk_adamw_args* args_host, void* stream);
+
+/* 8-bit moments to float32 and back. is_signed: the first moment's map
+ * (int8 codes, x = (q/127)·|q/127|·scale), else the second's (uint8 codes,
+ * x = (q/255)^4·scale, x >= 0). n elements, ceil(n / SLK_Q8_BLOCK) scales.  */
+SLK_API int slk_q8_decode(const void* codes, const float* scales, int64_t n, int is_signed,
+                          float* out, void* stream);
+SLK_API int slk_q8_encode(const float* x, int64_t n, int is_signed, void* codes, float* scales,
+                          void* stream);
+
+/* A state of slk_carry_slots: total entries, float32 or 8-bit codes with
+ * their scales. dst must not be src.                                        */
+enum slk_state_kind { SLK_STATE_F32 = 0, SLK_STATE_Q8_SIGNED = 1, SLK_STATE_Q8_UNSIGNED = 2 };
+#define SLK_CARRY_STATES 4
+typedef struct slk_carry_state {
+    const void* src;
+    const float* src_scale;
+    void* dst;
+    float* dst_scale;
+    int32_t kind;
+} slk_carry_state;
+
+/* Moves per-slot states of a padded-CSR matrix to its topology after a
+ * rewrite (slk_drop_grow, slk_rigl_finish, rewrite_row), which keeps
+ * row_start: the live slot of (row, column) takes the state that the same
+ * (row, column) had before, a grown connection and every padding slot 0.
+ * old_cols / new_cols: total entries, each row's live ones ascending.       */
+SLK_API int slk_carry_slots(const int32_t* row_start, int64_t nrows, int64_t total,
+                            const int32_t* old_cols, const int32_t* old_nnz,
+                            const int32_t* new_cols, const int32_t* new_nnz,
+                            const slk_carry_state* states_host, int64_t n_states, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,10 +20,12 @@ from .layout import PaddedCSR
 from .ops import spmm
 from .nn import SparseLinear
 from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Static
-from . import _lib, nn, ops, router
+from . import _lib, nn, ops, optim, router
+from .optim import AdamW
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
-           "DynamicSparsityAlgorithm", "SET", "RigL", "install_as_sparselab"]
+           "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
+           "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

@@ -21,7 +21,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libsparsecore_amd.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 SLK_OK, SLK_EINVAL, SLK_EDEVICE = 0, 1, 2
 SLK_DW_SIMD, SLK_DW_SCALAR = 0, 1
@@ -81,6 +81,10 @@ EXPORTS = (
     "slk_strip_build",
     "slk_strip_layout_bytes",
     "slk_sddmm_strips",
+    "slk_adamw",
+    "slk_q8_decode",
+    "slk_q8_encode",
+    "slk_carry_slots",
 )
 
 RIGL_INFO_BYTES = 32  # per row, slk_rigl_count's info
@@ -98,6 +102,13 @@ FORCED_KNOBS: set[str] = set()  # knobs that set_tuning holds off their automati
 BIN_MAX_CHUNKS = 960  # SLK_BIN_MAX_CHUNKS
 
 SEG_GROUP = 128  # SLK_SEG_GROUP
+
+SLK_F32, SLK_BF16 = 0, 1
+DTYPES = {torch.float32: SLK_F32, torch.bfloat16: SLK_BF16}
+
+Q8_BLOCK = 256  # SLK_Q8_BLOCK
+STATE_F32, STATE_Q8_SIGNED, STATE_Q8_UNSIGNED = 0, 1, 2
+CARRY_STATES = 4  # SLK_CARRY_STATES
 
 NARROW_MAX_ROWS = 64        # SLK_NARROW_MAX_ROWS
 NARROW_MAX_CAPACITY = 8192  # SLK_NARROW_MAX_CAPACITY
@@ -167,6 +178,47 @@ class StripView(ctypes.Structure):
         ("slots", ctypes.c_int64),
         ("per_wave", ctypes.c_int64),
         ("parts", ctypes.c_int64),
+    ]
+
+
+class AdamTensor(ctypes.Structure):
+    """Mirror of ``slk_adamw_tensor`` (include/sparsecore_amd.h)."""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p),
+        ("exp_avg_scale", ctypes.c_void_p),
+        ("exp_avg_sq_scale", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+    ]
+
+
+class AdamArgs(ctypes.Structure):
+    """Mirror of ``slk_adamw_args`` (include/sparsecore_amd.h)."""
+
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("step", ctypes.c_double),
+        ("step_dev", ctypes.c_void_p),
+        ("lr_dev", ctypes.c_void_p),
+    ]
+
+
+class CarryState(ctypes.Structure):
+    """Mirror of ``slk_carry_state`` (include/sparsecore_amd.h)."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p),
+        ("src_scale", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("dst_scale", ctypes.c_void_p),
+        ("kind", ctypes.c_int32),
     ]
 
 
@@ -251,6 +303,12 @@ def _declare(lib) -> None:
                                   ctypes.POINTER(_i64)]
     lib.slk_bin_build.argtypes = [_csrp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]
     lib.slk_rigl_mfma_probe.argtypes = [_vp, _vp, _vp, _vp, _i64, _vp]
+    lib.slk_adamw.argtypes = [_vp, _i64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(AdamArgs),
+                              _vp]
+    lib.slk_q8_decode.argtypes = [_vp, _vp, _i64, ctypes.c_int, _vp, _vp]
+    lib.slk_q8_encode.argtypes = [_vp, _i64, ctypes.c_int, _vp, _vp, _vp]
+    lib.slk_carry_slots.argtypes = [_vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                                    ctypes.POINTER(CarryState), _i64, _vp]
     sized = ("slk_last_error", "slk_abi_version", "slk_transpose_workspace_bytes",
              "slk_drop_grow_workspace_bytes", "slk_rigl_bound_factor", "slk_rigl_partial_factor",
              "slk_dense_grad_approx_workspace_bytes",
@@ -744,6 +802,40 @@ def rigl_finish(view: CsrView, thr: torch.Tensor, G: torch.Tensor, G_code: torch
                                 ptr(dY), ptr(X), dY.shape[1], ptr(info), amb_off.data_ptr(),
                                 ptr(amb_ws), amb_ws.numel(), ptr(ws), ws.numel(),
                                 removed.data_ptr(), stream_of(removed))
+    if rc:
+        _raise(rc)
+
+
+def adamw(table, n: int, dtype: int, bits: int, args: AdamArgs, stream: int) -> None:
+    """One AdamW step of the n tensors of a table of slk_adamw_tensor words (a
+    contiguous int64 array of n x 7, read before the call returns)."""
+    rc = load().slk_adamw(table.ctypes.data, n, dtype, bits, ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def q8_decode(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> None:
+    rc = load().slk_q8_decode(ptr(codes), ptr(scales), codes.numel(), codes.dtype == torch.int8,
+                              ptr(out), stream_of(out))
+    if rc:
+        _raise(rc)
+
+
+def q8_encode(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    rc = load().slk_q8_encode(ptr(x), x.numel(), codes.dtype == torch.int8, ptr(codes),
+                              ptr(scales), stream_of(codes))
+    if rc:
+        _raise(rc)
+
+
+def carry_slots(row_start: torch.Tensor, old_cols: torch.Tensor, old_nnz: torch.Tensor,
+                new_cols: torch.Tensor, new_nnz: torch.Tensor, states: list) -> None:
+    """states: (src, src_scale, dst, dst_scale, kind) each."""
+    table = (CarryState * max(1, len(states)))(
+        *(CarryState(ptr(a), ptr(sa), ptr(b), ptr(sb), kind) for a, sa, b, sb, kind in states))
+    rc = load().slk_carry_slots(ptr(row_start), row_start.numel(), old_cols.numel(),
+                                ptr(old_cols), ptr(old_nnz), ptr(new_cols), ptr(new_nnz), table,
+                                len(states), stream_of(row_start))
     if rc:
         _raise(rc)
 

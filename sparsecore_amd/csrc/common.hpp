@@ -78,6 +78,12 @@ __device__ __forceinline__ int64_t wave_id() {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// bfloat16 bits to float32 (exact) and back (round to nearest, ties to even)
+__device__ __forceinline__ float bf16_to_f32(uint32_t bits) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ uint16_t f32_to_bf16(float x) {
+    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+}
+
 // f(std::integral_constant<int, j>{}) for j = 0..N-1, unrolled at compile time
 // (so array indexes derived from j are constants, never private memory).
 template <class F, int... J>
