@@ -791,6 +791,46 @@ SLK_API int slk_carry_slots(const int32_t* row_start, int64_t nrows, int64_t tot
                             const int32_t* new_cols, const int32_t* new_nnz,
                             const slk_carry_state* states_host, int64_t n_states, void* stream);
 
+/* Arguments of slk_norm_forward and slk_norm_backward: what stands between
+ * two blocks of a model with n tokens of d features,
+ *   r = x + scale · gate ∘ post(branch),   y = pre(r),
+ * with pre the norm of weight and bias and post, if post_weight is given, the
+ * norm of post_weight and post_bias over each token's features: LayerNorm
+ * (layer = 1) or RMSNorm (layer = 0; biases are NULL). All arrays of
+ * features have the type dtype; arithmetic is float32, each result rounded
+ * once. Arrays are n x d, token by token, but branch, y, dy and dbranch are
+ * feature by feature (d x n, as the sparse layers keep activations) where
+ * branch_cols (branch, dbranch) or y_cols (y, dy) is set: d at most
+ * SLK_NORM_COLS_MAX then.
+ *   branch     NULL: y = pre(x), r is not written
+ *   gate       gate_rows x d: row i serves the i-th n / gate_rows consecutive
+ *              tokens (1: one gate for all, n: one each); NULL: none
+ *   stats      n x 4 floats: mean and 1/deviation of pre, of post; forward
+ *              writes them if not NULL, backward reads them
+ * Backward: dr (NULL: zeros) and dy (NULL: zeros, no gradient of weight or
+ * bias) in, r (x where there is no branch) and the forward's arrays in; every
+ * gradient that is not NULL is written. workspace: device memory of
+ * slk_norm_workspace_bytes.                                                  */
+#define SLK_NORM_MAX_D 16384
+#define SLK_NORM_COLS_MAX 1024
+typedef struct slk_norm {
+    int64_t n, d, gate_rows;
+    const void *x, *branch, *gate, *weight, *bias, *post_weight, *post_bias;
+    void *r, *y;
+    float* stats;
+    const void *dr, *dy;
+    void *dx, *dbranch, *dgate, *dweight, *dbias, *dpost_weight, *dpost_bias;
+    void* workspace;
+    int64_t workspace_bytes;
+    double scale, eps;
+    int32_t dtype, layer, branch_cols, y_cols;
+} slk_norm;
+
+/* Two launches at most beside the first; sums over tokens in a fixed order.  */
+SLK_API int64_t slk_norm_workspace_bytes(const slk_norm* args_host);
+SLK_API int slk_norm_forward(const slk_norm* args_host, void* stream);
+SLK_API int slk_norm_backward(const slk_norm* args_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,12 +20,13 @@ from .layout import PaddedCSR
 from .ops import spmm
 from .nn import SparseLinear
 from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Static
-from . import _lib, nn, ops, optim, router
+from .norm import residual_norm
 from .optim import AdamW
+from . import _lib, nn, ops, optim, router
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
            "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
-           "install_as_sparselab"]
+           "residual_norm", "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

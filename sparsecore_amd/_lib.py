@@ -85,6 +85,9 @@ EXPORTS = (
     "slk_q8_decode",
     "slk_q8_encode",
     "slk_carry_slots",
+    "slk_norm_workspace_bytes",
+    "slk_norm_forward",
+    "slk_norm_backward",
 )
 
 RIGL_INFO_BYTES = 32  # per row, slk_rigl_count's info
@@ -109,6 +112,9 @@ DTYPES = {torch.float32: SLK_F32, torch.bfloat16: SLK_BF16}
 Q8_BLOCK = 256  # SLK_Q8_BLOCK
 STATE_F32, STATE_Q8_SIGNED, STATE_Q8_UNSIGNED = 0, 1, 2
 CARRY_STATES = 4  # SLK_CARRY_STATES
+
+NORM_MAX_D = 16384     # SLK_NORM_MAX_D
+NORM_COLS_MAX = 1024   # SLK_NORM_COLS_MAX
 
 NARROW_MAX_ROWS = 64        # SLK_NARROW_MAX_ROWS
 NARROW_MAX_CAPACITY = 8192  # SLK_NARROW_MAX_CAPACITY
@@ -222,6 +228,20 @@ class CarryState(ctypes.Structure):
     ]
 
 
+class Norm(ctypes.Structure):
+    """Mirror of ``slk_norm`` (include/sparsecore_amd.h)."""
+
+    _fields_ = (
+        [(k, ctypes.c_int64) for k in ("n", "d", "gate_rows")]
+        + [(k, ctypes.c_void_p) for k in (
+            "x", "branch", "gate", "weight", "bias", "post_weight", "post_bias", "r", "y",
+            "stats", "dr", "dy", "dx", "dbranch", "dgate", "dweight", "dbias", "dpost_weight",
+            "dpost_bias", "workspace")]
+        + [("workspace_bytes", ctypes.c_int64), ("scale", ctypes.c_double),
+           ("eps", ctypes.c_double)]
+        + [(k, ctypes.c_int32) for k in ("dtype", "layer", "branch_cols", "y_cols")])
+
+
 _lib = None
 _load_error: str | None = None
 
@@ -309,11 +329,17 @@ def _declare(lib) -> None:
     lib.slk_q8_encode.argtypes = [_vp, _i64, ctypes.c_int, _vp, _vp, _vp]
     lib.slk_carry_slots.argtypes = [_vp, _i64, _i64, _vp, _vp, _vp, _vp,
                                     ctypes.POINTER(CarryState), _i64, _vp]
+    normp = ctypes.POINTER(Norm)
+    lib.slk_norm_workspace_bytes.restype = _i64
+    lib.slk_norm_workspace_bytes.argtypes = [normp]
+    lib.slk_norm_forward.argtypes = [normp, _vp]
+    lib.slk_norm_backward.argtypes = [normp, _vp]
     sized = ("slk_last_error", "slk_abi_version", "slk_transpose_workspace_bytes",
              "slk_drop_grow_workspace_bytes", "slk_rigl_bound_factor", "slk_rigl_partial_factor",
              "slk_dense_grad_approx_workspace_bytes",
              "slk_seg_list_capacity", "slk_seg_list_workspace_bytes", "slk_quad_windows",
-             "slk_quad_chunks", "slk_quad_halves", "slk_strip_layout_bytes")
+             "slk_quad_chunks", "slk_quad_halves", "slk_strip_layout_bytes",
+             "slk_norm_workspace_bytes")
     for name in EXPORTS:
         if name not in sized:
             getattr(lib, name).restype = ctypes.c_int
@@ -836,6 +862,22 @@ def carry_slots(row_start: torch.Tensor, old_cols: torch.Tensor, old_nnz: torch.
     rc = load().slk_carry_slots(ptr(row_start), row_start.numel(), old_cols.numel(),
                                 ptr(old_cols), ptr(old_nnz), ptr(new_cols), ptr(new_nnz), table,
                                 len(states), stream_of(row_start))
+    if rc:
+        _raise(rc)
+
+
+def norm_workspace_bytes(args: Norm) -> int:
+    return int(load().slk_norm_workspace_bytes(ctypes.byref(args)))
+
+
+def norm_forward(args: Norm, stream: int) -> None:
+    rc = load().slk_norm_forward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def norm_backward(args: Norm, stream: int) -> None:
+    rc = load().slk_norm_backward(ctypes.byref(args), stream)
     if rc:
         _raise(rc)
 

@@ -11,6 +11,7 @@
 // serves kAdamTensors tensors; a lane takes four consecutive elements with
 // one 16-byte load an array; a wave takes SLK_Q8_BLOCK elements, a whole
 // block of 8-bit codes, whose new scale is one wave reduction.
+#include "elem.hpp"
 #include "q8.hpp"
 
 namespace slk {
@@ -25,7 +26,6 @@ struct AdamTable {
     slk_adamw_tensor t[kAdamTensors];
     uint32_t first[kAdamTensors];  // first workgroup of each tensor
     int32_t n;
-    uint32_t vec;  // unused bits kept for alignment
     uint64_t aligned;  // bit i: tensor i's arrays take four elements a load
 };
 
@@ -36,51 +36,6 @@ struct AdamCoef {
     const float* step;
     const float* lr;
     double lr_host, wd, log_b1, log_b2, step_host;
-};
-
-struct F32 {
-    static constexpr int kBytes = 4;
-    using Raw = float;
-    static __device__ __forceinline__ float load(const void* p, int64_t i) {
-        return static_cast<const float*>(p)[i];
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t i, float v) {
-        static_cast<float*>(p)[i] = v;
-    }
-    static __device__ __forceinline__ void load4(const void* p, int64_t i, float (&v)[4]) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = x[j];
-    }
-    static __device__ __forceinline__ void store4(void* p, int64_t i, const float (&v)[4]) {
-        f32x4 x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = v[j];
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = x;
-    }
-};
-
-struct BF16 {
-    static constexpr int kBytes = 2;
-    static __device__ __forceinline__ float load(const void* p, int64_t i) {
-        return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t i, float v) {
-        static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
-    }
-    static __device__ __forceinline__ void load4(const void* p, int64_t i, float (&v)[4]) {
-        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-        v[0] = bf16_to_f32(x.x & 0xffffu);
-        v[1] = bf16_to_f32(x.x >> 16);
-        v[2] = bf16_to_f32(x.y & 0xffffu);
-        v[3] = bf16_to_f32(x.y >> 16);
-    }
-    static __device__ __forceinline__ void store4(void* p, int64_t i, const float (&v)[4]) {
-        uint2 x;
-        x.x = f32_to_bf16(v[0]) | (static_cast<uint32_t>(f32_to_bf16(v[1])) << 16);
-        x.y = f32_to_bf16(v[2]) | (static_cast<uint32_t>(f32_to_bf16(v[3])) << 16);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = x;
-    }
 };
 
 // four codes of a block: element i, i + 1, i + 2, i + 3 (those below n)
@@ -312,10 +267,6 @@ __global__ __launch_bounds__(kAdamThreads) void carry_kernel(
     }
 }
 
-bool aligned_to(const void* p, uintptr_t bytes) {
-    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
-}
-
 }  // namespace
 }  // namespace slk
 
@@ -373,7 +324,6 @@ extern "C" int slk_adamw(const slk_adamw_tensor* tensors_host, int64_t n_tensors
     }
     AdamTable tab;
     tab.n = 0;
-    tab.vec = 0;
     tab.aligned = 0;
     int64_t groups = 0;
     auto launch = [&]() -> int {

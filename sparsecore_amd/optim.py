@@ -319,8 +319,6 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(module, SparseLinear):
             self._attached[module._values] = _Attached(module)
 
-    __call__ = attach
-
     def _follow(self, p) -> None:
         at = self._attached[p]
         csr = at.layer._csr
