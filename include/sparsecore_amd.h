@@ -831,6 +831,42 @@ SLK_API int64_t slk_norm_workspace_bytes(const slk_norm* args_host);
 SLK_API int slk_norm_forward(const slk_norm* args_host, void* stream);
 SLK_API int slk_norm_backward(const slk_norm* args_host, void* stream);
 
+/* Arguments of slk_linear_ce_*: the head and its softmax cross entropy for n
+ * tokens of d features over v rows of vocabulary, logits never stored:
+ *   z = hidden·weight^T,  loss_i = log(sum_j exp(z_ij)) - z_i,target[i].
+ * hidden n x d, weight v x d (contiguous, dtype), target n int64. A token with
+ * target ignore_index has loss 0, no gradient, and reaches nothing else; one
+ * with any other target outside [0, v) has loss NaN (its softmax's gradient).
+ *   reduction  SLK_REDUCE_NONE: loss has n entries, upstream n; SUM, MEAN
+ *              (over the tokens not ignored; NaN if there is none): 1 each
+ *   keep       1 where a backward follows: forward then leaves its operands in
+ *              saved (slk_linear_ce_saved_bytes), which backward reads
+ *   scratch    slk_linear_ce_scratch_bytes(args, backward) bytes; its dhidden
+ *              and dweight as in the call (NULL: not wanted)
+ * float32 products run on the float16 matrix instructions in two parts an
+ * operand, about as exact as float32 products (in float32 the gradient of a
+ * logit is kept to 2^-39 of the largest one); bf16 gradients of logits are
+ * rounded to bf16. Sums in float32, in a fixed order.                        */
+enum slk_reduction { SLK_REDUCE_NONE = 0, SLK_REDUCE_SUM = 1, SLK_REDUCE_MEAN = 2 };
+typedef struct slk_linear_ce {
+    int64_t n, d, v, ignore_index;
+    const void *hidden, *weight;
+    const int64_t* target;
+    float* loss;
+    const float* upstream;
+    void *dhidden, *dweight;
+    void* saved;
+    int64_t saved_bytes;
+    void* scratch;
+    int64_t scratch_bytes;
+    int32_t dtype, reduction, keep, pad;
+} slk_linear_ce;
+
+SLK_API int64_t slk_linear_ce_saved_bytes(const slk_linear_ce* args_host);
+SLK_API int64_t slk_linear_ce_scratch_bytes(const slk_linear_ce* args_host, int backward);
+SLK_API int slk_linear_ce_forward(const slk_linear_ce* args_host, void* stream);
+SLK_API int slk_linear_ce_backward(const slk_linear_ce* args_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,13 +20,14 @@ from .layout import PaddedCSR
 from .ops import spmm
 from .nn import SparseLinear
 from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Static
+from .loss import linear_cross_entropy
 from .norm import residual_norm
 from .optim import AdamW
 from . import _lib, nn, ops, optim, router
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
            "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
-           "residual_norm", "install_as_sparselab"]
+           "residual_norm", "linear_cross_entropy", "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

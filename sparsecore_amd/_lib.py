@@ -88,6 +88,10 @@ EXPORTS = (
     "slk_norm_workspace_bytes",
     "slk_norm_forward",
     "slk_norm_backward",
+    "slk_linear_ce_saved_bytes",
+    "slk_linear_ce_scratch_bytes",
+    "slk_linear_ce_forward",
+    "slk_linear_ce_backward",
 )
 
 RIGL_INFO_BYTES = 32  # per row, slk_rigl_count's info
@@ -112,6 +116,8 @@ DTYPES = {torch.float32: SLK_F32, torch.bfloat16: SLK_BF16}
 Q8_BLOCK = 256  # SLK_Q8_BLOCK
 STATE_F32, STATE_Q8_SIGNED, STATE_Q8_UNSIGNED = 0, 1, 2
 CARRY_STATES = 4  # SLK_CARRY_STATES
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # enum slk_reduction
 
 NORM_MAX_D = 16384     # SLK_NORM_MAX_D
 NORM_COLS_MAX = 1024   # SLK_NORM_COLS_MAX
@@ -242,6 +248,18 @@ class Norm(ctypes.Structure):
         + [(k, ctypes.c_int32) for k in ("dtype", "layer", "branch_cols", "y_cols")])
 
 
+class LinearCE(ctypes.Structure):
+    """Mirror of ``slk_linear_ce`` (include/sparsecore_amd.h)."""
+
+    _fields_ = (
+        [(k, ctypes.c_int64) for k in ("n", "d", "v", "ignore_index")]
+        + [(k, ctypes.c_void_p) for k in ("hidden", "weight", "target", "loss", "upstream",
+                                          "dhidden", "dweight", "saved")]
+        + [("saved_bytes", ctypes.c_int64), ("scratch", ctypes.c_void_p),
+           ("scratch_bytes", ctypes.c_int64)]
+        + [(k, ctypes.c_int32) for k in ("dtype", "reduction", "keep", "pad")])
+
+
 _lib = None
 _load_error: str | None = None
 
@@ -334,12 +352,20 @@ def _declare(lib) -> None:
     lib.slk_norm_workspace_bytes.argtypes = [normp]
     lib.slk_norm_forward.argtypes = [normp, _vp]
     lib.slk_norm_backward.argtypes = [normp, _vp]
+    cep = ctypes.POINTER(LinearCE)
+    lib.slk_linear_ce_saved_bytes.restype = _i64
+    lib.slk_linear_ce_saved_bytes.argtypes = [cep]
+    lib.slk_linear_ce_scratch_bytes.restype = _i64
+    lib.slk_linear_ce_scratch_bytes.argtypes = [cep, ctypes.c_int]
+    lib.slk_linear_ce_forward.argtypes = [cep, _vp]
+    lib.slk_linear_ce_backward.argtypes = [cep, _vp]
     sized = ("slk_last_error", "slk_abi_version", "slk_transpose_workspace_bytes",
              "slk_drop_grow_workspace_bytes", "slk_rigl_bound_factor", "slk_rigl_partial_factor",
              "slk_dense_grad_approx_workspace_bytes",
              "slk_seg_list_capacity", "slk_seg_list_workspace_bytes", "slk_quad_windows",
              "slk_quad_chunks", "slk_quad_halves", "slk_strip_layout_bytes",
-             "slk_norm_workspace_bytes")
+             "slk_norm_workspace_bytes", "slk_linear_ce_saved_bytes",
+             "slk_linear_ce_scratch_bytes")
     for name in EXPORTS:
         if name not in sized:
             getattr(lib, name).restype = ctypes.c_int
@@ -878,6 +904,26 @@ def norm_forward(args: Norm, stream: int) -> None:
 
 def norm_backward(args: Norm, stream: int) -> None:
     rc = load().slk_norm_backward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def linear_ce_saved_bytes(args: LinearCE) -> int:
+    return int(load().slk_linear_ce_saved_bytes(ctypes.byref(args)))
+
+
+def linear_ce_scratch_bytes(args: LinearCE, backward: bool) -> int:
+    return int(load().slk_linear_ce_scratch_bytes(ctypes.byref(args), int(backward)))
+
+
+def linear_ce_forward(args: LinearCE, stream: int) -> None:
+    rc = load().slk_linear_ce_forward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def linear_ce_backward(args: LinearCE, stream: int) -> None:
+    rc = load().slk_linear_ce_backward(ctypes.byref(args), stream)
     if rc:
         _raise(rc)
 

@@ -1,0 +1,962 @@
+// The language-model head and its loss without the logits, slk_linear_ce_*:
+//   z = h·Wᵀ (n x v),  lse_n = log Σ_v exp(z_nv),  loss_n = lse_n - z_{n,target}
+//   dl = (exp(z - lse) - onehot(target))·g_n,  dh = dl·W,  dW = dlᵀ·h
+// Logits exist only as 256 x 128 tiles in registers. Forward: each tile leaves
+// its tokens' running maximum and sum, which a second kernel joins. Backward: a
+// piece of the vocabulary at a time, the tiles are computed again, turned into
+// dl in the epilogue and written as operands of the two gradient products (as
+// rows of tokens and as rows of the vocabulary); the piece's two products
+// follow. 2·n·v·d operations forward, 6 backward, where keeping the logits
+// would take 4 backward and 4 bytes a logit.
+//
+// Tokens whose target is ignore_index are left out before anything is computed
+// (a list of the live tokens is made on the device), so that they cost nothing
+// and what their hidden states hold reaches nothing.
+//
+// A score of at most 16 tokens reads W once, straight from memory, on 16 x 16
+// matrix instructions: bound by memory.
+#include "elem.hpp"
+#include "mma_tile.hpp"
+
+namespace slk {
+namespace {
+
+// float16 operands are scaled so that their largest finite magnitude lies in
+// [2^13, 2^14); dl (at most 1) by 2^kDlExp.
+constexpr int kTopExp = 14, kDlExp = 14;
+
+// What forward leaves for backward: counts and the operands' largest magnitudes.
+struct Header {
+    int32_t live;
+    uint32_t top_h, top_w;  // bits of the largest finite |h| (live tokens), |W|
+    int32_t pad[13];
+};
+static_assert(sizeof(Header) == 64, "one cache line");
+
+__device__ __forceinline__ int scale_exp(uint32_t top) {
+    // top in [2^(e-1), 2^e): x·2^(14-e) is below 2^14; no scaling of zeros
+    const int e = static_cast<int>(top >> 23) - 126;
+    if (top == 0) return 0;
+    const int s = kTopExp - e;
+    return s > 126 ? 126 : s;
+}
+__device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or inf past float32's range
+    return ldexpf(1.0f, e);
+}
+
+// ───────────────────────────── live tokens ─────────────────────────────
+
+// rows[i] = the i-th live token, pos[n] its place or -1, tgt[i] its target (-1
+// if it is no row of the vocabulary: its loss is NaN). One workgroup.
+constexpr int kListThreads = 1024, kListPer = 8;
+__global__ __launch_bounds__(kListThreads) void ce_list_kernel(
+    const int64_t* __restrict__ target, int64_t n, int64_t v, int64_t ignore,
+    Header* __restrict__ hd, int32_t* __restrict__ rows, int32_t* __restrict__ pos,
+    int32_t* __restrict__ tgt) {
+    __shared__ int sums[kListThreads / kWave];
+    const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x >> 6;
+    int64_t base = 0;
+    for (int64_t n0 = 0; n0 < n; n0 += kListThreads * kListPer) {
+        const int64_t at = n0 + static_cast<int64_t>(threadIdx.x) * kListPer;
+        int64_t t[kListPer];
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < kListPer; ++j) {
+            t[j] = at + j < n ? target[at + j] : ignore;
+            mine += t[j] != ignore;
+        }
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == kWave - 1) sums[wv] = incl;
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int w = 0; w < kListThreads / kWave; ++w) {
+            if (w < wv) before += sums[w];
+            all += sums[w];
+        }
+        int64_t i = base + before + incl - mine;
+#pragma unroll
+        for (int j = 0; j < kListPer; ++j) {
+            if (at + j >= n) break;
+            if (t[j] != ignore) {
+                rows[i] = static_cast<int32_t>(at + j);
+                tgt[i] = t[j] >= 0 && t[j] < v ? static_cast<int32_t>(t[j]) : -1;
+                pos[at + j] = static_cast<int32_t>(i);
+                ++i;
+            } else {
+                pos[at + j] = -1;
+            }
+        }
+        base += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        hd->live = static_cast<int32_t>(base);
+        hd->top_h = 0;
+        hd->top_w = 0;
+    }
+}
+
+// The largest finite magnitude of a float32 operand; rows of tokens that are
+// not live are skipped (pos; NULL: all rows).
+__global__ __launch_bounds__(256) void ce_top_kernel(const float* __restrict__ x, int64_t rows,
+                                                     int64_t d, const int32_t* __restrict__ pos,
+                                                     uint32_t* __restrict__ top) {
+    uint32_t m = 0;
+    const int64_t total = rows * d;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 4;
+    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < total;
+         i += step) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j >= total) break;
+            if (pos != nullptr && pos[(i + j) / d] < 0) continue;
+            const uint32_t b = __float_as_uint(x[i + j]) & 0x7fffffffu;
+            if (b < 0x7f800000u) m = max(m, b);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
+    // a maximum: the same whatever the order
+    if ((threadIdx.x & (kWave - 1)) == 0 && m != 0) atomicMax(top, m);
+}
+
+// ───────────────────────────── packing ─────────────────────────────
+
+// hi and lo of eight values scaled by `scale`
+__device__ __forceinline__ void split8(const float (&v)[8], float scale, f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = v[j] * scale;
+        hi[j] = static_cast<_Float16>(x);
+        lo[j] = static_cast<_Float16>(x - static_cast<float>(hi[j]));
+    }
+}
+
+struct PackArgs {
+    const void* src;
+    const int32_t* rows;  // source row of each row, NULL: itself
+    const int32_t* live;  // rows that count (device), NULL: R
+    const uint32_t* top;  // largest magnitude (float32 sources)
+    int64_t R, d;
+    char* by_row;  // rows of R rows, stages along d; NULL: not wanted
+    char* by_col;  // rows of d rows, stages along the R rows; NULL: not wanted
+};
+
+// A 64 x 64 piece of the source through LDS into both packed forms.
+template <class T, bool SPLIT>
+__global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
+    __shared__ float tile[64][65];
+    const int64_t R = p.live != nullptr ? *p.live : p.R;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
+    const int64_t c0 = static_cast<int64_t>(blockIdx.y) * 64;
+    if (r0 >= R) return;
+    const int c = threadIdx.x & 63;
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int64_t r = r0 + (threadIdx.x >> 6) + 4 * j;
+        const bool in = r < R && c0 + c < p.d;
+        const int64_t s = in ? (p.rows != nullptr ? p.rows[r] : r) : 0;
+        v[j] = in ? T::load(p.src, s * p.d + c0 + c) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) tile[(threadIdx.x >> 6) + 4 * j][c] = v[j];
+    __syncthreads();
+    const float scale = SPLIT ? pow2(scale_exp(*p.top)) : 1.0f;
+    constexpr int K = kStageK<SPLIT>;
+    const int64_t stages = ceil_div(p.d, K);
+    auto put = [&](char* row, int k, const float (&x)[8]) {  // elements k .. k + 7 of a stage
+        if constexpr (SPLIT) {
+            f16x8 hi, lo;
+            split8(x, scale, hi, lo);
+            *reinterpret_cast<f16x8*>(row + 2 * k) = hi;
+            *reinterpret_cast<f16x8*>(row + 64 + 2 * k) = lo;
+        } else {
+            b16x8 b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = static_cast<__bf16>(x[j]);
+            *reinterpret_cast<b16x8*>(row + 2 * k) = b;
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int at = threadIdx.x + 256 * q;
+        const int line = at >> 3, k = (at & 7) * 8;  // eight elements of a row, or of a column
+        float x[8];
+        if (p.by_row != nullptr && r0 + line < R) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = tile[line][k + j];
+            const int64_t st = (c0 + k) / K;
+            if (st < stages)
+                put(p.by_row + (st * p.R + r0 + line) * kStageBytes, (c0 + k) % K, x);
+        }
+        if (p.by_col != nullptr && c0 + line < p.d) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = tile[k + j][line];
+            const int64_t st = (r0 + k) / K;
+            if (st * K < R) put(p.by_col + (st * p.d + c0 + line) * kStageBytes, (r0 + k) % K, x);
+        }
+    }
+}
+
+// ───────────────────────────── epilogues ─────────────────────────────
+
+template <bool SPLIT>
+__device__ __forceinline__ float logit_scale(const Header* hd) {
+    return SPLIT ? pow2(-scale_exp(hd->top_h)) * pow2(-scale_exp(hd->top_w)) : 1.0f;
+}
+
+// Forward: rows are the vocabulary, columns tokens, so that a lane holds 32
+// logits of each of its two tokens and only their maximum and sum cross lanes.
+template <bool SPLIT>
+struct ScoreEpi {
+    const Header* hd;
+    const int32_t* tgt;
+    float2* part;  // vocabulary tiles x tokens
+    float* zt;
+    int64_t n;
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+        __syncthreads();  // the ring is free
+        float2* sh = reinterpret_cast<float2*>(t.lds);  // 4 x kTileN
+        const float scale = logit_scale<SPLIT>(hd);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int64_t tok = t.n0() + t.col(b);
+            const int32_t want = tok < t.N ? tgt[tok] : -1;
+            float m = -INFINITY, s = 0.0f;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t row = t.m0() + t.row(a, r);
+                    const float z = acc[a][b][r] * scale;
+                    if (row == want) zt[tok] = z;
+                    acc[a][b][r] = row < t.M ? z : -INFINITY;
+                    m = fmaxf(m, acc[a][b][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += expf(acc[a][b][r] - base);
+            s += __shfl_xor(s, 32);
+            if (t.lane < 32) sh[t.wm * kTileN + 64 * t.wn + t.col(b)] = make_float2(m, s);
+        }
+        __syncthreads();
+        if (threadIdx.x < kTileN) {
+            const int64_t tok = t.k0 + threadIdx.x;
+            float m = -INFINITY, s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, sh[w * kTileN + threadIdx.x].x);
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 x = sh[w * kTileN + threadIdx.x];
+                s += x.x == -INFINITY ? x.y : x.y * expf(x.x - base);
+            }
+            if (tok < t.N) part[t.i0 / kTileM * n + tok] = make_float2(m, s);
+        }
+    }
+};
+
+// Backward: the same tiles as dl, written as rows of tokens (stages along the
+// vocabulary) and as rows of the vocabulary (stages along the tokens).
+template <bool SPLIT>
+struct DlEpi {
+    const Header* hd;
+    const int32_t* tgt;
+    const float* lse;
+    const float* gr;  // upstream gradient of each token over the largest, NULL: all 1
+    char* by_tok;
+    char* by_voc;
+    int64_t v0;      // first row of the piece
+    int64_t n, voc;  // rows that the two are laid out for
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+        const float scale = logit_scale<SPLIT>(hd);
+        constexpr float up = SPLIT ? static_cast<float>(1 << kDlExp) : 1.0f;
+        constexpr int K = kStageK<SPLIT>;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int64_t tok = t.n0() + t.col(b);
+            const bool in = tok < t.N;
+            const int64_t want = in ? tgt[tok] - v0 : -1;
+            const float l = in ? lse[tok] : 0.0f;
+            const float g = (in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f) * up;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t row = t.m0() + t.row(a, r);
+                    float p = expf(acc[a][b][r] * scale - l);
+                    if (row == want) p -= 1.0f;
+                    acc[a][b][r] = in && row < t.M ? p * g : 0.0f;
+                }
+                const int64_t v = t.m0() + 32 * a;          // this block's 32 rows
+                const int64_t k = t.n0() + 32 * b;          // and 32 tokens
+                char* tk = by_tok + ((v / K) * n + tok) * kStageBytes + 2 * (v % K);
+                char* vc = by_voc + ((k / K) * voc + v) * kStageBytes + 2 * (k % K + (t.lane & 31));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = 8 * q + 4 * (t.lane >> 5);
+                    ushort4 hi, lo;
+                    uint16_t h[4], w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = acc[a][b][4 * q + j];
+                        if constexpr (SPLIT) {
+                            const _Float16 f = static_cast<_Float16>(x);
+                            h[j] = __builtin_bit_cast(uint16_t, f);
+                            w[j] = __builtin_bit_cast(
+                                uint16_t, static_cast<_Float16>(x - static_cast<float>(f)));
+                        } else {
+                            h[j] = f32_to_bf16(x);
+                            w[j] = 0;
+                        }
+                        char* to = vc + (at + j) * kStageBytes;
+                        *reinterpret_cast<uint16_t*>(to) = h[j];
+                        if (SPLIT) *reinterpret_cast<uint16_t*>(to + 64) = w[j];
+                    }
+                    hi = make_ushort4(h[0], h[1], h[2], h[3]);
+                    lo = make_ushort4(w[0], w[1], w[2], w[3]);
+                    if (in) {
+                        *reinterpret_cast<ushort4*>(tk + 2 * at) = hi;
+                        if (SPLIT) *reinterpret_cast<ushort4*>(tk + 64 + 2 * at) = lo;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Gradient products: float32 sums of each part of the K loop.
+struct SumEpi {
+    float* out;  // splits x rows x d
+    int64_t rows, d;
+    bool add;  // onto what the vocabulary's earlier pieces left
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+        float* to = out + t.split * rows * d;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int64_t c = t.n0() + t.col(b);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t row = t.m0() + t.row(a, r);
+                    if (row < t.M && c < t.N) {
+                        float* x = to + row * d + c;
+                        *x = add ? *x + acc[a][b][r] : acc[a][b][r];
+                    }
+                }
+            }
+    }
+};
+
+// A gradient from its sum: unscaled first (exactly), then times the upstream
+// factor. The two as one number could be subnormal where the result is not.
+template <bool SPLIT>
+struct GradScale {
+    float unscale, factor;
+    __device__ __forceinline__ GradScale(const Header* hd, const float* f, bool of_w)
+        : unscale(SPLIT ? pow2(-kDlExp - scale_exp(of_w ? hd->top_h : hd->top_w)) : 1.0f),
+          factor(*f) {}
+    __device__ __forceinline__ float operator()(float sum) const {
+        return (SPLIT ? sum * unscale : sum) * factor;
+    }
+};
+
+// dW where one workgroup has the whole sum: scaled, rounded and stored.
+template <class T, bool SPLIT>
+struct WeightEpi {
+    const Header* hd;
+    const float* factor;
+    void* out;  // of the piece's first row
+    int64_t d;
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+        const GradScale<SPLIT> s(hd, factor, true);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int64_t c = t.n0() + t.col(b);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t row = t.m0() + t.row(a, r);
+                    if (row < t.M && c < t.N) T::store(out, row * d + c, s(acc[a][b][r]));
+                }
+            }
+    }
+};
+
+// ───────────────────────────── joining ─────────────────────────────
+
+// lse and loss of each token from its partial maxima and sums: eight tokens a
+// workgroup, 32 threads a token.
+struct JoinArgs {
+    const float2* part;
+    const float* zt;
+    const int64_t* target;
+    const int32_t* pos;  // place of each token in part, NULL: its own
+    const int32_t* tgt;  // target of each place, -1: none (with pos)
+    float* lse;          // NULL: not wanted
+    float* losses;
+    int64_t n, v, ignore, parts;
+};
+__global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
+    __shared__ float2 sh[32][9];
+    const int j = threadIdx.x & 7, part = threadIdx.x >> 3;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + j;
+    int64_t i = -1;
+    bool valid = false;
+    if (n < p.n) {
+        if (p.pos != nullptr) {
+            i = p.pos[n];
+            valid = i >= 0 && p.tgt[i] >= 0;
+        } else if (p.target[n] != p.ignore) {
+            i = n;
+            valid = p.target[n] >= 0 && p.target[n] < p.v;
+        }
+    }
+    float m = -INFINITY, s = 0.0f;
+    if (i >= 0) {
+        for (int64_t k = part; k < p.parts; k += 32) {
+            const float2 x = p.part[k * p.n + i];
+            const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+            s = (m == -INFINITY ? s : s * expf(m - base)) +
+                (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
+            m = top;
+        }
+    }
+    sh[part][j] = make_float2(m, s);
+    __syncthreads();
+    if (part != 0 || n >= p.n) return;
+    for (int k = 1; k < 32; ++k) {
+        const float2 x = sh[k][j];
+        const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+        s = (m == -INFINITY ? s : s * expf(m - base)) +
+            (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
+        m = top;
+    }
+    if (i < 0) {
+        p.losses[n] = 0.0f;
+        return;
+    }
+    const float lse = (m == -INFINITY ? 0.0f : m) + logf(s);
+    if (p.lse != nullptr) p.lse[i] = lse;
+    p.losses[n] = valid ? lse - p.zt[i] : NAN;
+}
+
+// The sum or mean of the losses over the live tokens: one workgroup, sums in
+// float64 in a fixed order.
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ losses,
+                                                         const int64_t* __restrict__ target,
+                                                         int64_t n, int64_t ignore, bool mean,
+                                                         float* __restrict__ out) {
+    __shared__ double sh[2][1024 / kWave];
+    double s = 0.0, c = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        s += losses[i];
+        c += target[i] != ignore;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o);
+        c += __shfl_xor(c, o);
+    }
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+        sh[0][threadIdx.x >> 6] = s;
+        sh[1][threadIdx.x >> 6] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 1024 / kWave; ++w) {
+            s += sh[0][w];
+            c += sh[1][w];
+        }
+        *out = static_cast<float>(mean ? s / c : s);  // no live token: 0 / 0
+    }
+}
+
+// Upstream gradients: factor is the largest magnitude over the live tokens and
+// gr each token's own over it, so that dl stays within [-1, 1]. With one
+// upstream value for all (sum, mean) every gr is 1 and none is written.
+__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up,
+                                                           const Header* __restrict__ hd,
+                                                           const int32_t* __restrict__ rows,
+                                                           int reduction, float* __restrict__ gr,
+                                                           float* __restrict__ factor) {
+    __shared__ uint32_t sh[1024 / kWave];
+    const int64_t live = hd->live;
+    if (reduction != SLK_REDUCE_NONE) {
+        // no live token: gradients are 0, as the sum's over none
+        if (threadIdx.x == 0)
+            *factor = live == 0 ? 0.0f
+                      : reduction == SLK_REDUCE_MEAN ? *up / static_cast<float>(live) : *up;
+        return;
+    }
+    uint32_t m = 0;  // as bit patterns, a NaN is the largest
+    for (int64_t i = threadIdx.x; i < live; i += 1024)
+        m = max(m, __float_as_uint(up[rows[i]]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
+    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int w = 0; w < 1024 / kWave; ++w) m = max(m, sh[w]);
+    const float top = __uint_as_float(m);
+    for (int64_t i = threadIdx.x; i < live; i += 1024)
+        gr[i] = m == 0 ? 0.0f : up[rows[i]] / top;
+    if (threadIdx.x == 0) *factor = top;
+}
+
+// out[r][c] = the parts' sum, scaled and rounded; with pos, row r is token r and
+// the sums are at its place (0 where it has none).
+template <class T, bool SPLIT>
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict__ sums, int splits,
+                                                        int64_t rows, int64_t stride, int64_t d,
+                                                        const int32_t* __restrict__ pos,
+                                                        const Header* __restrict__ hd,
+                                                        const float* __restrict__ factor,
+                                                        bool of_w, void* __restrict__ out) {
+    const GradScale<SPLIT> s(hd, factor, of_w);
+    const int64_t total = rows * d, step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
+        const int64_t r = i / d;
+        const int64_t at = pos != nullptr ? pos[r] : r;
+        float x = 0.0f;
+        if (at >= 0) {
+            for (int k = 0; k < splits; ++k) x += sums[k * stride * d + at * d + (i - r * d)];
+            x = s(x);
+        }
+        T::store(out, i, x);
+    }
+}
+
+// ───────────────────────────── few tokens ─────────────────────────────
+
+constexpr int kFewTokens = 16;
+constexpr int kFewThreads = 256;
+
+// A wave takes 16 rows of W at a time against 16 tokens (fewer are repeated):
+// lane l holds row l % 16 of both, its columns 4 (l / 16) .. of each run of 16
+// (float32; 8 (l / 16) of 32 in bfloat16). The same columns meet in both
+// operands, so their order within an instruction does not matter.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
+    const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
+    int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt) {
+    constexpr bool kF32 = T::kBytes == 4;
+    constexpr int kRun = kF32 ? 16 : 32, kMine = kRun / 4;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int64_t tok = col < n ? col : n - 1;
+    const int64_t want = target[tok];
+    const int64_t blocks = ceil_div(v, 16);
+    float m = -INFINITY, s = 0.0f;
+    for (int64_t blk = static_cast<int64_t>(blockIdx.x) * (kFewThreads / kWave) + wv; blk < blocks;
+         blk += static_cast<int64_t>(gridDim.x) * (kFewThreads / kWave)) {
+        int64_t row = blk * 16 + col;
+        if (row >= v) row = v - 1;
+        const int64_t wo = row * d, ho = tok * d;
+        f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        auto step = [&](int64_t k, f32x4& c) {
+            float a[kMine], b[kMine];
+            const int64_t e = k + kMine * quarter;
+            if (VEC) {
+#pragma unroll
+                for (int j = 0; j < kMine; j += 4) {
+                    if (e + j < d) {
+                        T::load4(w, wo + e + j, &a[j]);
+                        T::load4(h, ho + e + j, &b[j]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[j + i] = b[j + i] = 0.0f;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kMine; ++j) {
+                    a[j] = e + j < d ? T::load(w, wo + e + j) : 0.0f;
+                    b[j] = e + j < d ? T::load(h, ho + e + j) : 0.0f;
+                }
+            }
+            if constexpr (kF32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+            } else {
+                b16x8 x, y;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] = static_cast<__bf16>(a[j]);
+                    y[j] = static_cast<__bf16>(b[j]);
+                }
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+            }
+        };
+        int64_t k = 0;
+        for (; k + 4 * kRun <= d; k += 4 * kRun) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) step(k + u * kRun, acc[u & 1]);
+        }
+        for (; k < d; k += kRun) step(k, acc[0]);
+        // lane l, register r: row 4 (l / 16) + r of the block, token l % 16
+        float z[4], top = m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t vr = blk * 16 + 4 * quarter + r;
+            z[r] = acc[0][r] + acc[1][r];
+            if (vr == want && col < n) zt[col] = z[r];
+            if (vr >= v) z[r] = -INFINITY;
+            top = fmaxf(top, z[r]);
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        s = m == -INFINITY ? s : s * expf(m - base);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += expf(z[r] - base);
+        m = top;
+    }
+    // the lanes of a token, then the waves
+    __shared__ float2 sh[kFewThreads / kWave][kFewTokens];
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+        const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+        s = (m == -INFINITY ? s : s * expf(m - base)) +
+            (m2 == -INFINITY ? s2 : s2 * expf(m2 - base));
+        m = top;
+    }
+    if (lane < kFewTokens) sh[wv][lane] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < n) {
+        m = sh[0][threadIdx.x].x;
+        s = sh[0][threadIdx.x].y;
+        for (int k = 1; k < kFewThreads / kWave; ++k) {
+            const float2 x = sh[k][threadIdx.x];
+            const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+            s = (m == -INFINITY ? s : s * expf(m - base)) +
+                (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
+            m = top;
+        }
+        part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = make_float2(m, s);
+    }
+}
+
+// ───────────────────────────── sizes ─────────────────────────────
+
+int64_t up256(int64_t x) { return (x + 255) & ~int64_t{255}; }
+
+struct Carve {
+    int64_t at = 0;
+    int64_t take(int64_t bytes) {
+        const int64_t o = at;
+        at = up256(at + bytes);
+        return o;
+    }
+};
+
+struct Saved {
+    int64_t header, rows, pos, tgt, lse, h_row, w_row, h_col, w_col, bytes;
+};
+
+bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
+int64_t stages(const slk_linear_ce* a, int64_t k) { return ceil_div(k, split_of(a) ? 32 : 64); }
+
+bool few(const slk_linear_ce* a) { return a->n <= kFewTokens && !a->keep; }
+
+Saved saved_of(const slk_linear_ce* a) {
+    Saved s;
+    Carve c;
+    s.header = c.take(sizeof(Header));
+    s.rows = c.take(4 * a->n);
+    s.pos = c.take(4 * a->n);
+    s.tgt = c.take(4 * a->n);
+    s.lse = c.take(4 * a->n);
+    s.h_row = c.take(stages(a, a->d) * a->n * kStageBytes);
+    s.w_row = c.take(stages(a, a->d) * a->v * kStageBytes);
+    s.h_col = s.w_col = 0;
+    if (a->keep) {
+        s.h_col = c.take(stages(a, a->n) * a->d * kStageBytes);
+        s.w_col = c.take(stages(a, a->v) * a->d * kStageBytes);
+    }
+    s.bytes = few(a) ? 0 : c.at;
+    return s;
+}
+
+constexpr int64_t kFewGroups = 512;  // workgroups of ce_few_kernel at most
+
+int64_t parts_of(const slk_linear_ce* a) {
+    if (few(a)) {
+        const int64_t g = ceil_div(ceil_div(a->v, 16), kFewThreads / kWave);
+        return g < kFewGroups ? g : kFewGroups;
+    }
+    return ceil_div(a->v, kTileM);
+}
+
+struct Forward {
+    int64_t part, zt, losses, bytes;
+};
+Forward forward_of(const slk_linear_ce* a) {
+    Forward f;
+    Carve c;
+    f.part = c.take(8 * parts_of(a) * a->n);
+    f.zt = c.take(4 * a->n);
+    f.losses = c.take(4 * a->n);
+    f.bytes = c.at;
+    return f;
+}
+
+// Vocabulary rows of a piece of the backward: dl of a piece, in its two forms,
+// takes at most kDlBytes.
+constexpr int64_t kDlBytes = int64_t{1} << 30;
+
+// Parts of a product's K loop: with one workgroup a CU, `tiles` of them take
+// ceil(tiles·s / 256) rounds of 1/s of the loop each; every part also costs
+// the writing and reading of its sums (taken as 2% of the loop).
+int splits_for(int64_t tiles, int64_t nst) {
+    int best = 1;
+    double cost = 1e30;
+    for (int s = 1; s <= 32; ++s) {
+        if (s > 1 && nst < 8 * s) break;
+        const double c = static_cast<double>(ceil_div(tiles * s, 256)) / s + 0.02 * s;
+        if (c < cost - 1e-9) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
+
+struct Backward {
+    int64_t piece;  // rows of a piece, a multiple of kTileM
+    int sh, sw;     // parts of the two products
+    int64_t gr, factor, by_tok, by_voc, dh, dw, bytes;
+};
+Backward backward_of(const slk_linear_ce* a) {
+    Backward b;
+    const int64_t n128 = ceil_div(a->n, kTileN) * kTileN;
+    const int64_t per_row = n128 * (split_of(a) ? 8 : 4);
+    int64_t rows = kDlBytes / per_row / kTileM * kTileM;
+    if (rows < kTileM) rows = kTileM;
+    const int64_t all = ceil_div(a->v, kTileM) * kTileM;
+    const int64_t pieces = ceil_div(all, rows < all ? rows : all);
+    b.piece = ceil_div(ceil_div(all, pieces), kTileM) * kTileM;
+    b.sh = splits_for(ceil_div(a->n, kTileM) * ceil_div(a->d, kTileN), stages(a, b.piece));
+    b.sw = splits_for(b.piece / kTileM * ceil_div(a->d, kTileN), stages(a, a->n));
+    Carve c;
+    b.factor = c.take(4);
+    b.gr = c.take(4 * a->n);
+    b.by_tok = c.take(stages(a, b.piece) * a->n * kStageBytes);
+    b.by_voc = c.take(stages(a, n128) * b.piece * kStageBytes);
+    b.dh = c.take(a->dhidden != nullptr ? 4 * b.sh * a->n * a->d : 0);
+    b.dw = c.take(a->dweight != nullptr && b.sw > 1 ? 4 * b.sw * b.piece * a->d : 0);
+    b.bytes = c.at;
+    return b;
+}
+
+int validate(const slk_linear_ce* a, const char* who) {
+    const std::string w(who);
+    if (a == nullptr) return fail(SLK_EINVAL, w + ": NULL arguments");
+    if (a->n < 0 || a->d < 1 || a->v < 1) {
+        return fail(SLK_EINVAL, w + ": n must be >= 0, d and v >= 1");
+    }
+    if (a->n > (1 << 25) || a->v > (1 << 25) || a->d > (1 << 20)) {
+        return fail(SLK_EINVAL, w + ": at most 2^25 tokens and vocabulary rows, 2^20 features");
+    }
+    if (a->dtype != SLK_F32 && a->dtype != SLK_BF16) {
+        return fail(SLK_EINVAL, w + ": dtype must be SLK_F32 or SLK_BF16");
+    }
+    if (a->reduction != SLK_REDUCE_NONE && a->reduction != SLK_REDUCE_SUM &&
+        a->reduction != SLK_REDUCE_MEAN) {
+        return fail(SLK_EINVAL, w + ": unknown reduction");
+    }
+    return SLK_OK;
+}
+
+template <class T, bool SPLIT>
+int pack(const PackArgs& p, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.R, 64)),
+                    static_cast<unsigned>(ceil_div(p.d, 64)));
+    hipLaunchKernelGGL((ce_pack_kernel<T, SPLIT>), grid, dim3(256), 0, st, p);
+    return check_launch("linear_ce pack");
+}
+
+template <class T, bool SPLIT>
+int forward(const slk_linear_ce* a, hipStream_t st) {
+    const Forward f = forward_of(a);
+    char* sc = static_cast<char*>(a->scratch);
+    float2* part = reinterpret_cast<float2*>(sc + f.part);
+    float* zt = reinterpret_cast<float*>(sc + f.zt);
+    float* losses = a->reduction == SLK_REDUCE_NONE ? a->loss
+                                                    : reinterpret_cast<float*>(sc + f.losses);
+    JoinArgs j{part, zt, a->target, nullptr, nullptr, nullptr, losses, a->n, a->v,
+               a->ignore_index, parts_of(a)};
+    int rc = SLK_OK;
+    if (few(a)) {
+        const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 4 * T::kBytes) &&
+                         aligned_to(a->weight, 4 * T::kBytes);
+        const dim3 grid(static_cast<unsigned>(parts_of(a)));
+        auto go = [&](auto k) {
+            hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target,
+                               a->n, a->d, a->v, part, zt);
+        };
+        if (vec) go(ce_few_kernel<T, true>);
+        else go(ce_few_kernel<T, false>);
+        rc = check_launch("linear_ce few");
+    } else {
+        const Saved s = saved_of(a);
+        char* sv = static_cast<char*>(a->saved);
+        Header* hd = reinterpret_cast<Header*>(sv + s.header);
+        int32_t* rows = reinterpret_cast<int32_t*>(sv + s.rows);
+        int32_t* pos = reinterpret_cast<int32_t*>(sv + s.pos);
+        int32_t* tgt = reinterpret_cast<int32_t*>(sv + s.tgt);
+        hipLaunchKernelGGL(ce_list_kernel, dim3(1), dim3(kListThreads), 0, st, a->target, a->n,
+                           a->v, a->ignore_index, hd, rows, pos, tgt);
+        if ((rc = check_launch("linear_ce list")) != SLK_OK) return rc;
+        if (SPLIT) {
+            auto top = [&](const void* x, int64_t r, const int32_t* ps, uint32_t* to) {
+                const int64_t g = ceil_div(r * a->d, 256 * 4 * 4);
+                hipLaunchKernelGGL(ce_top_kernel, dim3(static_cast<unsigned>(g < 2048 ? g : 2048)),
+                                   dim3(256), 0, st, static_cast<const float*>(x), r, a->d, ps, to);
+                return check_launch("linear_ce top");
+            };
+            if ((rc = top(a->hidden, a->n, pos, &hd->top_h)) != SLK_OK) return rc;
+            if ((rc = top(a->weight, a->v, nullptr, &hd->top_w)) != SLK_OK) return rc;
+        }
+        PackArgs ph{a->hidden, rows, &hd->live, &hd->top_h, a->n, a->d, sv + s.h_row,
+                    a->keep ? sv + s.h_col : nullptr};
+        PackArgs pw{a->weight, nullptr, nullptr, &hd->top_w, a->v, a->d, sv + s.w_row,
+                    a->keep ? sv + s.w_col : nullptr};
+        if ((rc = pack<T, SPLIT>(ph, st)) != SLK_OK) return rc;
+        if ((rc = pack<T, SPLIT>(pw, st)) != SLK_OK) return rc;
+        const MmaArgs g{sv + s.w_row, sv + s.h_row, a->v, a->n, stages(a, a->d), a->v, a->n,
+                        &hd->live, kLiveN, 1};
+        rc = mma<SPLIT>(g, ScoreEpi<SPLIT>{hd, tgt, part, zt, a->n}, st, "linear_ce logits");
+        j.pos = pos;
+        j.tgt = tgt;
+        j.lse = reinterpret_cast<float*>(sv + s.lse);
+    }
+    if (rc != SLK_OK) return rc;
+    hipLaunchKernelGGL(ce_join_kernel, dim3(static_cast<unsigned>(ceil_div(a->n, 8))), dim3(256),
+                       0, st, j);
+    if ((rc = check_launch("linear_ce join")) != SLK_OK) return rc;
+    if (a->reduction != SLK_REDUCE_NONE) {
+        hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, losses, a->target, a->n,
+                           a->ignore_index, a->reduction == SLK_REDUCE_MEAN, a->loss);
+        rc = check_launch("linear_ce reduce");
+    }
+    return rc;
+}
+
+template <class T, bool SPLIT>
+int backward(const slk_linear_ce* a, hipStream_t st) {
+    const Saved s = saved_of(a);
+    const Backward b = backward_of(a);
+    char* sv = static_cast<char*>(a->saved);
+    char* sc = static_cast<char*>(a->scratch);
+    const Header* hd = reinterpret_cast<const Header*>(sv + s.header);
+    const int32_t* rows = reinterpret_cast<const int32_t*>(sv + s.rows);
+    const int32_t* pos = reinterpret_cast<const int32_t*>(sv + s.pos);
+    const int32_t* tgt = reinterpret_cast<const int32_t*>(sv + s.tgt);
+    const float* lse = reinterpret_cast<const float*>(sv + s.lse);
+    float* factor = reinterpret_cast<float*>(sc + b.factor);
+    float* gr = reinterpret_cast<float*>(sc + b.gr);
+    hipLaunchKernelGGL(ce_upstream_kernel, dim3(1), dim3(1024), 0, st, a->upstream, hd, rows,
+                       a->reduction, gr, factor);
+    int rc = check_launch("linear_ce upstream");
+    if (rc != SLK_OK) return rc;
+    constexpr int K = kStageK<SPLIT>;
+    float* dh = reinterpret_cast<float*>(sc + b.dh);
+    float* dw = reinterpret_cast<float*>(sc + b.dw);
+    auto finish = [&](const float* sums, int splits, int64_t r, int64_t stride,
+                      const int32_t* ps, bool of_w, void* out) {
+        const int64_t g = ceil_div(r * a->d, 256 * 4);
+        hipLaunchKernelGGL((ce_finish_kernel<T, SPLIT>),
+                           dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st,
+                           sums, splits, r, stride, a->d, ps, hd, factor, of_w, out);
+        return check_launch("linear_ce finish");
+    };
+    for (int64_t v0 = 0; v0 < a->v; v0 += b.piece) {
+        const int64_t vn = a->v - v0 < b.piece ? a->v - v0 : b.piece;
+        const MmaArgs gl{sv + s.w_row + v0 * kStageBytes, sv + s.h_row, vn, a->n,
+                         stages(a, a->d), a->v, a->n, &hd->live, kLiveN, 1};
+        const DlEpi<SPLIT> el{hd, tgt, lse, a->reduction == SLK_REDUCE_NONE ? gr : nullptr,
+                              sc + b.by_tok, sc + b.by_voc, v0, a->n, b.piece};
+        if ((rc = mma<SPLIT>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+        if (a->dhidden != nullptr) {
+            const MmaArgs g{sc + b.by_tok, sv + s.w_col + v0 / K * a->d * kStageBytes, a->n, a->d,
+                            stages(a, vn), a->n, a->d, &hd->live, kLiveM, b.sh};
+            if ((rc = mma<SPLIT>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st, "linear_ce dhidden")) !=
+                SLK_OK) {
+                return rc;
+            }
+        }
+        if (a->dweight != nullptr) {
+            const MmaArgs g{sc + b.by_voc, sv + s.h_col, vn, a->d, stages(a, a->n), b.piece, a->d,
+                            &hd->live, kLiveK, b.sw};
+            void* out = static_cast<char*>(a->dweight) + v0 * a->d * T::kBytes;
+            if (b.sw == 1) {
+                rc = mma<SPLIT>(g, WeightEpi<T, SPLIT>{hd, factor, out, a->d}, st,
+                                "linear_ce dweight");
+            } else {
+                rc = mma<SPLIT>(g, SumEpi{dw, b.piece, a->d, false}, st, "linear_ce dweight");
+                if (rc == SLK_OK) rc = finish(dw, b.sw, vn, b.piece, nullptr, true, out);
+            }
+            if (rc != SLK_OK) return rc;
+        }
+    }
+    if (a->dhidden != nullptr) rc = finish(dh, b.sh, a->n, a->n, pos, false, a->dhidden);
+    return rc;
+}
+
+}  // namespace
+}  // namespace slk
+
+extern "C" int64_t slk_linear_ce_saved_bytes(const slk_linear_ce* a) {
+    using namespace slk;
+    return validate(a, "linear_ce_saved_bytes") == SLK_OK && a->n > 0 ? saved_of(a).bytes : 0;
+}
+
+extern "C" int64_t slk_linear_ce_scratch_bytes(const slk_linear_ce* a, int backward) {
+    using namespace slk;
+    if (validate(a, "linear_ce_scratch_bytes") != SLK_OK || a->n == 0) return 0;
+    return backward ? backward_of(a).bytes : forward_of(a).bytes;
+}
+
+extern "C" int slk_linear_ce_forward(const slk_linear_ce* a, void* stream) {
+    using namespace slk;
+    clear_error();
+    const int rc = validate(a, "linear_ce_forward");
+    if (rc != SLK_OK || a->n == 0) return rc;
+    if (a->hidden == nullptr || a->weight == nullptr || a->target == nullptr ||
+        a->loss == nullptr) {
+        return fail(SLK_EINVAL, "linear_ce_forward: NULL hidden, weight, target or loss");
+    }
+    if (a->scratch_bytes < forward_of(a).bytes || a->saved_bytes < saved_of(a).bytes ||
+        a->scratch == nullptr || (a->saved == nullptr && saved_of(a).bytes > 0)) {
+        return fail(SLK_EINVAL, "linear_ce_forward: saved or scratch too small");
+    }
+    return a->dtype == SLK_F32 ? forward<F32, true>(a, as_stream(stream))
+                               : forward<BF16, false>(a, as_stream(stream));
+}
+
+extern "C" int slk_linear_ce_backward(const slk_linear_ce* a, void* stream) {
+    using namespace slk;
+    clear_error();
+    const int rc = validate(a, "linear_ce_backward");
+    if (rc != SLK_OK || a->n == 0) return rc;
+    if (!a->keep) return fail(SLK_EINVAL, "linear_ce_backward: the forward kept nothing");
+    if (a->upstream == nullptr) return fail(SLK_EINVAL, "linear_ce_backward: NULL upstream");
+    if (a->scratch_bytes < backward_of(a).bytes || a->saved_bytes < saved_of(a).bytes ||
+        a->scratch == nullptr || a->saved == nullptr) {
+        return fail(SLK_EINVAL, "linear_ce_backward: saved or scratch too small");
+    }
+    return a->dtype == SLK_F32 ? backward<F32, true>(a, as_stream(stream))
+                               : backward<BF16, false>(a, as_stream(stream));
+}

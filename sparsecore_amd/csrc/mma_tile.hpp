@@ -1,0 +1,245 @@
+// Matrix-core product of two packed operands, C = A·Bᵀ, with the epilogue as a
+// functor: the loop behind the head and its loss (linear_ce.hip).
+//
+// Packed operand: R rows of K elements as stages of 128 bytes a row, stage by
+// stage: P[stage][row][128 bytes], zero beyond K. A tile's stage is then one
+// contiguous piece of memory, whatever K is. A stage holds, of a row,
+//   SPLIT   32 elements in float16, high parts (64 bytes) then low parts: a
+//           float32 x, scaled by a power of two, as hi + lo. The product takes
+//           hi·hi + hi·lo + lo·hi in float32: x is kept to 2^-22 of itself (or
+//           2^-39 of the operand's largest element), about float32's own
+//           rounding, at a third of the float16 rate, where the matrix cores'
+//           float32 instructions run at a sixteenth;
+//   else    64 elements in bfloat16.
+//
+// Tile: 256 x 128, eight waves of 64 x 64 (2 x 2 blocks of 32 x 32). Stages go
+// from memory straight into a ring of three LDS buffers of 48 KiB, two stages
+// ahead, one barrier a stage; the 16-byte pieces of a staged row are permuted
+// (piece c of row r at slot c ^ ((r >> 1) & 7)), so that the 16 lanes of an
+// LDS pass meet all banks once. Buffer indexes are compile-time constants (the
+// loop is unrolled by three): otherwise the compiler makes every LDS read wait
+// for the loads just issued.
+#pragma once
+
+#include "common.hpp"
+
+namespace slk {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStageBytes = 128;
+template <bool SPLIT>
+constexpr int kStageK = SPLIT ? 32 : 64;
+
+constexpr int kTileM = 256, kTileN = 128;
+constexpr int kMmaThreads = 512;
+constexpr int kMmaBufs = 3;
+constexpr int kMmaLds = kMmaBufs * (kTileM + kTileN) * kStageBytes;
+constexpr int kMmaGroup = 4;  // tile rows of a group of the tile order
+
+// s_waitcnt operand: at most n vector-memory loads outstanding, no LDS reads
+// or scalar loads outstanding (n <= 63)
+constexpr int wait_vm(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0x0 << 8); }
+
+// Which dimension is the device-side count of live tokens.
+enum MmaLive { kLiveNone = 0, kLiveM = 1, kLiveN = 2, kLiveK = 3 };
+
+struct MmaArgs {
+    const void* A;
+    const void* B;
+    int64_t M, N, nst;       // rows of A and B, stages (upper bounds where live says so)
+    int64_t rows_a, rows_b;  // rows that the packed operands are laid out for
+    const int32_t* live;
+    int which;               // MmaLive
+    int splits;              // parts of the K loop, each a workgroup of its own
+};
+
+// What an epilogue gets: its wave's 64 x 64 of the tile. Lane l, register r of
+// block [a][b]: row  m0 + 32 a + 8 (r / 4) + 4 (l / 32) + r % 4,
+//               column n0 + 32 b + l % 32.
+struct MmaTile {
+    int64_t i0, k0;  // the workgroup's tile
+    int wm, wn, lane;
+    int64_t M, N;
+    int split;
+    char* lds;  // kMmaLds bytes, free after a barrier
+    __device__ __forceinline__ int64_t m0() const { return i0 + 64 * wm; }
+    __device__ __forceinline__ int64_t n0() const { return k0 + 64 * wn; }
+    __device__ __forceinline__ int row(int a, int r) const {
+        return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+    }
+    __device__ __forceinline__ int col(int b) const { return 32 * b + (lane & 31); }
+};
+
+template <bool SPLIT, class Epi>
+__global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const Epi epi) {
+    __shared__ __align__(16) unsigned char ring[kMmaBufs][(kTileM + kTileN) * kStageBytes];
+
+    int64_t M = g.M, N = g.N, nst = g.nst;
+    if (g.which != kLiveNone) {
+        const int64_t live = *g.live;
+        if (g.which == kLiveM) M = live;
+        else if (g.which == kLiveN) N = live;
+        else nst = ceil_div(live, kStageK<SPLIT>);
+    }
+    const int64_t nTi = ceil_div(M, kTileM), nTk = ceil_div(N, kTileN);
+    const int64_t tiles = nTi * nTk, total = tiles * g.splits;
+    if (static_cast<int64_t>(blockIdx.x) >= total) return;  // the whole workgroup
+    // grouped, XCD-contiguous tile order: consecutive tiles share rows of A and B
+    const int64_t L = xcd_logical_block(blockIdx.x, total);
+    const int split = static_cast<int>(L / tiles);
+    const int64_t tile = L - split * tiles;
+    const int64_t grp = tile / (kMmaGroup * nTk);
+    const int64_t first = grp * kMmaGroup;
+    const int64_t gsize = nTi - first < kMmaGroup ? nTi - first : kMmaGroup;
+    const int64_t in_grp = tile - grp * kMmaGroup * nTk;
+    const int64_t i0 = (first + in_grp % gsize) * kTileM;
+    const int64_t k0 = (in_grp / gsize) * kTileN;
+    const int64_t s0 = split * nst / g.splits, s1 = (split + 1) * nst / g.splits;
+
+    const int t = threadIdx.x;
+    const int lane = t & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wm = wv >> 1, wn = wv & 1;
+
+    // Load i of a stage fills rows 8 i .. 8 i + 7 of its operand's buffer: lane
+    // l fetches piece (l mod 8) ^ swizzle of row 8 i + l / 8. Rows past the
+    // operand are clamped to its last row; their results are not used.
+    constexpr int kPerA = kTileM / 64, kPerB = kTileN / 64;
+    uint32_t offA[kPerA], offB[kPerB];
+    auto plan = [&](int64_t R, int64_t r0, int i) {
+        const int rr = 8 * i + lane / 8;
+        int64_t r = r0 + rr;
+        if (r >= R) r = R - 1;
+        return static_cast<uint32_t>(r * kStageBytes + 16 * ((lane & 7) ^ ((rr >> 1) & 7)));
+    };
+#pragma unroll
+    for (int q = 0; q < kPerA; ++q) offA[q] = plan(M, i0, wv + 8 * q);
+#pragma unroll
+    for (int q = 0; q < kPerB; ++q) offB[q] = plan(N, k0, wv + 8 * q);
+    const char* A = static_cast<const char*>(g.A);
+    const char* B = static_cast<const char*>(g.B);
+    auto issue = [&](int buf, int64_t st) {
+        const char* a = A + st * g.rows_a * kStageBytes;
+        const char* b = B + st * g.rows_b * kStageBytes;
+#pragma unroll
+        for (int q = 0; q < kPerA; ++q)
+            __builtin_amdgcn_global_load_lds(a + offA[q], &ring[buf][1024 * (wv + 8 * q)], 16, 0,
+                                             0);
+#pragma unroll
+        for (int q = 0; q < kPerB; ++q)
+            __builtin_amdgcn_global_load_lds(
+                b + offB[q], &ring[buf][kTileM * kStageBytes + 1024 * (wv + 8 * q)], 16, 0, 0);
+    };
+
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
+
+    const int half = lane >> 5;
+    const int rA = wm * 64 + (lane & 31), rB = wn * 64 + (lane & 31);
+    using Frag = std::conditional_t<SPLIT, f16x8, b16x8>;
+    auto frag = [&](const unsigned char* lds, int r, int c) {
+        return *reinterpret_cast<const Frag*>(lds + 16 * (r * 8 + (c ^ ((r >> 1) & 7))));
+    };
+    // fragments of half a stage: SPLIT, a k-step's high and low parts; else two k-steps
+    Frag af[2][2][2], bf[2][2][2];  // [half stage][block][part]
+    auto reads = [&](const unsigned char* buf, int h) {
+        const unsigned char* lb = buf + kTileM * kStageBytes;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int c = (SPLIT ? 4 * p + 2 * h : 4 * h + 2 * p) + half;
+                af[h][b][p] = frag(buf, rA + 32 * b, c);
+                bf[h][b][p] = frag(lb, rB + 32 * b, c);
+            }
+    };
+    auto mfmas = [&](int h, int pa, int pb) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if constexpr (SPLIT) {
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[h][a][pa], bf[h][b][pb],
+                                                                       acc[a][b], 0, 0, 0);
+                } else {
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        af[h][a][pa], bf[h][b][pb], acc[a][b], 0, 0, 0);
+                }
+            }
+    };
+    constexpr int kLoads = kPerA + kPerB;
+    // Stage st reads buffer st mod 3 and loads stage st + 2 into the buffer that
+    // stage st - 1 left. The barrier sits after the stage's last LDS reads: by
+    // then this wave's loads of stage st + 1 have landed (its loads of stage
+    // st + 2 may be in flight), so behind it every wave's have, and the buffer
+    // of stage st is free. A bare s_barrier: __syncthreads would also wait for
+    // the loads of stage st + 2. Past the end the last stage is loaded again,
+    // so that every stage waits for the same count.
+    auto stage = [&](auto I, int64_t st) {
+        constexpr int buf = decltype(I)::value;
+        mfmas(0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        reads(ring[buf], 1);
+        issue((buf + 2) % kMmaBufs, st + 2 < s1 ? st + 2 : s1 - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (SPLIT) {
+            mfmas(0, 0, 1);
+            mfmas(0, 1, 0);
+        } else {
+            mfmas(0, 1, 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(wait_vm(kLoads));
+        asm volatile("s_barrier" ::: "memory");
+        reads(ring[(buf + 1) % kMmaBufs], 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(1, 0, 0);
+        if constexpr (SPLIT) {
+            mfmas(1, 0, 1);
+            mfmas(1, 1, 0);
+        } else {
+            mfmas(1, 1, 1);
+        }
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    using B2 = std::integral_constant<int, 2>;
+    if (s0 < s1) {
+        issue(0, s0);
+        issue(1, s0 + 1 < s1 ? s0 + 1 : s0);
+        __builtin_amdgcn_s_waitcnt(wait_vm(kLoads));
+        asm volatile("s_barrier" ::: "memory");
+        reads(ring[0], 0);
+        int64_t st = s0;
+        for (; st + 3 <= s1; st += 3) {
+            stage(B0{}, st);
+            stage(B1{}, st + 1);
+            stage(B2{}, st + 2);
+        }
+        if (st < s1) stage(B0{}, st);
+        if (st + 1 < s1) stage(B1{}, st + 1);
+        __builtin_amdgcn_s_waitcnt(0);  // no direct load still writing LDS
+    }
+    epi(acc, MmaTile{i0, k0, wm, wn, lane, M, N, split, reinterpret_cast<char*>(&ring[0][0])});
+}
+
+// Launches C = A·Bᵀ over an upper bound of its tiles.
+template <bool SPLIT, class Epi>
+int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
+    const int64_t groups = ceil_div(g.M, kTileM) * ceil_div(g.N, kTileN) * g.splits;
+    if (groups == 0) return SLK_OK;
+    if (groups > INT32_MAX) return fail(SLK_EINVAL, std::string(who) + ": too many tiles");
+    hipLaunchKernelGGL((mma_kernel<SPLIT, Epi>), dim3(static_cast<unsigned>(groups)),
+                       dim3(kMmaThreads), 0, st, g, epi);
+    return check_launch(who);
+}
+
+}  // namespace slk

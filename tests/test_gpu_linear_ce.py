@@ -1,0 +1,306 @@
+"""linear_cross_entropy against its definition in float64, and its gradient against
+differences.
+
+Bounds, with S = Σ_k |h_k w_k| of a logit. A float32 operand is kept to 2^-22 of itself,
+the product of the two low parts is dropped (2^-22) and the sum is float32: a logit is off
+by e_z = 2^-20 S at most (bfloat16 operands: exact products, the same sum). A loss is then
+off by 2 max e_z and its own rounding. A softmax entry p is off by 2 p max e_z and a few
+units of p, dl = p - onehot is kept to 2^-38 of 1 (float32) or 2^-8 of itself
+(bfloat16), and the gradients are sums of |dl error| · |operand| plus 2^-20 of their own
+terms' absolute sum; bfloat16 results round once more, by 2^-8 at most.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import sparsecore_amd as slk
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -20
+
+
+def make(n, d, v, dtype, dev, seed=0, ignored=0.0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    h = (torch.randn(n, d, generator=g) * scale).to(dtype)
+    w = (torch.randn(v, d, generator=g) * 2 / math.sqrt(d)).to(dtype)
+    t = torch.randint(0, v, (n,), generator=g)
+    t[torch.rand(n, generator=g) < ignored] = -100
+    return h.to(dev), w.to(dev), t.to(dev)
+
+
+def reference(h, w, t, up, ignore=-100):
+    """(losses, dh, dw, and their bounds) for upstream gradients `up` of each token."""
+    dtype = h.dtype
+    h, w, t, up = h.detach().double(), w.detach().double(), t, up.double()
+    live = t != ignore
+    h = torch.where(live[:, None], h, 0.0)
+    z = h @ w.t()
+    ez = 2 * E * (h.abs() @ w.abs().t()).amax(1, keepdim=True) if w.numel() else z
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    idx = torch.where(live, t, 0)[:, None]
+    losses = torch.where(live, (lse - z.gather(1, idx)).squeeze(1), 0.0)
+    loss_err = torch.where(live, ez.squeeze(1) + 2e-6 * (1 + lse.squeeze(1).abs()
+                                                        + z.gather(1, idx).squeeze(1).abs()), 0.0)
+    p = torch.exp(z - lse)
+    dl = p.scatter_add(1, idx, -torch.ones_like(lse))
+    err = p * (ez + 2e-6) + 2.0 ** -38
+    if dtype is torch.bfloat16:
+        err = err + 2.0 ** -8 * dl.abs()
+    g = torch.where(live, up, 0.0)[:, None]
+    top = g.abs().max() if g.numel() else 0.0
+    dl, err = dl * g, torch.where(live[:, None], err * g.abs() + 2.0 ** -38 * top, 0.0)
+    dh, dw = dl @ w, dl.t() @ h
+    dh_err = err @ w.abs() + E * (dl.abs() @ w.abs())
+    dw_err = err.t() @ h.abs() + E * (dl.abs().t() @ h.abs())
+    if dtype is torch.bfloat16:
+        dh_err, dw_err = dh_err + 2.0 ** -8 * dh.abs(), dw_err + 2.0 ** -8 * dw.abs()
+    return losses, loss_err, dh, dh_err, dw, dw_err
+
+
+def within(got, want, err, what):
+    got = got.detach().double()
+    assert got.shape == want.shape, what
+    far = (got - want).abs() - err
+    assert bool((far <= 0).all()), f"{what}: {float(far.max()):.3g} beyond"
+
+
+def check(dev, n, d, v, dtype, ignored=0.0, reduction="mean", seed=0, scale=1.0):
+    h, w, t = make(n, d, v, dtype, dev, seed, ignored, scale)
+    h.requires_grad_(), w.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t, reduction=reduction)
+    live = int((t != -100).sum())
+    if reduction == "none":
+        up = torch.randn(n, generator=torch.Generator().manual_seed(9)).to(dev)
+        losses, lerr, dh, eh, dw, ew = reference(h, w, t, up)
+        within(loss, losses, lerr, "loss")
+    else:
+        up = torch.tensor(0.37, device=dev)
+        share = 0.37 / live if reduction == "mean" and live else 0.37
+        each = torch.full((n,), share, dtype=torch.float64, device=dev)
+        losses, lerr, dh, eh, dw, ew = reference(h, w, t, each)
+        if reduction == "mean" and not live:
+            assert bool(torch.isnan(loss))
+        else:
+            by = live if reduction == "mean" else 1
+            within(loss, losses.sum() / by, lerr.sum() / by + 1e-6 * losses.sum() / by, "loss")
+        eh, ew = eh + 2e-7 * dh.abs(), ew + 2e-7 * dw.abs()  # the factor's rounding
+    gh, gw = torch.autograd.grad(loss, [h, w], up)
+    within(gh, dh, eh, "dh")
+    within(gw, dw, ew, "dw")
+    assert gh.dtype == dtype and gw.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (1, 64, 65), (2, 3, 2), (31, 32, 33), (128, 64, 256),
+                                   (129, 65, 257), (300, 200, 1000), (1000, 384, 65),
+                                   (65, 1000, 4099), (513, 96, 513)])
+def test_sizes(dev, dtype, n, d, v):
+    check(dev, n, d, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("ignored", [0.0, 0.3, 0.97, 1.0])
+def test_reductions_and_ignored_tokens(dev, dtype, reduction, ignored):
+    check(dev, 200, 80, 300, dtype, ignored, reduction)
+    check(dev, 1, 80, 300, dtype, ignored, reduction)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_tokens_and_a_large_vocabulary(dev, dtype):
+    check(dev, 9000, 64, 300, dtype, 0.2)
+    check(dev, 70, 128, 33000, dtype, 0.2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pieces_of_the_vocabulary(dev, dtype):
+    """More logits than a piece of the backward holds: 2^30 bytes of logit gradients are
+    8192 x 16384 in float32 and twice as many in bfloat16."""
+    n, d, v = 8192, 48, 40000
+    h, w, t = make(n, d, v, dtype, dev, 1, 0.1)
+    h.requires_grad_(), w.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t, reduction="sum")
+    gh, gw = torch.autograd.grad(loss, [h, w])
+    for lo in (0, 16384 - 100, 32768 - 100, v - 100):  # rows of dw around the pieces' ends
+        rows = slice(lo, lo + 200)
+        z = h.detach().double() @ w.detach().double().t()
+        p = torch.exp(z[:, rows] - torch.logsumexp(z, 1, keepdim=True))
+        del z
+        live = (t != -100)[:, None]
+        hit = (t[:, None] == torch.arange(v, device=dev)[rows]) & live
+        dl = torch.where(live, p - hit.double(), 0.0)
+        want = dl.t() @ h.detach().double()
+        terms = dl.abs().t() @ h.detach().double().abs()
+        tol = (2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -17) * terms \
+            + 2.0 ** -38 * h.detach().double().abs().sum(0)
+        within(gw[rows], want, tol + 2.0 ** -8 * want.abs() * (dtype is torch.bfloat16), "dw")
+    some = torch.arange(0, n, 331, device=dev)
+    _, _, dh, eh, _, _ = reference(h[some], w, t[some], torch.ones(len(some), device=dev))
+    within(gh[some], dh, eh, "dh")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 15, 16, 17])
+@pytest.mark.parametrize("d,v", [(1, 3), (40, 17), (100, 1), (768, 5000), (130, 777)])
+def test_scores_of_a_few_tokens(dev, dtype, n, d, v):
+    h, w, t = make(n, d, v, dtype, dev, 2)
+    if n > 2:
+        t[1] = -100
+    got = slk.linear_cross_entropy(h, w, t, reduction="none")
+    losses, err, *_ = reference(h, w, t, torch.zeros(n, device=dev))
+    within(got, losses, err, "loss")
+    mean = slk.linear_cross_entropy(h, w, t)
+    live = int((t != -100).sum())
+    within(mean, losses.sum() / live, err.sum() / live + 1e-6 * losses.sum() / live, "mean")
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 30.0, 1e4])
+def test_ranges_of_float32(dev, scale):
+    """Hidden states far from 1 keep their relative precision (the power-of-two scaling);
+    at 30 and 1e4 the softmax is one-hot."""
+    check(dev, 100, 64, 200, torch.float32, scale=scale)
+
+
+def test_small_rows_beside_large_ones(dev):
+    """Rows a thousandth of the largest: every logit stays within its own bound."""
+    h, w, t = make(64, 96, 300, torch.float32, dev, 3)
+    h = h * torch.logspace(-3, 1, 64, device=dev)[:, None]
+    losses, err, *_ = reference(h, w, t, torch.zeros(64, device=dev))
+    within(slk.linear_cross_entropy(h, w, t, reduction="none"), losses, err, "loss")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_ignored_tokens_reach_nothing(dev, dtype, bad):
+    h, w, t = make(50, 64, 100, dtype, dev, 4)
+    t[::3] = -100
+    h[::3] = bad
+    h.requires_grad_(), w.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t)
+    gh, gw = torch.autograd.grad(loss, [h, w])
+    up = torch.full((50,), 1.0 / int((t != -100).sum()), dtype=torch.float64, device=dev)
+    losses, lerr, dh, eh, dw, ew = reference(h, w, t, up)
+    count = int((t != -100).sum())
+    within(loss, losses.sum() / count, lerr.sum() / count + 1e-6, "loss")
+    within(gh, dh, eh + 2e-7 * dh.abs(), "dh")
+    within(gw, dw, ew + 2e-7 * dw.abs(), "dw")
+    assert bool((gh[::3] == 0).all())
+
+
+def test_a_live_nan_stays_in_its_loss_and_dh(dev):
+    h, w, t = make(40, 64, 100, torch.float32, dev, 5)
+    clean = slk.linear_cross_entropy(h, w, t, reduction="none")
+    h[7, 3] = float("nan")
+    h.requires_grad_()
+    got = slk.linear_cross_entropy(h, w, t, reduction="none")
+    keep = torch.arange(40, device=dev) != 7
+    torch.testing.assert_close(got[keep], clean[keep], rtol=1e-6, atol=1e-6)
+    assert bool(torch.isnan(got[7]))
+    gh, = torch.autograd.grad(got, h, torch.ones_like(got))
+    assert bool(torch.isfinite(gh[keep]).all()) and bool(torch.isnan(gh[7]).all())
+
+
+def test_targets_outside_the_vocabulary(dev):
+    for n in (8, 40):
+        h, w, t = make(n, 64, 100, torch.float32, dev, 6)
+        clean = slk.linear_cross_entropy(h, w, t, reduction="none")
+        t[2], t[5] = 100, -7
+        got = slk.linear_cross_entropy(h, w, t, reduction="none")
+        assert bool(torch.isnan(got[[2, 5]]).all())
+        keep = [i for i in range(n) if i not in (2, 5)]
+        assert torch.equal(got[keep], clean[keep])
+        h.requires_grad_(), w.requires_grad_()
+        loss = slk.linear_cross_entropy(h, w, t)
+        assert bool(torch.isnan(loss))
+        gh, gw = torch.autograd.grad(loss, [h, w])
+        assert bool(torch.isfinite(gh).all()) and bool(torch.isfinite(gw).all())
+
+
+def test_another_ignore_index_and_leading_sizes(dev):
+    h, w, t = make(24, 64, 100, torch.float32, dev, 7)
+    t[3] = 0
+    a = slk.linear_cross_entropy(h.reshape(2, 12, 64), w, t.reshape(2, 12), ignore_index=0,
+                                 reduction="none")
+    losses, err, *_ = reference(h, w, t, torch.zeros(24, device=dev), ignore=0)
+    assert a.shape == (2, 12)
+    within(a.reshape(-1), losses, err, "loss")
+
+
+def test_gradient_against_differences(dev):
+    """Central differences along random directions, step 2^-6: truncation h² times a
+    third derivative of order 1 (2e-4), rounding about 2^-20 / h (6e-5)."""
+    h, w, t = make(20, 32, 50, torch.float32, dev, 8)
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    grads = torch.autograd.grad(slk.linear_cross_entropy(hg, wg, t), [hg, wg])
+    step = 2.0 ** -6
+    for k, g in enumerate(grads):
+        way = torch.randn(g.shape, generator=torch.Generator().manual_seed(k)).to(dev)
+        way /= way.norm()
+        f = [slk.linear_cross_entropy(h + s * step * way * (k == 0) if k == 0 else h,
+                                      w + s * step * way if k == 1 else w, t, reduction="none")
+             .double().mean() for s in (1, -1)]
+        assert abs(float(f[0] - f[1]) / (2 * step) - float((g * way).sum())) < 3e-4
+
+
+def test_results_repeat_and_other_streams(dev):
+    h, w, t = make(700, 200, 900, torch.float32, dev, 9, 0.2)
+    h.requires_grad_(), w.requires_grad_()
+
+    def once():
+        loss = slk.linear_cross_entropy(h, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, w]))
+
+    a = once()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        b = once()
+    s.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_one_gradient_alone_and_none(dev):
+    h, w, t = make(100, 64, 300, torch.float32, dev, 10)
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    both = torch.autograd.grad(slk.linear_cross_entropy(hg, wg, t), [hg, wg])
+    one, = torch.autograd.grad(slk.linear_cross_entropy(hg, w, t), hg)
+    other, = torch.autograd.grad(slk.linear_cross_entropy(h, wg, t), wg)
+    assert torch.equal(one, both[0]) and torch.equal(other, both[1])
+    assert not slk.linear_cross_entropy(h, w, t).requires_grad
+
+
+def test_no_tokens(dev):
+    h = torch.zeros(0, 64, device=dev, requires_grad=True)
+    w = torch.ones(10, 64, device=dev, requires_grad=True)
+    t = torch.zeros(0, dtype=torch.int64, device=dev)
+    loss = slk.linear_cross_entropy(h, w, t, reduction="sum")
+    loss.backward()
+    assert float(loss) == 0 and bool((w.grad == 0).all()) and h.grad.shape == (0, 64)
+    assert bool(torch.isnan(slk.linear_cross_entropy(h, w, t)))
+
+
+def test_refusals(dev):
+    h, w, t = make(4, 8, 10, torch.float32, dev)
+    f = slk.linear_cross_entropy
+    with pytest.raises(TypeError):
+        f(h, w, [1, 2, 3, 4])
+    with pytest.raises(RuntimeError, match="HIP"):
+        f(h.cpu(), w, t)
+    with pytest.raises(RuntimeError, match="HIP"):
+        f(h, w, t.cpu())
+    with pytest.raises(ValueError, match="reduction"):
+        f(h, w, t, reduction="max")
+    with pytest.raises(ValueError, match="int64"):
+        f(h, w, t.int())
+    with pytest.raises(ValueError, match="float32 or both"):
+        f(h, w.bfloat16(), t)
+    with pytest.raises(ValueError, match="float32 or both"):
+        f(h.half(), w.half(), t)
+    for bad in ((h[:, :7], w, t), (h, w, t[:3]), (h, w[0], t), (h[0], w, t)):
+        with pytest.raises(ValueError):
+            f(*bad)
