@@ -211,8 +211,22 @@ __device__ __forceinline__ float logit_scale(const Header* hd) {
     return SPLIT ? pow2(-scale_exp(hd->top_h)) * pow2(-scale_exp(hd->top_w)) : 1.0f;
 }
 
-// Forward: rows are the vocabulary, columns tokens, so that a lane holds 32
-// logits of each of its two tokens and only their maximum and sum cross lanes.
+// Logits are exponentiated in base 2: the factor log2(e) goes into the scale of
+// the accumulator, and v_exp_f32 is one instruction (1 ulp). Maxima and sums
+// travel in base 2 too (m, Σ 2^(z·log2 e - m)).
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// (m, s) joined with (m2, s2); an empty part has m = -inf, s = 0. A NaN stays in s.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+    s = (m == -INFINITY ? s : s * exp2_(m - base)) + (m2 == -INFINITY ? s2 : s2 * exp2_(m2 - base));
+    m = top;
+}
+
+// Forward: rows are the vocabulary, columns tokens, so that a lane holds half of
+// its wave's logits of each of its two tokens and only their maximum and sum
+// cross lanes.
 template <bool SPLIT>
 struct ScoreEpi {
     const Header* hd;
@@ -220,45 +234,53 @@ struct ScoreEpi {
     float2* part;  // vocabulary tiles x tokens
     float* zt;
     int64_t n;
-    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         __syncthreads();  // the ring is free
-        float2* sh = reinterpret_cast<float2*>(t.lds);  // 4 x kTileN
-        const float scale = logit_scale<SPLIT>(hd);
+        float2* sh = reinterpret_cast<float2*>(t.lds);  // kWavesM x kBN
+        const float scale = logit_scale<SPLIT>(hd), scale2 = scale * kLog2e;
+        const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t tok = t.n0() + t.col(b);
-            const int32_t want = tok < t.N ? tgt[tok] : -1;
+            const int64_t want = (tok < t.N ? tgt[tok] : -1) - t.m0();
+            const bool here = want >= 0 && want < 32 * Tile::kNA;
+            if (__any(here)) {
+#pragma unroll
+                for (int a = 0; a < Tile::kNA; ++a)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (t.row(a, r) == want) zt[tok] = acc[a][b][r] * scale;
+            }
             float m = -INFINITY, s = 0.0f;
+            if (rows < 32 * Tile::kNA) {  // past the vocabulary
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int64_t row = t.m0() + t.row(a, r);
-                    const float z = acc[a][b][r] * scale;
-                    if (row == want) zt[tok] = z;
-                    acc[a][b][r] = row < t.M ? z : -INFINITY;
-                    m = fmaxf(m, acc[a][b][r]);
-                }
-            m = fmaxf(m, __shfl_xor(m, 32));
+                    for (int r = 0; r < 16; ++r)
+                        if (t.row(a, r) >= rows) acc[a][b][r] = -INFINITY;
+            }
+#pragma unroll
+            for (int a = 0; a < Tile::kNA; ++a)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[a][b][r]);
+            m = fmaxf(m, __shfl_xor(m, 32)) * scale2;  // the scale is positive
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += expf(acc[a][b][r] - base);
+                for (int r = 0; r < 16; ++r) s += exp2_(fmaf(acc[a][b][r], scale2, -base));
             s += __shfl_xor(s, 32);
-            if (t.lane < 32) sh[t.wm * kTileN + 64 * t.wn + t.col(b)] = make_float2(m, s);
+            if (t.lane < 32) sh[t.wm * Tile::kBN + 64 * t.wn + t.col(b)] = make_float2(m, s);
         }
         __syncthreads();
-        if (threadIdx.x < kTileN) {
+        if (threadIdx.x < Tile::kBN) {
             const int64_t tok = t.k0 + threadIdx.x;
             float m = -INFINITY, s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, sh[w * kTileN + threadIdx.x].x);
-            const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float2 x = sh[w * kTileN + threadIdx.x];
-                s += x.x == -INFINITY ? x.y : x.y * expf(x.x - base);
+            for (int w = 0; w < Tile::kWavesM; ++w) {
+                const float2 x = sh[w * Tile::kBN + threadIdx.x];
+                join(m, s, x.x, x.y);
             }
             if (tok < t.N) part[t.i0 / kTileM * n + tok] = make_float2(m, s);
         }
@@ -277,25 +299,28 @@ struct DlEpi {
     char* by_voc;
     int64_t v0;      // first row of the piece
     int64_t n, voc;  // rows that the two are laid out for
-    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
-        const float scale = logit_scale<SPLIT>(hd);
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
+        const float scale2 = logit_scale<SPLIT>(hd) * kLog2e;
+        const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
         constexpr float up = SPLIT ? static_cast<float>(1 << kDlExp) : 1.0f;
         constexpr int K = kStageK<SPLIT>;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t tok = t.n0() + t.col(b);
             const bool in = tok < t.N;
-            const int64_t want = in ? tgt[tok] - v0 : -1;
-            const float l = in ? lse[tok] : 0.0f;
+            const int64_t want = (in ? tgt[tok] - v0 : -1) - t.m0();
+            const bool here = want >= 0 && want < 32 * Tile::kNA;
+            const bool any = __any(here);
+            const float l = in ? lse[tok] * kLog2e : 0.0f;
             const float g = (in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f) * up;
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
+            for (int a = 0; a < Tile::kNA; ++a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t row = t.m0() + t.row(a, r);
-                    float p = expf(acc[a][b][r] * scale - l);
-                    if (row == want) p -= 1.0f;
-                    acc[a][b][r] = in && row < t.M ? p * g : 0.0f;
+                    float p = exp2_(fmaf(acc[a][b][r], scale2, -l));
+                    if (any && t.row(a, r) == want) p -= 1.0f;
+                    acc[a][b][r] = in && t.row(a, r) < rows ? p * g : 0.0f;
                 }
                 const int64_t v = t.m0() + 32 * a;          // this block's 32 rows
                 const int64_t k = t.n0() + 32 * b;          // and 32 tokens
@@ -339,10 +364,11 @@ struct SumEpi {
     float* out;  // splits x rows x d
     int64_t rows, d;
     bool add;  // onto what the vocabulary's earlier pieces left
-    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         float* to = out + t.split * rows * d;
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+        for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int64_t c = t.n0() + t.col(b);
@@ -378,10 +404,11 @@ struct WeightEpi {
     const float* factor;
     void* out;  // of the piece's first row
     int64_t d;
-    __device__ __forceinline__ void operator()(f32x16 (&acc)[2][2], const MmaTile& t) const {
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         const GradScale<SPLIT> s(hd, factor, true);
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+        for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int64_t c = t.n0() + t.col(b);
@@ -409,7 +436,7 @@ struct JoinArgs {
     int64_t n, v, ignore, parts;
 };
 __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
-    __shared__ float2 sh[32][9];
+    __shared__ float2 sh[4][8];
     const int j = threadIdx.x & 7, part = threadIdx.x >> 3;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + j;
     int64_t i = -1;
@@ -427,27 +454,25 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
     if (i >= 0) {
         for (int64_t k = part; k < p.parts; k += 32) {
             const float2 x = p.part[k * p.n + i];
-            const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
-            s = (m == -INFINITY ? s : s * expf(m - base)) +
-                (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
-            m = top;
+            join(m, s, x.x, x.y);
         }
     }
-    sh[part][j] = make_float2(m, s);
+    // lanes 8 apart hold a token's parts: within the wave, then over the four waves
+#pragma unroll
+    for (int o = 8; o < kWave; o <<= 1) {
+        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+        join(m, s, m2, s2);
+    }
+    if ((threadIdx.x & (kWave - 1)) < 8) sh[threadIdx.x >> 6][j] = make_float2(m, s);
     __syncthreads();
     if (part != 0 || n >= p.n) return;
-    for (int k = 1; k < 32; ++k) {
-        const float2 x = sh[k][j];
-        const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
-        s = (m == -INFINITY ? s : s * expf(m - base)) +
-            (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
-        m = top;
-    }
+#pragma unroll
+    for (int k = 1; k < 4; ++k) join(m, s, sh[k][j].x, sh[k][j].y);
     if (i < 0) {
         p.losses[n] = 0.0f;
         return;
     }
-    const float lse = (m == -INFINITY ? 0.0f : m) + logf(s);
+    const float lse = ((m == -INFINITY ? 0.0f : m) + log2f(s)) * kLn2;
     if (p.lse != nullptr) p.lse[i] = lse;
     p.losses[n] = valid ? lse - p.zt[i] : NAN;
 }
@@ -613,13 +638,13 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
             const int64_t vr = blk * 16 + 4 * quarter + r;
             z[r] = acc[0][r] + acc[1][r];
             if (vr == want && col < n) zt[col] = z[r];
-            if (vr >= v) z[r] = -INFINITY;
+            z[r] = vr >= v ? -INFINITY : z[r] * kLog2e;
             top = fmaxf(top, z[r]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
-        s = m == -INFINITY ? s : s * expf(m - base);
+        s = m == -INFINITY ? s : s * exp2_(m - base);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += expf(z[r] - base);
+        for (int r = 0; r < 4; ++r) s += exp2_(z[r] - base);
         m = top;
     }
     // the lanes of a token, then the waves
@@ -627,10 +652,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) {
         const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
-        const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
-        s = (m == -INFINITY ? s : s * expf(m - base)) +
-            (m2 == -INFINITY ? s2 : s2 * expf(m2 - base));
-        m = top;
+        join(m, s, m2, s2);
     }
     if (lane < kFewTokens) sh[wv][lane] = make_float2(m, s);
     __syncthreads();
@@ -639,10 +661,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
         s = sh[0][threadIdx.x].y;
         for (int k = 1; k < kFewThreads / kWave; ++k) {
             const float2 x = sh[k][threadIdx.x];
-            const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
-            s = (m == -INFINITY ? s : s * expf(m - base)) +
-                (x.x == -INFINITY ? x.y : x.y * expf(x.x - base));
-            m = top;
+            join(m, s, x.x, x.y);
         }
         part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = make_float2(m, s);
     }
@@ -716,16 +735,21 @@ Forward forward_of(const slk_linear_ce* a) {
 // takes at most kDlBytes.
 constexpr int64_t kDlBytes = int64_t{1} << 30;
 
-// Parts of a product's K loop: with one workgroup a CU, `tiles` of them take
-// ceil(tiles·s / 256) rounds of 1/s of the loop each; every part also costs
-// the writing and reading of its sums (taken as 2% of the loop).
-int splits_for(int64_t tiles, int64_t nst) {
+// Parts of a product's K loop. With one workgroup a CU, tiles·s of them take
+// ceil(tiles·s / 256) rounds of 1/s of the loop each (about 1.1 us a stage of a
+// 256 x 128 tile); more than one part also writes and reads its sums.
+int splits_for(int64_t m, int64_t n, int64_t nst) {
+    const double sums = 1e-6 * static_cast<double>(m) * static_cast<double>(n) / 4.5;  // us a byte
     int best = 1;
     double cost = 1e30;
     for (int s = 1; s <= 32; ++s) {
         if (s > 1 && nst < 8 * s) break;
-        const double c = static_cast<double>(ceil_div(tiles * s, 256)) / s + 0.02 * s;
-        if (c < cost - 1e-9) {
+        const bool wide = mma_wide(m, n, s);
+        const int64_t tiles = ceil_div(m, kTileM) * ceil_div(n, wide ? kWideN : kTileN);
+        const double c = static_cast<double>(ceil_div(tiles * s, 256)) * (wide ? 1.7 : 1.0) * 1.1 *
+                             static_cast<double>(nst) / s +
+                         (s > 1 ? sums * (8.0 * s + 4.0) + 5.0 : 0.0);
+        if (c < cost) {
             cost = c;
             best = s;
         }
@@ -740,20 +764,21 @@ struct Backward {
 };
 Backward backward_of(const slk_linear_ce* a) {
     Backward b;
-    const int64_t n128 = ceil_div(a->n, kTileN) * kTileN;
-    const int64_t per_row = n128 * (split_of(a) ? 8 : 4);
+    // (the epilogue writes whole tiles of tokens)
+    const int64_t n_up = ceil_div(a->n, kWideN) * kWideN;
+    const int64_t per_row = n_up * (split_of(a) ? 8 : 4);
     int64_t rows = kDlBytes / per_row / kTileM * kTileM;
     if (rows < kTileM) rows = kTileM;
     const int64_t all = ceil_div(a->v, kTileM) * kTileM;
     const int64_t pieces = ceil_div(all, rows < all ? rows : all);
     b.piece = ceil_div(ceil_div(all, pieces), kTileM) * kTileM;
-    b.sh = splits_for(ceil_div(a->n, kTileM) * ceil_div(a->d, kTileN), stages(a, b.piece));
-    b.sw = splits_for(b.piece / kTileM * ceil_div(a->d, kTileN), stages(a, a->n));
+    b.sh = splits_for(a->n, a->d, stages(a, b.piece));
+    b.sw = splits_for(b.piece, a->d, stages(a, a->n));
     Carve c;
     b.factor = c.take(4);
     b.gr = c.take(4 * a->n);
     b.by_tok = c.take(stages(a, b.piece) * a->n * kStageBytes);
-    b.by_voc = c.take(stages(a, n128) * b.piece * kStageBytes);
+    b.by_voc = c.take(stages(a, n_up) * b.piece * kStageBytes);
     b.dh = c.take(a->dhidden != nullptr ? 4 * b.sh * a->n * a->d : 0);
     b.dw = c.take(a->dweight != nullptr && b.sw > 1 ? 4 * b.sw * b.piece * a->d : 0);
     b.bytes = c.at;

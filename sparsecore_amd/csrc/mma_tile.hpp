@@ -56,16 +56,18 @@ struct MmaArgs {
     int splits;              // parts of the K loop, each a workgroup of its own
 };
 
-// What an epilogue gets: its wave's 64 x 64 of the tile. Lane l, register r of
-// block [a][b]: row  m0 + 32 a + 8 (r / 4) + 4 (l / 32) + r % 4,
-//               column n0 + 32 b + l % 32.
+// What an epilogue gets: its wave's NA x 2 blocks of 32 x 32 of a tile of
+// 256 x BN. Lane l, register r of block [a][b]:
+//   row  m0 + 32 a + 8 (r / 4) + 4 (l / 32) + r % 4,  column  n0 + 32 b + l % 32.
+template <int NA, int BN>
 struct MmaTile {
+    static constexpr int kNA = NA, kBN = BN, kWavesM = kTileM / (32 * NA);
     int64_t i0, k0;  // the workgroup's tile
     int wm, wn, lane;
     int64_t M, N;
     int split;
-    char* lds;  // kMmaLds bytes, free after a barrier
-    __device__ __forceinline__ int64_t m0() const { return i0 + 64 * wm; }
+    char* lds;  // at least 96 KiB, free after a barrier
+    __device__ __forceinline__ int64_t m0() const { return i0 + 32 * NA * wm; }
     __device__ __forceinline__ int64_t n0() const { return k0 + 64 * wn; }
     __device__ __forceinline__ int row(int a, int r) const {
         return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
@@ -228,17 +230,222 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
         if (st + 1 < s1) stage(B1{}, st + 1);
         __builtin_amdgcn_s_waitcnt(0);  // no direct load still writing LDS
     }
-    epi(acc, MmaTile{i0, k0, wm, wn, lane, M, N, split, reinterpret_cast<char*>(&ring[0][0])});
+    epi(acc, MmaTile<2, kTileN>{i0, k0, wm, wn, lane, M, N, split,
+                                reinterpret_cast<char*>(&ring[0][0])});
 }
 
-// Launches C = A·Bᵀ over an upper bound of its tiles.
+// The same product in tiles of 256 x 256: eight waves of 128 x 64 (2 x 4), a
+// ring of two stages of 64 KiB. A wave reads six fragments for eight
+// instructions (24 of a split operand's), where the smaller tile reads eight
+// for eight: with one a stage of the bfloat16 product kept the LDS busy for
+// 1408 cycles (reads, and the direct loads' writes) against 1024 of the matrix
+// cores, now for 2048 against 2048. Fragments are read one k-step ahead. The
+// barrier sits before a stage's last k-step, whose fragments are in registers:
+// every wave has read the stage, and its loads of the next have landed; the
+// stage's buffer is then filled with the stage after the next, a whole stage's
+// time before that is read.
+constexpr int kWideN = 256;
+
+template <bool SPLIT, class Epi>
+__global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, const Epi epi) {
+    __shared__ __align__(16) unsigned char ring[2][(kTileM + kWideN) * kStageBytes];
+
+    int64_t M = g.M, N = g.N, nst = g.nst;
+    if (g.which != kLiveNone) {
+        const int64_t live = *g.live;
+        if (g.which == kLiveM) M = live;
+        else if (g.which == kLiveN) N = live;
+        else nst = ceil_div(live, kStageK<SPLIT>);
+    }
+    const int64_t nTi = ceil_div(M, kTileM), nTk = ceil_div(N, kWideN);
+    const int64_t tiles = nTi * nTk, total = tiles * g.splits;
+    if (static_cast<int64_t>(blockIdx.x) >= total) return;  // the whole workgroup
+    const int64_t L = xcd_logical_block(blockIdx.x, total);
+    const int split = static_cast<int>(L / tiles);
+    const int64_t tile = L - split * tiles;
+    const int64_t grp = tile / (kMmaGroup * nTk);
+    const int64_t first = grp * kMmaGroup;
+    const int64_t gsize = nTi - first < kMmaGroup ? nTi - first : kMmaGroup;
+    const int64_t in_grp = tile - grp * kMmaGroup * nTk;
+    const int64_t i0 = (first + in_grp % gsize) * kTileM;
+    const int64_t k0 = (in_grp / gsize) * kWideN;
+    const int64_t s0 = split * nst / g.splits, s1 = (split + 1) * nst / g.splits;
+
+    const int t = threadIdx.x;
+    const int lane = t & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wm = wv >> 2, wn = wv & 3;
+
+    constexpr int kPer = kTileM / 64;  // loads of a wave and stage, of each operand
+    uint32_t offA[kPer], offB[kPer];
+    auto plan = [&](int64_t R, int64_t r0, int i) {
+        const int rr = 8 * i + lane / 8;
+        int64_t r = r0 + rr;
+        if (r >= R) r = R - 1;
+        return static_cast<uint32_t>(r * kStageBytes + 16 * ((lane & 7) ^ ((rr >> 1) & 7)));
+    };
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        offA[q] = plan(M, i0, wv + 8 * q);
+        offB[q] = plan(N, k0, wv + 8 * q);
+    }
+    const char* A = static_cast<const char*>(g.A);
+    const char* B = static_cast<const char*>(g.B);
+    auto issue = [&](int buf, int64_t st) {
+        const char* a = A + st * g.rows_a * kStageBytes;
+        const char* b = B + st * g.rows_b * kStageBytes;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+            __builtin_amdgcn_global_load_lds(a + offA[q], &ring[buf][1024 * (wv + 8 * q)], 16, 0,
+                                             0);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+            __builtin_amdgcn_global_load_lds(
+                b + offB[q], &ring[buf][kTileM * kStageBytes + 1024 * (wv + 8 * q)], 16, 0, 0);
+    };
+
+    f32x16 acc[4][2];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
+
+    const int half = lane >> 5;
+    const int rA = wm * 128 + (lane & 31), rB = wn * 64 + (lane & 31);
+    using Frag = std::conditional_t<SPLIT, f16x8, b16x8>;
+    // [set][block]; a set is a k-step's parity, or (SPLIT) 0: high parts, 1: low parts
+    Frag af[2][4], bf[2][2];
+    auto frag = [&](const unsigned char* lds, int r, int c) {
+        return *reinterpret_cast<const Frag*>(lds + 16 * (r * 8 + (c ^ ((r >> 1) & 7))));
+    };
+    // piece c of the rows of A (first two, last two blocks) and of B
+    auto read_a = [&](const unsigned char* buf, int c, int set, int a0) {
+#pragma unroll
+        for (int a = a0; a < a0 + 2; ++a) af[set][a] = frag(buf, rA + 32 * a, c + half);
+    };
+    auto read_b = [&](const unsigned char* buf, int c, int set) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            bf[set][b] = frag(buf + kTileM * kStageBytes, rB + 32 * b, c + half);
+    };
+    auto mfmas = [&](int a, int sa, int sb) {  // one row of blocks
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if constexpr (SPLIT) {
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[sa][a], bf[sb][b], acc[a][b],
+                                                                   0, 0, 0);
+            } else {
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[sa][a], bf[sb][b],
+                                                                    acc[a][b], 0, 0, 0);
+            }
+        }
+    };
+    // Eight instructions with other work between them: the matrix cores take 32
+    // cycles each, during which the wave issues the work. The reads that they
+    // use were issued eight instructions ago, so the wait before them is free.
+    auto eight = [&](int sa, int sb, auto&& w0, auto&& w1, auto&& w2) {
+        __builtin_amdgcn_s_waitcnt(wait_vm(63));
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(0, sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        w0();
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(1, sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        w1();
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(2, sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        w2();
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(3, sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto none = [] {};
+    auto meet = [&] {
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+        asm volatile("s_barrier" ::: "memory");
+    };
+    // A k-step's fragments ahead of its instructions: all of the next k-step's
+    // (bfloat16); of a split operand the part whose registers the last eight
+    // instructions freed (the order lo·hi, hi·hi, hi·lo makes that three groups).
+    auto stage = [&](auto I, int64_t st) {
+        constexpr int buf = decltype(I)::value;
+        const unsigned char* cur = ring[buf];
+        const unsigned char* nxt = ring[buf ^ 1];
+        // past the end the last stage is loaded again, unused
+        const int64_t ahead = st + 2 < s1 ? st + 2 : s1 - 1;
+        if constexpr (SPLIT) {
+            eight(1, 0, [&] { read_a(cur, 0, 0, 0); }, [&] { read_a(cur, 0, 0, 2); },
+                  [&] { read_b(cur, 4, 1); });
+            eight(0, 0, [&] { read_a(cur, 6, 1, 0); }, [&] { read_a(cur, 6, 1, 2); }, none);
+            eight(0, 1, [&] { read_b(cur, 2, 0); }, none, none);
+            eight(1, 0, [&] { read_a(cur, 2, 0, 0); }, [&] { read_a(cur, 2, 0, 2); },
+                  [&] { read_b(cur, 6, 1); });
+            meet();
+            eight(0, 0, [&] { read_a(nxt, 4, 1, 0); },
+                  [&] { read_a(nxt, 4, 1, 2); }, [&] { issue(buf, ahead); });
+            eight(0, 1, [&] { read_b(nxt, 0, 0); }, none, none);
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < 3; ++ks) {
+                const int c = 2 * ks + 2, set = (ks + 1) & 1;
+                eight(ks & 1, ks & 1, [&] { read_b(cur, c, set); }, [&] { read_a(cur, c, set, 0); },
+                      [&] { read_a(cur, c, set, 2); });
+            }
+            meet();
+            eight(1, 1, [&] { read_b(nxt, 0, 0); read_a(nxt, 0, 0, 0); },
+                  [&] { read_a(nxt, 0, 0, 2); }, [&] { issue(buf, ahead); });
+        }
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    if (s0 < s1) {
+        issue(0, s0);
+        issue(1, s0 + 1 < s1 ? s0 + 1 : s0);
+        __builtin_amdgcn_s_waitcnt(wait_vm(2 * kPer));
+        asm volatile("s_barrier" ::: "memory");
+        if (SPLIT) {
+            read_a(ring[0], 4, 1, 0);
+            read_a(ring[0], 4, 1, 2);
+        } else {
+            read_a(ring[0], 0, 0, 0);
+            read_a(ring[0], 0, 0, 2);
+        }
+        read_b(ring[0], 0, 0);
+        int64_t st = s0;
+        for (; st + 2 <= s1; st += 2) {
+            stage(B0{}, st);
+            stage(B1{}, st + 1);
+        }
+        if (st < s1) stage(B0{}, st);
+        __builtin_amdgcn_s_waitcnt(0);  // no direct load still writing LDS
+    }
+    epi(acc, MmaTile<4, kWideN>{i0, k0, wm, wn, lane, M, N, split,
+                                reinterpret_cast<char*>(&ring[0][0])});
+}
+
+// Launches C = A·Bᵀ over an upper bound of its tiles. Wide tiles where their
+// rounds on the card's 256 CUs take no longer: a wide stage takes about 1.7
+// times a small one's.
+inline bool mma_wide(int64_t M, int64_t N, int splits) {
+    const int64_t small = ceil_div(ceil_div(M, kTileM) * ceil_div(N, kTileN) * splits, 256);
+    const int64_t wide = ceil_div(ceil_div(M, kTileM) * ceil_div(N, kWideN) * splits, 256);
+    return 17 * wide <= 10 * small;
+}
+
 template <bool SPLIT, class Epi>
 int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
-    const int64_t groups = ceil_div(g.M, kTileM) * ceil_div(g.N, kTileN) * g.splits;
+    const bool wide = mma_wide(g.M, g.N, g.splits);
+    const int64_t groups =
+        ceil_div(g.M, kTileM) * ceil_div(g.N, wide ? kWideN : kTileN) * g.splits;
     if (groups == 0) return SLK_OK;
     if (groups > INT32_MAX) return fail(SLK_EINVAL, std::string(who) + ": too many tiles");
-    hipLaunchKernelGGL((mma_kernel<SPLIT, Epi>), dim3(static_cast<unsigned>(groups)),
-                       dim3(kMmaThreads), 0, st, g, epi);
+    const dim3 grid(static_cast<unsigned>(groups)), wg(kMmaThreads);
+    if (wide) hipLaunchKernelGGL((mma_wide_kernel<SPLIT, Epi>), grid, wg, 0, st, g, epi);
+    else hipLaunchKernelGGL((mma_kernel<SPLIT, Epi>), grid, wg, 0, st, g, epi);
     return check_launch(who);
 }
 
