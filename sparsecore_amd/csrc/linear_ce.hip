@@ -26,12 +26,18 @@ namespace {
 constexpr int kTopExp = 14, kDlExp = 14;
 
 // What forward leaves for backward: counts and the operands' largest magnitudes.
+// The magnitudes are maxima over kTops places, each its own 128 bytes: on one
+// place the atomics of a few hundred workgroups took longer than the reading.
+constexpr int kTops = 8;
+struct Top {
+    uint32_t h, w;  // bits of the largest finite |h| (live tokens), |W|
+    uint32_t pad[30];
+};
 struct Header {
     int32_t live;
-    uint32_t top_h, top_w;  // bits of the largest finite |h| (live tokens), |W|
-    int32_t pad[13];
+    int32_t pad[31];
+    Top top[kTops];
 };
-static_assert(sizeof(Header) == 64, "one cache line");
 
 __device__ __forceinline__ int scale_exp(uint32_t top) {
     // top in [2^(e-1), 2^e): x·2^(14-e) is below 2^14; no scaling of zeros
@@ -40,6 +46,13 @@ __device__ __forceinline__ int scale_exp(uint32_t top) {
     const int s = kTopExp - e;
     return s > 126 ? 126 : s;
 }
+template <uint32_t Top::*Of>
+__device__ __forceinline__ int scale_exp(const Header* hd) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < kTops; ++k) m = max(m, hd->top[k].*Of);
+    return scale_exp(m);
+}
 __device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or inf past float32's range
     return ldexpf(1.0f, e);
 }
@@ -47,82 +60,122 @@ __device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or inf past float32's 
 // ───────────────────────────── live tokens ─────────────────────────────
 
 // rows[i] = the i-th live token, pos[n] its place or -1, tgt[i] its target (-1
-// if it is no row of the vocabulary: its loss is NaN). One workgroup.
-constexpr int kListThreads = 1024, kListPer = 8;
+// if it is no row of the vocabulary: its loss is NaN). One workgroup, kListPer
+// slabs of consecutive tokens at a time: a token's place is the live tokens of
+// the slabs before, of its slab's earlier waves and of its wave's lower lanes.
+constexpr int kListThreads = 1024, kListPer = 8, kListWaves = kListThreads / kWave;
 __global__ __launch_bounds__(kListThreads) void ce_list_kernel(
     const int64_t* __restrict__ target, int64_t n, int64_t v, int64_t ignore,
     Header* __restrict__ hd, int32_t* __restrict__ rows, int32_t* __restrict__ pos,
     int32_t* __restrict__ tgt) {
-    __shared__ int sums[kListThreads / kWave];
+    static_assert(kListPer * kListWaves == 2 * kWave, "two counts a lane below");
+    __shared__ int counts[kListPer * kListWaves];
     const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x >> 6;
-    int64_t base = 0;
+    int base = 0;
     for (int64_t n0 = 0; n0 < n; n0 += kListThreads * kListPer) {
-        const int64_t at = n0 + static_cast<int64_t>(threadIdx.x) * kListPer;
         int64_t t[kListPer];
-        int mine = 0;
+        uint64_t live[kListPer];
 #pragma unroll
         for (int j = 0; j < kListPer; ++j) {
-            t[j] = at + j < n ? target[at + j] : ignore;
-            mine += t[j] != ignore;
+            const int64_t at = n0 + j * kListThreads + threadIdx.x;
+            t[j] = at < n ? target[at] : ignore;
         }
-        int incl = mine;
+#pragma unroll
+        for (int j = 0; j < kListPer; ++j) {
+            live[j] = __ballot(t[j] != ignore);
+            if (lane == 0) counts[j * kListWaves + wv] = __popcll(live[j]);
+        }
+        __syncthreads();
+        // every wave scans all counts: lane l has 2 l and 2 l + 1
+        const int a = counts[2 * lane], b = counts[2 * lane + 1];
+        int incl = a + b;
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) {
             const int up = __shfl_up(incl, o);
             if (lane >= o) incl += up;
         }
-        if (lane == kWave - 1) sums[wv] = incl;
-        __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < kListThreads / kWave; ++w) {
-            if (w < wv) before += sums[w];
-            all += sums[w];
-        }
-        int64_t i = base + before + incl - mine;
 #pragma unroll
         for (int j = 0; j < kListPer; ++j) {
-            if (at + j >= n) break;
+            const int64_t at = n0 + j * kListThreads + threadIdx.x;
+            const int k = j * kListWaves + wv;  // this wave's count, half of lane k / 2's
+            const int before = __shfl(incl - b - (k & 1 ? 0 : a), k >> 1);
+            const int i = base + before + __popcll(live[j] & ((uint64_t{1} << lane) - 1));
+            if (at >= n) continue;
             if (t[j] != ignore) {
-                rows[i] = static_cast<int32_t>(at + j);
+                rows[i] = static_cast<int32_t>(at);
                 tgt[i] = t[j] >= 0 && t[j] < v ? static_cast<int32_t>(t[j]) : -1;
-                pos[at + j] = static_cast<int32_t>(i);
-                ++i;
+                pos[at] = i;
             } else {
-                pos[at + j] = -1;
+                pos[at] = -1;
             }
         }
-        base += all;
+        base += __shfl(incl, kWave - 1);
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        hd->live = static_cast<int32_t>(base);
-        hd->top_h = 0;
-        hd->top_w = 0;
-    }
+    if (threadIdx.x == 0) hd->live = base;
+    if (threadIdx.x < kTops) hd->top[threadIdx.x].h = hd->top[threadIdx.x].w = 0;
 }
 
-// The largest finite magnitude of a float32 operand; rows of tokens that are
-// not live are skipped (pos; NULL: all rows).
-__global__ __launch_bounds__(256) void ce_top_kernel(const float* __restrict__ x, int64_t rows,
+// The largest finite magnitudes of hidden (live tokens) and weight, float32: a
+// wave a row of either.
+template <bool VEC>
+__global__ __launch_bounds__(256) void ce_top_kernel(const float* __restrict__ h, int64_t n,
+                                                     const float* __restrict__ w, int64_t v,
                                                      int64_t d, const int32_t* __restrict__ pos,
-                                                     uint32_t* __restrict__ top) {
-    uint32_t m = 0;
-    const int64_t total = rows * d;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 4;
-    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < total;
-         i += step) {
+                                                     Header* __restrict__ hd) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
+    uint32_t top[2] = {0, 0};
+    auto see = [](uint32_t& m, float x) {
+        const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+        if (b < 0x7f800000u) m = max(m, b);
+    };
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+         row < n + v; row += waves) {
+        const bool of_h = row < n;
+        if (of_h && pos[row] < 0) continue;
+        const float* x = of_h ? h + row * d : w + (row - n) * d;
+        uint32_t m = 0;
+        if (VEC) {
+            int64_t e = 4 * lane;
+            for (; e + 4 * 3 * kWave < d; e += 4 * 4 * kWave) {
+                f32x4 q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (i + j >= total) break;
-            if (pos != nullptr && pos[(i + j) / d] < 0) continue;
-            const uint32_t b = __float_as_uint(x[i + j]) & 0x7fffffffu;
-            if (b < 0x7f800000u) m = max(m, b);
+                for (int j = 0; j < 4; ++j)
+                    q[j] = *reinterpret_cast<const f32x4*>(x + e + 4 * j * kWave);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) see(m, q[j][i]);
+            }
+            for (; e < d; e += 4 * kWave) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(x + e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) see(m, q[i]);
+            }
+        } else {
+            for (int64_t e = lane; e < d; e += kWave) see(m, x[e]);
         }
+        if (of_h) top[0] = max(top[0], m);
+        else top[1] = max(top[1], m);
     }
+    __shared__ uint32_t sh[2][4];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
-    // a maximum: the same whatever the order
-    if ((threadIdx.x & (kWave - 1)) == 0 && m != 0) atomicMax(top, m);
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            top[k] = max(top[k], static_cast<uint32_t>(__shfl_xor(top[k], o)));
+        if (lane == 0) sh[k][threadIdx.x >> 6] = top[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const uint32_t* x = sh[threadIdx.x];
+        const uint32_t m = max(max(x[0], x[1]), max(x[2], x[3]));
+        Top& t = hd->top[blockIdx.x % kTops];
+        // a maximum: the same whatever the order
+        if (m != 0) atomicMax(threadIdx.x == 0 ? &t.h : &t.w, m);
+    }
 }
 
 // ───────────────────────────── packing ─────────────────────────────
@@ -141,7 +194,8 @@ struct PackArgs {
     const void* src;
     const int32_t* rows;  // source row of each row, NULL: itself
     const int32_t* live;  // rows that count (device), NULL: R
-    const uint32_t* top;  // largest magnitude (float32 sources)
+    const Header* hd;     // largest magnitudes (float32 sources)
+    bool of_w;
     int64_t R, d;
     char* by_row;  // rows of R rows, stages along d; NULL: not wanted
     char* by_col;  // rows of d rows, stages along the R rows; NULL: not wanted
@@ -167,7 +221,8 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) tile[(threadIdx.x >> 6) + 4 * j][c] = v[j];
     __syncthreads();
-    const float scale = SPLIT ? pow2(scale_exp(*p.top)) : 1.0f;
+    const float scale =
+        SPLIT ? pow2(p.of_w ? scale_exp<&Top::w>(p.hd) : scale_exp<&Top::h>(p.hd)) : 1.0f;
     constexpr int K = kStageK<SPLIT>;
     const int64_t stages = ceil_div(p.d, K);
     auto put = [&](char* row, int k, const float (&x)[8]) {  // elements k .. k + 7 of a stage
@@ -208,7 +263,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
 
 template <bool SPLIT>
 __device__ __forceinline__ float logit_scale(const Header* hd) {
-    return SPLIT ? pow2(-scale_exp(hd->top_h)) * pow2(-scale_exp(hd->top_w)) : 1.0f;
+    return SPLIT ? pow2(-scale_exp<&Top::h>(hd)) * pow2(-scale_exp<&Top::w>(hd)) : 1.0f;
 }
 
 // Logits are exponentiated in base 2: the factor log2(e) goes into the scale of
@@ -287,6 +342,10 @@ struct ScoreEpi {
     }
 };
 
+// Bytes of a row of 32 16-bit values in LDS while a block is turned: the two
+// half waves that write it meet different banks.
+constexpr int kTurnPitch = 80;
+
 // Backward: the same tiles as dl, written as rows of tokens (stages along the
 // vocabulary) and as rows of the vocabulary (stages along the tokens).
 template <bool SPLIT>
@@ -305,6 +364,8 @@ struct DlEpi {
         const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
         constexpr float up = SPLIT ? static_cast<float>(1 << kDlExp) : 1.0f;
         constexpr int K = kStageK<SPLIT>;
+        __syncthreads();  // the ring is free
+        uint16_t* sh = reinterpret_cast<uint16_t*>(t.lds + (threadIdx.x >> 6) * 64 * kTurnPitch);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t tok = t.n0() + t.col(b);
@@ -325,11 +386,10 @@ struct DlEpi {
                 const int64_t v = t.m0() + 32 * a;          // this block's 32 rows
                 const int64_t k = t.n0() + 32 * b;          // and 32 tokens
                 char* tk = by_tok + ((v / K) * n + tok) * kStageBytes + 2 * (v % K);
-                char* vc = by_voc + ((k / K) * voc + v) * kStageBytes + 2 * (k % K + (t.lane & 31));
+                char* vc = by_voc + ((k / K) * voc + v) * kStageBytes + 2 * (k % K);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int at = 8 * q + 4 * (t.lane >> 5);
-                    ushort4 hi, lo;
                     uint16_t h[4], w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -343,17 +403,32 @@ struct DlEpi {
                             h[j] = f32_to_bf16(x);
                             w[j] = 0;
                         }
-                        char* to = vc + (at + j) * kStageBytes;
-                        *reinterpret_cast<uint16_t*>(to) = h[j];
-                        if (SPLIT) *reinterpret_cast<uint16_t*>(to + 64) = w[j];
+                        uint16_t* to = sh + (at + j) * (kTurnPitch / 2) + (t.lane & 31);
+                        *to = h[j];
+                        if (SPLIT) to[32 * kTurnPitch / 2] = w[j];
                     }
-                    hi = make_ushort4(h[0], h[1], h[2], h[3]);
-                    lo = make_ushort4(w[0], w[1], w[2], w[3]);
                     if (in) {
-                        *reinterpret_cast<ushort4*>(tk + 2 * at) = hi;
-                        if (SPLIT) *reinterpret_cast<ushort4*>(tk + 64 + 2 * at) = lo;
+                        *reinterpret_cast<ushort4*>(tk + 2 * at) =
+                            make_ushort4(h[0], h[1], h[2], h[3]);
+                        if (SPLIT)
+                            *reinterpret_cast<ushort4*>(tk + 64 + 2 * at) =
+                                make_ushort4(w[0], w[1], w[2], w[3]);
                     }
                 }
+                // turned in the wave's own LDS: 16 bytes of a vocabulary row a lane
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+                for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 16 * i + (t.lane >> 2), piece = t.lane & 3;
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(
+                            reinterpret_cast<const char*>(sh) + (32 * p + row) * kTurnPitch +
+                            16 * piece);
+                        *reinterpret_cast<f32x4*>(vc + row * kStageBytes + 64 * p + 16 * piece) =
+                            x;
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             }
         }
     }
@@ -390,7 +465,9 @@ template <bool SPLIT>
 struct GradScale {
     float unscale, factor;
     __device__ __forceinline__ GradScale(const Header* hd, const float* f, bool of_w)
-        : unscale(SPLIT ? pow2(-kDlExp - scale_exp(of_w ? hd->top_h : hd->top_w)) : 1.0f),
+        : unscale(SPLIT ? pow2(-kDlExp - (of_w ? scale_exp<&Top::h>(hd)
+                                              : scale_exp<&Top::w>(hd)))
+                        : 1.0f),
           factor(*f) {}
     __device__ __forceinline__ float operator()(float sum) const {
         return (SPLIT ? sum * unscale : sum) * factor;
@@ -416,6 +493,33 @@ struct WeightEpi {
                 for (int r = 0; r < 16; ++r) {
                     const int64_t row = t.m0() + t.row(a, r);
                     if (row < t.M && c < t.N) T::store(out, row * d + c, s(acc[a][b][r]));
+                }
+            }
+    }
+};
+
+// dh where one workgroup has the whole sum: to the token's row.
+template <class T, bool SPLIT>
+struct TokenEpi {
+    const Header* hd;
+    const float* factor;
+    const int32_t* rows;
+    void* out;
+    int64_t d;
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
+        const GradScale<SPLIT> s(hd, factor, false);
+#pragma unroll
+        for (int a = 0; a < Tile::kNA; ++a)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t row = t.m0() + t.row(a, r);
+                if (row >= t.M) continue;
+                const int64_t at = rows[row] * d;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int64_t c = t.n0() + t.col(b);
+                    if (c < t.N) T::store(out, at + c, s(acc[a][b][r]));
                 }
             }
     }
@@ -511,11 +615,29 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
 // Upstream gradients: factor is the largest magnitude over the live tokens and
 // gr each token's own over it, so that dl stays within [-1, 1]. With one
 // upstream value for all (sum, mean) every gr is 1 and none is written.
-__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up,
-                                                           const Header* __restrict__ hd,
-                                                           const int32_t* __restrict__ rows,
-                                                           int reduction, float* __restrict__ gr,
-                                                           float* __restrict__ factor) {
+// The workgroups beside the first clear the rows of dh that are no live token's,
+// where the product writes only the others.
+template <class T>
+__global__ __launch_bounds__(1024) void ce_upstream_kernel(
+    const float* __restrict__ up, const Header* __restrict__ hd, const int32_t* __restrict__ rows,
+    int reduction, float* __restrict__ gr, float* __restrict__ factor,
+    const int32_t* __restrict__ pos, int64_t n, int64_t d, void* __restrict__ dh) {
+    if (blockIdx.x > 0) {
+        const int lane = threadIdx.x & (kWave - 1);
+        const int64_t waves = static_cast<int64_t>(gridDim.x - 1) * (1024 / kWave);
+        for (int64_t w = static_cast<int64_t>(blockIdx.x - 1) * (1024 / kWave) +
+                         (threadIdx.x >> 6);
+             w * kWave < n; w += waves) {
+            const int64_t mine = w * kWave + lane;
+            uint64_t clear = __ballot(mine < n && pos[mine < n ? mine : 0] < 0);
+            while (clear != 0) {
+                const int64_t row = w * kWave + __ffsll(static_cast<unsigned long long>(clear)) - 1;
+                clear &= clear - 1;
+                for (int64_t e = lane; e < d; e += kWave) T::store(dh, row * d + e, 0.0f);
+            }
+        }
+        return;
+    }
     __shared__ uint32_t sh[1024 / kWave];
     const int64_t live = hd->live;
     if (reduction != SLK_REDUCE_NONE) {
@@ -555,7 +677,16 @@ __global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict_
         const int64_t at = pos != nullptr ? pos[r] : r;
         float x = 0.0f;
         if (at >= 0) {
-            for (int k = 0; k < splits; ++k) x += sums[k * stride * d + at * d + (i - r * d)];
+            const float* from = sums + at * d + (i - r * d);
+            int k = 0;
+            for (; k + 8 <= splits; k += 8) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = from[(k + j) * stride * d];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x += v[j];
+            }
+            for (; k < splits; ++k) x += from[k * stride * d];
             x = s(x);
         }
         T::store(out, i, x);
@@ -779,7 +910,8 @@ Backward backward_of(const slk_linear_ce* a) {
     b.gr = c.take(4 * a->n);
     b.by_tok = c.take(stages(a, b.piece) * a->n * kStageBytes);
     b.by_voc = c.take(stages(a, n_up) * b.piece * kStageBytes);
-    b.dh = c.take(a->dhidden != nullptr ? 4 * b.sh * a->n * a->d : 0);
+    const bool whole = b.sh == 1 && b.piece >= a->v;
+    b.dh = c.take(a->dhidden != nullptr && !whole ? 4 * b.sh * a->n * a->d : 0);
     b.dw = c.take(a->dweight != nullptr && b.sw > 1 ? 4 * b.sw * b.piece * a->d : 0);
     b.bytes = c.at;
     return b;
@@ -845,18 +977,20 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
                            a->v, a->ignore_index, hd, rows, pos, tgt);
         if ((rc = check_launch("linear_ce list")) != SLK_OK) return rc;
         if (SPLIT) {
-            auto top = [&](const void* x, int64_t r, const int32_t* ps, uint32_t* to) {
-                const int64_t g = ceil_div(r * a->d, 256 * 4 * 4);
-                hipLaunchKernelGGL(ce_top_kernel, dim3(static_cast<unsigned>(g < 2048 ? g : 2048)),
-                                   dim3(256), 0, st, static_cast<const float*>(x), r, a->d, ps, to);
-                return check_launch("linear_ce top");
+            const int64_t g = ceil_div(a->n + a->v, 4);
+            const dim3 grid(static_cast<unsigned>(g < 1024 ? g : 1024));
+            const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 16) && aligned_to(a->weight, 16);
+            auto go = [&](auto k) {
+                hipLaunchKernelGGL(k, grid, dim3(256), 0, st, static_cast<const float*>(a->hidden),
+                                   a->n, static_cast<const float*>(a->weight), a->v, a->d, pos, hd);
             };
-            if ((rc = top(a->hidden, a->n, pos, &hd->top_h)) != SLK_OK) return rc;
-            if ((rc = top(a->weight, a->v, nullptr, &hd->top_w)) != SLK_OK) return rc;
+            if (vec) go(ce_top_kernel<true>);
+            else go(ce_top_kernel<false>);
+            if ((rc = check_launch("linear_ce top")) != SLK_OK) return rc;
         }
-        PackArgs ph{a->hidden, rows, &hd->live, &hd->top_h, a->n, a->d, sv + s.h_row,
+        PackArgs ph{a->hidden, rows, &hd->live, hd, false, a->n, a->d, sv + s.h_row,
                     a->keep ? sv + s.h_col : nullptr};
-        PackArgs pw{a->weight, nullptr, nullptr, &hd->top_w, a->v, a->d, sv + s.w_row,
+        PackArgs pw{a->weight, nullptr, nullptr, hd, true, a->v, a->d, sv + s.w_row,
                     a->keep ? sv + s.w_col : nullptr};
         if ((rc = pack<T, SPLIT>(ph, st)) != SLK_OK) return rc;
         if ((rc = pack<T, SPLIT>(pw, st)) != SLK_OK) return rc;
@@ -892,8 +1026,12 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     const float* lse = reinterpret_cast<const float*>(sv + s.lse);
     float* factor = reinterpret_cast<float*>(sc + b.factor);
     float* gr = reinterpret_cast<float*>(sc + b.gr);
-    hipLaunchKernelGGL(ce_upstream_kernel, dim3(1), dim3(1024), 0, st, a->upstream, hd, rows,
-                       a->reduction, gr, factor);
+    const bool whole = b.sh == 1 && b.piece >= a->v;  // a tile of dh has its whole sum
+    const int64_t clears = whole && a->dhidden != nullptr ? ceil_div(a->n, 1024) : 0;
+    hipLaunchKernelGGL(ce_upstream_kernel<T>,
+                       dim3(static_cast<unsigned>(1 + (clears < 256 ? clears : 256))), dim3(1024),
+                       0, st, a->upstream, hd, rows, a->reduction, gr, factor, pos, a->n, a->d,
+                       a->dhidden);
     int rc = check_launch("linear_ce upstream");
     if (rc != SLK_OK) return rc;
     constexpr int K = kStageK<SPLIT>;
@@ -901,7 +1039,7 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     float* dw = reinterpret_cast<float*>(sc + b.dw);
     auto finish = [&](const float* sums, int splits, int64_t r, int64_t stride,
                       const int32_t* ps, bool of_w, void* out) {
-        const int64_t g = ceil_div(r * a->d, 256 * 4);
+        const int64_t g = ceil_div(r * a->d, 256);
         hipLaunchKernelGGL((ce_finish_kernel<T, SPLIT>),
                            dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st,
                            sums, splits, r, stride, a->d, ps, hd, factor, of_w, out);
@@ -917,10 +1055,13 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
         if (a->dhidden != nullptr) {
             const MmaArgs g{sc + b.by_tok, sv + s.w_col + v0 / K * a->d * kStageBytes, a->n, a->d,
                             stages(a, vn), a->n, a->d, &hd->live, kLiveM, b.sh};
-            if ((rc = mma<SPLIT>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st, "linear_ce dhidden")) !=
-                SLK_OK) {
-                return rc;
+            if (whole) {
+                rc = mma<SPLIT>(g, TokenEpi<T, SPLIT>{hd, factor, rows, a->dhidden, a->d}, st,
+                                "linear_ce dhidden");
+            } else {
+                rc = mma<SPLIT>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st, "linear_ce dhidden");
             }
+            if (rc != SLK_OK) return rc;
         }
         if (a->dweight != nullptr) {
             const MmaArgs g{sc + b.by_voc, sv + s.h_col, vn, a->d, stages(a, a->n), b.piece, a->d,
@@ -936,7 +1077,7 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
             if (rc != SLK_OK) return rc;
         }
     }
-    if (a->dhidden != nullptr) rc = finish(dh, b.sh, a->n, a->n, pos, false, a->dhidden);
+    if (a->dhidden != nullptr && !whole) rc = finish(dh, b.sh, a->n, a->n, pos, false, a->dhidden);
     return rc;
 }
 
