@@ -14,6 +14,7 @@ kernel call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -417,6 +418,16 @@ def stream_of(t: torch.Tensor) -> int:
     if device.type != "cuda":
         return torch.cuda.current_stream(device).cuda_stream  # raises as it did
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """A context in which t's device is the current one (none where it is already)."""
+    if torch._C._cuda_getDevice() == t.get_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -909,7 +920,7 @@ def norm_backward(args: Norm, stream: int) -> None:
 
 
 def linear_ce_saved_bytes(args: LinearCE) -> int:
-    return int(load().slk_linear_ce_saved_bytes(ctypes.byref(args)))
+    return load().slk_linear_ce_saved_bytes(ctypes.byref(args))
 
 
 def linear_ce_scratch_bytes(args: LinearCE, backward: bool) -> int:

@@ -21,7 +21,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d, v = weight.shape[1], weight.shape[0]
         n = target.numel()
         dev = hidden.device
-        h, w, t = hidden.reshape(n, d).contiguous(), weight.contiguous(), target.contiguous()
+        h, w, t = (x if x.is_contiguous() else x.contiguous() for x in (hidden, weight, target))
         keep = any(ctx.needs_input_grad)
         loss = torch.empty(target.shape if reduction == "none" else (), device=dev)
         p = _lib.ptr
@@ -34,10 +34,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         else:
             args.saved_bytes = _lib.linear_ce_saved_bytes(args)
             args.scratch_bytes = _lib.linear_ce_scratch_bytes(args, False)
-            saved = torch.empty(args.saved_bytes, dtype=torch.uint8, device=dev)
+            saved = torch.empty(args.saved_bytes, dtype=torch.uint8, device=dev) \
+                if args.saved_bytes else None
             scratch = torch.empty(args.scratch_bytes, dtype=torch.uint8, device=dev)
             args.saved, args.scratch = p(saved), p(scratch)
-            with torch.cuda.device(dev):
+            with _lib.on_device(h):
                 _lib.linear_ce_forward(args, _lib.stream_of(h))
         if keep:
             ctx.save_for_backward(saved)
@@ -49,7 +50,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         saved, = ctx.saved_tensors
         n, d, v, ignore_index, reduction, shape, dtype = ctx.rest
         dev = grad.device
-        dh = torch.empty((n, d), dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dh = torch.empty(shape, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:
             dw = (torch.empty if n else torch.zeros)((v, d), dtype=dtype, device=dev)
@@ -63,9 +64,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
             args.scratch_bytes = _lib.linear_ce_scratch_bytes(args, True)
             scratch = torch.empty(args.scratch_bytes, dtype=torch.uint8, device=dev)
             args.scratch = p(scratch)
-            with torch.cuda.device(dev):
+            with _lib.on_device(up):
                 _lib.linear_ce_backward(args, _lib.stream_of(up))
-        return dh.reshape(shape) if dh is not None else None, dw, None, None, None
+        return dh, dw, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,

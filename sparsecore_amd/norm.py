@@ -37,12 +37,17 @@ def _as_cols(t: torch.Tensor) -> torch.Tensor:
 
 def _layout(t: torch.Tensor, n: int, d: int) -> tuple[torch.Tensor, int]:
     """(N x D tensor, 1 if it is feature-major): a layout that the kernels read."""
-    t = t.reshape(n, d)
     if t.is_contiguous():
         return t, 0
-    if t.t().is_contiguous():
+    if t.dim() != 2:
+        t = t.reshape(n, d)
+    if t.stride(0) == 1 and t.stride(1) == n:
         return (t, 1) if d <= _lib.NORM_COLS_MAX else (_as_rows(t), 0)
     return t.contiguous(), 0
+
+
+def _packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _gate_rows(gate: torch.Tensor, x: torch.Tensor, n: int, d: int) -> int:
@@ -72,75 +77,84 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, branch, gate, post_weight, post_bias, scale, layer, eps,
                 feature_major):
-        ctx.set_materialize_grads(False)
-        d = x.shape[-1]
+        # Small calls are bound by this host work: as few tensor operations as possible.
+        shape, dt, dev = x.shape, x.dtype, x.device
+        d = shape[-1]
         n = x.numel() // d
-        dt, dev = x.dtype, x.device
-        x2 = x.reshape(n, d).contiguous()
+        x = _packed(x)
         u, u_cols = _layout(branch, n, d) if branch is not None else (None, 0)
         rows = _gate_rows(gate, x, n, d) if gate is not None else 0
-        weight, bias, gate, post_weight, post_bias = (
-            t.contiguous() if t is not None else None
-            for t in (weight, bias, gate, post_weight, post_bias))
+        weight, bias, gate = _packed(weight), _packed(bias), _packed(gate)
+        post_weight, post_bias = _packed(post_weight), _packed(post_bias)
         y_cols = int(feature_major and d <= _lib.NORM_COLS_MAX)
-        y = (torch.empty((d, n), dtype=dt, device=dev).t() if y_cols
-             else torch.empty((n, d), dtype=dt, device=dev))
-        r = torch.empty((n, d), dtype=dt, device=dev) if u is not None else x2
-        stats = torch.empty((n, 4), device=dev) if any(ctx.needs_input_grad) else None
-        p = _lib.ptr
-        args = _lib.Norm(n=n, d=d, gate_rows=rows, x=p(x2), branch=p(u), gate=p(gate),
-                         weight=p(weight), bias=p(bias), post_weight=p(post_weight),
-                         post_bias=p(post_bias), r=p(r), y=p(y), stats=p(stats), scale=scale,
-                         eps=eps, dtype=_lib.DTYPES[dt], layer=layer, branch_cols=u_cols,
-                         y_cols=y_cols)
+        if y_cols:
+            y = torch.empty((d, n), dtype=dt, device=dev).t()
+            if len(shape) != 2:
+                y = y.reshape(shape)
+        else:
+            y = torch.empty(shape, dtype=dt, device=dev)
+        r = torch.empty(shape, dtype=dt, device=dev) if u is not None else x
+        need = ctx.needs_input_grad
+        stats = torch.empty((n, 4), device=dev) if any(need) else None
         if n:
-            with torch.cuda.device(dev):
+            p = _lib.ptr
+            args = _lib.Norm(n=n, d=d, gate_rows=rows, x=p(x), branch=p(u), gate=p(gate),
+                             weight=p(weight), bias=p(bias), post_weight=p(post_weight),
+                             post_bias=p(post_bias), r=p(r), y=p(y), stats=p(stats), scale=scale,
+                             eps=eps, dtype=_lib.DTYPES[dt], layer=layer, branch_cols=u_cols,
+                             y_cols=y_cols)
+            with _lib.on_device(x):
                 _lib.norm_forward(args, _lib.stream_of(x))
         if feature_major and not y_cols:
-            y = _as_cols(y)
+            y = _as_cols(y.reshape(n, d)).reshape(shape)
         if stats is not None:
-            keep_u = post_weight is not None or (gate is not None and ctx.needs_input_grad[4])
+            ctx.set_materialize_grads(False)
+            keep_u = post_weight is not None or (gate is not None and need[4])
             ctx.save_for_backward(r, stats, weight, bias, u if keep_u else None, gate,
                                   post_weight, post_bias)
-            ctx.shape = x.shape
             # the branch's gradient goes back in the branch's layout
-            ctx.back_cols = (u is not None and not u_cols and n > 1 and d > 1
-                             and branch.reshape(n, d).t().is_contiguous())
-            ctx.rest = (n, d, rows, scale, layer, eps, u_cols, branch is not None,
-                        gate.shape if gate is not None else None)
-        y = y.reshape(x.shape)
-        return (r.reshape(x.shape), y) if branch is not None else y
+            back_cols = (u is not None and not u_cols and n > 1 and d > 1
+                         and not branch.is_contiguous()
+                         and branch.reshape(n, d).t().is_contiguous())
+            ctx.rest = (shape, n, d, rows, scale, layer, eps, u_cols, back_cols,
+                        branch is not None)
+        return (r, y) if branch is not None else y
 
     @staticmethod
     def backward(ctx, *grads):
         r, stats, weight, bias, u, gate, post_weight, post_bias = ctx.saved_tensors
-        n, d, rows, scale, layer, eps, u_cols, has_branch, gate_shape = ctx.rest
+        shape, n, d, rows, scale, layer, eps, u_cols, back_cols, has_branch = ctx.rest
         need = ctx.needs_input_grad
         dr, dy = grads if has_branch else (None, grads[0])
         dt, dev = r.dtype, r.device
         y_cols = 0
-        if dr is not None:
+        if dr is not None and not dr.is_contiguous():
             dr = _as_rows(dr.reshape(n, d))
         if dy is not None:
             dy, y_cols = _layout(dy, n, d)
 
-        def vector(i, like):
-            if not need[i] or like is None:
-                return None
-            # without dy there is nothing to sum; without tokens neither
-            return (torch.zeros if n == 0 or (dy is None and i in (1, 2)) else
-                    torch.empty)(d, dtype=dt, device=dev)
-
-        dx = torch.empty((n, d), dtype=dt, device=dev) if need[0] else None
+        dx = torch.empty(shape, dtype=dt, device=dev) if need[0] else None
         du = None
         if has_branch and need[3]:
-            du = (torch.empty((d, n), dtype=dt, device=dev).t() if u_cols
-                  else torch.empty((n, d), dtype=dt, device=dev))
+            if u_cols:
+                du = torch.empty((d, n), dtype=dt, device=dev).t()
+                if len(shape) != 2:
+                    du = du.reshape(shape)
+            else:
+                du = torch.empty(shape, dtype=dt, device=dev)
         dgate = None
         if gate is not None and need[4]:
-            dgate = (torch.zeros if n == 0 else torch.empty)(gate_shape, dtype=dt, device=dev)
-        dw, db = vector(1, weight), vector(2, bias)
-        dpw, dpb = vector(5, post_weight), vector(6, post_bias)
+            dgate = (torch.zeros if n == 0 else torch.empty)(gate.shape, dtype=dt, device=dev)
+        # weight's, bias's, post_weight's and post_bias's gradients; without dy there is
+        # nothing to sum for the first two, without tokens for any
+        wanted = [(need[1], dy is None), (need[2] and bias is not None, dy is None),
+                  (need[5] and post_weight is not None, False),
+                  (need[6] and post_bias is not None, False)]
+        sums = [None] * 4
+        for k, (want, empty) in enumerate(wanted):
+            if want:
+                sums[k] = (torch.zeros if empty or n == 0 else torch.empty)(d, dtype=dt,
+                                                                           device=dev)
         if n:
             p = _lib.ptr
             # where the branch itself is not needed any address stands for it (not read)
@@ -148,21 +162,19 @@ class _ResidualNorm(torch.autograd.Function):
             args = _lib.Norm(n=n, d=d, gate_rows=rows, branch=branch, gate=p(gate),
                              weight=p(weight), bias=p(bias), post_weight=p(post_weight),
                              post_bias=p(post_bias), r=p(r), stats=p(stats), dr=p(dr), dy=p(dy),
-                             dx=p(dx), dbranch=p(du), dgate=p(dgate), dweight=p(dw),
-                             dbias=p(db), dpost_weight=p(dpw), dpost_bias=p(dpb), scale=scale,
-                             eps=eps, dtype=_lib.DTYPES[dt], layer=layer, branch_cols=u_cols,
-                             y_cols=y_cols)
+                             dx=p(dx), dbranch=p(du), dgate=p(dgate), dweight=p(sums[0]),
+                             dbias=p(sums[1]), dpost_weight=p(sums[2]), dpost_bias=p(sums[3]),
+                             scale=scale, eps=eps, dtype=_lib.DTYPES[dt], layer=layer,
+                             branch_cols=u_cols, y_cols=y_cols)
             nbytes = _lib.norm_workspace_bytes(args)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            args.workspace, args.workspace_bytes = p(ws), nbytes
-            with torch.cuda.device(dev):
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+            with _lib.on_device(r):
                 _lib.norm_backward(args, _lib.stream_of(r))
-            if du is not None and ctx.back_cols:
-                du = _as_cols(du)
-        shape = ctx.shape
-        return (dx.reshape(shape) if dx is not None else None, dw, db,
-                du.reshape(shape) if du is not None else None, dgate, dpw, dpb,
-                None, None, None, None)
+            if du is not None and back_cols:
+                du = _as_cols(du.reshape(n, d)).reshape(shape)
+        return (dx, sums[0], sums[1], du, dgate, sums[2], sums[3], None, None, None, None)
 
 
 def residual_norm(x, weight, bias=None, *, branch=None, gate=None, post_weight=None,

@@ -64,7 +64,7 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     codes are a first moment's, uint8 codes a second moment's."""
     _check_q8("dequantize", codes, scales)
     out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
-    with torch.cuda.device(codes.device):
+    with _lib.on_device(codes):
         _lib.q8_decode(codes, scales, out)
     return out
 
@@ -78,7 +78,7 @@ def quantize(x: torch.Tensor, signed: bool) -> tuple[torch.Tensor, torch.Tensor]
     x = x.contiguous()
     codes = torch.empty(x.shape, dtype=torch.int8 if signed else torch.uint8, device=x.device)
     scales = torch.empty(_blocks(x.numel()), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x):
         _lib.q8_encode(x, codes, scales)
     return codes, scales
 
@@ -108,32 +108,31 @@ def _check_hyper(lr, betas, eps, weight_decay, step) -> None:
         raise ValueError(f"adamw_step: step must be >= 1, got {step}")
 
 
-def _check_lists(params, grads, moments, scales) -> None:
+def _check_lists(params, grads, moments, scales) -> list:
     """Everything the kernel relies on, over whole lists at a time (a step of a small
-    model is bound by this host work)."""
+    model is bound by this host work). Returns the parameters' sizes."""
     n = len(params)
-    every = [*params, *grads]
-    for t in moments:
-        every += t
-    if scales:
-        for t in scales:
-            every += t
-    if len(every) != n * (6 if scales else 4):
+    lists = [params, grads, *moments, *(scales or ())]
+    if {len(t) for t in lists} - {n}:
         raise ValueError("adamw_step: params, grads, moments (and scales) must be lists of the "
                          "same length")
-    if not all([isinstance(t, torch.Tensor) for t in every]):
-        raise TypeError("adamw_step: lists of torch.Tensor expected")
-    if not all([t.is_cuda for t in every]):
+    every = [t for part in lists for t in part]
+    try:
+        devices = {t.get_device() for t in every}
+        packed = all([t.is_contiguous() for t in every])
+        sizes = [t.numel() for t in params]
+        kinds = [t.dtype for t in params]
+    except (AttributeError, TypeError):
+        raise TypeError("adamw_step: lists of torch.Tensor expected") from None
+    if -1 in devices:
         raise RuntimeError("adamw_step: every tensor must be on a HIP (ROCm) device")
-    if len({t.get_device() for t in every}) > 1:
+    if len(devices) > 1:
         raise RuntimeError("adamw_step: all tensors of a call must be on one device")
-    if not all([t.is_contiguous() for t in every]):
+    if not packed:
         raise ValueError("adamw_step: tensors must be contiguous")
-    sizes = [t.numel() for t in params]
     for what, have in (("grads", grads), ("exp_avgs", moments[0]), ("exp_avg_sqs", moments[1])):
         if [t.numel() for t in have] != sizes:
             raise ValueError(f"adamw_step: {what} must have their parameters' sizes")
-    kinds = [t.dtype for t in params]
     if [t.dtype for t in grads] != kinds:
         raise ValueError("adamw_step: a gradient must have its parameter's dtype")
     bad = set(kinds) - set(_lib.DTYPES)
@@ -149,6 +148,7 @@ def _check_lists(params, grads, moments, scales) -> None:
                 raise ValueError("adamw_step: scales must be float32")
             if [x.numel() for x in t] != [_blocks(k) for k in sizes]:
                 raise ValueError(f"adamw_step: one scale per {BLOCK} elements expected")
+    return sizes
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None,
@@ -173,11 +173,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None,
         raise ValueError("adamw_step: scales of both moments or of none")
     scales = None if exp_avg_scales is None else (exp_avg_scales, exp_avg_sq_scales)
     _check_hyper(lr, betas, eps, weight_decay, step)
-    _check_lists(params, grads, (exp_avgs, exp_avg_sqs), scales)
-    _launch(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas, eps, weight_decay)
+    sizes = _check_lists(params, grads, (exp_avgs, exp_avg_sqs), scales)
+    _launch(sizes, params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas, eps,
+            weight_decay)
 
 
-def _launch(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas, eps, weight_decay):
+def _launch(sizes, params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas, eps,
+            weight_decay):
     if not params:
         return
     dev = params[0].get_device()
@@ -185,13 +187,13 @@ def _launch(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas, eps, 
     lr, lr_dev = _scalar("lr", lr, dev)
     args = _lib.AdamArgs(lr, betas[0], betas[1], eps, weight_decay, step, step_dev, lr_dev)
     cols = [params, grads, exp_avgs, exp_avg_sqs, *(scales or ())]
-    table = np.zeros((len(params), 7), dtype=np.int64)
-    for k, tensors in enumerate(cols):
-        table[:, k] = [t.data_ptr() for t in tensors]
-    table[:, 6] = [t.numel() for t in params]
+    rows = [[t.data_ptr() for t in tensors] for tensors in cols]
+    if not scales:
+        rows += [[0] * len(params)] * 2
+    table = np.array([*rows, sizes], dtype=np.int64).T.copy()  # a row a tensor
     bits = 8 if scales else 32
     kinds = [t.dtype for t in params]
-    with torch.cuda.device(dev):
+    with _lib.on_device(params[0]):
         stream = _lib.stream_of(params[0])
         for dtype in dict.fromkeys(kinds):
             part = table
@@ -249,7 +251,7 @@ def carry_slots(row_start, old, new, states) -> list:
             to_scales = torch.empty_like(scales)
             out.append((to, to_scales))
             table.append((codes, scales, to, to_scales, kind))
-    with torch.cuda.device(row_start.device):
+    with _lib.on_device(row_start):
         _lib.carry_slots(row_start, old[0], old[1], new[0], new[1], table)
     return out
 
@@ -417,6 +419,6 @@ class AdamW(torch.optim.Optimizer):
             gs = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
             lists = [[states[i][k] for i in part] for k in names]
             scales = tuple(lists[2:]) or None
-            _check_lists(ps, gs, lists[:2], scales)
-            _launch(ps, gs, lists[0], lists[1], scales, states[part[0]]["step"], group["lr"],
+            sizes = _check_lists(ps, gs, lists[:2], scales)
+            _launch(sizes, ps, gs, lists[0], lists[1], scales, states[part[0]]["step"], group["lr"],
                     group["betas"], group["eps"], group["weight_decay"])
