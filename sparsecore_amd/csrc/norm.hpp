@@ -62,6 +62,25 @@ __device__ __forceinline__ void row_store(void* p, int64_t off, int d, int l,
     }
 }
 
+// The sum over a wave, in every lane: cross-lane adds inside rows of 16 lanes,
+// then across rows towards lane 63 (six vector instructions, where shuffles
+// through LDS wait six times).
+__device__ __forceinline__ float wave_sum(float x) {
+    auto add = [&](auto ctrl, auto rows) {
+        constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+        x += __int_as_float(
+            __builtin_amdgcn_update_dpp(0, __float_as_int(x), C, R, 0xf, true));
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0xB1>{}, integral_constant<int, 0xf>{});   // lane ^ 1
+    add(integral_constant<int, 0x4E>{}, integral_constant<int, 0xf>{});   // lane ^ 2
+    add(integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});  // half row mirrored
+    add(integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});  // row mirrored
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // rows 0, 2 to 1, 3
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // lane 31 to rows 2, 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // Sums of NV values over the team. With more than one wave, through LDS: red
 // holds two buffers of NV x TW floats, used in turn (a wave that writes a
 // buffer again has passed the barrier of the sum between, which every wave
@@ -72,9 +91,7 @@ struct TeamSum {
     int turn = 0;
     __device__ __forceinline__ void operator()(float (&v)[NV]) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o);
+        for (int k = 0; k < NV; ++k) v[k] = wave_sum(v[k]);
         if constexpr (TW > 1) {
             float* b = red + turn * NV * TW;
             turn ^= 1;
@@ -85,10 +102,48 @@ struct TeamSum {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                float s = b[k * TW];
+                f32x4 s = *reinterpret_cast<const f32x4*>(b + k * TW);
 #pragma unroll
-                for (int w = 1; w < TW; ++w) s += b[k * TW + w];
-                v[k] = s;
+                for (int w = 4; w < TW; w += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(b + k * TW + w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[j] += x[j];
+                }
+                v[k] = (s[0] + s[1]) + (s[2] + s[3]);
+            }
+        }
+    }
+};
+
+// A row's features as they are in memory (VEC layout): fetched ahead at the
+// cost of their own registers, converted when used.
+template <class T, int EPL, int TW>
+struct RawRow {
+    using Piece = std::conditional_t<T::kBytes == 4, f32x4, uint2>;
+    Piece p[EPL / 4];
+    __device__ __forceinline__ void load(const void* from, int64_t off, int d, int l) {
+#pragma unroll
+        for (int q = 0; q < EPL / 4; ++q) {
+            const int e = RowLay<EPL, TW, true>::at(4 * q, l);
+            if (e < d) {
+                p[q] = *reinterpret_cast<const Piece*>(static_cast<const char*>(from) +
+                                                       (off + e) * T::kBytes);
+            } else {
+                p[q] = Piece{};
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[EPL]) const {
+#pragma unroll
+        for (int q = 0; q < EPL / 4; ++q) {
+            if constexpr (T::kBytes == 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * q + j] = p[q][j];
+            } else {
+                v[4 * q] = bf16_to_f32(p[q].x & 0xffffu);
+                v[4 * q + 1] = __uint_as_float(p[q].x & 0xffff0000u);
+                v[4 * q + 2] = bf16_to_f32(p[q].y & 0xffffu);
+                v[4 * q + 3] = __uint_as_float(p[q].y & 0xffff0000u);
             }
         }
     }
@@ -120,9 +175,9 @@ __device__ __forceinline__ void row_stats(const float (&v)[EPL], int d, int l, b
 }
 
 // Shape of the row kernels for d features, as f(features a lane, waves a
-// team): a wave a token up to 1024, else a workgroup. Eight features of each
-// array a lane where a workgroup's 16 waves reach: the backward with a post
-// norm and a gate holds some twelve arrays in registers.
+// team): a wave a token up to 1024, else a workgroup. The backward with a post
+// norm and a gate holds some twelve arrays in registers, which 16 features a
+// lane make 256 of: eight waves at most then, so 16 only above 8192.
 constexpr int kNormThreads = 256;
 
 template <class F>
@@ -132,7 +187,7 @@ void norm_shape(int d, F&& f) {
     else if (d <= 1024) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
     else if (d <= 2048) f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
     else if (d <= 4096) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-    else if (d <= 8192) f(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+    else if (d <= 8192) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
 }
 
@@ -150,11 +205,47 @@ inline bool norm_vec(const slk_norm* a, std::initializer_list<const void*> ps) {
 // token, as one that walks tokens, meets every bank once).
 constexpr int kTileWaves = 8;
 constexpr int kTileThreads = kTileWaves * kWave;
+constexpr int64_t kTileMinGroups = 512;
+
+// The tile's row of feature e: lanes that hold runs of four features (VEC) then
+// walk consecutive rows, an odd number of banks apart.
+__device__ __forceinline__ int tile_row(int e, int quarter) {
+    return (e & 3) * quarter + (e >> 2);
+}
+__host__ __device__ inline int tile_quarter(int64_t d) { return static_cast<int>((d + 3) / 4); }
 
 // Copies a feature-major d x n array's columns [n0, n0 + TT) into LDS, and back.
+// bfloat16 columns go two tokens a lane (pairs: n is even and the array is
+// 4-byte aligned), or a row of the tile would be 2 TT bytes of 2-byte accesses.
 template <class T, int TT>
 __device__ __forceinline__ void tile_load(const void* src, int64_t n, int d, int64_t n0,
-                                          float* tile) {
+                                          bool pairs, float* tile) {
+    const int quarter = tile_quarter(d);
+    if (T::kBytes == 2 && pairs) {
+        constexpr int kCols = TT / 2, kRows = kTileThreads / kCols;
+        const int t = 2 * (threadIdx.x % kCols);
+        const bool in = n0 + t < n;
+        const uint16_t* s = static_cast<const uint16_t*>(src);
+        for (int e0 = threadIdx.x / kCols; e0 < d; e0 += 4 * kRows) {
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = e0 + j * kRows;
+                v[j] = in && e < d ? *reinterpret_cast<const uint32_t*>(
+                                         s + static_cast<int64_t>(e) * n + n0 + t)
+                                   : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = e0 + j * kRows;
+                if (e >= d) break;
+                float* to = tile + tile_row(e, quarter) * (TT + 1) + t;
+                to[0] = bf16_to_f32(v[j] & 0xffffu);
+                to[1] = __uint_as_float(v[j] & 0xffff0000u);
+            }
+        }
+        return;
+    }
     const int t = threadIdx.x % TT;
     const bool in = n0 + t < n;
     for (int e0 = threadIdx.x / TT; e0 < d; e0 += 8 * (kTileThreads / TT)) {
@@ -167,38 +258,81 @@ __device__ __forceinline__ void tile_load(const void* src, int64_t n, int d, int
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int e = e0 + j * (kTileThreads / TT);
-            if (e < d) tile[e * (TT + 1) + t] = v[j];
+            if (e < d) tile[tile_row(e, quarter) * (TT + 1) + t] = v[j];
         }
     }
 }
 
 template <class T, int TT>
-__device__ __forceinline__ void tile_store(void* dst, int64_t n, int d, int64_t n0,
+__device__ __forceinline__ void tile_store(void* dst, int64_t n, int d, int64_t n0, bool pairs,
                                            const float* tile) {
+    const int quarter = tile_quarter(d);
+    if (T::kBytes == 2 && pairs) {
+        constexpr int kCols = TT / 2, kRows = kTileThreads / kCols;
+        const int t = 2 * (threadIdx.x % kCols);
+        if (n0 + t >= n) return;
+        uint16_t* to = static_cast<uint16_t*>(dst);
+        for (int e = threadIdx.x / kCols; e < d; e += kRows) {
+            const float* x = tile + tile_row(e, quarter) * (TT + 1) + t;
+            *reinterpret_cast<uint32_t*>(to + static_cast<int64_t>(e) * n + n0 + t) =
+                f32_to_bf16(x[0]) | (static_cast<uint32_t>(f32_to_bf16(x[1])) << 16);
+        }
+        return;
+    }
     const int t = threadIdx.x % TT;
     if (n0 + t >= n) return;
     for (int e = threadIdx.x / TT; e < d; e += kTileThreads / TT)
-        T::store(dst, static_cast<int64_t>(e) * n + n0 + t, tile[e * (TT + 1) + t]);
+        T::store(dst, static_cast<int64_t>(e) * n + n0 + t,
+                 tile[tile_row(e, quarter) * (TT + 1) + t]);
 }
 
-template <int EPL, int TT>
+// Tokens of a tile: 32 (128 bytes of a float32 feature) where it takes at most
+// `lds` bytes and the workgroups still fill the card, else 16.
+inline int tile_tokens(int64_t n, int64_t d, int64_t lds) {
+    return 4 * tile_quarter(d) * 33 * 4 <= lds && n >= 32 * kTileMinGroups ? 32 : 16;
+}
+
+inline bool tile_pairs(const slk_norm* a, std::initializer_list<const void*> cols) {
+    if (a->dtype != SLK_BF16 || a->n % 2 != 0) return false;
+    for (const void* p : cols)
+        if (p != nullptr && !aligned_to(p, 4)) return false;
+    return true;
+}
+
+template <int EPL, int TT, bool VEC>
 __device__ __forceinline__ void tile_row_load(const float* tile, int t, int d, int l,
                                               float (&v)[EPL]) {
+    const int quarter = tile_quarter(d);
 #pragma unroll
     for (int q = 0; q < EPL; ++q) {
-        const int e = q * kWave + l;
-        v[q] = e < d ? tile[e * (TT + 1) + t] : 0.0f;
+        const int e = RowLay<EPL, 1, VEC>::at(q, l);
+        v[q] = e < d ? tile[tile_row(e, quarter) * (TT + 1) + t] : 0.0f;
     }
 }
 
-template <int EPL, int TT>
+template <int EPL, int TT, bool VEC>
 __device__ __forceinline__ void tile_row_store(float* tile, int t, int d, int l,
                                                const float (&v)[EPL]) {
+    const int quarter = tile_quarter(d);
 #pragma unroll
     for (int q = 0; q < EPL; ++q) {
-        const int e = q * kWave + l;
-        if (e < d) tile[e * (TT + 1) + t] = v[q];
+        const int e = RowLay<EPL, 1, VEC>::at(q, l);
+        if (e < d) tile[tile_row(e, quarter) * (TT + 1) + t] = v[q];
     }
 }
+
+// A token-major row fetched ahead (AHEAD), or loaded when asked for.
+template <class T, int EPL, bool VEC, bool AHEAD>
+struct Ahead {
+    RawRow<T, EPL, 1> raw;
+    __device__ __forceinline__ void fetch(const void* p, int64_t off, int d, int l) {
+        if constexpr (VEC && AHEAD) raw.load(p, off, d, l);
+    }
+    __device__ __forceinline__ void get(const void* p, int64_t off, int d, int l,
+                                        float (&v)[EPL]) const {
+        if constexpr (VEC && AHEAD) raw.get(v);
+        else row_load<T, EPL, 1, VEC>(p, off, d, l, v);
+    }
+};
 
 }  // namespace slk

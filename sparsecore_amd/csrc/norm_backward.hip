@@ -40,26 +40,19 @@ struct Acc {
 };
 constexpr int kGateSum = 4;
 
-// One token: dy, dr and the branch u as this lane's features; leaves dbranch in
-// u. POST and GATE are compile-time: without them their sums take no registers.
-template <class T, int EPL, int TW, bool VEC, bool POST, bool GATE, class Sum>
-__device__ __forceinline__ void backward_row(const BwdRow& p, int64_t n, int l,
-                                             float (&dy)[EPL], float (&u)[EPL], Acc<EPL>& acc,
-                                             Sum& sum) {
-    using Lay = RowLay<EPL, TW, VEC>;
-    const int64_t off = n * p.d;
-    const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + 4 * n);
-    float g[EPL], s[EPL];
-    if (p.dr != nullptr) {
-        row_load<T, EPL, TW, VEC>(p.dr, off, p.d, l, g);
-    } else {
-#pragma unroll
-        for (int q = 0; q < EPL; ++q) g[q] = 0.0f;
-    }
+// One token: dy, xh (r), g (dr) and the branch u as this lane's features; leaves
+// dx in g and dbranch in u. vec(k, v) gives v the features of weight (k = 0),
+// post_weight (1), post_bias (2) or the token's gate (3). POST and GATE are
+// compile-time: without them their sums take no registers. Features past d hold
+// 0 in every array read, so they add nothing to a sum; what they leave in g and
+// u is not stored.
+template <int EPL, bool POST, bool GATE, class Vec, class Sum, class Dx>
+__device__ __forceinline__ void backward_row(const BwdRow& p, const f32x4 st, float (&dy)[EPL],
+                                             float (&xh)[EPL], float (&g)[EPL], float (&u)[EPL],
+                                             Acc<EPL>& acc, Vec&& vec, Sum& sum, Dx&& store_dx) {
+    float s[EPL];
     if (p.dy != nullptr) {
-        float xh[EPL];
-        row_load<T, EPL, TW, VEC>(p.r, off, p.d, l, xh);
-        row_load<T, EPL, TW, VEC>(p.weight, 0, p.d, l, s);
+        vec(0, s);
         float m[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int q = 0; q < EPL; ++q) {
@@ -71,31 +64,32 @@ __device__ __forceinline__ void backward_row(const BwdRow& p, int64_t n, int l,
             m[1] = fmaf(s[q], xh[q], m[1]);
         }
         sum(m);
-        const float ma = p.layer ? m[0] * p.inv_d : 0.0f, mx = m[1] * p.inv_d;
+        // g += rstd·(s - ma - xh·mx)
+        const float ma = p.layer ? m[0] * p.inv_d * st[1] : 0.0f, mx = m[1] * p.inv_d * st[1];
 #pragma unroll
-        for (int q = 0; q < EPL; ++q) g[q] = fmaf(st[1], s[q] - ma - xh[q] * mx, g[q]);
+        for (int q = 0; q < EPL; ++q)
+            g[q] = fmaf(-xh[q], mx, fmaf(st[1], s[q], g[q] - ma));
     }
-    if (p.dx != nullptr) row_store<T, EPL, TW, VEC>(p.dx, off, p.d, l, g);
+    store_dx(g);
     if (!p.need_u && p.dbranch == nullptr) return;
-    if (POST) {
-#pragma unroll
-        for (int q = 0; q < EPL; ++q) {
-            u[q] = Lay::at(q, l) < p.d ? (u[q] - st[2]) * st[3] : 0.0f;  // uhat
-        }
-    }
 #pragma unroll
     for (int q = 0; q < EPL; ++q) g[q] *= p.scale;
+    if (POST) {
+#pragma unroll
+        for (int q = 0; q < EPL; ++q) u[q] = (u[q] - st[2]) * st[3];  // uhat
+    }
     if (GATE) {
         if (p.dgate != nullptr || p.at[kGateSum] >= 0) {
             if (POST) {
-                row_load<T, EPL, TW, VEC>(p.post_weight, 0, p.d, l, s);
                 float o[EPL];
-#pragma unroll
-                for (int q = 0; q < EPL; ++q) o[q] = u[q] * s[q];
+                vec(1, o);
                 if (p.post_bias != nullptr) {
-                    row_load<T, EPL, TW, VEC>(p.post_bias, 0, p.d, l, s);
+                    vec(2, s);
 #pragma unroll
-                    for (int q = 0; q < EPL; ++q) o[q] += s[q];
+                    for (int q = 0; q < EPL; ++q) o[q] = fmaf(u[q], o[q], s[q]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < EPL; ++q) o[q] *= u[q];
                 }
 #pragma unroll
                 for (int q = 0; q < EPL; ++q)
@@ -106,13 +100,13 @@ __device__ __forceinline__ void backward_row(const BwdRow& p, int64_t n, int l,
                     acc.v[kGateSum][q] = fmaf(g[q], u[q], acc.v[kGateSum][q]);
             }
         }
-        row_load<T, EPL, TW, VEC>(p.gate, n / p.per_gate * p.d, p.d, l, s);
+        vec(3, s);
 #pragma unroll
         for (int q = 0; q < EPL; ++q) g[q] *= s[q];
     }
     if (POST) {
         float m[2] = {0.0f, 0.0f};
-        row_load<T, EPL, TW, VEC>(p.post_weight, 0, p.d, l, s);
+        vec(1, s);
 #pragma unroll
         for (int q = 0; q < EPL; ++q) {
             acc.v[2][q] = fmaf(g[q], u[q], acc.v[2][q]);
@@ -122,9 +116,9 @@ __device__ __forceinline__ void backward_row(const BwdRow& p, int64_t n, int l,
             m[1] = fmaf(s[q], u[q], m[1]);
         }
         sum(m);
-        const float ma = p.layer ? m[0] * p.inv_d : 0.0f, mx = m[1] * p.inv_d;
+        const float ma = p.layer ? m[0] * p.inv_d * st[3] : 0.0f, mx = m[1] * p.inv_d * st[3];
 #pragma unroll
-        for (int q = 0; q < EPL; ++q) u[q] = st[3] * (s[q] - ma - u[q] * mx);
+        for (int q = 0; q < EPL; ++q) u[q] = fmaf(-u[q], mx, fmaf(st[3], s[q], -ma));
     } else {
 #pragma unroll
         for (int q = 0; q < EPL; ++q) u[q] = g[q];
@@ -148,20 +142,32 @@ __device__ __forceinline__ void store_f32(float* to, int d, int l, const float (
     }
 }
 
-// dgate of the tokens [lo, n] of a team, n their group's last or the team's
-// last: the gate's own gradient if the group is whole, else a partial row: a
-// team has at most two, of the group that began before it (slot 0) and of the
-// one that goes on after it (slot 1).
+// The tokens that share a gate's row, followed token by token (a division a
+// token costs more than its arithmetic).
+struct GateRun {
+    int64_t row, lo, hi;  // the gate's row, its tokens [lo, hi)
+    __device__ __forceinline__ GateRun(const BwdRow& p, int64_t n)
+        : row(n / p.per_gate), lo(row * p.per_gate), hi(lo + p.per_gate) {}
+    __device__ __forceinline__ void next(const BwdRow& p, int64_t n) {
+        if (n == hi) {
+            ++row;
+            lo = hi;
+            hi += p.per_gate;
+        }
+    }
+};
+
+// dgate of a run's tokens in [t0, t1), a team's: the gate's own gradient if they
+// are the whole run, else a partial row: a team has at most two, of the run
+// that began before it (slot 0) and of the one that goes on after it (slot 1).
 template <class T, int EPL, int TW, bool VEC>
-__device__ __forceinline__ void flush(const BwdRow& p, int64_t team, int64_t n, int l,
-                                      float (&dgate)[EPL]) {
-    const int64_t grp = n / p.per_gate;
-    const int64_t lo = grp * p.per_gate, hi = lo + p.per_gate;
-    const int64_t t0 = team * p.per_team;
-    const int64_t t1 = t0 + p.per_team < p.n ? t0 + p.per_team : p.n;
-    if (lo >= t0 && hi <= t1) row_store<T, EPL, TW, VEC>(p.dgate, grp * p.d, p.d, l, dgate);
-    else store_f32<EPL, TW, VEC>(p.gate_partial + (2 * team + (lo < t0 ? 0 : 1)) * p.d, p.d, l,
-                                 dgate);
+__device__ __forceinline__ void flush(const BwdRow& p, int64_t team, int64_t t0, int64_t t1,
+                                      const GateRun& run, int l, float (&dgate)[EPL]) {
+    if (run.lo >= t0 && run.hi <= t1)
+        row_store<T, EPL, TW, VEC>(p.dgate, run.row * p.d, p.d, l, dgate);
+    else
+        store_f32<EPL, TW, VEC>(p.gate_partial + (2 * team + (run.lo < t0 ? 0 : 1)) * p.d, p.d, l,
+                                dgate);
     clear(dgate);
 }
 
@@ -190,6 +196,23 @@ __device__ __forceinline__ void write_partials(const BwdRow& p, int64_t group, i
     }
 }
 
+// backward_row with the vectors loaded where they are used.
+template <class T, int EPL, int TW, bool VEC, bool POST, bool GATE, class Sum>
+__device__ __forceinline__ void backward_token(const BwdRow& p, int64_t n, int64_t gate_row, int l,
+                                               float (&dy)[EPL], float (&r)[EPL], float (&g)[EPL],
+                                               float (&u)[EPL], Acc<EPL>& acc, Sum& sum) {
+    const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + 4 * n);
+    auto vec = [&](int k, float (&v)[EPL]) {
+        const void* from = k == 0 ? p.weight : k == 1 ? p.post_weight : k == 2 ? p.post_bias
+                                                                              : p.gate;
+        row_load<T, EPL, TW, VEC>(from, k == 3 ? gate_row * p.d : 0, p.d, l, v);
+    };
+    auto store_dx = [&](const float (&v)[EPL]) {
+        if (p.dx != nullptr) row_store<T, EPL, TW, VEC>(p.dx, n * p.d, p.d, l, v);
+    };
+    backward_row<EPL, POST, GATE>(p, st, dy, r, g, u, acc, vec, sum, store_dx);
+}
+
 template <class T, int EPL, int TW, bool VEC, bool POST, bool GATE>
 __global__ __launch_bounds__(TW > 4 ? TW * kWave : kNormThreads) void norm_backward_kernel(
     const BwdRow p) {
@@ -204,14 +227,83 @@ __global__ __launch_bounds__(TW > 4 ? TW * kWave : kNormThreads) void norm_backw
     Acc<EPL> acc;
 #pragma unroll
     for (int k = 0; k < kColSums; ++k) clear(acc.v[k]);
-    for (int64_t n = begin; n < end; ++n) {
-        float dy[EPL], u[EPL];
-        if (p.dy != nullptr) row_load<T, EPL, TW, VEC>(p.dy, n * p.d, p.d, l, dy);
-        if (p.need_u) row_load<T, EPL, TW, VEC>(p.branch, n * p.d, p.d, l, u);
-        backward_row<T, EPL, TW, VEC, POST, GATE>(p, n, l, dy, u, acc, sum);
-        if (GATE && p.dgate != nullptr && ((n + 1) % p.per_gate == 0 || n + 1 == end))
-            flush<T, EPL, TW, VEC>(p, team, n, l, acc.v[kGateSum]);
-        if (p.dbranch != nullptr) row_store<T, EPL, TW, VEC>(p.dbranch, n * p.d, p.d, l, u);
+    GateRun run(p, begin);
+    // sixteen waves leave a lane 128 registers: no room for a row ahead at 16 features
+    if constexpr (VEC && !(TW == 16 && EPL == 16)) {
+        // The next token's arrays are on their way while one is worked on; the
+        // vectors stay in registers as they are in memory.
+        using Raw = RawRow<T, EPL, TW>;
+        Raw w, pw, pb, gate, dy, r, dr, u;
+        f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.dy != nullptr) w.load(p.weight, 0, p.d, l);
+        if (POST) {
+            pw.load(p.post_weight, 0, p.d, l);
+            if (p.post_bias != nullptr) pb.load(p.post_bias, 0, p.d, l);
+        }
+        auto fetch = [&](int64_t n) {
+            const int64_t off = n * p.d;
+            if (p.dy != nullptr) {
+                dy.load(p.dy, off, p.d, l);
+                r.load(p.r, off, p.d, l);
+            }
+            if (p.dr != nullptr) dr.load(p.dr, off, p.d, l);
+            if (p.need_u) u.load(p.branch, off, p.d, l);
+            st = *reinterpret_cast<const f32x4*>(p.stats + 4 * n);
+        };
+        if (begin < end) {
+            fetch(begin);
+            if (GATE) gate.load(p.gate, run.row * p.d, p.d, l);
+        }
+        for (int64_t n = begin; n < end; ++n) {
+            float vdy[EPL], vr[EPL], g[EPL], vu[EPL];
+            if (p.dy != nullptr) {
+                dy.get(vdy);
+                r.get(vr);
+            }
+            if (p.dr != nullptr) dr.get(g);
+            else clear(g);
+            if (p.need_u) u.get(vu);
+            const f32x4 s = st;
+            if (n + 1 < end) fetch(n + 1);
+            auto vec = [&](int k, float (&v)[EPL]) {
+                if (k == 0) w.get(v);
+                else if (k == 1) pw.get(v);
+                else if (k == 2) pb.get(v);
+                else gate.get(v);
+            };
+            auto store_dx = [&](const float (&v)[EPL]) {
+                if (p.dx != nullptr) row_store<T, EPL, TW, VEC>(p.dx, n * p.d, p.d, l, v);
+            };
+            backward_row<EPL, POST, GATE>(p, s, vdy, vr, g, vu, acc, vec, sum, store_dx);
+            if (p.dbranch != nullptr) row_store<T, EPL, TW, VEC>(p.dbranch, n * p.d, p.d, l, vu);
+            if (GATE) {
+                if (p.dgate != nullptr && (n + 1 == run.hi || n + 1 == end))
+                    flush<T, EPL, TW, VEC>(p, team, begin, end, run, l, acc.v[kGateSum]);
+                if (n + 1 == run.hi && n + 1 < end) {
+                    run.next(p, n + 1);
+                    gate.load(p.gate, run.row * p.d, p.d, l);
+                }
+            }
+        }
+    } else {
+        for (int64_t n = begin; n < end; ++n) {
+            float dy[EPL], r[EPL], g[EPL], u[EPL];
+            const int64_t off = n * p.d;
+            if (p.dy != nullptr) {
+                row_load<T, EPL, TW, VEC>(p.dy, off, p.d, l, dy);
+                row_load<T, EPL, TW, VEC>(p.r, off, p.d, l, r);
+            }
+            if (p.dr != nullptr) row_load<T, EPL, TW, VEC>(p.dr, off, p.d, l, g);
+            else clear(g);
+            if (p.need_u) row_load<T, EPL, TW, VEC>(p.branch, off, p.d, l, u);
+            backward_token<T, EPL, TW, VEC, POST, GATE>(p, n, run.row, l, dy, r, g, u, acc, sum);
+            if (p.dbranch != nullptr) row_store<T, EPL, TW, VEC>(p.dbranch, off, p.d, l, u);
+            if (GATE) {
+                if (p.dgate != nullptr && (n + 1 == run.hi || n + 1 == end))
+                    flush<T, EPL, TW, VEC>(p, team, begin, end, run, l, acc.v[kGateSum]);
+                run.next(p, n + 1);
+            }
+        }
     }
     if (p.arrays == 0) return;
     if (TW > 1) __syncthreads();
@@ -221,10 +313,10 @@ __global__ __launch_bounds__(TW > 4 ? TW * kWave : kNormThreads) void norm_backw
 // Feature-major dy or branch (and dbranch): TT tokens a workgroup, TT /
 // kTileWaves consecutive ones a wave. dy's tile takes dbranch where the branch
 // has none of its own.
-template <class T, int EPL, int TT, bool POST, bool GATE>
+template <class T, int EPL, int TT, bool VEC, bool POST, bool GATE>
 __global__ __launch_bounds__(kTileThreads) void norm_backward_tile_kernel(const BwdRow p,
                                                                           int branch_cols,
-                                                                          int y_cols) {
+                                                                          int y_cols, int pairs) {
     extern __shared__ float sh[];
     TeamSum<1, 2> sum{nullptr};
     const int l = threadIdx.x & (kWave - 1);
@@ -234,38 +326,57 @@ __global__ __launch_bounds__(kTileThreads) void norm_backward_tile_kernel(const 
     const bool dy_tile = y_cols && p.dy != nullptr;
     const bool u_tile = branch_cols && p.need_u;
     float* ty = sh;
-    float* tu = dy_tile && u_tile ? sh + static_cast<int64_t>(p.d) * (TT + 1) : sh;
-    if (dy_tile) tile_load<T, TT>(p.dy, p.n, p.d, n0, ty);
-    if (u_tile) tile_load<T, TT>(p.branch, p.n, p.d, n0, tu);
-    __syncthreads();
+    float* tu = dy_tile && u_tile ? sh + 4 * tile_quarter(p.d) * (TT + 1) : sh;
     constexpr int kPer = TT / kTileWaves;
+    const int64_t begin = n0 + wv * kPer;
+    const int64_t end = begin + kPer < p.n ? begin + kPer : p.n;
+    Ahead<T, EPL, VEC, (EPL == 16 && !POST)> ar, adr;
+    auto fetch = [&](int64_t n) {
+        if (p.dy != nullptr) ar.fetch(p.r, n * p.d, p.d, l);
+        if (p.dr != nullptr) adr.fetch(p.dr, n * p.d, p.d, l);
+    };
+    if (begin < end) fetch(begin);
+    if (dy_tile) tile_load<T, TT>(p.dy, p.n, p.d, n0, pairs, ty);
+    if (u_tile) tile_load<T, TT>(p.branch, p.n, p.d, n0, pairs, tu);
+    __syncthreads();
     const int64_t team = group * kTileWaves + wv;
     Acc<EPL> acc;
 #pragma unroll
     for (int k = 0; k < kColSums; ++k) clear(acc.v[k]);
-    const int64_t end = n0 + (wv + 1) * kPer < p.n ? n0 + (wv + 1) * kPer : p.n;
-    for (int64_t n = n0 + wv * kPer; n < end; ++n) {
+    GateRun run(p, begin);
+#pragma unroll 1  // unrolled, the tokens' registers add up
+    for (int64_t n = begin; n < end; ++n) {
         const int t = static_cast<int>(n - n0);
-        float dy[EPL], u[EPL];
-        if (dy_tile) tile_row_load<EPL, TT>(ty, t, p.d, l, dy);
-        else if (p.dy != nullptr) row_load<T, EPL, 1, false>(p.dy, n * p.d, p.d, l, dy);
-        if (u_tile) tile_row_load<EPL, TT>(tu, t, p.d, l, u);
-        else if (p.need_u) row_load<T, EPL, 1, false>(p.branch, n * p.d, p.d, l, u);
-        backward_row<T, EPL, 1, false, POST, GATE>(p, n, l, dy, u, acc, sum);
-        if (GATE && p.dgate != nullptr && ((n + 1) % p.per_gate == 0 || n + 1 == end))
-            flush<T, EPL, 1, false>(p, team, n, l, acc.v[kGateSum]);
+        float dy[EPL], r[EPL], g[EPL], u[EPL];
+        const int64_t off = n * p.d;
+        if (p.dy != nullptr) {
+            ar.get(p.r, off, p.d, l, r);
+            if (dy_tile) tile_row_load<EPL, TT, VEC>(ty, t, p.d, l, dy);
+            else row_load<T, EPL, 1, VEC>(p.dy, off, p.d, l, dy);
+        }
+        if (p.dr != nullptr) adr.get(p.dr, off, p.d, l, g);
+        else clear(g);
+        if (n + 1 < end) fetch(n + 1);
+        if (u_tile) tile_row_load<EPL, TT, VEC>(tu, t, p.d, l, u);
+        else if (p.need_u) row_load<T, EPL, 1, VEC>(p.branch, off, p.d, l, u);
+        backward_token<T, EPL, 1, VEC, POST, GATE>(p, n, run.row, l, dy, r, g, u, acc, sum);
         if (p.dbranch != nullptr) {
-            if (branch_cols) tile_row_store<EPL, TT>(tu, t, p.d, l, u);
-            else row_store<T, EPL, 1, false>(p.dbranch, n * p.d, p.d, l, u);
+            if (branch_cols) tile_row_store<EPL, TT, VEC>(tu, t, p.d, l, u);
+            else row_store<T, EPL, 1, VEC>(p.dbranch, off, p.d, l, u);
+        }
+        if (GATE) {
+            if (p.dgate != nullptr && (n + 1 == run.hi || n + 1 == end))
+                flush<T, EPL, 1, VEC>(p, team, begin, end, run, l, acc.v[kGateSum]);
+            run.next(p, n + 1);
         }
     }
     __syncthreads();
     if (p.dbranch != nullptr && branch_cols) {
-        tile_store<T, TT>(p.dbranch, p.n, p.d, n0, tu);
+        tile_store<T, TT>(p.dbranch, p.n, p.d, n0, pairs, tu);
         __syncthreads();
     }
     if (p.arrays == 0) return;
-    write_partials<EPL, 1, false, kTileWaves>(p, group, wv, l, acc, sh);
+    write_partials<EPL, 1, VEC, kTileWaves>(p, group, wv, l, acc, sh);
 }
 
 // out[c] = Σ over the partials of column c, in order: 64 columns a workgroup,
@@ -306,20 +417,43 @@ __global__ __launch_bounds__(1024) void norm_colsum_kernel(const ColSums p) {
     }
 }
 
-// dgate of a gate row whose tokens more than one team held: its teams'
-// partial rows, in order.
-template <class T>
-__global__ __launch_bounds__(kNormThreads) void norm_gate_kernel(const BwdRow p) {
+// dgate of a gate row whose tokens more than one team held: its teams' partial
+// rows, in order; PARTS threads a column, each a run of consecutive teams.
+template <class T, int PARTS>
+__global__ __launch_bounds__(PARTS * kWave) void norm_gate_kernel(const BwdRow p) {
+    __shared__ float sh[PARTS][kWave];
     const int64_t grp = blockIdx.x;
     const int64_t lo = grp * p.per_gate, hi = lo + p.per_gate;
     const int64_t t0 = lo / p.per_team, t1 = (hi - 1) / p.per_team;
     if (t0 == t1) return;  // written by its team
-    const int e = blockIdx.y * kNormThreads + threadIdx.x;
-    if (e >= p.d) return;
+    const int c = threadIdx.x & (kWave - 1), part = threadIdx.x >> 6;
+    const int e = blockIdx.y * kWave + c;
+    const int64_t per = (t1 - t0 + PARTS) / PARTS;
+    const int64_t a = t0 + part * per, b = a + per < t1 + 1 ? a + per : t1 + 1;
     float s = 0.0f;
-    for (int64_t t = t0; t <= t1; ++t)
-        s += p.gate_partial[(2 * t + (lo < t * p.per_team ? 0 : 1)) * p.d + e];
-    T::store(p.dgate, grp * p.d + e, s);
+    if (e < p.d) {
+        // slot 0 of a team that began inside the run, slot 1 of the one it began in
+        auto at = [&](int64_t t) {
+            return p.gate_partial[(2 * t + (lo < t * p.per_team ? 0 : 1)) * p.d + e];
+        };
+        int64_t t = a;
+        for (; t + 8 <= b; t += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = at(t + j);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; t < b; ++t) s += at(t);
+    }
+    if (PARTS > 1) {
+        sh[part][c] = s;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int k = 1; k < PARTS; ++k) s += sh[k][c];
+    }
+    if (e < p.d) T::store(p.dgate, grp * p.d + e, s);
 }
 
 // Teams and workgroups of a backward, and its workspace.
@@ -342,6 +476,12 @@ struct Plan {
 // enough that their partial rows cost little beside the arrays themselves.
 constexpr int64_t kBwdGroups = 512;
 
+// Whether the branch itself is read (else only its gradient is written).
+bool needs_branch(const slk_norm* a) {
+    return a->branch != nullptr && (a->post_weight != nullptr ||
+                                    (a->gate != nullptr && a->dgate != nullptr));
+}
+
 Plan make_plan(const slk_norm* a) {
     Plan p;
     p.d = a->d;
@@ -354,7 +494,9 @@ Plan make_plan(const slk_norm* a) {
                                    p.gate_all};
     p.arrays = 0;
     for (int k = 0; k < kColSums; ++k) p.at[k] = wanted[k] ? p.arrays++ : -1;
-    p.tile = (a->branch_cols && a->branch != nullptr) || a->y_cols ? 16 : 0;
+    const bool cols = (a->branch_cols && a->branch != nullptr) || a->y_cols;
+    const bool both = a->branch_cols && needs_branch(a) && a->y_cols && a->dy != nullptr;
+    p.tile = cols ? tile_tokens(a->n, a->d, (both ? 75 : 150) * 1024) : 0;
     if (p.tile) {
         p.tw = 1;
         p.per_team = p.tile / kTileWaves;
@@ -378,13 +520,32 @@ int backward(const slk_norm* a, const Plan& plan, const BwdRow& p, hipStream_t s
     if (plan.tile) {
         const bool dy_tile = a->y_cols && p.dy != nullptr, u_tile = a->branch_cols && p.need_u;
         const size_t tiles = dy_tile && u_tile ? 2 : 1;
-        const size_t lds = tiles * p.d * (16 + 1) * sizeof(float);
-        auto go = [&](auto k) {
-            hipLaunchKernelGGL(k, grid, dim3(kTileThreads), lds, st, p, a->branch_cols,
-                               a->y_cols);
+        const size_t lds = tiles * 4 * tile_quarter(p.d) * (plan.tile + 1) * sizeof(float);
+        const int pairs = tile_pairs(a, {dy_tile ? a->dy : nullptr, u_tile ? a->branch : nullptr,
+                                         a->branch_cols ? a->dbranch : nullptr});
+        const bool vec = norm_vec(a, {a->r, a->branch_cols ? nullptr : a->branch, a->gate,
+                                      a->weight, a->post_weight, a->post_bias, a->dr,
+                                      a->y_cols ? nullptr : a->dy, a->dx,
+                                      a->branch_cols ? nullptr : a->dbranch, a->dgate});
+        auto go = [&](auto kv, auto ks) {
+            if (vec) {
+                hipLaunchKernelGGL(kv, grid, dim3(kTileThreads), lds, st, p, a->branch_cols,
+                                   a->y_cols, pairs);
+            } else {
+                hipLaunchKernelGGL(ks, grid, dim3(kTileThreads), lds, st, p, a->branch_cols,
+                                   a->y_cols, pairs);
+            }
         };
-        if (p.d <= 512) go(norm_backward_tile_kernel<T, 8, 16, POST, GATE>);
-        else go(norm_backward_tile_kernel<T, 16, 16, POST, GATE>);
+        auto pick = [&](auto epl, auto tt) {
+            constexpr int E = decltype(epl)::value, TT = decltype(tt)::value;
+            go(norm_backward_tile_kernel<T, E, TT, true, POST, GATE>,
+               norm_backward_tile_kernel<T, E, TT, false, POST, GATE>);
+        };
+        using std::integral_constant;
+        if (p.d <= 512 && plan.tile == 32) pick(integral_constant<int, 8>{}, integral_constant<int, 32>{});
+        else if (p.d <= 512) pick(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+        else if (plan.tile == 32) pick(integral_constant<int, 16>{}, integral_constant<int, 32>{});
+        else pick(integral_constant<int, 16>{}, integral_constant<int, 16>{});
         return check_launch("norm_backward");
     }
     const bool vec = norm_vec(a, {a->r, a->branch, a->gate, a->weight, a->post_weight,
@@ -429,10 +590,13 @@ int backward_any(const slk_norm* a, const Plan& plan, const BwdRow& p, hipStream
         if (rc != SLK_OK) return rc;
     }
     if (plan.gate_some) {
-        hipLaunchKernelGGL(norm_gate_kernel<T>,
-                           dim3(static_cast<unsigned>(a->gate_rows),
-                                static_cast<unsigned>(ceil_div(p.d, kNormThreads))),
-                           dim3(kNormThreads), 0, st, p);
+        const dim3 grid(static_cast<unsigned>(a->gate_rows),
+                        static_cast<unsigned>(ceil_div(p.d, kWave)));
+        if (p.per_gate >= 32 * p.per_team) {
+            hipLaunchKernelGGL((norm_gate_kernel<T, 16>), grid, dim3(16 * kWave), 0, st, p);
+        } else {
+            hipLaunchKernelGGL((norm_gate_kernel<T, 1>), grid, dim3(kWave), 0, st, p);
+        }
         rc = check_launch("norm_backward gate");
     }
     return rc;
@@ -486,8 +650,7 @@ extern "C" int slk_norm_backward(const slk_norm* a, void* stream) {
     p.arrays = plan.arrays;
     for (int k = 0; k < kColSums; ++k) p.at[k] = plan.at[k];
     p.layer = a->layer != 0;
-    p.need_u = a->branch != nullptr &&
-               (a->post_weight != nullptr || (a->gate != nullptr && a->dgate != nullptr));
+    p.need_u = needs_branch(a);
     p.scale = static_cast<float>(a->scale);
     p.inv_d = 1.0f / static_cast<float>(a->d);
     return a->dtype == SLK_F32 ? backward_any<F32>(a, plan, p, as_stream(stream))

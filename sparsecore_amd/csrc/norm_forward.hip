@@ -17,14 +17,12 @@ struct FwdRow {
     float scale, eps, inv_d;
 };
 
-// r and y of token n from its branch features u (changed in place: r), x and y
-// as this lane's features.
+// r and y of token n from its branch features u (changed in place: r) and x,
+// which is in y.
 template <class T, int EPL, int TW, bool VEC, class Sum>
 __device__ __forceinline__ void forward_row(const FwdRow& p, int64_t n, int l, float (&u)[EPL],
                                             float (&y)[EPL], Sum& sum) {
-    const int64_t off = n * p.d;
     float s[EPL];
-    row_load<T, EPL, TW, VEC>(p.x, off, p.d, l, y);
     float pmean = 0.0f, prstd = 0.0f;
     if (p.has_branch) {
         if (p.post_weight != nullptr) {
@@ -77,6 +75,7 @@ __global__ __launch_bounds__(TW > 4 ? TW * kWave : kNormThreads) void norm_forwa
                               : blockIdx.x;
     if (n >= p.n) return;  // a whole team
     float u[EPL], v[EPL];
+    row_load<T, EPL, TW, VEC>(p.x, n * p.d, p.d, l, v);
     if (p.has_branch) row_load<T, EPL, TW, VEC>(branch, n * p.d, p.d, l, u);
     forward_row<T, EPL, TW, VEC>(p, n, l, u, v, sum);
     if (p.has_branch) row_store<T, EPL, TW, VEC>(r, n * p.d, p.d, l, u);
@@ -85,35 +84,41 @@ __global__ __launch_bounds__(TW > 4 ? TW * kWave : kNormThreads) void norm_forwa
 
 // branch or y feature-major: TT tokens a workgroup, the feature-major arrays
 // through one LDS tile (y overwrites the branch token by token).
-template <class T, int EPL, int TT>
+template <class T, int EPL, int TT, bool VEC>
 __global__ __launch_bounds__(kTileThreads) void norm_forward_tile_kernel(
     const FwdRow p, const void* __restrict__ branch, void* __restrict__ r, void* __restrict__ y,
-    int branch_cols, int y_cols) {
+    int branch_cols, int y_cols, int pairs) {
     extern __shared__ float tile[];
     TeamSum<1, 1> sum{nullptr};
     const int l = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t n0 = xcd_logical_block(blockIdx.x, gridDim.x) * TT;
+    Ahead<T, EPL, VEC, true> x;
+    if (n0 + wv < p.n) x.fetch(p.x, (n0 + wv) * p.d, p.d, l);
     if (branch_cols) {
-        tile_load<T, TT>(branch, p.n, p.d, n0, tile);
+        tile_load<T, TT>(branch, p.n, p.d, n0, pairs, tile);
         __syncthreads();
     }
+#pragma unroll 1  // unrolled, the tokens' registers add up
     for (int t = wv; t < TT; t += kTileWaves) {
         const int64_t n = n0 + t;
         if (n >= p.n) break;
         float u[EPL], v[EPL];
+        x.get(p.x, n * p.d, p.d, l, v);
+        if (t + kTileWaves < TT && n + kTileWaves < p.n)
+            x.fetch(p.x, (n + kTileWaves) * p.d, p.d, l);
         if (p.has_branch) {
-            if (branch_cols) tile_row_load<EPL, TT>(tile, t, p.d, l, u);
-            else row_load<T, EPL, 1, false>(branch, n * p.d, p.d, l, u);
+            if (branch_cols) tile_row_load<EPL, TT, VEC>(tile, t, p.d, l, u);
+            else row_load<T, EPL, 1, VEC>(branch, n * p.d, p.d, l, u);
         }
-        forward_row<T, EPL, 1, false>(p, n, l, u, v, sum);
-        if (p.has_branch) row_store<T, EPL, 1, false>(r, n * p.d, p.d, l, u);
-        if (y_cols) tile_row_store<EPL, TT>(tile, t, p.d, l, v);
-        else row_store<T, EPL, 1, false>(y, n * p.d, p.d, l, v);
+        forward_row<T, EPL, 1, VEC>(p, n, l, u, v, sum);
+        if (p.has_branch) row_store<T, EPL, 1, VEC>(r, n * p.d, p.d, l, u);
+        if (y_cols) tile_row_store<EPL, TT, VEC>(tile, t, p.d, l, v);
+        else row_store<T, EPL, 1, VEC>(y, n * p.d, p.d, l, v);
     }
     if (y_cols) {
         __syncthreads();
-        tile_store<T, TT>(y, p.n, p.d, n0, tile);
+        tile_store<T, TT>(y, p.n, p.d, n0, pairs, tile);
     }
 }
 
@@ -121,15 +126,33 @@ template <class T>
 int forward(const slk_norm* a, const FwdRow& p, hipStream_t st) {
     const bool cols = (a->branch_cols && a->branch != nullptr) || a->y_cols;
     if (cols) {
-        constexpr int TT = 16;
-        const dim3 grid(static_cast<unsigned>(ceil_div(a->n, TT))), wg(kTileThreads);
-        const size_t lds = static_cast<size_t>(p.d) * (TT + 1) * sizeof(float);
-        auto go = [&](auto k) {
-            hipLaunchKernelGGL(k, grid, wg, lds, st, p, a->branch, a->r, a->y, a->branch_cols,
-                               a->y_cols);
+        // two workgroups a CU: 65536 x 768 float32 takes 200 us at 16 tokens, 241 at 32
+        const int tokens = tile_tokens(a->n, p.d, 75 * 1024);
+        const int pairs = tile_pairs(a, {a->branch_cols ? a->branch : nullptr,
+                                         a->y_cols ? a->y : nullptr});
+        const bool vec = norm_vec(a, {a->x, a->branch_cols ? nullptr : a->branch, a->gate,
+                                      a->weight, a->bias, a->post_weight, a->post_bias, a->r,
+                                      a->y_cols ? nullptr : a->y});
+        const dim3 grid(static_cast<unsigned>(ceil_div(a->n, tokens))), wg(kTileThreads);
+        const size_t lds = 4 * static_cast<size_t>(tile_quarter(p.d)) * (tokens + 1) * sizeof(float);
+        auto go = [&](auto kv, auto ks) {
+            if (vec) {
+                hipLaunchKernelGGL(kv, grid, wg, lds, st, p, a->branch, a->r, a->y,
+                                   a->branch_cols, a->y_cols, pairs);
+            } else {
+                hipLaunchKernelGGL(ks, grid, wg, lds, st, p, a->branch, a->r, a->y,
+                                   a->branch_cols, a->y_cols, pairs);
+            }
         };
-        if (p.d <= 512) go(norm_forward_tile_kernel<T, 8, TT>);
-        else go(norm_forward_tile_kernel<T, 16, TT>);
+        auto pick = [&](auto epl, auto tt) {
+            constexpr int E = decltype(epl)::value, TT = decltype(tt)::value;
+            go(norm_forward_tile_kernel<T, E, TT, true>, norm_forward_tile_kernel<T, E, TT, false>);
+        };
+        using std::integral_constant;
+        if (p.d <= 512 && tokens == 32) pick(integral_constant<int, 8>{}, integral_constant<int, 32>{});
+        else if (p.d <= 512) pick(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+        else if (tokens == 32) pick(integral_constant<int, 16>{}, integral_constant<int, 32>{});
+        else pick(integral_constant<int, 16>{}, integral_constant<int, 16>{});
         return check_launch("norm_forward");
     }
     const bool vec = norm_vec(a, {a->x, a->branch, a->gate, a->weight, a->bias, a->post_weight,
