@@ -63,9 +63,11 @@ template <bool SIGNED>
 __device__ __forceinline__ void encode4(void* codes, int64_t i, int64_t n, bool vec, float scale,
                                         const float (&v)[4]) {
     uint32_t w = 0;
+    const float rcp = q8_reciprocal(scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int q = SIGNED ? q8_encode_signed(v[j], scale) : q8_encode_unsigned(v[j], scale);
+        const int q = SIGNED ? q8_encode_signed(v[j], scale, rcp)
+                             : q8_encode_unsigned(v[j], scale, rcp);
         w |= (static_cast<uint32_t>(q) & 0xffu) << (8 * j);
     }
     uint8_t* c = static_cast<uint8_t*>(codes);
@@ -141,8 +143,12 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamTable tab
     for (int j = 0; j < 4; ++j) {
         m[j] = c.b1 * m[j] + c.omb1 * g[j];
         v[j] = c.b2 * v[j] + c.omb2 * (g[j] * g[j]);
-        const float root = sqrtf(v[j]) * inv_root + c.eps;
-        p[j] = p[j] * decay - step_size * (m[j] / root);
+        // the instructions' square root and reciprocal are within an ulp; the
+        // root's takes no subnormals, so a tiny v is scaled by 2^64 around it
+        const bool tiny = v[j] < 0x1p-96f;
+        float root = __builtin_amdgcn_sqrtf(tiny ? v[j] * 0x1p64f : v[j]);
+        root = (tiny ? root * 0x1p-32f : root) * inv_root + c.eps;
+        p[j] = p[j] * decay - step_size * (m[j] * __builtin_amdgcn_rcpf(root));
     }
     store_some<T>(t.param, i, t.n, vec, p);
     if (Q8) {
@@ -197,71 +203,188 @@ struct CarryTable {
     int32_t n;
 };
 
+// How many of row_start[lo, hi) are at most s, plus lo; all before lo are. The
+// wave looks at 64 places at a time: three dependent loads for 16384 rows.
+__device__ __forceinline__ int wave_rows_upto(const int32_t* __restrict__ row_start, int s, int lo,
+                                              int hi, int lane) {
+    while (lo < hi) {
+        const int step = (hi - lo + kWave - 1) / kWave;
+        // (lo + 63 step can pass int32 for two thousand million rows)
+        const int64_t at = lo + static_cast<int64_t>(lane) * step;
+        const int c = __popcll(__ballot(at < hi && row_start[at < hi ? at : lo] <= s));
+        if (c == 0) break;
+        const int64_t up = lo + static_cast<int64_t>(c) * step;
+        lo += (c - 1) * step + 1;
+        hi = up < hi ? static_cast<int>(up) : hi;
+    }
+    return lo;
+}
+
+// col's place among old_cols[lo, hi), ascending, or -1.
+__device__ inline int find_slot(const int32_t* __restrict__ old_cols, int lo, int hi, int col) {
+    const int stop = hi;
+    while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (old_cols[mid] < col) lo = mid + 1; else hi = mid;
+    }
+    return lo < stop && old_cols[lo] == col ? lo : -1;
+}
+
 // One thread per four slots, one wave per SLK_Q8_BLOCK slots. Each live slot
 // of the new topology looks its column up among its row's old columns (both
 // ascending) and takes that slot's state; a grown connection and padding take
 // 0. Out of place: a row's slots move both ways.
+//
+// Bound by its instructions (16 million slots in 8 bits moved in 185 us when
+// every slot searched its row by itself with 64-bit places), then by the
+// latency of dependent loads. The wave finds its first row 64 places at a time
+// and brings the old columns of its own slots and kNear on either side into
+// LDS: a column is mostly that near to where it was (a rewrite that moves a
+// third of a row of 16384 shifts the rest by about a hundred slots). A lane
+// searches its first column of a row in ten steps without a branch and its next
+// ones within seven places of the last; what these miss is searched in memory.
+// Slots are below 2^31.
+constexpr int kNear = 256, kWindow = kQ8Block + 2 * kNear;
+
 __global__ __launch_bounds__(kAdamThreads) void carry_kernel(
-    const int32_t* __restrict__ row_start, int64_t nrows, int64_t total,
+    const int32_t* __restrict__ row_start, int nrows, int total,
     const int32_t* __restrict__ old_cols, const int32_t* __restrict__ old_nnz,
     const int32_t* __restrict__ new_cols, const int32_t* __restrict__ new_nnz,
     const CarryTable tab) {
-    const int64_t block = static_cast<int64_t>(blockIdx.x) * kAdamWaves + (threadIdx.x >> 6);
+    __shared__ int32_t windows[kAdamWaves][kWindow + 8];
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int block = static_cast<int>(blockIdx.x) * kAdamWaves + wv;
     const int lane = threadIdx.x & (kWave - 1);
-    if (block * kQ8Block >= total) return;
-    const int64_t i = block * kQ8Block + 4 * lane;
+    if (static_cast<int64_t>(block) * kQ8Block >= total) return;  // a wave; no barrier below
+    const int first = block * kQ8Block;
+    const int last = total - first > kQ8Block ? first + kQ8Block - 1 : total - 1;
+    const int i = first + 4 * lane;  // below 2^31 + 256: compared as total - i
 
-    // the row of slot i: the last that starts at or before it
-    int64_t lo = 0, hi = nrows;  // row in [lo - 1, hi - 1]
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (row_start[mid] <= i) lo = mid + 1; else hi = mid;
+    int32_t* win = windows[wv];
+    const int w0 = first > kNear ? first - kNear : 0;
+    const int w1 = total - last > kNear ? last + 1 + kNear : total;
+    int32_t col[4];
+#pragma unroll
+    for (int j = 0; j < kWindow / kWave; ++j) {
+        const int at = j * kWave + lane;
+        win[at] = at < w1 - w0 ? old_cols[w0 + at] : 0;
     }
-    int64_t row = lo - 1;
-    int64_t from[4];
+    const int mine = 4 * lane;  // this lane's place among the wave's slots
+#pragma unroll
+    for (int j = 0; j < 4; ++j) col[j] = mine + j <= last - first ? new_cols[i + j] : -1;
+    const int r0 = wave_rows_upto(row_start, first, 0, nrows, lane) - 1;
+    // mostly the same row or one of the next few
+    const int near = nrows - r0 > kWave + 1 ? r0 + 1 + kWave : nrows;
+    int r1 = wave_rows_upto(row_start, last, r0 + 1, near, lane) - 1;
+    if (r1 + 1 == near && near < nrows)
+        r1 = wave_rows_upto(row_start, last, near, nrows, lane) - 1;
+
+    // the lane's first row, its old columns [start, end), its live slots and its
+    // old columns' part of the window
+    int row = r0;
+    if (r0 != r1) {
+        const int s = mine <= last - first ? i : last;
+        int lo = r0 + 1, hi = r1 + 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (row_start[mid] <= s) lo = mid + 1; else hi = mid;
+        }
+        row = lo - 1;
+    }
+    int start, end, live, next, lo, hi;
+    auto enter = [&] {
+        const int r = row >= 0 ? row : 0;
+        start = row_start[r];
+        live = start + (row >= 0 ? new_nnz[r] : 0) - first;
+        next = (row + 1 < nrows ? row_start[row + 1] : total) - first;
+        const int64_t old_end = static_cast<int64_t>(start) + (row >= 0 ? old_nnz[r] : 0);
+        end = old_end < total ? static_cast<int>(old_end) : total;
+        lo = (start > w0 ? start : w0) - w0;
+        hi = (end < w1 ? end : w1) - w0;
+    };
+    enter();
+    int from[4], pos = lo;
+    bool fresh = true;  // pos says nothing about this row yet
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        from[j] = -1;
-        const int64_t s = i + j;
-        while (row + 1 < nrows && row_start[row + 1] <= s) ++row;
-        if (s >= total || row < 0) continue;
-        const int64_t start = row_start[row];
-        if (s - start >= new_nnz[row]) continue;
-        const int32_t col = new_cols[s];
-        int64_t a = start, b = start + old_nnz[row];
-        if (b > total) b = total;
-        while (a < b) {
-            const int64_t mid = (a + b) >> 1;
-            if (old_cols[mid] < col) a = mid + 1; else b = mid;
+        if (mine + j >= next && mine + j <= last - first) {
+            while (row < r1 && mine + j >= next) {
+                ++row;
+                next = (row + 1 < nrows ? row_start[row + 1] : total) - first;
+            }
+            enter();
+            pos = lo;
+            fresh = true;
         }
-        const int64_t end = start + old_nnz[row];
-        if (a < end && a < total && old_cols[a] == col) from[j] = a;
-    }
-    for (int k = 0; k < tab.n; ++k) {
-        const slk_carry_state& st = tab.s[k];
-        float v[4];
+        auto step = [&](int b) {
+            const int t = pos + b;
+            const int at = t <= hi ? t - 1 : 0;
+            pos = t <= hi && win[at] < col[j] ? t : pos;
+        };
+        if (__any(fresh)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = 0.0f;
-            if (from[j] < 0) continue;
-            if (st.kind == SLK_STATE_F32) {
-                v[j] = static_cast<const float*>(st.src)[from[j]];
-            } else {
-                const uint8_t q = static_cast<const uint8_t*>(st.src)[from[j]];
-                const float scale = st.src_scale[from[j] / kQ8Block];
-                v[j] = st.kind == SLK_STATE_Q8_SIGNED
-                           ? q8_decode_signed(static_cast<int8_t>(q), scale)
-                           : q8_decode_unsigned(q, scale);
+            for (int b = 512; b > 4; b >>= 1) step(b);
+        }
+#pragma unroll
+        for (int b = 4; b > 0; b >>= 1) step(b);
+        if (!fresh) {
+            while (pos < hi && win[pos] < col[j]) ++pos;
+        }
+        fresh = false;
+        const bool wanted = mine + j < live && mine + j <= last - first;
+        const bool in = lo < hi;
+        from[j] = wanted && in && pos < hi && win[pos] == col[j] ? w0 + pos : -1;
+        // not in the window: before it, behind it, or nowhere
+        const bool before = wanted && from[j] < 0 && in && pos == lo && w0 + lo > start;
+        const bool behind = wanted && from[j] < 0 && in && pos == hi && w0 + hi < end;
+        if (before || behind || (wanted && !in && start < end)) {
+            from[j] = find_slot(old_cols, behind ? w0 + hi : start, before ? w0 + lo : end, col[j]);
+        }
+    }
+
+    // all states' loads first, then their stores
+    const int64_t at = static_cast<int64_t>(first) + mine;
+    float v[SLK_CARRY_STATES][4];
+#pragma unroll
+    for (int k = 0; k < SLK_CARRY_STATES; ++k) {
+        if (k >= tab.n) break;
+        const slk_carry_state& st = tab.s[k];
+        if (st.kind == SLK_STATE_F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[k][j] = from[j] >= 0 ? static_cast<const float*>(st.src)[from[j]] : 0.0f;
+        } else {
+            int q[4];
+            float scale[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int f = from[j] >= 0 ? from[j] : 0;
+                q[j] = static_cast<const uint8_t*>(st.src)[f];
+                scale[j] = st.src_scale[f / kQ8Block];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = st.kind == SLK_STATE_Q8_SIGNED
+                                    ? q8_decode_signed(static_cast<int8_t>(q[j]), scale[j])
+                                    : q8_decode_unsigned(q[j], scale[j]);
+                v[k][j] = from[j] >= 0 ? x : 0.0f;
             }
         }
+    }
+#pragma unroll
+    for (int k = 0; k < SLK_CARRY_STATES; ++k) {
+        if (k >= tab.n) break;
+        const slk_carry_state& st = tab.s[k];
         if (st.kind == SLK_STATE_F32) {
-            const bool vec = i + 4 <= total && (reinterpret_cast<uintptr_t>(st.dst) & 15) == 0;
-            store_some<F32>(st.dst, i, total, vec, v);
+            const bool vec =
+                total - first >= mine + 4 && (reinterpret_cast<uintptr_t>(st.dst) & 15) == 0;
+            store_some<F32>(st.dst, at, total, vec, v[k]);
         } else {
-            const bool vec = i + 4 <= total && (reinterpret_cast<uintptr_t>(st.dst) & 3) == 0;
-            const float scale = q8_block_max(v);
-            if (st.kind == SLK_STATE_Q8_SIGNED) encode4<true>(st.dst, i, total, vec, scale, v);
-            else encode4<false>(st.dst, i, total, vec, scale, v);
+            const bool vec =
+                total - first >= mine + 4 && (reinterpret_cast<uintptr_t>(st.dst) & 3) == 0;
+            const float scale = q8_block_max(v[k]);
+            if (st.kind == SLK_STATE_Q8_SIGNED) encode4<true>(st.dst, at, total, vec, scale, v[k]);
+            else encode4<false>(st.dst, at, total, vec, scale, v[k]);
             if (lane == 0) st.dst_scale[block] = scale;
         }
     }
@@ -415,7 +538,7 @@ extern "C" int slk_carry_slots(const int32_t* row_start, int64_t nrows, int64_t 
                                void* stream) {
     using namespace slk;
     clear_error();
-    if (nrows < 0 || total < 0 || total > INT32_MAX) {
+    if (nrows < 0 || total < 0 || total > INT32_MAX || nrows > INT32_MAX) {
         return fail(SLK_EINVAL, "carry_slots: negative size, or slots beyond the int32 range");
     }
     if (n_states < 0 || n_states > SLK_CARRY_STATES || (n_states > 0 && states_host == nullptr)) {
@@ -446,7 +569,8 @@ extern "C" int slk_carry_slots(const int32_t* row_start, int64_t nrows, int64_t 
         tab.s[k] = s;
     }
     hipLaunchKernelGGL(carry_kernel, dim3(static_cast<unsigned>(ceil_div(total, kAdamSpan))),
-                       dim3(kAdamThreads), 0, as_stream(stream), row_start, nrows, total, old_cols,
+                       dim3(kAdamThreads), 0, as_stream(stream), row_start, static_cast<int>(nrows),
+                       static_cast<int>(total), old_cols,
                        old_nnz, new_cols, new_nnz, tab);
     return check_launch("carry_slots");
 }

@@ -757,9 +757,9 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
             }
         };
         int64_t k = 0;
-        for (; k + 4 * kRun <= d; k += 4 * kRun) {
+        for (; k + 8 * kRun <= d; k += 8 * kRun) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) step(k + u * kRun, acc[u & 1]);
+            for (int u = 0; u < 8; ++u) step(k + u * kRun, acc[u & 1]);
         }
         for (; k < d; k += kRun) step(k, acc[0]);
         // lane l, register r: row 4 (l / 16) + r of the block, token l % 16

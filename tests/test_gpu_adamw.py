@@ -445,3 +445,40 @@ def test_refusals(dev):
         optim.carry_slots(start, (cols, nnz), (cols, nnz), [m[0]] * 5)
     with pytest.raises(RuntimeError, match="HIP"):
         optim.carry_slots(start, (cols.cpu(), nnz), (cols, nnz), [m[0]])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_carried_states_of_long_rows_that_shift_far(dev, seed):
+    """Rows far longer than the slots around a place that the kernel looks at first:
+    columns that stay, shift by a few slots, by hundreds (a block of columns dropped at
+    one end and grown at the other) or by the whole row; rows of one slot between them."""
+    rng = np.random.default_rng(seed)
+    cols = 6000
+    rows_old, rows_new, cap = [], [], []
+    for _ in range(40):
+        n = int(rng.choice([1, 3, 700, 2500, 5000]))
+        a = np.sort(rng.choice(cols, n, replace=False))
+        how = rng.integers(0, 4)
+        keep = a[rng.random(n) > 0.3] if how == 0 else a[n // 3:] if how == 1 \
+            else a[: n - n // 3] if how == 2 else a[:0]
+        free = np.setdiff1d(np.arange(cols), a)
+        grow = rng.choice(free, min(n - keep.size, free.size), replace=False)
+        if how == 1:
+            grow = np.sort(free)[-(n - keep.size):] if n > keep.size else free[:0]
+        elif how == 2:
+            grow = np.sort(free)[: n - keep.size]
+        b = np.sort(np.concatenate([keep, grow]))
+        rows_old.append(a), rows_new.append(b), cap.append(max(n, b.size) + int(rng.integers(1, 9)))
+    start = np.concatenate([[0], np.cumsum(cap)[:-1]]).astype(np.int32)
+    total = int(np.sum(cap))
+    out = []
+    for rows in (rows_old, rows_new):
+        at, nnz = np.full(total, -1, np.int32), np.array([r.size for r in rows], np.int32)
+        for s, r in zip(start, rows):
+            at[s:s + r.size] = r
+        out.append((at, nnz))
+    old, new = out
+    m = rng.standard_normal(total).astype(np.float32)
+    t = [torch.from_numpy(x).to(dev) for x in (start, *old, *new, m)]
+    got, = optim.carry_slots(t[0], (t[1], t[2]), (t[3], t[4]), [t[5]])
+    assert np.array_equal(got.cpu().numpy(), moved(start, old, new, m))
