@@ -527,8 +527,8 @@ struct TokenEpi {
 
 // ───────────────────────────── joining ─────────────────────────────
 
-// lse and loss of each token from its partial maxima and sums: eight tokens a
-// workgroup, 32 threads a token.
+// lse and loss of each token from its partial maxima and sums: TOK tokens a
+// workgroup, 256 / TOK threads a token.
 struct JoinArgs {
     const float2* part;
     const float* zt;
@@ -539,10 +539,11 @@ struct JoinArgs {
     float* losses;
     int64_t n, v, ignore, parts;
 };
+template <int TOK>
 __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
-    __shared__ float2 sh[4][8];
-    const int j = threadIdx.x & 7, part = threadIdx.x >> 3;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + j;
+    __shared__ float2 sh[4][TOK];
+    const int j = threadIdx.x % TOK, part = threadIdx.x / TOK;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * TOK + j;
     int64_t i = -1;
     bool valid = false;
     if (n < p.n) {
@@ -556,18 +557,18 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
     }
     float m = -INFINITY, s = 0.0f;
     if (i >= 0) {
-        for (int64_t k = part; k < p.parts; k += 32) {
+        for (int64_t k = part; k < p.parts; k += 256 / TOK) {
             const float2 x = p.part[k * p.n + i];
             join(m, s, x.x, x.y);
         }
     }
-    // lanes 8 apart hold a token's parts: within the wave, then over the four waves
+    // lanes TOK apart hold a token's parts: within the wave, then over the four waves
 #pragma unroll
-    for (int o = 8; o < kWave; o <<= 1) {
+    for (int o = TOK; o < kWave; o <<= 1) {
         const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
         join(m, s, m2, s2);
     }
-    if ((threadIdx.x & (kWave - 1)) < 8) sh[threadIdx.x >> 6][j] = make_float2(m, s);
+    if ((threadIdx.x & (kWave - 1)) < TOK) sh[threadIdx.x >> 6][j] = make_float2(m, s);
     __syncthreads();
     if (part != 0 || n >= p.n) return;
 #pragma unroll
@@ -898,11 +899,29 @@ Backward backward_of(const slk_linear_ce* a) {
     // (the epilogue writes whole tiles of tokens)
     const int64_t n_up = ceil_div(a->n, kWideN) * kWideN;
     const int64_t per_row = n_up * (split_of(a) ? 8 : 4);
-    int64_t rows = kDlBytes / per_row / kTileM * kTileM;
-    if (rows < kTileM) rows = kTileM;
+    int64_t most = kDlBytes / per_row / kTileM * kTileM;  // rows of a piece
+    if (most < kTileM) most = kTileM;
     const int64_t all = ceil_div(a->v, kTileM) * kTileM;
-    const int64_t pieces = ceil_div(all, rows < all ? rows : all);
-    b.piece = ceil_div(ceil_div(all, pieces), kTileM) * kTileM;
+    if (most > all) most = all;
+    // as few pieces as fit, or a few more where their tiles fill the last round of
+    // the 256 CUs better: stages of a tile times rounds, and dh read and written
+    // once a piece (about 130 stages' time at 8192 x 4096)
+    double cost = 1e30;
+    for (int64_t k = ceil_div(all, most); k < ceil_div(all, most) + 4; ++k) {
+        const int64_t rows = ceil_div(ceil_div(all, k), kTileM) * kTileM;
+        double c = 0.0;
+        for (int64_t v0 = 0; v0 < a->v; v0 += rows) {
+            const int64_t vn = a->v - v0 < rows ? a->v - v0 : rows;
+            c += mma_rounds(vn, a->n) * static_cast<double>(stages(a, a->d)) +
+                 mma_rounds(vn, a->d) * static_cast<double>(stages(a, a->n)) +
+                 mma_rounds(a->n, a->d) * static_cast<double>(stages(a, vn)) + 20.0 +
+                 static_cast<double>(a->n) * static_cast<double>(a->d) * 4e-6;
+        }
+        if (c < cost) {
+            cost = c;
+            b.piece = rows;
+        }
+    }
     b.sh = splits_for(a->n, a->d, stages(a, b.piece));
     b.sw = splits_for(b.piece, a->d, stages(a, a->n));
     Carve c;
@@ -1002,8 +1021,13 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
         j.lse = reinterpret_cast<float*>(sv + s.lse);
     }
     if (rc != SLK_OK) return rc;
-    hipLaunchKernelGGL(ce_join_kernel, dim3(static_cast<unsigned>(ceil_div(a->n, 8))), dim3(256),
-                       0, st, j);
+    if (few(a)) {
+        hipLaunchKernelGGL(ce_join_kernel<1>, dim3(static_cast<unsigned>(a->n)), dim3(256), 0, st,
+                           j);
+    } else {
+        hipLaunchKernelGGL(ce_join_kernel<8>, dim3(static_cast<unsigned>(ceil_div(a->n, 8))),
+                           dim3(256), 0, st, j);
+    }
     if ((rc = check_launch("linear_ce join")) != SLK_OK) return rc;
     if (a->reduction != SLK_REDUCE_NONE) {
         hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, losses, a->target, a->n,

@@ -436,6 +436,13 @@ inline bool mma_wide(int64_t M, int64_t N, int splits) {
     return 17 * wide <= 10 * small;
 }
 
+// Rounds of 256 workgroups that a product takes, in small tiles' time.
+inline double mma_rounds(int64_t M, int64_t N) {
+    const bool wide = mma_wide(M, N, 1);
+    const int64_t tiles = ceil_div(M, kTileM) * ceil_div(N, wide ? kWideN : kTileN);
+    return static_cast<double>(ceil_div(tiles, 256)) * (wide ? 1.7 : 1.0);
+}
+
 template <bool SPLIT, class Epi>
 int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
     const bool wide = mma_wide(g.M, g.N, g.splits);
