@@ -7,6 +7,13 @@ A GPU drop-in for the hot path of SparseLab (DarshanFofadiya/sparsecore):
     SparseLinear   nn.Linear replacement backed by PaddedCSR   (sparselab.SparseLinear)
     Static/SET/RigL  sparsity policies, updates on the device  (sparselab.router)
 
+and, for the training step around the sparse layers (no counterpart there):
+
+    linear_cross_entropy   head and loss without storing the logits
+    residual_norm, ResidualNorm   residual sum, gate and the norms around a block
+    AdamW, optim     the whole model's step in a launch or two, 32- or 8-bit moments
+                     that follow their weights through SET / RigL rewrites
+
 The kernels (forward SpMM, live-slot dW, device transpose and cache refresh,
 invariant scan) are hand-written HIP for gfx950 in ``csrc/``, built into
 ``_lib/libsparsecore_amd.so`` and reached through the C-ABI declared in
@@ -21,13 +28,13 @@ from .ops import spmm
 from .nn import SparseLinear
 from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Static
 from .loss import linear_cross_entropy
-from .norm import residual_norm
+from .norm import ResidualNorm, residual_norm
 from .optim import AdamW
 from . import _lib, nn, ops, optim, router
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
            "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
-           "residual_norm", "linear_cross_entropy", "install_as_sparselab"]
+           "residual_norm", "ResidualNorm", "linear_cross_entropy", "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

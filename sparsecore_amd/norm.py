@@ -15,10 +15,11 @@ so that a block's norm, sparse layers and residual need no transposing copies.
 from __future__ import annotations
 
 import torch
+from torch import nn
 
 from . import _lib
 
-__all__ = ["residual_norm"]
+__all__ = ["residual_norm", "ResidualNorm"]
 
 _KINDS = {"layer": 1, "rms": 0}
 
@@ -245,3 +246,51 @@ def residual_norm(x, weight, bias=None, *, branch=None, gate=None, post_weight=N
     out = _ResidualNorm.apply(x, weight, bias, branch, gate, post_weight, post_bias,
                               float(scale), _KINDS[kind], float(eps), bool(feature_major))
     return out if branch is not None else (x, out)
+
+
+class ResidualNorm(nn.Module):
+    """The residual sum of a block and the norm before the next one, with its parameters.
+
+    ``r, y = norm(x, branch)``: r = x + scale · gate ∘ post(branch), y = pre(r); with no
+    branch yet, ``r`` is ``x``.
+
+    Args:
+        d: features.
+        kind: "layer" or "rms".
+        post: norm the branch too, with a weight (and bias) of its own.
+        gate: learn a gate of each feature, initialised to this value (None: none).
+        scale: constant factor of the branch.
+        bias: biases of a LayerNorm.
+        feature_major: write y as a SparseLinear takes it without a copy.
+    """
+
+    def __init__(self, d: int, kind: str = "layer", *, post: bool = False,
+                 gate: float | None = None, scale: float = 1.0, eps: float = 1e-5,
+                 bias: bool = True, feature_major: bool = True, device=None, dtype=None):
+        super().__init__()
+        if kind not in _KINDS:
+            raise ValueError(f"ResidualNorm: kind must be 'layer' or 'rms', got {kind!r}")
+        self.d, self.kind, self.scale, self.eps = d, kind, scale, eps
+        self.feature_major = feature_major
+        make = dict(device=device, dtype=dtype)
+        bias = bias and kind == "layer"
+
+        def vector(value, wanted):
+            return nn.Parameter(torch.full((d,), float(value), **make)) if wanted else None
+
+        self.weight, self.bias = vector(1.0, True), vector(0.0, bias)
+        self.post_weight, self.post_bias = vector(1.0, post), vector(0.0, post and bias)
+        self.gate = vector(0.0 if gate is None else gate, gate is not None)
+
+    def forward(self, x, branch=None):
+        if branch is None:
+            return residual_norm(x, self.weight, self.bias, kind=self.kind, eps=self.eps,
+                                 feature_major=self.feature_major)
+        return residual_norm(x, self.weight, self.bias, branch=branch, gate=self.gate,
+                             post_weight=self.post_weight, post_bias=self.post_bias,
+                             scale=self.scale, kind=self.kind, eps=self.eps,
+                             feature_major=self.feature_major)
+
+    def extra_repr(self) -> str:
+        return (f"{self.d}, kind={self.kind!r}, post={self.post_weight is not None}, "
+                f"gate={self.gate is not None}, scale={self.scale}")
