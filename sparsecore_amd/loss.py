@@ -9,6 +9,7 @@ computes the logits again a piece of the vocabulary at a time (``slk_linear_ce_*
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -17,12 +18,12 @@ __all__ = ["linear_cross_entropy"]
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, target, ignore_index, reduction):
+    def forward(ctx, hidden, weight, target, ignore_index, reduction, grad):
         d, v = weight.shape[1], weight.shape[0]
         n = target.numel()
         dev = hidden.device
         h, w, t = (x if x.is_contiguous() else x.contiguous() for x in (hidden, weight, target))
-        keep = any(ctx.needs_input_grad)
+        keep = grad and any(ctx.needs_input_grad)
         loss = torch.empty(target.shape if reduction == "none" else (), device=dev)
         p = _lib.ptr
         args = _lib.LinearCE(n=n, d=d, v=v, ignore_index=ignore_index, hidden=p(h), weight=p(w),
@@ -46,6 +47,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         saved, = ctx.saved_tensors
         n, d, v, ignore_index, reduction, shape, dtype = ctx.rest
@@ -66,7 +68,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             args.scratch = p(scratch)
             with _lib.on_device(up):
                 _lib.linear_ce_backward(args, _lib.stream_of(up))
-        return dh, dw, None, None, None
+        return dh, dw, None, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
@@ -116,4 +118,5 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
                          f"bfloat16, got {hidden.dtype} and {weight.dtype}")
     if target.dtype != torch.int64:
         raise ValueError(f"linear_cross_entropy: target must be int64, got {target.dtype}")
-    return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), reduction)
+    return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), reduction,
+                                     torch.is_grad_enabled())

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -77,7 +78,7 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, branch, gate, post_weight, post_bias, scale, layer, eps,
-                feature_major):
+                feature_major, grad):
         # Small calls are bound by this host work: as few tensor operations as possible.
         shape, dt, dev = x.shape, x.dtype, x.device
         d = shape[-1]
@@ -96,7 +97,7 @@ class _ResidualNorm(torch.autograd.Function):
             y = torch.empty(shape, dtype=dt, device=dev)
         r = torch.empty(shape, dtype=dt, device=dev) if u is not None else x
         need = ctx.needs_input_grad
-        stats = torch.empty((n, 4), device=dev) if any(need) else None
+        stats = torch.empty((n, 4), device=dev) if grad and any(need) else None
         if n:
             p = _lib.ptr
             args = _lib.Norm(n=n, d=d, gate_rows=rows, x=p(x), branch=p(u), gate=p(gate),
@@ -122,6 +123,7 @@ class _ResidualNorm(torch.autograd.Function):
         return (r, y) if branch is not None else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         r, stats, weight, bias, u, gate, post_weight, post_bias = ctx.saved_tensors
         shape, n, d, rows, scale, layer, eps, u_cols, back_cols, has_branch = ctx.rest
@@ -175,7 +177,7 @@ class _ResidualNorm(torch.autograd.Function):
                 _lib.norm_backward(args, _lib.stream_of(r))
             if du is not None and back_cols:
                 du = _as_cols(du.reshape(n, d)).reshape(shape)
-        return (dx, sums[0], sums[1], du, dgate, sums[2], sums[3], None, None, None, None)
+        return (dx, sums[0], sums[1], du, dgate, sums[2], sums[3], None, None, None, None, None)
 
 
 def residual_norm(x, weight, bias=None, *, branch=None, gate=None, post_weight=None,
@@ -244,7 +246,8 @@ def residual_norm(x, weight, bias=None, *, branch=None, gate=None, post_weight=N
     if gate is not None:
         _gate_rows(gate, x, x.numel() // d, d)
     out = _ResidualNorm.apply(x, weight, bias, branch, gate, post_weight, post_bias,
-                              float(scale), _KINDS[kind], float(eps), bool(feature_major))
+                              float(scale), _KINDS[kind], float(eps), bool(feature_major),
+                              torch.is_grad_enabled())
     return out if branch is not None else (x, out)
 
 

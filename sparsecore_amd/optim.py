@@ -335,6 +335,11 @@ class AdamW(torch.optim.Optimizer):
         if s:
             names = [k for k in ("exp_avg", "exp_avg_sq") if k in s]
             states = [(s[k], s[k + "_scale"]) if k + "_scale" in s else s[k] for k in names]
+            # what is replaced below may have been made on another stream than this one
+            now = torch.cuda.current_stream(p.device)
+            for k, t in [*s.items(), ("cols", at.cols), ("nnz", at.nnz)]:
+                if isinstance(t, torch.Tensor) and k != "step":
+                    t.record_stream(now)
             for k, got in zip(names, carry_slots(csr.row_start, (at.cols, at.nnz),
                                                  (csr.col_indices, csr.row_nnz), states)):
                 if isinstance(got, tuple):

@@ -304,3 +304,100 @@ def test_refusals(dev):
     for bad in ((h[:, :7], w, t), (h, w, t[:3]), (h, w[0], t), (h[0], w, t)):
         with pytest.raises(ValueError):
             f(*bad)
+
+
+def test_scores_without_gradients_keep_nothing(dev, monkeypatch):
+    """Under no_grad the head's own requires_grad must not cost the packed operands."""
+    from sparsecore_amd import _lib
+
+    h, w, t = make(8, 64, 300, torch.float32, dev, 11)
+    w.requires_grad_()
+    seen = []
+    real = _lib.linear_ce_forward
+    monkeypatch.setattr(_lib, "linear_ce_forward", lambda a, s: (seen.append(a.keep), real(a, s)))
+    with torch.no_grad():
+        slk.linear_cross_entropy(h, w, t)
+    slk.linear_cross_entropy(h, w, t)
+    assert seen == [0, 1]
+
+
+def test_double_backward_is_refused(dev):
+    h, w, t = make(8, 64, 300, torch.float32, dev, 12)
+    h.requires_grad_()
+    up = torch.ones((), device=dev, requires_grad=True)
+    g, = torch.autograd.grad(slk.linear_cross_entropy(h, w, t), h, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (5, 33, 70), (300, 130, 517), (16, 50, 300)])
+@pytest.mark.parametrize("keep", [0, 1])
+def test_writes_stay_in_range(dev, dtype, n, d, v, keep):
+    """Through the C-ABI with guard bytes around every array that it may write."""
+    from sparsecore_amd import _lib
+
+    h, w, t = make(n, d, v, dtype, dev, 13, 0.3)
+    size = h.element_size()
+    args = _lib.LinearCE(n=n, d=d, v=v, ignore_index=-100, hidden=h.data_ptr(),
+                         weight=w.data_ptr(), target=t.data_ptr(), dtype=_lib.DTYPES[dtype],
+                         reduction=0, keep=keep)
+    up = torch.ones(n, device=dev)
+
+    def guarded(nbytes):
+        buf = torch.full((nbytes + 1024,), 0xA5, dtype=torch.uint8, device=dev)
+        return buf, buf.data_ptr() + 512
+
+    def intact(buf):
+        return bool((buf[:512] == 0xA5).all()) and bool((buf[-512:] == 0xA5).all())
+
+    def up256(x):  # addresses of the workspaces keep torch's alignment
+        return (x + 255) // 256 * 256
+
+    loss, args.loss = guarded(4 * n)
+    args.saved_bytes = _lib.linear_ce_saved_bytes(args)
+    args.scratch_bytes = _lib.linear_ce_scratch_bytes(args, False)
+    saved, args.saved = guarded(up256(args.saved_bytes))
+    scratch, args.scratch = guarded(up256(args.scratch_bytes))
+    _lib.linear_ce_forward(args, _lib.stream_of(h))
+    torch.cuda.synchronize()
+    assert intact(loss) and intact(saved) and intact(scratch)
+    if not keep:
+        return
+    dh, args.dhidden = guarded(size * n * d)
+    dw, args.dweight = guarded(size * v * d)
+    args.upstream = up.data_ptr()
+    args.scratch_bytes = _lib.linear_ce_scratch_bytes(args, True)
+    scratch, args.scratch = guarded(up256(args.scratch_bytes))
+    _lib.linear_ce_backward(args, _lib.stream_of(h))
+    torch.cuda.synchronize()
+    assert all(intact(b) for b in (dh, dw, saved, scratch))
+
+
+def test_captured_loss_and_gradients_replay(dev):
+    h, w, t = make(300, 64, 500, torch.float32, dev, 14, 0.2)
+    h.requires_grad_(), w.requires_grad_()
+
+    def once():
+        loss = slk.linear_cross_entropy(h, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, w]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        got = once()
+    from sparsecore_amd import _lib
+
+    assert "memset" not in _lib.graph_node_types(graph)
+    graph.instantiate()
+    for k in range(4):
+        with torch.no_grad():
+            h.copy_(torch.randn(300, 64, generator=torch.Generator().manual_seed(k)))
+            t.copy_(torch.where(torch.rand(300, generator=torch.Generator().manual_seed(k)) < 0.1 * k,
+                                -100, torch.randint(0, 500, (300,))))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, once()))

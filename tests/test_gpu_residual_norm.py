@@ -373,3 +373,79 @@ def test_refusals(dev):
     two = x.reshape(24, 32)
     with pytest.raises(ValueError, match="gate"):
         f(two, w, branch=two, gate=two[:5])
+
+
+def test_double_backward_is_refused(dev):
+    t, _, _ = make((4,), 64, "layer", False, "none", torch.float32, dev)
+    x = t["x"].requires_grad_()
+    up = torch.ones(4, 64, device=dev, requires_grad=True)
+    g, = torch.autograd.grad(slk.residual_norm(x, t["weight"], t["bias"])[1], x, up,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,gate_rows,cols", [(1, 1, 1, 0), (7, 100, 7, 0), (9, 1027, 3, 0),
+                                                (50, 300, 2, 1), (33, 1024, 1, 1), (6, 9000, 2, 0),
+                                                (600, 64, 30, 1), (5000, 68, 5, 0)])
+def test_writes_stay_in_range(dev, dtype, n, d, gate_rows, cols):
+    """Through the C-ABI with guard bytes around every array that it may write."""
+    g = torch.Generator().manual_seed(0)
+    size = torch.empty(0, dtype=dtype).element_size()
+
+    def rand(*s):
+        return torch.randn(*s, generator=g).to(dtype).to(dev)
+
+    guards = []
+
+    def out(nbytes):
+        buf = torch.full((nbytes + 1024,), 0xA5, dtype=torch.uint8, device=dev)
+        guards.append(buf)
+        return buf.data_ptr() + 512
+
+    keep = {k: rand(n, d) for k in ("x", "branch", "dr", "dy")}
+    keep |= {k: rand(d) for k in ("weight", "bias", "post_weight", "post_bias")}
+    keep["gate"] = rand(gate_rows, d)
+    args = _lib.Norm(n=n, d=d, gate_rows=gate_rows, scale=0.5, eps=1e-5,
+                     dtype=_lib.DTYPES[dtype], layer=1, branch_cols=cols, y_cols=cols,
+                     **{k: v.data_ptr() for k, v in keep.items()})
+    args.r, args.y, args.stats = out(size * n * d), out(size * n * d), out(16 * n)
+    _lib.norm_forward(args, _lib.stream_of(keep["x"]))
+    args.dx, args.dbranch = out(size * n * d), out(size * n * d)
+    args.dgate = out(size * gate_rows * d)
+    for k in ("dweight", "dbias", "dpost_weight", "dpost_bias"):
+        setattr(args, k, out(size * d))
+    args.workspace_bytes = _lib.norm_workspace_bytes(args)
+    args.workspace = out(args.workspace_bytes)
+    _lib.norm_backward(args, _lib.stream_of(keep["x"]))
+    torch.cuda.synchronize()
+    for b in guards:
+        assert bool((b[:512] == 0xA5).all()) and bool((b[-512:] == 0xA5).all())
+
+
+def test_captured_norm_replays(dev):
+    t, dr, dy = make((2, 100), 96, "layer", True, "sequence", torch.float32, dev)
+    for v in t.values():
+        v.requires_grad_()
+    args = {k: v for k, v in t.items() if k not in ("x", "weight", "bias")}
+
+    def once():
+        r, y = slk.residual_norm(t["x"], t["weight"], t["bias"], **args)
+        return (r.detach(), y.detach(), *torch.autograd.grad([r, y], list(t.values()), [dr, dy]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        got = once()
+    assert "memset" not in _lib.graph_node_types(graph)
+    graph.instantiate()
+    for k in range(4):
+        with torch.no_grad():
+            t["x"].copy_(torch.randn(2, 100, 96, generator=torch.Generator().manual_seed(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, once()))
