@@ -267,8 +267,12 @@ __device__ __forceinline__ float logit_scale(const Header* hd) {
 }
 
 // Logits are exponentiated in base 2: the factor log2(e) goes into the scale of
-// the accumulator, and v_exp_f32 is one instruction (1 ulp). Maxima and sums
-// travel in base 2 too (m, Σ 2^(z·log2 e - m)).
+// the accumulator, and v_exp_f32 is one instruction (1 ulp). Maxima, sums and
+// targets' logits travel in base 2 too (m, s = Σ 2^(z·log2 e - m)). A token keeps
+// m and 1/s rather than the logarithm of its sum: 2^(z' - m) / s is then as exact
+// as the difference, where a rounded logarithm near 20 would put 1e-6 into every
+// entry of the token's softmax; and m - z' of a token whose target has the
+// largest logit is 0 exactly.
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -293,7 +297,7 @@ struct ScoreEpi {
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         __syncthreads();  // the ring is free
         float2* sh = reinterpret_cast<float2*>(t.lds);  // kWavesM x kBN
-        const float scale = logit_scale<SPLIT>(hd), scale2 = scale * kLog2e;
+        const float scale2 = logit_scale<SPLIT>(hd) * kLog2e;
         const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -305,7 +309,7 @@ struct ScoreEpi {
                 for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (t.row(a, r) == want) zt[tok] = acc[a][b][r] * scale;
+                        if (t.row(a, r) == want) zt[tok] = acc[a][b][r] * scale2;
             }
             float m = -INFINITY, s = 0.0f;
             if (rows < 32 * Tile::kNA) {  // past the vocabulary
@@ -352,7 +356,7 @@ template <bool SPLIT>
 struct DlEpi {
     const Header* hd;
     const int32_t* tgt;
-    const float* lse;
+    const float2* norm;  // (m, 1 / s) of each token
     const float* gr;  // upstream gradient of each token over the largest, NULL: all 1
     char* by_tok;
     char* by_voc;
@@ -373,15 +377,16 @@ struct DlEpi {
             const int64_t want = (in ? tgt[tok] - v0 : -1) - t.m0();
             const bool here = want >= 0 && want < 32 * Tile::kNA;
             const bool any = __any(here);
-            const float l = in ? lse[tok] * kLog2e : 0.0f;
+            const float2 ms = in ? norm[tok] : make_float2(0.0f, 0.0f);
             const float g = (in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f) * up;
+            const float gs = g * ms.y;
 #pragma unroll
             for (int a = 0; a < Tile::kNA; ++a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float p = exp2_(fmaf(acc[a][b][r], scale2, -l));
-                    if (any && t.row(a, r) == want) p -= 1.0f;
-                    acc[a][b][r] = in && t.row(a, r) < rows ? p * g : 0.0f;
+                    float p = exp2_(fmaf(acc[a][b][r], scale2, -ms.x)) * gs;
+                    if (any && t.row(a, r) == want) p -= g;
+                    acc[a][b][r] = in && t.row(a, r) < rows ? p : 0.0f;
                 }
                 const int64_t v = t.m0() + 32 * a;          // this block's 32 rows
                 const int64_t k = t.n0() + 32 * b;          // and 32 tokens
@@ -527,7 +532,7 @@ struct TokenEpi {
 
 // ───────────────────────────── joining ─────────────────────────────
 
-// lse and loss of each token from its partial maxima and sums: TOK tokens a
+// Maximum, sum and loss of each token from its partial maxima and sums: TOK tokens a
 // workgroup, 256 / TOK threads a token.
 struct JoinArgs {
     const float2* part;
@@ -535,7 +540,7 @@ struct JoinArgs {
     const int64_t* target;
     const int32_t* pos;  // place of each token in part, NULL: its own
     const int32_t* tgt;  // target of each place, -1: none (with pos)
-    float* lse;          // NULL: not wanted
+    float2* norm;        // (m, 1 / s) of each place, NULL: not wanted
     float* losses;
     int64_t n, v, ignore, parts;
 };
@@ -577,9 +582,9 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
         p.losses[n] = 0.0f;
         return;
     }
-    const float lse = ((m == -INFINITY ? 0.0f : m) + log2f(s)) * kLn2;
-    if (p.lse != nullptr) p.lse[i] = lse;
-    p.losses[n] = valid ? lse - p.zt[i] : NAN;
+    if (m == -INFINITY) m = 0.0f;
+    if (p.norm != nullptr) p.norm[i] = make_float2(m, 1.0f / s);
+    p.losses[n] = valid ? ((m - p.zt[i]) + log2f(s)) * kLn2 : NAN;
 }
 
 // The sum or mean of the losses over the live tokens: one workgroup, sums in
@@ -768,9 +773,9 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t vr = blk * 16 + 4 * quarter + r;
-            z[r] = acc[0][r] + acc[1][r];
+            z[r] = (acc[0][r] + acc[1][r]) * kLog2e;
             if (vr == want && col < n) zt[col] = z[r];
-            z[r] = vr >= v ? -INFINITY : z[r] * kLog2e;
+            if (vr >= v) z[r] = -INFINITY;
             top = fmaxf(top, z[r]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
@@ -813,7 +818,7 @@ struct Carve {
 };
 
 struct Saved {
-    int64_t header, rows, pos, tgt, lse, h_row, w_row, h_col, w_col, bytes;
+    int64_t header, rows, pos, tgt, norm, h_row, w_row, h_col, w_col, bytes;
 };
 
 bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
@@ -828,7 +833,7 @@ Saved saved_of(const slk_linear_ce* a) {
     s.rows = c.take(4 * a->n);
     s.pos = c.take(4 * a->n);
     s.tgt = c.take(4 * a->n);
-    s.lse = c.take(4 * a->n);
+    s.norm = c.take(8 * a->n);
     s.h_row = c.take(stages(a, a->d) * a->n * kStageBytes);
     s.w_row = c.take(stages(a, a->d) * a->v * kStageBytes);
     s.h_col = s.w_col = 0;
@@ -1018,7 +1023,7 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
         rc = mma<SPLIT>(g, ScoreEpi<SPLIT>{hd, tgt, part, zt, a->n}, st, "linear_ce logits");
         j.pos = pos;
         j.tgt = tgt;
-        j.lse = reinterpret_cast<float*>(sv + s.lse);
+        j.norm = reinterpret_cast<float2*>(sv + s.norm);
     }
     if (rc != SLK_OK) return rc;
     if (few(a)) {
@@ -1047,7 +1052,7 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     const int32_t* rows = reinterpret_cast<const int32_t*>(sv + s.rows);
     const int32_t* pos = reinterpret_cast<const int32_t*>(sv + s.pos);
     const int32_t* tgt = reinterpret_cast<const int32_t*>(sv + s.tgt);
-    const float* lse = reinterpret_cast<const float*>(sv + s.lse);
+    const float2* norm = reinterpret_cast<const float2*>(sv + s.norm);
     float* factor = reinterpret_cast<float*>(sc + b.factor);
     float* gr = reinterpret_cast<float*>(sc + b.gr);
     const bool whole = b.sh == 1 && b.piece >= a->v;  // a tile of dh has its whole sum
@@ -1073,7 +1078,7 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
         const int64_t vn = a->v - v0 < b.piece ? a->v - v0 : b.piece;
         const MmaArgs gl{sv + s.w_row + v0 * kStageBytes, sv + s.h_row, vn, a->n,
                          stages(a, a->d), a->v, a->n, &hd->live, kLiveN, 1};
-        const DlEpi<SPLIT> el{hd, tgt, lse, a->reduction == SLK_REDUCE_NONE ? gr : nullptr,
+        const DlEpi<SPLIT> el{hd, tgt, norm, a->reduction == SLK_REDUCE_NONE ? gr : nullptr,
                               sc + b.by_tok, sc + b.by_voc, v0, a->n, b.piece};
         if ((rc = mma<SPLIT>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
         if (a->dhidden != nullptr) {
