@@ -4,9 +4,8 @@
 // Logits exist only as 256 x 128 tiles in registers. Forward: each tile leaves
 // its tokens' running maximum and sum, which a second kernel joins. Backward: a
 // piece of the vocabulary at a time, the tiles are computed again, turned into
-// dl in the epilogue and written as operands of the two gradient products (as
-// rows of tokens and as rows of the vocabulary); the piece's two products
-// follow. 2·n·v·d operations forward, 6 backward, where keeping the logits
+// dl in the epilogue and written as the operand of the piece's two gradient
+// products, which follow. 2·n·v·d operations forward, 6 backward, where keeping the logits
 // would take 4 backward and 4 bytes a logit.
 //
 // Tokens whose target is ignore_index are left out before anything is computed
@@ -197,64 +196,63 @@ struct PackArgs {
     const Header* hd;     // largest magnitudes (float32 sources)
     bool of_w;
     int64_t R, d;
-    char* by_row;  // rows of R rows, stages along d; NULL: not wanted
-    char* by_col;  // rows of d rows, stages along the R rows; NULL: not wanted
+    int64_t out_rows;  // rows that the packed form is laid out for
+    char* out;
 };
 
-// A 64 x 64 piece of the source through LDS into both packed forms.
-template <class T, bool SPLIT>
+// Eight elements a thread: consecutive threads take a stage of a row, then its
+// next rows. The rows up to the next multiple of 64 are zero.
+template <class T, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
-    __shared__ float tile[64][65];
+    constexpr int K = kStageK<SPLIT>, kParts = K / 8;
     const int64_t R = p.live != nullptr ? *p.live : p.R;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
-    const int64_t c0 = static_cast<int64_t>(blockIdx.y) * 64;
-    if (r0 >= R) return;
-    const int c = threadIdx.x & 63;
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const int64_t r = r0 + (threadIdx.x >> 6) + 4 * j;
-        const bool in = r < R && c0 + c < p.d;
-        const int64_t s = in ? (p.rows != nullptr ? p.rows[r] : r) : 0;
-        v[j] = in ? T::load(p.src, s * p.d + c0 + c) : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) tile[(threadIdx.x >> 6) + 4 * j][c] = v[j];
-    __syncthreads();
+    const int64_t rows = ceil_div(R, 64) * 64;
     const float scale =
         SPLIT ? pow2(p.of_w ? scale_exp<&Top::w>(p.hd) : scale_exp<&Top::h>(p.hd)) : 1.0f;
-    constexpr int K = kStageK<SPLIT>;
-    const int64_t stages = ceil_div(p.d, K);
-    auto put = [&](char* row, int k, const float (&x)[8]) {  // elements k .. k + 7 of a stage
+    // four rows a thread, their loads in flight together
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int part = static_cast<int>(t % kParts);
+    const int64_t st = blockIdx.y;
+    const int64_t r0 = t / kParts, step = (rows + 3) / 4;
+    if (r0 >= step) return;
+    const int64_t e = st * K + 8 * part;
+    float x[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t r = r0 + j * step;
+        const bool in = r < R;
+        const int64_t off = in ? (p.rows != nullptr ? p.rows[r] : r) * p.d + e : 0;
+        if (VEC) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                if (in && e + k < p.d) {
+                    T::load4(p.src, off + k, &x[j][k]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[j][k + i] = 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                x[j][k] = in && e + k < p.d ? T::load(p.src, off + k) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t r = r0 + j * step;
+        if (r >= rows) break;
+        char* to = p.out + (st * p.out_rows + r) * kStageBytes + 16 * part;
         if constexpr (SPLIT) {
             f16x8 hi, lo;
-            split8(x, scale, hi, lo);
-            *reinterpret_cast<f16x8*>(row + 2 * k) = hi;
-            *reinterpret_cast<f16x8*>(row + 64 + 2 * k) = lo;
+            split8(x[j], scale, hi, lo);
+            *reinterpret_cast<f16x8*>(to) = hi;
+            *reinterpret_cast<f16x8*>(to + 64) = lo;
         } else {
             b16x8 b;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = static_cast<__bf16>(x[j]);
-            *reinterpret_cast<b16x8*>(row + 2 * k) = b;
-        }
-    };
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int at = threadIdx.x + 256 * q;
-        const int line = at >> 3, k = (at & 7) * 8;  // eight elements of a row, or of a column
-        float x[8];
-        if (p.by_row != nullptr && r0 + line < R) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = tile[line][k + j];
-            const int64_t st = (c0 + k) / K;
-            if (st < stages)
-                put(p.by_row + (st * p.R + r0 + line) * kStageBytes, (c0 + k) % K, x);
-        }
-        if (p.by_col != nullptr && c0 + line < p.d) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = tile[k + j][line];
-            const int64_t st = (r0 + k) / K;
-            if (st * K < R) put(p.by_col + (st * p.d + c0 + line) * kStageBytes, (r0 + k) % K, x);
+            for (int k = 0; k < 8; ++k) b[k] = static_cast<__bf16>(x[j][k]);
+            *reinterpret_cast<b16x8*>(to) = b;
         }
     }
 }
@@ -346,94 +344,62 @@ struct ScoreEpi {
     }
 };
 
-// Bytes of a row of 32 16-bit values in LDS while a block is turned: the two
-// half waves that write it meet different banks.
-constexpr int kTurnPitch = 80;
-
-// Backward: the same tiles as dl, written as rows of tokens (stages along the
-// vocabulary) and as rows of the vocabulary (stages along the tokens).
+// Backward: the same tiles as dl, an operand whose rows are tokens and whose
+// stages run along the piece of the vocabulary; zero where either ends inside
+// the tile.
 template <bool SPLIT>
 struct DlEpi {
     const Header* hd;
     const int32_t* tgt;
     const float2* norm;  // (m, 1 / s) of each token
-    const float* gr;  // upstream gradient of each token over the largest, NULL: all 1
-    char* by_tok;
-    char* by_voc;
-    int64_t v0;      // first row of the piece
-    int64_t n, voc;  // rows that the two are laid out for
+    const float* gr;     // upstream gradient of each token over the largest, NULL: all 1
+    char* out;
+    int64_t v0;    // first row of the piece
+    int64_t rows;  // tokens that it is laid out for: whole tiles
     template <class Tile>
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         const float scale2 = logit_scale<SPLIT>(hd) * kLog2e;
-        const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
+        const int have = static_cast<int>(t.M - t.m0());  // those rows of this wave that exist
         constexpr float up = SPLIT ? static_cast<float>(1 << kDlExp) : 1.0f;
         constexpr int K = kStageK<SPLIT>;
-        __syncthreads();  // the ring is free
-        uint16_t* sh = reinterpret_cast<uint16_t*>(t.lds + (threadIdx.x >> 6) * 64 * kTurnPitch);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t tok = t.n0() + t.col(b);
             const bool in = tok < t.N;
             const int64_t want = (in ? tgt[tok] - v0 : -1) - t.m0();
-            const bool here = want >= 0 && want < 32 * Tile::kNA;
-            const bool any = __any(here);
+            const bool any = __any(want >= 0 && want < 32 * Tile::kNA);
             const float2 ms = in ? norm[tok] : make_float2(0.0f, 0.0f);
             const float g = (in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f) * up;
             const float gs = g * ms.y;
 #pragma unroll
             for (int a = 0; a < Tile::kNA; ++a) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float p = exp2_(fmaf(acc[a][b][r], scale2, -ms.x)) * gs;
-                    if (any && t.row(a, r) == want) p -= g;
-                    acc[a][b][r] = in && t.row(a, r) < rows ? p : 0.0f;
-                }
-                const int64_t v = t.m0() + 32 * a;          // this block's 32 rows
-                const int64_t k = t.n0() + 32 * b;          // and 32 tokens
-                char* tk = by_tok + ((v / K) * n + tok) * kStageBytes + 2 * (v % K);
-                char* vc = by_voc + ((k / K) * voc + v) * kStageBytes + 2 * (k % K);
+                const int64_t v = t.m0() + 32 * a;  // this block's 32 rows
+                char* to = out + ((v / K) * rows + tok) * kStageBytes + 2 * (v % K);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int at = 8 * q + 4 * (t.lane >> 5);
                     uint16_t h[4], w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float x = acc[a][b][4 * q + j];
+                        const int r = 4 * q + j;
+                        float p = exp2_(fmaf(acc[a][b][r], scale2, -ms.x)) * gs;
+                        if (any && t.row(a, r) == want) p -= g;
+                        p = in && t.row(a, r) < have ? p : 0.0f;
                         if constexpr (SPLIT) {
-                            const _Float16 f = static_cast<_Float16>(x);
+                            const _Float16 f = static_cast<_Float16>(p);
                             h[j] = __builtin_bit_cast(uint16_t, f);
                             w[j] = __builtin_bit_cast(
-                                uint16_t, static_cast<_Float16>(x - static_cast<float>(f)));
+                                uint16_t, static_cast<_Float16>(p - static_cast<float>(f)));
                         } else {
-                            h[j] = f32_to_bf16(x);
+                            h[j] = f32_to_bf16(p);
                             w[j] = 0;
                         }
-                        uint16_t* to = sh + (at + j) * (kTurnPitch / 2) + (t.lane & 31);
-                        *to = h[j];
-                        if (SPLIT) to[32 * kTurnPitch / 2] = w[j];
                     }
-                    if (in) {
-                        *reinterpret_cast<ushort4*>(tk + 2 * at) =
-                            make_ushort4(h[0], h[1], h[2], h[3]);
-                        if (SPLIT)
-                            *reinterpret_cast<ushort4*>(tk + 64 + 2 * at) =
-                                make_ushort4(w[0], w[1], w[2], w[3]);
-                    }
+                    const int at = 2 * (8 * q + 4 * (t.lane >> 5));
+                    *reinterpret_cast<ushort4*>(to + at) = make_ushort4(h[0], h[1], h[2], h[3]);
+                    if (SPLIT)
+                        *reinterpret_cast<ushort4*>(to + 64 + at) =
+                            make_ushort4(w[0], w[1], w[2], w[3]);
                 }
-                // turned in the wave's own LDS: 16 bytes of a vocabulary row a lane
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-#pragma unroll
-                for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = 16 * i + (t.lane >> 2), piece = t.lane & 3;
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(
-                            reinterpret_cast<const char*>(sh) + (32 * p + row) * kTurnPitch +
-                            16 * piece);
-                        *reinterpret_cast<f32x4*>(vc + row * kStageBytes + 64 * p + 16 * piece) =
-                            x;
-                    }
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             }
         }
     }
@@ -806,6 +772,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
 
 // ───────────────────────────── sizes ─────────────────────────────
 
+int64_t up64(int64_t x) { return (x + 63) & ~int64_t{63}; }
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t{255}; }
 
 struct Carve {
@@ -818,7 +785,7 @@ struct Carve {
 };
 
 struct Saved {
-    int64_t header, rows, pos, tgt, norm, h_row, w_row, h_col, w_col, bytes;
+    int64_t header, rows, pos, tgt, norm, h, w, bytes;
 };
 
 bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
@@ -834,13 +801,8 @@ Saved saved_of(const slk_linear_ce* a) {
     s.pos = c.take(4 * a->n);
     s.tgt = c.take(4 * a->n);
     s.norm = c.take(8 * a->n);
-    s.h_row = c.take(stages(a, a->d) * a->n * kStageBytes);
-    s.w_row = c.take(stages(a, a->d) * a->v * kStageBytes);
-    s.h_col = s.w_col = 0;
-    if (a->keep) {
-        s.h_col = c.take(stages(a, a->n) * a->d * kStageBytes);
-        s.w_col = c.take(stages(a, a->v) * a->d * kStageBytes);
-    }
+    s.h = c.take(stages(a, a->d) * up64(a->n) * kStageBytes);
+    s.w = c.take(stages(a, a->d) * up64(a->v) * kStageBytes);
     s.bytes = few(a) ? 0 : c.at;
     return s;
 }
@@ -868,9 +830,9 @@ Forward forward_of(const slk_linear_ce* a) {
     return f;
 }
 
-// Vocabulary rows of a piece of the backward: dl of a piece, in its two forms,
-// takes at most kDlBytes.
-constexpr int64_t kDlBytes = int64_t{1} << 30;
+// Vocabulary rows of a piece of the backward: dl of a piece takes at most
+// kDlBytes.
+constexpr int64_t kDlBytes = int64_t{1} << 29;
 
 // Parts of a product's K loop. With one workgroup a CU, tiles·s of them take
 // ceil(tiles·s / 256) rounds of 1/s of the loop each (about 1.1 us a stage of a
@@ -897,13 +859,13 @@ int splits_for(int64_t m, int64_t n, int64_t nst) {
 struct Backward {
     int64_t piece;  // rows of a piece, a multiple of kTileM
     int sh, sw;     // parts of the two products
-    int64_t gr, factor, by_tok, by_voc, dh, dw, bytes;
+    int64_t gr, factor, dl, dl_rows, dh, dw, bytes;
 };
 Backward backward_of(const slk_linear_ce* a) {
     Backward b;
     // (the epilogue writes whole tiles of tokens)
-    const int64_t n_up = ceil_div(a->n, kWideN) * kWideN;
-    const int64_t per_row = n_up * (split_of(a) ? 8 : 4);
+    b.dl_rows = ceil_div(a->n, kWideN) * kWideN;
+    const int64_t per_row = b.dl_rows * (split_of(a) ? 4 : 2);
     int64_t most = kDlBytes / per_row / kTileM * kTileM;  // rows of a piece
     if (most < kTileM) most = kTileM;
     const int64_t all = ceil_div(a->v, kTileM) * kTileM;
@@ -932,8 +894,7 @@ Backward backward_of(const slk_linear_ce* a) {
     Carve c;
     b.factor = c.take(4);
     b.gr = c.take(4 * a->n);
-    b.by_tok = c.take(stages(a, b.piece) * a->n * kStageBytes);
-    b.by_voc = c.take(stages(a, n_up) * b.piece * kStageBytes);
+    b.dl = c.take(stages(a, b.piece) * b.dl_rows * kStageBytes);
     const bool whole = b.sh == 1 && b.piece >= a->v;
     b.dh = c.take(a->dhidden != nullptr && !whole ? 4 * b.sh * a->n * a->d : 0);
     b.dw = c.take(a->dweight != nullptr && b.sw > 1 ? 4 * b.sw * b.piece * a->d : 0);
@@ -962,9 +923,12 @@ int validate(const slk_linear_ce* a, const char* who) {
 
 template <class T, bool SPLIT>
 int pack(const PackArgs& p, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(p.R, 64)),
-                    static_cast<unsigned>(ceil_div(p.d, 64)));
-    hipLaunchKernelGGL((ce_pack_kernel<T, SPLIT>), grid, dim3(256), 0, st, p);
+    constexpr int K = kStageK<SPLIT>;
+    const dim3 grid(static_cast<unsigned>(ceil_div(ceil_div(up64(p.R), 4) * (K / 8), 256)),
+                    static_cast<unsigned>(ceil_div(p.d, K)));
+    const bool vec = p.d % 4 == 0 && aligned_to(p.src, 4 * T::kBytes);
+    if (vec) hipLaunchKernelGGL((ce_pack_kernel<T, SPLIT, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((ce_pack_kernel<T, SPLIT, false>), grid, dim3(256), 0, st, p);
     return check_launch("linear_ce pack");
 }
 
@@ -1012,15 +976,14 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
             else go(ce_top_kernel<false>);
             if ((rc = check_launch("linear_ce top")) != SLK_OK) return rc;
         }
-        PackArgs ph{a->hidden, rows, &hd->live, hd, false, a->n, a->d, sv + s.h_row,
-                    a->keep ? sv + s.h_col : nullptr};
-        PackArgs pw{a->weight, nullptr, nullptr, hd, true, a->v, a->d, sv + s.w_row,
-                    a->keep ? sv + s.w_col : nullptr};
+        const PackArgs ph{a->hidden, rows, &hd->live, hd, false, a->n, a->d, up64(a->n), sv + s.h};
+        const PackArgs pw{a->weight, nullptr, nullptr, hd, true, a->v, a->d, up64(a->v), sv + s.w};
         if ((rc = pack<T, SPLIT>(ph, st)) != SLK_OK) return rc;
         if ((rc = pack<T, SPLIT>(pw, st)) != SLK_OK) return rc;
-        const MmaArgs g{sv + s.w_row, sv + s.h_row, a->v, a->n, stages(a, a->d), a->v, a->n,
+        const MmaArgs g{sv + s.w, sv + s.h, a->v, a->n, stages(a, a->d), up64(a->v), up64(a->n),
                         &hd->live, kLiveN, 1};
-        rc = mma<SPLIT>(g, ScoreEpi<SPLIT>{hd, tgt, part, zt, a->n}, st, "linear_ce logits");
+        rc = mma<SPLIT, false, false>(g, ScoreEpi<SPLIT>{hd, tgt, part, zt, a->n}, st,
+                                      "linear_ce logits");
         j.pos = pos;
         j.tgt = tgt;
         j.norm = reinterpret_cast<float2*>(sv + s.norm);
@@ -1063,7 +1026,6 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
                        a->dhidden);
     int rc = check_launch("linear_ce upstream");
     if (rc != SLK_OK) return rc;
-    constexpr int K = kStageK<SPLIT>;
     float* dh = reinterpret_cast<float*>(sc + b.dh);
     float* dw = reinterpret_cast<float*>(sc + b.dw);
     auto finish = [&](const float* sums, int splits, int64_t r, int64_t stride,
@@ -1076,31 +1038,35 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     };
     for (int64_t v0 = 0; v0 < a->v; v0 += b.piece) {
         const int64_t vn = a->v - v0 < b.piece ? a->v - v0 : b.piece;
-        const MmaArgs gl{sv + s.w_row + v0 * kStageBytes, sv + s.h_row, vn, a->n,
-                         stages(a, a->d), a->v, a->n, &hd->live, kLiveN, 1};
+        const MmaArgs gl{sv + s.w + v0 * kStageBytes, sv + s.h, vn, a->n, stages(a, a->d),
+                         up64(a->v), up64(a->n), &hd->live, kLiveN, 1};
         const DlEpi<SPLIT> el{hd, tgt, norm, a->reduction == SLK_REDUCE_NONE ? gr : nullptr,
-                              sc + b.by_tok, sc + b.by_voc, v0, a->n, b.piece};
-        if ((rc = mma<SPLIT>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+                              sc + b.dl, v0, b.dl_rows};
+        if ((rc = mma<SPLIT, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
         if (a->dhidden != nullptr) {
-            const MmaArgs g{sc + b.by_tok, sv + s.w_col + v0 / K * a->d * kStageBytes, a->n, a->d,
-                            stages(a, vn), a->n, a->d, &hd->live, kLiveM, b.sh};
+            // dh = dl·W: W's rows, from v0, run along K
+            const MmaArgs g{sc + b.dl, sv + s.w + v0 * kStageBytes, a->n, a->d, stages(a, vn),
+                            b.dl_rows, up64(a->v), &hd->live, kLiveM, b.sh};
             if (whole) {
-                rc = mma<SPLIT>(g, TokenEpi<T, SPLIT>{hd, factor, rows, a->dhidden, a->d}, st,
-                                "linear_ce dhidden");
+                rc = mma<SPLIT, false, true>(g, TokenEpi<T, SPLIT>{hd, factor, rows, a->dhidden,
+                                                                   a->d}, st, "linear_ce dhidden");
             } else {
-                rc = mma<SPLIT>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st, "linear_ce dhidden");
+                rc = mma<SPLIT, false, true>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st,
+                                             "linear_ce dhidden");
             }
             if (rc != SLK_OK) return rc;
         }
         if (a->dweight != nullptr) {
-            const MmaArgs g{sc + b.by_voc, sv + s.h_col, vn, a->d, stages(a, a->n), b.piece, a->d,
-                            &hd->live, kLiveK, b.sw};
+            // dW = dlᵀ·h: both operands' rows, the tokens, run along K
+            const MmaArgs g{sc + b.dl, sv + s.h, vn, a->d, stages(a, a->n), b.dl_rows,
+                            up64(a->n), &hd->live, kLiveK, b.sw};
             void* out = static_cast<char*>(a->dweight) + v0 * a->d * T::kBytes;
             if (b.sw == 1) {
-                rc = mma<SPLIT>(g, WeightEpi<T, SPLIT>{hd, factor, out, a->d}, st,
-                                "linear_ce dweight");
+                rc = mma<SPLIT, true, true>(g, WeightEpi<T, SPLIT>{hd, factor, out, a->d}, st,
+                                            "linear_ce dweight");
             } else {
-                rc = mma<SPLIT>(g, SumEpi{dw, b.piece, a->d, false}, st, "linear_ce dweight");
+                rc = mma<SPLIT, true, true>(g, SumEpi{dw, b.piece, a->d, false}, st,
+                                            "linear_ce dweight");
                 if (rc == SLK_OK) rc = finish(dw, b.sw, vn, b.piece, nullptr, true, out);
             }
             if (rc != SLK_OK) return rc;

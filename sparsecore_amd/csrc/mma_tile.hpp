@@ -11,6 +11,12 @@
 //           rounding, at a third of the float16 rate, where the matrix cores'
 //           float32 instructions run at a sixteenth;
 //   else    64 elements in bfloat16.
+// An operand is used along its stages (K inside a row) or across its rows: the
+// same memory with K as the row and a stage as a panel of 32 (64) rows of the
+// product ("turned" below). Turned fragments come out of LDS through the
+// transposing read: a lane of each 16 names four columns of one of four rows and
+// gets one column of all four. So every operand is packed once, whichever of the
+// three products reads it.
 //
 // Tile: 256 x 128, eight waves of 64 x 64 (2 x 2 blocks of 32 x 32). Stages go
 // from memory straight into a ring of three LDS buffers of 48 KiB, two stages
@@ -46,6 +52,8 @@ constexpr int wait_vm(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) 
 // Which dimension is the device-side count of live tokens.
 enum MmaLive { kLiveNone = 0, kLiveM = 1, kLiveN = 2, kLiveK = 3 };
 
+// A turned operand's rows run along K: whole stages of them are there, zero (or
+// finite, against zeros) where K ends inside one.
 struct MmaArgs {
     const void* A;
     const void* B;
@@ -75,7 +83,101 @@ struct MmaTile {
     __device__ __forceinline__ int col(int b) const { return 32 * b + (lane & 31); }
 };
 
-template <bool SPLIT, class Epi>
+// The direct loads of a wave for an operand's stage of 64·PER rows (or of that
+// many panel rows): load i = wv + 8 q fills lines 8 i .. 8 i + 7 of 128 bytes of
+// the operand's buffer, lane l piece l mod 8 of line 8 i + l / 8. Pieces are
+// permuted so that the lanes that read together meet all banks once: along the
+// stage by the row, turned by rows 2, 3 of every four and by rows 4 to 7. A load
+// is a scalar base (64 rows, or a panel; past the end the last one again) and
+// one lane offset for all of them: an offset a load spilled registers.
+template <bool SPLIT, bool TURN, int PER>
+struct Loads {
+    static constexpr int K = kStageK<SPLIT>;
+    const char* base[PER];
+    uint32_t off;
+    int64_t step;
+    __device__ __forceinline__ Loads(const void* P, int64_t R, int64_t limit, int64_t r0, int wv,
+                                     int lane) {
+        step = (TURN ? K : R) * kStageBytes;
+        const int line = 8 * wv + lane / 8;
+        off = TURN ? line % K * kStageBytes +
+                         16 * ((lane & 7) ^ (4 * ((line >> 1) & 1) + 2 * ((line >> 2) & 1)))
+                   : line * kStageBytes + 16 * ((lane & 7) ^ ((line >> 1) & 7));
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            constexpr int unit = TURN ? K : 64;
+            const int64_t units = ceil_div(limit, unit);
+            int64_t u = r0 / unit + (TURN ? 8 * (wv + 8 * q) / K : q);
+            if (u >= units) u = units - 1;
+            base[q] = static_cast<const char*>(P) + u * (TURN ? R : 64) * kStageBytes;
+        }
+    }
+    __device__ __forceinline__ void issue(unsigned char* to, int wv, int64_t st) const {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass emits no stub of a kernel that calls this
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const char* from = base[q] + st * step;
+            uint32_t o = off;
+            asm("" : "+s"(from), "+v"(o));  // so that their sum is the load's own
+            __builtin_amdgcn_global_load_lds(from + o, to + 1024 * (wv + 8 * q), 16, 0, 0);
+        }
+#endif
+    }
+};
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// The transposing LDS read: each lane of 16 names four 16-bit elements; lane l
+// gets element l % 4 of what lanes l / 4, 4 + l / 4, 8 + l / 4, 12 + l / 4 named.
+__device__ __forceinline__ i16x4 read_turned(const unsigned char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using Piece = __attribute__((address_space(3))) i16x4*;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)(const_cast<unsigned char*>(lds)));
+#else
+    (void)lds;  // the host pass has no LDS
+    return i16x4{};
+#endif
+}
+
+// Fragments of the operand's 32-row blocks from a staged buffer: block `b` of
+// the wave's rows (first row r0 of the tile), k-step ks, part 0 (high or only)
+// or 1 (low). Lane l gets row l % 32, K 16 ks + 8 (l / 32) ...
+template <bool SPLIT, bool TURN>
+struct Frags {
+    using Frag = std::conditional_t<SPLIT, f16x8, b16x8>;
+    static constexpr int K = kStageK<SPLIT>;
+    int row, half;    // along the stage
+    int at[2][2];     // turned: byte of [part, or odd block][four rows of eight]
+    __device__ __forceinline__ Frags(int r0, int lane) {
+        half = lane >> 5;
+        row = r0 + (lane & 31);
+        const int i = lane & 15, ch = (lane >> 4) & 1;
+        // row r0 is the first of a panel: 32 rows of a split operand, 64 of the other
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int piece = (4 * p + 2 * ch + ((i >> 1) & 1)) ^ (4 * ((i >> 3) & 1) + 2 * h);
+                at[p][h] = (r0 / K * K + 8 * half + 4 * h + (i >> 2)) * kStageBytes + 16 * piece +
+                           8 * (i & 1);
+            }
+    }
+    __device__ __forceinline__ Frag read(const unsigned char* buf, int b, int ks, int part) const {
+        if constexpr (TURN) {
+            const int p = SPLIT ? part : b & 1, panel = SPLIT ? b : b >> 1;
+            const int o = (panel * K + 16 * ks) * kStageBytes;
+            const i16x4 lo = read_turned(buf + at[p][0] + o);
+            const i16x4 hi = read_turned(buf + at[p][1] + o);
+            return __builtin_bit_cast(Frag,
+                                      __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int r = row + 32 * b, c = (SPLIT ? 4 * part : 0) + 2 * ks + half;
+            return *reinterpret_cast<const Frag*>(buf + 16 * (r * 8 + (c ^ ((r >> 1) & 7))));
+        }
+    }
+};
+
+template <bool SPLIT, bool TA, bool TB, class Epi>
 __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const Epi epi) {
     __shared__ __align__(16) unsigned char ring[kMmaBufs][(kTileM + kTileN) * kStageBytes];
 
@@ -106,34 +208,12 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wv >> 1, wn = wv & 1;
 
-    // Load i of a stage fills rows 8 i .. 8 i + 7 of its operand's buffer: lane
-    // l fetches piece (l mod 8) ^ swizzle of row 8 i + l / 8. Rows past the
-    // operand are clamped to its last row; their results are not used.
     constexpr int kPerA = kTileM / 64, kPerB = kTileN / 64;
-    uint32_t offA[kPerA], offB[kPerB];
-    auto plan = [&](int64_t R, int64_t r0, int i) {
-        const int rr = 8 * i + lane / 8;
-        int64_t r = r0 + rr;
-        if (r >= R) r = R - 1;
-        return static_cast<uint32_t>(r * kStageBytes + 16 * ((lane & 7) ^ ((rr >> 1) & 7)));
-    };
-#pragma unroll
-    for (int q = 0; q < kPerA; ++q) offA[q] = plan(M, i0, wv + 8 * q);
-#pragma unroll
-    for (int q = 0; q < kPerB; ++q) offB[q] = plan(N, k0, wv + 8 * q);
-    const char* A = static_cast<const char*>(g.A);
-    const char* B = static_cast<const char*>(g.B);
+    const Loads<SPLIT, TA, kPerA> la(g.A, g.rows_a, M, i0, wv, lane);
+    const Loads<SPLIT, TB, kPerB> lb(g.B, g.rows_b, N, k0, wv, lane);
     auto issue = [&](int buf, int64_t st) {
-        const char* a = A + st * g.rows_a * kStageBytes;
-        const char* b = B + st * g.rows_b * kStageBytes;
-#pragma unroll
-        for (int q = 0; q < kPerA; ++q)
-            __builtin_amdgcn_global_load_lds(a + offA[q], &ring[buf][1024 * (wv + 8 * q)], 16, 0,
-                                             0);
-#pragma unroll
-        for (int q = 0; q < kPerB; ++q)
-            __builtin_amdgcn_global_load_lds(
-                b + offB[q], &ring[buf][kTileM * kStageBytes + 1024 * (wv + 8 * q)], 16, 0, 0);
+        la.issue(ring[buf], wv, st);
+        lb.issue(ring[buf] + kTileM * kStageBytes, wv, st);
     };
 
     f32x16 acc[2][2];
@@ -144,23 +224,18 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
 
-    const int half = lane >> 5;
-    const int rA = wm * 64 + (lane & 31), rB = wn * 64 + (lane & 31);
-    using Frag = std::conditional_t<SPLIT, f16x8, b16x8>;
-    auto frag = [&](const unsigned char* lds, int r, int c) {
-        return *reinterpret_cast<const Frag*>(lds + 16 * (r * 8 + (c ^ ((r >> 1) & 7))));
-    };
+    const Frags<SPLIT, TA> fa(wm * 64, lane);
+    const Frags<SPLIT, TB> fb(wn * 64, lane);
     // fragments of half a stage: SPLIT, a k-step's high and low parts; else two k-steps
-    Frag af[2][2][2], bf[2][2][2];  // [half stage][block][part]
+    typename Frags<SPLIT, TA>::Frag af[2][2][2], bf[2][2][2];  // [half stage][block][part]
     auto reads = [&](const unsigned char* buf, int h) {
-        const unsigned char* lb = buf + kTileM * kStageBytes;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const int c = (SPLIT ? 4 * p + 2 * h : 4 * h + 2 * p) + half;
-                af[h][b][p] = frag(buf, rA + 32 * b, c);
-                bf[h][b][p] = frag(lb, rB + 32 * b, c);
+                const int ks = SPLIT ? h : 2 * h + p, part = SPLIT ? p : 0;
+                af[h][b][p] = fa.read(buf, b, ks, part);
+                bf[h][b][p] = fb.read(buf + kTileM * kStageBytes, b, ks, part);
             }
     };
     auto mfmas = [&](int h, int pa, int pb) {
@@ -246,7 +321,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
 // time before that is read.
 constexpr int kWideN = 256;
 
-template <bool SPLIT, class Epi>
+template <bool SPLIT, bool TA, bool TB, class Epi>
 __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, const Epi epi) {
     __shared__ __align__(16) unsigned char ring[2][(kTileM + kWideN) * kStageBytes];
 
@@ -277,31 +352,11 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
     const int wm = wv >> 2, wn = wv & 3;
 
     constexpr int kPer = kTileM / 64;  // loads of a wave and stage, of each operand
-    uint32_t offA[kPer], offB[kPer];
-    auto plan = [&](int64_t R, int64_t r0, int i) {
-        const int rr = 8 * i + lane / 8;
-        int64_t r = r0 + rr;
-        if (r >= R) r = R - 1;
-        return static_cast<uint32_t>(r * kStageBytes + 16 * ((lane & 7) ^ ((rr >> 1) & 7)));
-    };
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        offA[q] = plan(M, i0, wv + 8 * q);
-        offB[q] = plan(N, k0, wv + 8 * q);
-    }
-    const char* A = static_cast<const char*>(g.A);
-    const char* B = static_cast<const char*>(g.B);
+    const Loads<SPLIT, TA, kPer> la(g.A, g.rows_a, M, i0, wv, lane);
+    const Loads<SPLIT, TB, kPer> lb(g.B, g.rows_b, N, k0, wv, lane);
     auto issue = [&](int buf, int64_t st) {
-        const char* a = A + st * g.rows_a * kStageBytes;
-        const char* b = B + st * g.rows_b * kStageBytes;
-#pragma unroll
-        for (int q = 0; q < kPer; ++q)
-            __builtin_amdgcn_global_load_lds(a + offA[q], &ring[buf][1024 * (wv + 8 * q)], 16, 0,
-                                             0);
-#pragma unroll
-        for (int q = 0; q < kPer; ++q)
-            __builtin_amdgcn_global_load_lds(
-                b + offB[q], &ring[buf][kTileM * kStageBytes + 1024 * (wv + 8 * q)], 16, 0, 0);
+        la.issue(ring[buf], wv, st);
+        lb.issue(ring[buf] + kTileM * kStageBytes, wv, st);
     };
 
     f32x16 acc[4][2];
@@ -312,23 +367,19 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
 
-    const int half = lane >> 5;
-    const int rA = wm * 128 + (lane & 31), rB = wn * 64 + (lane & 31);
-    using Frag = std::conditional_t<SPLIT, f16x8, b16x8>;
+    const Frags<SPLIT, TA> fa(wm * 128, lane);
+    const Frags<SPLIT, TB> fb(wn * 64, lane);
     // [set][block]; a set is a k-step's parity, or (SPLIT) 0: high parts, 1: low parts
-    Frag af[2][4], bf[2][2];
-    auto frag = [&](const unsigned char* lds, int r, int c) {
-        return *reinterpret_cast<const Frag*>(lds + 16 * (r * 8 + (c ^ ((r >> 1) & 7))));
-    };
-    // piece c of the rows of A (first two, last two blocks) and of B
-    auto read_a = [&](const unsigned char* buf, int c, int set, int a0) {
+    typename Frags<SPLIT, TA>::Frag af[2][4], bf[2][2];
+    // k-step ks of A's rows (first two, last two blocks) and of B's, into a set
+    auto read_a = [&](const unsigned char* buf, int ks, int set, int a0) {
 #pragma unroll
-        for (int a = a0; a < a0 + 2; ++a) af[set][a] = frag(buf, rA + 32 * a, c + half);
+        for (int a = a0; a < a0 + 2; ++a) af[set][a] = fa.read(buf, a, ks, SPLIT ? set : 0);
     };
-    auto read_b = [&](const unsigned char* buf, int c, int set) {
+    auto read_b = [&](const unsigned char* buf, int ks, int set) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            bf[set][b] = frag(buf + kTileM * kStageBytes, rB + 32 * b, c + half);
+            bf[set][b] = fb.read(buf + kTileM * kStageBytes, b, ks, SPLIT ? set : 0);
     };
     auto mfmas = [&](int a, int sa, int sb) {  // one row of blocks
 #pragma unroll
@@ -379,21 +430,21 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
         const int64_t ahead = st + 2 < s1 ? st + 2 : s1 - 1;
         if constexpr (SPLIT) {
             eight(1, 0, [&] { read_a(cur, 0, 0, 0); }, [&] { read_a(cur, 0, 0, 2); },
-                  [&] { read_b(cur, 4, 1); });
-            eight(0, 0, [&] { read_a(cur, 6, 1, 0); }, [&] { read_a(cur, 6, 1, 2); }, none);
-            eight(0, 1, [&] { read_b(cur, 2, 0); }, none, none);
-            eight(1, 0, [&] { read_a(cur, 2, 0, 0); }, [&] { read_a(cur, 2, 0, 2); },
-                  [&] { read_b(cur, 6, 1); });
+                  [&] { read_b(cur, 0, 1); });
+            eight(0, 0, [&] { read_a(cur, 1, 1, 0); }, [&] { read_a(cur, 1, 1, 2); }, none);
+            eight(0, 1, [&] { read_b(cur, 1, 0); }, none, none);
+            eight(1, 0, [&] { read_a(cur, 1, 0, 0); }, [&] { read_a(cur, 1, 0, 2); },
+                  [&] { read_b(cur, 1, 1); });
             meet();
-            eight(0, 0, [&] { read_a(nxt, 4, 1, 0); },
-                  [&] { read_a(nxt, 4, 1, 2); }, [&] { issue(buf, ahead); });
+            eight(0, 0, [&] { read_a(nxt, 0, 1, 0); },
+                  [&] { read_a(nxt, 0, 1, 2); }, [&] { issue(buf, ahead); });
             eight(0, 1, [&] { read_b(nxt, 0, 0); }, none, none);
         } else {
 #pragma unroll
             for (int ks = 0; ks < 3; ++ks) {
-                const int c = 2 * ks + 2, set = (ks + 1) & 1;
-                eight(ks & 1, ks & 1, [&] { read_b(cur, c, set); }, [&] { read_a(cur, c, set, 0); },
-                      [&] { read_a(cur, c, set, 2); });
+                const int set = (ks + 1) & 1;
+                eight(ks & 1, ks & 1, [&] { read_b(cur, ks + 1, set); },
+                      [&] { read_a(cur, ks + 1, set, 0); }, [&] { read_a(cur, ks + 1, set, 2); });
             }
             meet();
             eight(1, 1, [&] { read_b(nxt, 0, 0); read_a(nxt, 0, 0, 0); },
@@ -407,13 +458,8 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
         issue(1, s0 + 1 < s1 ? s0 + 1 : s0);
         __builtin_amdgcn_s_waitcnt(wait_vm(2 * kPer));
         asm volatile("s_barrier" ::: "memory");
-        if (SPLIT) {
-            read_a(ring[0], 4, 1, 0);
-            read_a(ring[0], 4, 1, 2);
-        } else {
-            read_a(ring[0], 0, 0, 0);
-            read_a(ring[0], 0, 0, 2);
-        }
+        read_a(ring[0], 0, SPLIT ? 1 : 0, 0);
+        read_a(ring[0], 0, SPLIT ? 1 : 0, 2);
         read_b(ring[0], 0, 0);
         int64_t st = s0;
         for (; st + 2 <= s1; st += 2) {
@@ -443,7 +489,7 @@ inline double mma_rounds(int64_t M, int64_t N) {
     return static_cast<double>(ceil_div(tiles, 256)) * (wide ? 1.7 : 1.0);
 }
 
-template <bool SPLIT, class Epi>
+template <bool SPLIT, bool TA, bool TB, class Epi>
 int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
     const bool wide = mma_wide(g.M, g.N, g.splits);
     const int64_t groups =
@@ -451,8 +497,8 @@ int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
     if (groups == 0) return SLK_OK;
     if (groups > INT32_MAX) return fail(SLK_EINVAL, std::string(who) + ": too many tiles");
     const dim3 grid(static_cast<unsigned>(groups)), wg(kMmaThreads);
-    if (wide) hipLaunchKernelGGL((mma_wide_kernel<SPLIT, Epi>), grid, wg, 0, st, g, epi);
-    else hipLaunchKernelGGL((mma_kernel<SPLIT, Epi>), grid, wg, 0, st, g, epi);
+    if (wide) hipLaunchKernelGGL((mma_wide_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);
+    else hipLaunchKernelGGL((mma_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);
     return check_launch(who);
 }
 
