@@ -418,13 +418,20 @@ struct SumEpi {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int64_t c = t.n0() + t.col(b);
+                if (add) {  // the block's loads in flight together
+                    float old[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t row = t.m0() + t.row(a, r);
+                        old[r] = row < t.M && c < t.N ? to[row * d + c] : 0.0f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[a][b][r] += old[r];
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int64_t row = t.m0() + t.row(a, r);
-                    if (row < t.M && c < t.N) {
-                        float* x = to + row * d + c;
-                        *x = add ? *x + acc[a][b][r] : acc[a][b][r];
-                    }
+                    if (row < t.M && c < t.N) to[row * d + c] = acc[a][b][r];
                 }
             }
     }

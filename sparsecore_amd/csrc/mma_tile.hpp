@@ -22,9 +22,9 @@
 // from memory straight into a ring of three LDS buffers of 48 KiB, two stages
 // ahead, one barrier a stage; the 16-byte pieces of a staged row are permuted
 // (piece c of row r at slot c ^ ((r >> 1) & 7)), so that the 16 lanes of an
-// LDS pass meet all banks once. Buffer indexes are compile-time constants (the
-// loop is unrolled by three): otherwise the compiler makes every LDS read wait
-// for the loads just issued.
+// LDS pass meet all banks once. Each buffer is an LDS variable of its own, named
+// by a compile-time constant (the loop is unrolled by three): otherwise the
+// compiler makes an LDS read wait for the loads just issued into another buffer.
 #pragma once
 
 #include "common.hpp"
@@ -74,7 +74,7 @@ struct MmaTile {
     int wm, wn, lane;
     int64_t M, N;
     int split;
-    char* lds;  // at least 96 KiB, free after a barrier
+    char* lds;  // a buffer of the ring (at least 48 KiB), free after a barrier
     __device__ __forceinline__ int64_t m0() const { return i0 + 32 * NA * wm; }
     __device__ __forceinline__ int64_t n0() const { return k0 + 64 * wn; }
     __device__ __forceinline__ int row(int a, int r) const {
@@ -116,9 +116,13 @@ struct Loads {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass emits no stub of a kernel that calls this
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
-            const char* from = base[q] + st * step;
+            const uint64_t at = reinterpret_cast<uint64_t>(base[q] + st * step);
+            const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+            const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+            const char* from =
+                reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
             uint32_t o = off;
-            asm("" : "+s"(from), "+v"(o));  // so that their sum is the load's own
+            asm("" : "+v"(o));  // keeps their sum with the load, whose own it is
             __builtin_amdgcn_global_load_lds(from + o, to + 1024 * (wv + 8 * q), 16, 0, 0);
         }
 #endif
@@ -177,31 +181,63 @@ struct Frags {
     }
 };
 
+// A workgroup's tile and part of the K loop. Grouped, XCD-contiguous tile order:
+// consecutive tiles share rows of A and B. The launch keeps tiles x splits under
+// 2^31, so that the divisions take 32 bits; the results are put back into scalar
+// registers, which the loads' bases come from.
+struct MmaWork {
+    int64_t M, N, i0, k0, s0, s1;
+    int split;
+    bool any;  // false for the whole workgroup: past the live tiles
+    template <int K, int TN>
+    static __device__ __forceinline__ MmaWork of(const MmaArgs& g) {
+        MmaWork w;
+        w.M = g.M;
+        w.N = g.N;
+        int64_t nst = g.nst;
+        if (g.which != kLiveNone) {
+            const int64_t live = *g.live;
+            if (g.which == kLiveM) w.M = live;
+            else if (g.which == kLiveN) w.N = live;
+            else nst = ceil_div(live, K);
+        }
+        const uint32_t nTi = static_cast<uint32_t>(ceil_div(w.M, kTileM));
+        const uint32_t nTk = static_cast<uint32_t>(ceil_div(w.N, TN));
+        const uint32_t tiles = nTi * nTk, splits = g.splits, total = tiles * splits;
+        w.any = blockIdx.x < total;
+        if (!w.any) return w;
+        const uint32_t L = static_cast<uint32_t>(xcd_logical_block(blockIdx.x, total));
+        const uint32_t split = splits > 1 ? L / tiles : 0;
+        const uint32_t tile = L - split * tiles;
+        const uint32_t grp = tile / (kMmaGroup * nTk);
+        const uint32_t first = grp * kMmaGroup;
+        const uint32_t gsize = nTi - first < kMmaGroup ? nTi - first : kMmaGroup;
+        const uint32_t in_grp = tile - grp * kMmaGroup * nTk;
+        const uint32_t col = in_grp / gsize;
+        const uint32_t per = static_cast<uint32_t>(nst) / splits;
+        const uint32_t extra = static_cast<uint32_t>(nst) % splits;
+        auto uniform = [](uint32_t x) {
+            return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+        };
+        w.i0 = uniform(first + in_grp - col * gsize) * kTileM;
+        w.k0 = uniform(col) * TN;
+        w.split = static_cast<int>(uniform(split));
+        w.s0 = uniform(split * per + (split < extra ? split : extra));
+        w.s1 = uniform(split * per + per + (split < extra ? split + 1 : extra));
+        return w;
+    }
+};
+
 template <bool SPLIT, bool TA, bool TB, class Epi>
 __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const Epi epi) {
-    __shared__ __align__(16) unsigned char ring[kMmaBufs][(kTileM + kTileN) * kStageBytes];
+    __shared__ __align__(16) unsigned char ring0[(kTileM + kTileN) * kStageBytes];
+    __shared__ __align__(16) unsigned char ring1[(kTileM + kTileN) * kStageBytes];
+    __shared__ __align__(16) unsigned char ring2[(kTileM + kTileN) * kStageBytes];
 
-    int64_t M = g.M, N = g.N, nst = g.nst;
-    if (g.which != kLiveNone) {
-        const int64_t live = *g.live;
-        if (g.which == kLiveM) M = live;
-        else if (g.which == kLiveN) N = live;
-        else nst = ceil_div(live, kStageK<SPLIT>);
-    }
-    const int64_t nTi = ceil_div(M, kTileM), nTk = ceil_div(N, kTileN);
-    const int64_t tiles = nTi * nTk, total = tiles * g.splits;
-    if (static_cast<int64_t>(blockIdx.x) >= total) return;  // the whole workgroup
-    // grouped, XCD-contiguous tile order: consecutive tiles share rows of A and B
-    const int64_t L = xcd_logical_block(blockIdx.x, total);
-    const int split = static_cast<int>(L / tiles);
-    const int64_t tile = L - split * tiles;
-    const int64_t grp = tile / (kMmaGroup * nTk);
-    const int64_t first = grp * kMmaGroup;
-    const int64_t gsize = nTi - first < kMmaGroup ? nTi - first : kMmaGroup;
-    const int64_t in_grp = tile - grp * kMmaGroup * nTk;
-    const int64_t i0 = (first + in_grp % gsize) * kTileM;
-    const int64_t k0 = (in_grp / gsize) * kTileN;
-    const int64_t s0 = split * nst / g.splits, s1 = (split + 1) * nst / g.splits;
+    const MmaWork w = MmaWork::of<kStageK<SPLIT>, kTileN>(g);
+    if (!w.any) return;
+    const int64_t M = w.M, N = w.N, i0 = w.i0, k0 = w.k0, s0 = w.s0, s1 = w.s1;
+    const int split = w.split;
 
     const int t = threadIdx.x;
     const int lane = t & 63;
@@ -212,8 +248,9 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
     const Loads<SPLIT, TA, kPerA> la(g.A, g.rows_a, M, i0, wv, lane);
     const Loads<SPLIT, TB, kPerB> lb(g.B, g.rows_b, N, k0, wv, lane);
     auto issue = [&](int buf, int64_t st) {
-        la.issue(ring[buf], wv, st);
-        lb.issue(ring[buf] + kTileM * kStageBytes, wv, st);
+        unsigned char* to = buf == 0 ? ring0 : buf == 1 ? ring1 : ring2;
+        la.issue(to, wv, st);
+        lb.issue(to + kTileM * kStageBytes, wv, st);
     };
 
     f32x16 acc[2][2];
@@ -264,7 +301,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
         constexpr int buf = decltype(I)::value;
         mfmas(0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        reads(ring[buf], 1);
+        reads(buf == 0 ? ring0 : buf == 1 ? ring1 : ring2, 1);
         issue((buf + 2) % kMmaBufs, st + 2 < s1 ? st + 2 : s1 - 1);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (SPLIT) {
@@ -276,7 +313,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(wait_vm(kLoads));
         asm volatile("s_barrier" ::: "memory");
-        reads(ring[(buf + 1) % kMmaBufs], 0);
+        reads(buf == 0 ? ring1 : buf == 1 ? ring2 : ring0, 0);
         __builtin_amdgcn_sched_barrier(0);
         mfmas(1, 0, 0);
         if constexpr (SPLIT) {
@@ -294,7 +331,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
         issue(1, s0 + 1 < s1 ? s0 + 1 : s0);
         __builtin_amdgcn_s_waitcnt(wait_vm(kLoads));
         asm volatile("s_barrier" ::: "memory");
-        reads(ring[0], 0);
+        reads(ring0, 0);
         int64_t st = s0;
         for (; st + 3 <= s1; st += 3) {
             stage(B0{}, st);
@@ -306,7 +343,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_kernel(const MmaArgs g, const
         __builtin_amdgcn_s_waitcnt(0);  // no direct load still writing LDS
     }
     epi(acc, MmaTile<2, kTileN>{i0, k0, wm, wn, lane, M, N, split,
-                                reinterpret_cast<char*>(&ring[0][0])});
+                                reinterpret_cast<char*>(ring0)});
 }
 
 // The same product in tiles of 256 x 256: eight waves of 128 x 64 (2 x 4), a
@@ -323,28 +360,13 @@ constexpr int kWideN = 256;
 
 template <bool SPLIT, bool TA, bool TB, class Epi>
 __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, const Epi epi) {
-    __shared__ __align__(16) unsigned char ring[2][(kTileM + kWideN) * kStageBytes];
+    __shared__ __align__(16) unsigned char ring0[(kTileM + kWideN) * kStageBytes];
+    __shared__ __align__(16) unsigned char ring1[(kTileM + kWideN) * kStageBytes];
 
-    int64_t M = g.M, N = g.N, nst = g.nst;
-    if (g.which != kLiveNone) {
-        const int64_t live = *g.live;
-        if (g.which == kLiveM) M = live;
-        else if (g.which == kLiveN) N = live;
-        else nst = ceil_div(live, kStageK<SPLIT>);
-    }
-    const int64_t nTi = ceil_div(M, kTileM), nTk = ceil_div(N, kWideN);
-    const int64_t tiles = nTi * nTk, total = tiles * g.splits;
-    if (static_cast<int64_t>(blockIdx.x) >= total) return;  // the whole workgroup
-    const int64_t L = xcd_logical_block(blockIdx.x, total);
-    const int split = static_cast<int>(L / tiles);
-    const int64_t tile = L - split * tiles;
-    const int64_t grp = tile / (kMmaGroup * nTk);
-    const int64_t first = grp * kMmaGroup;
-    const int64_t gsize = nTi - first < kMmaGroup ? nTi - first : kMmaGroup;
-    const int64_t in_grp = tile - grp * kMmaGroup * nTk;
-    const int64_t i0 = (first + in_grp % gsize) * kTileM;
-    const int64_t k0 = (in_grp / gsize) * kWideN;
-    const int64_t s0 = split * nst / g.splits, s1 = (split + 1) * nst / g.splits;
+    const MmaWork w = MmaWork::of<kStageK<SPLIT>, kWideN>(g);
+    if (!w.any) return;
+    const int64_t M = w.M, N = w.N, i0 = w.i0, k0 = w.k0, s0 = w.s0, s1 = w.s1;
+    const int split = w.split;
 
     const int t = threadIdx.x;
     const int lane = t & 63;
@@ -355,8 +377,9 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
     const Loads<SPLIT, TA, kPer> la(g.A, g.rows_a, M, i0, wv, lane);
     const Loads<SPLIT, TB, kPer> lb(g.B, g.rows_b, N, k0, wv, lane);
     auto issue = [&](int buf, int64_t st) {
-        la.issue(ring[buf], wv, st);
-        lb.issue(ring[buf] + kTileM * kStageBytes, wv, st);
+        unsigned char* to = buf ? ring1 : ring0;
+        la.issue(to, wv, st);
+        lb.issue(to + kTileM * kStageBytes, wv, st);
     };
 
     f32x16 acc[4][2];
@@ -424,8 +447,8 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
     // instructions freed (the order lo·hi, hi·hi, hi·lo makes that three groups).
     auto stage = [&](auto I, int64_t st) {
         constexpr int buf = decltype(I)::value;
-        const unsigned char* cur = ring[buf];
-        const unsigned char* nxt = ring[buf ^ 1];
+        const unsigned char* cur = buf ? ring1 : ring0;
+        const unsigned char* nxt = (buf ? ring0 : ring1);
         // past the end the last stage is loaded again, unused
         const int64_t ahead = st + 2 < s1 ? st + 2 : s1 - 1;
         if constexpr (SPLIT) {
@@ -458,9 +481,9 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
         issue(1, s0 + 1 < s1 ? s0 + 1 : s0);
         __builtin_amdgcn_s_waitcnt(wait_vm(2 * kPer));
         asm volatile("s_barrier" ::: "memory");
-        read_a(ring[0], 0, SPLIT ? 1 : 0, 0);
-        read_a(ring[0], 0, SPLIT ? 1 : 0, 2);
-        read_b(ring[0], 0, 0);
+        read_a(ring0, 0, SPLIT ? 1 : 0, 0);
+        read_a(ring0, 0, SPLIT ? 1 : 0, 2);
+        read_b(ring0, 0, 0);
         int64_t st = s0;
         for (; st + 2 <= s1; st += 2) {
             stage(B0{}, st);
@@ -470,7 +493,7 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
         __builtin_amdgcn_s_waitcnt(0);  // no direct load still writing LDS
     }
     epi(acc, MmaTile<4, kWideN>{i0, k0, wm, wn, lane, M, N, split,
-                                reinterpret_cast<char*>(&ring[0][0])});
+                                reinterpret_cast<char*>(ring0)});
 }
 
 // Launches C = A·Bᵀ over an upper bound of its tiles. Wide tiles where their
