@@ -1,19 +1,25 @@
 // The language-model head and its loss without the logits, slk_linear_ce_*:
 //   z = h·Wᵀ (n x v),  lse_n = log Σ_v exp(z_nv),  loss_n = lse_n - z_{n,target}
 //   dl = (exp(z - lse) - onehot(target))·g_n,  dh = dl·W,  dW = dlᵀ·h
-// Logits exist only as 256 x 128 tiles in registers. Forward: each tile leaves
-// its tokens' running maximum and sum, which a second kernel joins. Backward: a
-// piece of the vocabulary at a time, the tiles are computed again, turned into
-// dl in the epilogue and written as the operand of the piece's two gradient
-// products, which follow. 2·n·v·d operations forward, 6 backward, where keeping the logits
-// would take 4 backward and 4 bytes a logit.
+// Logits exist only as tiles in registers. Forward: each tile leaves its tokens'
+// running maximum and sum, which a second kernel joins. Backward: a piece of the
+// vocabulary at a time, the tiles are computed again, turned into dl in the
+// epilogue and written as the operand of the piece's two gradient products, which
+// follow. 2·n·v·d operations forward, 6 backward, where keeping the logits would
+// take 4 backward and 4 bytes a logit.
 //
 // Tokens whose target is ignore_index are left out before anything is computed
 // (a list of the live tokens is made on the device), so that they cost nothing
 // and what their hidden states hold reaches nothing.
 //
-// A score of at most 16 tokens reads W once, straight from memory, on 16 x 16
-// matrix instructions: bound by memory.
+// Bound by the matrix cores from some hundred tokens on. 8192 x 4096 x 100000
+// bfloat16, forward and backward: 21.5 ms, the logits at 1334 TFLOP/s, dhidden's
+// and dweight's products at 1305 and 1203 (a large library product: 1388). 4001 x
+// 768 x 32000 float32: 1.59 ms, 500 TFLOP/s of float32 counted as the three
+// float16 products are one.
+//
+// Few tokens are bound by reading W, which they do where it lies: 8 x 2048 x
+// 80000 at 4.6 TB/s, forward.
 #include "elem.hpp"
 #include "mma_tile.hpp"
 
@@ -674,107 +680,338 @@ __global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict_
 
 // ───────────────────────────── few tokens ─────────────────────────────
 
-constexpr int kFewTokens = 16;
-constexpr int kFewThreads = 256;
+// Few tokens read W where it lies, once forward and once backward: its packed
+// copy alone would be read and written three times more. Up to how many, by what
+// the two ways took at 2048 features and 80000 rows: a score 529 against 570 us at
+// 128 tokens (float32; bfloat16 236 against 253), a score and its gradients 889
+// against 1240 us at 64 (float32), 445 against 620 at 32 but 870 against 628 at 64
+// (bfloat16, whose backward here is on the float32 instructions).
+constexpr int kFewScores = 128;
+template <class T>
+constexpr int kFewTokens = T::kBytes == 4 ? 64 : 32;
+constexpr int kFewThreads = 256, kFewWaves = kFewThreads / kWave;
 
-// A wave takes 16 rows of W at a time against 16 tokens (fewer are repeated):
-// lane l holds row l % 16 of both, its columns 4 (l / 16) .. of each run of 16
-// (float32; 8 (l / 16) of 32 in bfloat16). The same columns meet in both
-// operands, so their order within an instruction does not matter.
+// Sixteen bytes of a row (four float32, eight bfloat16), zeros past its end.
+template <class T>
+using FewPiece = std::conditional_t<T::kBytes == 4, f32x4, b16x8>;
 template <class T, bool VEC>
+__device__ __forceinline__ FewPiece<T> few_piece(const void* p, int64_t i, int64_t left) {
+    constexpr int kMine = 16 / T::kBytes;
+    FewPiece<T> x;
+    if (VEC) {  // the row's length is a multiple of the piece
+        x = *reinterpret_cast<const FewPiece<T>*>(static_cast<const char*>(p) + i * T::kBytes);
+        if (left <= 0) x = FewPiece<T>{};
+    } else {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const float v = T::load(p, j < left ? i + j : i);
+            if constexpr (kMine == 4) x[j] = j < left ? v : 0.0f;
+            else x[j] = static_cast<__bf16>(j < left ? v : 0.0f);
+        }
+    }
+    return x;
+}
+
+// Forward. A wave takes 16 MB rows of W at a time against 16 NB tokens (fewer
+// are repeated): lane l holds row l % 16 of both, piece l / 16 of each run of 64
+// bytes. The same columns meet in both operands, so their order within an
+// instruction does not matter. The loads of U runs are in flight together. z is
+// kept for the backward where it is wanted, 16 NB tokens a row.
+template <class T, bool VEC, int MB, int NB, int U>
 __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
     const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
-    int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt) {
-    constexpr bool kF32 = T::kBytes == 4;
-    constexpr int kRun = kF32 ? 16 : 32, kMine = kRun / 4;
+    int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt,
+    float* __restrict__ keep) {
+    constexpr int kMine = 16 / T::kBytes, kRun = 4 * kMine, kTok = 16 * NB;
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
-    const int64_t tok = col < n ? col : n - 1;
-    const int64_t want = target[tok];
-    const int64_t blocks = ceil_div(v, 16);
-    float m = -INFINITY, s = 0.0f;
-    for (int64_t blk = static_cast<int64_t>(blockIdx.x) * (kFewThreads / kWave) + wv; blk < blocks;
-         blk += static_cast<int64_t>(gridDim.x) * (kFewThreads / kWave)) {
-        int64_t row = blk * 16 + col;
-        if (row >= v) row = v - 1;
-        const int64_t wo = row * d, ho = tok * d;
-        f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-        auto step = [&](int64_t k, f32x4& c) {
-            float a[kMine], b[kMine];
-            const int64_t e = k + kMine * quarter;
-            if (VEC) {
+    int64_t want[NB], ho[NB];
+    float m[NB], s[NB];
 #pragma unroll
-                for (int j = 0; j < kMine; j += 4) {
-                    if (e + j < d) {
-                        T::load4(w, wo + e + j, &a[j]);
-                        T::load4(h, ho + e + j, &b[j]);
+    for (int b = 0; b < NB; ++b) {
+        const int64_t tok = 16 * b + col < n ? 16 * b + col : n - 1;
+        want[b] = 16 * b + col < n ? target[tok] : -1;
+        ho[b] = tok * d + kMine * quarter;
+        m[b] = -INFINITY;
+        s[b] = 0.0f;
+    }
+    const int64_t blocks = ceil_div(v, 16 * MB);
+    for (int64_t blk = static_cast<int64_t>(blockIdx.x) * kFewWaves + wv; blk < blocks;
+         blk += static_cast<int64_t>(gridDim.x) * kFewWaves) {
+        int64_t wo[MB];
+#pragma unroll
+        for (int a = 0; a < MB; ++a) {
+            const int64_t row = (blk * MB + a) * 16 + col;
+            wo[a] = (row < v ? row : v - 1) * d + kMine * quarter;
+        }
+        f32x4 acc[MB][NB];
+#pragma unroll
+        for (int a = 0; a < MB; ++a)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        FewPiece<T> x[U][MB], y[U][NB];
+        auto products = [&](int u) {
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if constexpr (kMine == 4) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[u][a][j], y[u][b][j],
+                                                                             acc[a][b], 0, 0, 0);
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) a[j + i] = b[j + i] = 0.0f;
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][a], y[u][b],
+                                                                            acc[a][b], 0, 0, 0);
                     }
                 }
-            } else {
+        };
+        auto runs = [&](int64_t k, auto end) {
 #pragma unroll
-                for (int j = 0; j < kMine; ++j) {
-                    a[j] = e + j < d ? T::load(w, wo + e + j) : 0.0f;
-                    b[j] = e + j < d ? T::load(h, ho + e + j) : 0.0f;
-                }
+            for (int u = 0; u < U; ++u) {
+                // past the row's end: its first piece, as zeros
+                const int64_t left = decltype(end)::value
+                                         ? d - k - u * kRun - kMine * quarter : kMine;
+                const int64_t at = left > 0 ? k + u * kRun : -kMine * quarter;
+#pragma unroll
+                for (int a = 0; a < MB; ++a) x[u][a] = few_piece<T, VEC>(w, wo[a] + at, left);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) y[u][b] = few_piece<T, VEC>(h, ho[b] + at, left);
             }
-            if constexpr (kF32) {
+            __builtin_amdgcn_sched_barrier(0);  // all loads before the first product's wait
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-            } else {
-                b16x8 x, y;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[j] = static_cast<__bf16>(a[j]);
-                    y[j] = static_cast<__bf16>(b[j]);
-                }
-                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
-            }
+            for (int u = 0; u < U; ++u) products(u);
         };
         int64_t k = 0;
-        for (; k + 8 * kRun <= d; k += 8 * kRun) {
-#pragma unroll
-            for (int u = 0; u < 8; ++u) step(k + u * kRun, acc[u & 1]);
-        }
-        for (; k < d; k += kRun) step(k, acc[0]);
+        for (; k + U * kRun <= d; k += U * kRun) runs(k, std::false_type{});
+        if (k < d) runs(k, std::true_type{});
         // lane l, register r: row 4 (l / 16) + r of the block, token l % 16
-        float z[4], top = m;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t vr = blk * 16 + 4 * quarter + r;
-            z[r] = (acc[0][r] + acc[1][r]) * kLog2e;
-            if (vr == want && col < n) zt[col] = z[r];
-            if (vr >= v) z[r] = -INFINITY;
-            top = fmaxf(top, z[r]);
+        for (int b = 0; b < NB; ++b) {
+            float top = m[b];
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t vr = (blk * MB + a) * 16 + 4 * quarter + r;
+                    float z = acc[a][b][r] * kLog2e;
+                    if (vr == want[b]) zt[16 * b + col] = z;
+                    if (keep != nullptr && vr < v) keep[vr * kTok + 16 * b + col] = z;
+                    if (vr >= v) z = -INFINITY;
+                    acc[a][b][r] = z;
+                    top = fmaxf(top, z);
+                }
+            const float base = top == -INFINITY ? 0.0f : top;
+            s[b] = m[b] == -INFINITY ? s[b] : s[b] * exp2_(m[b] - base);
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[b] += exp2_(acc[a][b][r] - base);
+            m[b] = top;
         }
-        const float base = top == -INFINITY ? 0.0f : top;
-        s = m == -INFINITY ? s : s * exp2_(m - base);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s += exp2_(z[r] - base);
-        m = top;
     }
     // the lanes of a token, then the waves
-    __shared__ float2 sh[kFewThreads / kWave][kFewTokens];
+    __shared__ float2 sh[kFewWaves][kTok];
 #pragma unroll
-    for (int o = 16; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
-        join(m, s, m2, s2);
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m[b], o), s2 = __shfl_xor(s[b], o);
+            join(m[b], s[b], m2, s2);
+        }
+        if (lane < 16) sh[wv][16 * b + lane] = make_float2(m[b], s[b]);
     }
-    if (lane < kFewTokens) sh[wv][lane] = make_float2(m, s);
     __syncthreads();
     if (threadIdx.x < n) {
-        m = sh[0][threadIdx.x].x;
-        s = sh[0][threadIdx.x].y;
-        for (int k = 1; k < kFewThreads / kWave; ++k) {
-            const float2 x = sh[k][threadIdx.x];
-            join(m, s, x.x, x.y);
-        }
-        part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = make_float2(m, s);
+        float2 x = sh[0][threadIdx.x];
+        for (int k = 1; k < kFewWaves; ++k) join(x.x, x.y, sh[k][threadIdx.x].x, sh[k][threadIdx.x].y);
+        part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = x;
     }
+}
+
+// Backward: dW = dlᵀ·h and dh = dl·W of a part of the vocabulary and 256
+// columns, 64 a wave, on the float32 matrix instructions (bfloat16 is widened).
+// For both products lane l holds columns 4 (l % 16) .. + 3 of row l / 16 of four,
+// sixteen bytes in float32: block i of an instruction's columns is the lanes'
+// i-th, so that rows of W are read and rows of dW written in runs of 256 bytes.
+// h stays in registers, as do the sums of dh; a part's dl is made from the
+// logits in LDS, 32 rows at a time, by all waves.
+constexpr int kFewRows = 32;  // rows of the vocabulary between barriers
+struct FewArgs {
+    const void *h, *w;
+    const int64_t* target;
+    const float* z;
+    const float2* norm;
+    const float* up;
+    int64_t n, d, v, ignore, per;  // per: rows of a part, a multiple of kFewRows
+    int reduction;
+    float* sums;     // dh: parts x n x d, NULL: not wanted
+    void* dw;        // NULL: not wanted
+    float* factor;   // left for the sums, with pos
+    int32_t* pos;
+};
+template <class T, bool VEC, int NB>
+__global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs p) {
+    constexpr int kTok = 16 * NB, kPitch = kTok + 1, kSub = kFewRows / 16;
+    __shared__ float dl[2][kFewRows * kPitch];
+    __shared__ float ms[kTok], gs[kTok], gg[kTok];
+    __shared__ int hit[kTok];
+    __shared__ float top_factor;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t v0 = blockIdx.y * p.per;
+    const int64_t v1 = v0 + p.per < p.v ? v0 + p.per : p.v;
+
+    if (wv == 0) {  // the tokens' upstream gradients over the largest of them
+        const bool in = lane < p.n;
+        const int64_t t = in ? p.target[lane] : p.ignore;
+        const bool live = in && t != p.ignore;
+        const int count = __popcll(__ballot(live));
+        float g = live ? 1.0f : 0.0f, f = 0.0f;
+        if (p.reduction != SLK_REDUCE_NONE) {
+            if (count > 0)
+                f = p.reduction == SLK_REDUCE_MEAN ? *p.up / static_cast<float>(count) : *p.up;
+        } else {
+            const float u = live ? p.up[lane] : 0.0f;
+            uint32_t m = __float_as_uint(u) & 0x7fffffffu;  // as bits, a NaN is the largest
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
+            f = __uint_as_float(m);
+            g = m == 0 ? 0.0f : u / f;
+        }
+        if (lane < kTok) {
+            const float2 x = live ? p.norm[lane] : make_float2(0.0f, 0.0f);
+            ms[lane] = x.x;
+            gs[lane] = g * x.y;
+            gg[lane] = g;
+            hit[lane] = live && t >= 0 && t < p.v ? static_cast<int>(t) : -1;
+        }
+        if (lane == 0) top_factor = f;
+        if (blockIdx.x == 0 && blockIdx.y == 0) {
+            if (in) p.pos[lane] = live ? lane : -1;
+            if (lane == 0) *p.factor = f;
+        }
+    }
+    __syncthreads();
+    const float factor = top_factor;
+
+    const int col = lane & 15, quarter = lane >> 4;
+    const int64_t c0 = blockIdx.x * 256 + 64 * wv + 4 * col;
+    auto load = [&](const void* from, int64_t row, f32x4& x) {
+        x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (VEC) {
+            if (c0 < p.d) {
+                float y[4];
+                T::load4(from, row * p.d + c0, y);
+                x = f32x4{y[0], y[1], y[2], y[3]};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c0 + i < p.d) x[i] = T::load(from, row * p.d + c0 + i);
+        }
+    };
+    f32x4 hv[4 * NB];  // token 4 j + l / 16; an ignored token's is 0, whatever it holds
+#pragma unroll
+    for (int j = 0; j < 4 * NB; ++j) {
+        const int tok = 4 * j + quarter;
+        hv[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.dw != nullptr && tok < p.n && p.target[tok] != p.ignore) load(p.h, tok, hv[j]);
+    }
+    f32x4 dh[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dh[b][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    f32x4 x[kSub][4];  // W's row 16 k + 4 j + l / 16
+    auto rows = [&](int64_t r0) {
+        if (p.sums == nullptr) return;
+#pragma unroll
+        for (int k = 0; k < kSub; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t r = r0 + 16 * k + 4 * j + quarter;
+                load(p.w, r < v1 ? r : v1 - 1, x[k][j]);
+            }
+    };
+    float zs[kFewRows * kTok / kFewThreads];
+    auto logits = [&](int64_t r0) {
+#pragma unroll
+        for (int k = 0; k < kFewRows * kTok / kFewThreads; ++k) {
+            const int at = k * kFewThreads + threadIdx.x;
+            zs[k] = r0 + at / kTok < v1 ? p.z[r0 * kTok + at] : 0.0f;
+        }
+    };
+    logits(v0);
+    int buf = 0;
+    for (int64_t r0 = v0; r0 < v1; r0 += kFewRows, buf ^= 1) {
+        rows(r0);
+#pragma unroll
+        for (int k = 0; k < kFewRows * kTok / kFewThreads; ++k) {
+            const int at = k * kFewThreads + threadIdx.x, row = at / kTok, tok = at % kTok;
+            float g = exp2_(zs[k] - ms[tok]) * gs[tok];
+            if (r0 + row == hit[tok]) g -= gg[tok];
+            dl[buf][row * kPitch + tok] = r0 + row < v1 && tok < p.n && gg[tok] != 0.0f ? g : 0.0f;
+        }
+        if (r0 + kFewRows < v1) logits(r0 + kFewRows);
+        __syncthreads();  // (the buffer was read two rounds ago, a barrier ago)
+        if (c0 - 4 * col >= p.d) continue;  // the whole wave: no column of its own
+#pragma unroll
+        for (int k = 0; k < kSub; ++k) {
+            const float* mine = dl[buf] + 16 * k * kPitch;
+            if (p.dw != nullptr) {
+                f32x4 acc[4] = {};
+#pragma unroll
+                for (int j = 0; j < 4 * NB; ++j) {
+                    const float a = mine[col * kPitch + 4 * j + quarter];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, hv[j][i], acc[i], 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t row = r0 + 16 * k + 4 * quarter + r;
+                    if (row >= v1) continue;
+                    float y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = acc[i][r] * factor;
+                    if (VEC) {
+                        if (c0 < p.d) T::store4(p.dw, row * p.d + c0, y);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (c0 + i < p.d) T::store(p.dw, row * p.d + c0 + i, y[i]);
+                    }
+                }
+            }
+            if (p.sums != nullptr) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float a = mine[(4 * j + quarter) * kPitch + 16 * b + col];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            dh[b][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[k][j][i],
+                                                                            dh[b][i], 0, 0, 0);
+                    }
+            }
+        }
+    }
+    if (p.sums == nullptr) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t tok = 16 * b + 4 * quarter + r;
+            if (tok >= p.n) continue;
+            float* to = p.sums + (blockIdx.y * p.n + tok) * p.d + c0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c0 + i < p.d) to[i] = dh[b][i][r];
+        }
 }
 
 // ───────────────────────────── sizes ─────────────────────────────
@@ -792,17 +1029,29 @@ struct Carve {
 };
 
 struct Saved {
-    int64_t header, rows, pos, tgt, norm, h, w, bytes;
+    int64_t header, rows, pos, tgt, norm, h, w, z, bytes;
 };
 
 bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
 int64_t stages(const slk_linear_ce* a, int64_t k) { return ceil_div(k, split_of(a) ? 32 : 64); }
 
-bool few(const slk_linear_ce* a) { return a->n <= kFewTokens && !a->keep; }
+bool few(const slk_linear_ce* a) {
+    return a->n <= (!a->keep ? kFewScores : split_of(a) ? kFewTokens<F32> : kFewTokens<BF16>);
+}
+// 16-token blocks of the few tokens' kernels: 1, 2, 4 or 8
+int64_t few_blocks(const slk_linear_ce* a) {
+    return a->n <= 16 ? 1 : a->n <= 32 ? 2 : a->n <= 64 ? 4 : 8;
+}
 
 Saved saved_of(const slk_linear_ce* a) {
-    Saved s;
+    Saved s{};
     Carve c;
+    if (few(a)) {  // the logits themselves: 4 bytes each, where W has 4 d / n for one
+        s.norm = c.take(8 * a->n);
+        s.z = c.take(a->v * few_blocks(a) * 64);
+        s.bytes = a->keep ? c.at : 0;
+        return s;
+    }
     s.header = c.take(sizeof(Header));
     s.rows = c.take(4 * a->n);
     s.pos = c.take(4 * a->n);
@@ -810,15 +1059,15 @@ Saved saved_of(const slk_linear_ce* a) {
     s.norm = c.take(8 * a->n);
     s.h = c.take(stages(a, a->d) * up64(a->n) * kStageBytes);
     s.w = c.take(stages(a, a->d) * up64(a->v) * kStageBytes);
-    s.bytes = few(a) ? 0 : c.at;
+    s.bytes = c.at;
     return s;
 }
 
-constexpr int64_t kFewGroups = 512;  // workgroups of ce_few_kernel at most
+constexpr int64_t kFewGroups = 2048;  // workgroups of ce_few_kernel at most
 
 int64_t parts_of(const slk_linear_ce* a) {
     if (few(a)) {
-        const int64_t g = ceil_div(ceil_div(a->v, 16), kFewThreads / kWave);
+        const int64_t g = ceil_div(ceil_div(a->v, few_blocks(a) > 1 ? 32 : 16), kFewWaves);
         return g < kFewGroups ? g : kFewGroups;
     }
     return ceil_div(a->v, kTileM);
@@ -866,10 +1115,22 @@ int splits_for(int64_t m, int64_t n, int64_t nst) {
 struct Backward {
     int64_t piece;  // rows of a piece, a multiple of kTileM
     int sh, sw;     // parts of the two products
-    int64_t gr, factor, dl, dl_rows, dh, dw, bytes;
+    int64_t gr, factor, pos, dl, dl_rows, dh, dw, bytes;
 };
 Backward backward_of(const slk_linear_ce* a) {
-    Backward b;
+    Backward b{};
+    if (few(a)) {
+        // parts of the vocabulary: two workgroups a CU over all columns
+        const int64_t cols = ceil_div(a->d, 256), most = ceil_div(512, cols);
+        b.piece = ceil_div(ceil_div(a->v, most), kFewRows) * kFewRows;
+        b.sh = static_cast<int>(ceil_div(a->v, b.piece));
+        Carve c;
+        b.factor = c.take(4);
+        b.pos = c.take(4 * a->n);
+        b.dh = c.take(a->dhidden != nullptr ? 4 * b.sh * a->n * a->d : 0);
+        b.bytes = c.at;
+        return b;
+    }
     // (the epilogue writes whole tiles of tokens)
     b.dl_rows = ceil_div(a->n, kWideN) * kWideN;
     const int64_t per_row = b.dl_rows * (split_of(a) ? 4 : 2);
@@ -951,15 +1212,36 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
                a->ignore_index, parts_of(a)};
     int rc = SLK_OK;
     if (few(a)) {
-        const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 4 * T::kBytes) &&
-                         aligned_to(a->weight, 4 * T::kBytes);
+        const bool vec = a->d % (16 / T::kBytes) == 0 && aligned_to(a->hidden, 16) &&
+                         aligned_to(a->weight, 16);
+        char* sv = static_cast<char*>(a->saved);
+        float* z = nullptr;
+        if (a->keep) {
+            z = reinterpret_cast<float*>(sv + saved_of(a).z);
+            j.norm = reinterpret_cast<float2*>(sv + saved_of(a).norm);
+        }
         const dim3 grid(static_cast<unsigned>(parts_of(a)));
         auto go = [&](auto k) {
             hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target,
-                               a->n, a->d, a->v, part, zt);
+                               a->n, a->d, a->v, part, zt, z);
         };
-        if (vec) go(ce_few_kernel<T, true>);
-        else go(ce_few_kernel<T, false>);
+        switch (few_blocks(a)) {
+            case 1:
+                vec ? go(ce_few_kernel<T, true, 1, 1, 8>)
+                    : go(ce_few_kernel<T, false, 1, 1, 8>);
+                break;
+            case 2:
+                vec ? go(ce_few_kernel<T, true, 2, 2, 4>)
+                    : go(ce_few_kernel<T, false, 2, 2, 4>);
+                break;
+            case 4:
+                vec ? go(ce_few_kernel<T, true, 2, 4, 2>)
+                    : go(ce_few_kernel<T, false, 2, 4, 2>);
+                break;
+            default:
+                vec ? go(ce_few_kernel<T, true, 2, 8, 2>)
+                    : go(ce_few_kernel<T, false, 2, 8, 2>);
+        }
         rc = check_launch("linear_ce few");
     } else {
         const Saved s = saved_of(a);
@@ -1012,8 +1294,47 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
     return rc;
 }
 
+template <class T>
+int backward_few(const slk_linear_ce* a, hipStream_t st) {
+    const Saved s = saved_of(a);
+    const Backward b = backward_of(a);
+    const char* sv = static_cast<const char*>(a->saved);
+    char* sc = static_cast<char*>(a->scratch);
+    float* sums = a->dhidden != nullptr ? reinterpret_cast<float*>(sc + b.dh) : nullptr;
+    float* factor = reinterpret_cast<float*>(sc + b.factor);
+    int32_t* pos = reinterpret_cast<int32_t*>(sc + b.pos);
+    const FewArgs p{a->hidden, a->weight, a->target, reinterpret_cast<const float*>(sv + s.z),
+                    reinterpret_cast<const float2*>(sv + s.norm), a->upstream, a->n, a->d, a->v,
+                    a->ignore_index, b.piece, a->reduction, sums, a->dweight, factor, pos};
+    if (sums == nullptr && a->dweight == nullptr) return SLK_OK;
+    const dim3 grid(static_cast<unsigned>(ceil_div(a->d, 256)), static_cast<unsigned>(b.sh));
+    const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 4 * T::kBytes) &&
+                     aligned_to(a->weight, 4 * T::kBytes) &&
+                     aligned_to(a->dweight, 4 * T::kBytes);
+    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, p); };
+    switch (few_blocks(a)) {
+        case 1:
+            vec ? go(ce_few_back_kernel<T, true, 1>) : go(ce_few_back_kernel<T, false, 1>);
+            break;
+        case 2:
+            vec ? go(ce_few_back_kernel<T, true, 2>) : go(ce_few_back_kernel<T, false, 2>);
+            break;
+        default:
+            if constexpr (kFewTokens<T> > 32)
+                vec ? go(ce_few_back_kernel<T, true, 4>) : go(ce_few_back_kernel<T, false, 4>);
+    }
+    int rc = check_launch("linear_ce few backward");
+    if (rc != SLK_OK || sums == nullptr) return rc;
+    const int64_t g = ceil_div(a->n * a->d, 256);
+    hipLaunchKernelGGL((ce_finish_kernel<T, false>),
+                       dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st, sums,
+                       b.sh, a->n, a->n, a->d, pos, nullptr, factor, false, a->dhidden);
+    return check_launch("linear_ce finish");
+}
+
 template <class T, bool SPLIT>
 int backward(const slk_linear_ce* a, hipStream_t st) {
+    if (few(a)) return backward_few<T>(a, st);
     const Saved s = saved_of(a);
     const Backward b = backward_of(a);
     char* sv = static_cast<char*>(a->saved);
@@ -1124,6 +1445,9 @@ extern "C" int slk_linear_ce_backward(const slk_linear_ce* a, void* stream) {
     if (a->scratch_bytes < backward_of(a).bytes || a->saved_bytes < saved_of(a).bytes ||
         a->scratch == nullptr || a->saved == nullptr) {
         return fail(SLK_EINVAL, "linear_ce_backward: saved or scratch too small");
+    }
+    if (few(a) && (a->hidden == nullptr || a->weight == nullptr || a->target == nullptr)) {
+        return fail(SLK_EINVAL, "linear_ce_backward: NULL hidden, weight or target");
     }
     return a->dtype == SLK_F32 ? backward<F32, true>(a, as_stream(stream))
                                : backward<BF16, false>(a, as_stream(stream));

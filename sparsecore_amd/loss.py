@@ -3,7 +3,8 @@
     z = hidden · weightᵀ,    loss = logsumexp(z) - z[target]
 
 without storing the logits: forward keeps a maximum and a sum of each token, backward
-computes the logits again a piece of the vocabulary at a time (``slk_linear_ce_*``).
+computes the logits again a piece of the vocabulary at a time (``slk_linear_ce_*``). Only
+those of a few tokens, far smaller than the head, are kept.
 """
 
 from __future__ import annotations
@@ -42,14 +43,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
             with _lib.on_device(h):
                 _lib.linear_ce_forward(args, _lib.stream_of(h))
         if keep:
-            ctx.save_for_backward(saved)
+            ctx.save_for_backward(saved, h, w, t)
             ctx.rest = (n, d, v, ignore_index, reduction, hidden.shape, hidden.dtype)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        saved, = ctx.saved_tensors
+        saved, h, w, t = ctx.saved_tensors
         n, d, v, ignore_index, reduction, shape, dtype = ctx.rest
         dev = grad.device
         dh = torch.empty(shape, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
@@ -59,8 +60,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if n:
             p = _lib.ptr
             up = grad.contiguous()
-            args = _lib.LinearCE(n=n, d=d, v=v, ignore_index=ignore_index, upstream=p(up),
-                                 dhidden=p(dh), dweight=p(dw), saved=p(saved),
+            args = _lib.LinearCE(n=n, d=d, v=v, ignore_index=ignore_index, hidden=p(h),
+                                 weight=p(w), target=p(t), upstream=p(up), dhidden=p(dh), dweight=p(dw), saved=p(saved),
                                  saved_bytes=saved.numel(), dtype=_lib.DTYPES[dtype],
                                  reduction=_lib.REDUCTIONS[reduction], keep=1)
             args.scratch_bytes = _lib.linear_ce_scratch_bytes(args, True)
@@ -86,8 +87,10 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
 
     Returns the float32 loss, with gradients for hidden and weight. float32 products are
     about as exact as float32 matrix products; bfloat16 gradients pass through logit
-    gradients rounded to bfloat16. A forward that a backward may follow keeps about twice
-    weight and hidden in a packed form until then. Results repeat bit for bit.
+    gradients rounded to bfloat16 (not those of few tokens). A forward that a backward may
+    follow keeps weight and hidden once more, packed, until then; of few tokens (at most
+    64, 32 in bfloat16) their logits instead. hidden, weight and target must not change in
+    place before the backward. Results repeat bit for bit.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, reduction).

@@ -401,3 +401,89 @@ def test_captured_loss_and_gradients_replay(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, once()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [2, 16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("d,v", [(4, 31), (63, 32), (64, 33), (257, 500), (520, 3001)])
+def test_gradients_of_few_tokens(dev, dtype, n, d, v):
+    check(dev, n, d, v, dtype, 0.2, "mean" if n % 2 else "none")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [32, 33, 64, 100, 128, 129])
+@pytest.mark.parametrize("d,v", [(72, 100), (100, 3001), (1030, 70)])
+def test_scores_of_some_tokens(dev, dtype, n, d, v):
+    h, w, t = make(n, d, v, dtype, dev, 20, 0.2)
+    losses, err, *_ = reference(h, w, t, torch.zeros(n, device=dev))
+    within(slk.linear_cross_entropy(h, w, t, reduction="none"), losses, err, "loss")
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 30.0, 1e4])
+def test_ranges_of_float32_few_tokens(dev, scale):
+    check(dev, 30, 64, 200, torch.float32, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_few_ignored_tokens_reach_nothing(dev, dtype, bad):
+    h, w, t = make(25, 64, 100, dtype, dev, 21)
+    clean = torch.where(torch.arange(25, device=dev)[:, None] % 3 == 0, 0, h)
+    t[::3] = -100
+    grads = []
+    for x in (torch.where(torch.arange(25, device=dev)[:, None] % 3 == 0, bad, h), clean):
+        x, y = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = slk.linear_cross_entropy(x, y, t)
+        grads.append((loss.detach(), *torch.autograd.grad(loss, [x, y])))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    assert bool((grads[0][1][::3] == 0).all()) and bool(torch.isfinite(grads[0][2]).all())
+
+
+def test_few_tokens_one_gradient_alone_alignment_and_targets(dev):
+    h, w, t = make(40, 64, 300, torch.float32, dev, 22)
+    t[3], t[9] = 300, -5  # no rows of the vocabulary
+
+    def grads(h, w):
+        want = [x for x in (h, w) if x.requires_grad]
+        return torch.autograd.grad(slk.linear_cross_entropy(h, w, t), want)
+
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    both = grads(hg, wg)
+    assert torch.equal(grads(hg, w)[0], both[0]) and torch.equal(grads(h, wg)[0], both[1])
+    assert bool(torch.isfinite(both[0]).all()) and bool(torch.isfinite(both[1]).all())
+    odd = torch.empty(h.numel() + 1, device=dev)[1:].view_as(h).copy_(h).requires_grad_()
+    torch.testing.assert_close(grads(odd, w)[0], both[0], rtol=1e-5, atol=1e-7)
+
+
+def test_few_tokens_refuse_a_weight_that_changed(dev):
+    """Their backward reads weight itself, so autograd must hold its version."""
+    h, w, t = make(8, 64, 100, torch.float32, dev, 23)
+    h.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t)
+    w.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+
+
+def test_captured_few_tokens_replay(dev):
+    h, w, t = make(20, 64, 500, torch.float32, dev, 24, 0.2)
+    h.requires_grad_(), w.requires_grad_()
+
+    def once():
+        loss = slk.linear_cross_entropy(h, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, w]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    for k in range(4):
+        with torch.no_grad():
+            h.copy_(torch.randn(20, 64, generator=torch.Generator().manual_seed(k)))
+            t.copy_(torch.randint(0, 500, (20,), generator=torch.Generator().manual_seed(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, once()))
