@@ -571,6 +571,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
 __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ losses,
                                                          const int64_t* __restrict__ target,
                                                          int64_t n, int64_t ignore, bool mean,
+                                                         float* __restrict__ live,
                                                          float* __restrict__ out) {
     __shared__ double sh[2][1024 / kWave];
     double s = 0.0, c = 0.0;
@@ -594,6 +595,7 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
             c += sh[1][w];
         }
         *out = static_cast<float>(mean ? s / c : s);  // no live token: 0 / 0
+        if (live != nullptr) *live = static_cast<float>(c);
     }
 }
 
@@ -712,17 +714,73 @@ __device__ __forceinline__ FewPiece<T> few_piece(const void* p, int64_t i, int64
     return x;
 }
 
-// Forward. A wave takes 16 MB rows of W at a time against 16 NB tokens (fewer
-// are repeated): lane l holds row l % 16 of both, piece l / 16 of each run of 64
-// bytes. The same columns meet in both operands, so their order within an
-// instruction does not matter. The loads of U runs are in flight together. z is
-// kept for the backward where it is wanted, 16 NB tokens a row.
+// 16 MB rows of one operand (block blk of them; past the end the last again)
+// against 16 NB of the other (few): lane l holds row l % 16 of both, piece l / 16
+// of each run of 64 bytes. The same columns meet in both operands, so their order
+// within an instruction does not matter. The loads of U runs are in flight
+// together. Lane l, register r of acc[a][b]: row 16 a + 4 (l / 16) + r, few
+// 16 b + l % 16. Columns k .. k1, whole times U runs but where k1 is d.
+template <class T, bool VEC, int MB, int NB, int U>
+__device__ __forceinline__ void few_products(const void* __restrict__ rows, int64_t nrows,
+                                             int64_t blk, const void* __restrict__ few,
+                                             const int64_t (&fo)[NB], int64_t d, int64_t k,
+                                             int64_t k1, int lane, f32x4 (&acc)[MB][NB]) {
+    constexpr int kMine = 16 / T::kBytes, kRun = 4 * kMine;
+    const int quarter = lane >> 4;
+    int64_t ro[MB];
+#pragma unroll
+    for (int a = 0; a < MB; ++a) {
+        const int64_t row = (blk * MB + a) * 16 + (lane & 15);
+        ro[a] = (row < nrows ? row : nrows - 1) * d + kMine * quarter;
+    }
+#pragma unroll
+    for (int a = 0; a < MB; ++a)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    FewPiece<T> x[U][MB], y[U][NB];
+    auto runs = [&](int64_t k, auto end) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // past the row's end: its first piece, as zeros
+            const int64_t left =
+                decltype(end)::value ? d - k - u * kRun - kMine * quarter : kMine;
+            const int64_t at = left > 0 ? k + u * kRun : -kMine * quarter;
+#pragma unroll
+            for (int a = 0; a < MB; ++a) x[u][a] = few_piece<T, VEC>(rows, ro[a] + at, left);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) y[u][b] = few_piece<T, VEC>(few, fo[b] + at, left);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all loads before the first product's wait
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if constexpr (kMine == 4) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                x[u][a][j], y[u][b][j], acc[a][b], 0, 0, 0);
+                    } else {
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][a], y[u][b],
+                                                                            acc[a][b], 0, 0, 0);
+                    }
+                }
+    };
+    for (; k + U * kRun <= k1; k += U * kRun) runs(k, std::false_type{});
+    if (k < k1) runs(k, std::true_type{});
+}
+
+// Forward of few tokens: a wave takes 16 MB rows of W at a time against all
+// tokens (the last is repeated). z is kept for the backward where it is wanted,
+// 16 NB tokens a row.
 template <class T, bool VEC, int MB, int NB, int U>
 __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
     const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
     int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt,
     float* __restrict__ keep) {
-    constexpr int kMine = 16 / T::kBytes, kRun = 4 * kMine, kTok = 16 * NB;
+    constexpr int kMine = 16 / T::kBytes, kTok = 16 * NB;
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
@@ -739,54 +797,8 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
     const int64_t blocks = ceil_div(v, 16 * MB);
     for (int64_t blk = static_cast<int64_t>(blockIdx.x) * kFewWaves + wv; blk < blocks;
          blk += static_cast<int64_t>(gridDim.x) * kFewWaves) {
-        int64_t wo[MB];
-#pragma unroll
-        for (int a = 0; a < MB; ++a) {
-            const int64_t row = (blk * MB + a) * 16 + col;
-            wo[a] = (row < v ? row : v - 1) * d + kMine * quarter;
-        }
         f32x4 acc[MB][NB];
-#pragma unroll
-        for (int a = 0; a < MB; ++a)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        FewPiece<T> x[U][MB], y[U][NB];
-        auto products = [&](int u) {
-#pragma unroll
-            for (int a = 0; a < MB; ++a)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if constexpr (kMine == 4) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[u][a][j], y[u][b][j],
-                                                                             acc[a][b], 0, 0, 0);
-                    } else {
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][a], y[u][b],
-                                                                            acc[a][b], 0, 0, 0);
-                    }
-                }
-        };
-        auto runs = [&](int64_t k, auto end) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                // past the row's end: its first piece, as zeros
-                const int64_t left = decltype(end)::value
-                                         ? d - k - u * kRun - kMine * quarter : kMine;
-                const int64_t at = left > 0 ? k + u * kRun : -kMine * quarter;
-#pragma unroll
-                for (int a = 0; a < MB; ++a) x[u][a] = few_piece<T, VEC>(w, wo[a] + at, left);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) y[u][b] = few_piece<T, VEC>(h, ho[b] + at, left);
-            }
-            __builtin_amdgcn_sched_barrier(0);  // all loads before the first product's wait
-#pragma unroll
-            for (int u = 0; u < U; ++u) products(u);
-        };
-        int64_t k = 0;
-        for (; k + U * kRun <= d; k += U * kRun) runs(k, std::false_type{});
-        if (k < d) runs(k, std::true_type{});
-        // lane l, register r: row 4 (l / 16) + r of the block, token l % 16
+        few_products<T, VEC, MB, NB, U>(w, v, blk, h, ho, d, 0, d, lane, acc);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float top = m[b];
@@ -825,50 +837,147 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
     __syncthreads();
     if (threadIdx.x < n) {
         float2 x = sh[0][threadIdx.x];
-        for (int k = 1; k < kFewWaves; ++k) join(x.x, x.y, sh[k][threadIdx.x].x, sh[k][threadIdx.x].y);
+        for (int k = 1; k < kFewWaves; ++k)
+            join(x.x, x.y, sh[k][threadIdx.x].x, sh[k][threadIdx.x].y);
         part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = x;
     }
 }
 
-// Backward: dW = dlᵀ·h and dh = dl·W of a part of the vocabulary and 256
-// columns, 64 a wave, on the float32 matrix instructions (bfloat16 is widened).
-// For both products lane l holds columns 4 (l % 16) .. + 3 of row l / 16 of four,
-// sixteen bytes in float32: block i of an instruction's columns is the lanes'
-// i-th, so that rows of W are read and rows of dW written in runs of 256 bytes.
-// h stays in registers, as do the sums of dh; a part's dl is made from the
-// logits in LDS, 32 rows at a time, by all waves.
-constexpr int kFewRows = 32;  // rows of the vocabulary between barriers
+// Forward of a small vocabulary, the same with the operands' parts exchanged: a
+// workgroup has all logits of 16 tokens, so their softmax and loss too. Its waves
+// take a quarter of the columns each (a wave for all of them left the card's
+// vector units half empty: 8192 x 4096 x 65 float32 took 187 us) and then, of the
+// joined logits, the tokens that are theirs modulo 4.
+template <class T, bool VEC, int NB, int U>
+__global__ __launch_bounds__(kFewThreads) void ce_small_kernel(
+    const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
+    int64_t n, int64_t d, int64_t v, int64_t ignore, float* __restrict__ losses,
+    float2* __restrict__ norm, float* __restrict__ keep) {
+    constexpr int kMine = 16 / T::kBytes, kVoc = 16 * NB, kStep = U * 4 * kMine;
+    __shared__ float sh[kFewWaves][NB][4][kWave];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int64_t steps = ceil_div(d, kStep);
+    const int64_t k0 = steps * wv / kFewWaves * kStep, ke = steps * (wv + 1) / kFewWaves * kStep;
+    const int64_t k1 = ke < d ? ke : d;
+    int64_t wo[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+        wo[b] = (16 * b + col < v ? 16 * b + col : v - 1) * d + kMine * quarter;
+    const int64_t blocks = ceil_div(n, 16);
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        f32x4 acc[1][NB];
+        few_products<T, VEC, 1, NB, U>(h, n, blk, w, wo, d, k0, k1, lane, acc);
+        __syncthreads();  // the last block's logits are read
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sh[wv][b][r][lane] = acc[0][b][r];
+        __syncthreads();
+        const int64_t tok = blk * 16 + 4 * quarter + wv;
+        const int64_t t = tok < n ? target[tok] : ignore;
+        float m = -INFINITY, s = 0.0f, zt = 0.0f, zs[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float z = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kFewWaves; ++k) z += sh[k][b][wv][lane];
+            z *= kLog2e;
+            if (keep != nullptr && tok < n) keep[tok * kVoc + 16 * b + col] = z;
+            if (16 * b + col == t) zt = z;
+            zs[b] = 16 * b + col < v ? z : -INFINITY;
+            m = fmaxf(m, zs[b]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (m == -INFINITY) m = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) s += exp2_(zs[b] - m);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            s += __shfl_xor(s, o);
+            zt += __shfl_xor(zt, o);
+        }
+        if (col != 0 || tok >= n) continue;
+        const bool valid = t >= 0 && t < v;
+        losses[tok] = t == ignore ? 0.0f : valid ? ((m - zt) + log2f(s)) * kLn2 : NAN;
+        if (norm != nullptr) norm[tok] = make_float2(m, 1.0f / s);
+    }
+}
+
+// Backward of both. Rows are those of the long operand (W of few tokens, the
+// hidden states of a small vocabulary), few those of the other; both products,
+//   d rows = dl·few,   d few = dlᵀ·rows     (dl rows x few),
+// of a part of the rows and 256 columns, 64 a wave, on the float32 matrix
+// instructions (bfloat16 is widened). Lane l holds columns 4 (l % 16) .. + 3 of
+// row l / 16 of four, sixteen bytes in float32: block i of an instruction's
+// columns is the lanes' i-th, so that rows are read and written in runs of 256
+// bytes. The few stay in registers, as do their sums; dl is made from the logits
+// in LDS, 32 rows at a time, by all waves. An ignored token's row or place in dl
+// is 0, and so is what is read of its hidden state, whatever it holds.
+constexpr int kFewRows = 32;  // rows between barriers
 struct FewArgs {
-    const void *h, *w;
+    const void *few, *rows;
     const int64_t* target;
-    const float* z;
-    const float2* norm;
+    const float* z;       // rows x 16 NB
+    const float2* norm;   // of the tokens
     const float* up;
-    int64_t n, d, v, ignore, per;  // per: rows of a part, a multiple of kFewRows
+    const float* live;    // small vocabulary: the tokens not ignored
+    int64_t nfew, nrows, d, ignore, per;  // per: rows of a part, a multiple of kFewRows
     int reduction;
-    float* sums;     // dh: parts x n x d, NULL: not wanted
-    void* dw;        // NULL: not wanted
-    float* factor;   // left for the sums, with pos
+    float* sums;     // d few: parts x nfew x d, NULL: not wanted
+    void* drows;     // NULL: not wanted
+    float* factor;   // left for the sums, with pos (few tokens)
     int32_t* pos;
 };
-template <class T, bool VEC, int NB>
+// What a token's column (few tokens) or row (small vocabulary) of dl takes:
+// p = exp2(z - m)·gs, less g at hit. gs = g / s; hit -1: none, -2: ignored.
+struct FewToken {
+    float m, gs, g;
+    int hit;
+};
+template <class T, bool VEC, int NB, bool SMALL>
 __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs p) {
-    constexpr int kTok = 16 * NB, kPitch = kTok + 1, kSub = kFewRows / 16;
+    constexpr int kFew = 16 * NB, kPitch = kFew + 1, kSub = kFewRows / 16;
+    constexpr int kEach = kFewRows * kFew / kFewThreads;
     __shared__ float dl[2][kFewRows * kPitch];
-    __shared__ float ms[kTok], gs[kTok], gg[kTok];
-    __shared__ int hit[kTok];
+    __shared__ FewToken tokens[SMALL ? 3 * kFewRows : kFew];  // (SMALL: of three rounds)
     __shared__ float top_factor;
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t v0 = blockIdx.y * p.per;
-    const int64_t v1 = v0 + p.per < p.v ? v0 + p.per : p.v;
+    const int64_t r_0 = blockIdx.y * p.per;
+    const int64_t r_1 = r_0 + p.per < p.nrows ? r_0 + p.per : p.nrows;
+    const int64_t classes = SMALL ? p.nfew : p.nrows;
 
-    if (wv == 0) {  // the tokens' upstream gradients over the largest of them
-        const bool in = lane < p.n;
+    auto token = [&](int64_t i, bool live, int64_t t, float g) {
+        const float2 x = live ? p.norm[i] : make_float2(0.0f, 0.0f);
+        return FewToken{x.x, live ? g * x.y : 0.0f, live ? g : 0.0f,
+                        !live ? -2 : t >= 0 && t < classes ? static_cast<int>(t) : -1};
+    };
+    // SMALL: row r0 + threadIdx.x of the next round, of the first 32 threads
+    auto row_token = [&](int64_t r0) {
+        const int64_t i = r0 + threadIdx.x;
+        const bool in = threadIdx.x < kFewRows && i < r_1;
+        const int64_t t = in ? p.target[i] : p.ignore;
+        const bool live = t != p.ignore;
+        return token(i, live, t, live && p.reduction == SLK_REDUCE_NONE ? p.up[i] : 1.0f);
+    };
+    if constexpr (SMALL) {
+        if (threadIdx.x < kFewRows) tokens[threadIdx.x] = row_token(r_0);
+        if (threadIdx.x == 0) {
+            float f = 1.0f;
+            if (p.reduction == SLK_REDUCE_SUM) f = *p.up;
+            if (p.reduction == SLK_REDUCE_MEAN) f = *p.live > 0.0f ? *p.up / *p.live : 0.0f;
+            top_factor = f;
+            if (blockIdx.x == 0 && blockIdx.y == 0) *p.factor = f;
+        }
+    } else if (wv == 0) {  // the tokens' upstream gradients over the largest of them
+        const bool in = lane < p.nfew;
         const int64_t t = in ? p.target[lane] : p.ignore;
         const bool live = in && t != p.ignore;
         const int count = __popcll(__ballot(live));
-        float g = live ? 1.0f : 0.0f, f = 0.0f;
+        float g = 1.0f, f = 0.0f;
         if (p.reduction != SLK_REDUCE_NONE) {
             if (count > 0)
                 f = p.reduction == SLK_REDUCE_MEAN ? *p.up / static_cast<float>(count) : *p.up;
@@ -880,13 +989,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
             f = __uint_as_float(m);
             g = m == 0 ? 0.0f : u / f;
         }
-        if (lane < kTok) {
-            const float2 x = live ? p.norm[lane] : make_float2(0.0f, 0.0f);
-            ms[lane] = x.x;
-            gs[lane] = g * x.y;
-            gg[lane] = g;
-            hit[lane] = live && t >= 0 && t < p.v ? static_cast<int>(t) : -1;
-        }
+        if (lane < kFew) tokens[lane] = token(lane, live, t, g);
         if (lane == 0) top_factor = f;
         if (blockIdx.x == 0 && blockIdx.y == 0) {
             if (in) p.pos[lane] = live ? lane : -1;
@@ -912,77 +1015,89 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
                 if (c0 + i < p.d) x[i] = T::load(from, row * p.d + c0 + i);
         }
     };
-    f32x4 hv[4 * NB];  // token 4 j + l / 16; an ignored token's is 0, whatever it holds
+    f32x4 few[4 * NB];  // row 4 j + l / 16
 #pragma unroll
     for (int j = 0; j < 4 * NB; ++j) {
-        const int tok = 4 * j + quarter;
-        hv[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (p.dw != nullptr && tok < p.n && p.target[tok] != p.ignore) load(p.h, tok, hv[j]);
+        const int i = 4 * j + quarter;
+        few[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.drows != nullptr && i < p.nfew && (SMALL || tokens[SMALL ? 0 : i].hit != -2))
+            load(p.few, i, few[j]);
     }
-    f32x4 dh[NB][4];
+    f32x4 sum[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dh[b][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 4; ++i) sum[b][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    f32x4 x[kSub][4];  // W's row 16 k + 4 j + l / 16
-    auto rows = [&](int64_t r0) {
-        if (p.sums == nullptr) return;
-#pragma unroll
-        for (int k = 0; k < kSub; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t r = r0 + 16 * k + 4 * j + quarter;
-                load(p.w, r < v1 ? r : v1 - 1, x[k][j]);
-            }
-    };
-    float zs[kFewRows * kTok / kFewThreads];
+    f32x4 x[kSub][4];  // row 16 k + 4 j + l / 16
+    float zs[kEach];
     auto logits = [&](int64_t r0) {
 #pragma unroll
-        for (int k = 0; k < kFewRows * kTok / kFewThreads; ++k) {
+        for (int k = 0; k < kEach; ++k) {
             const int at = k * kFewThreads + threadIdx.x;
-            zs[k] = r0 + at / kTok < v1 ? p.z[r0 * kTok + at] : 0.0f;
+            zs[k] = r0 + at / kFew < r_1 ? p.z[r0 * kFew + at] : 0.0f;
         }
     };
-    logits(v0);
-    int buf = 0;
-    for (int64_t r0 = v0; r0 < v1; r0 += kFewRows, buf ^= 1) {
-        rows(r0);
+    logits(r_0);
+    // dl of two rounds, tokens of three: a round's tokens are read until the next
+    // round's barrier, when those of the round after are written
+    int buf = 0, turn = 0;
+    for (int64_t r0 = r_0; r0 < r_1; r0 += kFewRows, buf ^= 1) {
+        const FewToken* mine_tokens = tokens + (SMALL ? turn * kFewRows : 0);
+        turn = turn == 2 ? 0 : turn + 1;
+        if (p.sums != nullptr) {
 #pragma unroll
-        for (int k = 0; k < kFewRows * kTok / kFewThreads; ++k) {
-            const int at = k * kFewThreads + threadIdx.x, row = at / kTok, tok = at % kTok;
-            float g = exp2_(zs[k] - ms[tok]) * gs[tok];
-            if (r0 + row == hit[tok]) g -= gg[tok];
-            dl[buf][row * kPitch + tok] = r0 + row < v1 && tok < p.n && gg[tok] != 0.0f ? g : 0.0f;
+            for (int k = 0; k < kSub; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = 16 * k + 4 * j + quarter;
+                    load(p.rows, r0 + i < r_1 ? r0 + i : r_1 - 1, x[k][j]);
+                    if (SMALL && mine_tokens[i].hit == -2) x[k][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
         }
-        if (r0 + kFewRows < v1) logits(r0 + kFewRows);
-        __syncthreads();  // (the buffer was read two rounds ago, a barrier ago)
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int at = k * kFewThreads + threadIdx.x, row = at / kFew, i = at % kFew;
+            const FewToken t = mine_tokens[SMALL ? row : i];
+            float g = exp2_(zs[k] - t.m) * t.gs;
+            if ((SMALL ? i : r0 + row) == t.hit) g -= t.g;
+            dl[buf][row * kPitch + i] = r0 + row < r_1 && i < p.nfew && t.hit != -2 ? g : 0.0f;
+        }
+        if (r0 + kFewRows < r_1) {
+            logits(r0 + kFewRows);
+            if (SMALL && threadIdx.x < kFewRows)
+                tokens[SMALL ? turn * kFewRows + threadIdx.x : 0] = row_token(r0 + kFewRows);
+        }
+        __syncthreads();  // (this dl was last read two rounds ago, a barrier ago)
         if (c0 - 4 * col >= p.d) continue;  // the whole wave: no column of its own
 #pragma unroll
         for (int k = 0; k < kSub; ++k) {
             const float* mine = dl[buf] + 16 * k * kPitch;
-            if (p.dw != nullptr) {
+            if (p.drows != nullptr) {
                 f32x4 acc[4] = {};
 #pragma unroll
                 for (int j = 0; j < 4 * NB; ++j) {
                     const float a = mine[col * kPitch + 4 * j + quarter];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, hv[j][i], acc[i], 0, 0, 0);
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, few[j][i], acc[i], 0, 0,
+                                                                      0);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int64_t row = r0 + 16 * k + 4 * quarter + r;
-                    if (row >= v1) continue;
+                    const int at = 16 * k + 4 * quarter + r;
+                    const int64_t row = r0 + at;
+                    if (row >= r_1) continue;
+                    const bool none = SMALL && mine_tokens[at].hit == -2;
                     float y[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = acc[i][r] * factor;
+                    for (int i = 0; i < 4; ++i) y[i] = none ? 0.0f : acc[i][r] * factor;
                     if (VEC) {
-                        if (c0 < p.d) T::store4(p.dw, row * p.d + c0, y);
+                        if (c0 < p.d) T::store4(p.drows, row * p.d + c0, y);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (c0 + i < p.d) T::store(p.dw, row * p.d + c0 + i, y[i]);
+                            if (c0 + i < p.d) T::store(p.drows, row * p.d + c0 + i, y[i]);
                     }
                 }
             }
@@ -994,8 +1109,8 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
                         const float a = mine[(4 * j + quarter) * kPitch + 16 * b + col];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            dh[b][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[k][j][i],
-                                                                            dh[b][i], 0, 0, 0);
+                            sum[b][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[k][j][i],
+                                                                             sum[b][i], 0, 0, 0);
                     }
             }
         }
@@ -1005,12 +1120,12 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int64_t tok = 16 * b + 4 * quarter + r;
-            if (tok >= p.n) continue;
-            float* to = p.sums + (blockIdx.y * p.n + tok) * p.d + c0;
+            const int64_t i = 16 * b + 4 * quarter + r;
+            if (i >= p.nfew) continue;
+            float* to = p.sums + (blockIdx.y * p.nfew + i) * p.d + c0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c0 + i < p.d) to[i] = dh[b][i][r];
+            for (int c = 0; c < 4; ++c)
+                if (c0 + c < p.d) to[c] = sum[b][c][r];
         }
 }
 
@@ -1029,7 +1144,7 @@ struct Carve {
 };
 
 struct Saved {
-    int64_t header, rows, pos, tgt, norm, h, w, z, bytes;
+    int64_t header, rows, pos, tgt, norm, h, w, z, live, bytes;
 };
 
 bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
@@ -1038,17 +1153,23 @@ int64_t stages(const slk_linear_ce* a, int64_t k) { return ceil_div(k, split_of(
 bool few(const slk_linear_ce* a) {
     return a->n <= (!a->keep ? kFewScores : split_of(a) ? kFewTokens<F32> : kFewTokens<BF16>);
 }
-// 16-token blocks of the few tokens' kernels: 1, 2, 4 or 8
+// A small vocabulary takes the few tokens' way with the operands exchanged, for any
+// number of tokens: the tiles' 256 rows of vocabulary would stay mostly empty.
+constexpr int kSmallVoc = 128;
+bool small(const slk_linear_ce* a) { return !few(a) && a->v <= kSmallVoc; }
+// blocks of 16 of the few: tokens 1, 2, 4 or 8, a small vocabulary 5 or 8
 int64_t few_blocks(const slk_linear_ce* a) {
+    if (small(a)) return a->v <= 80 ? 5 : 8;
     return a->n <= 16 ? 1 : a->n <= 32 ? 2 : a->n <= 64 ? 4 : 8;
 }
 
 Saved saved_of(const slk_linear_ce* a) {
     Saved s{};
     Carve c;
-    if (few(a)) {  // the logits themselves: 4 bytes each, where W has 4 d / n for one
+    if (few(a) || small(a)) {  // the logits themselves, far fewer than the long operand
         s.norm = c.take(8 * a->n);
-        s.z = c.take(a->v * few_blocks(a) * 64);
+        s.z = c.take((small(a) ? a->n : a->v) * few_blocks(a) * 64);
+        s.live = c.take(4);
         s.bytes = a->keep ? c.at : 0;
         return s;
     }
@@ -1066,6 +1187,7 @@ Saved saved_of(const slk_linear_ce* a) {
 constexpr int64_t kFewGroups = 2048;  // workgroups of ce_few_kernel at most
 
 int64_t parts_of(const slk_linear_ce* a) {
+    if (small(a)) return 0;
     if (few(a)) {
         const int64_t g = ceil_div(ceil_div(a->v, few_blocks(a) > 1 ? 32 : 16), kFewWaves);
         return g < kFewGroups ? g : kFewGroups;
@@ -1119,15 +1241,20 @@ struct Backward {
 };
 Backward backward_of(const slk_linear_ce* a) {
     Backward b{};
-    if (few(a)) {
-        // parts of the vocabulary: two workgroups a CU over all columns
-        const int64_t cols = ceil_div(a->d, 256), most = ceil_div(512, cols);
-        b.piece = ceil_div(ceil_div(a->v, most), kFewRows) * kFewRows;
-        b.sh = static_cast<int>(ceil_div(a->v, b.piece));
+    if (few(a) || small(a)) {
+        // parts of the rows: two workgroups a CU over all columns, or (a small
+        // vocabulary: few rows a part and all its sums to join, or registers for
+        // one) one
+        const int64_t nrows = small(a) ? a->n : a->v, nfew = small(a) ? a->v : a->n;
+        const int64_t cols = ceil_div(a->d, 256);
+        const bool one = small(a) && (few_blocks(a) == 8 || nrows * cols < 512 * 128);
+        const int64_t most = ceil_div(one ? 256 : 512, cols);
+        b.piece = ceil_div(ceil_div(nrows, most), kFewRows) * kFewRows;
+        b.sh = static_cast<int>(ceil_div(nrows, b.piece));
         Carve c;
         b.factor = c.take(4);
-        b.pos = c.take(4 * a->n);
-        b.dh = c.take(a->dhidden != nullptr ? 4 * b.sh * a->n * a->d : 0);
+        b.pos = c.take(small(a) ? 0 : 4 * a->n);
+        b.dh = c.take((small(a) ? a->dweight : a->dhidden) != nullptr ? 4 * b.sh * nfew * a->d : 0);
         b.bytes = c.at;
         return b;
     }
@@ -1211,15 +1338,28 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
     JoinArgs j{part, zt, a->target, nullptr, nullptr, nullptr, losses, a->n, a->v,
                a->ignore_index, parts_of(a)};
     int rc = SLK_OK;
-    if (few(a)) {
-        const bool vec = a->d % (16 / T::kBytes) == 0 && aligned_to(a->hidden, 16) &&
-                         aligned_to(a->weight, 16);
+    float *z = nullptr, *live = nullptr;
+    if (a->keep && (few(a) || small(a))) {
         char* sv = static_cast<char*>(a->saved);
-        float* z = nullptr;
-        if (a->keep) {
-            z = reinterpret_cast<float*>(sv + saved_of(a).z);
-            j.norm = reinterpret_cast<float2*>(sv + saved_of(a).norm);
-        }
+        z = reinterpret_cast<float*>(sv + saved_of(a).z);
+        j.norm = reinterpret_cast<float2*>(sv + saved_of(a).norm);
+        live = reinterpret_cast<float*>(sv + saved_of(a).live);
+    }
+    const bool vec = a->d % (16 / T::kBytes) == 0 && aligned_to(a->hidden, 16) &&
+                     aligned_to(a->weight, 16);
+    if (small(a)) {
+        const int64_t g = ceil_div(a->n, 16);
+        auto go = [&](auto k) {
+            hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(g < 4096 ? g : 4096)),
+                               dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target, a->n,
+                               a->d, a->v, a->ignore_index, losses, j.norm, z);
+        };
+        if (few_blocks(a) == 5)
+            vec ? go(ce_small_kernel<T, true, 5, 2>) : go(ce_small_kernel<T, false, 5, 2>);
+        else
+            vec ? go(ce_small_kernel<T, true, 8, 2>) : go(ce_small_kernel<T, false, 8, 2>);
+        rc = check_launch("linear_ce small");
+    } else if (few(a)) {
         const dim3 grid(static_cast<unsigned>(parts_of(a)));
         auto go = [&](auto k) {
             hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target,
@@ -1278,7 +1418,9 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
         j.norm = reinterpret_cast<float2*>(sv + s.norm);
     }
     if (rc != SLK_OK) return rc;
-    if (few(a)) {
+    if (small(a)) {
+        // the losses are there
+    } else if (few(a)) {
         hipLaunchKernelGGL(ce_join_kernel<1>, dim3(static_cast<unsigned>(a->n)), dim3(256), 0, st,
                            j);
     } else {
@@ -1288,7 +1430,7 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
     if ((rc = check_launch("linear_ce join")) != SLK_OK) return rc;
     if (a->reduction != SLK_REDUCE_NONE) {
         hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, losses, a->target, a->n,
-                           a->ignore_index, a->reduction == SLK_REDUCE_MEAN, a->loss);
+                           a->ignore_index, a->reduction == SLK_REDUCE_MEAN, live, a->loss);
         rc = check_launch("linear_ce reduce");
     }
     return rc;
@@ -1300,41 +1442,52 @@ int backward_few(const slk_linear_ce* a, hipStream_t st) {
     const Backward b = backward_of(a);
     const char* sv = static_cast<const char*>(a->saved);
     char* sc = static_cast<char*>(a->scratch);
-    float* sums = a->dhidden != nullptr ? reinterpret_cast<float*>(sc + b.dh) : nullptr;
+    const bool sm = small(a);
+    void* few_out = sm ? a->dweight : a->dhidden;
+    void* rows_out = sm ? a->dhidden : a->dweight;
+    if (few_out == nullptr && rows_out == nullptr) return SLK_OK;
+    float* sums = few_out != nullptr ? reinterpret_cast<float*>(sc + b.dh) : nullptr;
     float* factor = reinterpret_cast<float*>(sc + b.factor);
-    int32_t* pos = reinterpret_cast<int32_t*>(sc + b.pos);
-    const FewArgs p{a->hidden, a->weight, a->target, reinterpret_cast<const float*>(sv + s.z),
-                    reinterpret_cast<const float2*>(sv + s.norm), a->upstream, a->n, a->d, a->v,
-                    a->ignore_index, b.piece, a->reduction, sums, a->dweight, factor, pos};
-    if (sums == nullptr && a->dweight == nullptr) return SLK_OK;
+    int32_t* pos = sm ? nullptr : reinterpret_cast<int32_t*>(sc + b.pos);
+    const int64_t nfew = sm ? a->v : a->n, nrows = sm ? a->n : a->v;
+    const FewArgs p{sm ? a->weight : a->hidden, sm ? a->hidden : a->weight, a->target,
+                    reinterpret_cast<const float*>(sv + s.z),
+                    reinterpret_cast<const float2*>(sv + s.norm), a->upstream,
+                    reinterpret_cast<const float*>(sv + s.live), nfew, nrows, a->d,
+                    a->ignore_index, b.piece, a->reduction, sums, rows_out, factor, pos};
     const dim3 grid(static_cast<unsigned>(ceil_div(a->d, 256)), static_cast<unsigned>(b.sh));
     const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 4 * T::kBytes) &&
                      aligned_to(a->weight, 4 * T::kBytes) &&
-                     aligned_to(a->dweight, 4 * T::kBytes);
-    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, p); };
-    switch (few_blocks(a)) {
-        case 1:
-            vec ? go(ce_few_back_kernel<T, true, 1>) : go(ce_few_back_kernel<T, false, 1>);
-            break;
-        case 2:
-            vec ? go(ce_few_back_kernel<T, true, 2>) : go(ce_few_back_kernel<T, false, 2>);
-            break;
-        default:
-            if constexpr (kFewTokens<T> > 32)
-                vec ? go(ce_few_back_kernel<T, true, 4>) : go(ce_few_back_kernel<T, false, 4>);
-    }
+                     aligned_to(rows_out, 4 * T::kBytes);
+    auto go = [&](auto blocks, auto swapped) {
+        constexpr int NB = decltype(blocks)::value;
+        constexpr bool SMALL = decltype(swapped)::value;
+        if (vec)
+            hipLaunchKernelGGL((ce_few_back_kernel<T, true, NB, SMALL>), grid, dim3(kFewThreads),
+                               0, st, p);
+        else
+            hipLaunchKernelGGL((ce_few_back_kernel<T, false, NB, SMALL>), grid, dim3(kFewThreads),
+                               0, st, p);
+    };
+    using std::false_type;
+    using std::true_type;
+    if (sm && few_blocks(a) == 5) go(std::integral_constant<int, 5>{}, true_type{});
+    else if (sm) go(std::integral_constant<int, 8>{}, true_type{});
+    else if (few_blocks(a) == 1) go(std::integral_constant<int, 1>{}, false_type{});
+    else if (few_blocks(a) == 2) go(std::integral_constant<int, 2>{}, false_type{});
+    else if constexpr (kFewTokens<T> > 32) go(std::integral_constant<int, 4>{}, false_type{});
     int rc = check_launch("linear_ce few backward");
     if (rc != SLK_OK || sums == nullptr) return rc;
-    const int64_t g = ceil_div(a->n * a->d, 256);
+    const int64_t g = ceil_div(nfew * a->d, 256);
     hipLaunchKernelGGL((ce_finish_kernel<T, false>),
                        dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st, sums,
-                       b.sh, a->n, a->n, a->d, pos, nullptr, factor, false, a->dhidden);
+                       b.sh, nfew, nfew, a->d, pos, nullptr, factor, false, few_out);
     return check_launch("linear_ce finish");
 }
 
 template <class T, bool SPLIT>
 int backward(const slk_linear_ce* a, hipStream_t st) {
-    if (few(a)) return backward_few<T>(a, st);
+    if (few(a) || small(a)) return backward_few<T>(a, st);
     const Saved s = saved_of(a);
     const Backward b = backward_of(a);
     char* sv = static_cast<char*>(a->saved);
@@ -1446,7 +1599,8 @@ extern "C" int slk_linear_ce_backward(const slk_linear_ce* a, void* stream) {
         a->scratch == nullptr || a->saved == nullptr) {
         return fail(SLK_EINVAL, "linear_ce_backward: saved or scratch too small");
     }
-    if (few(a) && (a->hidden == nullptr || a->weight == nullptr || a->target == nullptr)) {
+    if ((few(a) || small(a)) &&
+        (a->hidden == nullptr || a->weight == nullptr || a->target == nullptr)) {
         return fail(SLK_EINVAL, "linear_ce_backward: NULL hidden, weight or target");
     }
     return a->dtype == SLK_F32 ? backward<F32, true>(a, as_stream(stream))

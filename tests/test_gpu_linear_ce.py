@@ -487,3 +487,61 @@ def test_captured_few_tokens_replay(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, once()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 16, 65, 80, 81, 128, 129])
+@pytest.mark.parametrize("n,d", [(65, 4), (129, 63), (300, 260), (1000, 520), (5000, 64)])
+def test_small_vocabularies(dev, dtype, v, n, d):
+    check(dev, n, d, v, dtype, 0.2, ("mean", "none", "sum")[n % 3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_small_vocabularys_ignored_tokens_reach_nothing(dev, dtype, bad):
+    h, w, t = make(500, 70, 65, dtype, dev, 25)
+    t[::3] = -100
+    at = (torch.arange(500, device=dev) % 3 == 0)[:, None]
+    runs = []
+    for x in (torch.where(at, bad, h), torch.where(at, 0, h)):
+        x, y = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = slk.linear_cross_entropy(x, y, t)
+        runs.append((loss.detach(), *torch.autograd.grad(loss, [x, y])))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert bool((runs[0][1][::3] == 0).all()) and bool(torch.isfinite(runs[0][2]).all())
+
+
+def test_a_small_vocabularys_gradients_alone_targets_and_captures(dev):
+    h, w, t = make(700, 64, 65, torch.float32, dev, 26, 0.2)
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+
+    def once(h, w):
+        loss = slk.linear_cross_entropy(h, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, [x for x in (h, w) if x.requires_grad]))
+
+    both = once(hg, wg)
+    assert torch.equal(once(hg, w)[1], both[1]) and torch.equal(once(h, wg)[1], both[2])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once(hg, wg)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once(hg, wg)
+    for k in range(4):
+        with torch.no_grad():
+            hg.copy_(torch.randn(700, 64, generator=torch.Generator().manual_seed(k)))
+            t.copy_(torch.randint(0, 65, (700,), generator=torch.Generator().manual_seed(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, once(hg, wg)))
+    t[3], t[9] = 65, -5  # no rows of the vocabulary
+    loss, gh, gw = once(hg, wg)
+    assert bool(torch.isnan(loss)) and bool(torch.isfinite(gh).all() & torch.isfinite(gw).all())
+
+
+@pytest.mark.parametrize("keep", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(130, 33, 70), (65, 260, 128), (40, 50, 300), (64, 257, 31)])
+def test_unpacked_writes_stay_in_range(dev, dtype, n, d, v, keep):
+    test_writes_stay_in_range(dev, dtype, n, d, v, keep)
