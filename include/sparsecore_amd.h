@@ -841,15 +841,15 @@ SLK_API int slk_norm_backward(const slk_norm* args_host, void* stream);
  *              (over the tokens not ignored; NaN if there is none): 1 each
  *   keep       1 where a backward follows: forward then leaves in saved
  *              (slk_linear_ce_saved_bytes) its operands, packed, or for few tokens
- *              the logits. backward reads it, and hidden, weight and target as
- *              forward had them (few tokens: the arrays themselves, unchanged)
+ *              or a small vocabulary the logits. backward reads it, and then also
+ *              hidden, weight and target, unchanged since forward
  *   scratch    slk_linear_ce_scratch_bytes(args, backward) bytes; its dhidden
  *              and dweight as in the call (NULL: not wanted)
  * float32 products run on the float16 matrix instructions in two parts an
  * operand, about as exact as float32 products (in float32 the gradient of a
- * logit is kept to 2^-39 of the largest one), for few tokens on the float32
- * ones; bf16 gradients of logits are rounded to bf16 (few tokens: not). Sums in
- * float32, in a fixed order.                                                  */
+ * logit is kept to 2^-39 of the largest one), for few tokens or a small
+ * vocabulary on the float32 ones; bf16 gradients of logits are rounded to bf16,
+ * but not those. Sums in float32, in a fixed order.                           */
 enum slk_reduction { SLK_REDUCE_NONE = 0, SLK_REDUCE_SUM = 1, SLK_REDUCE_MEAN = 2 };
 typedef struct slk_linear_ce {
     int64_t n, d, v, ignore_index;

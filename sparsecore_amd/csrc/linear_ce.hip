@@ -19,7 +19,9 @@
 // float16 products are one.
 //
 // Few tokens are bound by reading W, which they do where it lies: 8 x 2048 x
-// 80000 at 4.6 TB/s, forward.
+// 80000 at 4.6 TB/s, forward. A small vocabulary goes the same way, tokens and
+// vocabulary exchanged: 8192 x 384 x 65 forward in 15 us, backward in 30 + 7,
+// bound by the float32 instructions (13 us of both) and the loads they wait for.
 #include "elem.hpp"
 #include "mma_tile.hpp"
 
@@ -1153,10 +1155,19 @@ int64_t stages(const slk_linear_ce* a, int64_t k) { return ceil_div(k, split_of(
 bool few(const slk_linear_ce* a) {
     return a->n <= (!a->keep ? kFewScores : split_of(a) ? kFewTokens<F32> : kFewTokens<BF16>);
 }
-// A small vocabulary takes the few tokens' way with the operands exchanged, for any
-// number of tokens: the tiles' 256 rows of vocabulary would stay mostly empty.
+// A small vocabulary takes the few tokens' way with the operands exchanged: the
+// tiles' 256 rows of vocabulary would stay mostly empty. 8192 x 384 x 65 float32,
+// forward and backward: 57 us of kernels against 107; 8192 x 4096 x 65: 261 against
+// 439. Of bfloat16, whose backward is on the float32 instructions here, only up to
+// 2^23 hidden values: 8192 x 1024 x 128 takes 121 us against 148, but 8192 x 4096 x
+// 65 240 against 209 and 65536 x 384 x 65 255 against 198 (scores alone: 46 against
+// 91, 61 against 96).
 constexpr int kSmallVoc = 128;
-bool small(const slk_linear_ce* a) { return !few(a) && a->v <= kSmallVoc; }
+constexpr int64_t kSmallHidden = int64_t{1} << 23;
+bool small(const slk_linear_ce* a) {
+    return !few(a) && a->v <= kSmallVoc &&
+           (!a->keep || split_of(a) || a->n * a->d <= kSmallHidden);
+}
 // blocks of 16 of the few: tokens 1, 2, 4 or 8, a small vocabulary 5 or 8
 int64_t few_blocks(const slk_linear_ce* a) {
     if (small(a)) return a->v <= 80 ? 5 : 8;

@@ -4,7 +4,7 @@
 
 without storing the logits: forward keeps a maximum and a sum of each token, backward
 computes the logits again a piece of the vocabulary at a time (``slk_linear_ce_*``). Only
-those of a few tokens, far smaller than the head, are kept.
+those of a few tokens or a small vocabulary, far smaller than the other operand, are kept.
 """
 
 from __future__ import annotations
@@ -87,10 +87,10 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
 
     Returns the float32 loss, with gradients for hidden and weight. float32 products are
     about as exact as float32 matrix products; bfloat16 gradients pass through logit
-    gradients rounded to bfloat16 (not those of few tokens). A forward that a backward may
-    follow keeps weight and hidden once more, packed, until then; of few tokens (at most
-    64, 32 in bfloat16) their logits instead. hidden, weight and target must not change in
-    place before the backward. Results repeat bit for bit.
+    gradients rounded to bfloat16 where there are many. A forward that a backward may
+    follow keeps weight and hidden once more, packed, until then; with few tokens (at most
+    64, 32 in bfloat16) or a small vocabulary (128) the logits instead. hidden, weight and
+    target must not change in place before the backward. Results repeat bit for bit.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, reduction).
