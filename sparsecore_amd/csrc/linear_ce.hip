@@ -20,7 +20,7 @@
 //
 // Few tokens are bound by reading W, which they do where it lies: 8 x 2048 x
 // 80000 at 4.6 TB/s, forward. A small vocabulary goes the same way, tokens and
-// vocabulary exchanged: 8192 x 384 x 65 forward in 15 us, backward in 30 + 7,
+// vocabulary exchanged: 8192 x 384 x 65 forward in 13 us, backward in 30 + 7,
 // bound by the float32 instructions (13 us of both) and the loads they wait for.
 #include "elem.hpp"
 #include "mma_tile.hpp"
@@ -687,7 +687,7 @@ __global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict_
 // Few tokens read W where it lies, once forward and once backward: its packed
 // copy alone would be read and written three times more. Up to how many, by what
 // the two ways took at 2048 features and 80000 rows: a score 529 against 570 us at
-// 128 tokens (float32; bfloat16 236 against 253), a score and its gradients 889
+// 128 tokens (float32; bfloat16 236 against 253), a score and its gradients 788
 // against 1240 us at 64 (float32), 445 against 620 at 32 but 870 against 628 at 64
 // (bfloat16, whose backward here is on the float32 instructions).
 constexpr int kFewScores = 128;
@@ -774,10 +774,45 @@ __device__ __forceinline__ void few_products(const void* __restrict__ rows, int6
     if (k < k1) runs(k, std::true_type{});
 }
 
-// Forward of few tokens: a wave takes 16 MB rows of W at a time against all
-// tokens (the last is repeated). z is kept for the backward where it is wanted,
-// 16 NB tokens a row.
+// The same with the columns split among a workgroup's four waves: z[a][b] is the
+// joined sum of row 16 a + 4 (l / 16) + wv, few 16 b + l % 16.
 template <class T, bool VEC, int MB, int NB, int U>
+__device__ __forceinline__ void few_split(const void* __restrict__ rows, int64_t nrows,
+                                          int64_t blk, const void* __restrict__ few,
+                                          const int64_t (&fo)[NB], int64_t d, int wv, int lane,
+                                          float (&sh)[kFewWaves][MB][NB][4][kWave],
+                                          float (&z)[MB][NB]) {
+    constexpr int kStep = U * 64 / T::kBytes;
+    const int64_t steps = ceil_div(d, kStep);
+    const int64_t k0 = steps * wv / kFewWaves * kStep, k1 = steps * (wv + 1) / kFewWaves * kStep;
+    f32x4 acc[MB][NB];
+    few_products<T, VEC, MB, NB, U>(rows, nrows, blk, few, fo, d, k0, k1 < d ? k1 : d, lane, acc);
+    __syncthreads();  // the last block's sums are read
+#pragma unroll
+    for (int a = 0; a < MB; ++a)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sh[wv][a][b][r][lane] = acc[a][b][r];
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < MB; ++a)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            z[a][b] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kFewWaves; ++k) z[a][b] += sh[k][a][b][wv][lane];
+        }
+}
+
+// Forward of few tokens: a wave (SPLIT: a workgroup) takes 16 MB rows of W at a
+// time against all tokens (the last is repeated). z is kept for the backward
+// where it is wanted, 16 NB tokens a row. More rows of W at a time read the
+// tokens from the L2 less often; split, there are still workgroups enough: 64
+// tokens, 2048 features, 80000 rows in 317 us at 32 rows a wave, 258 at 64 a
+// workgroup. 128 tokens' sums are too many for that (768 features, 32768 rows: 76
+// us, split 95).
+template <class T, bool VEC, int MB, int NB, int U, bool SPLIT>
 __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
     const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
     int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt,
@@ -796,24 +831,42 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
         m[b] = -INFINITY;
         s[b] = 0.0f;
     }
+    constexpr int R = SPLIT ? 1 : 4;  // rows of a lane and block
     const int64_t blocks = ceil_div(v, 16 * MB);
-    for (int64_t blk = static_cast<int64_t>(blockIdx.x) * kFewWaves + wv; blk < blocks;
-         blk += static_cast<int64_t>(gridDim.x) * kFewWaves) {
-        f32x4 acc[MB][NB];
-        few_products<T, VEC, MB, NB, U>(w, v, blk, h, ho, d, 0, d, lane, acc);
+    const int64_t per = SPLIT ? 1 : kFewWaves;
+    for (int64_t blk = blockIdx.x * per + (SPLIT ? 0 : wv); blk < blocks; blk += gridDim.x * per) {
+        float zs[MB][NB][R];
+        if constexpr (SPLIT) {
+            __shared__ float sums[kFewWaves][MB][NB][4][kWave];
+            float z[MB][NB];
+            few_split<T, VEC, MB, NB, U>(w, v, blk, h, ho, d, wv, lane, sums, z);
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) zs[a][b][0] = z[a][b];
+        } else {
+            f32x4 acc[MB][NB];
+            few_products<T, VEC, MB, NB, U>(w, v, blk, h, ho, d, 0, d, lane, acc);
+#pragma unroll
+            for (int a = 0; a < MB; ++a)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) zs[a][b][r] = acc[a][b][r];
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float top = m[b];
 #pragma unroll
             for (int a = 0; a < MB; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int64_t vr = (blk * MB + a) * 16 + 4 * quarter + r;
-                    float z = acc[a][b][r] * kLog2e;
+                for (int r = 0; r < R; ++r) {
+                    const int64_t vr = (blk * MB + a) * 16 + 4 * quarter + (SPLIT ? wv : r);
+                    float z = zs[a][b][r] * kLog2e;
                     if (vr == want[b]) zt[16 * b + col] = z;
                     if (keep != nullptr && vr < v) keep[vr * kTok + 16 * b + col] = z;
                     if (vr >= v) z = -INFINITY;
-                    acc[a][b][r] = z;
+                    zs[a][b][r] = z;
                     top = fmaxf(top, z);
                 }
             const float base = top == -INFINITY ? 0.0f : top;
@@ -821,7 +874,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
 #pragma unroll
             for (int a = 0; a < MB; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[b] += exp2_(acc[a][b][r] - base);
+                for (int r = 0; r < R; ++r) s[b] += exp2_(zs[a][b][r] - base);
             m[b] = top;
         }
     }
@@ -846,65 +899,55 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
 }
 
 // Forward of a small vocabulary, the same with the operands' parts exchanged: a
-// workgroup has all logits of 16 tokens, so their softmax and loss too. Its waves
-// take a quarter of the columns each (a wave for all of them left the card's
-// vector units half empty: 8192 x 4096 x 65 float32 took 187 us) and then, of the
-// joined logits, the tokens that are theirs modulo 4.
-template <class T, bool VEC, int NB, int U>
+// workgroup has all logits of 16 MB tokens, so their softmax and loss too. (With a
+// wave for all columns of 16 tokens 8192 x 4096 x 65 float32 took 187 us, split 97,
+// with 32 tokens 64: W comes from the L2 for each of them.)
+template <class T, bool VEC, int MB, int NB, int U>
 __global__ __launch_bounds__(kFewThreads) void ce_small_kernel(
     const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
     int64_t n, int64_t d, int64_t v, int64_t ignore, float* __restrict__ losses,
     float2* __restrict__ norm, float* __restrict__ keep) {
-    constexpr int kMine = 16 / T::kBytes, kVoc = 16 * NB, kStep = U * 4 * kMine;
-    __shared__ float sh[kFewWaves][NB][4][kWave];
+    constexpr int kMine = 16 / T::kBytes, kVoc = 16 * NB;
+    __shared__ float sums[kFewWaves][MB][NB][4][kWave];
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
-    const int64_t steps = ceil_div(d, kStep);
-    const int64_t k0 = steps * wv / kFewWaves * kStep, ke = steps * (wv + 1) / kFewWaves * kStep;
-    const int64_t k1 = ke < d ? ke : d;
     int64_t wo[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
         wo[b] = (16 * b + col < v ? 16 * b + col : v - 1) * d + kMine * quarter;
-    const int64_t blocks = ceil_div(n, 16);
+    const int64_t blocks = ceil_div(n, 16 * MB);
     for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-        f32x4 acc[1][NB];
-        few_products<T, VEC, 1, NB, U>(h, n, blk, w, wo, d, k0, k1, lane, acc);
-        __syncthreads();  // the last block's logits are read
+        float zs[MB][NB];
+        few_split<T, VEC, MB, NB, U>(h, n, blk, w, wo, d, wv, lane, sums, zs);
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int a = 0; a < MB; ++a) {
+            const int64_t tok = (blk * MB + a) * 16 + 4 * quarter + wv;
+            const int64_t t = tok < n ? target[tok] : ignore;
+            float m = -INFINITY, s = 0.0f, zt = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sh[wv][b][r][lane] = acc[0][b][r];
-        __syncthreads();
-        const int64_t tok = blk * 16 + 4 * quarter + wv;
-        const int64_t t = tok < n ? target[tok] : ignore;
-        float m = -INFINITY, s = 0.0f, zt = 0.0f, zs[NB];
+            for (int b = 0; b < NB; ++b) {
+                const float z = zs[a][b] * kLog2e;
+                if (keep != nullptr && tok < n) keep[tok * kVoc + 16 * b + col] = z;
+                if (16 * b + col == t) zt = z;
+                zs[a][b] = 16 * b + col < v ? z : -INFINITY;
+                m = fmaxf(m, zs[a][b]);
+            }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float z = 0.0f;
+            for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+            if (m == -INFINITY) m = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kFewWaves; ++k) z += sh[k][b][wv][lane];
-            z *= kLog2e;
-            if (keep != nullptr && tok < n) keep[tok * kVoc + 16 * b + col] = z;
-            if (16 * b + col == t) zt = z;
-            zs[b] = 16 * b + col < v ? z : -INFINITY;
-            m = fmaxf(m, zs[b]);
+            for (int b = 0; b < NB; ++b) s += exp2_(zs[a][b] - m);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                s += __shfl_xor(s, o);
+                zt += __shfl_xor(zt, o);
+            }
+            if (col != 0 || tok >= n) continue;
+            const bool valid = t >= 0 && t < v;
+            losses[tok] = t == ignore ? 0.0f : valid ? ((m - zt) + log2f(s)) * kLn2 : NAN;
+            if (norm != nullptr) norm[tok] = make_float2(m, 1.0f / s);
         }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if (m == -INFINITY) m = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) s += exp2_(zs[b] - m);
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            s += __shfl_xor(s, o);
-            zt += __shfl_xor(zt, o);
-        }
-        if (col != 0 || tok >= n) continue;
-        const bool valid = t >= 0 && t < v;
-        losses[tok] = t == ignore ? 0.0f : valid ? ((m - zt) + log2f(s)) * kLn2 : NAN;
-        if (norm != nullptr) norm[tok] = make_float2(m, 1.0f / s);
     }
 }
 
@@ -1200,7 +1243,9 @@ constexpr int64_t kFewGroups = 2048;  // workgroups of ce_few_kernel at most
 int64_t parts_of(const slk_linear_ce* a) {
     if (small(a)) return 0;
     if (few(a)) {
-        const int64_t g = ceil_div(ceil_div(a->v, few_blocks(a) > 1 ? 32 : 16), kFewWaves);
+        // (the rows that ce_few_kernel's variants take at a time)
+        const int64_t b = few_blocks(a);
+        const int64_t g = ceil_div(a->v, b == 1 ? 16 * kFewWaves : b == 4 ? 64 : 32 * kFewWaves);
         return g < kFewGroups ? g : kFewGroups;
     }
     return ceil_div(a->v, kTileM);
@@ -1359,16 +1404,24 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
     const bool vec = a->d % (16 / T::kBytes) == 0 && aligned_to(a->hidden, 16) &&
                      aligned_to(a->weight, 16);
     if (small(a)) {
-        const int64_t g = ceil_div(a->n, 16);
+        const bool more = a->n >= 8192;  // 32 tokens a workgroup, which fill the card
+        const int64_t g = ceil_div(a->n, more ? 32 : 16);
         auto go = [&](auto k) {
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(g < 4096 ? g : 4096)),
                                dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target, a->n,
                                a->d, a->v, a->ignore_index, losses, j.norm, z);
         };
-        if (few_blocks(a) == 5)
-            vec ? go(ce_small_kernel<T, true, 5, 2>) : go(ce_small_kernel<T, false, 5, 2>);
-        else
-            vec ? go(ce_small_kernel<T, true, 8, 2>) : go(ce_small_kernel<T, false, 8, 2>);
+        auto pick = [&](auto mb, auto nb) {
+            constexpr int MB = decltype(mb)::value, NB = decltype(nb)::value;
+            if (vec) go(ce_small_kernel<T, true, MB, NB, 2>);
+            else go(ce_small_kernel<T, false, MB, NB, 2>);
+        };
+        std::integral_constant<int, 1> one{};
+        std::integral_constant<int, 2> two{};
+        std::integral_constant<int, 5> five{};
+        std::integral_constant<int, 8> eight{};
+        if (few_blocks(a) == 5) more ? pick(two, five) : pick(one, five);
+        else more ? pick(two, eight) : pick(one, eight);
         rc = check_launch("linear_ce small");
     } else if (few(a)) {
         const dim3 grid(static_cast<unsigned>(parts_of(a)));
@@ -1376,22 +1429,23 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
             hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target,
                                a->n, a->d, a->v, part, zt, z);
         };
+        auto pick = [&](auto mb, auto nb, auto u, auto split) {
+            constexpr int MB = decltype(mb)::value, NB = decltype(nb)::value;
+            constexpr int U = decltype(u)::value;
+            constexpr bool S = decltype(split)::value;
+            if (vec) go(ce_few_kernel<T, true, MB, NB, U, S>);
+            else go(ce_few_kernel<T, false, MB, NB, U, S>);
+        };
+        using std::integral_constant;
+        integral_constant<int, 1> one{};
+        integral_constant<int, 2> two{};
+        integral_constant<int, 4> four{};
+        integral_constant<int, 8> eight{};
         switch (few_blocks(a)) {
-            case 1:
-                vec ? go(ce_few_kernel<T, true, 1, 1, 8>)
-                    : go(ce_few_kernel<T, false, 1, 1, 8>);
-                break;
-            case 2:
-                vec ? go(ce_few_kernel<T, true, 2, 2, 4>)
-                    : go(ce_few_kernel<T, false, 2, 2, 4>);
-                break;
-            case 4:
-                vec ? go(ce_few_kernel<T, true, 2, 4, 2>)
-                    : go(ce_few_kernel<T, false, 2, 4, 2>);
-                break;
-            default:
-                vec ? go(ce_few_kernel<T, true, 2, 8, 2>)
-                    : go(ce_few_kernel<T, false, 2, 8, 2>);
+            case 1: pick(one, one, eight, std::false_type{}); break;
+            case 2: pick(two, two, four, std::false_type{}); break;
+            case 4: pick(four, four, two, std::true_type{}); break;
+            default: pick(two, eight, two, std::false_type{});
         }
         rc = check_launch("linear_ce few");
     } else {
