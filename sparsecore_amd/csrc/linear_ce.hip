@@ -806,28 +806,30 @@ __device__ __forceinline__ void few_split(const void* __restrict__ rows, int64_t
 }
 
 // Forward of few tokens: a wave (SPLIT: a workgroup) takes 16 MB rows of W at a
-// time against all tokens (the last is repeated). z is kept for the backward
-// where it is wanted, 16 NB tokens a row. More rows of W at a time read the
-// tokens from the L2 less often; split, there are still workgroups enough: 64
-// tokens, 2048 features, 80000 rows in 317 us at 32 rows a wave, 258 at 64 a
-// workgroup. 128 tokens' sums are too many for that (768 features, 32768 rows: 76
-// us, split 95).
+// time against all live tokens (list[0 .. live); the last is repeated). z is kept
+// for the backward where it is wanted, `pitch` tokens a row. More rows of W at a
+// time read the tokens from the L2 less often; split, there are still workgroups
+// enough: 64 tokens, 2048 features, 80000 rows in 317 us at 32 rows a wave, 258 at
+// 64 a workgroup. 128 tokens' sums are too many for that (768 features, 32768
+// rows: 76 us, split 95).
 template <class T, bool VEC, int MB, int NB, int U, bool SPLIT>
-__global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
+__device__ __forceinline__ void few_forward(
     const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
-    int64_t n, int64_t d, int64_t v, float2* __restrict__ part, float* __restrict__ zt,
-    float* __restrict__ keep) {
-    constexpr int kMine = 16 / T::kBytes, kTok = 16 * NB;
+    const int* list, int live, int64_t n, int64_t d, int64_t v, float2* __restrict__ part,
+    float* __restrict__ zt, float* __restrict__ keep, int pitch) {
+    constexpr int kMine = 16 / T::kBytes;
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
     int64_t want[NB], ho[NB];
+    int tok[NB];
     float m[NB], s[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int64_t tok = 16 * b + col < n ? 16 * b + col : n - 1;
-        want[b] = 16 * b + col < n ? target[tok] : -1;
-        ho[b] = tok * d + kMine * quarter;
+        const bool in = 16 * b + col < live;
+        tok[b] = list[in ? 16 * b + col : live - 1];
+        want[b] = in ? target[tok[b]] : -1;
+        ho[b] = tok[b] * d + kMine * quarter;
         m[b] = -INFINITY;
         s[b] = 0.0f;
     }
@@ -863,8 +865,8 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
                 for (int r = 0; r < R; ++r) {
                     const int64_t vr = (blk * MB + a) * 16 + 4 * quarter + (SPLIT ? wv : r);
                     float z = zs[a][b][r] * kLog2e;
-                    if (vr == want[b]) zt[16 * b + col] = z;
-                    if (keep != nullptr && vr < v) keep[vr * kTok + 16 * b + col] = z;
+                    if (vr == want[b]) zt[tok[b]] = z;
+                    if (keep != nullptr && vr < v) keep[vr * pitch + tok[b]] = z;
                     if (vr >= v) z = -INFINITY;
                     zs[a][b][r] = z;
                     top = fmaxf(top, z);
@@ -879,7 +881,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
         }
     }
     // the lanes of a token, then the waves
-    __shared__ float2 sh[kFewWaves][kTok];
+    __shared__ float2 sh[kFewWaves][16 * NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -890,12 +892,48 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
         if (lane < 16) sh[wv][16 * b + lane] = make_float2(m[b], s[b]);
     }
     __syncthreads();
-    if (threadIdx.x < n) {
+    if (static_cast<int>(threadIdx.x) < live) {
         float2 x = sh[0][threadIdx.x];
         for (int k = 1; k < kFewWaves; ++k)
             join(x.x, x.y, sh[k][threadIdx.x].x, sh[k][threadIdx.x].y);
-        part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = x;
+        part[static_cast<int64_t>(blockIdx.x) * n + list[threadIdx.x]] = x;
     }
+}
+
+// The live tokens first, then as many blocks of 16 as they fill, of at most MOST.
+template <class T, bool VEC, int MOST>
+__global__ __launch_bounds__(kFewThreads) void ce_few_kernel(
+    const void* __restrict__ h, const void* __restrict__ w, const int64_t* __restrict__ target,
+    int64_t n, int64_t d, int64_t v, int64_t ignore, float2* __restrict__ part,
+    float* __restrict__ zt, float* __restrict__ keep) {
+    __shared__ int list[16 * MOST];
+    const int lane = threadIdx.x & (kWave - 1);
+    int live = 0;
+#pragma unroll
+    for (int t0 = 0; t0 < 16 * MOST; t0 += kWave) {  // every wave counts, the first writes
+        const int t = t0 + lane;
+        const bool in = t < n && target[t < n ? t : 0] != ignore;
+        const uint64_t mask = __ballot(in);
+        if (in && threadIdx.x < kWave)
+            list[live + __popcll(mask & ((uint64_t{1} << lane) - 1))] = t;
+        live += __popcll(mask);
+    }
+    __syncthreads();
+    if (live == 0) return;  // the whole grid; the joined losses are 0
+    constexpr int kPitch = 16 * MOST;
+#define SLK_FEW(MB, NB, U, S) \
+    few_forward<T, VEC, MB, NB, U, S>(h, w, target, list, live, n, d, v, part, zt, keep, kPitch)
+    if constexpr (MOST >= 8) {
+        if (live > 64) return SLK_FEW(2, 8, 2, false);
+    }
+    if constexpr (MOST >= 4) {
+        if (live > 32) return SLK_FEW(4, 4, 2, true);
+    }
+    if constexpr (MOST >= 2) {
+        if (live > 16) return SLK_FEW(2, 2, 4, false);
+    }
+    SLK_FEW(1, 1, 8, false);
+#undef SLK_FEW
 }
 
 // Forward of a small vocabulary, the same with the operands' parts exchanged: a
@@ -1427,25 +1465,18 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
         const dim3 grid(static_cast<unsigned>(parts_of(a)));
         auto go = [&](auto k) {
             hipLaunchKernelGGL(k, grid, dim3(kFewThreads), 0, st, a->hidden, a->weight, a->target,
-                               a->n, a->d, a->v, part, zt, z);
+                               a->n, a->d, a->v, a->ignore_index, part, zt, z);
         };
-        auto pick = [&](auto mb, auto nb, auto u, auto split) {
-            constexpr int MB = decltype(mb)::value, NB = decltype(nb)::value;
-            constexpr int U = decltype(u)::value;
-            constexpr bool S = decltype(split)::value;
-            if (vec) go(ce_few_kernel<T, true, MB, NB, U, S>);
-            else go(ce_few_kernel<T, false, MB, NB, U, S>);
+        auto pick = [&](auto most) {
+            constexpr int MOST = decltype(most)::value;
+            if (vec) go(ce_few_kernel<T, true, MOST>);
+            else go(ce_few_kernel<T, false, MOST>);
         };
-        using std::integral_constant;
-        integral_constant<int, 1> one{};
-        integral_constant<int, 2> two{};
-        integral_constant<int, 4> four{};
-        integral_constant<int, 8> eight{};
         switch (few_blocks(a)) {
-            case 1: pick(one, one, eight, std::false_type{}); break;
-            case 2: pick(two, two, four, std::false_type{}); break;
-            case 4: pick(four, four, two, std::true_type{}); break;
-            default: pick(two, eight, two, std::false_type{});
+            case 1: pick(std::integral_constant<int, 1>{}); break;
+            case 2: pick(std::integral_constant<int, 2>{}); break;
+            case 4: pick(std::integral_constant<int, 4>{}); break;
+            default: pick(std::integral_constant<int, 8>{});
         }
         rc = check_launch("linear_ce few");
     } else {

@@ -545,3 +545,13 @@ def test_a_small_vocabularys_gradients_alone_targets_and_captures(dev):
 @pytest.mark.parametrize("n,d,v", [(130, 33, 70), (65, 260, 128), (40, 50, 300), (64, 257, 31)])
 def test_unpacked_writes_stay_in_range(dev, dtype, n, d, v, keep):
     test_writes_stay_in_range(dev, dtype, n, d, v, keep)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [12, 30, 60, 128])
+@pytest.mark.parametrize("ignored", [0.6, 0.95, 1.0])
+def test_few_tokens_mostly_ignored(dev, dtype, n, ignored):
+    h, w, t = make(n, 200, 700, dtype, dev, 27, ignored)
+    losses, err, *_ = reference(h, w, t, torch.zeros(n, device=dev))
+    within(slk.linear_cross_entropy(h, w, t, reduction="none"), losses, err, "loss")
+    check(dev, n, 200, 700, dtype, ignored, "none", 27)
