@@ -10,7 +10,10 @@
 // argument (no copy to the device, nothing to keep alive) and one launch
 // serves kAdamTensors tensors; a lane takes four consecutive elements with
 // one 16-byte load an array; a wave takes SLK_Q8_BLOCK elements, a whole
-// block of 8-bit codes, whose new scale is one wave reduction.
+// block of 8-bit codes, whose new scale is one wave reduction. Measured: 64
+// million elements with 8-bit moments 217 us (4.7 TB/s, what a large copy
+// reaches), 53 tensors of 2.3 million with 32-bit ones 11.4 us (out of the
+// caches), 49 thousand elements 3.8 us.
 #include "elem.hpp"
 #include "q8.hpp"
 
@@ -236,8 +239,8 @@ __device__ inline int find_slot(const int32_t* __restrict__ old_cols, int lo, in
 // 0. Out of place: a row's slots move both ways.
 //
 // Bound by its instructions (16 million slots in 8 bits moved in 185 us when
-// every slot searched its row by itself with 64-bit places), then by the
-// latency of dependent loads. The wave finds its first row 64 places at a time
+// every slot searched its row by itself with 64-bit places, 153 now, where their
+// bytes take 41), then by the latency of dependent loads. The wave finds its first row 64 places at a time
 // and brings the old columns of its own slots and kNear on either side into
 // LDS: a column is mostly that near to where it was (a rewrite that moves a
 // third of a row of 16384 shifts the rest by about a hundred slots). A lane
