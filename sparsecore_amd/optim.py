@@ -367,17 +367,16 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         # torch casts states to their parameter's dtype: 8-bit codes and the float32
         # moments of bfloat16 parameters are taken from the dict as they are
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        steps: dict = {}
-        for i, p in zip(ids, params):
-            for k, v in state_dict["state"].get(i, {}).items():
-                if k == "step" and isinstance(v, torch.Tensor):  # shared, as _step_group makes it
-                    self.state[p][k] = steps.setdefault(
-                        (p.device, float(v)), v.detach().to(p.device, copy=True))
-                else:
-                    self.state[p][k] = (v.detach().to(p.device, copy=True)
-                                        if isinstance(v, torch.Tensor) else v)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            steps: dict = {}  # a count is shared within a group only, which advances it
+            for i, p in zip(saved["params"], group["params"]):
+                for k, v in state_dict["state"].get(i, {}).items():
+                    if k == "step" and isinstance(v, torch.Tensor):
+                        v = steps.setdefault((p.device, float(v)),
+                                             v.detach().to(p.device, copy=True))
+                    elif isinstance(v, torch.Tensor):
+                        v = v.detach().to(p.device, copy=True)
+                    self.state[p][k] = v
         for at in self._attached.values():
             at.snapshot()
 
