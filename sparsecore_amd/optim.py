@@ -380,6 +380,13 @@ class AdamW(torch.optim.Optimizer):
         for at in self._attached.values():
             at.snapshot()
 
+    def _idle_counts(self, group, params) -> set:
+        """Counts that parameters without a gradient stay at: those that go on leave them."""
+        if len(params) == len(group["params"]):
+            return set()
+        return {id(self.state[p]["step"]) for p in group["params"]
+                if p.grad is None and "step" in self.state.get(p, ())}
+
     # ─── the step ───
 
     @torch.no_grad()
@@ -410,7 +417,11 @@ class AdamW(torch.optim.Optimizer):
         names = ["exp_avg", "exp_avg_sq"]
         if group["state_bits"] == 8:
             names += ["exp_avg_scale", "exp_avg_sq_scale"]
-        by_step: dict = {}  # more than one part only where a first gradient came late
+        idle = self._idle_counts(group, params) if group["capturable"] else ()
+        if idle and capturing and any(id(s["step"]) in idle for s in states):
+            raise RuntimeError("AdamW: a parameter that has counted along with others has no "
+                               "gradient; take one such step before capturing")
+        by_step: dict = {}  # more than one part only where a gradient came late or not at all
         for i, s in enumerate(states):
             if not group["capturable"]:
                 s["step"] += 1
@@ -418,7 +429,12 @@ class AdamW(torch.optim.Optimizer):
                                []).append(i)
         for part in by_step.values():
             if group["capturable"]:
-                states[part[0]]["step"].add_(1.0)
+                step = states[part[0]]["step"]
+                if id(step) in idle:
+                    step = step.clone()
+                    for i in part:
+                        states[i]["step"] = step
+                step.add_(1.0)
             ps = [params[i] for i in part]
             gs = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
             lists = [[states[i][k] for i in part] for k in names]

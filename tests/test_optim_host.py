@@ -62,3 +62,32 @@ def test_groups_count_their_own_steps_after_loading(launches, capturable, throug
     assert counts(launches, p) == [[4.0, 5.0, 6.0]] * 3
     assert len(launches) == 6  # a launch a group: parameters of one count stay together
     assert [float(opt.state[q]["step"]) for q in p] == [3.0] * 3  # nothing shared with the source
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_parameter_without_a_gradient_keeps_its_count(launches, capturable):
+    p = parameters(3)
+    opt = slk.AdamW(p, capturable=capturable)
+    opt.step()
+    p[1].grad = None
+    opt.step()
+    opt.step()
+    p[1].grad = torch.ones(4)
+    opt.step()
+    assert counts(launches, p) == [[1, 2, 3, 4], [1, 2], [1, 2, 3, 4]]
+
+
+def test_a_capture_that_would_part_counts_is_refused(launches, monkeypatch):
+    p = parameters(2)
+    opt = slk.AdamW(p, capturable=True)
+    opt.step()
+    p[1].grad = None
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        opt.step()
+    with monkeypatch.context() as eager:
+        eager.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        opt.step()
+    opt.step()  # the counts are apart now
+    assert counts(launches, p) == [[1, 2, 3], [1]]
