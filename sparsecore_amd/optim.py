@@ -258,19 +258,31 @@ def carry_slots(row_start, old, new, states) -> list:
 
 # ─────────────────────────── the optimizer ───────────────────────────
 
+def _capturing() -> bool:
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
 class _Attached:
     """A SparseLinear's topology as its moments know it."""
 
     def __init__(self, layer):
         self.layer = layer
+        self.cols = self.nnz = None
         self.snapshot()
 
     def snapshot(self) -> None:
         csr = self.layer._csr
         self.csr = csr
         self.version = csr.topology_version
-        self.cols = csr.col_indices.clone()
-        self.nnz = csr.row_nnz.clone()
+        self.cols = _copied(self.cols, csr.col_indices)
+        self.nnz = _copied(self.nnz, csr.row_nnz)
+
+
+def _copied(to, t):
+    """t's values, in `to` where they fit it."""
+    if to is None or to.shape != t.shape or to.device != t.device:
+        return t.clone()
+    return to.copy_(t)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -284,11 +296,14 @@ class AdamW(torch.optim.Optimizer):
             A group's choice; small tensors such as norm weights can keep 32.
         capturable: keep the step count on the device, so that a captured graph counts
             its replays. Otherwise a step under capture raises RuntimeError, since the
-            graph would repeat one step's bias corrections.
+            graph would repeat one step's bias corrections. Moments begin in an eager
+            step: a capture before it raises too.
 
     A SET or RigL rewrite gives slots to other weights. ``model.apply(opt.attach)``
     makes the moments of each SparseLinear follow: the next ``step()`` first moves them
     to their weights' new slots (``carry_slots``) and starts grown connections at 0.
+    Replays of a captured step do not: call ``follow()`` after each rewrite, before the
+    next replay. The moments stay in their tensors, so the capture remains valid.
     A layer whose matrix was replaced (``load_state_dict``, ``reset_parameters``) is
     attached again, after loading the optimizer's own state.
     """
@@ -321,6 +336,14 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(module, SparseLinear):
             self._attached[module._values] = _Attached(module)
 
+    @torch.no_grad()
+    def follow(self) -> None:
+        """Moves the moments of attached layers to their weights' slots after SET or RigL
+        rewrites, as the next ``step()`` would first. A captured step cannot: between a
+        rewrite and its next replay (or the next capture) call this."""
+        for p in self._attached:
+            self._follow(p)
+
     def _follow(self, p) -> None:
         at = self._attached[p]
         csr = at.layer._csr
@@ -331,21 +354,21 @@ class AdamW(torch.optim.Optimizer):
             at.snapshot()  # the layer moved to another device, with its topology
         if csr.topology_version == at.version:
             return
+        if _capturing():
+            raise RuntimeError("AdamW: a layer was rewritten and its moments have not followed; "
+                               "call follow() (or take a step) before capturing")
         s = self.state[p]
         if s:
             names = [k for k in ("exp_avg", "exp_avg_sq") if k in s]
             states = [(s[k], s[k + "_scale"]) if k + "_scale" in s else s[k] for k in names]
-            # what is replaced below may have been made on another stream than this one
-            now = torch.cuda.current_stream(p.device)
-            for k, t in [*s.items(), ("cols", at.cols), ("nnz", at.nnz)]:
-                if isinstance(t, torch.Tensor) and k != "step":
-                    t.record_stream(now)
+            # back into the same tensors: a captured step reads them where they were
             for k, got in zip(names, carry_slots(csr.row_start, (at.cols, at.nnz),
                                                  (csr.col_indices, csr.row_nnz), states)):
                 if isinstance(got, tuple):
-                    s[k], s[k + "_scale"] = got
+                    s[k].copy_(got[0])
+                    s[k + "_scale"].copy_(got[1])
                 else:
-                    s[k] = got
+                    s[k].copy_(got)
         at.snapshot()
 
     # ─── state ───
@@ -400,12 +423,15 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, group) -> None:
-        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        capturing = _capturing()
         if capturing and not group["capturable"]:
             raise RuntimeError("AdamW: a step under graph capture needs capturable=True")
         params = [p for p in group["params"] if p.grad is not None]
         if not params:
             return
+        if capturing and not all(self.state[p] for p in params):
+            raise RuntimeError("AdamW: a captured step would begin the moments anew on every "
+                               "replay; take one step of all its parameters before capturing")
         states, first = [], 0
         if group["capturable"] and not all(self.state[p] for p in params):
             first = torch.zeros(1, device=params[0].device)  # one count for all that begin now

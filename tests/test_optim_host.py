@@ -91,3 +91,83 @@ def test_a_capture_that_would_part_counts_is_refused(launches, monkeypatch):
         opt.step()
     opt.step()  # the counts are apart now
     assert counts(launches, p) == [[1, 2, 3], [1]]
+
+
+@pytest.fixture
+def layer(launches, monkeypatch):
+    """A SparseLinear, and a carry of its moments that runs on the host."""
+    def carry(row_start, old, new, states):
+        out = []
+        for s in states:
+            to = torch.zeros_like(s)
+            for r, start in enumerate(row_start.tolist()):
+                was = {int(old[0][k]): k for k in range(start, start + int(old[1][r]))}
+                for k in range(start, start + int(new[1][r])):
+                    if int(new[0][k]) in was:
+                        to[k] = s[was[int(new[0][k])]]
+            out.append(to)
+        return out
+
+    monkeypatch.setattr(optim, "carry_slots", carry)
+    torch.manual_seed(0)
+    net = slk.SparseLinear(20, 12, sparsity=0.5, bias=False)
+    net._values.grad = torch.ones_like(net._values)
+    return net
+
+
+def rewrite(net):
+    """Moves the first connection of every row to a column that the row did not have."""
+    csr = net._csr
+    for r, start in enumerate(csr.row_start.tolist()):
+        n = int(csr.row_nnz[r])
+        cols = csr.col_indices[start:start + n]
+        free = next(c for c in range(csr.ncols) if c not in cols.tolist())
+        cols[0] = free
+        cols.copy_(cols.sort().values)
+    csr._topology_version += 1
+
+
+@pytest.mark.parametrize("how", ["step", "follow"])
+def test_carried_moments_stay_where_they_are(layer, how):
+    """A captured step's replays read the addresses of its capture."""
+    p = layer._values
+    opt = slk.AdamW([p], capturable=True)
+    opt.attach(layer)
+    opt.step()
+    s = opt.state[p]
+    s["exp_avg"].copy_(torch.arange(float(p.numel())))
+    before, at = dict(s), s["exp_avg"].data_ptr()
+    old = layer._csr.col_indices.clone(), layer._csr.row_nnz.clone()
+    want, = optim.carry_slots(layer._csr.row_start, old, old, [s["exp_avg"].clone()])
+    rewrite(layer)
+    want, = optim.carry_slots(layer._csr.row_start, old,
+                              (layer._csr.col_indices, layer._csr.row_nnz), [s["exp_avg"].clone()])
+    getattr(opt, how)()
+    assert all(s[k] is before[k] for k in before) and s["exp_avg"].data_ptr() == at
+    assert torch.equal(s["exp_avg"], want) and bool((want == 0).any())
+    opt.follow()  # nothing is left to move
+    assert torch.equal(s["exp_avg"], want)
+
+
+def test_a_capture_that_would_record_a_move_or_a_beginning_is_refused(layer, monkeypatch):
+    p = layer._values
+    opt = slk.AdamW([p], capturable=True)
+    opt.attach(layer)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    capturing = [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    with pytest.raises(RuntimeError, match="before capturing"):
+        opt.step()  # would zero the moments and the count on every replay
+    assert not opt.state[p]
+    capturing[0] = False
+    opt.step()
+    rewrite(layer)
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="follow"):
+        opt.step()  # would move the moments on every replay
+    with pytest.raises(RuntimeError, match="follow"):
+        opt.follow()
+    capturing[0] = False
+    opt.follow()
+    capturing[0] = True
+    opt.step()
