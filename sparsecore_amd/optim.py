@@ -200,6 +200,8 @@ def _launch(sizes, params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas
             if any(k is not dtype for k in kinds):
                 part = table[[k is dtype for k in kinds]]
             _lib.adamw(part, len(part), _lib.DTYPES[dtype], bits, args, stream)
+    # written through their addresses: a backward that has saved one of them must notice
+    torch.autograd.graph.increment_version([t for k, ts in enumerate(cols) if k != 1 for t in ts])
 
 
 # ─────────────────────── states that follow a rewrite ───────────────────────

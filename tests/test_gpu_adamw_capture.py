@@ -75,3 +75,21 @@ def test_captures_that_would_repeat_a_beginning_or_a_move_are_refused(dev):
     capture(opt.step).replay()
     torch.cuda.synchronize()
     assert float(opt.state[net._values]["step"]) == 2
+
+
+def test_a_backward_across_a_step_is_refused(dev):
+    """SparseLinear's backward and that of linear_cross_entropy over few tokens read the
+    weights themselves."""
+    net = slk.SparseLinear(64, 48, sparsity=0.5, bias=False).to(dev)
+    head = torch.nn.Parameter(torch.randn(100, 64, device=dev))
+    x = torch.randn(8, 64, device=dev, requires_grad=True)
+    t = torch.zeros(8, dtype=torch.int64, device=dev)
+    for p, loss in ((net._values, lambda: net(x).square().sum()),
+                    (head, lambda: slk.linear_cross_entropy(x, head, t))):
+        opt = slk.AdamW([p])
+        late = loss()
+        loss().backward()
+        opt.step()
+        with pytest.raises(RuntimeError, match="inplace"):
+            late.backward()
+        opt.zero_grad()

@@ -171,3 +171,21 @@ def test_a_capture_that_would_record_a_move_or_a_beginning_is_refused(layer, mon
     opt.follow()
     capturing[0] = True
     opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_a_step_writes_changes_its_version(monkeypatch, bits):
+    """As torch's in-place operations do, so that a backward which saved a parameter
+    raises after a step in place of computing with the new one."""
+    from sparsecore_amd import _lib
+
+    monkeypatch.setattr(_lib, "adamw", lambda *a: None)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_lib, "on_device", lambda t: _lib._SAME_DEVICE)
+    p, g = torch.nn.Parameter(torch.zeros(300)), torch.zeros(300)
+    kinds = (torch.int8, torch.uint8) if bits == 8 else (torch.float32,) * 2
+    m, v = (torch.zeros(300, dtype=k) for k in kinds)
+    scales = (torch.zeros(2), torch.zeros(2)) if bits == 8 else ()
+    optim._launch([300], [p], [g], [m], [v], tuple([s] for s in scales) or None, 1, 1e-3,
+                  (0.9, 0.99), 1e-8, 0.0)
+    assert all(t._version == 1 for t in (p, m, v, *scales)) and g._version == 0
