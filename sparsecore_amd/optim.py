@@ -307,7 +307,8 @@ class AdamW(torch.optim.Optimizer):
     Replays of a captured step do not: call ``follow()`` after each rewrite, before the
     next replay. The moments stay in their tensors, so the capture remains valid.
     A layer whose matrix was replaced (``load_state_dict``, ``reset_parameters``) is
-    attached again, after loading the optimizer's own state.
+    attached again, after loading the optimizer's own state. A deep copy or an unpickled
+    optimizer has no layers attached: ``attach`` its own.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -327,6 +328,10 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(g["lr"], torch.Tensor) and not g["capturable"]:
             raise ValueError("AdamW: a tensor lr needs capturable=True")
         super().add_param_group(group)
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self.__dict__.setdefault("_attached", {})  # a copy: it knows no layers yet
 
     # ─── topology ───
 

@@ -4,6 +4,7 @@ and the checks of device tensors are replaced by a recorder, so these run on CPU
 from __future__ import annotations
 
 import copy
+import pickle
 
 import pytest
 import torch
@@ -189,3 +190,21 @@ def test_what_a_step_writes_changes_its_version(monkeypatch, bits):
     optim._launch([300], [p], [g], [m], [v], tuple([s] for s in scales) or None, 1, 1e-3,
                   (0.9, 0.99), 1e-8, 0.0)
     assert all(t._version == 1 for t in (p, m, v, *scales)) and g._version == 0
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_of_an_optimizer_step(layer, launches, how):
+    opt = slk.AdamW([layer._values])
+    opt.attach(layer)
+    opt.step()
+    twin = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    p, = twin.param_groups[0]["params"]
+    p.grad = torch.ones_like(p)
+    launches.clear()
+    twin.step()
+    assert counts(launches, [p, layer._values]) == [[2], []]
+    twin.load_state_dict(opt.state_dict())
+    twin.step()
+    assert twin.state[p]["step"] == 2 and opt.state[layer._values]["step"] == 1
+    twin.attach(layer)  # a copy's own layers are attached anew
+    assert layer._values in twin._attached
