@@ -341,7 +341,9 @@ class AdamW(torch.optim.Optimizer):
         from .nn import SparseLinear
 
         if isinstance(module, SparseLinear):
-            self._attached[module._values] = _Attached(module)
+            at = self._attached.get(module._values)
+            if at is None or at.layer is not module or at.csr is not module._csr:
+                self._attached[module._values] = _Attached(module)
 
     @torch.no_grad()
     def follow(self) -> None:

@@ -208,3 +208,19 @@ def test_copies_of_an_optimizer_step(layer, launches, how):
     assert twin.state[p]["step"] == 2 and opt.state[layer._values]["step"] == 1
     twin.attach(layer)  # a copy's own layers are attached anew
     assert layer._values in twin._attached
+
+
+def test_attaching_again_keeps_a_move_that_is_due(layer):
+    p = layer._values
+    opt = slk.AdamW([p])
+    opt.attach(layer)
+    opt.step()
+    s = opt.state[p]
+    s["exp_avg"].copy_(torch.arange(float(p.numel())))
+    old = layer._csr.col_indices.clone(), layer._csr.row_nnz.clone()
+    rewrite(layer)
+    want, = optim.carry_slots(layer._csr.row_start, old,
+                              (layer._csr.col_indices, layer._csr.row_nnz), [s["exp_avg"].clone()])
+    opt.attach(layer)
+    opt.step()
+    assert torch.equal(s["exp_avg"], want)
