@@ -846,9 +846,9 @@ SLK_API int slk_norm_backward(const slk_norm* args_host, void* stream);
  *   scratch    slk_linear_ce_scratch_bytes(args, backward) bytes; its dhidden
  *              and dweight as in the call (NULL: not wanted)
  * float32 products run on the float16 matrix instructions in two parts an
- * operand, about as exact as float32 products (in float32 the gradient of a
- * logit is kept to 2^-39 of the largest one), for few tokens or a small
- * vocabulary on the float32 ones; bf16 gradients of logits are rounded to bf16,
+ * operand, 22 bits of an element down to 2^-39 of its row's largest (of the
+ * logits' gradients: of a token's, a class's largest term), for few tokens or a
+ * small vocabulary on the float32 ones; bf16 gradients of logits are rounded to bf16,
  * but not those. Sums in float32, in a fixed order.                           */
 enum slk_reduction { SLK_REDUCE_NONE = 0, SLK_REDUCE_SUM = 1, SLK_REDUCE_MEAN = 2 };
 typedef struct slk_linear_ce {

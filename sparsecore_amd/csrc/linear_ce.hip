@@ -15,8 +15,8 @@
 // Bound by the matrix cores from some hundred tokens on. 8192 x 4096 x 100000
 // bfloat16, forward and backward: 21.5 ms, the logits at 1334 TFLOP/s, dhidden's
 // and dweight's products at 1305 and 1203 (a large library product: 1388). 4001 x
-// 768 x 32000 float32: 1.59 ms, 500 TFLOP/s of float32 counted as the three
-// float16 products are one.
+// 768 x 32000 float32, 3 in 10 tokens ignored: 1.88 to 1.97 ms, 375 + 481 + 412 + 372
+// us in the four products (1100 TFLOP/s as float16), 289 in dl's two operands.
 //
 // Few tokens are bound by reading W, which they do where it lies: 8 x 2048 x
 // 80000 at 4.6 TB/s, forward. A small vocabulary goes the same way, tokens and
@@ -28,22 +28,18 @@
 namespace slk {
 namespace {
 
-// float16 operands are scaled so that their largest finite magnitude lies in
-// [2^13, 2^14); dl (at most 1) by 2^kDlExp.
-constexpr int kTopExp = 14, kDlExp = 14;
+// Float16 operands are scaled by a power of two a row, so that the row's largest
+// finite magnitude lies in [2^13, 2^14): one scale for a whole operand let a token
+// of 10^8 times the others' magnitude take the others' digits (their losses were off
+// by 1e-3). A row that is not summed over gives its power back in the epilogue, a row
+// along the sum has it folded into the other factor, dl, whose own rows are scaled
+// by the largest term that each then has.
+constexpr int kTopExp = 14;
 
-// What forward leaves for backward: counts and the operands' largest magnitudes.
-// The magnitudes are maxima over kTops places, each its own 128 bytes: on one
-// place the atomics of a few hundred workgroups took longer than the reading.
-constexpr int kTops = 8;
-struct Top {
-    uint32_t h, w;  // bits of the largest finite |h| (live tokens), |W|
-    uint32_t pad[30];
-};
+// What forward leaves for backward: the count of the live tokens.
 struct Header {
     int32_t live;
     int32_t pad[31];
-    Top top[kTops];
 };
 
 __device__ __forceinline__ int scale_exp(uint32_t top) {
@@ -53,16 +49,8 @@ __device__ __forceinline__ int scale_exp(uint32_t top) {
     const int s = kTopExp - e;
     return s > 126 ? 126 : s;
 }
-template <uint32_t Top::*Of>
-__device__ __forceinline__ int scale_exp(const Header* hd) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < kTops; ++k) m = max(m, hd->top[k].*Of);
-    return scale_exp(m);
-}
-__device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or inf past float32's range
-    return ldexpf(1.0f, e);
-}
+// x·2^e, rounded once, whatever e
+__device__ __forceinline__ float scaled(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
 // ───────────────────────────── live tokens ─────────────────────────────
 
@@ -120,27 +108,32 @@ __global__ __launch_bounds__(kListThreads) void ce_list_kernel(
         __syncthreads();
     }
     if (threadIdx.x == 0) hd->live = base;
-    if (threadIdx.x < kTops) hd->top[threadIdx.x].h = hd->top[threadIdx.x].w = 0;
 }
 
-// The largest finite magnitudes of hidden (live tokens) and weight, float32: a
-// wave a row of either.
+// The power of two of each row's scale, of hidden (live tokens, at their places) and
+// weight, float32: a wave a row of either. The rows past the vocabulary that a tile of
+// it covers get 0.
 template <bool VEC>
-__global__ __launch_bounds__(256) void ce_top_kernel(const float* __restrict__ h, int64_t n,
+__global__ __launch_bounds__(256) void ce_exp_kernel(const float* __restrict__ h, int64_t n,
                                                      const float* __restrict__ w, int64_t v,
-                                                     int64_t d, const int32_t* __restrict__ pos,
-                                                     Header* __restrict__ hd) {
+                                                     int64_t tiled, int64_t d,
+                                                     const int32_t* __restrict__ pos,
+                                                     int32_t* __restrict__ hx,
+                                                     int32_t* __restrict__ wx) {
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
-    uint32_t top[2] = {0, 0};
     auto see = [](uint32_t& m, float x) {
         const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
         if (b < 0x7f800000u) m = max(m, b);
     };
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-         row < n + v; row += waves) {
+         row < n + tiled; row += waves) {
         const bool of_h = row < n;
+        if (row >= n + v) {
+            if (lane == 0) wx[row - n] = 0;
+            continue;
+        }
         if (of_h && pos[row] < 0) continue;
         const float* x = of_h ? h + row * d : w + (row - n) * d;
         uint32_t m = 0;
@@ -164,36 +157,20 @@ __global__ __launch_bounds__(256) void ce_top_kernel(const float* __restrict__ h
         } else {
             for (int64_t e = lane; e < d; e += kWave) see(m, x[e]);
         }
-        if (of_h) top[0] = max(top[0], m);
-        else top[1] = max(top[1], m);
-    }
-    __shared__ uint32_t sh[2][4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            top[k] = max(top[k], static_cast<uint32_t>(__shfl_xor(top[k], o)));
-        if (lane == 0) sh[k][threadIdx.x >> 6] = top[k];
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const uint32_t* x = sh[threadIdx.x];
-        const uint32_t m = max(max(x[0], x[1]), max(x[2], x[3]));
-        Top& t = hd->top[blockIdx.x % kTops];
-        // a maximum: the same whatever the order
-        if (m != 0) atomicMax(threadIdx.x == 0 ? &t.h : &t.w, m);
+        for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
+        if (lane == 0) (of_h ? hx[pos[row]] : wx[row - n]) = scale_exp(m);
     }
 }
 
 // ───────────────────────────── packing ─────────────────────────────
 
-// hi and lo of eight values scaled by `scale`
-__device__ __forceinline__ void split8(const float (&v)[8], float scale, f16x8& hi, f16x8& lo) {
+// hi and lo of eight values
+__device__ __forceinline__ void split8(const float (&v)[8], f16x8& hi, f16x8& lo) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float x = v[j] * scale;
-        hi[j] = static_cast<_Float16>(x);
-        lo[j] = static_cast<_Float16>(x - static_cast<float>(hi[j]));
+        hi[j] = static_cast<_Float16>(v[j]);
+        lo[j] = static_cast<_Float16>(v[j] - static_cast<float>(hi[j]));
     }
 }
 
@@ -201,8 +178,7 @@ struct PackArgs {
     const void* src;
     const int32_t* rows;  // source row of each row, NULL: itself
     const int32_t* live;  // rows that count (device), NULL: R
-    const Header* hd;     // largest magnitudes (float32 sources)
-    bool of_w;
+    const int32_t* exps;  // power of two of each row's scale (float32 sources)
     int64_t R, d;
     int64_t out_rows;  // rows that the packed form is laid out for
     char* out;
@@ -215,8 +191,6 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
     constexpr int K = kStageK<SPLIT>, kParts = K / 8;
     const int64_t R = p.live != nullptr ? *p.live : p.R;
     const int64_t rows = ceil_div(R, 64) * 64;
-    const float scale =
-        SPLIT ? pow2(p.of_w ? scale_exp<&Top::w>(p.hd) : scale_exp<&Top::h>(p.hd)) : 1.0f;
     // four rows a thread, their loads in flight together
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int part = static_cast<int>(t % kParts);
@@ -252,8 +226,11 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
         if (r >= rows) break;
         char* to = p.out + (st * p.out_rows + r) * kStageBytes + 16 * part;
         if constexpr (SPLIT) {
+            const int scale = r < R ? p.exps[r] : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[j][k] = scaled(x[j][k], scale);
             f16x8 hi, lo;
-            split8(x[j], scale, hi, lo);
+            split8(x[j], hi, lo);
             *reinterpret_cast<f16x8*>(to) = hi;
             *reinterpret_cast<f16x8*>(to + 64) = lo;
         } else {
@@ -267,9 +244,27 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const PackArgs p) {
 
 // ───────────────────────────── epilogues ─────────────────────────────
 
-template <bool SPLIT>
-__device__ __forceinline__ float logit_scale(const Header* hd) {
-    return SPLIT ? pow2(-scale_exp<&Top::h>(hd)) * pow2(-scale_exp<&Top::w>(hd)) : 1.0f;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// The logits themselves: each accumulator by its row's and its token's power of two
+// (one exponent, so that nothing between overflows), of the wave's columns b.
+template <class Tile>
+__device__ __forceinline__ void unscale_logits(f32x16 (&acc)[Tile::kNA][2], const Tile& t, int b,
+                                               const int32_t* wx, const int32_t* hx) {
+    const int64_t tok = t.n0() + t.col(b);
+    const int th = tok < t.N ? hx[tok] : 0;
+    const int32_t* mine = wx + t.m0() + t.row(0, 0);
+#pragma unroll
+    for (int a = 0; a < Tile::kNA; ++a) {
+        i32x4 e[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            e[q] = *reinterpret_cast<const i32x4*>(mine + 32 * a + 8 * q);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            acc[a][b][r] = scaled(acc[a][b][r], -(e[r >> 2][r & 3] + th));
+        __builtin_amdgcn_sched_barrier(0);  // all blocks' exponents at once spilled registers
+    }
 }
 
 // Logits are exponentiated in base 2: the factor log2(e) goes into the scale of
@@ -294,7 +289,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // cross lanes.
 template <bool SPLIT>
 struct ScoreEpi {
-    const Header* hd;
+    const int32_t *wx, *hx;  // powers of two of the operands' rows (SPLIT)
     const int32_t* tgt;
     float2* part;  // vocabulary tiles x tokens
     float* zt;
@@ -303,10 +298,11 @@ struct ScoreEpi {
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         __syncthreads();  // the ring is free
         float2* sh = reinterpret_cast<float2*>(t.lds);  // kWavesM x kBN
-        const float scale2 = logit_scale<SPLIT>(hd) * kLog2e;
+        constexpr float scale2 = kLog2e;
         const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
+            if constexpr (SPLIT) unscale_logits(acc, t, b, wx, hx);
             const int64_t tok = t.n0() + t.col(b);
             const int64_t want = (tok < t.N ? tgt[tok] : -1) - t.m0();
             const bool here = want >= 0 && want < 32 * Tile::kNA;
@@ -352,24 +348,21 @@ struct ScoreEpi {
     }
 };
 
-// Backward: the same tiles as dl, an operand whose rows are tokens and whose
-// stages run along the piece of the vocabulary; zero where either ends inside
-// the tile.
+// Backward: the same tiles as dl, its rows tokens, zero where the live tokens or the
+// vocabulary end inside the tile. bfloat16: times the token's upstream gradient, as an
+// operand whose stages run along the piece of the vocabulary.
 template <bool SPLIT>
 struct DlEpi {
-    const Header* hd;
     const int32_t* tgt;
     const float2* norm;  // (m, 1 / s) of each token
-    const float* gr;     // upstream gradient of each token over the largest, NULL: all 1
+    const float* gr;     // upstream gradient of each token, NULL: all 1
     char* out;
     int64_t v0;    // first row of the piece
     int64_t rows;  // tokens that it is laid out for: whole tiles
     template <class Tile>
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
-        const float scale2 = logit_scale<SPLIT>(hd) * kLog2e;
         const int have = static_cast<int>(t.M - t.m0());  // those rows of this wave that exist
-        constexpr float up = SPLIT ? static_cast<float>(1 << kDlExp) : 1.0f;
-        constexpr int K = kStageK<SPLIT>;
+        constexpr int K = kStageK<false>;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t tok = t.n0() + t.col(b);
@@ -377,7 +370,7 @@ struct DlEpi {
             const int64_t want = (in ? tgt[tok] - v0 : -1) - t.m0();
             const bool any = __any(want >= 0 && want < 32 * Tile::kNA);
             const float2 ms = in ? norm[tok] : make_float2(0.0f, 0.0f);
-            const float g = (in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f) * up;
+            const float g = in ? (gr != nullptr ? gr[tok] : 1.0f) : 0.0f;
             const float gs = g * ms.y;
 #pragma unroll
             for (int a = 0; a < Tile::kNA; ++a) {
@@ -385,44 +378,262 @@ struct DlEpi {
                 char* to = out + ((v / K) * rows + tok) * kStageBytes + 2 * (v % K);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    uint16_t h[4], w[4];
+                    uint16_t h[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = 4 * q + j;
-                        float p = exp2_(fmaf(acc[a][b][r], scale2, -ms.x)) * gs;
+                        float p = exp2_(fmaf(acc[a][b][r], kLog2e, -ms.x)) * gs;
                         if (any && t.row(a, r) == want) p -= g;
                         p = in && t.row(a, r) < have ? p : 0.0f;
-                        if constexpr (SPLIT) {
-                            const _Float16 f = static_cast<_Float16>(p);
-                            h[j] = __builtin_bit_cast(uint16_t, f);
-                            w[j] = __builtin_bit_cast(
-                                uint16_t, static_cast<_Float16>(p - static_cast<float>(f)));
-                        } else {
-                            h[j] = f32_to_bf16(p);
-                            w[j] = 0;
-                        }
+                        h[j] = f32_to_bf16(p);
                     }
                     const int at = 2 * (8 * q + 4 * (t.lane >> 5));
                     *reinterpret_cast<ushort4*>(to + at) = make_ushort4(h[0], h[1], h[2], h[3]);
-                    if (SPLIT)
-                        *reinterpret_cast<ushort4*>(to + 64 + at) =
-                            make_ushort4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
     }
 };
 
+// Float32: dl itself, without the upstream gradients, 32 rows of vocabulary a stage
+// like the operands that ce_split_kernel makes of it. dl's rows (tokens) in dh = dl·W
+// and its columns in dW = dlᵀ·(g h) run over terms of very different sizes: softmax
+// entries of 1e-12 beside 1, rows of W and h of any magnitude. So each gets the power
+// of two of its own largest term, which this tile's part of is left here: of a token
+// max |dl|·2^-wx, of a row of the vocabulary max |dl g|·2^-hx, as exponents. (One array
+// of halves for both products, scaled by 2^14, kept 2^-39 of 1 and no more: it took
+// neither the second array nor the pass that makes the two, 0.3 of 1.6 ms at 4001 x
+// 768 x 32000, and lost the gradient of rows that softmax hardly reaches.)
+constexpr int kNoTerm = -(1 << 20);
+__device__ __forceinline__ int term_exp(float x, int e) {
+    return x == 0.0f ? kNoTerm : __builtin_amdgcn_frexp_expf(x) + e;
+}
+// the largest of 32 lanes, in lanes 31 and 63
+__device__ __forceinline__ int half_max(int x) {
+    auto step = [&](auto ctrl, auto rows) {
+        constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+        x = max(x, __builtin_amdgcn_update_dpp(x, x, C, R, 0xf, false));
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0xB1>{}, integral_constant<int, 0xf>{});   // lane ^ 1
+    step(integral_constant<int, 0x4E>{}, integral_constant<int, 0xf>{});   // lane ^ 2
+    step(integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});  // half row mirrored
+    step(integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});  // row mirrored
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // rows 0, 2 to 1, 3
+    return x;
+}
+template <>
+struct DlEpi<true> {
+    const int32_t *wx, *hx;  // of the piece's rows, of the tokens
+    const int32_t* tgt;
+    const float2* norm;
+    const float* gr;
+    char* out;
+    int64_t v0, rows;
+    int32_t* row_part;  // tiles of vocabulary x tokens (rows)
+    int32_t* col_part;  // tiles of tokens x rows of the piece
+    int64_t piece;
+    template <class Tile>
+    __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
+        constexpr int kWavesN = Tile::kBN / 64;
+        __syncthreads();  // the ring is free
+        int* sh_tok = reinterpret_cast<int*>(t.lds);         // kWavesM x kBN
+        int* sh_voc = sh_tok + Tile::kWavesM * Tile::kBN;    // kWavesN x kTileM
+        const int have = static_cast<int>(t.M - t.m0());  // those rows of this wave that exist
+        int want[2], hexp[2], big[2];
+        float2 ms[2];
+        float g[2];
+        bool in[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int64_t tok = t.n0() + t.col(b);
+            in[b] = tok < t.N;
+            const int64_t row = (in[b] ? tgt[tok] - v0 : -1) - t.m0();
+            want[b] = row >= 0 && row < 32 * Tile::kNA ? static_cast<int>(row) : -1;
+            ms[b] = in[b] ? norm[tok] : make_float2(0.0f, 0.0f);
+            g[b] = in[b] && gr != nullptr ? gr[tok] : 1.0f;
+            hexp[b] = in[b] ? -hx[tok] : 0;
+            big[b] = kNoTerm;
+        }
+        const bool any = __any(want[0] >= 0 || want[1] >= 0);
+#pragma unroll
+        for (int a = 0; a < Tile::kNA; ++a) {
+            const int64_t v = t.m0() + 32 * a;  // this block's 32 rows: a stage
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = t.row(a, 4 * q);
+                const i32x4 we = *reinterpret_cast<const i32x4*>(wx + t.m0() + row);
+                i32x4 most = {kNoTerm, kNoTerm, kNoTerm, kNoTerm};
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    f32x4 x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float z = scaled(acc[a][b][4 * q + j], hexp[b] - we[j]);
+                        float p = exp2_(fmaf(z, kLog2e, -ms[b].x)) * ms[b].y;
+                        if (any && row + j == want[b]) p -= 1.0f;
+                        p = in[b] && row + j < have ? p : 0.0f;
+                        x[j] = p;
+                        big[b] = max(big[b], term_exp(p, -we[j]));
+                        most[j] = max(most[j], term_exp(p * g[b], hexp[b]));
+                    }
+                    *reinterpret_cast<f32x4*>(out +
+                                              ((v / 32) * rows + t.n0() + t.col(b)) * kStageBytes +
+                                              4 * (row - 32 * a)) = x;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most[j] = half_max(most[j]);
+                if ((t.lane & 31) == 31)
+                    *reinterpret_cast<i32x4*>(sh_voc + t.wn * kTileM + 32 * Tile::kNA * t.wm +
+                                              row) = most;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int m = max(big[b], __shfl_xor(big[b], 32));
+            if (t.lane < 32) sh_tok[t.wm * Tile::kBN + 64 * t.wn + t.col(b)] = m;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < Tile::kBN; i += kMmaThreads) {
+            int m = kNoTerm;
+#pragma unroll
+            for (int w = 0; w < Tile::kWavesM; ++w) m = max(m, sh_tok[w * Tile::kBN + i]);
+            row_part[t.i0 / kTileM * rows + t.k0 + i] = m;
+        }
+        for (int i = threadIdx.x; i < kTileM; i += kMmaThreads) {
+            int m = kNoTerm;
+#pragma unroll
+            for (int w = 0; w < kWavesN; ++w) m = max(m, sh_voc[w * kTileM + i]);
+            col_part[t.k0 / Tile::kBN * piece + t.i0 + i] = m;
+        }
+    }
+};
+
+// The powers of two of dl's rows and columns from their tiles' parts: 32 of them a
+// workgroup, eight threads each; the tokens' workgroups first.
+struct TermArgs {
+    const int32_t *row_part, *col_part;
+    const int32_t* live;
+    int64_t rows, piece, vn;
+    int bn;  // tokens of a tile
+    int32_t *row_exp, *col_exp;
+};
+__global__ __launch_bounds__(256) void ce_term_kernel(const TermArgs p) {
+    __shared__ int sh[8][32];
+    const int64_t live = *p.live, groups = ceil_div(p.rows, 32);
+    const bool of_row = blockIdx.x < groups;
+    const int64_t i = 32 * (of_row ? blockIdx.x : blockIdx.x - groups) + (threadIdx.x & 31);
+    const int part = threadIdx.x >> 5;
+    const int64_t width = of_row ? p.rows : p.piece;
+    const int64_t parts = of_row ? ceil_div(p.vn, kTileM) : ceil_div(live, p.bn);
+    const bool in = of_row ? i < live : i < ceil_div(p.vn, kTileM) * kTileM;
+    const int32_t* from = of_row ? p.row_part : p.col_part;
+    int m = kNoTerm;
+    if (in) {
+        for (int64_t k = part; k < parts; k += 8) m = max(m, from[k * width + i]);
+    }
+    sh[part][threadIdx.x & 31] = m;
+    __syncthreads();
+    if (part != 0 || i >= width) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = max(m, sh[k][threadIdx.x]);
+    (of_row ? p.row_exp : p.col_exp)[i] = m == kNoTerm ? 0 : kTopExp - m;
+}
+
+// dl as the operands of its two products, scaled as above, in halves: dh's into its
+// own array, dW's in dl's place. Eight entries of a token a thread, four tokens.
+struct DlArgs {
+    char* dl;   // in: float32; out: dW's operand (NULL for neither: not wanted)
+    char* dlh;  // dh's operand
+    bool of_w;
+    const int32_t *wx, *hx, *row_exp, *col_exp;
+    const float* gr;  // NULL: all 1
+    const int32_t* live;
+    int64_t rows;
+};
+__global__ __launch_bounds__(256) void ce_split_kernel(const DlArgs p) {
+    const int64_t rows = ceil_div(static_cast<int64_t>(*p.live), 64) * 64;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int part = static_cast<int>(t & 3);
+    const int64_t st = blockIdx.y, r0 = t >> 2, step = rows / 4;
+    if (r0 >= step) return;
+    const int64_t v = 32 * st + 8 * part;
+    int we[8], ce[8];
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+        const i32x4 a = *reinterpret_cast<const i32x4*>(p.wx + v + k);
+        const i32x4 b = *reinterpret_cast<const i32x4*>(p.col_exp + v + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            we[k + j] = a[j];
+            ce[k + j] = b[j];
+        }
+    }
+    f32x4 x[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const char* from = p.dl + (st * p.rows + r0 + j * step) * kStageBytes + 32 * part;
+        x[j][0] = *reinterpret_cast<const f32x4*>(from);
+        x[j][1] = *reinterpret_cast<const f32x4*>(from + 16);
+    }
+    // a row's four threads are neighbours in one wave: what one overwrites below all
+    // have loaded above
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t r = r0 + j * step;
+        const int64_t at = (st * p.rows + r) * kStageBytes + 16 * part;
+        const bool in = r < *p.live;
+        float y[8];
+        f16x8 hi, lo;
+        if (p.dlh != nullptr) {
+            const int re = in ? p.row_exp[r] : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = scaled(x[j][k >> 2][k & 3], re - we[k]);
+            split8(y, hi, lo);
+            *reinterpret_cast<f16x8*>(p.dlh + at) = hi;
+            *reinterpret_cast<f16x8*>(p.dlh + at + 64) = lo;
+        }
+        if (p.of_w) {
+            const int he = in ? p.hx[r] : 0;
+            const float g = in && p.gr != nullptr ? p.gr[r] : 1.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = scaled(x[j][k >> 2][k & 3] * g, ce[k] - he);
+            split8(y, hi, lo);
+            *reinterpret_cast<f16x8*>(p.dl + at) = hi;
+            *reinterpret_cast<f16x8*>(p.dl + at + 64) = lo;
+        }
+    }
+}
+
+// The sums of a product whose first operand's rows were scaled: their powers of two
+// given back (before anything else, so that this rounds only what is subnormal).
+template <class Tile>
+__device__ __forceinline__ void unscale_rows(f32x16 (&acc)[2], const Tile& t, int a,
+                                             const int32_t* exps) {
+    i32x4 e[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        e[q] = *reinterpret_cast<const i32x4*>(exps + t.m0() + t.row(a, 4 * q));
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] = scaled(acc[b][r], -e[r >> 2][r & 3]);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // Gradient products: float32 sums of each part of the K loop.
+template <bool SPLIT>
 struct SumEpi {
     float* out;  // splits x rows x d
+    const int32_t* exps;  // of the first operand's rows (SPLIT)
     int64_t rows, d;
     bool add;  // onto what the vocabulary's earlier pieces left
     template <class Tile>
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         float* to = out + t.split * rows * d;
 #pragma unroll
-        for (int a = 0; a < Tile::kNA; ++a)
+        for (int a = 0; a < Tile::kNA; ++a) {
+            if constexpr (SPLIT) unscale_rows(acc[a], t, a, exps);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int64_t c = t.n0() + t.col(b);
@@ -442,72 +653,63 @@ struct SumEpi {
                     if (row < t.M && c < t.N) to[row * d + c] = acc[a][b][r];
                 }
             }
-    }
-};
-
-// A gradient from its sum: unscaled first (exactly), then times the upstream
-// factor. The two as one number could be subnormal where the result is not.
-template <bool SPLIT>
-struct GradScale {
-    float unscale, factor;
-    __device__ __forceinline__ GradScale(const Header* hd, const float* f, bool of_w)
-        : unscale(SPLIT ? pow2(-kDlExp - (of_w ? scale_exp<&Top::h>(hd)
-                                              : scale_exp<&Top::w>(hd)))
-                        : 1.0f),
-          factor(*f) {}
-    __device__ __forceinline__ float operator()(float sum) const {
-        return (SPLIT ? sum * unscale : sum) * factor;
+        }
     }
 };
 
 // dW where one workgroup has the whole sum: scaled, rounded and stored.
 template <class T, bool SPLIT>
 struct WeightEpi {
-    const Header* hd;
+    const int32_t* exps;
     const float* factor;
     void* out;  // of the piece's first row
     int64_t d;
     template <class Tile>
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
-        const GradScale<SPLIT> s(hd, factor, true);
+        const float f = *factor;
 #pragma unroll
-        for (int a = 0; a < Tile::kNA; ++a)
+        for (int a = 0; a < Tile::kNA; ++a) {
+            if constexpr (SPLIT) unscale_rows(acc[a], t, a, exps);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int64_t c = t.n0() + t.col(b);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int64_t row = t.m0() + t.row(a, r);
-                    if (row < t.M && c < t.N) T::store(out, row * d + c, s(acc[a][b][r]));
+                    if (row < t.M && c < t.N) T::store(out, row * d + c, acc[a][b][r] * f);
                 }
             }
+        }
     }
 };
 
 // dh where one workgroup has the whole sum: to the token's row.
 template <class T, bool SPLIT>
 struct TokenEpi {
-    const Header* hd;
-    const float* factor;
+    const int32_t* exps;
+    const float *factor, *gr;  // gr: each token's own in its place (SPLIT; NULL: none)
     const int32_t* rows;
     void* out;
     int64_t d;
     template <class Tile>
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
-        const GradScale<SPLIT> s(hd, factor, false);
+        const float f = *factor;
 #pragma unroll
-        for (int a = 0; a < Tile::kNA; ++a)
+        for (int a = 0; a < Tile::kNA; ++a) {
+            if constexpr (SPLIT) unscale_rows(acc[a], t, a, exps);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int64_t row = t.m0() + t.row(a, r);
                 if (row >= t.M) continue;
                 const int64_t at = rows[row] * d;
+                const float g = SPLIT && gr != nullptr ? gr[row] : f;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int64_t c = t.n0() + t.col(b);
-                    if (c < t.N) T::store(out, at + c, s(acc[a][b][r]));
+                    if (c < t.N) T::store(out, at + c, acc[a][b][r] * g);
                 }
             }
+        }
     }
 };
 
@@ -601,9 +803,8 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
     }
 }
 
-// Upstream gradients: factor is the largest magnitude over the live tokens and
-// gr each token's own over it, so that dl stays within [-1, 1]. With one
-// upstream value for all (sum, mean) every gr is 1 and none is written.
+// Upstream gradients: factor is the one for all tokens (sum, mean), or gr each live
+// token's own (none; factor is 1).
 // The workgroups beside the first clear the rows of dh that are no live token's,
 // where the product writes only the others.
 template <class T>
@@ -627,39 +828,27 @@ __global__ __launch_bounds__(1024) void ce_upstream_kernel(
         }
         return;
     }
-    __shared__ uint32_t sh[1024 / kWave];
     const int64_t live = hd->live;
-    if (reduction != SLK_REDUCE_NONE) {
+    if (reduction == SLK_REDUCE_NONE) {
+        for (int64_t i = threadIdx.x; i < live; i += 1024) gr[i] = up[rows[i]];
+        if (threadIdx.x == 0) *factor = 1.0f;
+    } else if (threadIdx.x == 0) {
         // no live token: gradients are 0, as the sum's over none
-        if (threadIdx.x == 0)
-            *factor = live == 0 ? 0.0f
-                      : reduction == SLK_REDUCE_MEAN ? *up / static_cast<float>(live) : *up;
-        return;
+        *factor = live == 0 ? 0.0f
+                  : reduction == SLK_REDUCE_MEAN ? *up / static_cast<float>(live) : *up;
     }
-    uint32_t m = 0;  // as bit patterns, a NaN is the largest
-    for (int64_t i = threadIdx.x; i < live; i += 1024)
-        m = max(m, __float_as_uint(up[rows[i]]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
-    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int w = 0; w < 1024 / kWave; ++w) m = max(m, sh[w]);
-    const float top = __uint_as_float(m);
-    for (int64_t i = threadIdx.x; i < live; i += 1024)
-        gr[i] = m == 0 ? 0.0f : up[rows[i]] / top;
-    if (threadIdx.x == 0) *factor = top;
 }
 
-// out[r][c] = the parts' sum, scaled and rounded; with pos, row r is token r and
-// the sums are at its place (0 where it has none).
-template <class T, bool SPLIT>
+// out[r][c] = the parts' sum times the upstream factor (gr: the token's own), rounded;
+// with pos, row r is token r and the sums are at its place (0 where it has none).
+template <class T>
 __global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict__ sums, int splits,
                                                         int64_t rows, int64_t stride, int64_t d,
                                                         const int32_t* __restrict__ pos,
-                                                        const Header* __restrict__ hd,
                                                         const float* __restrict__ factor,
-                                                        bool of_w, void* __restrict__ out) {
-    const GradScale<SPLIT> s(hd, factor, of_w);
+                                                        const float* __restrict__ gr,
+                                                        void* __restrict__ out) {
+    const float f = *factor;
     const int64_t total = rows * d, step = static_cast<int64_t>(gridDim.x) * 256;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
         const int64_t r = i / d;
@@ -676,7 +865,7 @@ __global__ __launch_bounds__(256) void ce_finish_kernel(const float* __restrict_
                 for (int j = 0; j < 8; ++j) x += v[j];
             }
             for (; k < splits; ++k) x += from[k * stride * d];
-            x = s(x);
+            x *= gr != nullptr ? gr[at] : f;
         }
         T::store(out, i, x);
     }
@@ -1217,6 +1406,8 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
 int64_t up64(int64_t x) { return (x + 63) & ~int64_t{63}; }
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t{255}; }
 
+int64_t tiled(int64_t rows) { return ceil_div(rows, kTileM) * kTileM; }
+
 struct Carve {
     int64_t at = 0;
     int64_t take(int64_t bytes) {
@@ -1227,7 +1418,7 @@ struct Carve {
 };
 
 struct Saved {
-    int64_t header, rows, pos, tgt, norm, h, w, z, live, bytes;
+    int64_t header, rows, pos, tgt, norm, hx, wx, h, w, z, live, bytes;
 };
 
 bool split_of(const slk_linear_ce* a) { return a->dtype == SLK_F32; }
@@ -1270,6 +1461,8 @@ Saved saved_of(const slk_linear_ce* a) {
     s.pos = c.take(4 * a->n);
     s.tgt = c.take(4 * a->n);
     s.norm = c.take(8 * a->n);
+    s.hx = c.take(split_of(a) ? 4 * a->n : 0);
+    s.wx = c.take(split_of(a) ? 4 * tiled(a->v) : 0);
     s.h = c.take(stages(a, a->d) * up64(a->n) * kStageBytes);
     s.w = c.take(stages(a, a->d) * up64(a->v) * kStageBytes);
     s.bytes = c.at;
@@ -1303,7 +1496,7 @@ Forward forward_of(const slk_linear_ce* a) {
 }
 
 // Vocabulary rows of a piece of the backward: dl of a piece takes at most
-// kDlBytes.
+// kDlBytes, and as much again in float32 as dh's operand.
 constexpr int64_t kDlBytes = int64_t{1} << 29;
 
 // Parts of a product's K loop. With one workgroup a CU, tiles·s of them take
@@ -1331,7 +1524,8 @@ int splits_for(int64_t m, int64_t n, int64_t nst) {
 struct Backward {
     int64_t piece;  // rows of a piece, a multiple of kTileM
     int sh, sw;     // parts of the two products
-    int64_t gr, factor, pos, dl, dl_rows, dh, dw, bytes;
+    int64_t gr, factor, pos, dl, dlh, dl_rows, dh, dw, bytes;
+    int64_t row_part, col_part, row_exp, col_exp;  // float32
 };
 Backward backward_of(const slk_linear_ce* a) {
     Backward b{};
@@ -1384,6 +1578,13 @@ Backward backward_of(const slk_linear_ce* a) {
     b.factor = c.take(4);
     b.gr = c.take(4 * a->n);
     b.dl = c.take(stages(a, b.piece) * b.dl_rows * kStageBytes);
+    if (split_of(a)) {
+        b.dlh = c.take(a->dhidden != nullptr ? stages(a, b.piece) * b.dl_rows * kStageBytes : 0);
+        b.row_part = c.take(4 * b.piece / kTileM * b.dl_rows);
+        b.col_part = c.take(4 * b.dl_rows / kTileN * b.piece);
+        b.row_exp = c.take(4 * b.dl_rows);
+        b.col_exp = c.take(4 * b.piece);
+    }
     const bool whole = b.sh == 1 && b.piece >= a->v;
     b.dh = c.take(a->dhidden != nullptr && !whole ? 4 * b.sh * a->n * a->d : 0);
     b.dw = c.take(a->dweight != nullptr && b.sw > 1 ? 4 * b.sw * b.piece * a->d : 0);
@@ -1486,6 +1687,8 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
         int32_t* rows = reinterpret_cast<int32_t*>(sv + s.rows);
         int32_t* pos = reinterpret_cast<int32_t*>(sv + s.pos);
         int32_t* tgt = reinterpret_cast<int32_t*>(sv + s.tgt);
+        int32_t* hx = reinterpret_cast<int32_t*>(sv + s.hx);
+        int32_t* wx = reinterpret_cast<int32_t*>(sv + s.wx);
         hipLaunchKernelGGL(ce_list_kernel, dim3(1), dim3(kListThreads), 0, st, a->target, a->n,
                            a->v, a->ignore_index, hd, rows, pos, tgt);
         if ((rc = check_launch("linear_ce list")) != SLK_OK) return rc;
@@ -1495,19 +1698,20 @@ int forward(const slk_linear_ce* a, hipStream_t st) {
             const bool vec = a->d % 4 == 0 && aligned_to(a->hidden, 16) && aligned_to(a->weight, 16);
             auto go = [&](auto k) {
                 hipLaunchKernelGGL(k, grid, dim3(256), 0, st, static_cast<const float*>(a->hidden),
-                                   a->n, static_cast<const float*>(a->weight), a->v, a->d, pos, hd);
+                                   a->n, static_cast<const float*>(a->weight), a->v, tiled(a->v),
+                                   a->d, pos, hx, wx);
             };
-            if (vec) go(ce_top_kernel<true>);
-            else go(ce_top_kernel<false>);
-            if ((rc = check_launch("linear_ce top")) != SLK_OK) return rc;
+            if (vec) go(ce_exp_kernel<true>);
+            else go(ce_exp_kernel<false>);
+            if ((rc = check_launch("linear_ce scales")) != SLK_OK) return rc;
         }
-        const PackArgs ph{a->hidden, rows, &hd->live, hd, false, a->n, a->d, up64(a->n), sv + s.h};
-        const PackArgs pw{a->weight, nullptr, nullptr, hd, true, a->v, a->d, up64(a->v), sv + s.w};
+        const PackArgs ph{a->hidden, rows, &hd->live, hx, a->n, a->d, up64(a->n), sv + s.h};
+        const PackArgs pw{a->weight, nullptr, nullptr, wx, a->v, a->d, up64(a->v), sv + s.w};
         if ((rc = pack<T, SPLIT>(ph, st)) != SLK_OK) return rc;
         if ((rc = pack<T, SPLIT>(pw, st)) != SLK_OK) return rc;
         const MmaArgs g{sv + s.w, sv + s.h, a->v, a->n, stages(a, a->d), up64(a->v), up64(a->n),
                         &hd->live, kLiveN, 1};
-        rc = mma<SPLIT, false, false>(g, ScoreEpi<SPLIT>{hd, tgt, part, zt, a->n}, st,
+        rc = mma<SPLIT, false, false>(g, ScoreEpi<SPLIT>{wx, hx, tgt, part, zt, a->n}, st,
                                       "linear_ce logits");
         j.pos = pos;
         j.tgt = tgt;
@@ -1575,9 +1779,9 @@ int backward_few(const slk_linear_ce* a, hipStream_t st) {
     int rc = check_launch("linear_ce few backward");
     if (rc != SLK_OK || sums == nullptr) return rc;
     const int64_t g = ceil_div(nfew * a->d, 256);
-    hipLaunchKernelGGL((ce_finish_kernel<T, false>),
-                       dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st, sums,
-                       b.sh, nfew, nfew, a->d, pos, nullptr, factor, false, few_out);
+    hipLaunchKernelGGL(ce_finish_kernel<T>, dim3(static_cast<unsigned>(g < 8192 ? g : 8192)),
+                       dim3(256), 0, st, sums, b.sh, nfew, nfew, a->d, pos, factor, nullptr,
+                       few_out);
     return check_launch("linear_ce finish");
 }
 
@@ -1606,29 +1810,57 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     float* dh = reinterpret_cast<float*>(sc + b.dh);
     float* dw = reinterpret_cast<float*>(sc + b.dw);
     auto finish = [&](const float* sums, int splits, int64_t r, int64_t stride,
-                      const int32_t* ps, bool of_w, void* out) {
+                      const int32_t* ps, const float* each, void* out) {
         const int64_t g = ceil_div(r * a->d, 256);
-        hipLaunchKernelGGL((ce_finish_kernel<T, SPLIT>),
-                           dim3(static_cast<unsigned>(g < 8192 ? g : 8192)), dim3(256), 0, st,
-                           sums, splits, r, stride, a->d, ps, hd, factor, of_w, out);
+        hipLaunchKernelGGL(ce_finish_kernel<T>, dim3(static_cast<unsigned>(g < 8192 ? g : 8192)),
+                           dim3(256), 0, st, sums, splits, r, stride, a->d, ps, factor, each, out);
         return check_launch("linear_ce finish");
     };
+    const float* each = a->reduction == SLK_REDUCE_NONE ? gr : nullptr;
+    // bfloat16: dl holds each token's upstream gradient already
+    const float* each_h = SPLIT ? each : nullptr;
+    auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(sc + at); };
+    int32_t* row_exp = SPLIT ? ints(b.row_exp) : nullptr;
+    int32_t* col_exp = SPLIT ? ints(b.col_exp) : nullptr;
+    char* dlh = SPLIT ? sc + b.dlh : sc + b.dl;  // dh's operand
     for (int64_t v0 = 0; v0 < a->v; v0 += b.piece) {
         const int64_t vn = a->v - v0 < b.piece ? a->v - v0 : b.piece;
         const MmaArgs gl{sv + s.w + v0 * kStageBytes, sv + s.h, vn, a->n, stages(a, a->d),
                          up64(a->v), up64(a->n), &hd->live, kLiveN, 1};
-        const DlEpi<SPLIT> el{hd, tgt, norm, a->reduction == SLK_REDUCE_NONE ? gr : nullptr,
-                              sc + b.dl, v0, b.dl_rows};
-        if ((rc = mma<SPLIT, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+        if constexpr (SPLIT) {
+            const int32_t* hx = reinterpret_cast<const int32_t*>(sv + s.hx);
+            const int32_t* wx = reinterpret_cast<const int32_t*>(sv + s.wx) + v0;
+            const DlEpi<true> el{wx, hx, tgt, norm, each, sc + b.dl, v0, b.dl_rows,
+                                 ints(b.row_part), ints(b.col_part), b.piece};
+            if ((rc = mma<true, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+            const TermArgs ta{ints(b.row_part), ints(b.col_part), &hd->live, b.dl_rows, b.piece, vn,
+                              mma_wide(vn, a->n, 1) ? kWideN : kTileN, row_exp, col_exp};
+            hipLaunchKernelGGL(ce_term_kernel,
+                               dim3(static_cast<unsigned>((b.dl_rows + b.piece) / 32)), dim3(256),
+                               0, st, ta);
+            if ((rc = check_launch("linear_ce terms")) != SLK_OK) return rc;
+            const DlArgs da{sc + b.dl, a->dhidden != nullptr ? dlh : nullptr,
+                            a->dweight != nullptr, wx, hx, row_exp, col_exp, each, &hd->live,
+                            b.dl_rows};
+            hipLaunchKernelGGL(ce_split_kernel,
+                               dim3(static_cast<unsigned>(ceil_div(up64(a->n), 256)),
+                                    static_cast<unsigned>(stages(a, vn))),
+                               dim3(256), 0, st, da);
+            if ((rc = check_launch("linear_ce split")) != SLK_OK) return rc;
+        } else {
+            const DlEpi<false> el{tgt, norm, each, sc + b.dl, v0, b.dl_rows};
+            if ((rc = mma<false, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+        }
         if (a->dhidden != nullptr) {
             // dh = dl·W: W's rows, from v0, run along K
-            const MmaArgs g{sc + b.dl, sv + s.w + v0 * kStageBytes, a->n, a->d, stages(a, vn),
+            const MmaArgs g{dlh, sv + s.w + v0 * kStageBytes, a->n, a->d, stages(a, vn),
                             b.dl_rows, up64(a->v), &hd->live, kLiveM, b.sh};
             if (whole) {
-                rc = mma<SPLIT, false, true>(g, TokenEpi<T, SPLIT>{hd, factor, rows, a->dhidden,
-                                                                   a->d}, st, "linear_ce dhidden");
+                rc = mma<SPLIT, false, true>(
+                    g, TokenEpi<T, SPLIT>{row_exp, factor, each_h, rows, a->dhidden, a->d}, st,
+                    "linear_ce dhidden");
             } else {
-                rc = mma<SPLIT, false, true>(g, SumEpi{dh, a->n, a->d, v0 > 0}, st,
+                rc = mma<SPLIT, false, true>(g, SumEpi<SPLIT>{dh, row_exp, a->n, a->d, v0 > 0}, st,
                                              "linear_ce dhidden");
             }
             if (rc != SLK_OK) return rc;
@@ -1639,17 +1871,17 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
                             up64(a->n), &hd->live, kLiveK, b.sw};
             void* out = static_cast<char*>(a->dweight) + v0 * a->d * T::kBytes;
             if (b.sw == 1) {
-                rc = mma<SPLIT, true, true>(g, WeightEpi<T, SPLIT>{hd, factor, out, a->d}, st,
+                rc = mma<SPLIT, true, true>(g, WeightEpi<T, SPLIT>{col_exp, factor, out, a->d}, st,
                                             "linear_ce dweight");
             } else {
-                rc = mma<SPLIT, true, true>(g, SumEpi{dw, b.piece, a->d, false}, st,
+                rc = mma<SPLIT, true, true>(g, SumEpi<SPLIT>{dw, col_exp, b.piece, a->d, false}, st,
                                             "linear_ce dweight");
-                if (rc == SLK_OK) rc = finish(dw, b.sw, vn, b.piece, nullptr, true, out);
+                if (rc == SLK_OK) rc = finish(dw, b.sw, vn, b.piece, nullptr, nullptr, out);
             }
             if (rc != SLK_OK) return rc;
         }
     }
-    if (a->dhidden != nullptr && !whole) rc = finish(dh, b.sh, a->n, a->n, pos, false, a->dhidden);
+    if (a->dhidden != nullptr && !whole) rc = finish(dh, b.sh, a->n, a->n, pos, each_h, a->dhidden);
     return rc;
 }
 

@@ -7,7 +7,7 @@
 //   SPLIT   32 elements in float16, high parts (64 bytes) then low parts: a
 //           float32 x, scaled by a power of two, as hi + lo. The product takes
 //           hi·hi + hi·lo + lo·hi in float32: x is kept to 2^-22 of itself (or
-//           2^-39 of the operand's largest element), about float32's own
+//           2^-39 of its row's largest element), about float32's own
 //           rounding, at a third of the float16 rate, where the matrix cores'
 //           float32 instructions run at a sixteenth;
 //   else    64 elements in bfloat16.

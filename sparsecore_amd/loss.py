@@ -86,8 +86,10 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
             "none" (a loss per token, in target's shape).
 
     Returns the float32 loss, with gradients for hidden and weight. float32 products are
-    about as exact as float32 matrix products; bfloat16 gradients pass through logit
-    gradients rounded to bfloat16 where there are many. A forward that a backward may
+    about as exact as float32 matrix products, measured row by row: an element of hidden
+    or weight keeps 22 bits down to 2^-39 of the largest in its row, a token's (a class's)
+    terms of the gradient down to 2^-39 of its own largest. bfloat16 gradients pass
+    through logit gradients rounded to bfloat16 where there are many. A forward that a backward may
     follow keeps weight and hidden once more, packed, until then; with few tokens (at most
     64, 32 in bfloat16) or a small vocabulary (128) the logits instead. hidden, weight and
     target must not change in place before the backward. Results repeat bit for bit.

@@ -1,0 +1,183 @@
+"""linear_cross_entropy where rows of its operands differ by many powers of ten, and where
+its packed kernels (more than 128 tokens over more than 128 rows of vocabulary) are what
+runs. The definition is computed in float64.
+
+Bounds. A packed float32 operand keeps 22 bits of an element (2^-22, with the dropped
+product of two low parts) down to 2^-39 of its row's largest, and sums are float32 (about
+2^-24 a term's magnitude, few hundred terms in random signs): with a = the row maxima of h
+and b those of W, a logit is off by at most
+
+    e_z = 2^-20 Σ|h w| + 2^-38 (a Σ|w| + b Σ|h|).
+
+p = exp(z - lse) is off by p (exp(2 max e_z + 2e-6) - 1). A product C = A·B whose K runs
+over B's packed rows of largest magnitude β, where A was scaled by its rows' largest terms,
+is off by 2^-20 Σ|A||B| + 2^-37 (Σ|A|β + K max|A|β). Where the kernels use float32
+instructions (few tokens, a small vocabulary) the same bounds hold with room.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import sparsecore_amd as slk
+
+pytestmark = pytest.mark.gpu
+
+U20, U37, U38 = 2.0 ** -20, 2.0 ** -37, 2.0 ** -38
+
+
+def product(a, b, ea):
+    """a·b and its bound, a off by ea."""
+    c = a @ b
+    beta = b.abs().amax(1)
+    terms = a.abs() @ beta
+    most = (a.abs() * beta).amax(1)
+    err = ea @ b.abs() + U20 * (a.abs() @ b.abs()) \
+        + (U37 * (terms + b.shape[0] * most))[:, None]
+    return c, err
+
+
+def reference(h, w, t, up):
+    """(losses, dh, dw) as (value, bound) pairs, for upstream gradients of each token."""
+    h, w, up = h.detach().double(), w.detach().double(), up.double()
+    live = t != -100
+    h = torch.where(live[:, None], h, 0.0)
+    hit = (t[:, None] == torch.arange(w.shape[0], device=t.device)).double()
+    z = h @ w.t()
+    ez = U20 * (h.abs() @ w.abs().t()) + U38 * (
+        h.abs().amax(1)[:, None] * w.abs().sum(1) + w.abs().amax(1) * h.abs().sum(1)[:, None])
+    e = 2 * ez.amax(1, keepdim=True) + 2e-6
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    losses = torch.where(live, lse.squeeze(1) - (z * hit).sum(1), 0.0)
+    loss_err = torch.where(live, e.squeeze(1) + 2e-6 * (1 + lse.squeeze(1).abs()
+                                                      + (z * hit).sum(1).abs()), 0.0)
+    p = torch.exp(z - lse)
+    ep = p * torch.expm1(e.clamp(max=80.0)) + 2.0 ** -126
+    g = torch.where(live, up, 0.0)[:, None]
+    # target's p - 1 rounds at 2^-24 of 1 where p is near 1
+    dl, edl = (p - hit) * g, (ep + 2.0 ** -24 * hit) * g.abs()
+    dh, dw = product(dl, w, edl), product(dl.t(), h, edl.t())
+    return (losses, loss_err), dh, dw
+
+
+def within(got, pair, what):
+    want, err = pair
+    far = (got.detach().double() - want).abs() - err
+    assert bool((far <= 0).all()), f"{what}: {int((far > 0).sum())} beyond, by {float(far.max()):.3g}"
+
+
+def inputs(n, d, v, dev, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, d, generator=g).to(dtype).to(dev)
+    w = (torch.randn(v, d, generator=g) * 2 / math.sqrt(d)).to(dtype).to(dev)
+    return h, w, torch.randint(0, v, (n,), generator=g).to(dev)
+
+
+def check(h, w, t, up=None, reduction="none"):
+    n = t.numel()
+    up = torch.ones(n, device=h.device) if up is None else up
+    h, w = h.clone().requires_grad_(), w.clone().requires_grad_()
+    losses, dh, dw = reference(h, w, t, up)
+    loss = slk.linear_cross_entropy(h, w, t, reduction="none")
+    within(loss, losses, "loss")
+    gh, gw = torch.autograd.grad(loss, [h, w], up)
+    within(gh, dh, "dh")
+    within(gw, dw, "dw")
+
+
+def mixed(n, low, high, dev, seed):
+    """n powers of ten between 10^low and 10^high, in no order."""
+    s = torch.logspace(low, high, n, dtype=torch.float64)
+    return s[torch.randperm(n, generator=torch.Generator().manual_seed(seed))].float().to(dev)
+
+
+SIZES = [(40, 64, 300), (300, 64, 520), (700, 130, 1500), (300, 64, 65)]
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("low,high", [(-6, 0), (-6, 6), (-12, 0)])
+def test_hidden_states_of_any_magnitude(dev, n, d, v, low, high):
+    h, w, t = inputs(n, d, v, dev, 1)
+    check(h * mixed(n, low, high, dev, 1)[:, None], w, t)
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("low,high", [(-6, 0), (-12, 0), (-8, 4)])
+def test_rows_of_the_head_of_any_magnitude(dev, n, d, v, low, high):
+    h, w, t = inputs(n, d, v, dev, 2)
+    check(h, w * mixed(v, low, high, dev, 2)[:, None], t)
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_upstream_gradients_of_any_magnitude(dev, n, d, v):
+    h, w, t = inputs(n, d, v, dev, 3)
+    check(h, w, t, mixed(n, -12, 0, dev, 3))
+    check(h, w, t, mixed(n, -30, 6, dev, 4))
+    check(h * mixed(n, -4, 0, dev, 5)[:, None], w * mixed(v, -6, 0, dev, 6)[:, None], t,
+          mixed(n, -6, 6, dev, 7))
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("big", [1e5, 1e8])
+def test_one_large_token_leaves_the_others_alone(dev, n, d, v, big):
+    """One element of one token, as models have in their first tokens, and one of a row
+    of the head."""
+    h, w, t = inputs(n, d, v, dev, 4)
+    h[7, 3] = big
+    check(h, w, t)
+    h, w, t = inputs(n, d, v, dev, 5)
+    w[v // 2, 1] = big
+    h[:, 1] = h[:, 1].abs() * -1.0  # the row's logits are far below the others'
+    check(h, w, t)
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_rows_that_softmax_hardly_reaches(dev, n, d, v):
+    """Half of the vocabulary with probabilities near 1e-12 and no token's target: the
+    gradient of its rows is that small, and as exact as the others'."""
+    h, w, t = inputs(n, d, v, dev, 6)
+    h[:, 0] = 1.0
+    w[:, 0] = 0.0
+    w[v // 2:, 0] = -24.0
+    t %= v // 2
+    check(h, w, t)
+    gw, = torch.autograd.grad(slk.linear_cross_entropy(h, w.requires_grad_(), t), w)
+    assert bool((gw[v // 2:, 1:] != 0).any(1).all())
+
+
+def test_pieces_keep_their_own_scales(dev):
+    """More logits than a piece of the backward holds, rows of the head from 1e-9 to 1:
+    dh adds pieces that were scaled differently."""
+    n, d, v = 4200, 40, 70000
+    h, w, t = inputs(n, d, v, dev, 7)
+    w *= torch.logspace(-9, 0, v, device=dev)[:, None]
+    up = mixed(n, -6, 0, dev, 8)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    gh, gw = torch.autograd.grad(slk.linear_cross_entropy(h, w, t, reduction="none"), [h, w], up)
+    some = torch.arange(0, n, 97, device=dev)
+    _, dh, _ = reference(h[some], w, t[some], up[some])
+    within(gh[some], dh, "dh")
+    # rows of dw need all tokens' softmax: lse once, then a block of rows at a time
+    hd, wd = h.detach().double(), w.detach().double()
+    lse = torch.cat([torch.logsumexp(x @ wd.t(), 1) for x in hd.split(300)])[:, None]
+    for lo in range(0, v, 7000):
+        rows = slice(lo, lo + 7000)
+        z = hd @ wd[rows].t()
+        p = torch.exp(z - lse)
+        hit = (t[:, None] == torch.arange(v, device=dev)[rows]).double()
+        dl = (p - hit) * up.double()[:, None]
+        edl = (p * 1e-4 + 2.0 ** -24 * hit) * up.double()[:, None]  # |z| below 10: e_z below 2e-5
+        within(gw[rows], product(dl.t(), hd, edl.t()), f"dw from {lo}")
+
+
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_extreme_magnitudes_stay_finite(dev, n, d, v):
+    """Tiny rows of one operand against huge ones of the other: no power of two in
+    between overflows or is lost."""
+    h, w, t = inputs(n, d, v, dev, 9)
+    check(h * 1e30, w * 1e-30, t)
+    check(h * 1e-30, w * 1e30, t)
+    check(h * 1e-36, w * 1e-3, t)
