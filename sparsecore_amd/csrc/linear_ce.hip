@@ -267,20 +267,20 @@ __device__ __forceinline__ void unscale_logits(f32x16 (&acc)[Tile::kNA][2], cons
     }
 }
 
-// Logits are exponentiated in base 2: the factor log2(e) goes into the scale of
-// the accumulator, and v_exp_f32 is one instruction (1 ulp). Maxima, sums and
-// targets' logits travel in base 2 too (m, s = Σ 2^(z·log2 e - m)). A token keeps
-// m and 1/s rather than the logarithm of its sum: 2^(z' - m) / s is then as exact
-// as the difference, where a rounded logarithm near 20 would put 1e-6 into every
-// entry of the token's softmax; and m - z' of a token whose target has the
-// largest logit is 0 exactly.
+// exp(x) as 2^(x·log2 e): v_exp_f32 is one instruction (1 ulp). The difference from
+// the maximum is taken first, so that it rounds relative to itself: with log2 e inside
+// a fused multiply-add the product's rounding, half an ulp of the logit, stayed in the
+// exponent, and logits beyond 2^32 overflowed it. A token keeps m and 1/s rather than the
+// logarithm of its sum: exp(z - m) / s is then as exact as the difference, where a
+// rounded logarithm near 20 would put 1e-6 into every entry of the token's softmax; and
+// m - z of a token whose target has the largest logit is 0 exactly.
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // (m, s) joined with (m2, s2); an empty part has m = -inf, s = 0. A NaN stays in s.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
-    s = (m == -INFINITY ? s : s * exp2_(m - base)) + (m2 == -INFINITY ? s2 : s2 * exp2_(m2 - base));
+    s = (m == -INFINITY ? s : s * exp_(m - base)) + (m2 == -INFINITY ? s2 : s2 * exp_(m2 - base));
     m = top;
 }
 
@@ -298,7 +298,6 @@ struct ScoreEpi {
     __device__ __forceinline__ void operator()(f32x16 (&acc)[Tile::kNA][2], const Tile& t) const {
         __syncthreads();  // the ring is free
         float2* sh = reinterpret_cast<float2*>(t.lds);  // kWavesM x kBN
-        constexpr float scale2 = kLog2e;
         const int rows = static_cast<int>(t.M - t.m0());  // those of this wave that exist
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -311,7 +310,7 @@ struct ScoreEpi {
                 for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (t.row(a, r) == want) zt[tok] = acc[a][b][r] * scale2;
+                        if (t.row(a, r) == want) zt[tok] = acc[a][b][r];
             }
             float m = -INFINITY, s = 0.0f;
             if (rows < 32 * Tile::kNA) {  // past the vocabulary
@@ -325,12 +324,12 @@ struct ScoreEpi {
             for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[a][b][r]);
-            m = fmaxf(m, __shfl_xor(m, 32)) * scale2;  // the scale is positive
+            m = fmaxf(m, __shfl_xor(m, 32));
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int a = 0; a < Tile::kNA; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += exp2_(fmaf(acc[a][b][r], scale2, -base));
+                for (int r = 0; r < 16; ++r) s += exp_(acc[a][b][r] - base);
             s += __shfl_xor(s, 32);
             if (t.lane < 32) sh[t.wm * Tile::kBN + 64 * t.wn + t.col(b)] = make_float2(m, s);
         }
@@ -382,7 +381,7 @@ struct DlEpi {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = 4 * q + j;
-                        float p = exp2_(fmaf(acc[a][b][r], kLog2e, -ms.x)) * gs;
+                        float p = exp_(acc[a][b][r] - ms.x) * gs;
                         if (any && t.row(a, r) == want) p -= g;
                         p = in && t.row(a, r) < have ? p : 0.0f;
                         h[j] = f32_to_bf16(p);
@@ -470,7 +469,7 @@ struct DlEpi<true> {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float z = scaled(acc[a][b][4 * q + j], hexp[b] - we[j]);
-                        float p = exp2_(fmaf(z, kLog2e, -ms[b].x)) * ms[b].y;
+                        float p = exp_(z - ms[b].x) * ms[b].y;
                         if (any && row + j == want[b]) p -= 1.0f;
                         p = in[b] && row + j < have ? p : 0.0f;
                         x[j] = p;
@@ -767,7 +766,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const JoinArgs p) {
     }
     if (m == -INFINITY) m = 0.0f;
     if (p.norm != nullptr) p.norm[i] = make_float2(m, 1.0f / s);
-    p.losses[n] = valid ? ((m - p.zt[i]) + log2f(s)) * kLn2 : NAN;
+    p.losses[n] = valid ? (m - p.zt[i]) + log2f(s) * kLn2 : NAN;
 }
 
 // The sum or mean of the losses over the live tokens: one workgroup, sums in
@@ -1053,7 +1052,7 @@ __device__ __forceinline__ void few_forward(
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const int64_t vr = (blk * MB + a) * 16 + 4 * quarter + (SPLIT ? wv : r);
-                    float z = zs[a][b][r] * kLog2e;
+                    float z = zs[a][b][r];
                     if (vr == want[b]) zt[tok[b]] = z;
                     if (keep != nullptr && vr < v) keep[vr * pitch + tok[b]] = z;
                     if (vr >= v) z = -INFINITY;
@@ -1061,11 +1060,11 @@ __device__ __forceinline__ void few_forward(
                     top = fmaxf(top, z);
                 }
             const float base = top == -INFINITY ? 0.0f : top;
-            s[b] = m[b] == -INFINITY ? s[b] : s[b] * exp2_(m[b] - base);
+            s[b] = m[b] == -INFINITY ? s[b] : s[b] * exp_(m[b] - base);
 #pragma unroll
             for (int a = 0; a < MB; ++a)
 #pragma unroll
-                for (int r = 0; r < R; ++r) s[b] += exp2_(zs[a][b][r] - base);
+                for (int r = 0; r < R; ++r) s[b] += exp_(zs[a][b][r] - base);
             m[b] = top;
         }
     }
@@ -1154,7 +1153,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_small_kernel(
             float m = -INFINITY, s = 0.0f, zt = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float z = zs[a][b] * kLog2e;
+                const float z = zs[a][b];
                 if (keep != nullptr && tok < n) keep[tok * kVoc + 16 * b + col] = z;
                 if (16 * b + col == t) zt = z;
                 zs[a][b] = 16 * b + col < v ? z : -INFINITY;
@@ -1164,7 +1163,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_small_kernel(
             for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
             if (m == -INFINITY) m = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) s += exp2_(zs[a][b] - m);
+            for (int b = 0; b < NB; ++b) s += exp_(zs[a][b] - m);
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) {
                 s += __shfl_xor(s, o);
@@ -1172,7 +1171,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_small_kernel(
             }
             if (col != 0 || tok >= n) continue;
             const bool valid = t >= 0 && t < v;
-            losses[tok] = t == ignore ? 0.0f : valid ? ((m - zt) + log2f(s)) * kLn2 : NAN;
+            losses[tok] = t == ignore ? 0.0f : valid ? (m - zt) + log2f(s) * kLn2 : NAN;
             if (norm != nullptr) norm[tok] = make_float2(m, 1.0f / s);
         }
     }
@@ -1204,7 +1203,7 @@ struct FewArgs {
     int32_t* pos;
 };
 // What a token's column (few tokens) or row (small vocabulary) of dl takes:
-// p = exp2(z - m)·gs, less g at hit. gs = g / s; hit -1: none, -2: ignored.
+// p = exp(z - m)·gs, less g at hit. gs = g / s; hit -1: none, -2: ignored.
 struct FewToken {
     float m, gs, g;
     int hit;
@@ -1331,7 +1330,7 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
         for (int k = 0; k < kEach; ++k) {
             const int at = k * kFewThreads + threadIdx.x, row = at / kFew, i = at % kFew;
             const FewToken t = mine_tokens[SMALL ? row : i];
-            float g = exp2_(zs[k] - t.m) * t.gs;
+            float g = exp_(zs[k] - t.m) * t.gs;
             if ((SMALL ? i : r0 + row) == t.hit) g -= t.g;
             dl[buf][row * kPitch + i] = r0 + row < r_1 && i < p.nfew && t.hit != -2 ? g : 0.0f;
         }

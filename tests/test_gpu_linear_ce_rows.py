@@ -121,7 +121,7 @@ def test_upstream_gradients_of_any_magnitude(dev, n, d, v):
 
 
 @pytest.mark.parametrize("n,d,v", SIZES)
-@pytest.mark.parametrize("big", [1e5, 1e8])
+@pytest.mark.parametrize("big", [1e5, 1e8, 1e12])
 def test_one_large_token_leaves_the_others_alone(dev, n, d, v, big):
     """One element of one token, as models have in their first tokens, and one of a row
     of the head."""
@@ -181,3 +181,36 @@ def test_extreme_magnitudes_stay_finite(dev, n, d, v):
     check(h * 1e30, w * 1e-30, t)
     check(h * 1e-30, w * 1e30, t)
     check(h * 1e-36, w * 1e-3, t)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(8, 64, 300), (40, 64, 300), (100, 64, 300), (300, 64, 520),
+                                   (700, 130, 1500), (300, 64, 65), (9000, 40, 65)])
+@pytest.mark.parametrize("power", [10, 30, 60, 110])
+def test_logits_of_any_size(dev, dtype, n, d, v, power):
+    """Whole numbers times 2^power: every product and sum is exact and the softmax is 0
+    but at the largest logits, which share it. One rounding of each result, of dl before it
+    (2^-8 in bfloat16), of the losses' difference and logarithm."""
+    g = torch.Generator().manual_seed(n + power)
+    h = torch.randint(-2, 3, (n, d), generator=g).double()
+    w = torch.randint(-2, 3, (v, d), generator=g).double()
+    t = torch.randint(0, v, (n,), generator=g)
+    z = h @ w.t()
+    top = z.amax(1, keepdim=True)
+    p = (z == top).double()
+    ties = p.sum(1, keepdim=True)
+    p /= ties
+    rest = (top - z.gather(1, t[:, None])).squeeze(1)
+    rest = torch.ldexp(rest, torch.tensor(power)) + ties.squeeze(1).log()
+    dl = p.scatter_add(1, t[:, None], -torch.ones(n, 1, dtype=torch.float64))
+    half = power // 2
+    hs, ws = torch.ldexp(h, torch.tensor(half)), torch.ldexp(w, torch.tensor(power - half))
+    hg = hs.to(dtype).to(dev).requires_grad_()
+    wg = ws.to(dtype).to(dev).requires_grad_()
+    loss = slk.linear_cross_entropy(hg, wg, t.to(dev), reduction="none")
+    assert bool(((loss.double().cpu() - rest).abs() <= 1e-6 * rest.abs() + 1e-6).all())
+    gh, gw = torch.autograd.grad(loss, [hg, wg], torch.ones(n, device=dev))
+    u = 2.0 ** -7 if dtype is torch.bfloat16 else 2.0 ** -19
+    for got, a, b in ((gh, dl, ws), (gw, dl.t(), hs)):
+        err = (got.double().cpu() - a @ b).abs() - u * (a.abs() @ b.abs())
+        assert bool((err <= 0).all()), float(err.max())
