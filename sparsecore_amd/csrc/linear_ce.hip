@@ -1822,6 +1822,9 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
     int32_t* row_exp = SPLIT ? ints(b.row_exp) : nullptr;
     int32_t* col_exp = SPLIT ? ints(b.col_exp) : nullptr;
     char* dlh = SPLIT ? sc + b.dlh : sc + b.dl;  // dh's operand
+    // The tiles of the forward's logits, whatever the piece: logits summed in another
+    // order differ in their last bit, which is 6% of a softmax entry at 1e6.
+    const bool wide = mma_wide(a->v, a->n, 1);
     for (int64_t v0 = 0; v0 < a->v; v0 += b.piece) {
         const int64_t vn = a->v - v0 < b.piece ? a->v - v0 : b.piece;
         const MmaArgs gl{sv + s.w + v0 * kStageBytes, sv + s.h, vn, a->n, stages(a, a->d),
@@ -1831,9 +1834,10 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
             const int32_t* wx = reinterpret_cast<const int32_t*>(sv + s.wx) + v0;
             const DlEpi<true> el{wx, hx, tgt, norm, each, sc + b.dl, v0, b.dl_rows,
                                  ints(b.row_part), ints(b.col_part), b.piece};
-            if ((rc = mma<true, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+            rc = mma<true, false, false>(gl, el, st, "linear_ce dlogits", wide);
+            if (rc != SLK_OK) return rc;
             const TermArgs ta{ints(b.row_part), ints(b.col_part), &hd->live, b.dl_rows, b.piece, vn,
-                              mma_wide(vn, a->n, 1) ? kWideN : kTileN, row_exp, col_exp};
+                              wide ? kWideN : kTileN, row_exp, col_exp};
             hipLaunchKernelGGL(ce_term_kernel,
                                dim3(static_cast<unsigned>((b.dl_rows + b.piece) / 32)), dim3(256),
                                0, st, ta);
@@ -1848,7 +1852,8 @@ int backward(const slk_linear_ce* a, hipStream_t st) {
             if ((rc = check_launch("linear_ce split")) != SLK_OK) return rc;
         } else {
             const DlEpi<false> el{tgt, norm, each, sc + b.dl, v0, b.dl_rows};
-            if ((rc = mma<false, false, false>(gl, el, st, "linear_ce dlogits")) != SLK_OK) return rc;
+            rc = mma<false, false, false>(gl, el, st, "linear_ce dlogits", wide);
+            if (rc != SLK_OK) return rc;
         }
         if (a->dhidden != nullptr) {
             // dh = dl·W: W's rows, from v0, run along K

@@ -496,9 +496,8 @@ __global__ __launch_bounds__(kMmaThreads) void mma_wide_kernel(const MmaArgs g, 
                                 reinterpret_cast<char*>(ring0)});
 }
 
-// Launches C = A·Bᵀ over an upper bound of its tiles. Wide tiles where their
-// rounds on the card's 256 CUs take no longer: a wide stage takes about 1.7
-// times a small one's.
+// Wide tiles where their rounds on the card's 256 CUs take no longer: a wide stage
+// takes about 1.7 times a small one's.
 inline bool mma_wide(int64_t M, int64_t N, int splits) {
     const int64_t small = ceil_div(ceil_div(M, kTileM) * ceil_div(N, kTileN) * splits, 256);
     const int64_t wide = ceil_div(ceil_div(M, kTileM) * ceil_div(N, kWideN) * splits, 256);
@@ -512,9 +511,11 @@ inline double mma_rounds(int64_t M, int64_t N) {
     return static_cast<double>(ceil_div(tiles, 256)) * (wide ? 1.7 : 1.0);
 }
 
+// Launches C = A·Bᵀ over an upper bound of its tiles. The two widths add the terms of
+// a stage in different orders: a product that has to repeat another's bits names its
+// width.
 template <bool SPLIT, bool TA, bool TB, class Epi>
-int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
-    const bool wide = mma_wide(g.M, g.N, g.splits);
+int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who, bool wide) {
     const int64_t groups =
         ceil_div(g.M, kTileM) * ceil_div(g.N, wide ? kWideN : kTileN) * g.splits;
     if (groups == 0) return SLK_OK;
@@ -523,6 +524,11 @@ int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
     if (wide) hipLaunchKernelGGL((mma_wide_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);
     else hipLaunchKernelGGL((mma_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);
     return check_launch(who);
+}
+
+template <bool SPLIT, bool TA, bool TB, class Epi>
+int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who) {
+    return mma<SPLIT, TA, TB>(g, epi, st, who, mma_wide(g.M, g.N, g.splits));
 }
 
 }  // namespace slk

@@ -214,3 +214,28 @@ def test_logits_of_any_size(dev, dtype, n, d, v, power):
     for got, a, b in ((gh, dl, ws), (gw, dl.t(), hs)):
         err = (got.double().cpu() - a @ b).abs() - u * (a.abs() @ b.abs())
         assert bool((err <= 0).all()), float(err.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(2100, 40, 60000), (700, 130, 1500)])
+def test_the_backwards_logits_are_the_forwards(dev, dtype, n, d, v):
+    """Logits near 1e6, whose last bit is 0.06: where the largest stands 40 above the
+    others the softmax is 1 there, to the last bit if both passes sum in the same order,
+    and dh = W[largest] - W[target] (in the first size a piece of the backward has other
+    tiles than the whole vocabulary)."""
+    h, w, t = inputs(n, d, v, dev, 10, dtype)
+    w = (w.double() / w.double().norm(dim=1, keepdim=True)).to(dtype)  # the largest: by angle
+    h = (h.double() * (1e6 / h.double().norm(dim=1, keepdim=True))).to(dtype)
+    top = torch.empty(n, dtype=torch.int64, device=dev)
+    alone = torch.empty(n, dtype=torch.bool, device=dev)
+    for i in range(0, n, 300):
+        z, at = (h[i:i + 300].double() @ w.double().t()).topk(2, dim=1)
+        top[i:i + 300], alone[i:i + 300] = at[:, 0], z[:, 0] - z[:, 1] > 40
+    assert int(alone.sum()) > n // 2
+    h.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t, reduction="none")
+    gh, = torch.autograd.grad(loss, h, torch.ones(n, device=dev))
+    want = w.double()[top] - w.double()[t]
+    u = 2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -19
+    err = (gh.double() - want).abs() - u * (w.double()[top].abs() + w.double()[t].abs())
+    assert bool((err[alone] <= 0).all()), float(err[alone].max())
