@@ -1243,23 +1243,14 @@ __global__ __launch_bounds__(kFewThreads) void ce_few_back_kernel(const FewArgs 
             top_factor = f;
             if (blockIdx.x == 0 && blockIdx.y == 0) *p.factor = f;
         }
-    } else if (wv == 0) {  // the tokens' upstream gradients over the largest of them
+    } else if (wv == 0) {
         const bool in = lane < p.nfew;
         const int64_t t = in ? p.target[lane] : p.ignore;
         const bool live = in && t != p.ignore;
         const int count = __popcll(__ballot(live));
-        float g = 1.0f, f = 0.0f;
-        if (p.reduction != SLK_REDUCE_NONE) {
-            if (count > 0)
-                f = p.reduction == SLK_REDUCE_MEAN ? *p.up / static_cast<float>(count) : *p.up;
-        } else {
-            const float u = live ? p.up[lane] : 0.0f;
-            uint32_t m = __float_as_uint(u) & 0x7fffffffu;  // as bits, a NaN is the largest
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
-            f = __uint_as_float(m);
-            g = m == 0 ? 0.0f : u / f;
-        }
+        float g = 1.0f, f = 1.0f;
+        if (p.reduction == SLK_REDUCE_NONE) g = live ? p.up[lane] : 0.0f;
+        else f = count == 0 ? 0.0f : p.reduction == SLK_REDUCE_MEAN ? *p.up / count : *p.up;
         if (lane < kFew) tokens[lane] = token(lane, live, t, g);
         if (lane == 0) top_factor = f;
         if (blockIdx.x == 0 && blockIdx.y == 0) {

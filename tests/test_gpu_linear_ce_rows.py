@@ -239,3 +239,31 @@ def test_the_backwards_logits_are_the_forwards(dev, dtype, n, d, v):
     u = 2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -19
     err = (gh.double() - want).abs() - u * (w.double()[top].abs() + w.double()[t].abs())
     assert bool((err[alone] <= 0).all()), float(err[alone].max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(20, 64, 300), (40, 64, 300), (300, 64, 520), (300, 64, 65)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_one_tokens_upstream_gradient_reaches_its_own_dh_alone(dev, dtype, n, d, v, bad):
+    h, w, t = inputs(n, d, v, dev, 11, dtype)
+    t[4] = -100
+    h.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t, reduction="none")
+    up = torch.randn(n, generator=torch.Generator().manual_seed(12)).to(dev)
+    clean, = torch.autograd.grad(loss, h, up, retain_graph=True)
+    up[7] = bad
+    up[4] = bad  # ignored: reaches nothing
+    got, = torch.autograd.grad(loss, h, up)
+    keep = torch.arange(n, device=dev) != 7
+    assert torch.equal(got[keep], clean[keep])
+    assert not bool(torch.isfinite(got[7]).any()) and bool((got[4] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [20, 300])
+def test_upstream_gradients_that_are_all_zero(dev, dtype, n):
+    h, w, t = inputs(n, 64, 300, dev, 13, dtype)
+    h.requires_grad_(), w.requires_grad_()
+    loss = slk.linear_cross_entropy(h, w, t, reduction="none")
+    gh, gw = torch.autograd.grad(loss, [h, w], torch.zeros(n, device=dev))
+    assert bool((gh == 0).all()) and bool((gw == 0).all())
