@@ -1439,7 +1439,7 @@ int64_t few_blocks(const slk_linear_ce* a) {
 Saved saved_of(const slk_linear_ce* a) {
     Saved s{};
     Carve c;
-    if (few(a) || small(a)) {  // the logits themselves, far fewer than the long operand
+    if (few(a) || small(a)) {  // the logits themselves
         s.norm = c.take(8 * a->n);
         s.z = c.take((small(a) ? a->n : a->v) * few_blocks(a) * 64);
         s.live = c.take(4);
@@ -1486,7 +1486,8 @@ Forward forward_of(const slk_linear_ce* a) {
 }
 
 // Vocabulary rows of a piece of the backward: dl of a piece takes at most
-// kDlBytes, and as much again in float32 as dh's operand.
+// kDlBytes, or 256 rows over all tokens where those take more (from 2^19 tokens in
+// float32, 2^20 in bfloat16), and as much again in float32 as dh's operand.
 constexpr int64_t kDlBytes = int64_t{1} << 29;
 
 // Parts of a product's K loop. With one workgroup a CU, tiles·s of them take

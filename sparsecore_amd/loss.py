@@ -4,7 +4,8 @@
 
 without storing the logits: forward keeps a maximum and a sum of each token, backward
 computes the logits again a piece of the vocabulary at a time (``slk_linear_ce_*``). Only
-those of a few tokens or a small vocabulary, far smaller than the other operand, are kept.
+those of few tokens (at most 64 a row of the head) or of a small vocabulary (at most 128 a
+token) are kept.
 """
 
 from __future__ import annotations
@@ -92,7 +93,9 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100,
     through logit gradients rounded to bfloat16 where there are many. A forward that a backward may
     follow keeps weight and hidden once more, packed, until then; with few tokens (at most
     64, 32 in bfloat16) or a small vocabulary (128) the logits instead. hidden, weight and
-    target must not change in place before the backward. Results repeat bit for bit.
+    target must not change in place before the backward, whose scratch holds the logit
+    gradients of a piece of the vocabulary: at most 512 MiB (twice that in float32), or 256
+    rows over all tokens where those take more. Results repeat bit for bit.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, reduction).
