@@ -67,8 +67,10 @@ __device__ __forceinline__ int q8_encode_unsigned(float x, float scale, float rc
     return static_cast<int>(q);
 }
 
+// Of 0 or a subnormal scale the instruction gives inf, of one whose reciprocal would be
+// subnormal it may give 0: with inf, codes are the definition's.
 __device__ __forceinline__ float q8_reciprocal(float scale) {
-    return __builtin_amdgcn_rcpf(scale);  // of 0 or a subnormal: inf, and codes by definition
+    return scale < 0x1p126f ? __builtin_amdgcn_rcpf(scale) : INFINITY;
 }
 
 // The largest magnitude over the wave's block, four values a lane, or NaN if
