@@ -444,7 +444,7 @@ extern "C" int slk_adamw(const slk_adamw_tensor* tensors_host, int64_t n_tensors
             (state_bits == 8 && (t.exp_avg_scale == nullptr || t.exp_avg_sq_scale == nullptr))) {
             return fail(SLK_EINVAL, "adamw: NULL pointer in tensor " + std::to_string(i));
         }
-        if (ceil_div(t.n, kAdamSpan) > INT32_MAX) {
+        if (ceil_div(t.n, kAdamSpan) > max_groups(kAdamThreads)) {
             return fail(SLK_EINVAL, "adamw: tensor " + std::to_string(i) + " is too large");
         }
     }
@@ -472,7 +472,7 @@ extern "C" int slk_adamw(const slk_adamw_tensor* tensors_host, int64_t n_tensors
         const slk_adamw_tensor& t = tensors_host[i];
         if (t.n == 0) continue;
         const int64_t need = ceil_div(t.n, kAdamSpan);
-        if (tab.n == kAdamTensors || groups + need > INT32_MAX) {
+        if (tab.n == kAdamTensors || groups + need > max_groups(kAdamThreads)) {
             const int rc = launch();
             if (rc != SLK_OK) return rc;
         }
@@ -498,7 +498,7 @@ extern "C" int slk_q8_decode(const void* codes, const float* scales, int64_t n, 
         return fail(SLK_EINVAL, "q8_decode: NULL pointer");
     }
     const int64_t groups = ceil_div(n, kAdamSpan);
-    if (groups > INT32_MAX) return fail(SLK_EINVAL, "q8_decode: too large");
+    if (groups > max_groups(kAdamThreads)) return fail(SLK_EINVAL, "q8_decode: too large");
     const bool al = aligned_to(codes, 4) && aligned_to(out, 16);
     const dim3 grid(static_cast<unsigned>(groups)), wg(kAdamThreads);
     if (is_signed) {
@@ -521,7 +521,7 @@ extern "C" int slk_q8_encode(const float* x, int64_t n, int is_signed, void* cod
         return fail(SLK_EINVAL, "q8_encode: NULL pointer");
     }
     const int64_t groups = ceil_div(n, kAdamSpan);
-    if (groups > INT32_MAX) return fail(SLK_EINVAL, "q8_encode: too large");
+    if (groups > max_groups(kAdamThreads)) return fail(SLK_EINVAL, "q8_encode: too large");
     const bool al = aligned_to(codes, 4) && aligned_to(x, 16);
     const dim3 grid(static_cast<unsigned>(groups)), wg(kAdamThreads);
     if (is_signed) {

@@ -76,6 +76,9 @@ __device__ __forceinline__ int64_t wave_id() {
     return xcd_logical_block(blockIdx.x, gridDim.x) * (blockDim.x >> 6) + w;
 }
 
+// Workgroups of a launch: the threads of a dimension stay below 2^32.
+inline int64_t max_groups(int64_t threads) { return ((int64_t{1} << 32) - 1) / threads; }
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // bfloat16 bits to float32 (exact) and back (round to nearest, ties to even)

@@ -1599,6 +1599,12 @@ int validate(const slk_linear_ce* a, const char* who) {
         a->reduction != SLK_REDUCE_MEAN) {
         return fail(SLK_EINVAL, w + ": unknown reduction");
     }
+    if (a->n > 0 && !few(a) && !small(a) &&
+        ceil_div(a->v, kTileM) * ceil_div(a->n, mma_wide(a->v, a->n, 1) ? kWideN : kTileN) >
+            max_groups(kMmaThreads)) {
+        return fail(SLK_EINVAL, w + ": too many logits in a call: n=" + std::to_string(a->n) +
+                                    ", v=" + std::to_string(a->v));
+    }
     return SLK_OK;
 }
 

@@ -519,7 +519,9 @@ int mma(const MmaArgs& g, const Epi& epi, hipStream_t st, const char* who, bool 
     const int64_t groups =
         ceil_div(g.M, kTileM) * ceil_div(g.N, wide ? kWideN : kTileN) * g.splits;
     if (groups == 0) return SLK_OK;
-    if (groups > INT32_MAX) return fail(SLK_EINVAL, std::string(who) + ": too many tiles");
+    if (groups > max_groups(kMmaThreads)) {
+        return fail(SLK_EINVAL, std::string(who) + ": too many tiles");
+    }
     const dim3 grid(static_cast<unsigned>(groups)), wg(kMmaThreads);
     if (wide) hipLaunchKernelGGL((mma_wide_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);
     else hipLaunchKernelGGL((mma_kernel<SPLIT, TA, TB, Epi>), grid, wg, 0, st, g, epi);

@@ -187,7 +187,16 @@ int validate_norm(const slk_norm* a, const char* who, bool backward) {
     if (a->dtype != SLK_F32 && a->dtype != SLK_BF16) {
         return fail(SLK_EINVAL, w + ": dtype must be SLK_F32 or SLK_BF16");
     }
-    if (a->n > INT32_MAX) return fail(SLK_EINVAL, w + ": too many tokens");
+    // threads of a token: a tile has 16 tokens at least, a row kernel a team each
+    int64_t threads = kTileThreads / 16;
+    if (!a->branch_cols && !a->y_cols)
+        norm_shape(static_cast<int>(a->d), [&](auto, auto tw) { threads = tw * kWave; });
+    const int64_t most = max_groups(threads) - 64;  // (the last workgroup's may be idle)
+    if (a->n > most) {
+        return fail(SLK_EINVAL, w + ": at most " + std::to_string(most) + " tokens of d=" +
+                                    std::to_string(a->d) + " in a call, got n=" +
+                                    std::to_string(a->n));
+    }
     if ((a->branch_cols || a->y_cols) && a->d > SLK_NORM_COLS_MAX) {
         return fail(SLK_EINVAL, w + ": feature-major arrays need d <= " +
                                     std::to_string(SLK_NORM_COLS_MAX));
