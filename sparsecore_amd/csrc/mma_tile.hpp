@@ -42,7 +42,6 @@ constexpr int kStageK = SPLIT ? 32 : 64;
 constexpr int kTileM = 256, kTileN = 128;
 constexpr int kMmaThreads = 512;
 constexpr int kMmaBufs = 3;
-constexpr int kMmaLds = kMmaBufs * (kTileM + kTileN) * kStageBytes;
 constexpr int kMmaGroup = 4;  // tile rows of a group of the tile order
 
 // s_waitcnt operand: at most n vector-memory loads outstanding, no LDS reads

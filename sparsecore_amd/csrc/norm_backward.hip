@@ -5,6 +5,8 @@
 //   dweight = Σ dy ∘ xhat,  dbias = Σ dy     (over tokens)
 //   b    = do ∘ gate,   dpost_weight = Σ b ∘ uhat,  dpost_bias = Σ b
 //   du   = prstd·(a' - mean(a') - uhat·mean(a' ∘ uhat)),  a' = b ∘ post_weight
+// xhat comes from r as it was stored: rounded in bfloat16, where a second, unrounded copy
+// would cost the forward and this pass 4 bytes a feature each.
 // One pass over the arrays (24 bytes a feature in float32 without a gate),
 // bound by memory. The sums over tokens stay in each lane's registers over the
 // consecutive tokens of its team and are then written as partial rows, which a

@@ -200,8 +200,10 @@ def residual_norm(x, weight, bias=None, *, branch=None, gate=None, post_weight=N
             a SparseLinear takes it without a copy.
 
     All tensors share x's dtype; arithmetic, means and sums are float32, and y is
-    computed from the unrounded r. Every gradient is computed in one pass and repeats bit
-    for bit.
+    computed from the unrounded r. The backward reads r as it was returned, so in
+    bfloat16 its normalised values carry r's rounding (2^-9 of r, about 1.4 times the
+    error of gradients from an unrounded r), with the forward's own mean and deviation.
+    Every gradient is computed in one pass and repeats bit for bit.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, kind).
