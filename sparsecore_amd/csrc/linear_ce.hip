@@ -13,10 +13,10 @@
 // and what their hidden states hold reaches nothing.
 //
 // Bound by the matrix cores from some hundred tokens on. 8192 x 4096 x 100000
-// bfloat16, forward and backward: 21.5 ms, the logits at 1334 TFLOP/s, dhidden's
+// bfloat16, forward and backward: 21.5 to 22.4 ms, the logits at 1334 TFLOP/s, dhidden's
 // and dweight's products at 1305 and 1203 (a large library product: 1388). 4001 x
-// 768 x 32000 float32, 3 in 10 tokens ignored: 1.88 to 1.97 ms, 375 + 481 + 412 + 372
-// us in the four products (1100 TFLOP/s as float16), 289 in dl's two operands.
+// 768 x 32000 float32, 3 in 10 tokens ignored: 1.88 to 1.97 ms, 366 + 471 + 400 + 361
+// us in the four products (1100 TFLOP/s as float16), 290 in dl's two operands.
 //
 // Few tokens are bound by reading W, which they do where it lies: 8 x 2048 x
 // 80000 at 4.6 TB/s, forward. A small vocabulary goes the same way, tokens and
