@@ -306,8 +306,9 @@ class AdamW(torch.optim.Optimizer):
     Replays of a captured step do not: call ``follow()`` after each rewrite, before the
     next replay. The moments stay in their tensors, so the capture remains valid.
     A layer whose matrix was replaced (``load_state_dict``, ``reset_parameters``) is
-    attached again, after loading the optimizer's own state. A deep copy or an unpickled
-    optimizer has no layers attached: ``attach`` its own.
+    attached again, after loading the optimizer's own state. Moments are saved and copied
+    as of the layers' present topology; a deep copy or an unpickled optimizer has no layers
+    attached: ``attach`` its own.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -327,6 +328,22 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(g["lr"], torch.Tensor) and not g["capturable"]:
             raise ValueError("AdamW: a tensor lr needs capturable=True")
         super().add_param_group(group)
+
+    def _settle(self) -> None:
+        """What is saved fits the topology that the model is saved with. (Moments of a
+        layer whose matrix was replaced fit none: the next step refuses them.)"""
+        with torch.no_grad():
+            for p, at in self._attached.items():
+                if at.layer._csr is at.csr:
+                    self._follow(p)
+
+    def state_dict(self) -> dict:
+        self._settle()
+        return super().state_dict()
+
+    def __getstate__(self) -> dict:
+        self._settle()
+        return super().__getstate__()
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)

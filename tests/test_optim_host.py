@@ -224,3 +224,38 @@ def test_attaching_again_keeps_a_move_that_is_due(layer):
     opt.attach(layer)
     opt.step()
     assert torch.equal(s["exp_avg"], want)
+
+
+@pytest.mark.parametrize("how", ["state_dict", "deepcopy", "pickle"])
+def test_what_is_saved_after_a_rewrite_fits_the_new_slots(layer, how):
+    """A loop that steps, rewrites and then saves: the model is saved with the topology
+    after the rewrite, so the moments must be at that topology's slots."""
+    p = layer._values
+    opt = slk.AdamW([p])
+    opt.attach(layer)
+    opt.step()
+    s = opt.state[p]
+    s["exp_avg"].copy_(torch.arange(float(p.numel())))
+    old = layer._csr.col_indices.clone(), layer._csr.row_nnz.clone()
+    rewrite(layer)
+    want, = optim.carry_slots(layer._csr.row_start, old,
+                              (layer._csr.col_indices, layer._csr.row_nnz), [s["exp_avg"].clone()])
+    if how == "state_dict":
+        got = opt.state_dict()["state"][0]["exp_avg"]
+    else:
+        twin = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+        got = twin.state[twin.param_groups[0]["params"][0]]["exp_avg"]
+    assert torch.equal(got, want) and torch.equal(s["exp_avg"], want)
+
+
+def test_a_replaced_matrix_does_not_stop_a_checkpoint(layer):
+    opt = slk.AdamW([layer._values])
+    opt.attach(layer)
+    opt.step()
+    layer.load_state_dict({k: v.clone() for k, v in layer.state_dict().items()})
+    saved = opt.state_dict()
+    with pytest.raises(RuntimeError, match="attach"):
+        opt.step()
+    opt.load_state_dict(saved)
+    opt.step()
+    assert opt.state[layer._values]["step"] == 2
