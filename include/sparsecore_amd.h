@@ -805,8 +805,8 @@ SLK_API int slk_carry_slots(const int32_t* row_start, int64_t nrows, int64_t tot
  *   branch     NULL: y = pre(x), r is not written
  *   gate       gate_rows x d: row i serves the i-th n / gate_rows consecutive
  *              tokens (1: one gate for all, n: one each); NULL: none
- *   stats      n x 4 floats: mean and 1/deviation of pre, of post; forward
- *              writes them if not NULL, backward reads them
+ *   stats      n x 4 floats, 16-byte aligned: mean and 1/deviation of pre, of
+ *              post; forward writes them if not NULL, backward reads them
  * Backward: dr (NULL: zeros) and dy (NULL: zeros, no gradient of weight or
  * bias) in, r (x where there is no branch) and the forward's arrays in; every
  * gradient that is not NULL is written. workspace: device memory of
@@ -844,7 +844,8 @@ SLK_API int slk_norm_backward(const slk_norm* args_host, void* stream);
  *              or a small vocabulary the logits. backward reads it, and then also
  *              hidden, weight and target, unchanged since forward
  *   scratch    slk_linear_ce_scratch_bytes(args, backward) bytes; its dhidden
- *              and dweight as in the call (NULL: not wanted)
+ *              and dweight as in the call (NULL: not wanted). saved and scratch are
+ *              16-byte aligned
  * float32 products run on the float16 matrix instructions in two parts an
  * operand, 22 bits of an element down to 2^-39 of its row's largest (of the
  * logits' gradients: of a token's, a class's largest term), for few tokens or a

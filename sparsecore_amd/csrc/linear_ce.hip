@@ -1914,6 +1914,9 @@ extern "C" int slk_linear_ce_forward(const slk_linear_ce* a, void* stream) {
         a->scratch == nullptr || (a->saved == nullptr && saved_of(a).bytes > 0)) {
         return fail(SLK_EINVAL, "linear_ce_forward: saved or scratch too small");
     }
+    if (!aligned_to(a->saved, 16) || !aligned_to(a->scratch, 16)) {
+        return fail(SLK_EINVAL, "linear_ce_forward: saved and scratch must be 16-byte aligned");
+    }
     return a->dtype == SLK_F32 ? forward<F32, true>(a, as_stream(stream))
                                : forward<BF16, false>(a, as_stream(stream));
 }
@@ -1928,6 +1931,9 @@ extern "C" int slk_linear_ce_backward(const slk_linear_ce* a, void* stream) {
     if (a->scratch_bytes < backward_of(a).bytes || a->saved_bytes < saved_of(a).bytes ||
         a->scratch == nullptr || a->saved == nullptr) {
         return fail(SLK_EINVAL, "linear_ce_backward: saved or scratch too small");
+    }
+    if (!aligned_to(a->saved, 16) || !aligned_to(a->scratch, 16)) {
+        return fail(SLK_EINVAL, "linear_ce_backward: saved and scratch must be 16-byte aligned");
     }
     if ((few(a) || small(a)) &&
         (a->hidden == nullptr || a->weight == nullptr || a->target == nullptr)) {

@@ -222,6 +222,9 @@ int validate_norm(const slk_norm* a, const char* who, bool backward) {
                                   (a->branch != nullptr && a->r == nullptr))) {
         return fail(SLK_EINVAL, w + ": NULL x, r or y");
     }
+    if (!aligned_to(a->stats, 16)) {
+        return fail(SLK_EINVAL, w + ": stats must be 16-byte aligned");
+    }
     if (a->n > 0 && backward && (a->r == nullptr || a->stats == nullptr)) {
         return fail(SLK_EINVAL, w + ": NULL r or stats");
     }

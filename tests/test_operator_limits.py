@@ -48,3 +48,17 @@ def test_head():
     refused(lib.slk_linear_ce_backward(ctypes.byref(a), None), "too many logits")
     a.v -= 256
     refused(lib.slk_linear_ce_forward(ctypes.byref(a), None), "scratch too small")
+
+
+def test_alignment():
+    """The arrays that the kernels themselves lay out are read sixteen bytes at a time."""
+    lib = _lib.load()
+    a = _lib.LinearCE(n=200, d=64, v=300, hidden=16, weight=16, target=16, loss=16, upstream=16,
+                      dtype=0, reduction=0, keep=1, saved_bytes=1 << 40, scratch_bytes=1 << 40)
+    for a.saved, a.scratch in ((24, 32), (32, 24)):
+        refused(lib.slk_linear_ce_forward(ctypes.byref(a), None), "aligned")
+        refused(lib.slk_linear_ce_backward(ctypes.byref(a), None), "aligned")
+    b = _lib.Norm(n=4, d=8, x=16, weight=16, r=16, y=16, stats=20, dtype=0, layer=1, scale=1.0,
+                  eps=1e-5)
+    refused(lib.slk_norm_forward(ctypes.byref(b), None), "aligned")
+    refused(lib.slk_norm_backward(ctypes.byref(b), None), "aligned")
