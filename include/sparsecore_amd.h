@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define SLK_ABI_VERSION 19
+#define SLK_ABI_VERSION 20
 
 #if defined(__GNUC__)
 #define SLK_API __attribute__((visibility("default")))
@@ -870,6 +870,67 @@ SLK_API int64_t slk_linear_ce_saved_bytes(const slk_linear_ce* args_host);
 SLK_API int64_t slk_linear_ce_scratch_bytes(const slk_linear_ce* args_host, int backward);
 SLK_API int slk_linear_ce_forward(const slk_linear_ce* args_host, void* stream);
 SLK_API int slk_linear_ce_backward(const slk_linear_ce* args_host, void* stream);
+
+/* A tensor of attention: pointer and strides in elements. Packed rows have no
+ * batch stride (0).                                                          */
+typedef struct slk_attn_tensor {
+    void* p;
+    int64_t batch, row, head, feature;
+} slk_attn_tensor;
+
+/* Arguments of slk_attention_*:
+ *   S = scale·Q·K^T + bias,  P = softmax of S over the keys that a query sees,
+ *   out = P·V,
+ * of heads query heads and kv_heads key heads (each serves heads / kv_heads
+ * consecutive query heads), dim features, strides of any kind.
+ *   rows       batch: n entries of rows_q queries and rows_k keys, of which the
+ *              first q_lengths[i] and k_lengths[i] are live (NULL: all). Packed:
+ *              rows_q rows in all, sequence i from q_offsets[i] to
+ *              q_offsets[i + 1] (n + 1 entries; k_offsets for keys, NULL: the
+ *              same). Offsets and lengths are int32 on the device; one that is
+ *              out of range or falls counts as the nearest that is not.
+ *   causal     a sequence's last query stands at its last key: query i of nq
+ *              sees keys 0 .. i + nk - nq of nk. Else every live key.
+ *   bias       buckets x heads (bias_dtype), NULL: none. Distance d = position
+ *              of the query less that of the key; bucket k of a side begins at
+ *              bucket_starts[k] (host, ascending, the first 0, at most
+ *              max_distance) and ends before the next; the last takes all
+ *              further ones. causal: all buckets are for d >= 0; else the first
+ *              half is, and the second half for d < 0.
+ * A query that sees no key, and a row of no sequence, has output 0 and gradient
+ * 0. What is masked reaches nothing, whatever it holds.
+ * float32 products run on the float16 matrix instructions in two parts an
+ * operand (22 bits of an element down to 2^-39 of the largest in its 32 rows of
+ * a head); bf16 weights and their gradients are rounded to bf16 between
+ * products. Softmax statistics and sums are float32, in a fixed order.
+ *   keep       1 where a backward follows: forward leaves log-sums and packed
+ *              operands in saved (slk_attention_saved_bytes); backward takes the
+ *              same arguments, q, k, v unchanged (float32 ones are not read)
+ *   scratch    slk_attention_scratch_bytes; saved and scratch 16-byte aligned
+ * backward: dq, and dk with dv, where not NULL; dbias (as bias) where not NULL.  */
+#define SLK_ATTN_MAX_DIM 128
+#define SLK_ATTN_MAX_BUCKETS 128
+#define SLK_ATTN_MAX_DISTANCE 256
+typedef struct slk_attention {
+    int64_t n, rows_q, rows_k, heads, kv_heads, dim;
+    slk_attn_tensor q, k, v, out, dout, dq, dk, dv;
+    const int32_t *q_offsets, *k_offsets, *q_lengths, *k_lengths;
+    const void* bias;
+    void* dbias;
+    const int32_t* bucket_starts;
+    int64_t buckets, max_distance;
+    void* saved;
+    int64_t saved_bytes;
+    void* scratch;
+    int64_t scratch_bytes;
+    double scale;
+    int32_t dtype, bias_dtype, causal, keep;
+} slk_attention;
+
+SLK_API int64_t slk_attention_saved_bytes(const slk_attention* args_host);
+SLK_API int64_t slk_attention_scratch_bytes(const slk_attention* args_host, int backward);
+SLK_API int slk_attention_forward(const slk_attention* args_host, void* stream);
+SLK_API int slk_attention_backward(const slk_attention* args_host, void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,11 +30,13 @@ from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Stat
 from .loss import linear_cross_entropy
 from .norm import ResidualNorm, residual_norm
 from .optim import AdamW
+from .attn import attention
 from . import _lib, nn, ops, optim, router
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
            "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
-           "residual_norm", "ResidualNorm", "linear_cross_entropy", "install_as_sparselab"]
+           "residual_norm", "ResidualNorm", "linear_cross_entropy", "attention",
+           "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

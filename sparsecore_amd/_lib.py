@@ -22,7 +22,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libsparsecore_amd.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 SLK_OK, SLK_EINVAL, SLK_EDEVICE = 0, 1, 2
 SLK_DW_SIMD, SLK_DW_SCALAR = 0, 1
@@ -93,6 +93,10 @@ EXPORTS = (
     "slk_linear_ce_scratch_bytes",
     "slk_linear_ce_forward",
     "slk_linear_ce_backward",
+    "slk_attention_saved_bytes",
+    "slk_attention_scratch_bytes",
+    "slk_attention_forward",
+    "slk_attention_backward",
 )
 
 RIGL_INFO_BYTES = 32  # per row, slk_rigl_count's info
@@ -117,6 +121,10 @@ DTYPES = {torch.float32: SLK_F32, torch.bfloat16: SLK_BF16}
 Q8_BLOCK = 256  # SLK_Q8_BLOCK
 STATE_F32, STATE_Q8_SIGNED, STATE_Q8_UNSIGNED = 0, 1, 2
 CARRY_STATES = 4  # SLK_CARRY_STATES
+
+ATTN_MAX_DIM = 128  # SLK_ATTN_MAX_DIM
+ATTN_MAX_BUCKETS = 128  # SLK_ATTN_MAX_BUCKETS
+ATTN_MAX_DISTANCE = 256  # SLK_ATTN_MAX_DISTANCE
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # enum slk_reduction
 
@@ -261,6 +269,28 @@ class LinearCE(ctypes.Structure):
         + [(k, ctypes.c_int32) for k in ("dtype", "reduction", "keep", "pad")])
 
 
+class AttnTensor(ctypes.Structure):
+    """Mirror of ``slk_attn_tensor`` (include/sparsecore_amd.h)."""
+
+    _fields_ = [("p", ctypes.c_void_p)] + [(k, ctypes.c_int64)
+                                           for k in ("batch", "row", "head", "feature")]
+
+
+class Attention(ctypes.Structure):
+    """Mirror of ``slk_attention`` (include/sparsecore_amd.h)."""
+
+    _fields_ = (
+        [(k, ctypes.c_int64) for k in ("n", "rows_q", "rows_k", "heads", "kv_heads", "dim")]
+        + [(k, AttnTensor) for k in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")]
+        + [(k, ctypes.c_void_p) for k in ("q_offsets", "k_offsets", "q_lengths", "k_lengths",
+                                          "bias", "dbias", "bucket_starts")]
+        + [("buckets", ctypes.c_int64), ("max_distance", ctypes.c_int64),
+           ("saved", ctypes.c_void_p), ("saved_bytes", ctypes.c_int64),
+           ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_int64),
+           ("scale", ctypes.c_double)]
+        + [(k, ctypes.c_int32) for k in ("dtype", "bias_dtype", "causal", "keep")])
+
+
 _lib = None
 _load_error: str | None = None
 
@@ -360,13 +390,21 @@ def _declare(lib) -> None:
     lib.slk_linear_ce_scratch_bytes.argtypes = [cep, ctypes.c_int]
     lib.slk_linear_ce_forward.argtypes = [cep, _vp]
     lib.slk_linear_ce_backward.argtypes = [cep, _vp]
+    atp = ctypes.POINTER(Attention)
+    lib.slk_attention_saved_bytes.restype = _i64
+    lib.slk_attention_saved_bytes.argtypes = [atp]
+    lib.slk_attention_scratch_bytes.restype = _i64
+    lib.slk_attention_scratch_bytes.argtypes = [atp, ctypes.c_int]
+    lib.slk_attention_forward.argtypes = [atp, _vp]
+    lib.slk_attention_backward.argtypes = [atp, _vp]
     sized = ("slk_last_error", "slk_abi_version", "slk_transpose_workspace_bytes",
              "slk_drop_grow_workspace_bytes", "slk_rigl_bound_factor", "slk_rigl_partial_factor",
              "slk_dense_grad_approx_workspace_bytes",
              "slk_seg_list_capacity", "slk_seg_list_workspace_bytes", "slk_quad_windows",
              "slk_quad_chunks", "slk_quad_halves", "slk_strip_layout_bytes",
              "slk_norm_workspace_bytes", "slk_linear_ce_saved_bytes",
-             "slk_linear_ce_scratch_bytes")
+             "slk_linear_ce_scratch_bytes", "slk_attention_saved_bytes",
+             "slk_attention_scratch_bytes")
     for name in EXPORTS:
         if name not in sized:
             getattr(lib, name).restype = ctypes.c_int
@@ -935,6 +973,26 @@ def linear_ce_forward(args: LinearCE, stream: int) -> None:
 
 def linear_ce_backward(args: LinearCE, stream: int) -> None:
     rc = load().slk_linear_ce_backward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def attention_saved_bytes(args: Attention) -> int:
+    return load().slk_attention_saved_bytes(ctypes.byref(args))
+
+
+def attention_scratch_bytes(args: Attention, backward: bool) -> int:
+    return load().slk_attention_scratch_bytes(ctypes.byref(args), int(backward))
+
+
+def attention_forward(args: Attention, stream: int) -> None:
+    rc = load().slk_attention_forward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def attention_backward(args: Attention, stream: int) -> None:
+    rc = load().slk_attention_backward(ctypes.byref(args), stream)
     if rc:
         _raise(rc)
 

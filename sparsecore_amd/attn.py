@@ -1,0 +1,267 @@
+"""sparsecore_amd.attn — attention between two projections of a model:
+
+    S = scale · Q·Kᵀ (+ bias of the distance),   P = softmax(S),   out = P·V
+
+forward and backward, scores never stored (``slk_attention_*``): a batch, a padded batch
+or packed sequences, grouped heads, causal or not, with a learned bias of the relative
+position.
+
+A SparseLinear returns its output feature by feature in memory (the transposed view of a
+feature-major array). Queries, keys, values and the output's gradient are read with any
+strides, gradients come back in their tensors' layout, and ``feature_major=True`` writes
+the output as the next SparseLinear takes it without a copy.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+__all__ = ["attention", "relative_buckets"]
+
+
+@functools.lru_cache(maxsize=64)
+def relative_buckets(buckets: int, max_distance: int) -> tuple[int, ...]:
+    """First distance of each of one side's buckets: the first half hold one distance each
+    (0, 1, ...), the others grow by a constant factor up to ``max_distance``, where the last
+    one would end. With e of the first kind and r = buckets - e, bucket e + t begins at the
+    first n with (n / e)^r >= (max_distance / e)^t, decided in whole numbers."""
+    if buckets < 2:
+        raise ValueError(f"relative_buckets: at least 2 buckets a side, got {buckets}")
+    e = buckets // 2
+    r = buckets - e
+    if max_distance <= e:
+        raise ValueError(f"relative_buckets: max_distance must be above {e}, got {max_distance}")
+    starts = list(range(e + 1))
+    n = e
+    for t in range(1, r):
+        bar = e ** (r - t) * max_distance ** t
+        while n ** r < bar:
+            n += 1
+        starts.append(n)
+    return tuple(starts[:buckets])
+
+
+@functools.lru_cache(maxsize=64)
+def _starts(buckets: int, max_distance: int):
+    table = relative_buckets(buckets, max_distance)
+    return (ctypes.c_int32 * len(table))(*table)
+
+
+def _tensor(t: torch.Tensor | None) -> _lib.AttnTensor:
+    if t is None:
+        return _lib.AttnTensor()
+    s = t.stride()
+    if t.dim() == 3:
+        return _lib.AttnTensor(t.data_ptr(), 0, *s)
+    return _lib.AttnTensor(t.data_ptr(), *s)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor of t's shape, in t's order of dimensions in memory, without its gaps."""
+    order = sorted(range(t.dim()), key=lambda i: -t.stride(i))
+    out = torch.empty([t.shape[i] for i in order], dtype=t.dtype, device=t.device)
+    back = [0] * t.dim()
+    for at, i in enumerate(order):
+        back[i] = at
+    return out.permute(back)
+
+
+def _output(q: torch.Tensor, feature_major: bool) -> torch.Tensor:
+    if not feature_major:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    h, d = q.shape[-2:]
+    flat = torch.empty((h * d, q.numel() // max(1, h * d)), dtype=q.dtype, device=q.device)
+    return flat.t().reshape(*q.shape[:-2], h * d).unflatten(-1, (h, d))
+
+
+def _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal, scale,
+          keep):
+    p = _lib.ptr
+    packed = offsets is not None
+    a = _lib.Attention(
+        n=offsets.numel() - 1 if packed else q.shape[0], rows_q=q.shape[-3], rows_k=k.shape[-3],
+        heads=q.shape[-2], kv_heads=k.shape[-2], dim=q.shape[-1], q=_tensor(q), k=_tensor(k),
+        v=_tensor(v), q_offsets=p(offsets), k_offsets=p(k_offsets), q_lengths=p(lengths),
+        k_lengths=p(k_lengths), scale=scale, dtype=_lib.DTYPES[q.dtype], causal=causal, keep=keep)
+    if bias is not None:
+        a.bias, a.bias_dtype = p(bias), _lib.DTYPES[bias.dtype]
+        a.buckets, a.max_distance = bias.shape[0], max_distance
+        a.bucket_starts = ctypes.addressof(
+            _starts(bias.shape[0] if causal else bias.shape[0] // 2, max_distance))
+    return a
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, offsets, k_offsets, lengths, k_lengths, max_distance, causal,
+                scale, feature_major, grad):
+        dev = q.device
+        keep = grad and any(ctx.needs_input_grad)
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        out = _output(q, feature_major)
+        a = _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal,
+                  scale, int(keep))
+        a.out = _tensor(out)
+        saved = None
+        with _lib.on_device(q):
+            if keep:
+                a.saved_bytes = _lib.attention_saved_bytes(a)
+                saved = torch.empty(a.saved_bytes, dtype=torch.uint8, device=dev)
+                a.saved = saved.data_ptr()
+            a.scratch_bytes = _lib.attention_scratch_bytes(a, False)
+            if a.scratch_bytes:
+                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=dev)
+                a.scratch = scratch.data_ptr()
+            _lib.attention_forward(a, _lib.stream_of(q))
+        if keep:
+            ctx.save_for_backward(saved, q, k, v, out, bias, offsets, k_offsets, lengths,
+                                  k_lengths)
+            ctx.rest = (max_distance, causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        saved, q, k, v, out, bias, offsets, k_offsets, lengths, k_lengths = ctx.saved_tensors
+        max_distance, causal, scale = ctx.rest
+        need = ctx.needs_input_grad
+        a = _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal,
+                  scale, 1)
+        dq = _like(q) if need[0] else None
+        dk, dv = (_like(k), _like(v)) if need[1] or need[2] else (None, None)
+        dbias = torch.empty_like(bias) if bias is not None and need[3] else None
+        a.out, a.dout, a.dq, a.dk, a.dv = (_tensor(t) for t in (out, dout, dq, dk, dv))
+        a.saved, a.saved_bytes, a.dbias = saved.data_ptr(), saved.numel(), _lib.ptr(dbias)
+        with _lib.on_device(q):
+            a.scratch_bytes = _lib.attention_scratch_bytes(a, True)
+            if a.scratch_bytes:
+                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=q.device)
+                a.scratch = scratch.data_ptr()
+            _lib.attention_backward(a, _lib.stream_of(q))
+        return (dq, dk if need[1] else None, dv if need[2] else None, dbias) + (None,) * 9
+
+
+def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offsets=None,
+              k_offsets=None, lengths=None, k_lengths=None, bias=None, max_distance: int = 128,
+              feature_major: bool = False):
+    """softmax(scale · q·kᵀ + bias) · v over the keys that each query sees, autograd-aware.
+
+    Args:
+        q: (B, T, H, D) queries, or (N, H, D) packed ones, float32 or bfloat16, D <= 128.
+        k, v: (B, S, G, D) or (M, G, D) keys and values, q's dtype; G divides H, and key head
+            i serves the query heads i·H/G .. (i + 1)·H/G - 1.
+        causal: a sequence's last query stands at its last key: of n queries and m keys,
+            query i sees the keys up to i + m - n. Else every query sees every key.
+        scale: factor of the scores, not negative; default D ** -0.5.
+        offsets: (sequences + 1,) int32: packed sequence i is the rows offsets[i] to
+            offsets[i + 1] of q, and of k and v unless k_offsets is given.
+        lengths: (B,) int32: the first lengths[b] queries of entry b are live, and as many
+            keys unless k_lengths is given. k_lengths alone: live keys, all queries live, as
+            when new tokens meet arrays of keys that are only partly filled.
+        bias: (buckets, H) learned bias of the relative position, float32 or q's dtype. With
+            causal, of how far the key is behind; else the first half is for keys at or
+            behind the query and the second half for those ahead. See relative_buckets.
+        max_distance: distances from here on share the last bucket; at most 256.
+        feature_major: write the output feature by feature in memory (a view whose features
+            are rows), as a SparseLinear takes it without a copy.
+
+    Returns q's shape. A query that sees no key has output 0 and no gradient, and so has a
+    row that belongs to no sequence; what is masked reaches nothing, whatever it holds. A
+    value that is not finite makes the results whose sums contain it NaN or infinite. Offsets
+    and lengths are read on the device: those out of range, or offsets that fall, count as
+    the nearest that do not.
+
+    float32 products run on the matrix cores' float16 instructions in two parts an operand:
+    an element keeps 22 bits down to 2^-39 of the largest in its block of 32 rows of a head,
+    about float32's own rounding. bfloat16 weights (and their gradients) are rounded to
+    bfloat16 between the products. Softmax and sums are float32, in a fixed order: results
+    repeat bit for bit. A forward that a backward may follow keeps log-sums and, in float32
+    or where the layout needs it, the operands once more. q, k, v, the output and the
+    lengths must not change in place before the backward.
+
+    Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
+    (shape, dtype, sizes).
+    """
+    given = [("q", q), ("k", k), ("v", v), ("bias", bias), ("offsets", offsets),
+             ("k_offsets", k_offsets), ("lengths", lengths), ("k_lengths", k_lengths)]
+    for name, t in given:
+        if t is None and name not in ("q", "k", "v"):
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"attention: {name} must be a torch.Tensor, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise RuntimeError(f"attention: {name} must be on a HIP (ROCm) device (got "
+                               f"device={t.device})")
+        if t.device != q.device:
+            raise RuntimeError(f"attention: {name} is on {t.device} but q on {q.device}")
+    if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"attention: q, k and v must all be float32 or all bfloat16, got "
+                         f"{q.dtype}, {k.dtype} and {v.dtype}")
+    packed = offsets is not None
+    rank = 3 if packed else 4
+    if q.dim() != rank or k.dim() != rank or v.shape != k.shape:
+        raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v "
+                         f"{tuple(v.shape)} must be "
+                         + ("(N, H, D), (M, G, D) and (M, G, D)" if packed else
+                            "(B, T, H, D), (B, S, G, D) and (B, S, G, D)"))
+    h, d = q.shape[-2:]
+    g = k.shape[-2]
+    if k.shape[-1] != d or not 1 <= d <= _lib.ATTN_MAX_DIM:
+        raise ValueError(f"attention: q and k must share a head size of 1 to "
+                         f"{_lib.ATTN_MAX_DIM}, got {d} and {k.shape[-1]}")
+    if g < 1 or h < 1 or h % g:
+        raise ValueError(f"attention: {h} query heads are no multiple of {g} key heads")
+    if packed:
+        if lengths is not None or k_lengths is not None:
+            raise ValueError("attention: offsets or lengths, not both")
+        if k_offsets is None and k.shape[0] != q.shape[0]:
+            raise ValueError(f"attention: {q.shape[0]} query rows but {k.shape[0]} key rows "
+                             f"share offsets")
+    else:
+        if k_offsets is not None:
+            raise ValueError("attention: k_offsets need offsets")
+        if q.shape[0] != k.shape[0]:
+            raise ValueError(f"attention: q has {q.shape[0]} entries but k {k.shape[0]}")
+    for name, t in given[4:]:
+        if t is None:
+            continue
+        want = (q.shape[0],) if name.endswith("lengths") else None
+        if t.dtype != torch.int32 or t.dim() != 1 or (want and t.shape != want) or \
+                (not want and t.numel() < 1):
+            raise ValueError(f"attention: {name} must be int32, "
+                             f"{'one for each entry' if want else 'one for each sequence and one more'}"
+                             f", got {t.dtype} {tuple(t.shape)}")
+    if k_offsets is not None and k_offsets.shape != offsets.shape:
+        raise ValueError("attention: offsets and k_offsets must have the same length")
+    if lengths is not None and k_lengths is None:
+        k_lengths = lengths
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] != h:
+            raise ValueError(f"attention: bias must be (buckets, {h}), got {tuple(bias.shape)}")
+        if bias.dtype not in (torch.float32, q.dtype):
+            raise ValueError(f"attention: bias must be float32 or {q.dtype}, got {bias.dtype}")
+        buckets = bias.shape[0]
+        if not 2 <= (buckets if causal else buckets // 2) or \
+                buckets > _lib.ATTN_MAX_BUCKETS or (not causal and buckets % 2):
+            raise ValueError(f"attention: bias must have 2 to {_lib.ATTN_MAX_BUCKETS} buckets "
+                             f"(causal), or an even number from 4 on, got {buckets}")
+        max_distance = int(max_distance)
+        if not 1 <= max_distance <= _lib.ATTN_MAX_DISTANCE:
+            raise ValueError(f"attention: max_distance must be between 1 and "
+                             f"{_lib.ATTN_MAX_DISTANCE}, got {max_distance}")
+        _starts(buckets if causal else buckets // 2, max_distance)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (0.0 <= scale < math.inf):
+        raise ValueError(f"attention: scale must be finite and not negative, got {scale}")
+    ints = [t if t is None or t.is_contiguous() else t.contiguous()
+            for t in (offsets, k_offsets, lengths, k_lengths)]
+    return _Attention.apply(q, k, v, bias, *ints, max_distance, bool(causal), scale,
+                            bool(feature_major), torch.is_grad_enabled())

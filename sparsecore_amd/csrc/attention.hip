@@ -1,0 +1,506 @@
+// slk_attention_*: argument checks, memory layout and launches.
+#include <algorithm>
+
+#include "attention.hpp"
+#include "attention_decode.hpp"
+#include "attention_prep.hpp"
+
+namespace slk {
+
+namespace {
+
+constexpr int64_t kTileRows = 128;   // rows of a workgroup of every tiled kernel
+constexpr int kFewRows = 16;         // queries of an entry that go the way of single tokens
+constexpr int64_t kCus = 256;
+
+int64_t pad64(int64_t n) { return ceil_div(n, kAttnRows) * kAttnRows; }
+
+bool packed_rows(const slk_attention& a) { return a.q_offsets != nullptr; }
+bool uniform(const slk_attention& a) {
+    return a.q_offsets == nullptr && a.q_lengths == nullptr && a.k_lengths == nullptr;
+}
+
+int blocks_of(int64_t dim) { return dim <= 32 ? 1 : dim <= 64 ? 2 : 4; }
+
+// Whether the kernels read a tensor where it lies: bfloat16, a head as wide as a
+// tile, features consecutive, rows of 16-byte pieces, a tile's 64 rows in 31 bits.
+bool direct(const slk_attn_tensor& t, const slk_attention& a) {
+    return a.dtype == SLK_BF16 && a.dim == 32 * blocks_of(a.dim) && t.feature == 1 &&
+           t.row % 8 == 0 && t.head % 8 == 0 && t.batch % 8 == 0 && t.row >= 0 &&
+           t.row < (int64_t{1} << 23) && aligned_to(t.p, 16);
+}
+
+struct Sizes {
+    int64_t pad_q, pad_k;         // padded rows, an upper bound
+    int64_t q_entries, k_entries; // tiles, an upper bound
+    int64_t elem, row;            // bytes of a packed element and row
+};
+
+Sizes sizes_of(const slk_attention& a) {
+    Sizes s;
+    if (packed_rows(a)) {
+        s.pad_q = pad64(a.rows_q) + kAttnRows * a.n;
+        s.pad_k = pad64(a.rows_k) + kAttnRows * a.n;
+        s.q_entries = a.rows_q / kTileRows + a.n + 2;
+        s.k_entries = a.rows_k / kTileRows + a.n + 2;
+    } else {
+        s.pad_q = a.n * pad64(a.rows_q);
+        s.pad_k = a.n * pad64(a.rows_k);
+        s.q_entries = a.n * ceil_div(a.rows_q, kTileRows);
+        s.k_entries = a.n * ceil_div(a.rows_k, kTileRows);
+    }
+    s.elem = a.dtype == SLK_F32 ? 4 : 2;
+    s.row = s.elem * 32 * blocks_of(a.dim);
+    return s;
+}
+
+// Consecutive pieces of a buffer, each 256-byte aligned.
+struct Carver {
+    char* base;
+    int64_t at = 0;
+    void* take(int64_t bytes) {
+        void* p = base != nullptr ? base + at : nullptr;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+struct Packed {
+    char* data;
+    int32_t* exps;
+};
+
+Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows, bool split) {
+    Packed p;
+    p.data = static_cast<char*>(c.take(heads * rows * s.row));
+    p.exps = split ? static_cast<int32_t*>(c.take(heads * (rows / 32) * 4)) : nullptr;
+    return p;
+}
+
+struct Saved {
+    float* lse;
+    Packed q, k, v;
+    int64_t bytes;
+};
+
+Saved saved_of(const slk_attention& a, void* base) {
+    const Sizes s = sizes_of(a);
+    const bool split = a.dtype == SLK_F32;
+    Carver c{static_cast<char*>(base)};
+    Saved r{};
+    r.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
+    if (!direct(a.q, a)) r.q = take_packed(c, s, a.heads, s.pad_q, split);
+    if (!direct(a.k, a)) r.k = take_packed(c, s, a.kv_heads, s.pad_k, split);
+    if (!direct(a.v, a)) r.v = take_packed(c, s, a.kv_heads, s.pad_k, split);
+    r.bytes = c.at;
+    return r;
+}
+
+bool few_rows(const slk_attention& a) {
+    return !a.keep && a.q_offsets == nullptr && a.q_lengths == nullptr && a.rows_q <= kFewRows;
+}
+
+struct Few {
+    int rows, chunks, splits;
+};
+
+// Rows of a key head that a workgroup takes, and parts of the keys: enough
+// workgroups for four on each CU, at least 512 keys each.
+Few few_of(const slk_attention& a) {
+    const int64_t rows = a.heads / a.kv_heads * a.rows_q;
+    Few f;
+    f.rows = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
+    f.chunks = static_cast<int>(ceil_div(rows, f.rows));
+    const int64_t groups = a.n * a.kv_heads * f.chunks;
+    const int64_t want = groups > 0 ? ceil_div(4 * kCus, groups) : 1;
+    const int64_t most = ceil_div(a.rows_k, 512);
+    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
+    return f;
+}
+
+// Parts of the keys in the tiled forward: where the query tiles leave CUs idle.
+int splits_of(const slk_attention& a, const Sizes& s) {
+    if (a.keep) return 1;
+    const int64_t groups = s.q_entries * a.heads;
+    if (groups == 0 || groups >= kCus) return 1;
+    const int64_t most = a.rows_k / 256;
+    return static_cast<int>(std::max<int64_t>(1, std::min(2 * kCus / groups, most)));
+}
+
+struct Plan {
+    AttnSeq* seqs;
+    int2 *q_list, *k_list;
+    int32_t* count;
+};
+
+Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s, bool keys) {
+    Plan p{};
+    if (uniform(a)) return p;
+    p.count = static_cast<int32_t*>(c.take(16));
+    p.seqs = static_cast<AttnSeq*>(c.take((a.n + 2) * sizeof(AttnSeq)));
+    p.q_list = static_cast<int2*>(c.take(s.q_entries * sizeof(int2)));
+    if (keys) p.k_list = static_cast<int2*>(c.take(s.k_entries * sizeof(int2)));
+    return p;
+}
+
+struct Forward {
+    Saved saved;  // its place, or a part of scratch
+    Plan plan;
+    float *part, *part_ml;
+    int splits;
+    Few few;
+    int64_t bytes;
+};
+
+Forward forward_of(const slk_attention& a, void* scratch) {
+    const Sizes s = sizes_of(a);
+    Carver c{static_cast<char*>(scratch)};
+    Forward f{};
+    if (few_rows(a)) {
+        f.few = few_of(a);
+        f.splits = f.few.splits;
+    } else {
+        f.plan = take_plan(c, a, s, false);
+        f.splits = splits_of(a, s);
+        if (a.keep) {
+            f.saved = saved_of(a, a.saved);
+        } else {
+            f.saved = saved_of(a, c.base != nullptr ? c.base + c.at : nullptr);
+            c.take(f.saved.bytes);
+            f.saved.lse = nullptr;
+        }
+    }
+    if (f.splits > 1) {
+        const int64_t rows = f.splits * a.heads * s.pad_q;
+        f.part = static_cast<float*>(c.take(rows * 32 * blocks_of(a.dim) * 4));
+        f.part_ml = static_cast<float*>(c.take(rows * 8));
+    }
+    f.bytes = c.at;
+    return f;
+}
+
+struct Backward {
+    Plan plan;
+    float* delta;
+    int32_t* dexps;
+    Packed dout;
+    float* dbias_part;
+    int64_t bytes;
+};
+
+Backward backward_of(const slk_attention& a, void* scratch) {
+    const Sizes s = sizes_of(a);
+    Carver c{static_cast<char*>(scratch)};
+    Backward b{};
+    b.plan = take_plan(c, a, s, true);
+    b.delta = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
+    if (a.dtype == SLK_F32) b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / 32) * 4));
+    if (!direct(a.dout, a)) b.dout = take_packed(c, s, a.heads, s.pad_q, a.dtype == SLK_F32);
+    if (a.dbias != nullptr)
+        b.dbias_part = static_cast<float*>(
+            c.take(a.heads * (s.pad_q / kAttnRows) * (2 * a.max_distance + 1) * 4));
+    b.bytes = c.at;
+    return b;
+}
+
+AttnIo io_of(const slk_attn_tensor& t) {
+    return AttnIo{static_cast<char*>(t.p), t.batch, t.row, t.head, t.feature};
+}
+
+AttnOp op_of(const slk_attn_tensor& t, const Packed& p, const slk_attention& a, const Sizes& s,
+             int64_t rows) {
+    AttnOp o{};
+    if (p.data == nullptr) {
+        o.p = static_cast<const char*>(t.p);
+        o.sb = 2 * t.batch;
+        o.sr = 2 * t.row;
+        o.sh = 2 * t.head;
+        return o;
+    }
+    o.p = p.data;
+    o.sr = s.row;
+    o.sh = rows * s.row;
+    o.plane = static_cast<int32_t>(s.row / 2);
+    o.packed = 1;
+    o.exps = p.exps;
+    o.exps_sh = rows / 32;
+    (void)a;
+    return o;
+}
+
+AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s, int64_t rows,
+                   int64_t heads, bool keys) {
+    AttnPackOp o{};
+    o.src = io_of(t);
+    o.dst = p.data;
+    o.dst_sr = s.row;
+    o.dst_sh = rows * s.row;
+    o.exps = p.exps;
+    o.exps_sh = rows / 32;
+    o.rows = rows;
+    o.heads = static_cast<int32_t>(heads);
+    o.keys = keys;
+    return o;
+}
+
+AttnPlan plan_of(const slk_attention& a, const Plan& p, bool keys) {
+    AttnPlan r{};
+    r.seqs = p.seqs;
+    r.list = keys ? p.k_list : p.q_list;
+    r.count = p.count != nullptr ? p.count + (keys ? 2 : 0) : nullptr;
+    r.batch = a.n;
+    r.t = a.rows_q;
+    r.s = a.rows_k;
+    r.pad_t = pad64(a.rows_q);
+    r.pad_s = pad64(a.rows_k);
+    return r;
+}
+
+int make_plan(const slk_attention& a, const Plan& p, hipStream_t st) {
+    if (p.seqs == nullptr) return SLK_OK;
+    AttnPlanArgs g{};
+    g.q_offsets = a.q_offsets;
+    g.k_offsets = a.k_offsets != nullptr ? a.k_offsets : a.q_offsets;
+    g.q_lengths = a.q_lengths;
+    g.k_lengths = a.k_lengths;
+    g.n = a.n;
+    g.rows_q = a.rows_q;
+    g.rows_k = a.rows_k;
+    g.seqs = p.seqs;
+    g.q_list = p.q_list;
+    g.k_list = p.k_list;
+    g.count = p.count;
+    g.tile_q = g.tile_k = kTileRows;
+    g.causal = a.causal;
+    while ((std::max(a.rows_q, a.rows_k) / kAttnRows) >> g.work_shift >= 1024) ++g.work_shift;
+    return attn_launch_plan(g, st);
+}
+
+AttnArgs args_of(const slk_attention& a) {
+    AttnArgs g{};
+    g.out = io_of(a.out);
+    g.dq = io_of(a.dq);
+    g.dk = io_of(a.dk);
+    g.dv = io_of(a.dv);
+    g.lse_sh = sizes_of(a).pad_q;
+    g.heads = static_cast<int32_t>(a.heads);
+    g.kv_heads = static_cast<int32_t>(a.kv_heads);
+    g.dim = static_cast<int32_t>(a.dim);
+    g.dtype = a.dtype;
+    g.causal = a.causal;
+    g.splits = 1;
+    g.scale = static_cast<float>(a.scale);
+    g.scale2 = static_cast<float>(a.scale * 1.4426950408889634);
+    if (a.bias != nullptr) {
+        g.bias.table = a.bias;
+        g.bias.dtype = a.bias_dtype;
+        g.bias.buckets = static_cast<int32_t>(a.buckets);
+        g.bias.max_distance = static_cast<int32_t>(a.max_distance);
+        g.bias.one_sided = a.causal;
+        const int64_t one = a.causal ? a.buckets : a.buckets / 2;
+        for (int64_t i = 0; i < one; ++i)
+            g.bias.starts[i] = static_cast<uint16_t>(a.bucket_starts[i]);
+    }
+    return g;
+}
+
+int check(const slk_attention* args, const char* who, bool backward) {
+    const std::string w = who;
+    if (args == nullptr) return fail(SLK_EINVAL, w + ": NULL arguments");
+    const slk_attention& a = *args;
+    if (a.n < 0 || a.rows_q < 0 || a.rows_k < 0) return fail(SLK_EINVAL, w + ": negative size");
+    if (a.dtype != SLK_F32 && a.dtype != SLK_BF16)
+        return fail(SLK_EINVAL, w + ": unknown dtype " + std::to_string(a.dtype));
+    if (a.dim < 1 || a.dim > SLK_ATTN_MAX_DIM)
+        return fail(SLK_EINVAL, w + ": dim in [1, " + std::to_string(SLK_ATTN_MAX_DIM) +
+                                    "], got " + std::to_string(a.dim));
+    if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.heads > 16384)
+        return fail(SLK_EINVAL, w + ": heads must be a multiple of kv_heads, at most 16384, got " +
+                                    std::to_string(a.heads) + " and " +
+                                    std::to_string(a.kv_heads));
+    if (!(a.scale >= 0.0) || !(a.scale <= 3e38))
+        return fail(SLK_EINVAL, w + ": scale must be finite and not negative");
+    if (packed_rows(a) && (a.q_lengths != nullptr || a.k_lengths != nullptr))
+        return fail(SLK_EINVAL, w + ": offsets or lengths, not both");
+    if (!packed_rows(a) && a.k_offsets != nullptr)
+        return fail(SLK_EINVAL, w + ": k_offsets need q_offsets");
+    if (packed_rows(a) && a.k_offsets == nullptr && a.rows_q != a.rows_k)
+        return fail(SLK_EINVAL, w + ": queries and keys share offsets but not their rows");
+    if (a.bias != nullptr) {
+        if (a.bias_dtype != SLK_F32 && a.bias_dtype != SLK_BF16)
+            return fail(SLK_EINVAL, w + ": unknown bias dtype");
+        const int64_t one = a.causal ? a.buckets : a.buckets / 2;
+        if (a.buckets < 1 || a.buckets > SLK_ATTN_MAX_BUCKETS || one < 1 ||
+            (!a.causal && a.buckets % 2 != 0))
+            return fail(SLK_EINVAL, w + ": buckets in [1, " +
+                                        std::to_string(SLK_ATTN_MAX_BUCKETS) +
+                                        "], even where both sides are seen");
+        if (a.max_distance < 1 || a.max_distance > SLK_ATTN_MAX_DISTANCE)
+            return fail(SLK_EINVAL, w + ": max_distance in [1, " +
+                                        std::to_string(SLK_ATTN_MAX_DISTANCE) + "]");
+        if (a.bucket_starts == nullptr || a.bucket_starts[0] != 0)
+            return fail(SLK_EINVAL, w + ": bucket_starts must begin with 0");
+        for (int64_t i = 1; i < one; ++i)
+            if (a.bucket_starts[i] < a.bucket_starts[i - 1] ||
+                a.bucket_starts[i] > a.max_distance)
+                return fail(SLK_EINVAL, w + ": bucket_starts must ascend to max_distance at most");
+    }
+    if (a.n == 0 && !packed_rows(a)) return SLK_OK;
+    // padded rows of all heads are counted in 64 bits, rows in 32
+    const Sizes s = sizes_of(a);
+    if (a.n > INT32_MAX / 64 || a.rows_q > INT32_MAX / 2 || a.rows_k > INT32_MAX / 2 ||
+        s.pad_q > INT32_MAX / 2 || s.pad_k > INT32_MAX / 2)
+        return fail(SLK_EINVAL, w + ": too many rows");
+    if (s.q_entries * a.heads > max_groups(kAttnThreads) ||
+        s.k_entries * a.heads > max_groups(kAttnThreads) || s.pad_q > max_groups(kWave) ||
+        s.pad_k > max_groups(kAttnThreads) * 32)
+        return fail(SLK_EINVAL, w + ": too many tiles");
+    if (!backward) {
+        if (a.rows_q > 0 && (a.q.p == nullptr || a.out.p == nullptr))
+            return fail(SLK_EINVAL, w + ": NULL q or out");
+        if (a.rows_k > 0 && (a.k.p == nullptr || a.v.p == nullptr))
+            return fail(SLK_EINVAL, w + ": NULL k or v");
+    } else {
+        if (a.rows_q > 0 && (a.out.p == nullptr || a.dout.p == nullptr))
+            return fail(SLK_EINVAL, w + ": NULL out or dout");
+        if ((a.dk.p == nullptr) != (a.dv.p == nullptr))
+            return fail(SLK_EINVAL, w + ": dk and dv go together");
+        if (a.dbias != nullptr && a.bias == nullptr)
+            return fail(SLK_EINVAL, w + ": dbias without a bias");
+    }
+    if (a.keep || backward) {
+        const int64_t need = saved_of(a, nullptr).bytes;
+        if (need > 0 && (a.saved == nullptr || a.saved_bytes < need))
+            return fail(SLK_EINVAL, w + ": saved too small (need " + std::to_string(need) + ")");
+    }
+    const int64_t need = backward ? backward_of(a, nullptr).bytes : forward_of(a, nullptr).bytes;
+    if (need > 0 && (a.scratch == nullptr || a.scratch_bytes < need))
+        return fail(SLK_EINVAL, w + ": scratch too small (need " + std::to_string(need) + ")");
+    if (!aligned_to(a.saved, 16) || !aligned_to(a.scratch, 16))
+        return fail(SLK_EINVAL, w + ": saved and scratch must be 16-byte aligned");
+    return SLK_OK;
+}
+
+int few_forward(const slk_attention& a, const Forward& f, hipStream_t st) {
+    AttnDecode d{};
+    d.g = args_of(a);
+    d.g.plan = plan_of(a, f.plan, false);
+    d.g.splits = f.splits;
+    d.g.part = f.part;
+    d.g.part_ml = f.part_ml;
+    d.g.part_rows = sizes_of(a).pad_q;
+    d.q = io_of(a.q);
+    d.k = io_of(a.k);
+    d.v = io_of(a.v);
+    d.k_lengths = a.k_lengths;
+    d.chunks = f.few.chunks;
+    const int64_t unit = a.dtype == SLK_F32 ? 4 : 8;
+    auto pieces = [&](const slk_attn_tensor& t) {
+        return t.feature == 1 && a.dim % 8 == 0 && t.row % unit == 0 && t.head % unit == 0 &&
+               t.batch % unit == 0 && aligned_to(t.p, 16);
+    };
+    d.vec = pieces(a.k) && pieces(a.v);
+    return attn_launch_decode(d, blocks_of(a.dim), f.few.rows, st);
+}
+
+}  // namespace
+
+}  // namespace slk
+
+extern "C" int64_t slk_attention_saved_bytes(const slk_attention* args) {
+    return args != nullptr && args->keep ? slk::saved_of(*args, nullptr).bytes : 0;
+}
+
+extern "C" int64_t slk_attention_scratch_bytes(const slk_attention* args, int backward) {
+    if (args == nullptr) return 0;
+    return backward ? slk::backward_of(*args, nullptr).bytes
+                    : slk::forward_of(*args, nullptr).bytes;
+}
+
+extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
+    using namespace slk;
+    clear_error();
+    int rc = check(args, "attention_forward", false);
+    if (rc != SLK_OK) return rc;
+    const slk_attention& a = *args;
+    if (a.rows_q == 0 || (a.n == 0 && !packed_rows(a))) return SLK_OK;
+    const hipStream_t st = as_stream(stream);
+    const Forward f = forward_of(a, a.scratch);
+    if (few_rows(a)) return few_forward(a, f, st);
+    const Sizes s = sizes_of(a);
+    const bool split = a.dtype == SLK_F32;
+    rc = make_plan(a, f.plan, st);
+    if (rc != SLK_OK) return rc;
+
+    AttnPack p{};
+    p.plan = plan_of(a, f.plan, false);
+    p.dim = static_cast<int32_t>(a.dim);
+    if (f.saved.q.data) p.op[p.n++] = pack_op(a.q, f.saved.q, s, s.pad_q, a.heads, false);
+    if (f.saved.k.data) p.op[p.n++] = pack_op(a.k, f.saved.k, s, s.pad_k, a.kv_heads, true);
+    if (f.saved.v.data) p.op[p.n++] = pack_op(a.v, f.saved.v, s, s.pad_k, a.kv_heads, true);
+    if (p.n > 0) {
+        rc = attn_launch_pack(p, split, blocks_of(a.dim), a.dtype, st);
+        if (rc != SLK_OK) return rc;
+    }
+    AttnArgs g = args_of(a);
+    g.plan = plan_of(a, f.plan, false);
+    g.tiles = ceil_div(a.rows_q, kTileRows);
+    g.q = op_of(a.q, f.saved.q, a, s, s.pad_q);
+    g.k = op_of(a.k, f.saved.k, a, s, s.pad_k);
+    g.v = op_of(a.v, f.saved.v, a, s, s.pad_k);
+    g.lse = f.saved.lse;
+    g.splits = f.splits;
+    g.part = f.part;
+    g.part_ml = f.part_ml;
+    g.part_rows = s.pad_q;
+    return attn_launch_forward(g, split, blocks_of(a.dim), s.q_entries, st);
+}
+
+extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
+    using namespace slk;
+    clear_error();
+    int rc = check(args, "attention_backward", true);
+    if (rc != SLK_OK) return rc;
+    const slk_attention& a = *args;
+    if (a.n == 0 && !packed_rows(a)) return SLK_OK;
+    const hipStream_t st = as_stream(stream);
+    const Sizes s = sizes_of(a);
+    const bool split = a.dtype == SLK_F32;
+    const Saved sv = saved_of(a, a.saved);
+    const Backward b = backward_of(a, a.scratch);
+    rc = make_plan(a, b.plan, st);
+    if (rc != SLK_OK) return rc;
+    if (a.rows_q > 0) {
+        AttnPack p{};
+        p.plan = plan_of(a, b.plan, false);
+        p.dim = static_cast<int32_t>(a.dim);
+        p.n = 1;
+        p.op[0] = pack_op(a.dout, b.dout, s, s.pad_q, a.heads, false);
+        p.op[0].exps_sh = s.pad_q / 32;
+        p.o = io_of(a.out);
+        p.delta = b.delta;
+        p.delta_sh = s.pad_q;
+        p.dexps = b.dexps;
+        rc = attn_launch_pack(p, split, blocks_of(a.dim), a.dtype, st);
+        if (rc != SLK_OK) return rc;
+    }
+    AttnArgs g = args_of(a);
+    g.plan = plan_of(a, b.plan, false);
+    g.tiles = ceil_div(a.rows_q, kTileRows);
+    g.q = op_of(a.q, sv.q, a, s, s.pad_q);
+    g.k = op_of(a.k, sv.k, a, s, s.pad_k);
+    g.v = op_of(a.v, sv.v, a, s, s.pad_k);
+    g.dout = op_of(a.dout, b.dout, a, s, s.pad_q);
+    g.q.exps_sh = s.pad_q / 32;
+    g.lse = sv.lse;
+    g.delta = b.delta;
+    g.dexps = b.dexps;
+    g.dbias_part = b.dbias_part;
+    g.dbias_slots = s.pad_q / kAttnRows;
+    const bool want_q = a.rows_q > 0 && (a.dq.p != nullptr || a.dbias != nullptr);
+    const bool want_kv = a.rows_k > 0 && a.dk.p != nullptr;
+    rc = attn_launch_backward(g, split, blocks_of(a.dim), plan_of(a, b.plan, true), s.q_entries,
+                              s.k_entries, want_q, want_kv, ceil_div(a.rows_k, kTileRows), st);
+    if (rc != SLK_OK || a.dbias == nullptr) return rc;
+    return attn_launch_dbias(g, a.dbias, st);
+}
