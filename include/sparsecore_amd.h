@@ -871,6 +871,38 @@ SLK_API int64_t slk_linear_ce_scratch_bytes(const slk_linear_ce* args_host, int 
 SLK_API int slk_linear_ce_forward(const slk_linear_ce* args_host, void* stream);
 SLK_API int slk_linear_ce_backward(const slk_linear_ce* args_host, void* stream);
 
+/* An activation y = f(x) of n elements, and what its backward needs of x in 8
+ * bits: SLK_ACT_BLOCK consecutive elements share a scale, the largest finite
+ * magnitude of them (top); q = round(x·(127 / top)) stands for q·(top·(1/127)),
+ * float32 operations. top < 2^-100: zeros; q = -128: not finite, NaN.
+ *   forward    x in; y (NULL: not wanted) and, where not NULL, codes (n bytes)
+ *              and scales (one a block, float32) out
+ *   backward   dx = dy·f'(x), x from the codes, or itself where codes is NULL;
+ *              dy NULL: dx is x
+ * Arithmetic is float32, each result rounded once. SLK_ACT_NONE: f(x) = x.
+ * Any alignment that the element types allow.                                */
+#define SLK_ACT_BLOCK 256
+enum slk_act_kind {
+    SLK_ACT_NONE = 0,
+    SLK_ACT_RELU = 1,
+    SLK_ACT_SILU = 2,
+    SLK_ACT_GELU = 3,
+    SLK_ACT_GELU_TANH = 4
+};
+typedef struct slk_activation {
+    int64_t n;
+    const void* x;
+    void* y;
+    const void* dy;
+    void* dx;
+    uint8_t* codes;
+    float* scales;
+    int32_t dtype, kind;
+} slk_activation;
+
+SLK_API int slk_activation_forward(const slk_activation* args_host, void* stream);
+SLK_API int slk_activation_backward(const slk_activation* args_host, void* stream);
+
 /* A tensor of attention: pointer and strides in elements. Packed rows have no
  * batch stride (0).                                                          */
 typedef struct slk_attn_tensor {

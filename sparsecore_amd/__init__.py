@@ -11,6 +11,8 @@ and, for the training step around the sparse layers (no counterpart there):
 
     linear_cross_entropy   head and loss without storing the logits
     residual_norm, ResidualNorm   residual sum, gate and the norms around a block
+    attention        causal or not, packed or padded, grouped heads, position bias
+    activation       gelu, silu, relu whose backward keeps 8 bits of its input
     AdamW, optim     the whole model's step in a launch or two, 32- or 8-bit moments
                      that follow their weights through SET / RigL rewrites
 
@@ -30,13 +32,14 @@ from .router import DynamicSparsityAlgorithm, RigL, SET, SparsityAlgorithm, Stat
 from .loss import linear_cross_entropy
 from .norm import ResidualNorm, residual_norm
 from .optim import AdamW
+from .act import activation
 from .attn import attention
 from . import _lib, nn, ops, optim, router
 
 __all__ = ["PaddedCSR", "spmm", "SparseLinear", "layout", "SparsityAlgorithm", "Static",
            "DynamicSparsityAlgorithm", "SET", "RigL", "AdamW", "optim",
            "residual_norm", "ResidualNorm", "linear_cross_entropy", "attention",
-           "install_as_sparselab"]
+           "activation", "install_as_sparselab"]
 __version__ = "0.1.0"
 
 

@@ -93,6 +93,8 @@ EXPORTS = (
     "slk_linear_ce_scratch_bytes",
     "slk_linear_ce_forward",
     "slk_linear_ce_backward",
+    "slk_activation_forward",
+    "slk_activation_backward",
     "slk_attention_saved_bytes",
     "slk_attention_scratch_bytes",
     "slk_attention_forward",
@@ -121,6 +123,9 @@ DTYPES = {torch.float32: SLK_F32, torch.bfloat16: SLK_BF16}
 Q8_BLOCK = 256  # SLK_Q8_BLOCK
 STATE_F32, STATE_Q8_SIGNED, STATE_Q8_UNSIGNED = 0, 1, 2
 CARRY_STATES = 4  # SLK_CARRY_STATES
+
+ACT_BLOCK = 256  # SLK_ACT_BLOCK
+ACT_KINDS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 ATTN_MAX_DIM = 128  # SLK_ATTN_MAX_DIM
 ATTN_MAX_BUCKETS = 128  # SLK_ATTN_MAX_BUCKETS
@@ -269,6 +274,15 @@ class LinearCE(ctypes.Structure):
         + [(k, ctypes.c_int32) for k in ("dtype", "reduction", "keep", "pad")])
 
 
+class Activation(ctypes.Structure):
+    """Mirror of ``slk_activation`` (include/sparsecore_amd.h)."""
+
+    _fields_ = (
+        [("n", ctypes.c_int64)]
+        + [(k, ctypes.c_void_p) for k in ("x", "y", "dy", "dx", "codes", "scales")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "kind")])
+
+
 class AttnTensor(ctypes.Structure):
     """Mirror of ``slk_attn_tensor`` (include/sparsecore_amd.h)."""
 
@@ -390,6 +404,8 @@ def _declare(lib) -> None:
     lib.slk_linear_ce_scratch_bytes.argtypes = [cep, ctypes.c_int]
     lib.slk_linear_ce_forward.argtypes = [cep, _vp]
     lib.slk_linear_ce_backward.argtypes = [cep, _vp]
+    lib.slk_activation_forward.argtypes = [ctypes.POINTER(Activation), _vp]
+    lib.slk_activation_backward.argtypes = [ctypes.POINTER(Activation), _vp]
     atp = ctypes.POINTER(Attention)
     lib.slk_attention_saved_bytes.restype = _i64
     lib.slk_attention_saved_bytes.argtypes = [atp]
@@ -973,6 +989,18 @@ def linear_ce_forward(args: LinearCE, stream: int) -> None:
 
 def linear_ce_backward(args: LinearCE, stream: int) -> None:
     rc = load().slk_linear_ce_backward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def activation_forward(args: Activation, stream: int) -> None:
+    rc = load().slk_activation_forward(ctypes.byref(args), stream)
+    if rc:
+        _raise(rc)
+
+
+def activation_backward(args: Activation, stream: int) -> None:
+    rc = load().slk_activation_backward(ctypes.byref(args), stream)
     if rc:
         _raise(rc)
 

@@ -252,7 +252,7 @@ struct AttnReads {
     }
 };
 
-// Eight results of a lane as an operand: rounded to bfloat16 (relative 2^-9, of
+// Eight results of a lane as an operand: rounded to bfloat16 (relative 2^-8, of
 // weights and of their gradients, as the tensors themselves are), or in two
 // float16 parts (22 bits).
 template <bool SPLIT>

@@ -24,6 +24,7 @@ import weakref
 import torch
 
 from . import _lib, layout
+from .act import decode8, encode8
 from .layout import PaddedCSR, transpose_with_perm, transposes_with_perm
 
 __all__ = ["spmm", "dense_grad"]
@@ -600,10 +601,11 @@ class _SparseLinearFunction(torch.autograd.Function):
     dW launch (slk_sddmm_bias); a narrow layer does all three gradients in one
     launch from the token-major gradient (slk_backward_narrow), with no
     transpose cache. dx is returned as the transposed view of dX (K x N).
+    With ``save_bits`` 8 the input waits for dW as 8-bit codes and their scales.
     """
 
     @staticmethod
-    def forward(ctx, W_values, bias, W, x_flat, kernel):
+    def forward(ctx, W_values, bias, W, x_flat, kernel, save_bits=32):
         if kernel not in _KERNELS:
             raise ValueError(f"spmm: unknown kernel={kernel!r}. Expected one of: "
                              f"{sorted(_KERNELS)}.")
@@ -615,7 +617,12 @@ class _SparseLinearFunction(torch.autograd.Function):
                 raise ValueError(f"spmm: bias must be float32 of shape ({W.nrows},), got "
                                  f"{bias.dtype} {tuple(bias.shape)}")
             bias = bias.contiguous()
-        ctx.save_for_backward(W_values, X)
+        ctx.kept = None
+        if save_bits == 8 and ctx.needs_input_grad[0]:
+            ctx.save_for_backward(W_values, *encode8(X))
+            ctx.kept = X.shape
+        else:
+            ctx.save_for_backward(W_values, X)
         ctx.W = W
         ctx.kernel = kernel
         ctx.narrow = _narrow_layer(W)
@@ -627,7 +634,11 @@ class _SparseLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dY):
-        W_values, X = ctx.saved_tensors
+        if ctx.kept is not None:
+            _, codes, scales = ctx.saved_tensors
+            X = decode8(codes, scales, ctx.kept)
+        else:
+            _, X = ctx.saved_tensors
         if ctx.narrow:
             return _narrow_backward(ctx, X, dY)
         dY_f32 = _as_row_major(dY)
@@ -639,7 +650,7 @@ class _SparseLinearFunction(torch.autograd.Function):
                 torch.sum(dY_f32, dim=1, out=dbias)
         dW_values, dX = _spmm_backward(ctx.W, X, dY_f32, ctx.kernel, need_dw,
                                        ctx.needs_input_grad[3], dbias if need_dw else None)
-        return dW_values, dbias, None, (dX.t() if dX is not None else None), None
+        return dW_values, dbias, None, (dX.t() if dX is not None else None), None, None
 
 
 def _narrow_backward(ctx, X: torch.Tensor, dYt: torch.Tensor):
@@ -654,7 +665,7 @@ def _narrow_backward(ctx, X: torch.Tensor, dYt: torch.Tensor):
     dX = torch.empty(X.shape, dtype=torch.float32, device=dev) if need_dx else None
     order = _lib.SLK_DW_SCALAR if ctx.kernel == "scalar" else _lib.SLK_DW_SIMD
     _lib.backward_narrow(W._view(), dYt, X, dW, dbias, dX, order)
-    return dW, dbias, None, (dX.t() if dX is not None else None), None
+    return dW, dbias, None, (dX.t() if dX is not None else None), None, None
 
 
 def spmm(W: PaddedCSR, X: torch.Tensor, *, kernel: str = "auto") -> torch.Tensor:

@@ -12,10 +12,10 @@ lo·lo by 12u, a sum of 128 of them in any order by at most 128u more: 140u of
 sum |q||k| for a score, which changes its weight by that share of A = scale sum |q||k| + |bias|.
 The weights' own rounding, the exponential and the sums over keys add less than 28u, as long
 as their roundings do not all point one way: 168u = 1e-5 of (1 + A)·mag covers both.
-bfloat16, h = 2^-9 (half a step): scores are float32; a weight is rounded to bfloat16 (h of
-its terms), the result too (h): 2h for out and dv. ds takes out rounded by the forward (h),
-is rounded itself (h) and summed into a result that is (h): 3h, and 4h = 2^-7 leaves room
-for the float32 part, 1e-5 (1 + A).
+bfloat16, h = finfo.eps / 2 = 2^-8 (half a step): scores are float32; a weight is rounded to
+bfloat16 (h of its terms), the result too (h): 2h = 2^-7 for out and dv. ds takes out rounded
+by the forward (h), is rounded itself (h) and summed into a result that is (h): 3h, and
+4h = 2^-6 leaves room for the float32 part, 1e-5 (1 + A).
 """
 
 from __future__ import annotations
@@ -107,7 +107,7 @@ def close(name, got, ref, dtype):
     want, mag = ref.val[name], ref.mag[name]
     got = got.detach().double().cpu().reshape(want.shape)
     rms = mag.square().mean().sqrt()
-    share = 1e-5 if dtype is F32 else 2.0 ** (-8 if name in ("out", "dv") else -7)
+    share = 1e-5 if dtype is F32 else 2.0 ** (-7 if name in ("out", "dv") else -6)
     off = (got - want).abs() - share * (mag + 1e-3 * rms)
     assert not got.isnan().any(), name
     assert float(off.max()) <= 0, (name, float(off.max()), float(rms),
