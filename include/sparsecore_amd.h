@@ -931,13 +931,17 @@ typedef struct slk_attn_tensor {
  *              half is, and the second half for d < 0.
  * A query that sees no key, and a row of no sequence, has output 0 and gradient
  * 0. What is masked reaches nothing, whatever it holds.
- * float32 products run on the float16 matrix instructions in two parts an
- * operand (22 bits of an element down to 2^-39 of the largest in its 32 rows of
- * a head); bf16 weights and their gradients are rounded to bf16 between
- * products. Softmax statistics and sums are float32, in a fixed order.
+ * A row with a value that is not finite makes NaN of the results that it has a
+ * part in.
+ * Products run on the float16 matrix instructions, 64 rows of a head scaled by a
+ * power of two: float32 in two parts an operand (22 bits of an element down to
+ * 2^-39 of the largest of those rows), bf16 exact down to 2^-31 of it, weights
+ * and their gradients in 11 bits. Softmax statistics and sums are float32, in a
+ * fixed order.
  *   keep       1 where a backward follows: forward leaves log-sums and packed
  *              operands in saved (slk_attention_saved_bytes); backward takes the
- *              same arguments, q, k, v unchanged (float32 ones are not read)
+ *              same arguments, out and saved as forward left them (q, k and v are
+ *              not read)
  *   scratch    slk_attention_scratch_bytes; saved and scratch 16-byte aligned
  * backward: dq, and dk with dv, where not NULL; dbias (as bias) where not NULL.  */
 #define SLK_ATTN_MAX_DIM 128

@@ -63,14 +63,19 @@ def _tensor(t: torch.Tensor | None) -> _lib.AttnTensor:
     return _lib.AttnTensor(t.data_ptr(), *s)
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """A new tensor of t's shape, in t's order of dimensions in memory, without its gaps."""
+def _order(t: torch.Tensor):
+    """(sizes in t's order of dimensions in memory, the permutation back, dtype, device)."""
     order = sorted(range(t.dim()), key=lambda i: -t.stride(i))
-    out = torch.empty([t.shape[i] for i in order], dtype=t.dtype, device=t.device)
     back = [0] * t.dim()
     for at, i in enumerate(order):
         back[i] = at
-    return out.permute(back)
+    return [t.shape[i] for i in order], back, t.dtype, t.device
+
+
+def _like(order) -> torch.Tensor:
+    """A new tensor of the noted one's shape and order in memory, without its gaps."""
+    sizes, back, dtype, device = order
+    return torch.empty(sizes, dtype=dtype, device=device).permute(back)
 
 
 def _output(q: torch.Tensor, feature_major: bool) -> torch.Tensor:
@@ -81,35 +86,33 @@ def _output(q: torch.Tensor, feature_major: bool) -> torch.Tensor:
     return flat.t().reshape(*q.shape[:-2], h * d).unflatten(-1, (h, d))
 
 
-def _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal, scale,
-          keep):
+def _set_ints(a, offsets, k_offsets, lengths, k_lengths) -> None:
     p = _lib.ptr
-    packed = offsets is not None
-    a = _lib.Attention(
-        n=offsets.numel() - 1 if packed else q.shape[0], rows_q=q.shape[-3], rows_k=k.shape[-3],
-        heads=q.shape[-2], kv_heads=k.shape[-2], dim=q.shape[-1], q=_tensor(q), k=_tensor(k),
-        v=_tensor(v), q_offsets=p(offsets), k_offsets=p(k_offsets), q_lengths=p(lengths),
-        k_lengths=p(k_lengths), scale=scale, dtype=_lib.DTYPES[q.dtype], causal=causal, keep=keep)
-    if bias is not None:
-        a.bias, a.bias_dtype = p(bias), _lib.DTYPES[bias.dtype]
-        a.buckets, a.max_distance = bias.shape[0], max_distance
-        a.bucket_starts = ctypes.addressof(
-            _starts(bias.shape[0] if causal else bias.shape[0] // 2, max_distance))
-    return a
+    a.q_offsets, a.k_offsets = p(offsets), p(k_offsets)
+    a.q_lengths, a.k_lengths = p(lengths), p(k_lengths)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, offsets, k_offsets, lengths, k_lengths, max_distance, causal,
                 scale, feature_major, grad):
+        # Small calls are bound by this host work: as few tensor operations as possible.
         dev = q.device
         keep = grad and any(ctx.needs_input_grad)
-        if bias is not None and not bias.is_contiguous():
-            bias = bias.contiguous()
         out = _output(q, feature_major)
-        a = _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal,
-                  scale, int(keep))
-        a.out = _tensor(out)
+        a = _lib.Attention(
+            n=offsets.shape[0] - 1 if offsets is not None else q.shape[0], rows_q=q.shape[-3],
+            rows_k=k.shape[-3], heads=q.shape[-2], kv_heads=k.shape[-2], dim=q.shape[-1],
+            q=_tensor(q), k=_tensor(k), v=_tensor(v), out=_tensor(out), scale=scale,
+            dtype=_lib.DTYPES[q.dtype], causal=causal, keep=keep)
+        _set_ints(a, offsets, k_offsets, lengths, k_lengths)
+        if bias is not None:
+            if not bias.is_contiguous():
+                bias = bias.contiguous()
+            a.bias, a.bias_dtype = bias.data_ptr(), _lib.DTYPES[bias.dtype]
+            a.buckets, a.max_distance = bias.shape[0], max_distance
+            starts = _starts(bias.shape[0] if causal else bias.shape[0] // 2, max_distance)
+            a.bucket_starts = ctypes.addressof(starts)
         saved = None
         with _lib.on_device(q):
             if keep:
@@ -122,30 +125,33 @@ class _Attention(torch.autograd.Function):
                 a.scratch = scratch.data_ptr()
             _lib.attention_forward(a, _lib.stream_of(q))
         if keep:
-            ctx.save_for_backward(saved, q, k, v, out, bias, offsets, k_offsets, lengths,
-                                  k_lengths)
-            ctx.rest = (max_distance, causal, scale)
+            ctx.save_for_backward(saved, out, bias, offsets, k_offsets, lengths, k_lengths)
+            ctx.args, ctx.starts = a, starts if bias is not None else None
+            ctx.like = [_order(t) if n else None
+                        for t, n in zip((q, k, v), ctx.needs_input_grad)]
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        saved, q, k, v, out, bias, offsets, k_offsets, lengths, k_lengths = ctx.saved_tensors
-        max_distance, causal, scale = ctx.rest
+        saved, out, bias, *ints = ctx.saved_tensors
         need = ctx.needs_input_grad
-        a = _args(q, k, v, offsets, k_offsets, lengths, k_lengths, bias, max_distance, causal,
-                  scale, 1)
-        dq = _like(q) if need[0] else None
-        dk, dv = (_like(k), _like(v)) if need[1] or need[2] else (None, None)
+        # a copy: the graph may be gone through again
+        a = _lib.Attention.from_buffer_copy(ctx.args)
+        _set_ints(a, *ints)
+        dq, dk, dv = (_like(x) if x is not None else None for x in ctx.like)
+        if (dk is None) != (dv is None):  # computed together
+            dk, dv = (torch.empty_like(x if x is not None else y)
+                      for x, y in ((dk, dv), (dv, dk)))
         dbias = torch.empty_like(bias) if bias is not None and need[3] else None
         a.out, a.dout, a.dq, a.dk, a.dv = (_tensor(t) for t in (out, dout, dq, dk, dv))
-        a.saved, a.saved_bytes, a.dbias = saved.data_ptr(), saved.numel(), _lib.ptr(dbias)
-        with _lib.on_device(q):
+        a.saved, a.bias, a.dbias = saved.data_ptr(), _lib.ptr(bias), _lib.ptr(dbias)
+        with _lib.on_device(out):
             a.scratch_bytes = _lib.attention_scratch_bytes(a, True)
             if a.scratch_bytes:
-                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=q.device)
+                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=out.device)
                 a.scratch = scratch.data_ptr()
-            _lib.attention_backward(a, _lib.stream_of(q))
+            _lib.attention_backward(a, _lib.stream_of(out))
         return (dq, dk if need[1] else None, dv if need[2] else None, dbias) + (None,) * 9
 
 
@@ -174,18 +180,20 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
             are rows), as a SparseLinear takes it without a copy.
 
     Returns q's shape. A query that sees no key has output 0 and no gradient, and so has a
-    row that belongs to no sequence; what is masked reaches nothing, whatever it holds. A
-    value that is not finite makes the results whose sums contain it NaN or infinite. Offsets
-    and lengths are read on the device: those out of range, or offsets that fall, count as
+    row that belongs to no sequence; what is masked reaches nothing, whatever it holds. A row
+    of q, k, v or of the output's gradient with a value that is not finite makes NaN of the
+    results that its row has a part in (for few queries without gradients, of what the value
+    itself reaches). Offsets and lengths are read on the device: those out of range, or offsets that fall, count as
     the nearest that do not.
 
-    float32 products run on the matrix cores' float16 instructions in two parts an operand:
-    an element keeps 22 bits down to 2^-39 of the largest in its block of 32 rows of a head,
-    about float32's own rounding. bfloat16 weights (and their gradients) are rounded to
-    bfloat16 between the products. Softmax and sums are float32, in a fixed order: results
-    repeat bit for bit. A forward that a backward may follow keeps log-sums and, in float32
-    or where the layout needs it, the operands once more. q, k, v, the output and the
-    lengths must not change in place before the backward.
+    Products run on the matrix cores' float16 instructions, each block of 64 rows of a head
+    scaled by a power of two of its own. float32 operands go in two parts: an element keeps
+    22 bits down to 2^-39 of the largest of its block, about float32's own rounding.
+    bfloat16 ones are exact down to 2^-31 of it; weights and their gradients are rounded to
+    11 bits between the products. Softmax and sums are float32, in a fixed order: results
+    repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
+    packed (not the tensors themselves), and the output, which must not change in place
+    before the backward, nor may offsets and lengths.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, sizes).

@@ -22,18 +22,10 @@ bool uniform(const slk_attention& a) {
 
 int blocks_of(int64_t dim) { return dim <= 32 ? 1 : dim <= 64 ? 2 : 4; }
 
-// Whether the kernels read a tensor where it lies: bfloat16, a head as wide as a
-// tile, features consecutive, rows of 16-byte pieces, a tile's 64 rows in 31 bits.
-bool direct(const slk_attn_tensor& t, const slk_attention& a) {
-    return a.dtype == SLK_BF16 && a.dim == 32 * blocks_of(a.dim) && t.feature == 1 &&
-           t.row % 8 == 0 && t.head % 8 == 0 && t.batch % 8 == 0 && t.row >= 0 &&
-           t.row < (int64_t{1} << 23) && aligned_to(t.p, 16);
-}
-
 struct Sizes {
     int64_t pad_q, pad_k;         // padded rows, an upper bound
     int64_t q_entries, k_entries; // tiles, an upper bound
-    int64_t elem, row;            // bytes of a packed element and row
+    int64_t row;                  // bytes of a packed row
 };
 
 Sizes sizes_of(const slk_attention& a) {
@@ -49,8 +41,7 @@ Sizes sizes_of(const slk_attention& a) {
         s.q_entries = a.n * ceil_div(a.rows_q, kTileRows);
         s.k_entries = a.n * ceil_div(a.rows_k, kTileRows);
     }
-    s.elem = a.dtype == SLK_F32 ? 4 : 2;
-    s.row = s.elem * 32 * blocks_of(a.dim);
+    s.row = (a.dtype == SLK_F32 ? 4 : 2) * 32 * blocks_of(a.dim);
     return s;
 }
 
@@ -68,30 +59,33 @@ struct Carver {
 struct Packed {
     char* data;
     int32_t* exps;
+    uint64_t* bad;
 };
 
-Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows, bool split) {
+Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows) {
     Packed p;
     p.data = static_cast<char*>(c.take(heads * rows * s.row));
-    p.exps = split ? static_cast<int32_t*>(c.take(heads * (rows / 32) * 4)) : nullptr;
+    p.exps = static_cast<int32_t*>(c.take(heads * (rows / kAttnRows) * 4));
+    p.bad = static_cast<uint64_t*>(c.take(heads * (rows / kAttnRows) * 8));
     return p;
 }
 
 struct Saved {
-    float* lse;
+    float *lse, *bias_rows;
     Packed q, k, v;
     int64_t bytes;
 };
 
 Saved saved_of(const slk_attention& a, void* base) {
     const Sizes s = sizes_of(a);
-    const bool split = a.dtype == SLK_F32;
     Carver c{static_cast<char*>(base)};
     Saved r{};
     r.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
-    if (!direct(a.q, a)) r.q = take_packed(c, s, a.heads, s.pad_q, split);
-    if (!direct(a.k, a)) r.k = take_packed(c, s, a.kv_heads, s.pad_k, split);
-    if (!direct(a.v, a)) r.v = take_packed(c, s, a.kv_heads, s.pad_k, split);
+    if (a.bias != nullptr)
+        r.bias_rows = static_cast<float*>(c.take(a.heads * (2 * a.max_distance + 1) * 4));
+    r.q = take_packed(c, s, a.heads, s.pad_q);
+    r.k = take_packed(c, s, a.kv_heads, s.pad_k);
+    r.v = take_packed(c, s, a.kv_heads, s.pad_k);
     r.bytes = c.at;
     return r;
 }
@@ -114,7 +108,8 @@ Few few_of(const slk_attention& a) {
     const int64_t groups = a.n * a.kv_heads * f.chunks;
     const int64_t want = groups > 0 ? ceil_div(4 * kCus, groups) : 1;
     const int64_t most = ceil_div(a.rows_k, 512);
-    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
+    f.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min({want, most, int64_t{kAttnMaxSplits}})));
     return f;
 }
 
@@ -124,7 +119,7 @@ int splits_of(const slk_attention& a, const Sizes& s) {
     const int64_t groups = s.q_entries * a.heads;
     if (groups == 0 || groups >= kCus) return 1;
     const int64_t most = a.rows_k / 256;
-    return static_cast<int>(std::max<int64_t>(1, std::min(2 * kCus / groups, most)));
+    return static_cast<int>(std::max<int64_t>(1, std::min({2 * kCus / groups, most, int64_t{kAttnMaxSplits}})));
 }
 
 struct Plan {
@@ -181,7 +176,7 @@ Forward forward_of(const slk_attention& a, void* scratch) {
 
 struct Backward {
     Plan plan;
-    float* delta;
+    float *delta, *lse;
     int32_t* dexps;
     Packed dout;
     float* dbias_part;
@@ -194,8 +189,9 @@ Backward backward_of(const slk_attention& a, void* scratch) {
     Backward b{};
     b.plan = take_plan(c, a, s, true);
     b.delta = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
-    if (a.dtype == SLK_F32) b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / 32) * 4));
-    if (!direct(a.dout, a)) b.dout = take_packed(c, s, a.heads, s.pad_q, a.dtype == SLK_F32);
+    b.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
+    b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / kAttnRows) * 4));
+    b.dout = take_packed(c, s, a.heads, s.pad_q);
     if (a.dbias != nullptr)
         b.dbias_part = static_cast<float*>(
             c.take(a.heads * (s.pad_q / kAttnRows) * (2 * a.max_distance + 1) * 4));
@@ -207,39 +203,36 @@ AttnIo io_of(const slk_attn_tensor& t) {
     return AttnIo{static_cast<char*>(t.p), t.batch, t.row, t.head, t.feature};
 }
 
-AttnOp op_of(const slk_attn_tensor& t, const Packed& p, const slk_attention& a, const Sizes& s,
-             int64_t rows) {
-    AttnOp o{};
-    if (p.data == nullptr) {
-        o.p = static_cast<const char*>(t.p);
-        o.sb = 2 * t.batch;
-        o.sr = 2 * t.row;
-        o.sh = 2 * t.head;
-        return o;
-    }
-    o.p = p.data;
-    o.sr = s.row;
-    o.sh = rows * s.row;
-    o.plane = static_cast<int32_t>(s.row / 2);
-    o.packed = 1;
-    o.exps = p.exps;
-    o.exps_sh = rows / 32;
-    (void)a;
-    return o;
+AttnOp op_of(const Packed& p, const Sizes& s, int64_t rows) {
+    return AttnOp{p.data, rows * s.row, p.exps, p.bad, rows / kAttnRows};
 }
 
-AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s, int64_t rows,
-                   int64_t heads, bool keys) {
+// Whether four elements that are consecutive along `unit` start at multiples of
+// four of them: those of the other strides, and the pointer.
+bool fours(const slk_attn_tensor& t, int64_t unit, int64_t a, int64_t b, int64_t c, int dtype) {
+    return unit == 1 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0 &&
+           aligned_to(t.p, dtype == SLK_F32 ? 16 : 8);
+}
+bool four_features(const slk_attn_tensor& t, const slk_attention& a) {
+    return a.dim % 4 == 0 && fours(t, t.feature, t.row, t.head, t.batch, a.dtype);
+}
+
+AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s,
+                   const slk_attention& a, bool keys, int64_t heads) {
+    const int64_t rows = keys ? s.pad_k : s.pad_q;
     AttnPackOp o{};
     o.src = io_of(t);
     o.dst = p.data;
-    o.dst_sr = s.row;
     o.dst_sh = rows * s.row;
     o.exps = p.exps;
-    o.exps_sh = rows / 32;
+    o.bad = p.bad;
+    o.exps_sh = rows / kAttnRows;
     o.rows = rows;
     o.heads = static_cast<int32_t>(heads);
     o.keys = keys;
+    o.vec = four_features(t, a) ? kVecFeatures
+            : fours(t, t.row, t.feature, t.head, t.batch, a.dtype) ? kVecRows
+                                                                   : kVecNone;
     return o;
 }
 
@@ -276,8 +269,11 @@ int make_plan(const slk_attention& a, const Plan& p, hipStream_t st) {
     return attn_launch_plan(g, st);
 }
 
-AttnArgs args_of(const slk_attention& a) {
+AttnArgs args_of(const slk_attention& a, float* bias_rows) {
     AttnArgs g{};
+    g.vec_out = four_features(a.out, a);
+    g.vec_q = four_features(a.dq, a);
+    g.vec_kv = four_features(a.dk, a) && four_features(a.dv, a);
     g.out = io_of(a.out);
     g.dq = io_of(a.dq);
     g.dk = io_of(a.dk);
@@ -293,6 +289,7 @@ AttnArgs args_of(const slk_attention& a) {
     g.scale2 = static_cast<float>(a.scale * 1.4426950408889634);
     if (a.bias != nullptr) {
         g.bias.table = a.bias;
+        g.bias.rows = bias_rows;
         g.bias.dtype = a.bias_dtype;
         g.bias.buckets = static_cast<int32_t>(a.buckets);
         g.bias.max_distance = static_cast<int32_t>(a.max_distance);
@@ -383,7 +380,7 @@ int check(const slk_attention* args, const char* who, bool backward) {
 
 int few_forward(const slk_attention& a, const Forward& f, hipStream_t st) {
     AttnDecode d{};
-    d.g = args_of(a);
+    d.g = args_of(a, nullptr);
     d.g.plan = plan_of(a, f.plan, false);
     d.g.splits = f.splits;
     d.g.part = f.part;
@@ -432,22 +429,23 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     rc = make_plan(a, f.plan, st);
     if (rc != SLK_OK) return rc;
 
-    AttnPack p{};
-    p.plan = plan_of(a, f.plan, false);
-    p.dim = static_cast<int32_t>(a.dim);
-    if (f.saved.q.data) p.op[p.n++] = pack_op(a.q, f.saved.q, s, s.pad_q, a.heads, false);
-    if (f.saved.k.data) p.op[p.n++] = pack_op(a.k, f.saved.k, s, s.pad_k, a.kv_heads, true);
-    if (f.saved.v.data) p.op[p.n++] = pack_op(a.v, f.saved.v, s, s.pad_k, a.kv_heads, true);
-    if (p.n > 0) {
-        rc = attn_launch_pack(p, split, blocks_of(a.dim), a.dtype, st);
-        if (rc != SLK_OK) return rc;
-    }
-    AttnArgs g = args_of(a);
+    AttnArgs g = args_of(a, f.saved.bias_rows);
     g.plan = plan_of(a, f.plan, false);
+    AttnPack p{};
+    p.plan = g.plan;
+    p.dim = g.dim;
+    p.heads = g.heads;
+    p.bias = g.bias;
+    p.n = 3;
+    p.op[0] = pack_op(a.q, f.saved.q, s, a, false, a.heads);
+    p.op[1] = pack_op(a.k, f.saved.k, s, a, true, a.kv_heads);
+    p.op[2] = pack_op(a.v, f.saved.v, s, a, true, a.kv_heads);
+    rc = attn_launch_pack(p, blocks_of(a.dim), a.dtype, st);
+    if (rc != SLK_OK) return rc;
     g.tiles = ceil_div(a.rows_q, kTileRows);
-    g.q = op_of(a.q, f.saved.q, a, s, s.pad_q);
-    g.k = op_of(a.k, f.saved.k, a, s, s.pad_k);
-    g.v = op_of(a.v, f.saved.v, a, s, s.pad_k);
+    g.q = op_of(f.saved.q, s, s.pad_q);
+    g.k = op_of(f.saved.k, s, s.pad_k);
+    g.v = op_of(f.saved.v, s, s.pad_k);
     g.lse = f.saved.lse;
     g.splits = f.splits;
     g.part = f.part;
@@ -470,29 +468,30 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     const Backward b = backward_of(a, a.scratch);
     rc = make_plan(a, b.plan, st);
     if (rc != SLK_OK) return rc;
+    AttnArgs g = args_of(a, sv.bias_rows);
+    g.plan = plan_of(a, b.plan, false);
     if (a.rows_q > 0) {
         AttnPack p{};
-        p.plan = plan_of(a, b.plan, false);
-        p.dim = static_cast<int32_t>(a.dim);
+        p.plan = g.plan;
+        p.dim = g.dim;
         p.n = 1;
-        p.op[0] = pack_op(a.dout, b.dout, s, s.pad_q, a.heads, false);
-        p.op[0].exps_sh = s.pad_q / 32;
+        p.op[0] = pack_op(a.dout, b.dout, s, a, false, a.heads);
         p.o = io_of(a.out);
+        p.o_vec = four_features(a.out, a);
         p.delta = b.delta;
         p.delta_sh = s.pad_q;
+        p.lse = sv.lse;
+        p.lse_out = b.lse;
         p.dexps = b.dexps;
-        rc = attn_launch_pack(p, split, blocks_of(a.dim), a.dtype, st);
+        rc = attn_launch_pack(p, blocks_of(a.dim), a.dtype, st);
         if (rc != SLK_OK) return rc;
     }
-    AttnArgs g = args_of(a);
-    g.plan = plan_of(a, b.plan, false);
     g.tiles = ceil_div(a.rows_q, kTileRows);
-    g.q = op_of(a.q, sv.q, a, s, s.pad_q);
-    g.k = op_of(a.k, sv.k, a, s, s.pad_k);
-    g.v = op_of(a.v, sv.v, a, s, s.pad_k);
-    g.dout = op_of(a.dout, b.dout, a, s, s.pad_q);
-    g.q.exps_sh = s.pad_q / 32;
-    g.lse = sv.lse;
+    g.q = op_of(sv.q, s, s.pad_q);
+    g.k = op_of(sv.k, s, s.pad_k);
+    g.v = op_of(sv.v, s, s.pad_k);
+    g.dout = op_of(b.dout, s, s.pad_q);
+    g.lse = b.lse;
     g.delta = b.delta;
     g.dexps = b.dexps;
     g.dbias_part = b.dbias_part;

@@ -10,7 +10,7 @@ namespace slk {
 
 namespace {
 
-// Exponent above the largest |dS| of a block: |dP| < DP·2^(oe + 1)·2^(ve + 1), and
+// Exponent above the largest |dS| of a pair of tiles: |dP| < DP·2^(oe + 1)·2^(ve + 1), and
 // |delta| < 2^(de + 1).
 __device__ __forceinline__ int ds_exponent(int oe, int ve, int de, int log_dp) {
     return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -100), 100);
@@ -43,10 +43,10 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 // holds 16 queries of one key, as the operands of dV^T = dO^T·P and
 // dK^T = Q^T·dS need them.
 template <bool SPLIT, int DB, bool BIAS>
-__global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 2 ? 2 : 1) void
+__global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dkv_kernel(const AttnArgs g) {
     using T = AttnTile<DB>;
-    constexpr int kPlanes = SPLIT ? 2 : 1, kBytes = kPlanes * T::kPlane, KS = 2 * DB;
+    constexpr int kBytes = (SPLIT ? 2 : 1) * T::kPlane, KS = 2 * DB;
     constexpr int kLogDp = DB == 1 ? 5 : DB == 2 ? 6 : 7;
     __shared__ __align__(16) unsigned char ring0[2 * kBytes + 512];
     __shared__ __align__(16) unsigned char ring1[2 * kBytes + 512];
@@ -62,11 +62,11 @@ attn_dkv_kernel(const AttnArgs g) {
     const int shift = seq.nk - seq.nq;
     const int key0 = tile * 128 + 32 * wv, key = key0 + (lane & 31);
 
-    f32x16 dk[DB][1], dv[DB][1];
+    f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[fb][0][r] = dv[fb][0][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) dk[fb][r] = dv[fb][r] = 0.0f;
     int co = 0, cq = 0;
 
     // tiles of 64 queries, from the first that sees a key of the workgroup
@@ -75,58 +75,47 @@ attn_dkv_kernel(const AttnArgs g) {
     const int nt = tile * 128 < seq.nk && first < n_q ? n_q - first : 0;
 
     if (nt > 0) {
-        const int qrows = g.q.packed ? n_q * kAttnRows : seq.nq;
-        const int orows = g.dout.packed ? n_q * kAttnRows : seq.nq;
-        const AttnLoads<SPLIT, DB> lq(g.q, g.q.rows(sid, seq.q0, seq.pq, kvh * rep), qrows, wv,
-                                      lane);
-        const AttnLoads<SPLIT, DB> lo(g.dout, g.dout.rows(sid, seq.q0, seq.pq, kvh * rep), orows,
-                                      wv, lane);
-        const AttnReads<SPLIT, DB> rd(lane);
+        const int64_t q0_tile = seq.pq / 64 + first;
         auto issue = [&](unsigned char* to, int hr, int qt) __attribute__((always_inline)) {
-            const int r0 = (first + qt) * kAttnRows;
-            lq.issue(to, r0, wv, hr * g.q.sh);
-            lo.issue(to + kBytes, r0, wv, hr * g.dout.sh);
-            const int64_t at = (kvh * rep + hr) * g.lse_sh + seq.pq + r0;
-            if (wv == 0) load_row(g.lse + at, to + 2 * kBytes, lane);
-            if (wv == 1) load_row(g.delta + at, to + 2 * kBytes + 256, lane);
+            const int head = kvh * rep + hr;
+            const int64_t at = (q0_tile + qt) * kBytes;
+            attn_stage<kBytes>(g.q.p + head * g.q.sh + at, to, wv, lane);
+            attn_stage<kBytes>(g.dout.p + head * g.dout.sh + at, to + kBytes, wv, lane);
+            const int64_t row = head * g.lse_sh + (q0_tile + qt) * 64;
+            if (wv == 0) load_row(g.lse + row, to + 2 * kBytes, lane);
+            if (wv == 1) load_row(g.delta + row, to + 2 * kBytes + 256, lane);
         };
         issue(ring0, 0, 0);
+        const AttnReads<SPLIT, DB> rd(lane);
 
         const bool live = key0 < seq.nk;
+        const int k_row = seq.pk + (live ? key0 : 0);
         AttnPair<SPLIT> kf[KS], vf[KS];
         {
-            const int pad = (seq.nk + kAttnRows - 1) / kAttnRows * kAttnRows;
-            const int64_t kr = min(key, (g.k.packed ? pad : seq.nk) - 1);
-            const int64_t vr = min(key, (g.v.packed ? pad : seq.nk) - 1);
-            const char* ka = g.k.rows(sid, seq.k0, seq.pk, kvh) + kr * g.k.sr + 16 * (lane >> 5);
-            const char* va = g.v.rows(sid, seq.k0, seq.pk, kvh) + vr * g.v.sr + 16 * (lane >> 5);
+            const int64_t at = static_cast<int64_t>(k_row / 64) * kBytes;
+            const unsigned char* ka =
+                reinterpret_cast<const unsigned char*>(g.k.p + kvh * g.k.sh + at);
+            const unsigned char* va =
+                reinterpret_cast<const unsigned char*>(g.v.p + kvh * g.v.sh + at);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int p = 0; p < kPlanes; ++p) {
-                    kf[ks].f[p] = *reinterpret_cast<const AttnFrag<SPLIT>*>(
-                        ka + 32 * ks + (p ? g.k.plane : 0));
-                    vf[ks].f[p] = *reinterpret_cast<const AttnFrag<SPLIT>*>(
-                        va + 32 * ks + (p ? g.v.plane : 0));
-                }
+            for (int ks = 0; ks < KS; ++ks) {
+                kf[ks] = rd.along(ka, (k_row >> 5) & 1, ks);
+                vf[ks] = rd.along(va, (k_row >> 5) & 1, ks);
+            }
         }
-        // packed float32: dV in units of 2^(co - 28), dK of 2^(cq - 28), the largest
-        // of the query blocks that this wave's keys are seen by
-        int ke = 0, ve = 0;
-        if constexpr (SPLIT) {
-            const int pk = seq.pk + (live ? key0 : 0);
-            ke = attn_exp(g.k, kvh, pk);
-            ve = attn_exp(g.v, kvh, pk);
-            co = cq = -400;
-            const int b0 = g.causal ? max(0, key0 - shift) / 32 : 0, b1 = 2 * n_q;
+        // dV in units of 2^(co - 28), dK of 2^(cq - 28), the largest of the query
+        // tiles that this wave's keys are seen by
+        const int ke = attn_exp(g.k, kvh, k_row), ve = attn_exp(g.v, kvh, k_row);
+        co = cq = -400;
+        {
+            const int b0 = g.causal ? max(0, key0 - shift) / 64 : 0;
             for (int hr = 0; hr < rep; ++hr) {
-                const int64_t at = seq.pq / 32;
-                const int* oe = g.dout.exps + (kvh * rep + hr) * g.dout.exps_sh + at;
-                const int* qe = g.q.exps + (kvh * rep + hr) * g.q.exps_sh + at;
-                const int* de = g.dexps + (kvh * rep + hr) * g.q.exps_sh + at;
-                for (int i = b0 + lane; i < b1; i += 64) {
-                    co = max(co, oe[i]);
-                    cq = max(cq, ds_exponent(oe[i], ve, de[i], kLogDp) + qe[i]);
+                const int64_t at = (kvh * rep + hr) * g.q.exps_sh + seq.pq / 64;
+                for (int i = b0 + lane; i < n_q; i += 64) {
+                    const int oe = g.dout.exps[at + i] >> 1;
+                    co = max(co, oe);
+                    cq = max(cq, ds_exponent(oe, ve, g.dexps[at + i], kLogDp) +
+                                     (g.q.exps[at + i] >> 1));
                 }
             }
             co = wave_max(co);
@@ -134,50 +123,34 @@ attn_dkv_kernel(const AttnArgs g) {
         }
         const int md = BIAS ? g.bias.max_distance : 0;
 
-        auto compute = [&](const unsigned char* buf, int hr, int q_tile) __attribute__((always_inline)) {
+        auto compute = [&](const unsigned char* buf, int hr, int q_tile)
+            __attribute__((always_inline)) {
+            const int head = kvh * rep + hr, row0 = seq.pq + q_tile;
+            const int qe = attn_exp(g.q, head, row0), oe = attn_exp(g.dout, head, row0);
+            const int de = __builtin_amdgcn_readfirstlane(
+                g.dexps[head * g.q.exps_sh + (row0 >> 6)]);
+            const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
+            // weights times 2^u; dS = weight · (alpha·dp - beta·delta)
+            const int u = kAttnUnit + max(oe - co, -60);
+            const int b = ds_exponent(oe, ve, de, kLogDp);
+            const int x = kAttnUnit - b + max(b + qe - cq, -60) - u;
+            const float unit = static_cast<float>(u);
+            const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit), beta = attn_pow2(x);
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
                 const int q0 = q_tile + 32 * qb;
                 if (q0 >= seq.nq || (g.causal && q0 + 31 + shift < key0)) continue;
                 const bool masked = q0 + 31 >= seq.nq || (g.causal && q0 + shift < key0 + 31);
-                const int head = kvh * rep + hr;
                 f32x16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks) {
                     s = attn_dot<SPLIT>(rd.along(buf, qb, ks), kf[ks], s);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
                     dp = attn_dot<SPLIT>(rd.along(buf + kBytes, qb, ks), vf[ks], dp);
-                float c = g.scale2, unit = 0.0f, alpha = 1.0f, beta = 1.0f;
-                if constexpr (SPLIT) {
-                    const int at = seq.pq + q0;
-                    const int qe = attn_exp(g.q, head, at), oe = attn_exp(g.dout, head, at);
-                    const int de = __builtin_amdgcn_readfirstlane(
-                        g.dexps[head * g.q.exps_sh + (at >> 5)]);
-                    c = ldexpf(c, qe + ke - 2 * kAttnUnit);
-                    // weights times 2^u; dS = weight · (alpha·dp - beta·delta)
-                    const int u = kAttnUnit + max(oe - co, -60);
-                    const int b = ds_exponent(oe, ve, de, kLogDp);
-                    const int x = kAttnUnit - b + max(b + qe - cq, -60) - u;
-                    unit = static_cast<float>(u);
-                    alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit);
-                    beta = attn_pow2(x);
                 }
                 const float* lse = reinterpret_cast<const float*>(buf + 2 * kBytes) + 32 * qb;
                 const float* delta = lse + 64;
-                // the lane's key is seen by rows [lo, hi) of the block
-                const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
-                uint32_t bits[1] = {0xffff};
-                if (masked) {
-                    bits[0] = 0;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = attn_row(r, lane);
-                        bits[0] |= (row >= lo && row < hi ? 1u : 0u) << r;
-                    }
-                }
                 float p[16], ds[16];
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
@@ -187,32 +160,33 @@ attn_dkv_kernel(const AttnArgs g) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = 4 * r4 + j;
-                        float add = SPLIT ? unit - z[j] : -z[j];
+                        float add = unit - z[j];
                         if constexpr (BIAS)
                             add += bias_row[md + attn_clamp(q0 + row + j + shift - key, md)];
                         p[r] = attn_exp2(__builtin_fmaf(s[r], c, add));
-                        if constexpr (SPLIT)
-                            ds[r] = p[r] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
-                        else ds[r] = p[r] * (dp[r] - d[j]);
+                        ds[r] = p[r] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
                     }
                 }
+                // the lane's key is seen by rows [lo, hi) of the block
+                const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const bool see = (bits[0] >> r) & 1;
+                        const int row = attn_row(r, lane);
+                        const bool see = row >= lo && row < hi;
                         p[r] = see ? p[r] : 0.0f;
                         ds[r] = see ? ds[r] : 0.0f;
                     }
                 }
-                AttnPair<SPLIT> w[1][2] = {{attn_operand<SPLIT>(p), attn_operand<SPLIT>(p + 8)}};
-                attn_accumulate<SPLIT, DB, 1>(rd, buf + kBytes, qb, w, dv, masked, bits);
-                w[0][0] = attn_operand<SPLIT>(ds);
-                w[0][1] = attn_operand<SPLIT>(ds + 8);
-                attn_accumulate<SPLIT, DB, 1>(rd, buf, qb, w, dk, masked, bits);
+                AttnPair<SPLIT> wp[2] = {attn_operand<SPLIT>(p), attn_operand<SPLIT>(p + 8)};
+                AttnPair<SPLIT> wd[2] = {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)};
+                attn_accumulate<SPLIT, DB>(rd, buf + kBytes, qb, wp, dv);
+                attn_accumulate<SPLIT, DB>(rd, buf, qb, wd, dk);
             }
         };
         int hr = 0, qt = 0;
-        auto stage = [&](const unsigned char* cur, unsigned char* next) __attribute__((always_inline)) {
+        auto stage = [&](const unsigned char* cur, unsigned char* next)
+            __attribute__((always_inline)) {
             const int h = hr, i = qt;
             if (++qt == nt) {
                 qt = 0;
@@ -222,7 +196,7 @@ attn_dkv_kernel(const AttnArgs g) {
             asm volatile("s_barrier" ::: "memory");
             if (hr < rep) issue(next, hr, qt);
             if (BIAS && i == 0) {  // a head's first tile
-                attn_bias_row(g.bias, g.heads, kvh * rep + h, bias_row);
+                attn_bias_row(g.bias, kvh * rep + h, bias_row);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (live) compute(cur, h, (first + i) * kAttnRows);
@@ -236,18 +210,17 @@ attn_dkv_kernel(const AttnArgs g) {
     }
 
     if (key >= seq.ek) return;
-    const float fk = SPLIT ? ldexpf(g.scale, cq - 2 * kAttnUnit) : g.scale;
-    const float fv = SPLIT ? attn_pow2(co - 2 * kAttnUnit) : 1.0f;
+    const float fk = ldexpf(g.scale, cq - 2 * kAttnUnit), fv = attn_pow2(co - 2 * kAttnUnit);
     const bool zero = key >= seq.nk || nt == 0;
     const AttnIo* const to[2] = {&g.dk, &g.dv};
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const AttnIo& io = *to[which];
         const int64_t at = sid * io.sb + (seq.k0 + key) * io.sr + kvh * io.sh;
-        const bool vec = io.sd == 1 && g.dim % 4 == 0;
+        const bool vec = io.sd == 1 && g.vec_kv;
 #pragma unroll
         for (int fb = 0; fb < DB; ++fb) {
-            f32x16 x = which ? dv[fb][0] : dk[fb][0];
+            f32x16 x = which ? dv[fb] : dk[fb];
             if (zero) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = 0.0f;
@@ -267,7 +240,7 @@ template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dq_kernel(const AttnArgs g) {
     using T = AttnTile<DB>;
-    constexpr int kPlanes = SPLIT ? 2 : 1, kBytes = kPlanes * T::kPlane, KS = 2 * DB;
+    constexpr int kBytes = (SPLIT ? 2 : 1) * T::kPlane, KS = 2 * DB;
     constexpr int kLogDp = DB == 1 ? 5 : DB == 2 ? 6 : 7;
     __shared__ __align__(16) unsigned char ring0[2 * kBytes];
     __shared__ __align__(16) unsigned char ring1[2 * kBytes];
@@ -293,58 +266,54 @@ attn_dq_kernel(const AttnArgs g) {
     float* const far = bins + 8 * width;         // [wave][below, above]
     float below = 0.0f, above = 0.0f;            // distances past the last bins
     if constexpr (BIAS) {
-        attn_bias_row(g.bias, g.heads, head, bias_row);
+        attn_bias_row(g.bias, head, bias_row);
         for (int i = t; i < 8 * width; i += kAttnThreads) bins[i] = 0.0f;
     }
 
-    f32x16 dq[DB][1];
+    f32x16 dq[DB];
 #pragma unroll
     for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dq[fb][0][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) dq[fb][r] = 0.0f;
     int ck = 0;
 
     if (t1 > 0) {
-        const int pad_k = (seq.nk + kAttnRows - 1) / kAttnRows * kAttnRows;
-        const int pad_q = (seq.nq + kAttnRows - 1) / kAttnRows * kAttnRows;
-        const AttnLoads<SPLIT, DB> lk(g.k, g.k.rows(sid, seq.k0, seq.pk, kvh),
-                                      g.k.packed ? pad_k : seq.nk, wv, lane);
-        const AttnLoads<SPLIT, DB> lv(g.v, g.v.rows(sid, seq.k0, seq.pk, kvh),
-                                      g.v.packed ? pad_k : seq.nk, wv, lane);
+        const int64_t k_tile = seq.pk / 64;
+        auto issue = [&](unsigned char* to, int kt) __attribute__((always_inline)) {
+            const int64_t at = (k_tile + kt) * kBytes;
+            attn_stage<kBytes>(g.k.p + kvh * g.k.sh + at, to, wv, lane);
+            attn_stage<kBytes>(g.v.p + kvh * g.v.sh + at, to + kBytes, wv, lane);
+        };
+        issue(ring0, 0);
         const AttnReads<SPLIT, DB> rd(lane);
-        lk.issue(ring0, 0, wv);
-        lv.issue(ring0 + kBytes, 0, wv);
 
+        const int q_row = seq.pq + min(wave0, (seq.nq + 63) / 64 * 64 - 32);
         AttnPair<SPLIT> qf[KS], of[KS];
-        const int64_t qr = min(q, (g.q.packed ? pad_q : seq.nq) - 1);
-        const int64_t orow = min(q, (g.dout.packed ? pad_q : seq.nq) - 1);
-        const char* qa = g.q.rows(sid, seq.q0, seq.pq, head) + qr * g.q.sr + 16 * (lane >> 5);
-        const char* oa =
-            g.dout.rows(sid, seq.q0, seq.pq, head) + orow * g.dout.sr + 16 * (lane >> 5);
+        {
+            const int64_t at = static_cast<int64_t>(q_row / 64) * kBytes;
+            const unsigned char* qa =
+                reinterpret_cast<const unsigned char*>(g.q.p + head * g.q.sh + at);
+            const unsigned char* oa =
+                reinterpret_cast<const unsigned char*>(g.dout.p + head * g.dout.sh + at);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int p = 0; p < kPlanes; ++p) {
-                qf[ks].f[p] = *reinterpret_cast<const AttnFrag<SPLIT>*>(qa + 32 * ks +
-                                                                        (p ? g.q.plane : 0));
-                of[ks].f[p] = *reinterpret_cast<const AttnFrag<SPLIT>*>(oa + 32 * ks +
-                                                                        (p ? g.dout.plane : 0));
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[ks] = rd.along(qa, (q_row >> 5) & 1, ks);
+                of[ks] = rd.along(oa, (q_row >> 5) & 1, ks);
             }
+        }
         const bool mine = q < seq.nq;
-        const int64_t ri = head * g.lse_sh + seq.pq + min(q, pad_q - 1);
+        const int64_t ri = head * g.lse_sh + q_row + (lane & 31);
         const float lse = mine ? g.lse[ri] : INFINITY;
         const float delta = mine ? g.delta[ri] : 0.0f;
-        int qe = 0, oe = 0, de = 0;
-        if constexpr (SPLIT) {
-            const int at = seq.pq + min(wave0, pad_q - 32);
-            qe = attn_exp(g.q, head, at);
-            oe = attn_exp(g.dout, head, at);
-            de = __builtin_amdgcn_readfirstlane(g.dexps[head * g.q.exps_sh + (at >> 5)]);
-            const int* ve = g.v.exps + kvh * g.v.exps_sh + seq.pk / 32;
-            const int* ke = g.k.exps + kvh * g.k.exps_sh + seq.pk / 32;
+        const int qe = attn_exp(g.q, head, q_row), oe = attn_exp(g.dout, head, q_row);
+        const int de =
+            __builtin_amdgcn_readfirstlane(g.dexps[head * g.q.exps_sh + (q_row >> 6)]);
+        {
+            const int* ve = g.v.exps + kvh * g.v.exps_sh + k_tile;
+            const int* ke = g.k.exps + kvh * g.k.exps_sh + k_tile;
             int e = -400;
-            for (int i = lane; i < 2 * t1; i += 64)
-                e = max(e, ds_exponent(oe, ve[i], de, kLogDp) + ke[i]);
+            for (int i = lane; i < t1; i += 64)
+                e = max(e, ds_exponent(oe, ve[i] >> 1, de, kLogDp) + (ke[i] >> 1));
             ck = wave_max(e);
         }
 
@@ -356,25 +325,20 @@ attn_dq_kernel(const AttnArgs g) {
                 if (g.causal && key0 > wave0 + 31 + shift) return;
                 const bool masked =
                     key0 + 31 >= seq.nk || (g.causal && key0 + 31 > wave0 + shift);
+                const int ke = attn_exp(g.k, kvh, seq.pk + key0);
+                const int ve = attn_exp(g.v, kvh, seq.pk + key0);
+                const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
+                const int b = ds_exponent(oe, ve, de, kLogDp);
+                const int x = kAttnUnit - b + max(b + ke - ck, -60);
+                const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit);
+                const float db = delta * attn_pow2(x);
                 f32x16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks) {
                     s = attn_dot<SPLIT>(rd.along(buf, kb, ks), qf[ks], s);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
                     dp = attn_dot<SPLIT>(rd.along(buf + kBytes, kb, ks), of[ks], dp);
-                float c = g.scale2, alpha = 1.0f, db = delta;
-                int x = 0;
-                if constexpr (SPLIT) {
-                    const int ke = attn_exp(g.k, kvh, seq.pk + key0);
-                    const int ve = attn_exp(g.v, kvh, seq.pk + key0);
-                    c = ldexpf(c, qe + ke - 2 * kAttnUnit);
-                    const int b = ds_exponent(oe, ve, de, kLogDp);
-                    x = kAttnUnit - b + max(b + ke - ck, -60);
-                    alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit);
-                    db = delta * attn_pow2(x);
                 }
                 const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
                 const int away = q + shift - key0;
@@ -385,7 +349,6 @@ attn_dq_kernel(const AttnArgs g) {
                     near = lo < md && hi > -md;
                     flat = bias_row[lo >= md ? 2 * md : 0];
                 }
-                uint32_t bits[1] = {0xffff};
                 float ds[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -394,20 +357,15 @@ attn_dq_kernel(const AttnArgs g) {
                         add += near ? bias_row[md + attn_clamp(away - attn_row(r, lane), md)]
                                     : flat;
                     const float p = attn_exp2(__builtin_fmaf(s[r], c, add));
-                    if constexpr (SPLIT) ds[r] = p * __builtin_fmaf(dp[r], alpha, -db);
-                    else ds[r] = p * (dp[r] - db);
+                    ds[r] = p * __builtin_fmaf(dp[r], alpha, -db);
                 }
                 if (masked) {
-                    bits[0] = 0;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const bool see = attn_row(r, lane) <= lim;
-                        ds[r] = see ? ds[r] : 0.0f;
-                        bits[0] |= (see ? 1u : 0u) << r;
-                    }
+                    for (int r = 0; r < 16; ++r)
+                        ds[r] = attn_row(r, lane) <= lim ? ds[r] : 0.0f;
                 }
                 if constexpr (BIAS) {
-                    const float back = SPLIT ? attn_pow2(-x) : 1.0f;
+                    const float back = attn_pow2(-x);
                     if (near) {
                         float* const mine_bins = bins + (2 * wv + (lane >> 5)) * width + md;
 #pragma unroll
@@ -429,17 +387,14 @@ attn_dq_kernel(const AttnArgs g) {
                         else below += y;
                     }
                 }
-                AttnPair<SPLIT> w[1][2] = {{attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)}};
-                attn_accumulate<SPLIT, DB, 1>(rd, buf, kb, w, dq, masked, bits);
+                AttnPair<SPLIT> w[2] = {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)};
+                attn_accumulate<SPLIT, DB>(rd, buf, kb, w, dq);
             }
         };
         auto stage = [&](const unsigned char* cur, unsigned char* next, int kt) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(wait_vm(0));
             asm volatile("s_barrier" ::: "memory");
-            if (kt + 1 < t1) {
-                lk.issue(next, (kt + 1) * kAttnRows, wv);
-                lv.issue(next + kBytes, (kt + 1) * kAttnRows, wv);
-            }
+            if (kt + 1 < t1) issue(next, kt + 1);
             if (wave0 < seq.nq) compute(cur, kt * kAttnRows);
         };
         int kt = 0;
@@ -452,12 +407,12 @@ attn_dq_kernel(const AttnArgs g) {
 
     if (q < seq.eq && g.dq.p != nullptr) {
         const bool zero = q >= seq.nq || t1 == 0;
-        const float f = zero ? 1.0f : SPLIT ? ldexpf(g.scale, ck - 2 * kAttnUnit) : g.scale;
+        const float f = zero ? 1.0f : ldexpf(g.scale, ck - 2 * kAttnUnit);
         const int64_t at = sid * g.dq.sb + (seq.q0 + q) * g.dq.sr + head * g.dq.sh;
-        const bool vec = g.dq.sd == 1 && g.dim % 4 == 0;
+        const bool vec = g.dq.sd == 1 && g.vec_q;
 #pragma unroll
         for (int fb = 0; fb < DB; ++fb) {
-            f32x16 x = dq[fb][0];
+            f32x16 x = dq[fb];
             if (zero) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = 0.0f;

@@ -116,7 +116,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void attn_decode_kernel(const At
     const int md = BIAS ? g.bias.max_distance : 0, width = 2 * md + 1;
     if constexpr (BIAS) {
         for (int r = 0; r < R && r0 + r < n_rows; ++r)
-            attn_bias_row(g.bias, g.heads, kvh * rep + (r0 + r) % rep, bias_rows + r * width);
+            for (int i = threadIdx.x; i < width; i += 64 * kDecodeWaves)
+                bias_rows[r * width + i] =
+                    attn_bias_of(g.bias, g.heads, kvh * rep + (r0 + r) % rep, i - md);
         __syncthreads();
     }
 

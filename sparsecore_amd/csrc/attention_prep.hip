@@ -11,26 +11,33 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kBins = 1024;  // classes of work in the tile order
 
-// Inclusive scan over the workgroup, by sum or maximum.
+// Inclusive scan over the workgroup, by sum or maximum, and its last value.
 template <bool MAX>
-__device__ int64_t scan(int64_t x, int64_t* lds) {
-    const int t = threadIdx.x;
-    lds[t] = x;
-    __syncthreads();
-    for (int o = 1; o < kPlanThreads; o <<= 1) {
-        const int64_t y = t >= o ? lds[t - o] : (MAX ? INT64_MIN : 0);
-        __syncthreads();
-        x = MAX ? (x > y ? x : y) : x + y;
-        lds[t] = x;
-        __syncthreads();
+__device__ int64_t scan(int64_t x, int64_t* lds, int64_t& last) {
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    auto both = [](int64_t a, int64_t b) { return MAX ? (a > b ? a : b) : a + b; };
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o) x = both(x, y);
     }
-    return x;
+    __syncthreads();  // lds may still be read
+    if (lane == 63) lds[wv] = x;
+    __syncthreads();
+    int64_t before = MAX ? INT64_MIN : 0, all = before;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        if (w == wv) before = all;
+        all = both(all, lds[w]);
+    }
+    last = all;
+    return wv == 0 ? x : both(before, x);
 }
 
 // One workgroup. Offsets that fall, or pass the arrays' end, are taken as the
 // nearest ones that do not: no row is written twice or outside.
 __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanArgs a) {
-    __shared__ int64_t lds[kPlanThreads];
+    __shared__ int64_t lds[kPlanThreads / 64];
     __shared__ int32_t bin[kBins];
     const int t = threadIdx.x;
     const bool packed = a.q_offsets != nullptr;
@@ -44,10 +51,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
             // starts: running maximum of the offsets so far, ends: with the next one
             const int64_t oq = in ? clamp(a.q_offsets[s], a.rows_q) : 0;
             const int64_t ok = in ? clamp(a.k_offsets[s], a.rows_k) : 0;
-            int64_t bq = scan<true>(oq, lds);
-            __syncthreads();
-            int64_t bk = scan<true>(ok, lds);
-            __syncthreads();
+            int64_t last;
+            int64_t bq = scan<true>(oq, lds, last), bk = scan<true>(ok, lds, last);
             bq = bq > endq ? bq : endq;
             bk = bk > endk ? bk : endk;
             const int64_t nq = in ? clamp(a.q_offsets[s + 1], a.rows_q) : 0;
@@ -56,18 +61,10 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
             x.k0 = static_cast<int32_t>(bk);
             x.nq = x.eq = static_cast<int32_t>(nq > bq ? nq - bq : 0);
             x.nk = x.ek = static_cast<int32_t>(nk > bk ? nk - bk : 0);
-            int64_t lq = scan<true>(in ? bq + x.nq : 0, lds);
-            lds[t] = lq;
-            __syncthreads();
-            lq = lds[kPlanThreads - 1];
-            __syncthreads();
-            int64_t lk = scan<true>(in ? bk + x.nk : 0, lds);
-            lds[t] = lk;
-            __syncthreads();
-            lk = lds[kPlanThreads - 1];
-            __syncthreads();
-            endq = lq > endq ? lq : endq;
-            endk = lk > endk ? lk : endk;
+            scan<true>(in ? bq + x.nq : 0, lds, last);
+            endq = last > endq ? last : endq;
+            scan<true>(in ? bk + x.nk : 0, lds, last);
+            endk = last > endk ? last : endk;
         } else {
             auto live = [&](const int32_t* p, int64_t rows) {
                 const int64_t n = p != nullptr ? p[s] : rows;
@@ -80,12 +77,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         }
         const int64_t wq = in ? ceil_div(x.nq, kAttnRows) * kAttnRows : 0;
         const int64_t wk = in ? ceil_div(x.nk, kAttnRows) * kAttnRows : 0;
-        const int64_t iq = scan<false>(wq, lds);
-        const int64_t totq = lds[kPlanThreads - 1];
-        __syncthreads();
-        const int64_t ik = scan<false>(wk, lds);
-        const int64_t totk = lds[kPlanThreads - 1];
-        __syncthreads();
+        int64_t totq, totk;
+        const int64_t iq = scan<false>(wq, lds, totq), ik = scan<false>(wk, lds, totk);
         x.pq = static_cast<int32_t>(pq + iq - wq);
         x.pk = static_cast<int32_t>(pk + ik - wk);
         pq += totq;
@@ -149,8 +142,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         each([&](int b, int, int) { atomicAdd(&bin[b], 1); });
         __syncthreads();
         const int64_t mine = bin[t];
-        const int64_t upto = scan<false>(mine, lds);
-        const int64_t all = lds[kPlanThreads - 1];
+        int64_t all;
+        const int64_t upto = scan<false>(mine, lds, all);
         bin[t] = static_cast<int32_t>(upto - mine);
         __syncthreads();
         // the order inside a class does not change a result: tiles are independent
@@ -192,101 +185,159 @@ __device__ __forceinline__ RowOf row_of(const AttnPlan& p, bool keys, int64_t pa
     return r;
 }
 
-// Loads 32 rows of one head of a tensor into LDS as float32, zeros past the
-// sequence's last row and past dim. Lanes run along whichever of rows and
-// features is consecutive in memory.
-template <class IO, int DP>
-__device__ __forceinline__ void load_rows(const AttnIo& x, int64_t at, int live, int dim,
-                                          float (*to)[DP + 1]) {
-    const bool rows_first = x.sr == 1 && x.sd != 1;
-    for (int i = threadIdx.x; i < 32 * DP; i += kAttnThreads) {
-        const int r = rows_first ? i % 32 : i / DP, f = rows_first ? i / 32 : i % DP;
-        to[r][f] = r < live && f < dim ? IO::load(x.p, at + r * x.sr + f * x.sd) : 0.0f;
-    }
-}
-
-// Packs 32 rows of one head: blockIdx.x the block of padded rows, blockIdx.y the
-// head of an operand. With o given (dO and O) also delta, and dO's part only if
-// it is packed.
-template <bool SPLIT, int DP, class IO>
+// Packs a tile of 64 rows of one head: blockIdx.x the tile, blockIdx.y the head of
+// an operand; one more y for the rows of biases, a head each. Lanes run along
+// whichever of rows and features is consecutive in memory. Of dO (with delta
+// given) also delta, from the same tile and O. What bounds it is memory.
+template <bool SPLIT, int DB, class IO>
 __global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(const AttnPack a) {
-    __shared__ float x[32][DP + 1];
+    constexpr int DP = 32 * DB;
+    __shared__ float x[kAttnRows][DP + 1];
     __shared__ int32_t top;
+    __shared__ uint32_t odd[2];  // rows with a value that is not finite
+    const int t = threadIdx.x;
     int which = 0, head = blockIdx.y;
-    while (head >= a.op[which].heads) head -= a.op[which++].heads;
+    while (which < a.n && head >= a.op[which].heads) head -= a.op[which++].heads;
+    if (which == a.n) {
+        const int width = 2 * a.bias.max_distance + 1;
+        for (int h = blockIdx.x; h < a.heads; h += gridDim.x)
+            for (int i = t; i < width; i += kAttnThreads)
+                a.bias.rows[static_cast<int64_t>(h) * width + i] =
+                    attn_bias_of(a.bias, a.heads, h, i - a.bias.max_distance);
+        return;
+    }
     const AttnPackOp& op = a.op[which];
-    const int64_t padded = static_cast<int64_t>(blockIdx.x) * 32;
+    const int64_t padded = static_cast<int64_t>(blockIdx.x) * kAttnRows;
     if (padded >= op.rows) return;
     const RowOf ro = row_of(a.plan, op.keys, padded);
     if (!ro.any) return;
     const int n = op.keys ? ro.seq.nk : ro.seq.nq, first = op.keys ? ro.seq.k0 : ro.seq.q0;
-    const int live = min(max(n - ro.row, 0), 32);
+    const int live = min(max(n - ro.row, 0), kAttnRows);
     const int64_t row = first + ro.row;
-    if (threadIdx.x == 0) top = 0;
-    load_rows<IO, DP>(op.src, ro.sid * op.src.sb + row * op.src.sr + head * op.src.sh, live,
-                      a.dim, x);
+    if (t == 0) top = odd[0] = odd[1] = 0;
     __syncthreads();
-
-    if (a.delta != nullptr && which == 0) {
-        // eight threads a row
-        const int r = threadIdx.x / 8, part = threadIdx.x % 8;
-        float d = 0.0f;
-        const int64_t at = ro.sid * a.o.sb + (row + r) * a.o.sr + head * a.o.sh;
-        if (r < live)
-            for (int f = part; f < a.dim; f += 8)
-                d = __builtin_fmaf(x[r][f], IO::load(a.o.p, at + f * a.o.sd), d);
+    const int64_t at = ro.sid * op.src.sb + row * op.src.sr + head * op.src.sh;
+    uint32_t m = 0;  // the largest finite magnitude
+    auto put = [&](int r, int f, float v) {
+        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+        if (b < 0x7f800000u) {
+            m = max(m, b);
+        } else {
+            v = 0.0f;
+            atomicOr(&odd[r >> 5], 1u << (r & 31));
+        }
+        x[r][f] = v;
+    };
+    if (op.vec == kVecFeatures) {
+        for (int i = t; i < kAttnRows * DP / 4; i += kAttnThreads) {
+            const int r = i / (DP / 4), f = 4 * (i % (DP / 4));
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (r < live && f < a.dim) IO::load4(op.src.p, at + r * op.src.sr + f, v);
 #pragma unroll
-        for (int s = 1; s < 8; s <<= 1) d += __shfl_xor(d, s);
-        if (part == 0) a.delta[head * a.delta_sh + padded + r] = r < live ? d : 0.0f;
-        if constexpr (SPLIT) {
-            const uint32_t bits = __float_as_uint(d) & 0x7fffffffu;
-            if (part == 0 && r < live && bits < 0x7f800000u) atomicMax(&top, static_cast<int>(bits));
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                a.dexps[head * op.exps_sh + padded / 32] =
-                    max(static_cast<int>(static_cast<uint32_t>(top) >> 23) - 127, -100);
-                top = 0;
+            for (int j = 0; j < 4; ++j) put(r, f + j, v[j]);
+        }
+    } else if (op.vec == kVecRows) {
+        for (int i = t; i < kAttnRows * DP / 4; i += kAttnThreads) {
+            const int r = 4 * (i % (kAttnRows / 4)), f = i / (kAttnRows / 4);
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int64_t from = at + r + f * op.src.sd;
+            if (f < a.dim) {
+                // four rows at once where they are aligned and all live
+                if (r + 4 <= live && ((row + r) & 3) == 0) {
+                    IO::load4(op.src.p, from, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (r + j < live) v[j] = IO::load(op.src.p, from + j);
+                }
             }
-            __syncthreads();
-        }
-    }
-    if (op.dst == nullptr) return;
-
-    float factor = 1.0f;
-    if constexpr (SPLIT) {
-        uint32_t m = 0;  // the largest finite magnitude
-        for (int i = threadIdx.x; i < 32 * DP; i += kAttnThreads) {
-            const uint32_t b = __float_as_uint(x[i / DP][i % DP]) & 0x7fffffffu;
-            if (b < 0x7f800000u) m = max(m, b);
-        }
 #pragma unroll
-        for (int s = 32; s > 0; s >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, s)));
-        if ((threadIdx.x & 63) == 0) atomicMax(&top, static_cast<int>(m));
-        __syncthreads();
-        const int e = max(static_cast<int>(static_cast<uint32_t>(top) >> 23) - 127, -100);
-        factor = ldexpf(1.0f, kAttnUnit - e);
-        if (threadIdx.x == 0) op.exps[head * op.exps_sh + padded / 32] = e;
+            for (int j = 0; j < 4; ++j) put(r + j, f, v[j]);
+        }
+    } else {
+        const bool rows_first = op.src.sr == 1 && op.src.sd != 1;
+        for (int i = t; i < kAttnRows * DP; i += kAttnThreads) {
+            const int r = rows_first ? i % kAttnRows : i / DP;
+            const int f = rows_first ? i / kAttnRows : i % DP;
+            float v = 0.0f;
+            if (r < live && f < a.dim) v = IO::load(op.src.p, at + r * op.src.sr + f * op.src.sd);
+            put(r, f, v);
+        }
     }
-    constexpr int kPieces = DP / 8;
-    char* const to = op.dst + head * op.dst_sh + padded * op.dst_sr;
-    for (int i = threadIdx.x; i < 32 * kPieces; i += kAttnThreads) {
-        const int r = i / kPieces, c = i % kPieces;
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, s)));
+    __syncthreads();
+    if ((t & 63) == 0) atomicMax(&top, static_cast<int>(m));
+    __syncthreads();
+    const int e = max(static_cast<int>(static_cast<uint32_t>(top) >> 23) - 127, -100);
+    const uint64_t bad = static_cast<uint64_t>(odd[1]) << 32 | odd[0];
+    if (t == 0) {
+        op.exps[head * op.exps_sh + padded / kAttnRows] = 2 * e + (bad != 0 ? 1 : 0);
+        op.bad[head * op.exps_sh + padded / kAttnRows] = bad;
+    }
+
+    // rows in pieces of eight features, permuted as they will lie in LDS
+    using T = AttnTile<DB>;
+    const float factor = ldexpf(1.0f, kAttnUnit - e);
+    char* const to = op.dst + head * op.dst_sh +
+                     static_cast<int64_t>(blockIdx.x) * ((SPLIT ? 2 : 1) * T::kPlane);
+    for (int i = t; i < kAttnRows * T::kPieces; i += kAttnThreads) {
+        const int r = i / T::kPieces, c = (i % T::kPieces) ^ T::swz(r);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x[r][8 * c + j] * factor;
         const AttnPair<SPLIT> f = attn_operand<SPLIT>(v);
-        *reinterpret_cast<AttnFrag<SPLIT>*>(to + r * op.dst_sr + 16 * c) = f.f[0];
-        if constexpr (SPLIT)
-            *reinterpret_cast<AttnFrag<SPLIT>*>(to + r * op.dst_sr + 2 * DP + 16 * c) = f.f[1];
+        *reinterpret_cast<f16x8*>(to + 16 * i) = f.f[0];
+        if constexpr (SPLIT) *reinterpret_cast<f16x8*>(to + T::kPlane + 16 * i) = f.f[1];
+    }
+
+    if (a.delta == nullptr) return;
+    __syncthreads();
+    if (t == 0) top = 0;
+    __syncthreads();
+    // delta: lanes over rows where O's rows are consecutive, else four lanes a row
+    const bool rows_first = a.o.sr == 1 && a.o.sd != 1;
+    const int r = rows_first ? t % 64 : t / 4, part = rows_first ? t / 64 : t % 4;
+    float d = 0.0f;
+    const int64_t from = ro.sid * a.o.sb + (row + r) * a.o.sr + head * a.o.sh;
+    if (r < live) {
+        if (a.o_vec && !rows_first) {
+            for (int f = 4 * part; f < a.dim; f += 16) {
+                float v[4];
+                IO::load4(a.o.p, from + f, v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d = __builtin_fmaf(x[r][f + j], v[j], d);
+            }
+        } else {
+            for (int f = part; f < a.dim; f += 4)
+                d = __builtin_fmaf(x[r][f], IO::load(a.o.p, from + f * a.o.sd), d);
+        }
+    }
+    __syncthreads();
+    float* const sums = &x[0][0];
+    sums[4 * r + part] = d;
+    __syncthreads();
+    if (t < kAttnRows) {
+        const float y = (sums[4 * t] + sums[4 * t + 1]) + (sums[4 * t + 2] + sums[4 * t + 3]);
+        const int64_t at_row = head * a.delta_sh + padded + t;
+        a.delta[at_row] = y;
+        a.lse_out[at_row] = (bad >> t) & 1 ? __builtin_nanf("") : a.lse[at_row];
+        uint32_t b = __float_as_uint(y) & 0x7fffffffu;
+        b = b < 0x7f800000u ? b : 0;
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) b = max(b, static_cast<uint32_t>(__shfl_xor(b, s)));
+        if (t == 0)
+            a.dexps[head * op.exps_sh + padded / kAttnRows] =
+                max(static_cast<int>(b >> 23) - 127, -100);
     }
 }
 
 template <bool SPLIT, class IO>
 int pack(const AttnPack& a, int db, dim3 grid, hipStream_t st) {
     const dim3 wg(kAttnThreads);
-    if (db == 1) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 32, IO>), grid, wg, 0, st, a);
-    else if (db == 2) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 64, IO>), grid, wg, 0, st, a);
-    else hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 128, IO>), grid, wg, 0, st, a);
+    if (db == 1) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 1, IO>), grid, wg, 0, st, a);
+    else if (db == 2) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 2, IO>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 4, IO>), grid, wg, 0, st, a);
     return check_launch("attention: pack");
 }
 
@@ -297,17 +348,16 @@ int attn_launch_plan(const AttnPlanArgs& a, hipStream_t st) {
     return check_launch("attention: plan");
 }
 
-int attn_launch_pack(const AttnPack& a, bool split, int db, int dtype, hipStream_t st) {
-    int64_t rows = 0, heads = 0;
+int attn_launch_pack(const AttnPack& a, int db, int dtype, hipStream_t st) {
+    int64_t rows = 0, heads = a.bias.table != nullptr ? 1 : 0;
     for (int i = 0; i < a.n; ++i) {
         rows = rows > a.op[i].rows ? rows : a.op[i].rows;
         heads += a.op[i].heads;
     }
-    if (rows == 0 || heads == 0) return SLK_OK;
+    if (rows == 0) return SLK_OK;
     if (heads > 65535) return fail(SLK_EINVAL, "attention: too many heads");
-    const dim3 grid(static_cast<unsigned>(rows / 32), static_cast<unsigned>(heads));
+    const dim3 grid(static_cast<unsigned>(rows / kAttnRows), static_cast<unsigned>(heads));
     if (dtype == SLK_F32) return pack<true, F32>(a, db, grid, st);
-    (void)split;
     return pack<false, BF16>(a, db, grid, st);
 }
 

@@ -15,26 +15,34 @@ struct AttnPlanArgs {
     int32_t tile_q, tile_k, causal, work_shift;
 };
 
+// How a pack reads four elements at once: not, four features, four rows.
+enum AttnVec { kVecNone = 0, kVecFeatures = 1, kVecRows = 2 };
+
 struct AttnPackOp {
     AttnIo src;
-    char* dst;       // NULL: delta only
-    int64_t dst_sr, dst_sh;
+    char* dst;
+    int64_t dst_sh;
     int32_t* exps;
+    uint64_t* bad;
     int64_t exps_sh, rows;
-    int32_t heads, keys;
+    int32_t heads, keys, vec;
 };
 
 struct AttnPack {
     AttnPlan plan;
     AttnPackOp op[3];
-    int32_t n, dim;
+    int32_t n, dim, heads;
+    AttnBias bias;   // with a table: its rows are made too
     AttnIo o;        // with delta: op[0] is dO, this is O
+    int32_t o_vec;
     float* delta;
+    const float* lse;
+    float* lse_out;  // lse, NaN where a row of dO is not finite
     int64_t delta_sh;
     int32_t* dexps;
 };
 
 int attn_launch_plan(const AttnPlanArgs& a, hipStream_t st);
-int attn_launch_pack(const AttnPack& a, bool split, int db, int dtype, hipStream_t st);
+int attn_launch_pack(const AttnPack& a, int db, int dtype, hipStream_t st);
 
 }  // namespace slk
