@@ -874,7 +874,8 @@ SLK_API int slk_linear_ce_backward(const slk_linear_ce* args_host, void* stream)
 /* An activation y = f(x) of n elements, and what its backward needs of x in 8
  * bits: SLK_ACT_BLOCK consecutive elements share a scale, the largest finite
  * magnitude of them (top); q = round(x·(127 / top)) stands for q·(top·(1/127)),
- * float32 operations. top < 2^-100: zeros; q = -128: not finite, NaN.
+ * float32 operations. top < 2^-100: zeros. Values that are not finite have
+ * q = -128 (NaN), and their block's scale has its sign bit set.
  *   forward    x in; y (NULL: not wanted) and, where not NULL, codes (n bytes)
  *              and scales (one a block, float32) out
  *   backward   dx = dy·f'(x), x from the codes, or itself where codes is NULL;

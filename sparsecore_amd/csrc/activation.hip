@@ -6,7 +6,9 @@
 // value q · (top · (1/127)): off by at most top / 254. Each operation is one
 // correctly rounded float32 operation in the order written, so codes do not
 // depend on the kernel that makes them. top < 2^-100 keeps zeros; an element that
-// is not finite has the code -128 and is NaN again, its neighbours keep theirs.
+// is not finite has the code -128 and is NaN again, its neighbours keep theirs,
+// and the block's scale is stored with its sign bit set, so that the others need
+// not look for such codes.
 //
 // One pass each way: x in, y and the codes out; dy and the codes in, dx out. What
 // bounds it is memory. A wave takes whole blocks, four elements a lane, four
@@ -22,38 +24,72 @@ static_assert(kActBlock == 4 * kWave, "four elements a lane: a wave holds one bl
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kManyBlocks = 4;  // blocks a wave takes at a time, of large arrays
 
-// f and its derivative. Float32, relative errors of a few 2^-24 of |f| + |x f'|.
-template <int KIND>
+// 0.5·erfc(|x| / sqrt 2) and exp(-x^2 / 2), for results that are rounded to
+// bfloat16: Abramowitz and Stegun's 7.1.26, off by at most 1e-7. (erfcf takes some
+// 60 instructions, and with it the kernel was bound by them.)
+__device__ __forceinline__ float half_erfc_fast(float x, float& bell) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164189f, fabsf(x), 1.0f));
+    bell = __builtin_amdgcn_exp2f(-0.72134752f * x * x);
+    float p = __builtin_fmaf(t, 0.53070271f, -0.72657601f);
+    p = __builtin_fmaf(t, p, 0.71070687f);
+    p = __builtin_fmaf(t, p, -0.14224837f);
+    p = __builtin_fmaf(t, p, 0.12741480f);
+    return t * p * bell;
+}
+
+// 1 / (1 + exp(-x))
+template <bool FAST>
+__device__ __forceinline__ float logistic(float x) {
+    if constexpr (FAST)
+        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+    else return 1.0f / (1.0f + expf(-x));
+}
+
+// f and its derivative. Float32, relative errors of a few 2^-24 of |f| + |x f'|;
+// FAST: 2^-20, for results that are rounded to bfloat16.
+template <int KIND, bool FAST>
 __device__ __forceinline__ float act(float x) {
     if constexpr (KIND == SLK_ACT_RELU) {
         return x <= 0.0f ? 0.0f : x;
     } else if constexpr (KIND == SLK_ACT_SILU) {
-        return x / (1.0f + expf(-x));
+        if constexpr (FAST) return x * logistic<true>(x);
+        else return x / (1.0f + expf(-x));
     } else if constexpr (KIND == SLK_ACT_GELU) {
+        if constexpr (FAST) {
+            float bell;
+            const float h = half_erfc_fast(x, bell);
+            return x * (x < 0.0f ? h : 1.0f - h);
+        }
         // x·Phi(x) by the complement, which keeps its digits for negative x
         return 0.5f * x * erfcf(-0.70710678f * x);
     } else if constexpr (KIND == SLK_ACT_GELU_TANH) {
         // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3)
         const float u2 = 1.5957691f * __builtin_fmaf(0.044715f * x * x, x, x);
-        return x / (1.0f + expf(-u2));
+        if constexpr (FAST) return x * logistic<true>(u2);
+        else return x / (1.0f + expf(-u2));
     } else {
         return x;
     }
 }
 
-template <int KIND>
+template <int KIND, bool FAST>
 __device__ __forceinline__ float slope(float x) {
     if constexpr (KIND == SLK_ACT_RELU) {
         return x > 0.0f ? 1.0f : x <= 0.0f ? 0.0f : x;
     } else if constexpr (KIND == SLK_ACT_SILU) {
-        const float s = 1.0f / (1.0f + expf(-x));
+        const float s = logistic<FAST>(x);
         return s * __builtin_fmaf(x, 1.0f - s, 1.0f);
     } else if constexpr (KIND == SLK_ACT_GELU) {
+        if constexpr (FAST) {
+            float bell;
+            const float h = half_erfc_fast(x, bell);
+            return __builtin_fmaf(x * 0.39894228f, bell, x < 0.0f ? h : 1.0f - h);
+        }
         return __builtin_fmaf(x * 0.39894228f, expf(-0.5f * x * x), 0.5f * erfcf(-0.70710678f * x));
     } else if constexpr (KIND == SLK_ACT_GELU_TANH) {
         const float u2 = 1.5957691f * __builtin_fmaf(0.044715f * x * x, x, x);
         const float d2 = 1.5957691f * __builtin_fmaf(0.134145f * x, x, 1.0f);
-        const float s = 1.0f / (1.0f + expf(-u2));
+        const float s = logistic<FAST>(u2);
         // s (1 - s) is 0 where u2 overflows; x d2 is not to make NaN of it
         const float t = s * (1.0f - s);
         return t == 0.0f ? s : __builtin_fmaf(x * d2, t, s);
@@ -85,34 +121,66 @@ __device__ __forceinline__ void store_four(void* p, int64_t i, int64_t n, bool v
     }
 }
 
-// Codes of a block's four elements of a lane, in one word; top in every lane.
-__device__ __forceinline__ uint32_t encode(const float (&x)[4], float& top) {
+// Maximum over the wave's lanes, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
+    auto dpp = [&](auto ctrl) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+            0, static_cast<int>(m), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    m = max(m, dpp(std::integral_constant<int, 0xb1>{}));   // lanes 1, 0, 3, 2 of four
+    m = max(m, dpp(std::integral_constant<int, 0x4e>{}));   // lanes 2, 3, 0, 1
+    m = max(m, dpp(std::integral_constant<int, 0x141>{}));  // half-row mirror
+    m = max(m, dpp(std::integral_constant<int, 0x140>{}));  // row mirror
+    m = max(m, static_cast<uint32_t>(__shfl_xor(m, 16)));
+    return max(m, static_cast<uint32_t>(__shfl_xor(m, 32)));
+}
+
+// Codes of a block's four elements of a lane, in one word; its scale in every
+// lane. x + 1.5·2^23 rounds to the nearest whole number (ties to even) and holds
+// it in its low bits.
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], float& scale) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-        if (b < 0x7f800000u) m = max(m, b);
-    }
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    m = __builtin_amdgcn_readfirstlane(wave_max(m));
+    const bool odd = m >= 0x7f800000u;  // the same for all lanes
+    if (odd) {
+        m = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, o)));
-    top = __uint_as_float(m);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
+            if (b < 0x7f800000u) m = max(m, b);
+        }
+        m = __builtin_amdgcn_readfirstlane(wave_max(m));
+    }
+    const float top = __uint_as_float(m);
     const float inv = top >= 0x1p-100f ? 127.0f / top : 0.0f;
+    scale = __uint_as_float(m | (odd ? 0x80000000u : 0u));
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const bool finite = (__float_as_uint(x[j]) & 0x7fffffffu) < 0x7f800000u;
-        const int q = finite ? static_cast<int>(rintf(x[j] * inv)) : -128;
-        w |= (static_cast<uint32_t>(q) & 0xffu) << (8 * j);
+        const float r = x[j] * inv + 12582912.0f;
+        w |= (__float_as_uint(r) & 0xffu) << (8 * j);
+    }
+    if (odd) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((__float_as_uint(x[j]) & 0x7fffffffu) >= 0x7f800000u)
+                w = (w & ~(0xffu << (8 * j))) | (0x80u << (8 * j));
     }
     return w;
 }
 
-__device__ __forceinline__ void decode(uint32_t w, float top, float (&x)[4]) {
+__device__ __forceinline__ void decode(uint32_t w, float scale, float (&x)[4]) {
+    const float top = fabsf(scale);
     const float step = top >= 0x1p-100f ? top * (1.0f / 127.0f) : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int q = static_cast<int>(w << (24 - 8 * j)) >> 24;
-        x[j] = q == -128 ? __builtin_nanf("") : static_cast<float>(q) * step;
+    for (int j = 0; j < 4; ++j)
+        x[j] = static_cast<float>(static_cast<int>(w << (24 - 8 * j)) >> 24) * step;
+    if (__float_as_uint(scale) >> 31) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (((w >> (8 * j)) & 0xffu) == 0x80u) x[j] = __builtin_nanf("");
     }
 }
 
@@ -164,15 +232,15 @@ __global__ __launch_bounds__(kThreads) void act_forward_kernel(const ActArgs a) 
         const int64_t at = (b0 + b) * kActBlock + 4 * (threadIdx.x & 63);
         if ((b0 + b) * kActBlock >= a.n) return;  // the same for all lanes
         if (a.codes != nullptr) {
-            float top;
-            const uint32_t w = encode(x[b], top);
+            float scale;
+            const uint32_t w = encode(x[b], scale);
             store_codes(a.codes, at, a.n, a.vec_codes, w);
-            if ((threadIdx.x & 63) == 0) a.scales[b0 + b] = top;
+            if ((threadIdx.x & 63) == 0) a.scales[b0 + b] = scale;
         }
         if (a.y != nullptr) {
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = act<KIND>(x[b][j]);
+            for (int j = 0; j < 4; ++j) y[j] = act<KIND, IO::kBytes == 2>(x[b][j]);
             store_four<IO>(a.y, at, a.n, a.vec_y, y);
         }
     }
@@ -185,13 +253,13 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(const ActArgs a)
     const int64_t b0 = first_block(PER);
     float dy[PER][4], x[PER][4];
     uint32_t w[PER];
-    float top[PER];
+    float scale[PER];
 #pragma unroll
     for (int b = 0; b < PER; ++b) {
         const int64_t at = (b0 + b) * kActBlock + 4 * (threadIdx.x & 63);
         if (a.codes != nullptr) {
             w[b] = load_codes(a.codes, at, a.n, a.vec_codes);
-            top[b] = (b0 + b) * kActBlock < a.n ? a.scales[b0 + b] : 0.0f;
+            scale[b] = (b0 + b) * kActBlock < a.n ? a.scales[b0 + b] : 0.0f;
         } else {
             load_four<IO>(a.x, at, a.n, a.vec_codes, x[b]);
         }
@@ -201,11 +269,11 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(const ActArgs a)
     for (int b = 0; b < PER; ++b) {
         const int64_t at = (b0 + b) * kActBlock + 4 * (threadIdx.x & 63);
         if ((b0 + b) * kActBlock >= a.n) return;
-        if (a.codes != nullptr) decode(w[b], top[b], x[b]);
+        if (a.codes != nullptr) decode(w[b], scale[b], x[b]);
         float dx[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            dx[j] = a.dy != nullptr ? dy[b][j] * slope<KIND>(x[b][j]) : x[b][j];
+            dx[j] = a.dy != nullptr ? dy[b][j] * slope<KIND, IO::kBytes == 2>(x[b][j]) : x[b][j];
         store_four<IO>(a.dx, at, a.n, a.vec_y, dx);
     }
 }

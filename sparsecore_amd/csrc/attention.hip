@@ -9,7 +9,7 @@ namespace slk {
 
 namespace {
 
-constexpr int64_t kTileRows = 128;   // rows of a workgroup of every tiled kernel
+constexpr int64_t kTileRows = kAttnTileRows;
 constexpr int kFewRows = 16;         // queries of an entry that go the way of single tokens
 constexpr int64_t kCus = 256;
 
@@ -70,7 +70,24 @@ Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows) {
     return p;
 }
 
+struct Plan {
+    AttnSeq* seqs;
+    int2 *q_list, *k_list;
+    int32_t* count;
+};
+
+Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s) {
+    Plan p{};
+    if (uniform(a)) return p;
+    p.count = static_cast<int32_t*>(c.take(16));
+    p.seqs = static_cast<AttnSeq*>(c.take((a.n + 2) * sizeof(AttnSeq)));
+    p.q_list = static_cast<int2*>(c.take(s.q_entries * sizeof(int2)));
+    if (a.keep) p.k_list = static_cast<int2*>(c.take(s.k_entries * sizeof(int2)));
+    return p;
+}
+
 struct Saved {
+    Plan plan;
     float *lse, *bias_rows;
     Packed q, k, v;
     int64_t bytes;
@@ -80,6 +97,7 @@ Saved saved_of(const slk_attention& a, void* base) {
     const Sizes s = sizes_of(a);
     Carver c{static_cast<char*>(base)};
     Saved r{};
+    r.plan = take_plan(c, a, s);
     r.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     if (a.bias != nullptr)
         r.bias_rows = static_cast<float*>(c.take(a.heads * (2 * a.max_distance + 1) * 4));
@@ -122,25 +140,8 @@ int splits_of(const slk_attention& a, const Sizes& s) {
     return static_cast<int>(std::max<int64_t>(1, std::min({2 * kCus / groups, most, int64_t{kAttnMaxSplits}})));
 }
 
-struct Plan {
-    AttnSeq* seqs;
-    int2 *q_list, *k_list;
-    int32_t* count;
-};
-
-Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s, bool keys) {
-    Plan p{};
-    if (uniform(a)) return p;
-    p.count = static_cast<int32_t*>(c.take(16));
-    p.seqs = static_cast<AttnSeq*>(c.take((a.n + 2) * sizeof(AttnSeq)));
-    p.q_list = static_cast<int2*>(c.take(s.q_entries * sizeof(int2)));
-    if (keys) p.k_list = static_cast<int2*>(c.take(s.k_entries * sizeof(int2)));
-    return p;
-}
-
 struct Forward {
     Saved saved;  // its place, or a part of scratch
-    Plan plan;
     float *part, *part_ml;
     int splits;
     Few few;
@@ -155,7 +156,6 @@ Forward forward_of(const slk_attention& a, void* scratch) {
         f.few = few_of(a);
         f.splits = f.few.splits;
     } else {
-        f.plan = take_plan(c, a, s, false);
         f.splits = splits_of(a, s);
         if (a.keep) {
             f.saved = saved_of(a, a.saved);
@@ -175,7 +175,6 @@ Forward forward_of(const slk_attention& a, void* scratch) {
 }
 
 struct Backward {
-    Plan plan;
     float *delta, *lse;
     int32_t* dexps;
     Packed dout;
@@ -187,7 +186,6 @@ Backward backward_of(const slk_attention& a, void* scratch) {
     const Sizes s = sizes_of(a);
     Carver c{static_cast<char*>(scratch)};
     Backward b{};
-    b.plan = take_plan(c, a, s, true);
     b.delta = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     b.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / kAttnRows) * 4));
@@ -263,7 +261,6 @@ int make_plan(const slk_attention& a, const Plan& p, hipStream_t st) {
     g.q_list = p.q_list;
     g.k_list = p.k_list;
     g.count = p.count;
-    g.tile_q = g.tile_k = kTileRows;
     g.causal = a.causal;
     while ((std::max(a.rows_q, a.rows_k) / kAttnRows) >> g.work_shift >= 1024) ++g.work_shift;
     return attn_launch_plan(g, st);
@@ -381,7 +378,7 @@ int check(const slk_attention* args, const char* who, bool backward) {
 int few_forward(const slk_attention& a, const Forward& f, hipStream_t st) {
     AttnDecode d{};
     d.g = args_of(a, nullptr);
-    d.g.plan = plan_of(a, f.plan, false);
+    d.g.plan = plan_of(a, f.saved.plan, false);
     d.g.splits = f.splits;
     d.g.part = f.part;
     d.g.part_ml = f.part_ml;
@@ -426,11 +423,11 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     if (few_rows(a)) return few_forward(a, f, st);
     const Sizes s = sizes_of(a);
     const bool split = a.dtype == SLK_F32;
-    rc = make_plan(a, f.plan, st);
+    rc = make_plan(a, f.saved.plan, st);
     if (rc != SLK_OK) return rc;
 
     AttnArgs g = args_of(a, f.saved.bias_rows);
-    g.plan = plan_of(a, f.plan, false);
+    g.plan = plan_of(a, f.saved.plan, false);
     AttnPack p{};
     p.plan = g.plan;
     p.dim = g.dim;
@@ -466,10 +463,8 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     const bool split = a.dtype == SLK_F32;
     const Saved sv = saved_of(a, a.saved);
     const Backward b = backward_of(a, a.scratch);
-    rc = make_plan(a, b.plan, st);
-    if (rc != SLK_OK) return rc;
     AttnArgs g = args_of(a, sv.bias_rows);
-    g.plan = plan_of(a, b.plan, false);
+    g.plan = plan_of(a, sv.plan, false);
     if (a.rows_q > 0) {
         AttnPack p{};
         p.plan = g.plan;
@@ -498,7 +493,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     g.dbias_slots = s.pad_q / kAttnRows;
     const bool want_q = a.rows_q > 0 && (a.dq.p != nullptr || a.dbias != nullptr);
     const bool want_kv = a.rows_k > 0 && a.dk.p != nullptr;
-    rc = attn_launch_backward(g, split, blocks_of(a.dim), plan_of(a, b.plan, true), s.q_entries,
+    rc = attn_launch_backward(g, split, blocks_of(a.dim), plan_of(a, sv.plan, true), s.q_entries,
                               s.k_entries, want_q, want_kv, ceil_div(a.rows_k, kTileRows), st);
     if (rc != SLK_OK || a.dbias == nullptr) return rc;
     return attn_launch_dbias(g, a.dbias, st);

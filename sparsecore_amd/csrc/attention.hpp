@@ -32,6 +32,7 @@
 namespace slk {
 
 constexpr int kAttnRows = 64;     // rows of a staged tile, and what packed sequences are padded to
+constexpr int kAttnTileRows = 128; // rows of a workgroup of the tiled kernels
 constexpr int kAttnThreads = 256;
 constexpr int kAttnMaxSplits = 128;  // parts of the keys
 constexpr int kAttnUnit = 14;     // a packed tile's largest element is in 2^[14, 15)
@@ -196,15 +197,18 @@ struct AttnReads {
         to_across = ar * T::kRowBytes +
                     16 * ((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ T::swz(ar)) + 8 * (i & 1);
     }
+    // PLANE: bytes between the parts, those of a tile or of a stage of fewer rows
+    template <int PLANE = T::kPlane>
     __device__ __forceinline__ AttnPair<SPLIT> along(const unsigned char* buf, int b,
                                                      int ks) const {
         AttnPair<SPLIT> r;
 #pragma unroll
         for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
-            r.f[p] = *reinterpret_cast<const f16x8*>(buf + (to_along ^ (32 * ks)) + p * T::kPlane +
+            r.f[p] = *reinterpret_cast<const f16x8*>(buf + (to_along ^ (32 * ks)) + p * PLANE +
                                                      32 * b * T::kRowBytes);
         return r;
     }
+    template <int PLANE = T::kPlane>
     __device__ __forceinline__ AttnPair<SPLIT> across(const unsigned char* buf, int b, int s,
                                                       int fb) const {
         AttnPair<SPLIT> r;
@@ -213,7 +217,7 @@ struct AttnReads {
             i16x4 x[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                x[u] = read_turned(buf + (to_across ^ (64 * fb) ^ (32 * u)) + p * T::kPlane +
+                x[u] = read_turned(buf + (to_across ^ (64 * fb) ^ (32 * u)) + p * PLANE +
                                    (32 * b + 16 * s + 8 * u) * T::kRowBytes);
             r.f[p] = __builtin_bit_cast(
                 f16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -246,7 +250,7 @@ __device__ __forceinline__ AttnPair<SPLIT> attn_operand(const float* x) {
 
 // acc[fb] += X^T·W over one block of 32 staged rows X, W a lane's 16 results (zero
 // where the pair is masked) as operands.
-template <bool SPLIT, int DB>
+template <bool SPLIT, int DB, int PLANE = AttnTile<DB>::kPlane>
 __device__ __forceinline__ void attn_accumulate(const AttnReads<SPLIT, DB>& rd,
                                                 const unsigned char* buf, int b,
                                                 const AttnPair<SPLIT> (&w)[2],
@@ -255,7 +259,7 @@ __device__ __forceinline__ void attn_accumulate(const AttnReads<SPLIT, DB>& rd,
     for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int fb = 0; fb < DB; ++fb)
-            acc[fb] = attn_dot<SPLIT>(rd.across(buf, b, s, fb), w[s], acc[fb]);
+            acc[fb] = attn_dot<SPLIT>(rd.template across<PLANE>(buf, b, s, fb), w[s], acc[fb]);
 }
 
 // Row (in a block of 32) that register r of a result belongs to.
@@ -268,9 +272,26 @@ __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_ex
 // 2^e for any e; 0 below the smallest.
 __device__ __forceinline__ float attn_pow2(int e) { return ldexpf(1.0f, e); }
 
+// A value at an address that is the same for the whole wave, by a scalar load: a
+// vector load's wait would be for the tiles on their way into LDS before it too
+// (vector loads return in order), and undo their reading ahead. Of memory that the
+// kernel does not write.
+template <class V>
+__device__ __forceinline__ V attn_scalar(const V* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+    return *reinterpret_cast<const __attribute__((address_space(4))) V*>(
+        static_cast<uint64_t>(hi) << 32 | lo);
+#else
+    return *p;
+#endif
+}
+
 // Exponent of a tile of an operand.
 __device__ __forceinline__ int attn_exp(const AttnOp& op, int head, int64_t padded_row) {
-    return __builtin_amdgcn_readfirstlane(op.exps[head * op.exps_sh + (padded_row >> 6)]) >> 1;
+    return attn_scalar(op.exps + head * op.exps_sh + (padded_row >> 6)) >> 1;
 }
 
 // The bias of a distance (query - key) of one head, times log2 e. Buckets are

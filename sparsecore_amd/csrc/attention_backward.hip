@@ -16,6 +16,16 @@ __device__ __forceinline__ int ds_exponent(int oe, int ve, int de, int log_dp) {
     return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -100), 100);
 }
 
+// The diagonals of a block of 32 queries x 8 keys: a row of LDS each, eight keys
+// wide and four more floats, so that 16-byte reads of 16 rows meet all banks.
+constexpr int kDiags = 39, kDiagRow = 12;
+
+// Between LDS writes and reads of one wave's lanes: they execute in order.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ int wave_max(int e) {
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) e = max(e, __shfl_xor(e, x));
@@ -37,19 +47,26 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 #endif
 }
 
-// dK, dV: a workgroup takes 128 keys of one key head, a wave 32 of them, whose
-// rows of K and V stay in registers. Q and dO come through LDS, 64 rows at a
-// time, for every query head of the group in turn. Scores are Q·K^T here: a lane
-// holds 16 queries of one key, as the operands of dV^T = dO^T·P and
-// dK^T = Q^T·dS need them.
+// dK, dV: a workgroup takes 128 keys of one key head, a wave 32 of them. Its rows
+// of K stay in registers, those of V too up to 64 features; at 128 they are read
+// from LDS (in registers they spilled, and a reload waits for the loads ahead).
+// Q and dO come through LDS, two buffers of 64 rows (32 at 128 features, which
+// leaves room for two workgroups a CU), for every query head of the group in
+// turn. Scores are Q·K^T here: a lane holds 16 queries of one key, as the operands
+// of dV^T = dO^T·P and dK^T = Q^T·dS need them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dkv_kernel(const AttnArgs g) {
     using T = AttnTile<DB>;
-    constexpr int kBytes = (SPLIT ? 2 : 1) * T::kPlane, KS = 2 * DB;
+    constexpr int kPlanes = SPLIT ? 2 : 1, kTile = kPlanes * T::kPlane, KS = 2 * DB;
     constexpr int kLogDp = DB == 1 ? 5 : DB == 2 ? 6 : 7;
+    constexpr bool kVInLds = DB == 4;
+    constexpr int kRows = kVInLds ? 32 : 64;             // queries of a stage
+    constexpr int kPart = kRows * T::kRowBytes;          // bytes of a plane of them
+    constexpr int kBytes = kPlanes * kPart;
     __shared__ __align__(16) unsigned char ring0[2 * kBytes + 512];
     __shared__ __align__(16) unsigned char ring1[2 * kBytes + 512];
+    __shared__ __align__(16) unsigned char values[kVInLds ? 2 * kTile : 16];
     extern __shared__ float bias_row[];
 
     const int t = threadIdx.x, lane = t & 63;
@@ -69,30 +86,40 @@ attn_dkv_kernel(const AttnArgs g) {
         for (int r = 0; r < 16; ++r) dk[fb][r] = dv[fb][r] = 0.0f;
     int co = 0, cq = 0;
 
-    // tiles of 64 queries, from the first that sees a key of the workgroup
-    const int first = g.causal ? max(0, tile * 128 - shift) / kAttnRows : 0;
-    const int n_q = (seq.nq + kAttnRows - 1) / kAttnRows;
+    // stages of queries, from the first that sees a key of the workgroup
+    const int first = g.causal ? max(0, tile * 128 - shift) / kRows : 0;
+    const int n_q = (seq.nq + kRows - 1) / kRows;
     const int nt = tile * 128 < seq.nk && first < n_q ? n_q - first : 0;
 
     if (nt > 0) {
-        const int64_t q0_tile = seq.pq / 64 + first;
+        const int64_t q_tile0 = seq.pq / 64;
         auto issue = [&](unsigned char* to, int hr, int qt) __attribute__((always_inline)) {
-            const int head = kvh * rep + hr;
-            const int64_t at = (q0_tile + qt) * kBytes;
-            attn_stage<kBytes>(g.q.p + head * g.q.sh + at, to, wv, lane);
-            attn_stage<kBytes>(g.dout.p + head * g.dout.sh + at, to + kBytes, wv, lane);
-            const int64_t row = head * g.lse_sh + (q0_tile + qt) * 64;
-            if (wv == 0) load_row(g.lse + row, to + 2 * kBytes, lane);
-            if (wv == 1) load_row(g.delta + row, to + 2 * kBytes + 256, lane);
+            const int head = kvh * rep + hr, row = (first + qt) * kRows;
+            const int64_t tq = q_tile0 + row / 64;
+            const int64_t at = tq * kTile + (row & 63) * T::kRowBytes;
+#pragma unroll
+            for (int p = 0; p < kPlanes; ++p) {
+                attn_stage<kPart>(g.q.p + head * g.q.sh + at + p * T::kPlane, to + p * kPart, wv,
+                                  lane);
+                attn_stage<kPart>(g.dout.p + head * g.dout.sh + at + p * T::kPlane,
+                                  to + kBytes + p * kPart, wv, lane);
+            }
+            // the whole tile's 64 rows each, of which a stage of 32 uses its half
+            if (wv == 0) load_row(g.lse + head * g.lse_sh + tq * 64, to + 2 * kBytes, lane);
+            if (wv == 1) load_row(g.delta + head * g.lse_sh + tq * 64, to + 2 * kBytes + 256, lane);
         };
         issue(ring0, 0, 0);
         const AttnReads<SPLIT, DB> rd(lane);
+        // a tile of 64 rows, and a stage's
+        auto row_of = [&](const unsigned char* buf, int b, int ks) __attribute__((always_inline)) {
+            return rd.template along<kPart>(buf, b, ks);
+        };
 
         const bool live = key0 < seq.nk;
         const int k_row = seq.pk + (live ? key0 : 0);
-        AttnPair<SPLIT> kf[KS], vf[KS];
+        AttnPair<SPLIT> kf[KS], vf[kVInLds ? 1 : KS];
         {
-            const int64_t at = static_cast<int64_t>(k_row / 64) * kBytes;
+            const int64_t at = static_cast<int64_t>(k_row / 64) * kTile;
             const unsigned char* ka =
                 reinterpret_cast<const unsigned char*>(g.k.p + kvh * g.k.sh + at);
             const unsigned char* va =
@@ -100,18 +127,26 @@ attn_dkv_kernel(const AttnArgs g) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 kf[ks] = rd.along(ka, (k_row >> 5) & 1, ks);
-                vf[ks] = rd.along(va, (k_row >> 5) & 1, ks);
+                if constexpr (!kVInLds) vf[ks] = rd.along(va, (k_row >> 5) & 1, ks);
+            }
+            if constexpr (kVInLds) {
+                // the second of the workgroup's two tiles is there if a key of it is
+                const char* from = g.v.p + kvh * g.v.sh + (seq.pk / 64 + 2 * tile) * int64_t{kTile};
+                attn_stage<kTile>(from, values, wv, lane);
+                if (tile * 128 + 64 < seq.nk)
+                    attn_stage<kTile>(from + kTile, values + kTile, wv, lane);
             }
         }
+        const unsigned char* const mine = values + (wv >> 1) * kTile;
         // dV in units of 2^(co - 28), dK of 2^(cq - 28), the largest of the query
         // tiles that this wave's keys are seen by
         const int ke = attn_exp(g.k, kvh, k_row), ve = attn_exp(g.v, kvh, k_row);
         co = cq = -400;
         {
-            const int b0 = g.causal ? max(0, key0 - shift) / 64 : 0;
+            const int b0 = g.causal ? max(0, key0 - shift) / 64 : 0, b1 = (seq.nq + 63) / 64;
             for (int hr = 0; hr < rep; ++hr) {
-                const int64_t at = (kvh * rep + hr) * g.q.exps_sh + seq.pq / 64;
-                for (int i = b0 + lane; i < n_q; i += 64) {
+                const int64_t at = (kvh * rep + hr) * g.q.exps_sh + q_tile0;
+                for (int i = b0 + lane; i < b1; i += 64) {
                     const int oe = g.dout.exps[at + i] >> 1;
                     co = max(co, oe);
                     cq = max(cq, ds_exponent(oe, ve, g.dexps[at + i], kLogDp) +
@@ -123,12 +158,11 @@ attn_dkv_kernel(const AttnArgs g) {
         }
         const int md = BIAS ? g.bias.max_distance : 0;
 
-        auto compute = [&](const unsigned char* buf, int hr, int q_tile)
+        auto compute = [&](const unsigned char* buf, int hr, int q_first)
             __attribute__((always_inline)) {
-            const int head = kvh * rep + hr, row0 = seq.pq + q_tile;
+            const int head = kvh * rep + hr, row0 = seq.pq + q_first;
             const int qe = attn_exp(g.q, head, row0), oe = attn_exp(g.dout, head, row0);
-            const int de = __builtin_amdgcn_readfirstlane(
-                g.dexps[head * g.q.exps_sh + (row0 >> 6)]);
+            const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (row0 >> 6));
             const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
             // weights times 2^u; dS = weight · (alpha·dp - beta·delta)
             const int u = kAttnUnit + max(oe - co, -60);
@@ -137,8 +171,8 @@ attn_dkv_kernel(const AttnArgs g) {
             const float unit = static_cast<float>(u);
             const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit), beta = attn_pow2(x);
 #pragma unroll
-            for (int qb = 0; qb < 2; ++qb) {
-                const int q0 = q_tile + 32 * qb;
+            for (int qb = 0; qb < kRows / 32; ++qb) {
+                const int q0 = q_first + 32 * qb;
                 if (q0 >= seq.nq || (g.causal && q0 + 31 + shift < key0)) continue;
                 const bool masked = q0 + 31 >= seq.nq || (g.causal && q0 + shift < key0 + 31);
                 f32x16 s, dp;
@@ -146,10 +180,14 @@ attn_dkv_kernel(const AttnArgs g) {
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    s = attn_dot<SPLIT>(rd.along(buf, qb, ks), kf[ks], s);
-                    dp = attn_dot<SPLIT>(rd.along(buf + kBytes, qb, ks), vf[ks], dp);
+                    s = attn_dot<SPLIT>(row_of(buf, qb, ks), kf[ks], s);
+                    if constexpr (kVInLds)
+                        dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks),
+                                             rd.along(mine, wv & 1, ks), dp);
+                    else dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks), vf[ks], dp);
                 }
-                const float* lse = reinterpret_cast<const float*>(buf + 2 * kBytes) + 32 * qb;
+                const float* lse =
+                    reinterpret_cast<const float*>(buf + 2 * kBytes) + (q0 & 63);
                 const float* delta = lse + 64;
                 float p[16], ds[16];
 #pragma unroll
@@ -167,9 +205,9 @@ attn_dkv_kernel(const AttnArgs g) {
                         ds[r] = p[r] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
                     }
                 }
-                // the lane's key is seen by rows [lo, hi) of the block
-                const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
                 if (masked) {
+                    // the lane's key is seen by rows [lo, hi) of the block
+                    const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int row = attn_row(r, lane);
@@ -178,10 +216,11 @@ attn_dkv_kernel(const AttnArgs g) {
                         ds[r] = see ? ds[r] : 0.0f;
                     }
                 }
-                AttnPair<SPLIT> wp[2] = {attn_operand<SPLIT>(p), attn_operand<SPLIT>(p + 8)};
-                AttnPair<SPLIT> wd[2] = {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)};
-                attn_accumulate<SPLIT, DB>(rd, buf + kBytes, qb, wp, dv);
-                attn_accumulate<SPLIT, DB>(rd, buf, qb, wd, dk);
+                const AttnPair<SPLIT> wp[2] = {attn_operand<SPLIT>(p), attn_operand<SPLIT>(p + 8)};
+                const AttnPair<SPLIT> wd[2] = {attn_operand<SPLIT>(ds),
+                                               attn_operand<SPLIT>(ds + 8)};
+                attn_accumulate<SPLIT, DB, kPart>(rd, buf + kBytes, qb, wp, dv);
+                attn_accumulate<SPLIT, DB, kPart>(rd, buf, qb, wd, dk);
             }
         };
         int hr = 0, qt = 0;
@@ -195,11 +234,11 @@ attn_dkv_kernel(const AttnArgs g) {
             __builtin_amdgcn_s_waitcnt(wait_vm(0));
             asm volatile("s_barrier" ::: "memory");
             if (hr < rep) issue(next, hr, qt);
-            if (BIAS && i == 0) {  // a head's first tile
+            if (BIAS && i == 0) {  // a head's first stage
                 attn_bias_row(g.bias, kvh * rep + h, bias_row);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
-            if (live) compute(cur, h, (first + i) * kAttnRows);
+            if (live) compute(cur, h, (first + i) * kRows);
         };
         int left = rep * nt;
         for (; left >= 2; left -= 2) {
@@ -233,9 +272,11 @@ attn_dkv_kernel(const AttnArgs g) {
 }
 
 // dQ: a workgroup takes 128 queries of one head, a wave 32 of them, whose rows of
-// Q and dO stay in registers; K and V come through LDS. The bias's gradient: each
-// wave half adds a lane's dS to bins of its own, one a distance (for one register
-// the 32 lanes' distances differ), so the sums need no atomicity and repeat.
+// Q and dO stay in registers; K and V come through LDS. The bias's gradient: a wave
+// lays eight keys' dS out by diagonals in LDS, sums each in one lane and adds it to
+// the wave's own bin of that distance, so the sums need no atomicity and repeat.
+// (Float atomics on LDS took some 260 cycles an instruction: the whole kernel 137
+// against @@ us at 16 x 512 tokens, 12 heads of 64, float32.)
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dq_kernel(const AttnArgs g) {
@@ -244,7 +285,7 @@ attn_dq_kernel(const AttnArgs g) {
     constexpr int kLogDp = DB == 1 ? 5 : DB == 2 ? 6 : 7;
     __shared__ __align__(16) unsigned char ring0[2 * kBytes];
     __shared__ __align__(16) unsigned char ring1[2 * kBytes];
-    extern __shared__ float bias_row[];
+    extern __shared__ __align__(16) float lds_floats[];
 
     const int t = threadIdx.x, lane = t & 63;
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -262,12 +303,16 @@ attn_dq_kernel(const AttnArgs g) {
     const int t1 = seen <= 0 ? 0 : (seen + kAttnRows - 1) / kAttnRows;
 
     const int md = BIAS ? g.bias.max_distance : 0, width = 2 * md + 1;
-    float* const bins = bias_row + width;        // [wave][half][distance]
-    float* const far = bins + 8 * width;         // [wave][below, above]
+    float* const diag = lds_floats + (threadIdx.x >> 6) * kDiags * kDiagRow;
+    float* const far = lds_floats + 4 * kDiags * kDiagRow;  // [wave][below, above]
+    float* const bias_row = far + 8;
+    float* const bins = bias_row + width;        // [wave][distance]
+    const int d_row = min(lane, kDiags - 1);
     float below = 0.0f, above = 0.0f;            // distances past the last bins
     if constexpr (BIAS) {
         attn_bias_row(g.bias, head, bias_row);
-        for (int i = t; i < 8 * width; i += kAttnThreads) bins[i] = 0.0f;
+        for (int i = t; i < 4 * width; i += kAttnThreads) bins[i] = 0.0f;
+        for (int i = lane; i < kDiags * kDiagRow; i += 64) diag[i] = 0.0f;
     }
 
     f32x16 dq[DB];
@@ -306,8 +351,7 @@ attn_dq_kernel(const AttnArgs g) {
         const float lse = mine ? g.lse[ri] : INFINITY;
         const float delta = mine ? g.delta[ri] : 0.0f;
         const int qe = attn_exp(g.q, head, q_row), oe = attn_exp(g.dout, head, q_row);
-        const int de =
-            __builtin_amdgcn_readfirstlane(g.dexps[head * g.q.exps_sh + (q_row >> 6)]);
+        const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (q_row >> 6));
         {
             const int* ve = g.v.exps + kvh * g.v.exps_sh + k_tile;
             const int* ke = g.k.exps + kvh * g.k.exps_sh + k_tile;
@@ -367,22 +411,33 @@ attn_dq_kernel(const AttnArgs g) {
                 if constexpr (BIAS) {
                     const float back = attn_pow2(-x);
                     if (near) {
-                        float* const mine_bins = bins + (2 * wv + (lane >> 5)) * width + md;
+                        // eight keys at a time: lane d sums the diagonal of distance
+                        // d - 7 from the first key's of the first query
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int d = away - attn_row(r, lane);
-                            const float y = mine ? ds[r] * back : 0.0f;
+                        for (int r4 = 0; r4 < 4; ++r4) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int k = 4 * (lane >> 5) + j;
+                                diag[((lane & 31) - k + 7) * kDiagRow + k] = ds[4 * r4 + j];
+                            }
+                            wave_lds_fence();
+                            const f32x4* const at =
+                                reinterpret_cast<const f32x4*>(diag + d_row * kDiagRow);
+                            const f32x4 lo = at[0], hi = at[1];
+                            float y = ((lo[0] + lo[1]) + (lo[2] + lo[3])) +
+                                      ((hi[0] + hi[1]) + (hi[2] + hi[3]));
+                            y = lane < kDiags ? y * back : 0.0f;
+                            const int d = wave0 + shift - key0 - 8 * r4 + d_row - 7;
                             if (d >= md) above += y;
                             else if (d <= -md) below += y;
-                            else
-                                __hip_atomic_fetch_add(mine_bins + d, y, __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+                            else if (lane < kDiags) bins[wv * width + md + d] += y;
+                            wave_lds_fence();
                         }
                     } else {
                         float y = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) y += ds[r];
-                        y = mine ? y * back : 0.0f;
+                        y *= back;
                         if (away >= md) above += y;
                         else below += y;
                     }
@@ -438,7 +493,7 @@ attn_dq_kernel(const AttnArgs g) {
         float* const out = g.dbias_part + (head * g.dbias_slots + slot) * static_cast<int64_t>(width);
         for (int i = t; i < width; i += kAttnThreads) {
             float y = 0.0f;
-            for (int j = 0; j < 8; ++j) y += bins[j * width + i];
+            for (int j = 0; j < 4; ++j) y += bins[j * width + i];
             for (int j = 0; j < 4; ++j) y += i == 0 ? far[2 * j] : i == 2 * md ? far[2 * j + 1] : 0.0f;
             out[i] = y;
             if (slots > 1) out[width + i] = 0.0f;
@@ -447,25 +502,33 @@ attn_dq_kernel(const AttnArgs g) {
 }
 
 // The bias's gradient from the workgroups' bins, in their order: a workgroup a
-// head, a thread a distance, then a thread a bucket.
+// head, four threads a distance (a quarter of the bins each), then a thread a
+// bucket.
 __global__ __launch_bounds__(1024) void attn_dbias_kernel(const AttnArgs g, void* dbias) {
-    __shared__ float per[2 * SLK_ATTN_MAX_DISTANCE + 1];
+    constexpr int kMost = 2 * SLK_ATTN_MAX_DISTANCE + 1;
+    __shared__ float quarter[4][kMost];
+    __shared__ float per[kMost];
     const int head = blockIdx.x, md = g.bias.max_distance, width = 2 * md + 1;
     const int64_t rows = g.plan.seqs != nullptr ? g.plan.count[1] : g.plan.batch * g.plan.pad_t;
     const int64_t slots = rows / kAttnRows;
     const float* from = g.dbias_part + head * g.dbias_slots * width;
-    for (int i = threadIdx.x; i < width; i += blockDim.x) {
+    const int part = threadIdx.x >> 8;
+    const int64_t s0 = slots * part / 4, s1 = slots * (part + 1) / 4;
+    for (int i = threadIdx.x & 255; i < width; i += 256) {
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-        int64_t s = 0;
-        for (; s + 8 <= slots; s += 8) {
+        int64_t s = s0;
+        for (; s + 8 <= s1; s += 8) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] += from[(s + j) * width + i];
         }
-        for (; s < slots; ++s) y[0] += from[s * width + i];
-        per[i] = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        for (; s < s1; ++s) y[0] += from[s * width + i];
+        quarter[part][i] = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 1024)
+        per[i] = (quarter[0][i] + quarter[1][i]) + (quarter[2][i] + quarter[3][i]);
     __syncthreads();
     const int one = g.bias.one_sided ? g.bias.buckets : g.bias.buckets / 2;
     for (int b = threadIdx.x; b < g.bias.buckets; b += blockDim.x) {
@@ -500,7 +563,7 @@ int launch(const AttnArgs& g, const AttnPlan& kplan, int64_t q_entries, int64_t 
     if (want_q) {
         hipLaunchKernelGGL((attn_dq_kernel<SPLIT, DB, BIAS>),
                            dim3(static_cast<unsigned>(q_entries * g.heads)), dim3(kAttnThreads),
-                           (9 * width + (BIAS ? 8 : 0)) * sizeof(float), st, g);
+                           BIAS ? (5 * width + 8 + 4 * kDiags * kDiagRow) * sizeof(float) : 0, st, g);
         return check_launch("attention_backward: dq");
     }
     return SLK_OK;

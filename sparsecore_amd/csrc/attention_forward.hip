@@ -100,8 +100,7 @@ attn_forward_kernel(const AttnArgs g) {
                 for (int kb = 0; kb < 2; ++kb)
                     s[kb] = attn_dot<SPLIT>(rd.along(buf, kb, ks), qf[ks], s[kb]);
             const int64_t et = kvh * g.k.exps_sh + tiles0 + kt;
-            const int ve = __builtin_amdgcn_readfirstlane(g.v.exps[et]);
-            const int ke = __builtin_amdgcn_readfirstlane(g.k.exps[et]);
+            const int ve = attn_scalar(g.v.exps + et), ke = attn_scalar(g.k.exps + et);
             const int d = max((ve >> 1) - vmax, -60);
             float c = ldexpf(g.scale2, qe + (ke >> 1) - 2 * kAttnUnit);
             // the last key that this query sees, from the tile's first
@@ -164,7 +163,7 @@ attn_forward_kernel(const AttnArgs g) {
             }
             l = __builtin_fmaf(sum, attn_pow2(-d), l);
             if (__builtin_expect((ve | ke) & 1, 0)) {  // rows that are not finite
-                const uint64_t bad = g.v.bad[et] | g.k.bad[et];
+                const uint64_t bad = attn_scalar(g.v.bad + et) | attn_scalar(g.k.bad + et);
                 const uint64_t sees = lim >= 63 ? ~uint64_t{0}
                                       : lim >= 0 ? (uint64_t{2} << lim) - 1
                                                  : 0;

@@ -10,6 +10,8 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kBins = 1024;  // classes of work in the tile order
+static_assert(kBins == kPlanThreads, "a thread a class");
+constexpr int kTileRows = kAttnTileRows;
 
 // Inclusive scan over the workgroup, by sum or maximum, and its last value.
 template <bool MAX>
@@ -110,34 +112,34 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
     __threadfence_block();
     __syncthreads();
     // tiles by falling work, counted in classes of blocks of 64 on the other side
-    const int64_t total = a.n + (packed ? 2 : 0);
+    const int total = static_cast<int>(a.n) + (packed ? 2 : 0);
+    const bool one_each = total <= kPlanThreads;  // a thread keeps its sequence
+    const AttnSeq own = one_each && t < total ? a.seqs[t] : AttnSeq{};
     for (int side = 0; side < 2; ++side) {
         int2* list = side ? a.k_list : a.q_list;
         if (list == nullptr) continue;
-        const int rows = side ? a.tile_k : a.tile_q;
         auto each = [&](auto&& f) {
-            for (int64_t s = t; s < total; s += kPlanThreads) {
-                const AttnSeq x = a.seqs[s];
+            for (int s = t; s < total; s += kPlanThreads) {
+                const AttnSeq x = one_each ? own : a.seqs[s];
                 const int shift = x.nk - x.nq;
-                const int tiles = static_cast<int>(ceil_div(side ? x.ek : x.eq, rows));
+                const int tiles = ((side ? x.ek : x.eq) + kTileRows - 1) / kTileRows;
                 for (int i = 0; i < tiles; ++i) {
-                    int64_t w;
+                    int w;
                     if (side) {
-                        w = x.nk <= i * rows ? 0
-                            : a.causal       ? x.nq - max(0, i * rows - shift)
-                                             : x.nq;
+                        w = x.nk <= i * kTileRows ? 0
+                            : a.causal            ? x.nq - max(0, i * kTileRows - shift)
+                                                  : x.nq;
                     } else {
-                        w = x.nq <= i * rows ? 0
-                            : a.causal       ? min(x.nk, min((i + 1) * rows, x.nq) + shift)
-                                             : x.nk;
+                        w = x.nq <= i * kTileRows ? 0
+                            : a.causal ? min(x.nk, min((i + 1) * kTileRows, x.nq) + shift)
+                                       : x.nk;
                     }
-                    w = ceil_div(w < 0 ? 0 : w, kAttnRows) >> a.work_shift;
-                    f(static_cast<int>(kBins - 1 - (w < kBins ? w : kBins - 1)),
-                      static_cast<int>(s), i);
+                    w = ((max(w, 0) + kAttnRows - 1) / kAttnRows) >> a.work_shift;
+                    f(kBins - 1 - min(w, kBins - 1), s, i);
                 }
             }
         };
-        for (int i = t; i < kBins; i += kPlanThreads) bin[i] = 0;
+        bin[t] = 0;
         __syncthreads();
         each([&](int b, int, int) { atomicAdd(&bin[b], 1); });
         __syncthreads();
@@ -147,9 +149,7 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         bin[t] = static_cast<int32_t>(upto - mine);
         __syncthreads();
         // the order inside a class does not change a result: tiles are independent
-        each([&](int b, int s, int i) {
-            list[atomicAdd(&bin[b], 1)] = int2{s, i};
-        });
+        each([&](int b, int s, int i) { list[atomicAdd(&bin[b], 1)] = int2{s, i}; });
         if (t == 0) a.count[2 * side] = static_cast<int32_t>(all);
         __syncthreads();
     }

@@ -12,7 +12,7 @@ struct AttnPlanArgs {
     AttnSeq* seqs;                         // n (+ 2 if packed)
     int2 *q_list, *k_list;                 // NULL: not wanted
     int32_t* count;  // tiles of queries, their padded rows, tiles of keys, padded rows
-    int32_t tile_q, tile_k, causal, work_shift;
+    int32_t causal, work_shift;
 };
 
 // How a pack reads four elements at once: not, four features, four rows.
