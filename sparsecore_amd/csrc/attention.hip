@@ -174,7 +174,23 @@ Forward forward_of(const slk_attention& a, void* scratch) {
     return f;
 }
 
+// Parts of a group's query heads in the keys' gradients: where the keys' tiles
+// leave CUs idle, the heads go to workgroups of their own, whose sums are joined.
+// 8191 packed tokens, 16 heads over 4, 128 wide, bf16: 351 us in one part, 193 + 26
+// for the join in two, 112 + 46 in four.
+int dkv_parts(const slk_attention& a, const Sizes& s) {
+    const int64_t rep = a.heads / a.kv_heads, groups = s.k_entries * a.kv_heads;
+    int64_t parts = 1;
+    while (parts < rep && groups * parts < 4 * kCus) {
+        do ++parts;
+        while (rep % parts != 0);
+    }
+    return static_cast<int>(parts);
+}
+
 struct Backward {
+    int parts;
+    float* dkv_part;
     float *delta, *lse;
     int32_t* dexps;
     Packed dout;
@@ -190,6 +206,10 @@ Backward backward_of(const slk_attention& a, void* scratch) {
     b.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / kAttnRows) * 4));
     b.dout = take_packed(c, s, a.heads, s.pad_q);
+    b.parts = dkv_parts(a, s);
+    if (b.parts > 1)
+        b.dkv_part = static_cast<float*>(
+            c.take(int64_t{b.parts} * 2 * a.kv_heads * s.pad_k * 32 * blocks_of(a.dim) * 4));
     if (a.dbias != nullptr)
         b.dbias_part = static_cast<float*>(
             c.take(a.heads * (s.pad_q / kAttnRows) * (2 * a.max_distance + 1) * 4));
@@ -490,6 +510,9 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     g.delta = b.delta;
     g.dexps = b.dexps;
     g.dbias_part = b.dbias_part;
+    g.dkv_part = b.dkv_part;
+    g.dkv_rows = s.pad_k;
+    g.dkv_parts = b.parts;
     g.dbias_slots = s.pad_q / kAttnRows;
     const bool want_q = a.rows_q > 0 && (a.dq.p != nullptr || a.dbias != nullptr);
     const bool want_kv = a.rows_k > 0 && a.dk.p != nullptr;

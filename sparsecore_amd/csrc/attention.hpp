@@ -117,6 +117,9 @@ struct AttnArgs {
     AttnBias bias;
     float* dbias_part;     // [head][padded rows / 64][2·max_distance + 1]
     int64_t dbias_slots;
+    float* dkv_part;       // heads of a group in parts: [part][dk, dv][key head][padded row][DP]
+    int64_t dkv_rows;      // padded rows of keys
+    int32_t dkv_parts;
     float* part;           // split keys: [split][head][padded row][DP] of O, then of m, l
     float* part_ml;
     int64_t part_rows;
@@ -160,7 +163,7 @@ __device__ __forceinline__ f32x16 attn_dot(const AttnPair<SPLIT>& a, const AttnP
     return attn_mfma(a.f[0], b.f[0], c);
 }
 
-// Copies a tile (planes of it) into LDS: wave wv takes pieces of 1 KB wv, wv + 4, ...
+// Copies bytes of a tile into LDS in pieces of 1 KB, wave by wave.
 template <int BYTES>
 __device__ __forceinline__ void attn_stage(const char* from, unsigned char* to, int wv,
                                            int lane) {

@@ -52,8 +52,9 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 // from LDS (in registers they spilled, and a reload waits for the loads ahead).
 // Q and dO come through LDS, two buffers of 64 rows (32 at 128 features, which
 // leaves room for two workgroups a CU), for every query head of the group in
-// turn. Scores are Q·K^T here: a lane holds 16 queries of one key, as the operands
-// of dV^T = dO^T·P and dK^T = Q^T·dS need them.
+// turn, or for some of them where a group is spread over workgroups. Scores are
+// Q·K^T here: a lane holds 16 queries of one key, as the operands of
+// dV^T = dO^T·P and dK^T = Q^T·dS need them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dkv_kernel(const AttnArgs g) {
@@ -67,14 +68,20 @@ attn_dkv_kernel(const AttnArgs g) {
     __shared__ __align__(16) unsigned char ring0[2 * kBytes + 512];
     __shared__ __align__(16) unsigned char ring1[2 * kBytes + 512];
     __shared__ __align__(16) unsigned char values[kVInLds ? 2 * kTile : 16];
+    // the last fragments of K, where registers would spill: each lane its own
+    constexpr int kSpare = kVInLds && !SPLIT ? 2 : 0;
+    __shared__ f16x8 spare[kSpare ? 4 * kSpare : 1][64];
     extern __shared__ float bias_row[];
 
     const int t = threadIdx.x, lane = t & 63;
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int rep = g.heads / g.kv_heads;
-    const int kvh = blockIdx.x % g.kv_heads;
+    // the query heads of the group that this part of it takes: rep from head0 on
+    const int rep = g.heads / g.kv_heads / g.dkv_parts;
+    const uint32_t u = blockIdx.x / g.kv_heads;
+    const int kvh = blockIdx.x % g.kv_heads, part = u % g.dkv_parts;
+    const int head0 = (kvh * g.dkv_parts + part) * rep;
     int sid, tile;
-    if (!attn_entry(g.plan, blockIdx.x / g.kv_heads, g.tiles, true, sid, tile)) return;
+    if (!attn_entry(g.plan, u / g.dkv_parts, g.tiles, true, sid, tile)) return;
     const AttnSeq seq = attn_seq(g.plan, sid);
     const int shift = seq.nk - seq.nq;
     const int key0 = tile * 128 + 32 * wv, key = key0 + (lane & 31);
@@ -94,7 +101,7 @@ attn_dkv_kernel(const AttnArgs g) {
     if (nt > 0) {
         const int64_t q_tile0 = seq.pq / 64;
         auto issue = [&](unsigned char* to, int hr, int qt) __attribute__((always_inline)) {
-            const int head = kvh * rep + hr, row = (first + qt) * kRows;
+            const int head = head0 + hr, row = (first + qt) * kRows;
             const int64_t tq = q_tile0 + row / 64;
             const int64_t at = tq * kTile + (row & 63) * T::kRowBytes;
 #pragma unroll
@@ -117,7 +124,7 @@ attn_dkv_kernel(const AttnArgs g) {
 
         const bool live = key0 < seq.nk;
         const int k_row = seq.pk + (live ? key0 : 0);
-        AttnPair<SPLIT> kf[KS], vf[kVInLds ? 1 : KS];
+        AttnPair<SPLIT> kf[KS - kSpare], vf[kVInLds ? 1 : KS];
         {
             const int64_t at = static_cast<int64_t>(k_row / 64) * kTile;
             const unsigned char* ka =
@@ -126,7 +133,9 @@ attn_dkv_kernel(const AttnArgs g) {
                 reinterpret_cast<const unsigned char*>(g.v.p + kvh * g.v.sh + at);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                kf[ks] = rd.along(ka, (k_row >> 5) & 1, ks);
+                const AttnPair<SPLIT> x = rd.along(ka, (k_row >> 5) & 1, ks);
+                if (ks < KS - kSpare) kf[ks < KS - kSpare ? ks : 0] = x;
+                else spare[kSpare * wv + ks - (KS - kSpare)][lane] = x.f[0];
                 if constexpr (!kVInLds) vf[ks] = rd.along(va, (k_row >> 5) & 1, ks);
             }
             if constexpr (kVInLds) {
@@ -137,7 +146,7 @@ attn_dkv_kernel(const AttnArgs g) {
                     attn_stage<kTile>(from + kTile, values + kTile, wv, lane);
             }
         }
-        const unsigned char* const mine = values + (wv >> 1) * kTile;
+        const unsigned char* const my_v = values + (wv >> 1) * kTile;
         // dV in units of 2^(co - 28), dK of 2^(cq - 28), the largest of the query
         // tiles that this wave's keys are seen by
         const int ke = attn_exp(g.k, kvh, k_row), ve = attn_exp(g.v, kvh, k_row);
@@ -145,7 +154,7 @@ attn_dkv_kernel(const AttnArgs g) {
         {
             const int b0 = g.causal ? max(0, key0 - shift) / 64 : 0, b1 = (seq.nq + 63) / 64;
             for (int hr = 0; hr < rep; ++hr) {
-                const int64_t at = (kvh * rep + hr) * g.q.exps_sh + q_tile0;
+                const int64_t at = (head0 + hr) * g.q.exps_sh + q_tile0;
                 for (int i = b0 + lane; i < b1; i += 64) {
                     const int oe = g.dout.exps[at + i] >> 1;
                     co = max(co, oe);
@@ -160,7 +169,7 @@ attn_dkv_kernel(const AttnArgs g) {
 
         auto compute = [&](const unsigned char* buf, int hr, int q_first)
             __attribute__((always_inline)) {
-            const int head = kvh * rep + hr, row0 = seq.pq + q_first;
+            const int head = head0 + hr, row0 = seq.pq + q_first;
             const int qe = attn_exp(g.q, head, row0), oe = attn_exp(g.dout, head, row0);
             const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (row0 >> 6));
             const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
@@ -180,11 +189,13 @@ attn_dkv_kernel(const AttnArgs g) {
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    s = attn_dot<SPLIT>(row_of(buf, qb, ks), kf[ks], s);
-                    if constexpr (kVInLds)
-                        dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks),
-                                             rd.along(mine, wv & 1, ks), dp);
-                    else dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks), vf[ks], dp);
+                    AttnPair<SPLIT> k = kf[ks < KS - kSpare ? ks : 0];
+                    if (ks >= KS - kSpare) k.f[0] = spare[kSpare * wv + ks - (KS - kSpare)][lane];
+                    s = attn_dot<SPLIT>(row_of(buf, qb, ks), k, s);
+                    dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks),
+                                         kVInLds ? rd.along(my_v, wv & 1, ks)
+                                                 : vf[kVInLds ? 0 : ks],
+                                         dp);
                 }
                 const float* lse =
                     reinterpret_cast<const float*>(buf + 2 * kBytes) + (q0 & 63);
@@ -235,7 +246,7 @@ attn_dkv_kernel(const AttnArgs g) {
             asm volatile("s_barrier" ::: "memory");
             if (hr < rep) issue(next, hr, qt);
             if (BIAS && i == 0) {  // a head's first stage
-                attn_bias_row(g.bias, kvh * rep + h, bias_row);
+                attn_bias_row(g.bias, head0 + h, bias_row);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (live) compute(cur, h, (first + i) * kRows);
@@ -251,6 +262,27 @@ attn_dkv_kernel(const AttnArgs g) {
     if (key >= seq.ek) return;
     const float fk = ldexpf(g.scale, cq - 2 * kAttnUnit), fv = attn_pow2(co - 2 * kAttnUnit);
     const bool zero = key >= seq.nk || nt == 0;
+    if (g.dkv_parts > 1 && key < seq.nk) {
+        const int64_t row = static_cast<int64_t>(kvh) * g.dkv_rows + seq.pk + key;
+        const int64_t step = static_cast<int64_t>(g.kv_heads) * g.dkv_rows;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float* const at = g.dkv_part + ((2 * part + which) * step + row) * T::DP;
+#pragma unroll
+            for (int fb = 0; fb < DB; ++fb)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    f32x4 x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[j] = zero ? 0.0f
+                                    : (which ? dv[fb] : dk[fb])[4 * r4 + j] * (which ? fv : fk);
+                    *reinterpret_cast<f32x4*>(at + 32 * fb + 8 * r4 + 4 * (lane >> 5)) = x;
+                }
+        }
+        return;
+    }
+    if (part != 0) return;  // the first part writes what no key stands behind
     const AttnIo* const to[2] = {&g.dk, &g.dv};
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -501,6 +533,54 @@ attn_dq_kernel(const AttnArgs g) {
     }
 }
 
+// Sums the parts of dk and dv: half a wave a row of one of them, four features a
+// lane.
+__global__ __launch_bounds__(kAttnThreads) void attn_dkv_join_kernel(const AttnArgs g, int dp) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int kvh = blockIdx.y, which = (threadIdx.x >> 5) & 1, f = 4 * (threadIdx.x & 31);
+    int sid, at;
+    AttnSeq seq;
+    if (g.plan.seqs == nullptr) {
+        sid = static_cast<int>(row / g.plan.pad_s);
+        at = static_cast<int>(row - sid * g.plan.pad_s);
+        if (sid >= g.plan.batch) return;
+        seq = attn_seq(g.plan, sid);
+    } else {
+        int lo = 0, hi = static_cast<int>(g.plan.batch);
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (g.plan.seqs[mid].pk <= row) lo = mid;
+            else hi = mid;
+        }
+        sid = lo;
+        seq = g.plan.seqs[sid];
+        at = static_cast<int>(row) - seq.pk;
+    }
+    if (at >= seq.nk || f >= g.dim) return;
+    const int64_t step = static_cast<int64_t>(g.kv_heads) * g.dkv_rows;
+    const float* from = g.dkv_part + (which * step + kvh * g.dkv_rows + row) * dp + f;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int p = 0; p < g.dkv_parts; ++p) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(from + 2 * p * step * dp);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[j];
+    }
+    const AttnIo& io = which ? g.dv : g.dk;
+    const int64_t to = sid * io.sb + (seq.k0 + at) * io.sr + kvh * io.sh;
+    if (io.sd == 1 && g.vec_kv) {
+        if (g.dtype == SLK_F32) F32::store4(io.p, to + f, x);
+        else BF16::store4(io.p, to + f, x);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (f + j >= g.dim) return;
+        if (g.dtype == SLK_F32) F32::store(io.p, to + (f + j) * io.sd, x[j]);
+        else BF16::store(io.p, to + (f + j) * io.sd, x[j]);
+    }
+}
+
 // The bias's gradient from the workgroups' bins, in their order: a workgroup a
 // head, four threads a distance (a quarter of the bins each), then a thread a
 // bucket.
@@ -548,17 +628,24 @@ int launch(const AttnArgs& g, const AttnPlan& kplan, int64_t q_entries, int64_t 
            bool want_q, bool want_kv, int64_t k_tiles, hipStream_t st) {
     const size_t width = BIAS ? 2 * g.bias.max_distance + 1 : 0;
     if (q_entries * g.heads > max_groups(kAttnThreads) ||
-        k_entries * g.kv_heads > max_groups(kAttnThreads))
+        k_entries * g.kv_heads * g.dkv_parts > max_groups(kAttnThreads))
         return fail(SLK_EINVAL, "attention_backward: too many tiles");
     if (want_kv) {
         AttnArgs a = g;
         a.plan = kplan;
         a.tiles = k_tiles;
-        hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS>),
-                           dim3(static_cast<unsigned>(k_entries * g.kv_heads)),
-                           dim3(kAttnThreads), width * sizeof(float), st, a);
+        const dim3 grid(static_cast<unsigned>(k_entries * g.kv_heads * g.dkv_parts));
+        hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS>), grid, dim3(kAttnThreads),
+                           width * sizeof(float), st, a);
         const int rc = check_launch("attention_backward: dk, dv");
         if (rc != SLK_OK) return rc;
+        if (g.dkv_parts > 1) {
+            hipLaunchKernelGGL(attn_dkv_join_kernel,
+                               dim3(static_cast<unsigned>(g.dkv_rows / 4), g.kv_heads),
+                               dim3(kAttnThreads), 0, st, a, 32 * DB);
+            const int rj = check_launch("attention_backward: join");
+            if (rj != SLK_OK) return rj;
+        }
     }
     if (want_q) {
         hipLaunchKernelGGL((attn_dq_kernel<SPLIT, DB, BIAS>),

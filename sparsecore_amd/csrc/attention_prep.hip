@@ -39,7 +39,7 @@ __device__ int64_t scan(int64_t x, int64_t* lds, int64_t& last) {
 // One workgroup. Offsets that fall, or pass the arrays' end, are taken as the
 // nearest ones that do not: no row is written twice or outside.
 __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanArgs a) {
-    __shared__ int64_t lds[kPlanThreads / 64];
+    __shared__ int64_t lds[kPlanThreads / 64], ends[2];
     __shared__ int32_t bin[kBins];
     const int t = threadIdx.x;
     const bool packed = a.q_offsets != nullptr;
@@ -50,23 +50,30 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         AttnSeq x{};
         if (packed) {
             auto clamp = [](int64_t v, int64_t hi) { return v < 0 ? 0 : v > hi ? hi : v; };
-            // starts: running maximum of the offsets so far, ends: with the next one
-            const int64_t oq = in ? clamp(a.q_offsets[s], a.rows_q) : 0;
-            const int64_t ok = in ? clamp(a.k_offsets[s], a.rows_k) : 0;
-            int64_t last;
-            int64_t bq = scan<true>(oq, lds, last), bk = scan<true>(ok, lds, last);
-            bq = bq > endq ? bq : endq;
-            bk = bk > endk ? bk : endk;
-            const int64_t nq = in ? clamp(a.q_offsets[s + 1], a.rows_q) : 0;
-            const int64_t nk = in ? clamp(a.k_offsets[s + 1], a.rows_k) : 0;
+            const int64_t oq = in ? clamp(a.q_offsets[s], a.rows_q) : a.rows_q;
+            const int64_t ok = in ? clamp(a.k_offsets[s], a.rows_k) : a.rows_k;
+            const int64_t nq = in ? clamp(a.q_offsets[s + 1], a.rows_q) : a.rows_q;
+            const int64_t nk = in ? clamp(a.k_offsets[s + 1], a.rows_k) : a.rows_k;
+            int64_t bq = oq, bk = ok;
+            // starts are the running maximum of the offsets: themselves if none falls
+            if (!__syncthreads_and(nq >= oq && nk >= ok && oq >= endq && ok >= endk)) {
+                int64_t last;
+                bq = scan<true>(oq, lds, last);
+                bk = scan<true>(ok, lds, last);
+                bq = bq > endq ? bq : endq;
+                bk = bk > endk ? bk : endk;
+            }
             x.q0 = static_cast<int32_t>(bq);
             x.k0 = static_cast<int32_t>(bk);
-            x.nq = x.eq = static_cast<int32_t>(nq > bq ? nq - bq : 0);
-            x.nk = x.ek = static_cast<int32_t>(nk > bk ? nk - bk : 0);
-            scan<true>(in ? bq + x.nq : 0, lds, last);
-            endq = last > endq ? last : endq;
-            scan<true>(in ? bk + x.nk : 0, lds, last);
-            endk = last > endk ? last : endk;
+            x.nq = x.eq = static_cast<int32_t>(in && nq > bq ? nq - bq : 0);
+            x.nk = x.ek = static_cast<int32_t>(in && nk > bk ? nk - bk : 0);
+            if (in && (t == kPlanThreads - 1 || s == a.n - 1)) {
+                ends[0] = bq + x.nq;
+                ends[1] = bk + x.nk;
+            }
+            __syncthreads();
+            endq = ends[0];
+            endk = ends[1];
         } else {
             auto live = [&](const int32_t* p, int64_t rows) {
                 const int64_t n = p != nullptr ? p[s] : rows;
@@ -79,8 +86,10 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         }
         const int64_t wq = in ? ceil_div(x.nq, kAttnRows) * kAttnRows : 0;
         const int64_t wk = in ? ceil_div(x.nk, kAttnRows) * kAttnRows : 0;
-        int64_t totq, totk;
-        const int64_t iq = scan<false>(wq, lds, totq), ik = scan<false>(wk, lds, totk);
+        int64_t both;  // sums of queries' and keys' rows, each below 2^31
+        const int64_t upto = scan<false>(wq << 32 | wk, lds, both);
+        const int64_t iq = upto >> 32, ik = upto & 0xffffffff;
+        const int64_t totq = both >> 32, totk = both & 0xffffffff;
         x.pq = static_cast<int32_t>(pq + iq - wq);
         x.pk = static_cast<int32_t>(pk + ik - wk);
         pq += totq;
