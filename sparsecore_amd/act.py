@@ -10,6 +10,8 @@ save_bits=8)`` keeps its input in the same way.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -18,17 +20,20 @@ from . import _lib
 __all__ = ["activation"]
 
 
-def _dense(t: torch.Tensor) -> bool:
-    """Whether t's elements fill one piece of memory, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
+@functools.lru_cache(maxsize=256)
+def _fills(shape, stride) -> bool:
     want = 1
-    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1),
-                               key=lambda x: x[1]):
-        if stride != want:
+    for size, step in sorted(((n, s) for n, s in zip(shape, stride) if n != 1),
+                             key=lambda x: x[1]):
+        if step != want:
             return False
         want *= size
     return True
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one piece of memory, in any order of its dimensions."""
+    return t.is_contiguous() or _fills(t.shape, t.stride())
 
 
 def _in_layout(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:

@@ -54,36 +54,38 @@ def _starts(buckets: int, max_distance: int):
     return (ctypes.c_int32 * len(table))(*table)
 
 
-def _tensor(t: torch.Tensor | None) -> _lib.AttnTensor:
-    if t is None:
-        return _lib.AttnTensor()
-    s = t.stride()
+def _tensor(t: torch.Tensor) -> _lib.AttnTensor:
     if t.dim() == 3:
-        return _lib.AttnTensor(t.data_ptr(), 0, *s)
-    return _lib.AttnTensor(t.data_ptr(), *s)
+        return _lib.AttnTensor(t.data_ptr(), 0, *t.stride())
+    return _lib.AttnTensor(t.data_ptr(), *t.stride())
 
 
-def _order(t: torch.Tensor):
-    """(sizes in t's order of dimensions in memory, the permutation back, dtype, device)."""
-    order = sorted(range(t.dim()), key=lambda i: -t.stride(i))
-    back = [0] * t.dim()
-    for at, i in enumerate(order):
-        back[i] = at
-    return [t.shape[i] for i in order], back, t.dtype, t.device
+@functools.lru_cache(maxsize=256)
+def _compact(shape, stride) -> tuple[int, ...]:
+    """Strides of a tensor of this shape in the same order of dimensions, without gaps."""
+    out, step = [0] * len(shape), 1
+    for i in sorted(range(len(shape)), key=lambda i: (stride[i], -i)):
+        out[i] = step
+        step *= shape[i]
+    return tuple(out)
 
 
-def _like(order) -> torch.Tensor:
-    """A new tensor of the noted one's shape and order in memory, without its gaps."""
-    sizes, back, dtype, device = order
-    return torch.empty(sizes, dtype=dtype, device=device).permute(back)
+def _gradient(like, dtype, device) -> tuple[torch.Tensor, _lib.AttnTensor]:
+    """A new tensor for the gradient of one of this shape and these strides."""
+    shape, stride = like
+    stride = _compact(shape, stride)
+    t = torch.empty_strided(shape, stride, dtype=dtype, device=device)
+    return t, _lib.AttnTensor(t.data_ptr(), *((0,) if len(shape) == 3 else ()), *stride)
 
 
 def _output(q: torch.Tensor, feature_major: bool) -> torch.Tensor:
     if not feature_major:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    h, d = q.shape[-2:]
-    flat = torch.empty((h * d, q.numel() // max(1, h * d)), dtype=q.dtype, device=q.device)
-    return flat.t().reshape(*q.shape[:-2], h * d).unflatten(-1, (h, d))
+    *lead, h, d = q.shape
+    rows = lead[0] * lead[1] if len(lead) == 2 else lead[0]
+    stride = (d * rows, rows) if rows else (d, 1)
+    return torch.empty_strided(q.shape, ((lead[1], 1) if len(lead) == 2 else (1,)) + stride,
+                               dtype=q.dtype, device=q.device)
 
 
 def _set_ints(a, offsets, k_offsets, lengths, k_lengths) -> None:
@@ -127,8 +129,7 @@ class _Attention(torch.autograd.Function):
         if keep:
             ctx.save_for_backward(saved, out, bias, offsets, k_offsets, lengths, k_lengths)
             ctx.args, ctx.starts = a, starts if bias is not None else None
-            ctx.like = [_order(t) if n else None
-                        for t, n in zip((q, k, v), ctx.needs_input_grad)]
+            ctx.like = [(t.shape, t.stride()) for t in (q, k, v)]
         return out
 
     @staticmethod
@@ -139,17 +140,23 @@ class _Attention(torch.autograd.Function):
         # a copy: the graph may be gone through again
         a = _lib.Attention.from_buffer_copy(ctx.args)
         _set_ints(a, *ints)
-        dq, dk, dv = (_like(x) if x is not None else None for x in ctx.like)
-        if (dk is None) != (dv is None):  # computed together
-            dk, dv = (torch.empty_like(x if x is not None else y)
-                      for x, y in ((dk, dv), (dv, dk)))
-        dbias = torch.empty_like(bias) if bias is not None and need[3] else None
-        a.out, a.dout, a.dq, a.dk, a.dv = (_tensor(t) for t in (out, dout, dq, dk, dv))
-        a.saved, a.bias, a.dbias = saved.data_ptr(), _lib.ptr(bias), _lib.ptr(dbias)
+        dtype, dev = out.dtype, out.device
+        dq = dk = dv = dbias = None
+        if need[0]:
+            dq, a.dq = _gradient(ctx.like[0], dtype, dev)
+        if need[1] or need[2]:  # computed together
+            dk, a.dk = _gradient(ctx.like[1], dtype, dev)
+            dv, a.dv = _gradient(ctx.like[2], dtype, dev)
+        if bias is not None:
+            a.bias = bias.data_ptr()
+            if need[3]:
+                dbias = torch.empty_like(bias)
+                a.dbias = dbias.data_ptr()
+        a.out, a.dout, a.saved = _tensor(out), _tensor(dout), saved.data_ptr()
         with _lib.on_device(out):
             a.scratch_bytes = _lib.attention_scratch_bytes(a, True)
             if a.scratch_bytes:
-                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=out.device)
+                scratch = torch.empty(a.scratch_bytes, dtype=torch.uint8, device=dev)
                 a.scratch = scratch.data_ptr()
             _lib.attention_backward(a, _lib.stream_of(out))
         return (dq, dk if need[1] else None, dv if need[2] else None, dbias) + (None,) * 9
@@ -198,9 +205,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, sizes).
     """
-    given = [("q", q), ("k", k), ("v", v), ("bias", bias), ("offsets", offsets),
-             ("k_offsets", k_offsets), ("lengths", lengths), ("k_lengths", k_lengths)]
-    for name, t in given:
+    for name, t in (("q", q), ("k", k), ("v", v), ("bias", bias), ("offsets", offsets),
+                    ("k_offsets", k_offsets), ("lengths", lengths), ("k_lengths", k_lengths)):
         if t is None and name not in ("q", "k", "v"):
             continue
         if not isinstance(t, torch.Tensor):
@@ -208,7 +214,7 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
         if not t.is_cuda:
             raise RuntimeError(f"attention: {name} must be on a HIP (ROCm) device (got "
                                f"device={t.device})")
-        if t.device != q.device:
+        if t.get_device() != q.get_device():
             raise RuntimeError(f"attention: {name} is on {t.device} but q on {q.device}")
     if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"attention: q, k and v must all be float32 or all bfloat16, got "
@@ -238,15 +244,16 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
             raise ValueError("attention: k_offsets need offsets")
         if q.shape[0] != k.shape[0]:
             raise ValueError(f"attention: q has {q.shape[0]} entries but k {k.shape[0]}")
-    for name, t in given[4:]:
+    for name, t in (("offsets", offsets), ("k_offsets", k_offsets), ("lengths", lengths),
+                    ("k_lengths", k_lengths)):
         if t is None:
             continue
-        want = (q.shape[0],) if name.endswith("lengths") else None
-        if t.dtype != torch.int32 or t.dim() != 1 or (want and t.shape != want) or \
-                (not want and t.numel() < 1):
-            raise ValueError(f"attention: {name} must be int32, "
-                             f"{'one for each entry' if want else 'one for each sequence and one more'}"
-                             f", got {t.dtype} {tuple(t.shape)}")
+        each = name.endswith("lengths")
+        if t.dtype != torch.int32 or t.dim() != 1 or \
+                (t.shape[0] != q.shape[0] if each else t.shape[0] < 1):
+            raise ValueError(f"attention: {name} must be int32, one for each "
+                             f"{'entry' if each else 'sequence and one more'}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
     if k_offsets is not None and k_offsets.shape != offsets.shape:
         raise ValueError("attention: offsets and k_offsets must have the same length")
     if lengths is not None and k_lengths is None:
@@ -269,7 +276,9 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     scale = d ** -0.5 if scale is None else float(scale)
     if not (0.0 <= scale < math.inf):
         raise ValueError(f"attention: scale must be finite and not negative, got {scale}")
-    ints = [t if t is None or t.is_contiguous() else t.contiguous()
-            for t in (offsets, k_offsets, lengths, k_lengths)]
-    return _Attention.apply(q, k, v, bias, *ints, max_distance, bool(causal), scale,
-                            bool(feature_major), torch.is_grad_enabled())
+    if offsets is not None or k_lengths is not None:
+        offsets, k_offsets, lengths, k_lengths = (
+            t if t is None or t.is_contiguous() else t.contiguous()
+            for t in (offsets, k_offsets, lengths, k_lengths))
+    return _Attention.apply(q, k, v, bias, offsets, k_offsets, lengths, k_lengths, max_distance,
+                            bool(causal), scale, bool(feature_major), torch.is_grad_enabled())

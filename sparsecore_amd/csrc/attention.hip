@@ -143,6 +143,7 @@ int splits_of(const slk_attention& a, const Sizes& s) {
 struct Forward {
     Saved saved;  // its place, or a part of scratch
     float *part, *part_ml;
+    int64_t part_rows;
     int splits;
     Few few;
     int64_t bytes;
@@ -166,7 +167,9 @@ Forward forward_of(const slk_attention& a, void* scratch) {
         }
     }
     if (f.splits > 1) {
-        const int64_t rows = f.splits * a.heads * s.pad_q;
+        // padded rows of queries; few queries are not padded
+        f.part_rows = few_rows(a) ? a.n * a.rows_q : s.pad_q;
+        const int64_t rows = f.splits * a.heads * f.part_rows;
         f.part = static_cast<float*>(c.take(rows * 32 * blocks_of(a.dim) * 4));
         f.part_ml = static_cast<float*>(c.take(rows * 8));
     }
@@ -402,7 +405,8 @@ int few_forward(const slk_attention& a, const Forward& f, hipStream_t st) {
     d.g.splits = f.splits;
     d.g.part = f.part;
     d.g.part_ml = f.part_ml;
-    d.g.part_rows = sizes_of(a).pad_q;
+    d.g.part_rows = f.part_rows;
+    d.g.plan.pad_t = a.rows_q;
     d.q = io_of(a.q);
     d.k = io_of(a.k);
     d.v = io_of(a.v);
@@ -467,7 +471,7 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     g.splits = f.splits;
     g.part = f.part;
     g.part_ml = f.part_ml;
-    g.part_rows = s.pad_q;
+    g.part_rows = f.part_rows;
     return attn_launch_forward(g, split, blocks_of(a.dim), s.q_entries, st);
 }
 
@@ -477,8 +481,10 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     int rc = check(args, "attention_backward", true);
     if (rc != SLK_OK) return rc;
     const slk_attention& a = *args;
-    if (a.n == 0 && !packed_rows(a)) return SLK_OK;
     const hipStream_t st = as_stream(stream);
+    if (a.n == 0 && !packed_rows(a)) {  // nothing to sum: zeros
+        return a.dbias != nullptr ? attn_launch_dbias(args_of(a, nullptr), a.dbias, st) : SLK_OK;
+    }
     const Sizes s = sizes_of(a);
     const bool split = a.dtype == SLK_F32;
     const Saved sv = saved_of(a, a.saved);

@@ -13,7 +13,7 @@ namespace {
 // Exponent above the largest |dS| of a pair of tiles: |dP| < DP·2^(oe + 1)·2^(ve + 1), and
 // |delta| < 2^(de + 1).
 __device__ __forceinline__ int ds_exponent(int oe, int ve, int de, int log_dp) {
-    return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -100), 100);
+    return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -100), 120);
 }
 
 // The diagonals of a block of 32 queries x 8 keys: a row of LDS each, eight keys
