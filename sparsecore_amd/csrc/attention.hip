@@ -238,6 +238,12 @@ bool four_features(const slk_attn_tensor& t, const slk_attention& a) {
     return a.dim % 4 == 0 && fours(t, t.feature, t.row, t.head, t.batch, a.dtype);
 }
 
+AttnVec vec_of(const slk_attn_tensor& t, const slk_attention& a) {
+    return four_features(t, a)                                           ? kVecFeatures
+           : fours(t, t.row, t.feature, t.head, t.batch, a.dtype)        ? kVecRows
+                                                                         : kVecNone;
+}
+
 AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s,
                    const slk_attention& a, bool keys, int64_t heads) {
     const int64_t rows = keys ? s.pad_k : s.pad_q;
@@ -251,9 +257,7 @@ AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s,
     o.rows = rows;
     o.heads = static_cast<int32_t>(heads);
     o.keys = keys;
-    o.vec = four_features(t, a) ? kVecFeatures
-            : fours(t, t.row, t.feature, t.head, t.batch, a.dtype) ? kVecRows
-                                                                   : kVecNone;
+    o.vec = vec_of(t, a);
     return o;
 }
 
@@ -498,7 +502,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
         p.n = 1;
         p.op[0] = pack_op(a.dout, b.dout, s, a, false, a.heads);
         p.o = io_of(a.out);
-        p.o_vec = four_features(a.out, a);
+        p.o_vec = vec_of(a.out, a);
         p.delta = b.delta;
         p.delta_sh = s.pad_q;
         p.lse = sv.lse;

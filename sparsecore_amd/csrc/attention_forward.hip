@@ -234,12 +234,14 @@ attn_forward_kernel(const AttnArgs g) {
     }
 }
 
-// Joins the parts of split keys: a wave a query and head. Lanes read the parts'
-// maxima and sums side by side, then features of one part after another.
-__global__ __launch_bounds__(kWave) void attn_join_kernel(const AttnArgs g, int dp) {
-    __shared__ float weight[kAttnMaxSplits];
-    const int64_t e = blockIdx.x;
-    const int head = blockIdx.y, lane = threadIdx.x;
+// Joins the parts of split keys: a wave a query and head. Its lanes read the parts'
+// maxima and sums side by side; then each sixteen lanes add up every fourth part,
+// four features a lane.
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs g, int dp) {
+    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const int64_t rows = g.plan.seqs != nullptr ? g.part_rows : g.plan.batch * g.plan.t;
+    const int64_t e = static_cast<int64_t>(blockIdx.x) * (kAttnThreads / 64) + threadIdx.x / 64;
+    if (e >= rows) return;
     int sid, at;
     AttnSeq seq;
     int64_t row;
@@ -263,42 +265,63 @@ __global__ __launch_bounds__(kWave) void attn_join_kernel(const AttnArgs g, int 
     }
     const int64_t step = static_cast<int64_t>(g.heads) * g.part_rows;
     const int64_t r0 = head * g.part_rows + row;
-    float top = -INFINITY, mine[kAttnMaxSplits / kWave], sums[kAttnMaxSplits / kWave];
+    constexpr int kMost = kAttnMaxSplits / 64;
+    float top = -INFINITY, mine[kMost], sums[kMost];
 #pragma unroll
-    for (int i = 0; i < kAttnMaxSplits / kWave; ++i) {
-        const int s = lane + kWave * i;
-        const bool in = s < g.splits;
-        mine[i] = in ? g.part_ml[2 * (r0 + s * step)] : -INFINITY;
-        sums[i] = in ? g.part_ml[2 * (r0 + s * step) + 1] : 0.0f;
+    for (int i = 0; i < kMost; ++i) {
+        const int s = lane + 64 * i;
+        mine[i] = -INFINITY;
+        sums[i] = 0.0f;
+        if (s < g.splits) {
+            const float2 x = *reinterpret_cast<const float2*>(g.part_ml + 2 * (r0 + s * step));
+            mine[i] = x.x;
+            sums[i] = x.y;
+        }
         top = fmaxf(top, mine[i]);
     }
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kAttnMaxSplits / kWave; ++i) {
+    for (int i = 0; i < kMost; ++i) {
         // a part that saw no key has sum 0 (and maximum -inf)
-        const float a = sums[i] == 0.0f ? 0.0f : attn_exp2(mine[i] - top);
-        weight[lane + kWave * i] = a;
-        sum += sums[i] == 0.0f ? 0.0f : sums[i] * a;
+        mine[i] = sums[i] == 0.0f ? 0.0f : attn_exp2(mine[i] - top);
+        sum += sums[i] == 0.0f ? 0.0f : sums[i] * mine[i];
     }
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
-    __syncthreads();
+    const float inv = 1.0f / sum;
     const int64_t to = sid * g.out.sb + (seq.q0 + at) * g.out.sr + head * g.out.sh;
-    for (int f = lane; f < g.dim; f += kWave) {
-        const float* p = g.part + r0 * dp + f;
-        float x = 0.0f;
+    for (int f0 = 0; f0 < dp; f0 += 64) {
+        const int f = f0 + 4 * (lane & 15);
+        const float* p = g.part + r0 * dp + (f < dp ? f : 0);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-        for (int s = 0; s < g.splits; ++s) {
-            // a weight of 0 is a part that holds zeros, or whose weights all vanished
-            x = __builtin_fmaf(p[s * step * dp], weight[s], x);
+        for (int s0 = 0; s0 < g.splits; s0 += 4) {
+            const int s = s0 + (lane >> 4);
+            const float w = __shfl(s0 < 64 ? mine[0] : mine[1], s & 63);
+            const f32x4 y =
+                *reinterpret_cast<const f32x4*>(p + min(s, g.splits - 1) * step * dp);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x[j] = __builtin_fmaf(y[j], s < g.splits ? w : 0.0f, x[j]);
         }
-        const float y = sum != 0.0f ? x / sum : 0.0f;
-        if (g.dtype == SLK_F32) F32::store(g.out.p, to + f * g.out.sd, y);
-        else BF16::store(g.out.p, to + f * g.out.sd, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] += __shfl_xor(x[j], 16);
+            x[j] += __shfl_xor(x[j], 32);
+        }
+        if (lane >= 16 || f >= dp) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (f + j >= g.dim) break;
+            const float y = sum != 0.0f ? x[j] * inv : 0.0f;
+            if (g.dtype == SLK_F32) F32::store(g.out.p, to + (f + j) * g.out.sd, y);
+            else BF16::store(g.out.p, to + (f + j) * g.out.sd, y);
+        }
     }
 }
+static_assert(kAttnMaxSplits == 128, "two parts a lane");
 
 template <bool SPLIT, int DB>
 int launch(const AttnArgs& g, int64_t entries, hipStream_t st) {
@@ -321,8 +344,8 @@ int launch(const AttnArgs& g, int64_t entries, hipStream_t st) {
 
 int attn_launch_join(const AttnArgs& g, int db, hipStream_t st) {
     const int64_t rows = g.plan.seqs != nullptr ? g.part_rows : g.plan.batch * g.plan.t;
-    const dim3 grid(static_cast<unsigned>(rows), g.heads);
-    hipLaunchKernelGGL(attn_join_kernel, grid, dim3(kWave), 0, st, g, 32 * db);
+    const dim3 grid(static_cast<unsigned>(ceil_div(rows, kAttnThreads / 64)), g.heads);
+    hipLaunchKernelGGL(attn_join_kernel, grid, dim3(kAttnThreads), 0, st, g, 32 * db);
     return check_launch("attention_forward: join");
 }
 

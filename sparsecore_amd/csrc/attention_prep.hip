@@ -194,23 +194,193 @@ __device__ __forceinline__ RowOf row_of(const AttnPlan& p, bool keys, int64_t pa
     return r;
 }
 
+// A tile of 64 rows x DP features of a tensor in registers. BY_ROWS, for tensors
+// whose rows are consecutive in memory: four rows of one feature a piece; else
+// eight features of one row. All loads are issued before the first value is
+// used: a loop that used each as it came took its memory latency sixteen times
+// over (15 us where the bytes take 4).
+template <class IO, int DP, bool BY_ROWS>
+struct TileRegs {
+    static constexpr int kWide = BY_ROWS ? 4 : 8;
+    static constexpr int kPer = kAttnRows * DP / kWide / kAttnThreads;
+    float v[kPer][kWide];
+    // Element j of piece k: row and feature.
+    static __device__ __forceinline__ void place(int k, int j, int& r, int& f) {
+        const int i = threadIdx.x + kAttnThreads * k;
+        if constexpr (BY_ROWS) {
+            r = 4 * (i % (kAttnRows / 4)) + j;
+            f = i / (kAttnRows / 4);
+        } else {
+            r = i / (DP / 8);
+            f = 8 * (i % (DP / 8)) + j;
+        }
+    }
+    // `at`: the first element; `row`: its row in the tensor (four rows are loaded at
+    // once where it is a multiple of four and vec says that the rest is).
+    __device__ __forceinline__ void load(const AttnIo& x, int64_t at, int64_t row, int live,
+                                         int dim, int vec) {
+        const bool four = BY_ROWS ? vec == kVecRows && (row & 3) == 0 : vec == kVecFeatures;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+#pragma unroll
+            for (int h = 0; h < kWide; h += 4) {
+                int r, f;
+                place(k, h, r, f);
+                const int64_t from = at + r * x.sr + f * x.sd;
+                const bool whole = BY_ROWS ? r + 4 <= live && f < dim : r < live && f + 4 <= dim;
+                if (four && whole) {
+                    IO::load4(x.p, from, v[k] + h);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool in =
+                            BY_ROWS ? r + j < live && f < dim : r < live && f + j < dim;
+                        v[k][h + j] =
+                            in ? IO::load(x.p, from + j * (BY_ROWS ? x.sr : x.sd)) : 0.0f;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Largest of the workgroup's values (bits of non-negative floats) in every thread.
+__device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t* lds) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, s)));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+}
+
+__device__ __forceinline__ int tile_exponent(uint32_t top) {
+    return max(static_cast<int>(top >> 23) - 127, -100);
+}
+
 // Packs a tile of 64 rows of one head: blockIdx.x the tile, blockIdx.y the head of
-// an operand; one more y for the rows of biases, a head each. Lanes run along
-// whichever of rows and features is consecutive in memory. Of dO (with delta
-// given) also delta, from the same tile and O. What bounds it is memory.
-template <bool SPLIT, int DB, class IO>
-__global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(const AttnPack a) {
+// an operand; one more y for the rows of biases, a head each. Of dO (with delta
+// given) also delta, from the same tile and O's. Rows of consecutive features go
+// from registers to their place; consecutive rows are turned through LDS. What
+// bounds it is memory.
+template <bool SPLIT, int DB, class IO, bool DELTA, bool BY_ROWS>
+__device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& op, int head,
+                                          const RowOf& ro) {
     constexpr int DP = 32 * DB;
-    __shared__ float x[kAttnRows][DP + 1];
-    __shared__ int32_t top;
-    __shared__ uint32_t odd[2];  // rows with a value that is not finite
+    using T = AttnTile<DB>;
+    using Regs = TileRegs<IO, DP, BY_ROWS>;
+    __shared__ float turn[BY_ROWS ? kAttnRows : 1][BY_ROWS ? DP + 1 : 1];
+    __shared__ float sums[DELTA && BY_ROWS ? 16 : 1][kAttnRows];
+    __shared__ uint32_t most[2][4], odd[2];  // odd: rows with a value that is not finite
     const int t = threadIdx.x;
+    const int64_t padded = static_cast<int64_t>(blockIdx.x) * kAttnRows;
+    const int n = op.keys ? ro.seq.nk : ro.seq.nq, first = op.keys ? ro.seq.k0 : ro.seq.q0;
+    const int live = min(max(n - ro.row, 0), kAttnRows);
+    const int64_t row = first + ro.row;
+    Regs in, out;
+    in.load(op.src, ro.sid * op.src.sb + row * op.src.sr + head * op.src.sh, row, live, a.dim,
+            op.vec);
+    // O in the same pieces as dO, whatever its own order
+    if constexpr (DELTA)
+        out.load(a.o, ro.sid * a.o.sb + row * a.o.sr + head * a.o.sh, row, live, a.dim, a.o_vec);
+    if (t < 2) odd[t] = 0;
+    __syncthreads();
+    float d[Regs::kWide];  // BY_ROWS: a thread's share of four rows' delta
+#pragma unroll
+    for (int j = 0; j < Regs::kWide; ++j) d[j] = 0.0f;
+    float rows_d[Regs::kPer];
+    uint32_t m = 0;  // the largest finite magnitude
+#pragma unroll
+    for (int k = 0; k < Regs::kPer; ++k) {
+        rows_d[k] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < Regs::kWide; ++j) {
+            int r, f;
+            Regs::place(k, j, r, f);
+            float& v = in.v[k][j];
+            if constexpr (DELTA) {
+                if constexpr (BY_ROWS) d[j] = __builtin_fmaf(v, out.v[k][j], d[j]);
+                else rows_d[k] = __builtin_fmaf(v, out.v[k][j], rows_d[k]);
+            }
+            const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+            if (b < 0x7f800000u) {
+                m = max(m, b);
+            } else {
+                v = 0.0f;
+                atomicOr(&odd[r >> 5], 1u << (r & 31));
+            }
+            if constexpr (BY_ROWS) turn[r][f] = v;
+        }
+    }
+    const int e = tile_exponent(block_max(m, most[0]));
+    const uint64_t bad = static_cast<uint64_t>(odd[1]) << 32 | odd[0];
+    if (t == 0) {
+        op.exps[head * op.exps_sh + padded / kAttnRows] = 2 * e + (bad != 0 ? 1 : 0);
+        op.bad[head * op.exps_sh + padded / kAttnRows] = bad;
+    }
+
+    // rows in pieces of eight features, permuted as they will lie in LDS
+    const float factor = ldexpf(1.0f, kAttnUnit - e);
+    char* const to = op.dst + head * op.dst_sh +
+                     static_cast<int64_t>(blockIdx.x) * ((SPLIT ? 2 : 1) * T::kPlane);
+#pragma unroll
+    for (int k = 0; k < kAttnRows * T::kPieces / kAttnThreads; ++k) {
+        const int i = kAttnThreads * k + t, r = i / T::kPieces, c = i % T::kPieces;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (BY_ROWS) v[j] = turn[r][8 * c + j] * factor;
+            else v[j] = in.v[k][j] * factor;
+        }
+        const AttnPair<SPLIT> f = attn_operand<SPLIT>(v);
+        char* const at = to + r * T::kRowBytes + 16 * (c ^ T::swz(r));
+        *reinterpret_cast<f16x8*>(at) = f.f[0];
+        if constexpr (SPLIT) *reinterpret_cast<f16x8*>(at + T::kPlane) = f.f[1];
+    }
+
+    if constexpr (DELTA) {
+        const int64_t at = head * a.delta_sh + padded;
+        uint32_t largest = 0;
+        auto put = [&](int r, float y) {
+            a.delta[at + r] = y;
+            a.lse_out[at + r] = (bad >> r) & 1 ? __builtin_nanf("") : a.lse[at + r];
+            const uint32_t b = __float_as_uint(y) & 0x7fffffffu;
+            if (b < 0x7f800000u) largest = max(largest, b);
+        };
+        if constexpr (BY_ROWS) {
+            // a thread's four rows are the same in every piece; sixteen threads share them
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[t / 16][4 * (t % 16) + j] = d[j];
+            __syncthreads();
+            if (t < kAttnRows) {
+                float y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y += sums[i][t];
+                put(t, y);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < Regs::kPer; ++k) {
+                float y = rows_d[k];
+#pragma unroll
+                for (int s = 1; s < DP / 8; s <<= 1) y += __shfl_xor(y, s);
+                int r, f;
+                Regs::place(k, 0, r, f);
+                if (f == 0) put(r, y);
+            }
+        }
+        const int de = tile_exponent(block_max(largest, most[1]));
+        if (t == 0) a.dexps[head * op.exps_sh + padded / kAttnRows] = de;
+    }
+}
+
+template <bool SPLIT, int DB, class IO, bool DELTA>
+__global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(const AttnPack a) {
     int which = 0, head = blockIdx.y;
     while (which < a.n && head >= a.op[which].heads) head -= a.op[which++].heads;
     if (which == a.n) {
         const int width = 2 * a.bias.max_distance + 1;
         for (int h = blockIdx.x; h < a.heads; h += gridDim.x)
-            for (int i = t; i < width; i += kAttnThreads)
+            for (int i = threadIdx.x; i < width; i += kAttnThreads)
                 a.bias.rows[static_cast<int64_t>(h) * width + i] =
                     attn_bias_of(a.bias, a.heads, h, i - a.bias.max_distance);
         return;
@@ -220,134 +390,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(const AttnPack 
     if (padded >= op.rows) return;
     const RowOf ro = row_of(a.plan, op.keys, padded);
     if (!ro.any) return;
-    const int n = op.keys ? ro.seq.nk : ro.seq.nq, first = op.keys ? ro.seq.k0 : ro.seq.q0;
-    const int live = min(max(n - ro.row, 0), kAttnRows);
-    const int64_t row = first + ro.row;
-    if (t == 0) top = odd[0] = odd[1] = 0;
-    __syncthreads();
-    const int64_t at = ro.sid * op.src.sb + row * op.src.sr + head * op.src.sh;
-    uint32_t m = 0;  // the largest finite magnitude
-    auto put = [&](int r, int f, float v) {
-        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        if (b < 0x7f800000u) {
-            m = max(m, b);
-        } else {
-            v = 0.0f;
-            atomicOr(&odd[r >> 5], 1u << (r & 31));
-        }
-        x[r][f] = v;
-    };
-    if (op.vec == kVecFeatures) {
-        for (int i = t; i < kAttnRows * DP / 4; i += kAttnThreads) {
-            const int r = i / (DP / 4), f = 4 * (i % (DP / 4));
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (r < live && f < a.dim) IO::load4(op.src.p, at + r * op.src.sr + f, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) put(r, f + j, v[j]);
-        }
-    } else if (op.vec == kVecRows) {
-        for (int i = t; i < kAttnRows * DP / 4; i += kAttnThreads) {
-            const int r = 4 * (i % (kAttnRows / 4)), f = i / (kAttnRows / 4);
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const int64_t from = at + r + f * op.src.sd;
-            if (f < a.dim) {
-                // four rows at once where they are aligned and all live
-                if (r + 4 <= live && ((row + r) & 3) == 0) {
-                    IO::load4(op.src.p, from, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (r + j < live) v[j] = IO::load(op.src.p, from + j);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) put(r + j, f, v[j]);
-        }
-    } else {
-        const bool rows_first = op.src.sr == 1 && op.src.sd != 1;
-        for (int i = t; i < kAttnRows * DP; i += kAttnThreads) {
-            const int r = rows_first ? i % kAttnRows : i / DP;
-            const int f = rows_first ? i / kAttnRows : i % DP;
-            float v = 0.0f;
-            if (r < live && f < a.dim) v = IO::load(op.src.p, at + r * op.src.sr + f * op.src.sd);
-            put(r, f, v);
-        }
-    }
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(m, s)));
-    __syncthreads();
-    if ((t & 63) == 0) atomicMax(&top, static_cast<int>(m));
-    __syncthreads();
-    const int e = max(static_cast<int>(static_cast<uint32_t>(top) >> 23) - 127, -100);
-    const uint64_t bad = static_cast<uint64_t>(odd[1]) << 32 | odd[0];
-    if (t == 0) {
-        op.exps[head * op.exps_sh + padded / kAttnRows] = 2 * e + (bad != 0 ? 1 : 0);
-        op.bad[head * op.exps_sh + padded / kAttnRows] = bad;
-    }
+    if (op.src.sr == 1 && op.src.sd != 1) pack_tile<SPLIT, DB, IO, DELTA, true>(a, op, head, ro);
+    else pack_tile<SPLIT, DB, IO, DELTA, false>(a, op, head, ro);
+}
 
-    // rows in pieces of eight features, permuted as they will lie in LDS
-    using T = AttnTile<DB>;
-    const float factor = ldexpf(1.0f, kAttnUnit - e);
-    char* const to = op.dst + head * op.dst_sh +
-                     static_cast<int64_t>(blockIdx.x) * ((SPLIT ? 2 : 1) * T::kPlane);
-    for (int i = t; i < kAttnRows * T::kPieces; i += kAttnThreads) {
-        const int r = i / T::kPieces, c = (i % T::kPieces) ^ T::swz(r);
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = x[r][8 * c + j] * factor;
-        const AttnPair<SPLIT> f = attn_operand<SPLIT>(v);
-        *reinterpret_cast<f16x8*>(to + 16 * i) = f.f[0];
-        if constexpr (SPLIT) *reinterpret_cast<f16x8*>(to + T::kPlane + 16 * i) = f.f[1];
-    }
-
-    if (a.delta == nullptr) return;
-    __syncthreads();
-    if (t == 0) top = 0;
-    __syncthreads();
-    // delta: lanes over rows where O's rows are consecutive, else four lanes a row
-    const bool rows_first = a.o.sr == 1 && a.o.sd != 1;
-    const int r = rows_first ? t % 64 : t / 4, part = rows_first ? t / 64 : t % 4;
-    float d = 0.0f;
-    const int64_t from = ro.sid * a.o.sb + (row + r) * a.o.sr + head * a.o.sh;
-    if (r < live) {
-        if (a.o_vec && !rows_first) {
-            for (int f = 4 * part; f < a.dim; f += 16) {
-                float v[4];
-                IO::load4(a.o.p, from + f, v);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) d = __builtin_fmaf(x[r][f + j], v[j], d);
-            }
-        } else {
-            for (int f = part; f < a.dim; f += 4)
-                d = __builtin_fmaf(x[r][f], IO::load(a.o.p, from + f * a.o.sd), d);
-        }
-    }
-    __syncthreads();
-    float* const sums = &x[0][0];
-    sums[4 * r + part] = d;
-    __syncthreads();
-    if (t < kAttnRows) {
-        const float y = (sums[4 * t] + sums[4 * t + 1]) + (sums[4 * t + 2] + sums[4 * t + 3]);
-        const int64_t at_row = head * a.delta_sh + padded + t;
-        a.delta[at_row] = y;
-        a.lse_out[at_row] = (bad >> t) & 1 ? __builtin_nanf("") : a.lse[at_row];
-        uint32_t b = __float_as_uint(y) & 0x7fffffffu;
-        b = b < 0x7f800000u ? b : 0;
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) b = max(b, static_cast<uint32_t>(__shfl_xor(b, s)));
-        if (t == 0)
-            a.dexps[head * op.exps_sh + padded / kAttnRows] =
-                max(static_cast<int>(b >> 23) - 127, -100);
-    }
+template <bool SPLIT, int DB, class IO>
+int pack_as(const AttnPack& a, dim3 grid, hipStream_t st) {
+    const dim3 wg(kAttnThreads);
+    if (a.delta != nullptr)
+        hipLaunchKernelGGL((attn_pack_kernel<SPLIT, DB, IO, true>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((attn_pack_kernel<SPLIT, DB, IO, false>), grid, wg, 0, st, a);
+    return check_launch("attention: pack");
 }
 
 template <bool SPLIT, class IO>
 int pack(const AttnPack& a, int db, dim3 grid, hipStream_t st) {
-    const dim3 wg(kAttnThreads);
-    if (db == 1) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 1, IO>), grid, wg, 0, st, a);
-    else if (db == 2) hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 2, IO>), grid, wg, 0, st, a);
-    else hipLaunchKernelGGL((attn_pack_kernel<SPLIT, 4, IO>), grid, wg, 0, st, a);
-    return check_launch("attention: pack");
+    return db == 1   ? pack_as<SPLIT, 1, IO>(a, grid, st)
+           : db == 2 ? pack_as<SPLIT, 2, IO>(a, grid, st)
+                     : pack_as<SPLIT, 4, IO>(a, grid, st);
 }
 
 }  // namespace
