@@ -73,7 +73,7 @@ Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows) {
 struct Plan {
     AttnSeq* seqs;
     int2 *q_list, *k_list;
-    int32_t* count;
+    int32_t *count, *q_map, *k_map;
 };
 
 Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s) {
@@ -81,6 +81,8 @@ Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s) {
     if (uniform(a)) return p;
     p.count = static_cast<int32_t*>(c.take(16));
     p.seqs = static_cast<AttnSeq*>(c.take((a.n + 2) * sizeof(AttnSeq)));
+    p.q_map = static_cast<int32_t*>(c.take(s.pad_q / kAttnRows * 4));
+    p.k_map = static_cast<int32_t*>(c.take(s.pad_k / kAttnRows * 4));
     p.q_list = static_cast<int2*>(c.take(s.q_entries * sizeof(int2)));
     if (a.keep) p.k_list = static_cast<int2*>(c.take(s.k_entries * sizeof(int2)));
     return p;
@@ -116,15 +118,18 @@ struct Few {
     int rows, chunks, splits;
 };
 
-// Rows of a key head that a workgroup takes, and parts of the keys: enough
-// workgroups for four on each CU, at least 512 keys each.
+// Rows of a key head that a workgroup takes, and parts of the keys, at least 512
+// each: as many workgroups as the card holds at once (by registers three a CU with
+// one row, else two). 16 x 8192 keys, 32 heads over 8, 128 wide, bf16: 108 us with
+// 512 workgroups, 120 with 1024, 168 with 256; 131071 keys, 12 heads, 64 wide,
+// float32: 159 us with 768, 170 with 1032, 183 with 516.
 Few few_of(const slk_attention& a) {
     const int64_t rows = a.heads / a.kv_heads * a.rows_q;
     Few f;
-    f.rows = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
+    f.rows = rows == 1 ? 1 : rows == 2 ? 2 : 4;
     f.chunks = static_cast<int>(ceil_div(rows, f.rows));
     const int64_t groups = a.n * a.kv_heads * f.chunks;
-    const int64_t want = groups > 0 ? ceil_div(4 * kCus, groups) : 1;
+    const int64_t want = groups > 0 ? (f.rows == 1 ? 3 : 2) * kCus / groups : 1;
     const int64_t most = ceil_div(a.rows_k, 512);
     f.splits = static_cast<int>(
         std::max<int64_t>(1, std::min({want, most, int64_t{kAttnMaxSplits}})));
@@ -266,6 +271,8 @@ AttnPlan plan_of(const slk_attention& a, const Plan& p, bool keys) {
     r.seqs = p.seqs;
     r.list = keys ? p.k_list : p.q_list;
     r.count = p.count != nullptr ? p.count + (keys ? 2 : 0) : nullptr;
+    r.q_map = p.q_map;
+    r.k_map = p.k_map;
     r.batch = a.n;
     r.t = a.rows_q;
     r.s = a.rows_k;
@@ -288,6 +295,11 @@ int make_plan(const slk_attention& a, const Plan& p, hipStream_t st) {
     g.q_list = p.q_list;
     g.k_list = p.k_list;
     g.count = p.count;
+    const Sizes s = sizes_of(a);
+    g.q_map = p.q_map;
+    g.k_map = p.k_map;
+    g.q_tiles = s.pad_q / kAttnRows;
+    g.k_tiles = s.pad_k / kAttnRows;
     g.causal = a.causal;
     while ((std::max(a.rows_q, a.rows_k) / kAttnRows) >> g.work_shift >= 1024) ++g.work_shift;
     return attn_launch_plan(g, st);

@@ -50,6 +50,7 @@ struct AttnPlan {
     const AttnSeq* seqs;
     const int2* list;
     const int32_t* count;
+    const int32_t *q_map, *k_map;  // the sequence of each tile of 64 padded rows
     int64_t batch, t, s;
     int64_t pad_t, pad_s;
 };
@@ -63,6 +64,31 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnPlan& p, int s) {
     q.pq = static_cast<int32_t>(s * p.pad_t);
     q.pk = static_cast<int32_t>(s * p.pad_s);
     return q;
+}
+
+// Sequence and row in it of a padded row of queries or keys; rows past the last
+// sequence's have none.
+struct AttnRow {
+    int sid, row;
+    AttnSeq seq;
+    bool any;
+};
+__device__ __forceinline__ AttnRow attn_row_of(const AttnPlan& p, bool keys, int64_t padded) {
+    AttnRow r;
+    if (p.seqs == nullptr) {
+        const int64_t pad = keys ? p.pad_s : p.pad_t;
+        r.sid = static_cast<int>(padded / pad);
+        r.any = r.sid < p.batch;
+        r.seq = attn_seq(p, r.sid);
+        r.row = static_cast<int>(padded - r.sid * pad);
+        return r;
+    }
+    r.sid = (keys ? p.k_map : p.q_map)[padded >> 6];
+    r.any = r.sid >= 0;
+    if (!r.any) return r;
+    r.seq = p.seqs[r.sid];
+    r.row = static_cast<int>(padded - (keys ? r.seq.pk : r.seq.pq));
+    return r;
 }
 
 // Entry e of the tile order: sequence and tile. first_long: tile 0 has the most

@@ -538,25 +538,8 @@ attn_dq_kernel(const AttnArgs g) {
 __global__ __launch_bounds__(kAttnThreads) void attn_dkv_join_kernel(const AttnArgs g, int dp) {
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int kvh = blockIdx.y, which = (threadIdx.x >> 5) & 1, f = 4 * (threadIdx.x & 31);
-    int sid, at;
-    AttnSeq seq;
-    if (g.plan.seqs == nullptr) {
-        sid = static_cast<int>(row / g.plan.pad_s);
-        at = static_cast<int>(row - sid * g.plan.pad_s);
-        if (sid >= g.plan.batch) return;
-        seq = attn_seq(g.plan, sid);
-    } else {
-        int lo = 0, hi = static_cast<int>(g.plan.batch);
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (g.plan.seqs[mid].pk <= row) lo = mid;
-            else hi = mid;
-        }
-        sid = lo;
-        seq = g.plan.seqs[sid];
-        at = static_cast<int>(row) - seq.pk;
-    }
-    if (at >= seq.nk || f >= g.dim) return;
+    const AttnRow r = attn_row_of(g.plan, true, row);
+    if (!r.any || r.row >= r.seq.nk || f >= g.dim) return;
     const int64_t step = static_cast<int64_t>(g.kv_heads) * g.dkv_rows;
     const float* from = g.dkv_part + (which * step + kvh * g.dkv_rows + row) * dp + f;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -567,7 +550,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_join_kernel(const AttnA
         for (int j = 0; j < 4; ++j) x[j] += y[j];
     }
     const AttnIo& io = which ? g.dv : g.dk;
-    const int64_t to = sid * io.sb + (seq.k0 + at) * io.sr + kvh * io.sh;
+    const int64_t to = r.sid * io.sb + (r.seq.k0 + r.row) * io.sr + kvh * io.sh;
     if (io.sd == 1 && g.vec_kv) {
         if (g.dtype == SLK_F32) F32::store4(io.p, to + f, x);
         else BF16::store4(io.p, to + f, x);

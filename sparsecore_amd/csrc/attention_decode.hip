@@ -7,7 +7,8 @@
 // reads 64 / (DP/8) keys with one or two 16-byte loads a lane, four such groups in
 // flight; a score is eight fused multiply-adds and a sum over those lanes (DPP).
 // Every group of lanes keeps its own running maximum, sum and weighted values of
-// up to eight rows; they are joined once at the end, over lanes, waves and, where
+// up to four rows (eight took registers that left one wave a SIMD: slower than
+// reading the keys twice, the second time from the L2); they are joined once at the end, over lanes, waves and, where
 // the keys are split over workgroups to fill the card, by the join kernel.
 #include "attention_decode.hpp"
 
@@ -33,36 +34,26 @@ __device__ __forceinline__ float lane_sum(float x) {
     return x;
 }
 
-// Eight consecutive features of a row; zeros past dim.
-template <class IO>
-__device__ __forceinline__ void load8(const AttnIo& x, int64_t at, int f, int dim, bool vec,
-                                      float (&v)[8]) {
-    if (vec) {
-        if (f < dim) {
-            IO::load4(x.p, at + f, v);
-            if (f + 4 < dim) IO::load4(x.p, at + f + 4, v + 4);
-            else v[4] = v[5] = v[6] = v[7] = 0.0f;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = f + j < dim ? IO::load(x.p, at + (f + j) * x.sd) : 0.0f;
-    }
-}
-
-// Eight bfloat16 or four float32 of a 16-byte load are the unit of the fast form:
-// dim a multiple of 8, rows of consecutive features, 16-byte aligned.
+// Eight consecutive features of a row as they are loaded. The fast form: dim a
+// multiple of 8, rows of consecutive features, 16-byte aligned; lanes past dim read
+// the row's first features (their part of the query is zero).
 template <class IO>
 struct Raw;
 template <>
 struct Raw<F32> {
     f32x4 a, b;
-    __device__ __forceinline__ void load(const char* p) {
-        a = *reinterpret_cast<const f32x4*>(p);
-        b = *reinterpret_cast<const f32x4*>(p + 16);
+    __device__ __forceinline__ void load(const AttnIo& x, int64_t at, int f, int dim, bool vec) {
+        if (vec) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(x.p + 4 * (at + (f < dim ? f : 0)));
+            a = p[0];
+            b = p[1];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a[j] = f + j < dim ? F32::load(x.p, at + (f + j) * x.sd) : 0.0f;
+                b[j] = f + 4 + j < dim ? F32::load(x.p, at + (f + 4 + j) * x.sd) : 0.0f;
+            }
+        }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
@@ -71,10 +62,23 @@ struct Raw<F32> {
 };
 template <>
 struct Raw<BF16> {
-    uint4 a;
-    __device__ __forceinline__ void load(const char* p) { a = *reinterpret_cast<const uint4*>(p); }
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const AttnIo& x, int64_t at, int f, int dim, bool vec) {
+        if (vec) {
+            const uint4 a = *reinterpret_cast<const uint4*>(x.p + 2 * (at + (f < dim ? f : 0)));
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(x.p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int g = f + 2 * j;
+                const uint32_t lo = g < dim ? p[at + g * x.sd] : 0;
+                const uint32_t hi = g + 1 < dim ? p[at + (g + 1) * x.sd] : 0;
+                w[j] = lo | hi << 16;
+            }
+        }
+    }
     __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             v[2 * j] = __uint_as_float(w[j] << 16);
@@ -128,8 +132,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void attn_decode_kernel(const At
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = min(r0 + r, n_rows - 1), t = i / rep, h = kvh * rep + i % rep;
-        load8<IO>(a.q, sid * a.q.sb + (seq.q0 + min(t, max(seq.nq - 1, 0))) * a.q.sr + h * a.q.sh,
-                  f, g.dim, false, q[r]);
+        Raw<IO> raw;
+        raw.load(a.q, sid * a.q.sb + (seq.q0 + min(t, max(seq.nq - 1, 0))) * a.q.sr + h * a.q.sh,
+                 f, g.dim, false);
+        raw.get(q[r]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             q[r][j] *= g.scale2;
@@ -146,60 +152,59 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void attn_decode_kernel(const At
 
     const int64_t kb = sid * a.k.sb + static_cast<int64_t>(seq.k0) * a.k.sr + kvh * a.k.sh;
     const int64_t vb = sid * a.v.sb + static_cast<int64_t>(seq.k0) * a.v.sr + kvh * a.v.sh;
-    for (int key0 = k_lo + wv * kStep; key0 < k_hi; key0 += kDecodeWaves * kStep) {
-        float x[kInFlight][8], y[kInFlight][8];
-        const bool masked = key0 + kStep > k_hi || key0 + kStep - 1 > lim_lo;
-        if (a.vec) {
-            Raw<IO> rk[kInFlight], rv[kInFlight];
+    // The next pass's keys are asked for when this one's are in the scores, its
+    // values when this one's are added: one or the other is always on its way.
+    Raw<IO> rk[kInFlight], rv[kInFlight];
+    auto load = [&](Raw<IO>(&to)[kInFlight], const AttnIo& x, int64_t base, int key0)
+        __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < kInFlight; ++i) {
-                const int64_t key = min(key0 + i * KP + slot, k_hi - 1);
-                const int ff = f < g.dim ? f : 0;  // lanes past dim: q is zero there
-                rk[i].load(a.k.p + (kb + key * a.k.sr + ff) * IO::kBytes);
-                rv[i].load(a.v.p + (vb + key * a.v.sr + ff) * IO::kBytes);
-            }
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) {
-                rk[i].get(x[i]);
-                rv[i].get(y[i]);
-                if (f >= g.dim) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) {
-                const int64_t key = min(key0 + i * KP + slot, k_hi - 1);
-                load8<IO>(a.k, kb + key * a.k.sr, f, g.dim, false, x[i]);
-                load8<IO>(a.v, vb + key * a.v.sr, f, g.dim, false, y[i]);
-            }
+        for (int i = 0; i < kInFlight; ++i) {
+            const int64_t key = min(key0 + i * KP + slot, k_hi - 1);
+            to[i].load(x, base + key * x.sr, f, g.dim, a.vec);
         }
+    };
+    constexpr int kNext = kDecodeWaves * kStep;
+    if (k_lo + wv * kStep < k_hi) {
+        load(rk, a.k, kb, k_lo + wv * kStep);
+        load(rv, a.v, vb, k_lo + wv * kStep);
+    }
+    for (int key0 = k_lo + wv * kStep; key0 < k_hi; key0 += kNext) {
+        const bool masked = key0 + kStep > k_hi || key0 + kStep - 1 > lim_lo;
+        float s[R][kInFlight];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float s[kInFlight];
+        for (int i = 0; i < kInFlight; ++i) {
+            float x[8];
+            rk[i].get(x);
 #pragma unroll
-            for (int i = 0; i < kInFlight; ++i) {
+            for (int r = 0; r < R; ++r) {
                 float z = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z = __builtin_fmaf(x[i][j], q[r][j], z);
-                s[i] = lane_sum<L>(z);
+                for (int j = 0; j < 8; ++j) z = __builtin_fmaf(x[j], q[r][j], z);
+                s[r][i] = lane_sum<L>(z);
                 if constexpr (BIAS)
-                    s[i] += bias_rows[r * width + md +
-                                      attn_clamp(at[r] - (key0 + i * KP + slot), md)];
+                    s[r][i] += bias_rows[r * width + md +
+                                         attn_clamp(at[r] - (key0 + i * KP + slot), md)];
             }
-            bool see[kInFlight];
-            if (masked) {
+        }
+        if (key0 + kNext < k_hi) load(rk, a.k, kb, key0 + kNext);
+        uint32_t see = ~0u;  // bit 4 r + i
+        if (masked) {
+            see = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int i = 0; i < kInFlight; ++i) {
                     const int key = key0 + i * KP + slot;
-                    see[i] = key < k_hi && key <= lim[r];
-                    s[i] = see[i] ? s[i] : -INFINITY;
+                    const bool in = key < k_hi && key <= lim[r];
+                    s[r][i] = in ? s[r][i] : -INFINITY;
+                    see |= (in ? 1u : 0u) << (kInFlight * r + i);
                 }
-            }
-            float top = s[0];
+        }
 #pragma unroll
-            for (int i = 1; i < kInFlight; ++i) top = fmaxf(top, s[i]);
+        for (int r = 0; r < R; ++r) {
+            float top = s[r][0];
+#pragma unroll
+            for (int i = 1; i < kInFlight; ++i) top = fmaxf(top, s[r][i]);
             if (top > m[r]) {
                 const float scale = attn_exp2(m[r] - top);
                 m[r] = top;
@@ -210,18 +215,29 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void attn_decode_kernel(const At
             const float ref = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
             for (int i = 0; i < kInFlight; ++i) {
-                const float p = attn_exp2(s[i] - ref);
-                l[r] += p;
+                s[r][i] = attn_exp2(s[r][i] - ref);
+                l[r] += s[r][i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+            float y[8];
+            rv[i].get(y);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
                 if (masked) {  // a value that is not seen may be anything
+                    const bool in = (see >> (kInFlight * r + i)) & 1;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        o[r][j] = see[i] ? __builtin_fmaf(p, y[i][j], o[r][j]) : o[r][j];
+                        o[r][j] = in ? __builtin_fmaf(s[r][i], y[j], o[r][j]) : o[r][j];
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[r][j] = __builtin_fmaf(p, y[i][j], o[r][j]);
+                    for (int j = 0; j < 8; ++j)
+                        o[r][j] = __builtin_fmaf(s[r][i], y[j], o[r][j]);
                 }
             }
         }
+        if (key0 + kNext < k_hi) load(rv, a.v, vb, key0 + kNext);
     }
 
     // over the wave's groups of lanes, then over the waves
@@ -297,8 +313,7 @@ template <class IO, int DB>
 int launch_rows(const AttnDecode& a, int rows, int64_t groups, hipStream_t st) {
     if (rows == 1) return launch<IO, DB, 1>(a, groups, st);
     if (rows == 2) return launch<IO, DB, 2>(a, groups, st);
-    if (rows == 4) return launch<IO, DB, 4>(a, groups, st);
-    return launch<IO, DB, 8>(a, groups, st);
+    return launch<IO, DB, 4>(a, groups, st);
 }
 
 template <class IO>

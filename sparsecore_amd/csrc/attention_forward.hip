@@ -252,16 +252,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
         row = seq.pq + at;
     } else {
         row = e;
-        int lo = 0, hi = static_cast<int>(g.plan.batch);
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (g.plan.seqs[mid].pq <= row) lo = mid;
-            else hi = mid;
-        }
-        sid = lo;
-        seq = g.plan.seqs[sid];
-        at = static_cast<int>(row) - seq.pq;
-        if (at >= seq.nq) return;
+        const AttnRow r = attn_row_of(g.plan, false, row);
+        if (!r.any || r.row >= r.seq.nq) return;
+        sid = r.sid;
+        at = r.row;
+        seq = r.seq;
     }
     const int64_t step = static_cast<int64_t>(g.heads) * g.part_rows;
     const int64_t r0 = head * g.part_rows + row;

@@ -125,6 +125,17 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
     const bool one_each = total <= kPlanThreads;  // a thread keeps its sequence
     const AttnSeq own = one_each && t < total ? a.seqs[t] : AttnSeq{};
     for (int side = 0; side < 2; ++side) {
+        // the map from tiles of 64 padded rows to sequences, -1 past the last one's
+        int32_t* const map = side ? a.k_map : a.q_map;
+        const int64_t have = a.count[2 * side + 1] / kAttnRows;
+        for (int64_t i = have + t; i < (side ? a.k_tiles : a.q_tiles); i += kPlanThreads)
+            map[i] = -1;
+        for (int s = t; s < static_cast<int>(a.n); s += kPlanThreads) {
+            const AttnSeq x = one_each ? own : a.seqs[s];
+            const int first = (side ? x.pk : x.pq) / kAttnRows;
+            const int tiles = ((side ? x.nk : x.nq) + kAttnRows - 1) / kAttnRows;
+            for (int i = 0; i < tiles; ++i) map[first + i] = s;
+        }
         int2* list = side ? a.k_list : a.q_list;
         if (list == nullptr) continue;
         auto each = [&](auto&& f) {
@@ -162,36 +173,6 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
         if (t == 0) a.count[2 * side] = static_cast<int32_t>(all);
         __syncthreads();
     }
-}
-
-struct RowOf {
-    int sid, row;  // row of the sequence; at or past its last live row: none
-    AttnSeq seq;
-    bool any;
-};
-
-// Sequence and row of a padded row of queries or keys.
-__device__ __forceinline__ RowOf row_of(const AttnPlan& p, bool keys, int64_t padded) {
-    RowOf r;
-    if (p.seqs == nullptr) {
-        const int64_t pad = keys ? p.pad_s : p.pad_t;
-        r.sid = static_cast<int>(padded / pad);
-        r.any = r.sid < p.batch;
-        r.seq = attn_seq(p, r.sid);
-        r.row = static_cast<int>(padded - r.sid * pad);
-        return r;
-    }
-    r.any = padded < p.count[keys ? 3 : 1];
-    int lo = 0, hi = static_cast<int>(p.batch);
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((keys ? p.seqs[mid].pk : p.seqs[mid].pq) <= padded) lo = mid;
-        else hi = mid;
-    }
-    r.sid = lo;
-    r.seq = p.seqs[lo];
-    r.row = static_cast<int>(padded - (keys ? r.seq.pk : r.seq.pq));
-    return r;
 }
 
 // A tile of 64 rows x DP features of a tensor in registers. BY_ROWS, for tensors
@@ -264,7 +245,7 @@ __device__ __forceinline__ int tile_exponent(uint32_t top) {
 // bounds it is memory.
 template <bool SPLIT, int DB, class IO, bool DELTA, bool BY_ROWS>
 __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& op, int head,
-                                          const RowOf& ro) {
+                                          const AttnRow& ro) {
     constexpr int DP = 32 * DB;
     using T = AttnTile<DB>;
     using Regs = TileRegs<IO, DP, BY_ROWS>;
@@ -388,7 +369,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(const AttnPack 
     const AttnPackOp& op = a.op[which];
     const int64_t padded = static_cast<int64_t>(blockIdx.x) * kAttnRows;
     if (padded >= op.rows) return;
-    const RowOf ro = row_of(a.plan, op.keys, padded);
+    const AttnRow ro = attn_row_of(a.plan, op.keys, padded);
     if (!ro.any) return;
     if (op.src.sr == 1 && op.src.sd != 1) pack_tile<SPLIT, DB, IO, DELTA, true>(a, op, head, ro);
     else pack_tile<SPLIT, DB, IO, DELTA, false>(a, op, head, ro);

@@ -11,6 +11,8 @@ struct AttnPlanArgs {
     int64_t n, rows_q, rows_k;             // rows of the arrays, or of a batch entry
     AttnSeq* seqs;                         // n (+ 2 if packed)
     int2 *q_list, *k_list;                 // NULL: not wanted
+    int32_t *q_map, *k_map;                // sequences of q_tiles and k_tiles tiles of 64
+    int64_t q_tiles, k_tiles;
     int32_t* count;  // tiles of queries, their padded rows, tiles of keys, padded rows
     int32_t causal, work_shift;
 };
