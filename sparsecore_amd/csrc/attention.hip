@@ -10,7 +10,11 @@ namespace slk {
 namespace {
 
 constexpr int64_t kTileRows = kAttnTileRows;
-constexpr int kFewRows = 16;         // queries of an entry that go the way of single tokens
+// Rows of a key head (new tokens times the query heads of its group) that go the way
+// of single tokens: it reads the keys once for four rows, the tiled way packs them
+// once. 4 x 16384 keys, 32 heads over 8, bf16: 199 us against 257 with 16 rows, 349
+// against 258 with 32; 16 x 2048 keys, 16 heads: 89 against 91 with 12, 101 with 16.
+constexpr int64_t kFewRows = 16;
 constexpr int64_t kCus = 256;
 
 int64_t pad64(int64_t n) { return ceil_div(n, kAttnRows) * kAttnRows; }
@@ -111,7 +115,8 @@ Saved saved_of(const slk_attention& a, void* base) {
 }
 
 bool few_rows(const slk_attention& a) {
-    return !a.keep && a.q_offsets == nullptr && a.q_lengths == nullptr && a.rows_q <= kFewRows;
+    return !a.keep && a.q_offsets == nullptr && a.q_lengths == nullptr &&
+           a.heads / a.kv_heads * a.rows_q <= kFewRows;
 }
 
 struct Few {
