@@ -94,7 +94,7 @@ Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s) {
 
 struct Saved {
     Plan plan;
-    float *lse, *bias_rows;
+    float *lse, *inv, *bias_rows;
     Packed q, k, v;
     int64_t bytes;
 };
@@ -105,8 +105,10 @@ Saved saved_of(const slk_attention& a, void* base) {
     Saved r{};
     r.plan = take_plan(c, a, s);
     r.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
-    if (a.bias != nullptr)
+    if (a.bias != nullptr) {
+        r.inv = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
         r.bias_rows = static_cast<float*>(c.take(a.heads * (2 * a.max_distance + 1) * 4));
+    }
     r.q = take_packed(c, s, a.heads, s.pad_q);
     r.k = take_packed(c, s, a.kv_heads, s.pad_k);
     r.v = take_packed(c, s, a.kv_heads, s.pad_k);
@@ -189,8 +191,8 @@ Forward forward_of(const slk_attention& a, void* scratch) {
 
 // Parts of a group's query heads in the keys' gradients: where the keys' tiles
 // leave CUs idle, the heads go to workgroups of their own, whose sums are joined.
-// 8191 packed tokens, 16 heads over 4, 128 wide, bf16: 351 us in one part, 193 + 26
-// for the join in two, 112 + 46 in four.
+// 8191 packed tokens, 16 heads over 4, 128 wide, bf16: two parts took 0.62 of one
+// part's time, the join counted, four 0.45 (106 us + 25 for the join).
 int dkv_parts(const slk_attention& a, const Sizes& s) {
     const int64_t rep = a.heads / a.kv_heads, groups = s.k_entries * a.kv_heads;
     int64_t parts = 1;
@@ -489,6 +491,7 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     g.k = op_of(f.saved.k, s, s.pad_k);
     g.v = op_of(f.saved.v, s, s.pad_k);
     g.lse = f.saved.lse;
+    g.inv = f.saved.inv;
     g.splits = f.splits;
     g.part = f.part;
     g.part_ml = f.part_ml;
@@ -534,6 +537,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     g.v = op_of(sv.v, s, s.pad_k);
     g.dout = op_of(b.dout, s, s.pad_q);
     g.lse = b.lse;
+    g.inv = sv.inv;
     g.delta = b.delta;
     g.dexps = b.dexps;
     g.dbias_part = b.dbias_part;

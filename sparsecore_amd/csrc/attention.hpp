@@ -137,6 +137,8 @@ struct AttnArgs {
     AttnIo out, dq, dk, dv;
     float* lse;            // [head][padded row]: log2 of the sum; +inf: no key seen, or no query;
                            // NaN: a value that is not finite is seen
+    float* inv;            // with biases, lse is the row's maximum and inv 1 / the sum below it:
+                           // a bias of the type's lowest value would swallow the logarithm
     float* delta;          // [head][padded row]: rowsum(dO∘O)
     int32_t* dexps;        // [head][padded rows / 64]: exponent of the largest |delta|
     int64_t lse_sh;
@@ -277,18 +279,41 @@ __device__ __forceinline__ AttnPair<SPLIT> attn_operand(const float* x) {
     return r;
 }
 
-// acc[fb] += X^T·W over one block of 32 staged rows X, W a lane's 16 results (zero
-// where the pair is masked) as operands.
-template <bool SPLIT, int DB, int PLANE = AttnTile<DB>::kPlane>
+// N steps of a read from LDS and its use in a product, the reads D steps ahead: left
+// to itself the compiler puts each read right before its use, and the matrix
+// cores wait for the LDS at every step.
+template <bool SPLIT, int N, int D, class Read, class Use>
+__device__ __forceinline__ void attn_pipeline(Read&& read, Use&& use) {
+    AttnPair<SPLIT> f[D];
+    static_for<(D < N ? D : N)>([&](auto i) { f[i.value] = read(i); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<N>([&](auto i) {
+        use(i, f[i.value % D]);
+        if constexpr (i.value + D < N) {
+            f[i.value % D] = read(std::integral_constant<int, i.value + D>{});
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+}
+template <bool SPLIT>
+constexpr int kAttnAhead = SPLIT ? 2 : 4;
+
+// acc[fb] += X^T·W over NB blocks of 32 staged rows X, W a lane's 16 results of
+// each (zero where the pair is masked) as operands.
+template <bool SPLIT, int DB, int NB, int PLANE = AttnTile<DB>::kPlane>
 __device__ __forceinline__ void attn_accumulate(const AttnReads<SPLIT, DB>& rd,
-                                                const unsigned char* buf, int b,
-                                                const AttnPair<SPLIT> (&w)[2],
+                                                const unsigned char* buf, int b0,
+                                                const AttnPair<SPLIT> (&w)[NB][2],
                                                 f32x16 (&acc)[DB]) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int fb = 0; fb < DB; ++fb)
-            acc[fb] = attn_dot<SPLIT>(rd.template across<PLANE>(buf, b, s, fb), w[s], acc[fb]);
+    attn_pipeline<SPLIT, 2 * NB * DB, kAttnAhead<SPLIT>>(
+        [&](auto i) __attribute__((always_inline)) {
+            constexpr int fb = i.value % DB, s = i.value / DB % 2, b = i.value / DB / 2;
+            return rd.template across<PLANE>(buf, b0 + b, s, fb);
+        },
+        [&](auto i, const AttnPair<SPLIT>& x) __attribute__((always_inline)) {
+            constexpr int fb = i.value % DB, s = i.value / DB % 2, b = i.value / DB / 2;
+            acc[fb] = attn_dot<SPLIT>(x, w[b][s], acc[fb]);
+        });
 }
 
 // Row (in a block of 32) that register r of a result belongs to.
@@ -333,14 +358,24 @@ __device__ __forceinline__ float attn_bias_of(const AttnBias& b, int heads, int 
     const int64_t at = static_cast<int64_t>(bucket) * heads + head;
     const float x = b.dtype == SLK_F32 ? static_cast<const float*>(b.table)[at]
                                        : bf16_to_f32(static_cast<const uint16_t*>(b.table)[at]);
-    return x * kLog2e;
+    // a finite one stays finite: a bias of the type's lowest value outweighs the others,
+    // it does not hide a key whose row has no other
+    const float y = x * kLog2e;
+    return fabsf(x) < INFINITY ? fminf(fmaxf(y, -3e38f), 3e38f) : y;
 }
 
-// A head's biases into LDS (all threads; a barrier follows).
+// A head's biases into LDS (all threads; a barrier follows), the last ones on both
+// sides repeated so far that a block of 32 x 32 with a pair nearer than
+// max_distance needs no clamping: distance d at row[max_distance + kAttnFar + d].
+constexpr int kAttnFar = 64;
+__host__ __device__ constexpr int attn_bias_floats(int md) { return 2 * (md + kAttnFar) + 1; }
 __device__ __forceinline__ void attn_bias_row(const AttnBias& b, int head, float* row) {
-    const int width = 2 * b.max_distance + 1;
-    for (int i = threadIdx.x; i < width; i += blockDim.x)
-        row[i] = b.rows[static_cast<int64_t>(head) * width + i];
+    const int md = b.max_distance;
+    const float* from = b.rows + static_cast<int64_t>(head) * (2 * md + 1) + md;
+    for (int i = threadIdx.x; i < attn_bias_floats(md); i += blockDim.x) {
+        const int d = i - md - kAttnFar;
+        row[i] = from[d < -md ? -md : d > md ? md : d];
+    }
 }
 
 __device__ __forceinline__ int attn_clamp(int x, int m) { return x < -m ? -m : x > m ? m : x; }

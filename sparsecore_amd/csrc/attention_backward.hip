@@ -54,7 +54,10 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 // leaves room for two workgroups a CU), for every query head of the group in
 // turn, or for some of them where a group is spread over workgroups. Scores are
 // Q·K^T here: a lane holds 16 queries of one key, as the operands of
-// dV^T = dO^T·P and dK^T = Q^T·dS need them.
+// dV^T = dO^T·P and dK^T = Q^T·dS need them. One sequence of 16384, 32 heads over 8
+// of 128, bfloat16, causal: 4.84 ms, 0.91 PFLOP/s in its four products; the 512
+// registers of a SIMD's lane hold two waves, too few to keep the matrix cores busy
+// while both compute weights.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dkv_kernel(const AttnArgs g) {
@@ -65,11 +68,12 @@ attn_dkv_kernel(const AttnArgs g) {
     constexpr int kRows = kVInLds ? 32 : 64;             // queries of a stage
     constexpr int kPart = kRows * T::kRowBytes;          // bytes of a plane of them
     constexpr int kBytes = kPlanes * kPart;
-    __shared__ __align__(16) unsigned char ring0[2 * kBytes + 512];
-    __shared__ __align__(16) unsigned char ring1[2 * kBytes + 512];
+    constexpr int kRing = 2 * kBytes + (BIAS ? 768 : 512);
+    __shared__ __align__(16) unsigned char ring0[kRing];
+    __shared__ __align__(16) unsigned char ring1[kRing];
     __shared__ __align__(16) unsigned char values[kVInLds ? 2 * kTile : 16];
     // the last fragments of K, where registers would spill: each lane its own
-    constexpr int kSpare = kVInLds && !SPLIT ? 2 : 0;
+    constexpr int kSpare = !kVInLds || SPLIT ? 0 : 3;
     __shared__ f16x8 spare[kSpare ? 4 * kSpare : 1][64];
     extern __shared__ float bias_row[];
 
@@ -114,6 +118,8 @@ attn_dkv_kernel(const AttnArgs g) {
             // the whole tile's 64 rows each, of which a stage of 32 uses its half
             if (wv == 0) load_row(g.lse + head * g.lse_sh + tq * 64, to + 2 * kBytes, lane);
             if (wv == 1) load_row(g.delta + head * g.lse_sh + tq * 64, to + 2 * kBytes + 256, lane);
+            if (BIAS && wv == 2)
+                load_row(g.inv + head * g.lse_sh + tq * 64, to + 2 * kBytes + 512, lane);
         };
         issue(ring0, 0, 0);
         const AttnReads<SPLIT, DB> rd(lane);
@@ -187,51 +193,72 @@ attn_dkv_kernel(const AttnArgs g) {
                 f32x16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    AttnPair<SPLIT> k = kf[ks < KS - kSpare ? ks : 0];
-                    if (ks >= KS - kSpare) k.f[0] = spare[kSpare * wv + ks - (KS - kSpare)][lane];
-                    s = attn_dot<SPLIT>(row_of(buf, qb, ks), k, s);
-                    dp = attn_dot<SPLIT>(row_of(buf + kBytes, qb, ks),
-                                         kVInLds ? rd.along(my_v, wv & 1, ks)
-                                                 : vf[kVInLds ? 0 : ks],
-                                         dp);
-                }
+                attn_pipeline<SPLIT, 2 * KS, kAttnAhead<SPLIT>>(
+                    [&](auto i) __attribute__((always_inline)) {
+                        return row_of(i.value % 2 ? buf + kBytes : buf, qb, i.value / 2);
+                    },
+                    [&](auto i, const AttnPair<SPLIT>& x) __attribute__((always_inline)) {
+                        constexpr int ks = i.value / 2;
+                        if constexpr (i.value % 2 == 0) {
+                            AttnPair<SPLIT> k = kf[ks < KS - kSpare ? ks : 0];
+                            if constexpr (ks >= KS - kSpare)
+                                k.f[0] = spare[kSpare * wv + ks - (KS - kSpare)][lane];
+                            s = attn_dot<SPLIT>(x, k, s);
+                        } else {
+                            dp = attn_dot<SPLIT>(x, kVInLds ? rd.along(my_v, wv & 1, ks)
+                                                            : vf[kVInLds ? 0 : ks], dp);
+                        }
+                    });
                 const float* lse =
                     reinterpret_cast<const float*>(buf + 2 * kBytes) + (q0 & 63);
                 const float* delta = lse + 64;
-                float p[16], ds[16];
+                // the bias of the block's first query and this key; far: the same for all
+                const int lo_d = q0 + shift - key0 - 31;
+                const bool far = BIAS && (lo_d >= md || lo_d + 62 <= -md);
+                const float flat = BIAS ? bias_row[kAttnFar + (lo_d >= md ? 2 * md : 0)] : 0.0f;
+                const float* const near_at =
+                    BIAS ? bias_row + md + kAttnFar + (far ? 0 : q0 + shift - key) +
+                               4 * (lane >> 5)
+                         : nullptr;
+                // the lane's key is seen by rows [lo, hi) of the block
+                const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
+                AttnPair<SPLIT> wp[1][2], wd[1][2];
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const int row = 8 * r4 + 4 * (lane >> 5);
-                    const f32x4 z = *reinterpret_cast<const f32x4*>(lse + row);
-                    const f32x4 d = *reinterpret_cast<const f32x4*>(delta + row);
+                for (int half = 0; half < 2; ++half) {
+                    float p[8], ds[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * r4 + j;
-                        float add = unit - z[j];
-                        if constexpr (BIAS)
-                            add += bias_row[md + attn_clamp(q0 + row + j + shift - key, md)];
-                        p[r] = attn_exp2(__builtin_fmaf(s[r], c, add));
-                        ds[r] = p[r] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
+                    for (int r4 = 0; r4 < 2; ++r4) {
+                        const int at = 16 * half + 8 * r4, row = at + 4 * (lane >> 5);
+                        const f32x4 z = *reinterpret_cast<const f32x4*>(lse + row);
+                        const f32x4 d = *reinterpret_cast<const f32x4*>(delta + row);
+                        f32x4 inv = z;
+                        if constexpr (BIAS) inv = *reinterpret_cast<const f32x4*>(lse + 128 + row);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int i = 4 * r4 + j, r = 8 * half + i;
+                            // with a bias, rounded as in the forward: it may swallow the score
+                            if constexpr (BIAS)
+                                p[i] = attn_exp2(__builtin_fmaf(s[r], c,
+                                                                far ? flat : near_at[at + j]) -
+                                                 z[j] + unit) * inv[j];
+                            else p[i] = attn_exp2(__builtin_fmaf(s[r], c, unit - z[j]));
+                            ds[i] = p[i] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
+                        }
                     }
-                }
-                if (masked) {
-                    // the lane's key is seen by rows [lo, hi) of the block
-                    const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
+                    if (masked) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = attn_row(r, lane);
-                        const bool see = row >= lo && row < hi;
-                        p[r] = see ? p[r] : 0.0f;
-                        ds[r] = see ? ds[r] : 0.0f;
+                        for (int i = 0; i < 8; ++i) {
+                            const int row = attn_row(8 * half + i, lane);
+                            const bool see = row >= lo && row < hi;
+                            p[i] = see ? p[i] : 0.0f;
+                            ds[i] = see ? ds[i] : 0.0f;
+                        }
                     }
+                    wp[0][half] = attn_operand<SPLIT>(p);
+                    wd[0][half] = attn_operand<SPLIT>(ds);
                 }
-                const AttnPair<SPLIT> wp[2] = {attn_operand<SPLIT>(p), attn_operand<SPLIT>(p + 8)};
-                const AttnPair<SPLIT> wd[2] = {attn_operand<SPLIT>(ds),
-                                               attn_operand<SPLIT>(ds + 8)};
-                attn_accumulate<SPLIT, DB, kPart>(rd, buf + kBytes, qb, wp, dv);
-                attn_accumulate<SPLIT, DB, kPart>(rd, buf, qb, wd, dk);
+                attn_accumulate<SPLIT, DB, 1, kPart>(rd, buf + kBytes, qb, wp, dv);
+                attn_accumulate<SPLIT, DB, 1, kPart>(rd, buf, qb, wd, dk);
             }
         };
         int hr = 0, qt = 0;
@@ -308,7 +335,9 @@ attn_dkv_kernel(const AttnArgs g) {
 // lays eight keys' dS out by diagonals in LDS, sums each in one lane and adds it to
 // the wave's own bin of that distance, so the sums need no atomicity and repeat.
 // (Float atomics on LDS took some 260 cycles an instruction: the whole kernel 137
-// against @@ us at 16 x 512 tokens, 12 heads of 64, float32.)
+// us, without them 65, at 16 x 512 tokens, 12 heads of 64, float32.) One sequence of
+// 16384, 32 heads over 8 of 128, bfloat16, causal: 2.99 ms, 1.10 PFLOP/s in its three
+// products, bound by the matrix cores and the softmax's instructions between them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dq_kernel(const AttnArgs g) {
@@ -338,7 +367,7 @@ attn_dq_kernel(const AttnArgs g) {
     float* const diag = lds_floats + (threadIdx.x >> 6) * kDiags * kDiagRow;
     float* const far = lds_floats + 4 * kDiags * kDiagRow;  // [wave][below, above]
     float* const bias_row = far + 8;
-    float* const bins = bias_row + width;        // [wave][distance]
+    float* const bins = bias_row + attn_bias_floats(md);  // [wave][distance]
     const int d_row = min(lane, kDiags - 1);
     float below = 0.0f, above = 0.0f;            // distances past the last bins
     if constexpr (BIAS) {
@@ -380,7 +409,7 @@ attn_dq_kernel(const AttnArgs g) {
         }
         const bool mine = q < seq.nq;
         const int64_t ri = head * g.lse_sh + q_row + (lane & 31);
-        const float lse = mine ? g.lse[ri] : INFINITY;
+        const float lse = mine ? g.lse[ri] : INFINITY, inv = BIAS && mine ? g.inv[ri] : 0.0f;
         const float delta = mine ? g.delta[ri] : 0.0f;
         const int qe = attn_exp(g.q, head, q_row), oe = attn_exp(g.dout, head, q_row);
         const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (q_row >> 6));
@@ -411,11 +440,15 @@ attn_dq_kernel(const AttnArgs g) {
                 f32x16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    s = attn_dot<SPLIT>(rd.along(buf, kb, ks), qf[ks], s);
-                    dp = attn_dot<SPLIT>(rd.along(buf + kBytes, kb, ks), of[ks], dp);
-                }
+                attn_pipeline<SPLIT, 2 * KS, kAttnAhead<SPLIT>>(
+                    [&](auto i) __attribute__((always_inline)) {
+                        return rd.along(i.value % 2 ? buf + kBytes : buf, kb, i.value / 2);
+                    },
+                    [&](auto i, const AttnPair<SPLIT>& x) __attribute__((always_inline)) {
+                        if constexpr (i.value % 2 == 0)
+                            s = attn_dot<SPLIT>(x, qf[i.value / 2], s);
+                        else dp = attn_dot<SPLIT>(x, of[i.value / 2], dp);
+                    });
                 const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
                 const int away = q + shift - key0;
                 bool near = false;
@@ -423,16 +456,20 @@ attn_dq_kernel(const AttnArgs g) {
                 if constexpr (BIAS) {
                     const int lo = wave0 + shift - key0 - 31, hi = lo + 62;
                     near = lo < md && hi > -md;
-                    flat = bias_row[lo >= md ? 2 * md : 0];
+                    flat = bias_row[kAttnFar + (lo >= md ? 2 * md : 0)];
                 }
+                const float* const near_at = BIAS ? bias_row + md + kAttnFar +
+                                                        (near ? away - 4 * (lane >> 5) : 27) - 27
+                                                  : nullptr;
                 float ds[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float add = -lse;
+                    float p;
                     if constexpr (BIAS)
-                        add += near ? bias_row[md + attn_clamp(away - attn_row(r, lane), md)]
-                                    : flat;
-                    const float p = attn_exp2(__builtin_fmaf(s[r], c, add));
+                        p = attn_exp2(__builtin_fmaf(s[r], c,
+                                                     near ? near_at[27 - 8 * (r >> 2) - (r & 3)]
+                                                          : flat) - lse) * inv;
+                    else p = attn_exp2(__builtin_fmaf(s[r], c, -lse));
                     ds[r] = p * __builtin_fmaf(dp[r], alpha, -db);
                 }
                 if (masked) {
@@ -474,8 +511,9 @@ attn_dq_kernel(const AttnArgs g) {
                         else below += y;
                     }
                 }
-                AttnPair<SPLIT> w[2] = {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)};
-                attn_accumulate<SPLIT, DB>(rd, buf, kb, w, dq);
+                const AttnPair<SPLIT> w[1][2] = {
+                    {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)}};
+                attn_accumulate<SPLIT, DB, 1>(rd, buf, kb, w, dq);
             }
         };
         auto stage = [&](const unsigned char* cur, unsigned char* next, int kt) __attribute__((always_inline)) {
@@ -619,7 +657,8 @@ int launch(const AttnArgs& g, const AttnPlan& kplan, int64_t q_entries, int64_t 
         a.tiles = k_tiles;
         const dim3 grid(static_cast<unsigned>(k_entries * g.kv_heads * g.dkv_parts));
         hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS>), grid, dim3(kAttnThreads),
-                           width * sizeof(float), st, a);
+                           BIAS ? attn_bias_floats(g.bias.max_distance) * sizeof(float) : 0, st,
+                           a);
         const int rc = check_launch("attention_backward: dk, dv");
         if (rc != SLK_OK) return rc;
         if (g.dkv_parts > 1) {
@@ -633,7 +672,10 @@ int launch(const AttnArgs& g, const AttnPlan& kplan, int64_t q_entries, int64_t 
     if (want_q) {
         hipLaunchKernelGGL((attn_dq_kernel<SPLIT, DB, BIAS>),
                            dim3(static_cast<unsigned>(q_entries * g.heads)), dim3(kAttnThreads),
-                           BIAS ? (5 * width + 8 + 4 * kDiags * kDiagRow) * sizeof(float) : 0, st, g);
+                           BIAS ? (attn_bias_floats(g.bias.max_distance) + 4 * width + 8 +
+                                   4 * kDiags * kDiagRow) * sizeof(float)
+                                : 0,
+                           st, g);
         return check_launch("attention_backward: dq");
     }
     return SLK_OK;

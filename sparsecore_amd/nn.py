@@ -35,8 +35,9 @@ class SparseLinear(nn.Module):
             move it to the GPU with ``.cuda()`` before running it).
         save_bits: 32 (default), or 8 to keep the input of a forward pass in 8 bits until
             its backward, which computes the weights' gradient from them: a quarter of the
-            memory. 256 tokens of a feature share a scale and each value is off by at most
-            1/254 of their largest; output and input gradient stay as they are.
+            memory. 256 consecutive values (tokens of a feature, then of the next) share a
+            scale and each is off by at most 1/254 of their largest; output and input
+            gradient stay as they are.
 
     Shape: input (*, in_features) -> output (*, out_features).
     """

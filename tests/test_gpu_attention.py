@@ -423,3 +423,43 @@ def test_offsets_out_of_range_are_clamped(dev):
 
 def test_buckets():
     assert relative_buckets(16, 128) == (0, 1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 23, 32, 46, 64, 91)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [torch.finfo(F32).min, -float("inf")])
+def test_biases_that_hide(dev, dtype, value):
+    """Buckets of the type's lowest value, and of minus infinity: what has another key to look
+    at does not see them. Of the lowest value, a row that has nothing else sees all alike."""
+    b, t, h, d = 1, 150, 2, 64
+    q, k, v, do = make((b, t), (b, t), h, h, d, dtype, dev)
+    bias = torch.randn(8, h, device=dev)
+    bias[3:6] = value  # distances 3 to ..
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5, bias.clamp(min=-1e30), 20)
+    leaves = [x.requires_grad_() for x in (q, k, v, bias)]
+    out = slk.attention(q, k, v, bias=bias, max_distance=20)
+    for n, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        got = x.detach().double().cpu().reshape(ref.val[n].shape)
+        assert got.isfinite().all(), n
+        off = (got - ref.val[n]).norm() / ref.val[n].norm()
+        assert float(off) <= (1e-5 if dtype is F32 else 2.0 ** -7), n
+    with torch.no_grad():
+        all_low = torch.full_like(bias, value)
+        out = slk.attention(q, k, v, bias=all_low, max_distance=20)
+        if value > -float("inf"):
+            mean = torch.cumsum(v.double(), 1) / torch.arange(1, t + 1, device=dev)[:, None, None]
+            torch.testing.assert_close(out.double(), mean, rtol=2 ** -7, atol=2 ** -7)
+        else:
+            assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_packed_without_gradients_feature_major(dev, dtype):
+    lens = [70, 1, 0, 200, 33]
+    n = sum(lens) + 9
+    q, k, v, do = make((n,), (n,), 4, 2, 64, dtype, dev, layout="cols")
+    off = torch.tensor([0] + lens).cumsum(0)
+    ref = Ref(q, k, v, do, [(int(a), m, int(a), m) for a, m in zip(off, lens)], True, 0.125)
+    with torch.no_grad():
+        out = slk.attention(q, k, v, offsets=off.int().to(dev), feature_major=True)
+    close("out", out, ref, dtype)
+    assert out.stride(0) == 1 and out.flatten(1).t().is_contiguous()
