@@ -190,8 +190,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     row that belongs to no sequence; what is masked reaches nothing, whatever it holds. A row
     of q, k, v or of the output's gradient with a value that is not finite makes NaN of the
     results that its row has a part in (for few queries without gradients, of what the value
-    itself reaches). Offsets and lengths are read on the device: those out of range, or offsets that fall, count as
-    the nearest that do not.
+    itself reaches). Offsets and lengths are read on the device: those out of range, or
+    offsets that fall, count as the nearest that do not.
 
     Products run on the matrix cores' float16 instructions, each block of 64 rows of a head
     scaled by a power of two of its own. float32 operands go in two parts: an element keeps

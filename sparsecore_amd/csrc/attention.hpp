@@ -191,6 +191,14 @@ __device__ __forceinline__ f32x16 attn_dot(const AttnPair<SPLIT>& a, const AttnP
     return attn_mfma(a.f[0], b.f[0], c);
 }
 
+// The same with the products of the small parts in a sum of their own.
+__device__ __forceinline__ f32x16 attn_dot_apart(const AttnPair<true>& a, const AttnPair<true>& b,
+                                                 f32x16 c, f32x16& small) {
+    small = attn_mfma(a.f[1], b.f[0], small);
+    small = attn_mfma(a.f[0], b.f[1], small);
+    return attn_mfma(a.f[0], b.f[0], c);
+}
+
 // Copies bytes of a tile into LDS in pieces of 1 KB, wave by wave.
 template <int BYTES>
 __device__ __forceinline__ void attn_stage(const char* from, unsigned char* to, int wv,

@@ -437,9 +437,12 @@ attn_dq_kernel(const AttnArgs g) {
                 const int x = kAttnUnit - b + max(b + ke - ck, -60);
                 const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit);
                 const float db = delta * attn_pow2(x);
-                f32x16 s, dp;
+                // The matrix cores' sums err downwards, which the bias's gradient, a sum
+                // of many dS that cancel, would collect: its small products go apart.
+                constexpr bool kApart = SPLIT && BIAS;
+                f32x16 s, dp, small;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+                for (int r = 0; r < 16; ++r) s[r] = dp[r] = small[r] = 0.0f;
                 attn_pipeline<SPLIT, 2 * KS, kAttnAhead<SPLIT>>(
                     [&](auto i) __attribute__((always_inline)) {
                         return rd.along(i.value % 2 ? buf + kBytes : buf, kb, i.value / 2);
@@ -447,8 +450,14 @@ attn_dq_kernel(const AttnArgs g) {
                     [&](auto i, const AttnPair<SPLIT>& x) __attribute__((always_inline)) {
                         if constexpr (i.value % 2 == 0)
                             s = attn_dot<SPLIT>(x, qf[i.value / 2], s);
+                        else if constexpr (kApart)
+                            dp = attn_dot_apart(x, of[i.value / 2], dp, small);
                         else dp = attn_dot<SPLIT>(x, of[i.value / 2], dp);
                     });
+                if constexpr (kApart) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] += small[r];
+                }
                 const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
                 const int away = q + shift - key0;
                 bool near = false;

@@ -37,8 +37,9 @@ __device__ int64_t scan(int64_t x, int64_t* lds, int64_t& last) {
 }
 
 // One workgroup, as each sequence's place follows from those before it: 16 us for 23
-// sequences of 8191 tokens, its loads and barriers one after the other. Offsets that fall, or pass the arrays' end, are taken as the
-// nearest ones that do not: no row is written twice or outside.
+// sequences of 8191 tokens, its loads and barriers one after the other. Offsets that
+// fall, or pass the arrays' end, are taken as the nearest ones that do not: no row is
+// written twice or outside.
 __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanArgs a) {
     __shared__ int64_t lds[kPlanThreads / 64], ends[2];
     __shared__ int32_t bin[kBins];

@@ -463,3 +463,19 @@ def test_packed_without_gradients_feature_major(dev, dtype):
         out = slk.attention(q, k, v, offsets=off.int().to(dev), feature_major=True)
     close("out", out, ref, dtype)
     assert out.stride(0) == 1 and out.flatten(1).t().is_contiguous()
+
+
+def test_bias_gradient_of_many_pairs(dev):
+    """The last bucket holds most pairs, and their dS cancel. dP, a sum of d products of
+    normal values, is about sqrt(d) and off by 2^-23 of it or so; a row's weights sum to 1,
+    and so is its sum of dS. At random that makes sqrt(rows) of them, four times for what is
+    rare; an error of one sign would add up over all rows."""
+    b, t, h, d = 16, 512, 4, 64
+    q, k, v, do = make((b, t), (b, t), h, h, d, F32, dev)
+    bias = torch.randn(32, h, device=dev)
+    leaves = [x.requires_grad_() for x in (q, k, v, bias)]
+    out = slk.attention(q, k, v, bias=bias)
+    got = torch.autograd.grad(out, leaves, do)[3]
+    # every row's dS sum to 0, so all buckets of a head do
+    most = 4 * 2.0 ** -23 * d ** 0.5 * (b * t) ** 0.5
+    assert float(got.double().sum(0).abs().max()) <= most
