@@ -200,7 +200,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     11 bits between the products. Softmax and sums are float32, in a fixed order: results
     repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
     packed (not the tensors themselves), and the output, which must not change in place
-    before the backward, nor may offsets and lengths.
+    before the backward, nor may offsets and lengths; of a bfloat16 output also what its
+    rounding took off, in two bytes an element.
 
     Raises TypeError (not a tensor), RuntimeError (not on the HIP device) and ValueError
     (shape, dtype, sizes).

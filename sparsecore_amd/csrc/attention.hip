@@ -95,6 +95,7 @@ Plan take_plan(Carver& c, const slk_attention& a, const Sizes& s) {
 struct Saved {
     Plan plan;
     float *lse, *inv, *bias_rows;
+    char* o_rest;
     Packed q, k, v;
     int64_t bytes;
 };
@@ -109,6 +110,8 @@ Saved saved_of(const slk_attention& a, void* base) {
         r.inv = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
         r.bias_rows = static_cast<float*>(c.take(a.heads * (2 * a.max_distance + 1) * 4));
     }
+    if (a.dtype == SLK_BF16)
+        r.o_rest = static_cast<char*>(c.take(a.heads * s.pad_q * 64 * blocks_of(a.dim)));
     r.q = take_packed(c, s, a.heads, s.pad_q);
     r.k = take_packed(c, s, a.kv_heads, s.pad_k);
     r.v = take_packed(c, s, a.kv_heads, s.pad_k);
@@ -251,7 +254,10 @@ bool four_features(const slk_attn_tensor& t, const slk_attention& a) {
 }
 
 AttnVec vec_of(const slk_attn_tensor& t, const slk_attention& a) {
-    return four_features(t, a)                                           ? kVecFeatures
+    const bool eight = a.dtype == SLK_BF16 && t.feature == 1 && aligned_to(t.p, 16) &&
+                       (a.dim | t.row | t.head | t.batch) % 8 == 0;
+    return eight                                                         ? kVecEight
+           : four_features(t, a)                                         ? kVecFeatures
            : fours(t, t.row, t.feature, t.head, t.batch, a.dtype)        ? kVecRows
                                                                          : kVecNone;
 }
@@ -493,6 +499,7 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     g.v = op_of(f.saved.v, s, s.pad_k);
     g.lse = f.saved.lse;
     g.inv = f.saved.inv;
+    g.o_rest = a.keep ? f.saved.o_rest : nullptr;
     g.splits = f.splits;
     g.part = f.part;
     g.part_ml = f.part_ml;
@@ -524,6 +531,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
         p.op[0] = pack_op(a.dout, b.dout, s, a, false, a.heads);
         p.o = io_of(a.out);
         p.o_vec = vec_of(a.out, a);
+        p.o_rest = sv.o_rest;
         p.delta = b.delta;
         p.delta_sh = s.pad_q;
         p.lse = sv.lse;

@@ -22,7 +22,7 @@
 // zeros (masked, they would make 0 · inf of a zero weight) and their rows noted:
 // the forward makes NaN of what sees them, log-sums included, from which the
 // backward's weights are NaN in their turn. bfloat16 products would save the packing
-// (a twentieth of a long sequence's time), but weights and their gradients would
+// (a fiftieth of a long sequence's time), but weights and their gradients would
 // be rounded to 8 bits on the way: errors of the gradients of 1.7 times the
 // rounding of the result alone.
 #pragma once
@@ -142,6 +142,7 @@ struct AttnArgs {
     float* delta;          // [head][padded row]: rowsum(dO∘O)
     int32_t* dexps;        // [head][padded rows / 64]: exponent of the largest |delta|
     int64_t lse_sh;
+    char* o_rest;          // what rounding to bfloat16 took off O, in bfloat16: see attn_rest_at
     AttnBias bias;
     float* dbias_part;     // [head][padded rows / 64][2·max_distance + 1]
     int64_t dbias_slots;
@@ -327,6 +328,13 @@ __device__ __forceinline__ void attn_accumulate(const AttnReads<SPLIT, DB>& rd,
 // Row (in a block of 32) that register r of a result belongs to.
 __device__ __forceinline__ int attn_row(int r, int lane) {
     return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+}
+
+// Where O's rests of a padded row (of all heads) and a feature lie: for 32 rows and
+// eight features as the lanes of a wave hold them, four each, in one piece. (Row by
+// row the forward took 61 us at 8191 packed tokens, 16 heads of 128, so 57.)
+__device__ __forceinline__ int64_t attn_rest_at(int64_t row, int f, int dp) {
+    return (row / 32 * (dp / 8) + f / 8) * 256 + (f / 4 & 1) * 128 + (row & 31) * 4 + (f & 3);
 }
 
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -17,7 +17,7 @@ constexpr int kWeightUnit = 7;
 // lanes away): the softmax's maximum and sum are the lane's own, and its weights
 // are the operand of O^T = V^T·P^T as they are. The row's maximum is only raised
 // when a new one is more than 2^8 times above. One sequence of 16384, 32 heads over 8
-// of 128, bfloat16, causal: 2.21 ms, 1.00 PFLOP/s (a large library product of bfloat16
+// of 128, bfloat16, causal: 2.23 ms, 0.99 PFLOP/s (a large library product of bfloat16
 // reaches 1.24), bound by the matrix cores and the exponentials between them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
@@ -246,6 +246,20 @@ attn_forward_kernel(const AttnArgs g) {
         }
         if (g.dtype == SLK_F32) attn_store<F32>(g.out, to, fb, lane, g.dim, vec, x, f);
         else attn_store<BF16>(g.out, to, fb, lane, g.dim, vec, x, f);
+        if (g.o_rest != nullptr && q < seq.nq) {
+            const int64_t row = head * g.lse_sh + seq.pq + q;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                float rest[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float y = x[4 * r4 + j] * f;
+                    rest[j] = y - bf16_to_f32(f32_to_bf16(y));
+                }
+                BF16::store4(g.o_rest,
+                             attn_rest_at(row, 32 * fb + 8 * r4 + 4 * (lane >> 5), T::DP), rest);
+            }
+        }
     }
 }
 

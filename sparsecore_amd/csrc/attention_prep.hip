@@ -36,10 +36,10 @@ __device__ int64_t scan(int64_t x, int64_t* lds, int64_t& last) {
     return wv == 0 ? x : both(before, x);
 }
 
-// One workgroup, as each sequence's place follows from those before it: 16 us for 23
-// sequences of 8191 tokens, its loads and barriers one after the other. Offsets that
-// fall, or pass the arrays' end, are taken as the nearest ones that do not: no row is
-// written twice or outside.
+// One workgroup, as each sequence's place follows from those before it: 10 us for 23
+// sequences of 8191 tokens, its loads and barriers one after the other (16 with a
+// thread for all tiles of a sequence). Offsets that fall, or pass the arrays' end, are
+// taken as the nearest ones that do not: no row is written twice or outside.
 __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanArgs a) {
     __shared__ int64_t lds[kPlanThreads / 64], ends[2];
     __shared__ int32_t bin[kBins];
@@ -124,28 +124,32 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(const AttnPlanA
     __syncthreads();
     // tiles by falling work, counted in classes of blocks of 64 on the other side
     const int total = static_cast<int>(a.n) + (packed ? 2 : 0);
-    const bool one_each = total <= kPlanThreads;  // a thread keeps its sequence
-    const AttnSeq own = one_each && t < total ? a.seqs[t] : AttnSeq{};
+    // threads of a sequence, over its tiles; one that has only one sequence keeps it
+    int team = 1;
+    while (team < 64 && 2 * team * total <= kPlanThreads) team *= 2;
+    const int first_s = t / team, at = t % team, step = kPlanThreads / team;
+    const bool one_each = total <= step;
+    const AttnSeq own = one_each && first_s < total ? a.seqs[first_s] : AttnSeq{};
     for (int side = 0; side < 2; ++side) {
         // the map from tiles of 64 padded rows to sequences, -1 past the last one's
         int32_t* const map = side ? a.k_map : a.q_map;
         const int64_t have = a.count[2 * side + 1] / kAttnRows;
         for (int64_t i = have + t; i < (side ? a.k_tiles : a.q_tiles); i += kPlanThreads)
             map[i] = -1;
-        for (int s = t; s < static_cast<int>(a.n); s += kPlanThreads) {
+        for (int s = first_s; s < static_cast<int>(a.n); s += step) {
             const AttnSeq x = one_each ? own : a.seqs[s];
             const int first = (side ? x.pk : x.pq) / kAttnRows;
             const int tiles = ((side ? x.nk : x.nq) + kAttnRows - 1) / kAttnRows;
-            for (int i = 0; i < tiles; ++i) map[first + i] = s;
+            for (int i = at; i < tiles; i += team) map[first + i] = s;
         }
         int2* list = side ? a.k_list : a.q_list;
         if (list == nullptr) continue;
         auto each = [&](auto&& f) {
-            for (int s = t; s < total; s += kPlanThreads) {
+            for (int s = first_s; s < total; s += step) {
                 const AttnSeq x = one_each ? own : a.seqs[s];
                 const int shift = x.nk - x.nq;
                 const int tiles = ((side ? x.ek : x.eq) + kTileRows - 1) / kTileRows;
-                for (int i = 0; i < tiles; ++i) {
+                for (int i = at; i < tiles; i += team) {
                     int w;
                     if (side) {
                         w = x.nk <= i * kTileRows ? 0
@@ -199,31 +203,79 @@ struct TileRegs {
         }
     }
     // `at`: the first element; `row`: its row in the tensor (four rows are loaded at
-    // once where it is a multiple of four and vec says that the rest is).
+    // once where it is a multiple of four and vec says that the rest is). Pieces past
+    // the last row or feature load the first instead: no branch, within which a load's
+    // conversion would have to wait for it.
     __device__ __forceinline__ void load(const AttnIo& x, int64_t at, int64_t row, int live,
                                          int dim, int vec) {
-        const bool four = BY_ROWS ? vec == kVecRows && (row & 3) == 0 : vec == kVecFeatures;
+        auto clear = [&](int k, int h, int n) {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
+            for (int j = 0; j < n; ++j) v[k][h + j] = 0.0f;
+        };
+        if (live <= 0) {
 #pragma unroll
-            for (int h = 0; h < kWide; h += 4) {
-                int r, f;
-                place(k, h, r, f);
-                const int64_t from = at + r * x.sr + f * x.sd;
-                const bool whole = BY_ROWS ? r + 4 <= live && f < dim : r < live && f + 4 <= dim;
-                if (four && whole) {
-                    IO::load4(x.p, from, v[k] + h);
-                } else {
+            for (int k = 0; k < kPer; ++k) clear(k, 0, kWide);
+            return;
+        }
+        if constexpr (!BY_ROWS && IO::kBytes == 2) {
+            if (vec == kVecEight) {
+                uint4 raw[kPer];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    int r, f;
+                    place(k, 0, r, f);
+                    raw[k] = *reinterpret_cast<const uint4*>(
+                        x.p + 2 * (at + (r < live ? r : 0) * x.sr + (f < dim ? f : 0)));
+                }
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    int r, f;
+                    place(k, 0, r, f);
+                    const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const bool in =
-                            BY_ROWS ? r + j < live && f < dim : r < live && f + j < dim;
-                        v[k][h + j] =
-                            in ? IO::load(x.p, from + j * (BY_ROWS ? x.sr : x.sd)) : 0.0f;
+                        v[k][2 * j] = bf16_to_f32(w[j] & 0xffffu);
+                        v[k][2 * j + 1] = bf16_to_f32(w[j] >> 16);
                     }
+                    if (r >= live || f >= dim) clear(k, 0, kWide);
                 }
+                return;
             }
         }
+        const bool four = BY_ROWS ? vec == kVecRows && ((row | live) & 3) == 0
+                                  : vec == kVecFeatures || vec == kVecEight;
+        if (four) {
+            using Raw = std::conditional_t<IO::kBytes == 4, f32x4, uint2>;
+            Raw raw[kPer][kWide / 4];
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                for (int h = 0; h < kWide; h += 4) {
+                    int r, f;
+                    place(k, h, r, f);
+                    raw[k][h / 4] = *reinterpret_cast<const Raw*>(
+                        x.p + IO::kBytes * (at + (r < live ? r : 0) * x.sr +
+                                            (f < dim ? f : 0) * x.sd));
+                }
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                for (int h = 0; h < kWide; h += 4) {
+                    int r, f;
+                    place(k, h, r, f);
+                    IO::load4(&raw[k][h / 4], 0, v[k] + h);
+                    if (r >= live || f >= dim) clear(k, h, 4);
+                }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) {
+                int r, f;
+                place(k, j, r, f);
+                v[k][j] = r < live && f < dim ? IO::load(x.p, at + r * x.sr + f * x.sd) : 0.0f;
+            }
     }
 };
 
@@ -244,8 +296,9 @@ __device__ __forceinline__ int tile_exponent(uint32_t top) {
 // an operand; one more y for the rows of biases, a head each. Of dO (with delta
 // given) also delta, from the same tile and O's. Rows of consecutive features go
 // from registers to their place; consecutive rows are turned through LDS. What
-// bounds it is memory: 16384 tokens, 48 heads of 128 in all, bfloat16: 119 us, 3.4
-// TB/s; with delta, 32 heads: 131 us, 3.1 TB/s.
+// bounds it is memory: 16384 tokens, 48 heads of 128 in all, bfloat16: 80 us, 5.0
+// TB/s (with a branch around each load and eight bytes a load 119); with delta, 32
+// heads: 124 us, 4.3 TB/s.
 template <bool SPLIT, int DB, class IO, bool DELTA, bool BY_ROWS>
 __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& op, int head,
                                           const AttnRow& ro) {
@@ -266,6 +319,30 @@ __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& o
     // O in the same pieces as dO, whatever its own order
     if constexpr (DELTA)
         out.load(a.o, ro.sid * a.o.sb + row * a.o.sr + head * a.o.sh, row, live, a.dim, a.o_vec);
+    if (DELTA && IO::kBytes == 2 && live > 0) {
+        // delta from O before it was rounded: dP - delta cancels, most so in rows that
+        // see few keys.
+        const int64_t top = head * a.delta_sh + padded;
+#pragma unroll
+        for (int k = 0; k < Regs::kPer; ++k)
+#pragma unroll
+            for (int h = 0; h < Regs::kWide; h += 4) {
+                int r, f;
+                Regs::place(k, h, r, f);
+                float x[4];
+                if constexpr (BY_ROWS) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[j] = IO::load(a.o_rest,
+                                        attn_rest_at(top + (r + j < live ? r + j : 0), f, DP));
+                } else {
+                    IO::load4(a.o_rest, attn_rest_at(top + (r < live ? r : 0), f, DP), x);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    out.v[k][h + j] += r + (BY_ROWS ? j : 0) < live ? x[j] : 0.0f;
+            }
+    }
     if (t < 2) odd[t] = 0;
     __syncthreads();
     float d[Regs::kWide];  // BY_ROWS: a thread's share of four rows' delta

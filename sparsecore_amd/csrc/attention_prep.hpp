@@ -17,8 +17,8 @@ struct AttnPlanArgs {
     int32_t causal, work_shift;
 };
 
-// How a pack reads four elements at once: not, four features, four rows.
-enum AttnVec { kVecNone = 0, kVecFeatures = 1, kVecRows = 2 };
+// What a pack reads at once: an element, four features, four rows, eight features.
+enum AttnVec { kVecNone = 0, kVecFeatures = 1, kVecRows = 2, kVecEight = 3 };
 
 struct AttnPackOp {
     AttnIo src;
@@ -37,6 +37,7 @@ struct AttnPack {
     AttnBias bias;   // with a table: its rows are made too
     AttnIo o;        // with delta: op[0] is dO, this is O
     int32_t o_vec;
+    char* o_rest;    // what rounding took off O (bfloat16)
     float* delta;
     const float* lse;
     float* lse_out;  // lse, NaN where a row of dO is not finite

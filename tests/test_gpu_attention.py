@@ -479,3 +479,42 @@ def test_bias_gradient_of_many_pairs(dev):
     # every row's dS sum to 0, so all buckets of a head do
     most = 4 * 2.0 ** -23 * d ** 0.5 * (b * t) ** 0.5
     assert float(got.double().sum(0).abs().max()) <= most
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("start", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("d,gap", [(64, 8), (40, 4), (36, 0), (128, 1)])
+def test_alignment(dev, d, gap, start, dtype):
+    """Rows that begin at any element, heads a few elements apart: the same bits."""
+    b, t, h = 2, 70, 2
+    q, k, v, do = make((b, t), (b, t), h, h, d, dtype, dev)
+
+    def shifted(x):
+        buf = torch.full((b, t, h, d + gap), float("nan"), dtype=dtype, device=dev).flatten()
+        buf = torch.cat([buf.new_full((start,), float("nan")), buf])
+        y = buf[start:].view(b, t, h, d + gap)[..., :d]
+        y.copy_(x)
+        return y
+
+    want = [x.clone().requires_grad_() for x in (q, k, v)]
+    got = [shifted(x).requires_grad_() for x in (q, k, v)]
+    a, c = slk.attention(*want), slk.attention(*got)
+    assert torch.equal(a, c)
+    for x, y in zip(torch.autograd.grad(a, want, do), torch.autograd.grad(c, got, shifted(do))):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("t", [2, 3])
+def test_gradients_of_rows_with_few_keys(dev, t):
+    """dP - rowsum(dO∘O) cancels where a row sees few keys: with O as it is rounded to
+    bfloat16 these gradients were off by 0.004. A rounded result is off by anything up to
+    2^-8 of itself, 2^-8 / sqrt(3) in the mean; weights and their gradients by 2^-12."""
+    b, h, d = 400, 1, 64
+    q, k, v, do = make((b, t), (b, t), h, h, d, BF16, dev)
+    ref = Ref(q, k, v, do, [(i, t, i, t) for i in range(0, b * t, t)], True, d ** -0.5)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(slk.attention(*leaves), leaves, do)
+    for n, x in zip(("dq", "dk", "dv"), got):
+        want = ref.val[n]
+        off = (x.double().cpu().reshape(want.shape) - want).norm() / want.norm()
+        assert float(off) <= 2.0 ** -8 / 3 ** 0.5 + 2.0 ** -12, n
