@@ -939,10 +939,10 @@ typedef struct slk_attn_tensor {
  * 2^-39 of the largest of those rows), bf16 exact down to 2^-31 of it, weights
  * and their gradients in 11 bits. Softmax statistics and sums are float32, in a
  * fixed order.
- *   keep       1 where a backward follows: forward leaves log-sums and packed
- *              operands in saved (slk_attention_saved_bytes); backward takes the
- *              same arguments, out and saved as forward left them (q, k and v are
- *              not read)
+ *   keep       1 where a backward follows: forward leaves log-sums, packed
+ *              operands and what rounding took off a bf16 output in saved
+ *              (slk_attention_saved_bytes); backward takes the same arguments, out
+ *              and saved as forward left them (q, k and v are not read)
  *   scratch    slk_attention_scratch_bytes; saved and scratch 16-byte aligned
  * backward: dq, and dk with dv, where not NULL; dbias (as bias) where not NULL.  */
 #define SLK_ATTN_MAX_DIM 128

@@ -360,9 +360,9 @@ int check(const slk_attention* args, const char* who, bool backward) {
     if (a.dim < 1 || a.dim > SLK_ATTN_MAX_DIM)
         return fail(SLK_EINVAL, w + ": dim in [1, " + std::to_string(SLK_ATTN_MAX_DIM) +
                                     "], got " + std::to_string(a.dim));
-    // queries', keys', values' and biases' heads are one grid's second dimension
-    if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.heads > 16383)
-        return fail(SLK_EINVAL, w + ": heads must be a multiple of kv_heads, at most 16383, got " +
+    // heads of queries, keys and values are one grid's second dimension
+    if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.heads > 16384)
+        return fail(SLK_EINVAL, w + ": heads must be a multiple of kv_heads, at most 16384, got " +
                                     std::to_string(a.heads) + " and " +
                                     std::to_string(a.kv_heads));
     if (!(a.scale >= 0.0) || !(a.scale <= 3e38))
