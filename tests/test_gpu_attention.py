@@ -518,3 +518,40 @@ def test_gradients_of_rows_with_few_keys(dev, t):
         want = ref.val[n]
         off = (x.double().cpu().reshape(want.shape) - want).norm() / want.norm()
         assert float(off) <= 2.0 ** -8 / 3 ** 0.5 + 2.0 ** -12, n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", [[150], [3, 130, 1, 70]])
+def test_gradients_where_all_biases_are_the_lowest_value(dev, dtype, lens):
+    """Such a bias swallows every score: all keys that a query sees weigh the same, which is
+    what queries of zeros make of them; dq and dv do not depend on the queries otherwise."""
+    n, h, d = sum(lens), 2, 64
+    q, k, v, do = make((n,), (n,), h, h, d, dtype, dev)
+    off = torch.tensor([0] + lens).cumsum(0)
+    seqs = [(int(a), m, int(a), m) for a, m in zip(off, lens)]
+    ref = Ref(torch.zeros_like(q), k, v, do, seqs, True, d ** -0.5)
+    bias = torch.full((8, h), torch.finfo(F32).min, device=dev)
+    leaves = [x.requires_grad_() for x in (q, k, v, bias)]
+    out = slk.attention(q, k, v, offsets=off.int().to(dev), bias=bias, max_distance=20)
+    dq, dk, dv, dbias = torch.autograd.grad(out, leaves, do)
+    assert dk.isfinite().all() and dbias.isfinite().all()
+    for name, x in (("out", out), ("dq", dq), ("dv", dv)):
+        want = ref.val[name]
+        off_by = (x.detach().double().cpu().reshape(want.shape) - want).norm() / want.norm()
+        assert float(off_by) <= (1e-5 if dtype is F32 else 2.0 ** -8), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_sequences_than_the_plan_has_threads(dev, dtype):
+    """1100 sequences, some empty, one with more tiles than the others together."""
+    gen = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 4, (1100,), generator=gen).tolist()
+    lens[517] = 700
+    n = sum(lens) + 3
+    q, k, v, do = make((n,), (n,), 2, 1, 32, dtype, dev)
+    off = torch.tensor([0] + lens).cumsum(0)
+    ref = Ref(q, k, v, do, [(int(a), m, int(a), m) for a, m in zip(off, lens)], True, 32 ** -0.5)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(q, k, v, offsets=off.int().to(dev))
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        close(name, x, ref, dtype)
