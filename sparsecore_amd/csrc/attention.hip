@@ -471,8 +471,10 @@ extern "C" int slk_attention_forward(const slk_attention* args, void* stream) {
     int rc = check(args, "attention_forward", false);
     if (rc != SLK_OK) return rc;
     const slk_attention& a = *args;
-    if (a.rows_q == 0 || (a.n == 0 && !packed_rows(a))) return SLK_OK;
+    if (a.n == 0 && !packed_rows(a)) return SLK_OK;
     const hipStream_t st = as_stream(stream);
+    // without queries too the backward has keys' gradients to write, by the plan's list
+    if (a.rows_q == 0) return a.keep ? make_plan(a, saved_of(a, a.saved).plan, st) : SLK_OK;
     const Forward f = forward_of(a, a.scratch);
     if (few_rows(a)) return few_forward(a, f, st);
     const Sizes s = sizes_of(a);

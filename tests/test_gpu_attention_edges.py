@@ -1,0 +1,91 @@
+"""attention at its edges: calls without queries, whose keys' and biases' gradients are zeros."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import sparsecore_amd as slk
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def leave_garbage(dev, nbytes=1 << 20):
+    """Freed blocks of several sizes that hold ones in every bit: what the next call's saved
+    and scratch memory may hold."""
+    sizes = [nbytes >> i for i in range(12)]
+    blocks = [torch.full((n,), 0xff, dtype=torch.uint8, device=dev) for n in sizes for _ in "123"]
+    torch.cuda.synchronize()
+    del blocks
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("buckets", [0, 8])
+@pytest.mark.parametrize("h,g,s", [(2, 2, 7), (4, 1, 300), (6, 2, 129)])
+@pytest.mark.parametrize("mode", ["whole", "lengths", "k_lengths", "packed"])
+def test_no_queries_in_any_layout(dev, mode, h, g, s, buckets, causal, dtype):
+    leave_garbage(dev)
+    d, b = 32, 3
+    lead_q, lead_k = ((0,), (3 * s,)) if mode == "packed" else ((b, 0), (b, s))
+    q = torch.randn(*lead_q, h, d, device=dev).to(dtype).requires_grad_()
+    k, v = (torch.randn(*lead_k, g, d, device=dev).to(dtype).requires_grad_() for _ in range(2))
+    bias = torch.randn(buckets, h, device=dev, requires_grad=True) if buckets else None
+    ints = torch.tensor([s, 0, s // 2], dtype=torch.int32, device=dev)
+    more = {"whole": {}, "lengths": {"lengths": torch.zeros_like(ints), "k_lengths": ints},
+            "k_lengths": {"k_lengths": ints},
+            "packed": {"offsets": torch.zeros(4, dtype=torch.int32, device=dev),
+                       "k_offsets": torch.tensor([2, s, s, 2 * s], dtype=torch.int32,
+                                                 device=dev)}}[mode]
+    out = slk.attention(q, k, v, causal=causal, bias=bias, max_distance=20, **more)
+    assert out.shape == q.shape
+    leaves = [q, k, v] + ([bias] if buckets else [])
+    grads = torch.autograd.grad(out, leaves, torch.empty_like(out))
+    for x, y in zip(grads, leaves):
+        assert x.shape == y.shape and x.dtype == y.dtype and (x == 0).all()
+
+
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_packed_batch_of_nothing(dev, buckets):
+    """No sequences, and sequences that are all empty, with rows of none behind them."""
+    for off in ([0], [0, 0, 0], [4, 4]):
+        for rows in (0, 9):
+            leave_garbage(dev)
+            x = torch.randn(rows, 2, 32, device=dev, requires_grad=True)
+            bias = torch.randn(buckets, 2, device=dev, requires_grad=True) if buckets else None
+            out = slk.attention(x, x, x, bias=bias, max_distance=20,
+                                offsets=torch.tensor(off, dtype=torch.int32, device=dev))
+            leaves = [x] + ([bias] if buckets else [])
+            assert (out == 0).all()
+            for g, y in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), leaves):
+                assert g.shape == y.shape and (g == 0).all()
+
+
+def test_no_queries_captured(dev):
+    """The same in a graph, replayed with other lengths."""
+    k, v = (torch.randn(2, 70, 2, 64, device=dev, requires_grad=True) for _ in range(2))
+    q = torch.randn(2, 0, 2, 64, device=dev)
+    n = torch.tensor([70, 3], dtype=torch.int32, device=dev)
+
+    def step():
+        out = slk.attention(q, k, v, k_lengths=n)
+        return torch.autograd.grad(out, [k, v], torch.empty_like(out))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        for x in got:
+            x.fill_(1.0)
+        n.copy_(torch.tensor([20 * i, 70 - i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all((x == 0).all() for x in got)
