@@ -943,7 +943,8 @@ typedef struct slk_attn_tensor {
  *              operands and what rounding took off a bf16 output in saved
  *              (slk_attention_saved_bytes); backward takes the same arguments, out
  *              and saved as forward left them (q, k and v are not read)
- *   scratch    slk_attention_scratch_bytes; saved and scratch 16-byte aligned
+ *   scratch    slk_attention_scratch_bytes; saved and scratch 16-byte aligned. Both sizes
+ *              are 0 for sizes that forward and backward refuse
  * backward: dq, and dk with dv, where not NULL; dbias (as bias) where not NULL.  */
 #define SLK_ATTN_MAX_DIM 128
 #define SLK_ATTN_MAX_BUCKETS 128

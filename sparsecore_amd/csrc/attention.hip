@@ -350,6 +350,27 @@ AttnArgs args_of(const slk_attention& a, float* bias_rows) {
     return g;
 }
 
+// Heads of queries, keys and values are one grid's second dimension.
+bool heads_fit(const slk_attention& a) {
+    return a.heads >= 1 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.heads <= 16384;
+}
+
+// Padded rows of all heads are counted in 64 bits, rows in 32. Rows and sequences are
+// bounded before they are multiplied.
+bool rows_fit(const slk_attention& a) {
+    if (a.n > INT32_MAX / 64 || a.rows_q > INT32_MAX / 2 || a.rows_k > INT32_MAX / 2) return false;
+    const Sizes s = sizes_of(a);
+    return s.pad_q <= INT32_MAX / 2 && s.pad_k <= INT32_MAX / 2;
+}
+
+// Whether memory can be counted for these arguments; check() says what is wrong with others.
+bool countable(const slk_attention* a) {
+    return a != nullptr && a->n >= 0 && a->rows_q >= 0 && a->rows_k >= 0 && a->dim >= 1 &&
+           a->dim <= SLK_ATTN_MAX_DIM && heads_fit(*a) && rows_fit(*a) &&
+           (a->bias == nullptr ||
+            (a->max_distance >= 1 && a->max_distance <= SLK_ATTN_MAX_DISTANCE));
+}
+
 int check(const slk_attention* args, const char* who, bool backward) {
     const std::string w = who;
     if (args == nullptr) return fail(SLK_EINVAL, w + ": NULL arguments");
@@ -360,8 +381,7 @@ int check(const slk_attention* args, const char* who, bool backward) {
     if (a.dim < 1 || a.dim > SLK_ATTN_MAX_DIM)
         return fail(SLK_EINVAL, w + ": dim in [1, " + std::to_string(SLK_ATTN_MAX_DIM) +
                                     "], got " + std::to_string(a.dim));
-    // heads of queries, keys and values are one grid's second dimension
-    if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.heads > 16384)
+    if (!heads_fit(a))
         return fail(SLK_EINVAL, w + ": heads must be a multiple of kv_heads, at most 16384, got " +
                                     std::to_string(a.heads) + " and " +
                                     std::to_string(a.kv_heads));
@@ -393,11 +413,8 @@ int check(const slk_attention* args, const char* who, bool backward) {
                 return fail(SLK_EINVAL, w + ": bucket_starts must ascend to max_distance at most");
     }
     if (a.n == 0 && !packed_rows(a)) return SLK_OK;
-    // padded rows of all heads are counted in 64 bits, rows in 32
+    if (!rows_fit(a)) return fail(SLK_EINVAL, w + ": too many rows");
     const Sizes s = sizes_of(a);
-    if (a.n > INT32_MAX / 64 || a.rows_q > INT32_MAX / 2 || a.rows_k > INT32_MAX / 2 ||
-        s.pad_q > INT32_MAX / 2 || s.pad_k > INT32_MAX / 2)
-        return fail(SLK_EINVAL, w + ": too many rows");
     if (s.q_entries * a.heads > max_groups(kAttnThreads) ||
         s.k_entries * a.heads > max_groups(kAttnThreads) || s.pad_q > max_groups(kWave) ||
         s.pad_k > max_groups(kAttnThreads) * 32)
@@ -456,11 +473,11 @@ int few_forward(const slk_attention& a, const Forward& f, hipStream_t st) {
 }  // namespace slk
 
 extern "C" int64_t slk_attention_saved_bytes(const slk_attention* args) {
-    return args != nullptr && args->keep ? slk::saved_of(*args, nullptr).bytes : 0;
+    return slk::countable(args) && args->keep ? slk::saved_of(*args, nullptr).bytes : 0;
 }
 
 extern "C" int64_t slk_attention_scratch_bytes(const slk_attention* args, int backward) {
-    if (args == nullptr) return 0;
+    if (!slk::countable(args)) return 0;
     return backward ? slk::backward_of(*args, nullptr).bytes
                     : slk::forward_of(*args, nullptr).bytes;
 }
