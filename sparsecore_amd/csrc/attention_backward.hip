@@ -10,10 +10,51 @@ namespace slk {
 
 namespace {
 
-// Exponent above the largest |dS| of a pair of tiles: |dP| < DP·2^(oe + 1)·2^(ve + 1), and
-// |delta| < 2^(de + 1).
+// dS as a float16 operand. Its parts reach 2^-24, so it is scaled to the size that it has,
+// not to what it might have: a weight of 1 / keys and a dP far below its bound would leave
+// 16 of 22 bits at 8192 keys. Each result row (a lane's) has a unit 2^c of its own; dS goes
+// into the product times 2^(14 + e - c), e the exponent of the other operand's rows. Where
+// a row's largest passes 2^kDsMost, or is below 2^kDsLeast so far, the unit is moved so
+// that it comes to 2^kDsStart, and the sums with it, by powers of two (as the softmax's
+// maximum is raised): in the first tile, and seldom after it. Before that a bound sees to
+// it that nothing leaves float32: |dP - delta| < 2^b scaled stays below 2^kDsReach. That
+// is looked at only where a tile's exponents differ from those it was looked at for.
+constexpr int kDsMost = 15, kDsStart = 7, kDsLeast = 4, kDsReach = 80;
+constexpr int kUnset = -100000;  // the unit of a row that has seen nothing
+
+// Exponent above |dP| < DP·2^(oe + 1)·2^(ve + 1) and |delta| < 2^(de + 1), and their
+// difference. Not below -20: powers of two from it stay in float32.
 __device__ __forceinline__ int ds_exponent(int oe, int ve, int de, int log_dp) {
-    return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -100), 120);
+    return min(max(max(oe + ve + log_dp + 2, de + 1) + 1, -20), 120);
+}
+
+// Whether the largest scaled dS of some lane's row is out of range (0: none so far).
+__device__ __forceinline__ bool ds_out(float most) {
+    // no branches
+    return (most > static_cast<float>(1 << kDsMost)) |
+           ((most > 0.0f) & (most < static_cast<float>(1 << kDsLeast)));
+}
+
+// The unit that brings a row's largest to 2^kDsStart, from it and the present unit; not
+// below `least`.
+__device__ __forceinline__ int ds_unit(float most, int unit, int least) {
+    const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+    return max(unit + e - kDsStart, least);
+}
+
+template <int N>
+__device__ __forceinline__ void scale_sums(f32x16 (&x)[N], float f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[i][r] *= f;
+}
+
+__device__ __forceinline__ float largest(const float (&x)[16]) {
+    float m = fabsf(x[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) m = fmaxf(m, fabsf(x[r]));
+    return m;
 }
 
 // The diagonals of a block of 32 queries x 8 keys: a row of LDS each, eight keys
@@ -24,12 +65,6 @@ constexpr int kDiags = 39, kDiagRow = 12;
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-}
-
-__device__ __forceinline__ int wave_max(int e) {
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) e = max(e, __shfl_xor(e, x));
-    return __builtin_amdgcn_readfirstlane(e);
 }
 
 // 64 floats of a row array into LDS, by one wave.
@@ -55,7 +90,7 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 // turn, or for some of them where a group is spread over workgroups. Scores are
 // Q·K^T here: a lane holds 16 queries of one key, as the operands of
 // dV^T = dO^T·P and dK^T = Q^T·dS need them. One sequence of 16384, 32 heads over 8
-// of 128, bfloat16, causal: 4.84 ms, 0.91 PFLOP/s in its four products; the 512
+// of 128, bfloat16, causal: 5.0 ms, 0.88 PFLOP/s in its four products; the 512
 // registers of a SIMD's lane hold two waves, too few to keep the matrix cores busy
 // while both compute weights.
 template <bool SPLIT, int DB, bool BIAS>
@@ -95,7 +130,9 @@ attn_dkv_kernel(const AttnArgs g) {
     for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[fb][r] = dv[fb][r] = 0.0f;
-    int co = 0, cq = 0;
+    // dV in units of 2^(co - 28), dK of 2^(cq - 28), row by row: the largest exponent of
+    // dO's tiles that the row's key is seen by, and dS's unit
+    int co = kUnset, cq = kUnset;
 
     // stages of queries, from the first that sees a key of the workgroup
     const int first = g.causal ? max(0, tile * 128 - shift) / kRows : 0;
@@ -153,24 +190,12 @@ attn_dkv_kernel(const AttnArgs g) {
             }
         }
         const unsigned char* const my_v = values + (wv >> 1) * kTile;
-        // dV in units of 2^(co - 28), dK of 2^(cq - 28), the largest of the query
-        // tiles that this wave's keys are seen by
         const int ke = attn_exp(g.k, kvh, k_row), ve = attn_exp(g.v, kvh, k_row);
-        co = cq = -400;
-        {
-            const int b0 = g.causal ? max(0, key0 - shift) / 64 : 0, b1 = (seq.nq + 63) / 64;
-            for (int hr = 0; hr < rep; ++hr) {
-                const int64_t at = (head0 + hr) * g.q.exps_sh + q_tile0;
-                for (int i = b0 + lane; i < b1; i += 64) {
-                    const int oe = g.dout.exps[at + i] >> 1;
-                    co = max(co, oe);
-                    cq = max(cq, ds_exponent(oe, ve, g.dexps[at + i], kLogDp) +
-                                     (g.q.exps[at + i] >> 1));
-                }
-            }
-            co = wave_max(co);
-            cq = wave_max(cq);
-        }
+        float run = 0.0f;  // the largest scaled |dS| of the lane's key so far
+        // of the stage that they were set for: weights are times 2^unit, dS times 2^14 and the
+        // row's unit is weight · beta · (dP - delta)
+        float unit = 0.0f, beta = 0.0f;
+        int set_oe = kUnset, set_qe = kUnset, set_b = kUnset;
         const int md = BIAS ? g.bias.max_distance : 0;
 
         auto compute = [&](const unsigned char* buf, int hr, int q_first)
@@ -179,17 +204,23 @@ attn_dkv_kernel(const AttnArgs g) {
             const int qe = attn_exp(g.q, head, row0), oe = attn_exp(g.dout, head, row0);
             const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (row0 >> 6));
             const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
-            // weights times 2^u; dS = weight · (alpha·dp - beta·delta)
-            const int u = kAttnUnit + max(oe - co, -60);
+            const float alpha = attn_pow2(oe + ve - 2 * kAttnUnit);
             const int b = ds_exponent(oe, ve, de, kLogDp);
-            const int x = kAttnUnit - b + max(b + qe - cq, -60) - u;
-            const float unit = static_cast<float>(u);
-            const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit), beta = attn_pow2(x);
+            // the lane's key is seen by rows [from, to) of a block
+            auto seen_from = [&](int q0) { return g.causal ? max(key - shift - q0, 0) : 0; };
+            auto seen_to = [&](int q0) { return key < seq.nk ? min(seq.nq - q0, 32) : 0; };
+            auto move = [&](int to) __attribute__((always_inline)) {  // dK's unit
+                const float f = attn_pow2(cq - to);
+                scale_sums(dk, f);
+                run *= f;
+                cq = to;
+            };
 #pragma unroll
             for (int qb = 0; qb < kRows / 32; ++qb) {
                 const int q0 = q_first + 32 * qb;
                 if (q0 >= seq.nq || (g.causal && q0 + 31 + shift < key0)) continue;
-                const bool masked = q0 + 31 >= seq.nq || (g.causal && q0 + shift < key0 + 31);
+                const bool masked = q0 + 31 >= seq.nq || key0 + 31 >= seq.nk ||
+                                    (g.causal && q0 + shift < key0 + 31);
                 f32x16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
@@ -220,12 +251,27 @@ attn_dkv_kernel(const AttnArgs g) {
                     BIAS ? bias_row + md + kAttnFar + (far ? 0 : q0 + shift - key) +
                                4 * (lane >> 5)
                          : nullptr;
-                // the lane's key is seen by rows [lo, hi) of the block
-                const int lo = g.causal ? key - shift - q0 : 0, hi = seq.nq - q0;
+                if (masked || oe != set_oe || qe != set_qe || b > set_b) {
+                    const bool sees = !masked || seen_from(q0) < seen_to(q0);
+                    if (__builtin_amdgcn_ballot_w64(sees & (oe > co)) != 0) {
+                        const int to = sees ? max(co, oe) : co;
+                        scale_sums(dv, attn_pow2(co - to));
+                        co = to;
+                    }
+                    const int u = kAttnUnit + max(oe - co, -60);
+                    const int to = sees ? max(cq, qe + kAttnUnit - u + b - kDsReach) : cq;
+                    if (__builtin_amdgcn_ballot_w64(to != cq) != 0) move(to + (to != cq ? 14 : 0));
+                    unit = static_cast<float>(u);
+                    beta = attn_pow2(qe + kAttnUnit - u - cq);
+                    set_oe = masked ? kUnset : oe;  // other rows are seen in the next one
+                    set_qe = qe;
+                    set_b = b;
+                }
                 AttnPair<SPLIT> wp[1][2], wd[1][2];
+                float ds[16];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    float p[8], ds[8];
+                    float p[8];
 #pragma unroll
                     for (int r4 = 0; r4 < 2; ++r4) {
                         const int at = 16 * half + 8 * r4, row = at + 4 * (lane >> 5);
@@ -242,21 +288,39 @@ attn_dkv_kernel(const AttnArgs g) {
                                                                 far ? flat : near_at[at + j]) -
                                                  z[j] + unit) * inv[j];
                             else p[i] = attn_exp2(__builtin_fmaf(s[r], c, unit - z[j]));
-                            ds[i] = p[i] * __builtin_fmaf(dp[r], alpha, -(d[j] * beta));
+                            ds[r] = p[i] * beta * __builtin_fmaf(dp[r], alpha, -d[j]);
                         }
                     }
                     if (masked) {
+                        const int lo = seen_from(q0), hi = seen_to(q0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int row = attn_row(8 * half + i, lane);
                             const bool see = row >= lo && row < hi;
                             p[i] = see ? p[i] : 0.0f;
-                            ds[i] = see ? ds[i] : 0.0f;
+                            ds[8 * half + i] = see ? ds[8 * half + i] : 0.0f;
                         }
                     }
                     wp[0][half] = attn_operand<SPLIT>(p);
-                    wd[0][half] = attn_operand<SPLIT>(ds);
                 }
+                run = fmaxf(run, largest(ds));
+                if (__builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
+                    run = fmaxf(run, __shfl_xor(run, 32));  // the key's other half
+                    const bool out = ds_out(run);
+                    const int u = static_cast<int>(unit);
+                    const int to =
+                        out ? ds_unit(run, cq, qe + kAttnUnit - u + b - kDsReach) : cq;
+                    const float f = attn_pow2(cq - to);
+                    move(to);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] *= f;
+                    // where the bound kept it from rising it is not tried again
+                    if (out) run = fmaxf(run, static_cast<float>(1 << kDsLeast));
+                    beta *= f;
+                    set_b = b;
+                }
+                wd[0][0] = attn_operand<SPLIT>(ds);
+                wd[0][1] = attn_operand<SPLIT>(ds + 8);
                 attn_accumulate<SPLIT, DB, 1, kPart>(rd, buf + kBytes, qb, wp, dv);
                 attn_accumulate<SPLIT, DB, 1, kPart>(rd, buf, qb, wd, dk);
             }
@@ -336,7 +400,7 @@ attn_dkv_kernel(const AttnArgs g) {
 // the wave's own bin of that distance, so the sums need no atomicity and repeat.
 // (Float atomics on LDS took some 260 cycles an instruction: the whole kernel 137
 // us, without them 65, at 16 x 512 tokens, 12 heads of 64, float32.) One sequence of
-// 16384, 32 heads over 8 of 128, bfloat16, causal: 2.99 ms, 1.10 PFLOP/s in its three
+// 16384, 32 heads over 8 of 128, bfloat16, causal: 3.0 ms, 1.10 PFLOP/s in its three
 // products, bound by the matrix cores and the softmax's instructions between them.
 template <bool SPLIT, int DB, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
@@ -381,7 +445,8 @@ attn_dq_kernel(const AttnArgs g) {
     for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[fb][r] = 0.0f;
-    int ck = 0;
+    int ck = kUnset;  // dQ in units of 2^(ck - 28), row by row
+    float run = 0.0f;  // the largest scaled |dS| of the lane's query so far
 
     if (t1 > 0) {
         const int64_t k_tile = seq.pk / 64;
@@ -409,19 +474,19 @@ attn_dq_kernel(const AttnArgs g) {
         }
         const bool mine = q < seq.nq;
         const int64_t ri = head * g.lse_sh + q_row + (lane & 31);
-        const float lse = mine ? g.lse[ri] : INFINITY, inv = BIAS && mine ? g.inv[ri] : 0.0f;
+        const float lse = mine ? g.lse[ri] : INFINITY;
+        const float inv = BIAS && mine ? g.inv[ri] : 0.0f;
         const float delta = mine ? g.delta[ri] : 0.0f;
         const int qe = attn_exp(g.q, head, q_row), oe = attn_exp(g.dout, head, q_row);
         const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (q_row >> 6));
-        {
-            const int* ve = g.v.exps + kvh * g.v.exps_sh + k_tile;
-            const int* ke = g.k.exps + kvh * g.k.exps_sh + k_tile;
-            int e = -400;
-            for (int i = lane; i < t1; i += 64)
-                e = max(e, ds_exponent(oe, ve[i] >> 1, de, kLogDp) + (ke[i] >> 1));
-            ck = wave_max(e);
-        }
 
+        int set_b = kUnset;  // the largest exponent, K's counted, that ck was looked at for
+        auto move = [&](int to) __attribute__((always_inline)) {
+            const float f = attn_pow2(ck - to);
+            scale_sums(dq, f);
+            run *= f;
+            ck = to;
+        };
         auto compute = [&](const unsigned char* buf, int key_tile) __attribute__((always_inline)) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
@@ -434,7 +499,13 @@ attn_dq_kernel(const AttnArgs g) {
                 const int ve = attn_exp(g.v, kvh, seq.pk + key0);
                 const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
                 const int b = ds_exponent(oe, ve, de, kLogDp);
-                const int x = kAttnUnit - b + max(b + ke - ck, -60);
+                if (ke + b > set_b) {
+                    const int to = max(ck, ke + b - kDsReach);
+                    if (__builtin_amdgcn_ballot_w64(to != ck) != 0) move(to + (to != ck ? 14 : 0));
+                    set_b = ke + b;
+                }
+                // dS times 2^x: dP and delta are; in the weights' exponent x would round it
+                const int x = kAttnUnit + ke - ck;
                 const float alpha = attn_pow2(x + oe + ve - 2 * kAttnUnit);
                 const float db = delta * attn_pow2(x);
                 // The matrix cores' sums err downwards, which the bias's gradient, a sum
@@ -487,7 +558,6 @@ attn_dq_kernel(const AttnArgs g) {
                         ds[r] = attn_row(r, lane) <= lim ? ds[r] : 0.0f;
                 }
                 if constexpr (BIAS) {
-                    const float back = attn_pow2(-x);
                     if (near) {
                         // eight keys at a time: lane d sums the diagonal of distance
                         // d - 7 from the first key's of the first query
@@ -496,7 +566,8 @@ attn_dq_kernel(const AttnArgs g) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int k = 4 * (lane >> 5) + j;
-                                diag[((lane & 31) - k + 7) * kDiagRow + k] = ds[4 * r4 + j];
+                                diag[((lane & 31) - k + 7) * kDiagRow + k] =
+                                    ldexpf(ds[4 * r4 + j], -x);
                             }
                             wave_lds_fence();
                             const f32x4* const at =
@@ -504,7 +575,7 @@ attn_dq_kernel(const AttnArgs g) {
                             const f32x4 lo = at[0], hi = at[1];
                             float y = ((lo[0] + lo[1]) + (lo[2] + lo[3])) +
                                       ((hi[0] + hi[1]) + (hi[2] + hi[3]));
-                            y = lane < kDiags ? y * back : 0.0f;
+                            y = lane < kDiags ? y : 0.0f;
                             const int d = wave0 + shift - key0 - 8 * r4 + d_row - 7;
                             if (d >= md) above += y;
                             else if (d <= -md) below += y;
@@ -515,10 +586,22 @@ attn_dq_kernel(const AttnArgs g) {
                         float y = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) y += ds[r];
-                        y *= back;
+                        y = ldexpf(y, -x);
                         if (away >= md) above += y;
                         else below += y;
                     }
+                }
+                run = fmaxf(run, largest(ds));
+                if (__builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
+                    run = fmaxf(run, __shfl_xor(run, 32));  // the query's other half
+                    const bool out = ds_out(run);
+                    const int to = out ? ds_unit(run, ck, ke + b - kDsReach) : ck;
+                    const float f = attn_pow2(ck - to);
+                    move(to);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] *= f;
+                    if (out) run = fmaxf(run, static_cast<float>(1 << kDsLeast));
+                    set_b = ke + b;
                 }
                 const AttnPair<SPLIT> w[1][2] = {
                     {attn_operand<SPLIT>(ds), attn_operand<SPLIT>(ds + 8)}};

@@ -1,0 +1,102 @@
+"""attention's results against their own sizes: long rows, and rows of sizes far apart.
+
+Bounds. Long rows, float32, u = 2^-24: a log-sum below 16 is rounded by 8u of its weights, a
+weight's exponent by as much, an operand in two parts by 4u, dS likewise: 16u in the root of
+their squares. A result is summed by the matrix cores sixteen keys (queries) at a time in three
+products, each sum rounded by u of what it has reached: sqrt(3 n / 16) u for n keys, as roundings
+at random add up. Rows of different sizes are held against the bound of test_gpu_attention.py,
+each against its own row's terms.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import sparsecore_amd as slk
+from test_gpu_attention import BF16, F32, Ref, make
+
+pytestmark = pytest.mark.gpu
+
+
+def errors(got, want):
+    """Of the whole, and of each row."""
+    got, want = got.detach().double().cpu().reshape(want.shape), want
+    off = got - want
+    return float(off.norm() / want.norm()), off.norm(dim=-1) / want.norm(dim=-1)
+
+
+def bound(n):
+    return ((3 * n / 16) ** 0.5 + 16) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("tq,tk", [(64, 4096), (64, 8192), (40, 32768), (8192, 64), (1500, 1500)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_float32_gradients_at_length(dev, tq, tk, d):
+    q, k, v, do = make((1, tq), (1, tk), 1, 1, d, F32, dev)
+    ref = Ref(q, k, v, do, [(0, tq, 0, tk)], False, d ** -0.5)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, causal=False)
+    for name, x, n in zip(("out", "dq", "dk", "dv"),
+                          (out, *torch.autograd.grad(out, leaves, do)), (tk, tk, tq, tq)):
+        whole, _ = errors(x, ref.val[name])
+        assert whole <= bound(n), (name, whole, bound(n))
+
+
+@pytest.mark.parametrize("tk", [512, 8192])
+def test_one_large_gradient_among_small_ones(dev, tk):
+    """A row of dO a thousand times its neighbours: their gradients are as exact as without."""
+    q, k, v, do = make((1, 64), (1, tk), 1, 1, 64, F32, dev)
+    do[0, 5] *= 1000
+    ref = Ref(q, k, v, do, [(0, 64, 0, tk)], False, 0.125)
+    q.requires_grad_()
+    dq, = torch.autograd.grad(slk.attention(q, k, v, causal=False), [q], do)
+    _, rows = errors(dq, ref.val["dq"])
+    assert float(rows.median()) <= bound(tk), (float(rows.median()), bound(tk))
+
+
+def rows_close(name, got, ref, dtype):
+    """test_gpu_attention's bound with each row's own terms in place of all rows'."""
+    want, mag = ref.val[name], ref.mag[name]
+    got = got.detach().double().cpu().reshape(want.shape)
+    share = 1e-5 if dtype is F32 else 2.0 ** (-7 if name in ("out", "dv") else -6)
+    row = mag.square().mean(-1, keepdim=True).sqrt()
+    off = (got - want).abs() - share * (mag + 1e-3 * row)
+    assert not got.isnan().any(), name
+    worst = int(off.flatten().argmax())
+    assert float(off.max()) <= 1e-37, (name, worst, float(got.flatten()[worst]),
+                                       float(want.flatten()[worst]), float(mag.flatten()[worst]))
+
+
+def by_tiles(x, factors):
+    """Rows 64 i .. 64 i + 63 times factors[i]."""
+    t = x.shape[1]
+    f = torch.tensor([factors[min(i // 64, len(factors) - 1)] for i in range(t)],
+                     dtype=torch.float64)
+    return (x.double().cpu() * f[None, :, None, None]).to(x.dtype).to(x.device)
+
+
+SIZES = [[2.0 ** (20 * i) for i in range(5)], [2.0 ** (-20 * i) for i in range(5)],
+         [1.0, 2.0 ** 40, 1.0, 2.0 ** -40, 1.0], [1.0, 1.0, 1.0, 1.0, 2.0 ** 90]]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("which", ["dout", "k"])
+@pytest.mark.parametrize("d,buckets", [(64, 0), (128, 0), (32, 16)])
+def test_gradients_of_tiles_of_different_sizes(dev, d, buckets, which, sizes, dtype):
+    """dO or K over many powers of two from one 64 rows to the next of a causal sequence. (K so
+    small that no score reaches a thousand.) What a row does not see is in none of its sums."""
+    t, h = 300, 2
+    q, k, v, do = make((1, t), (1, t), h, 1, d, dtype, dev)
+    if which == "dout":
+        do = by_tiles(do, sizes)
+    else:
+        top = max(sizes)
+        k = by_tiles(k, [x / top for x in sizes])
+    bias = torch.randn(buckets, h, device=dev) if buckets else None
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5, bias, 20)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, bias=bias, max_distance=20)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        rows_close(name, x, ref, dtype)
