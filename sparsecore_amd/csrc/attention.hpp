@@ -36,6 +36,7 @@ constexpr int kAttnTileRows = 128; // rows of a workgroup of the tiled kernels
 constexpr int kAttnThreads = 256;
 constexpr int kAttnMaxSplits = 128;  // parts of the keys
 constexpr int kAttnUnit = 14;     // a packed tile's largest element is in 2^[14, 15)
+constexpr int kUnset = -100000;   // the exponent of a row's unit before it has seen anything
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // One sequence: rows [q0, q0 + nq) of its batch entry are queries, nq of eq rows

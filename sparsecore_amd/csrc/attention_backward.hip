@@ -20,7 +20,6 @@ namespace {
 // it that nothing leaves float32: |dP - delta| < 2^b scaled stays below 2^kDsReach. That
 // is looked at only where a tile's exponents differ from those it was looked at for.
 constexpr int kDsMost = 15, kDsStart = 7, kDsLeast = 4, kDsReach = 80;
-constexpr int kUnset = -100000;  // the unit of a row that has seen nothing
 
 // Exponent above |dP| < DP·2^(oe + 1)·2^(ve + 1) and |delta| < 2^(de + 1), and their
 // difference. Not below -20: powers of two from it stay in float32.

@@ -16,7 +16,10 @@ constexpr int kWeightUnit = 7;
 // computed as K·Q^T, so that a lane holds half of a query's 64 (the others are 32
 // lanes away): the softmax's maximum and sum are the lane's own, and its weights
 // are the operand of O^T = V^T·P^T as they are. The row's maximum is only raised
-// when a new one is more than 2^8 times above. One sequence of 16384, 32 heads over 8
+// when a new one is more than 2^8 times above. O has a unit of its own, 2^ev, as a tile's
+// values are in units of their largest: of the largest weight times value so far, row by
+// row, so that neither a tile that a row does not see nor one of large values that it
+// hardly looks at takes bits off its weights. One sequence of 16384, 32 heads over 8
 // of 128, bfloat16, causal: 2.23 ms, 0.99 PFLOP/s (a large library product of bfloat16
 // reaches 1.24), bound by the matrix cores and the exponentials between them.
 template <bool SPLIT, int DB, bool BIAS>
@@ -55,7 +58,7 @@ attn_forward_kernel(const AttnArgs g) {
     for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[fb][r] = 0.0f;
-    int vmax = -200;  // exponent that the accumulated values are in units of
+    int ev = kUnset;
 
     if (t0 < t1) {
         const char* const kp = g.k.p + kvh * g.k.sh + static_cast<int64_t>(seq.pk / 64) * kBytes;
@@ -77,14 +80,6 @@ attn_forward_kernel(const AttnArgs g) {
             for (int ks = 0; ks < KS; ++ks) qf[ks] = rd.along(at, (q_row >> 5) & 1, ks);
         }
         const int tiles0 = seq.pk / 64;
-        {
-            const int* ve = g.v.exps + kvh * g.v.exps_sh + tiles0;
-            int e = -400;
-            for (int i = t0 + lane; i < t1; i += 64) e = max(e, ve[i] >> 1);
-#pragma unroll
-            for (int x = 32; x > 0; x >>= 1) e = max(e, __shfl_xor(e, x));
-            vmax = __builtin_amdgcn_readfirstlane(e);
-        }
         if constexpr (BIAS) attn_bias_row(g.bias, head, bias_row);
         const int md = BIAS ? g.bias.max_distance : 0;
 
@@ -105,7 +100,6 @@ attn_forward_kernel(const AttnArgs g) {
                 });
             const int64_t et = kvh * g.k.exps_sh + tiles0 + kt;
             const int ve = attn_scalar(g.v.exps + et), ke = attn_scalar(g.k.exps + et);
-            const int d = max((ve >> 1) - vmax, -60);
             float c = ldexpf(g.scale2, qe + (ke >> 1) - 2 * kAttnUnit);
             // the last key that this query sees, from the tile's first
             const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
@@ -141,17 +135,30 @@ attn_forward_kernel(const AttnArgs g) {
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(s[0][r], s[1][r]), top);
             top = fmaxf(top, __shfl_xor(top, 32)) * c;
-            if (__builtin_amdgcn_ballot_w64(top > m + kGrowth) != 0) {
+            const float over = static_cast<float>(max((ve >> 1) - ev, 0));
+            if (__builtin_amdgcn_ballot_w64(top + over > m + kGrowth) != 0) {
                 const float up = fmaxf(m, top);
-                const float a = up == -INFINITY ? 1.0f : attn_exp2(m - up);
-                m = up;
-                l *= a;
+                if (up > -INFINITY) {
+                    // O shrinks with the weights: by whole powers of two its unit does. The
+                    // fraction of a power of two is the same factor for the sum and for O.
+                    const float grow = fminf(up - m, 1000.0f);
+                    const int whole = static_cast<int>(grow);
+                    const int mine = (ve >> 1) + static_cast<int>(fmaxf(top - up, -1000.0f));
+                    const int to = max(m > -INFINITY ? ev - whole : kUnset,
+                                       top > -INFINITY ? mine : kUnset);
+                    const float part = attn_exp2(static_cast<float>(whole) - grow);
+                    l *= m > -INFINITY ? ldexpf(part, -whole) : 0.0f;
+                    const float a = m > -INFINITY ? ldexpf(part, ev - to - whole) : 0.0f;
 #pragma unroll
-                for (int fb = 0; fb < DB; ++fb)
+                    for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[fb][r] *= a;
+                        for (int r = 0; r < 16; ++r) o[fb][r] *= a;
+                    m = up;
+                    ev = to;
+                }
             }
             // weights times 2^(unit + d): values of a smaller exponent weigh less
+            const int d = max((ve >> 1) - ev, -60);
             const float ref = m == -INFINITY ? 0.0f : m, unit = static_cast<float>(kWeightUnit + d);
             const float start = unit - ref;
             float sum = 0.0f;
@@ -207,7 +214,7 @@ attn_forward_kernel(const AttnArgs g) {
             g.part_ml[2 * row] = m;
             g.part_ml[2 * row + 1] = sum * attn_pow2(-kWeightUnit);
         }
-        const float f = attn_pow2(vmax - kAttnUnit - kWeightUnit);
+        const float f = attn_pow2(ev - kAttnUnit - kWeightUnit);
 #pragma unroll
         for (int fb = 0; fb < DB; ++fb)
 #pragma unroll
@@ -234,7 +241,7 @@ attn_forward_kernel(const AttnArgs g) {
     }
     if (q >= seq.eq) return;
     const bool zero = q >= seq.nq || sum == 0.0f;  // no query, or one that sees no key
-    const float f = zero ? 0.0f : attn_pow2(vmax - kAttnUnit) / sum;
+    const float f = zero ? 0.0f : attn_pow2(ev - kAttnUnit) / sum;
     const int64_t to = sid * g.out.sb + (seq.q0 + q) * g.out.sr + head * g.out.sh;
     const bool vec = g.out.sd == 1 && g.vec_out;
 #pragma unroll

@@ -100,3 +100,59 @@ def test_gradients_of_tiles_of_different_sizes(dev, d, buckets, which, sizes, dt
     out = slk.attention(*leaves, bias=bias, max_distance=20)
     for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
         rows_close(name, x, ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,buckets,t", [(64, 0, 300), (128, 0, 300), (32, 16, 300), (64, 0, 70)])
+def test_values_of_tiles_of_different_sizes(dev, d, buckets, t, causal, sizes, dtype):
+    """V over many powers of two from one 64 rows to the next: outputs and gradients, with and
+    without what a backward keeps."""
+    h = 2
+    q, k, v, do = make((1, t), (1, t), h, 1, d, dtype, dev)
+    v = by_tiles(v, sizes)
+    bias = torch.randn(buckets, h, device=dev) if buckets else None
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], causal, d ** -0.5, bias, 20)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, bias=bias, max_distance=20, causal=causal)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        rows_close(name, x, ref, dtype)
+    with torch.no_grad():
+        rows_close("out", slk.attention(q, k, v, bias=bias, max_distance=20, causal=causal),
+                   ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("s,size", [(70, 2.0 ** 60), (3000, 2.0 ** 60), (3000, 2.0 ** -60)])
+def test_values_that_hardly_count(dev, s, size, dtype):
+    """A tile of values of another size that all queries give weights of about 2^-70: where
+    these are large they still count, and where they are small nothing else is lost."""
+    t, h, d = 40, 1, 64
+    q, k, v, do = make((1, t), (1, s), h, h, d, dtype, dev)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, :64, :, 0] = -48.0  # scores of these keys lower by 48, about 2^-70 of the others' weight
+    v[:, :64] *= size
+    ref = Ref(q, k, v, do, [(0, t, 0, s)], False, 0.125)
+    with torch.no_grad():
+        rows_close("out", slk.attention(q, k, v, causal=False), ref, dtype)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, causal=False)
+    rows_close("out", out, ref, dtype)
+    dq, = torch.autograd.grad(out, [leaves[0]], do)
+    rows_close("dq", dq, ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_values_hidden_by_a_bias(dev, dtype):
+    """Far keys, behind a bias of the lowest value, with values of 2^60."""
+    t, h, d = 400, 2, 64
+    q, k, v, do = make((1, t), (1, t), h, h, d, dtype, dev)
+    v[:, :192] *= 2.0 ** 60
+    bias = torch.randn(8, h, device=dev)
+    bias[-1] = torch.finfo(F32).min
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5, bias.clamp(min=-1e30), 40)
+    out = slk.attention(q, k, v, bias=bias, max_distance=40)
+    got, want = out.double().cpu().reshape(ref.val["out"].shape), ref.val["out"]
+    rows = (got - want).norm(dim=-1) / want.norm(dim=-1)
+    assert float(rows.max()) <= (1e-5 if dtype is F32 else 2.0 ** -7)
