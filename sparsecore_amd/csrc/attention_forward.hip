@@ -135,8 +135,9 @@ attn_forward_kernel(const AttnArgs g) {
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(s[0][r], s[1][r]), top);
             top = fmaxf(top, __shfl_xor(top, 32)) * c;
+            // differences first: a bias of the lowest value would swallow what is added to it
             const float over = static_cast<float>(max((ve >> 1) - ev, 0));
-            if (__builtin_amdgcn_ballot_w64(top + over > m + kGrowth) != 0) {
+            if (__builtin_amdgcn_ballot_w64(top - m + over > kGrowth) != 0) {
                 const float up = fmaxf(m, top);
                 if (up > -INFINITY) {
                     // O shrinks with the weights: by whole powers of two its unit does. The

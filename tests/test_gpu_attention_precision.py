@@ -156,3 +156,15 @@ def test_large_values_hidden_by_a_bias(dev, dtype):
     got, want = out.double().cpu().reshape(ref.val["out"].shape), ref.val["out"]
     rows = (got - want).norm(dim=-1) / want.norm(dim=-1)
     assert float(rows.max()) <= (1e-5 if dtype is F32 else 2.0 ** -7)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("sizes", SIZES[:3])
+def test_values_of_different_sizes_behind_lowest_biases(dev, sizes, dtype):
+    """All biases of the lowest value: each output is the plain mean of the values it sees."""
+    t, h, d = 300, 2, 64
+    q, k, v, do = make((1, t), (1, t), h, h, d, dtype, dev)
+    v = by_tiles(v, sizes)
+    ref = Ref(torch.zeros_like(q), k, v, do, [(0, t, 0, t)], True, d ** -0.5)
+    bias = torch.full((8, h), torch.finfo(F32).min, device=dev)
+    rows_close("out", slk.attention(q, k, v, bias=bias, max_distance=20), ref, dtype)
