@@ -194,10 +194,12 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     offsets that fall, count as the nearest that do not.
 
     Products run on the matrix cores' float16 instructions, each block of 64 rows of a head
-    scaled by a power of two of its own. float32 operands go in two parts: an element keeps
-    22 bits down to 2^-39 of the largest of its block, about float32's own rounding.
-    bfloat16 ones are exact down to 2^-31 of it; weights and their gradients are rounded to
-    11 bits between the products. Softmax and sums are float32, in a fixed order: results
+    scaled by a power of two of its own, or each row where the block's rows are more than
+    2^12 apart (then 1.5 to 1.7 times the time). float32 operands go in two parts: an element
+    is off by at most 2^-22 of itself or 2^-27 of the largest of its row, about float32's own
+    rounding. bfloat16 ones are exact down to 2^-19 of that. Between the products weights and
+    their gradients are rounded to 22 bits (bfloat16: 11) down to 2^-32 of the largest that
+    their row of results has. Softmax and sums are float32, in a fixed order: results
     repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
     packed (not the tensors themselves), and the output, which must not change in place
     before the backward, nor may offsets and lengths; of a bfloat16 output also what its

@@ -64,6 +64,7 @@ struct Packed {
     char* data;
     int32_t* exps;
     uint64_t* bad;
+    int8_t* rows;
 };
 
 Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows) {
@@ -71,6 +72,7 @@ Packed take_packed(Carver& c, const Sizes& s, int64_t heads, int64_t rows) {
     p.data = static_cast<char*>(c.take(heads * rows * s.row));
     p.exps = static_cast<int32_t*>(c.take(heads * (rows / kAttnRows) * 4));
     p.bad = static_cast<uint64_t*>(c.take(heads * (rows / kAttnRows) * 8));
+    p.rows = static_cast<int8_t*>(c.take(heads * rows));
     return p;
 }
 
@@ -211,6 +213,7 @@ struct Backward {
     float* dkv_part;
     float *delta, *lse;
     int32_t* dexps;
+    int32_t* uneven;
     Packed dout;
     float* dbias_part;
     int64_t bytes;
@@ -223,6 +226,7 @@ Backward backward_of(const slk_attention& a, void* scratch) {
     b.delta = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     b.lse = static_cast<float*>(c.take(a.heads * s.pad_q * 4));
     b.dexps = static_cast<int32_t*>(c.take(a.heads * (s.pad_q / kAttnRows) * 4));
+    b.uneven = static_cast<int32_t*>(c.take(4));
     b.dout = take_packed(c, s, a.heads, s.pad_q);
     b.parts = dkv_parts(a, s);
     if (b.parts > 1)
@@ -240,7 +244,7 @@ AttnIo io_of(const slk_attn_tensor& t) {
 }
 
 AttnOp op_of(const Packed& p, const Sizes& s, int64_t rows) {
-    return AttnOp{p.data, rows * s.row, p.exps, p.bad, rows / kAttnRows};
+    return AttnOp{p.data, rows * s.row, p.exps, p.bad, p.rows, rows / kAttnRows};
 }
 
 // Whether four elements that are consecutive along `unit` start at multiples of
@@ -271,6 +275,7 @@ AttnPackOp pack_op(const slk_attn_tensor& t, const Packed& p, const Sizes& s,
     o.dst_sh = rows * s.row;
     o.exps = p.exps;
     o.bad = p.bad;
+    o.row_exps = p.rows;
     o.exps_sh = rows / kAttnRows;
     o.rows = rows;
     o.heads = static_cast<int32_t>(heads);
@@ -556,6 +561,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
         p.lse = sv.lse;
         p.lse_out = b.lse;
         p.dexps = b.dexps;
+        p.clear = b.uneven;
         rc = attn_launch_pack(p, blocks_of(a.dim), a.dtype, st);
         if (rc != SLK_OK) return rc;
     }
@@ -568,6 +574,7 @@ extern "C" int slk_attention_backward(const slk_attention* args, void* stream) {
     g.inv = sv.inv;
     g.delta = b.delta;
     g.dexps = b.dexps;
+    g.uneven = b.uneven;
     g.dbias_part = b.dbias_part;
     g.dkv_part = b.dkv_part;
     g.dkv_rows = s.pad_k;

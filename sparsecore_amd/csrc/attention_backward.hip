@@ -49,6 +49,20 @@ __device__ __forceinline__ void scale_sums(f32x16 (&x)[N], float f) {
         for (int r = 0; r < 16; ++r) x[i][r] *= f;
 }
 
+// The unit of a row (its sums, and the largest scaled dS so far) where exponents go row by
+// row: `most` is the exponent of the lane's largest dS times 2^e.
+template <int N>
+__device__ __forceinline__ void raise_unit(int most, int& unit, float& run, f32x16 (&sums)[N]) {
+    most = max(most, __shfl_xor(most, 32));  // the row's other half
+    if (run > 0.0f) most = max(most, attn_exponent(run) + unit - kAttnUnit);
+    int to = unit;
+    const int reach = kAttnUnit + most - unit;
+    if (most > kUnset && (reach >= kDsMost || reach < kDsLeast)) to = most + kAttnUnit - kDsStart;
+    scale_sums(sums, attn_pow2(unit - to));
+    unit = to;
+    run = most > kUnset ? attn_pow2(kAttnUnit + most - unit) : 0.0f;
+}
+
 __device__ __forceinline__ float largest(const float (&x)[16]) {
     float m = fabsf(x[0]);
 #pragma unroll
@@ -67,7 +81,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // 64 floats of a row array into LDS, by one wave.
-__device__ __forceinline__ void load_row(const float* from, unsigned char* to, int lane) {
+__device__ __forceinline__ void load_row(const float* from, AttnLds* to, int lane) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const uint64_t at = reinterpret_cast<uint64_t>(from);
     const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
@@ -92,7 +106,11 @@ __device__ __forceinline__ void load_row(const float* from, unsigned char* to, i
 // of 128, bfloat16, causal: 5.0 ms, 0.88 PFLOP/s in its four products; the 512
 // registers of a SIMD's lane hold two waves, too few to keep the matrix cores busy
 // while both compute weights.
-template <bool SPLIT, int DB, bool BIAS>
+//
+// ROWS: the form for workgroups that meet an uneven tile, exponents row by row; the other
+// form leaves them to it. Two kernels, as one would keep registers for both and spill;
+// where there are none the second reads a flag, 4.6 us with its launch.
+template <bool SPLIT, int DB, bool BIAS, bool ROWS>
 __global__ __launch_bounds__(kAttnThreads, DB * (SPLIT ? 2 : 1) <= 4 ? 2 : 1) void
 attn_dkv_kernel(const AttnArgs g) {
     using T = AttnTile<DB>;
@@ -111,6 +129,7 @@ attn_dkv_kernel(const AttnArgs g) {
     __shared__ f16x8 spare[kSpare ? 4 * kSpare : 1][64];
     extern __shared__ float bias_row[];
 
+    if (ROWS && attn_scalar(g.uneven) == 0) return;
     const int t = threadIdx.x, lane = t & 63;
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
     // the query heads of the group that this part of it takes: rep from head0 on
@@ -140,7 +159,7 @@ attn_dkv_kernel(const AttnArgs g) {
 
     if (nt > 0) {
         const int64_t q_tile0 = seq.pq / 64;
-        auto issue = [&](unsigned char* to, int hr, int qt) __attribute__((always_inline)) {
+        auto issue = [&](AttnLds* to, int hr, int qt) __attribute__((always_inline)) {
             const int head = head0 + hr, row = (first + qt) * kRows;
             const int64_t tq = q_tile0 + row / 64;
             const int64_t at = tq * kTile + (row & 63) * T::kRowBytes;
@@ -157,7 +176,7 @@ attn_dkv_kernel(const AttnArgs g) {
             if (BIAS && wv == 2)
                 load_row(g.inv + head * g.lse_sh + tq * 64, to + 2 * kBytes + 512, lane);
         };
-        issue(ring0, 0, 0);
+        issue((AttnLds*)ring0, 0, 0);
         const AttnReads<SPLIT, DB> rd(lane);
         // a tile of 64 rows, and a stage's
         auto row_of = [&](const unsigned char* buf, int b, int ks) __attribute__((always_inline)) {
@@ -183,13 +202,29 @@ attn_dkv_kernel(const AttnArgs g) {
             if constexpr (kVInLds) {
                 // the second of the workgroup's two tiles is there if a key of it is
                 const char* from = g.v.p + kvh * g.v.sh + (seq.pk / 64 + 2 * tile) * int64_t{kTile};
-                attn_stage<kTile>(from, values, wv, lane);
+                attn_stage<kTile>(from, (AttnLds*)values, wv, lane);
                 if (tile * 128 + 64 < seq.nk)
-                    attn_stage<kTile>(from + kTile, values + kTile, wv, lane);
+                    attn_stage<kTile>(from + kTile, (AttnLds*)values + kTile, wv, lane);
+            }
+        }
+        {
+            // of all the tiles that the workgroup meets
+            const int64_t k0 = seq.pk / 64 + 2 * tile;
+            const int64_t k1 = k0 + (min(seq.nk - tile * 128, 128) + 63) / 64;
+            const int64_t q0 = q_tile0 + first * kRows / 64, q1 = q_tile0 + (seq.nq + 63) / 64;
+            int flags = attn_flags(g.k, kvh, k0, k1, lane) | attn_flags(g.v, kvh, k0, k1, lane);
+            for (int h = head0; h < head0 + rep; ++h)
+                flags |= attn_flags(g.q, h, q0, q1, lane) | attn_flags(g.dout, h, q0, q1, lane) |
+                         attn_more_flags(g.q, h, q0, q1, lane) |
+                         attn_more_flags(g.dout, h, q0, q1, lane);
+            if (attn_uneven(flags) != ROWS) {
+                if (!ROWS && t == 0) *g.uneven = 1;
+                __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no loads into LDS outlive the workgroup
+                return;
             }
         }
         const unsigned char* const my_v = values + (wv >> 1) * kTile;
-        const int ke = attn_exp(g.k, kvh, k_row), ve = attn_exp(g.v, kvh, k_row);
+        const int even_ke = attn_exp(g.k, kvh, k_row), even_ve = attn_exp(g.v, kvh, k_row);
         float run = 0.0f;  // the largest scaled |dS| of the lane's key so far
         // of the stage that they were set for: weights are times 2^unit, dS times 2^14 and the
         // row's unit is weight · beta · (dP - delta)
@@ -200,9 +235,11 @@ attn_dkv_kernel(const AttnArgs g) {
         auto compute = [&](const unsigned char* buf, int hr, int q_first)
             __attribute__((always_inline)) {
             const int head = head0 + hr, row0 = seq.pq + q_first;
+            const int ke = ROWS ? *g.k.row(kvh, k_row + (lane & 31)) : even_ke;
+            const int ve = ROWS ? *g.v.row(kvh, k_row + (lane & 31)) : even_ve;
             const int qe = attn_exp(g.q, head, row0), oe = attn_exp(g.dout, head, row0);
             const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (row0 >> 6));
-            const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
+            const float c = ldexpf(g.scale2, min(qe + ke - 2 * kAttnUnit, 126));
             const float alpha = attn_pow2(oe + ve - 2 * kAttnUnit);
             const int b = ds_exponent(oe, ve, de, kLogDp);
             // the lane's key is seen by rows [from, to) of a block
@@ -250,7 +287,7 @@ attn_dkv_kernel(const AttnArgs g) {
                     BIAS ? bias_row + md + kAttnFar + (far ? 0 : q0 + shift - key) +
                                4 * (lane >> 5)
                          : nullptr;
-                if (masked || oe != set_oe || qe != set_qe || b > set_b) {
+                if (!ROWS && (masked || oe != set_oe || qe != set_qe || b > set_b)) {
                     const bool sees = !masked || seen_from(q0) < seen_to(q0);
                     if (__builtin_amdgcn_ballot_w64(sees & (oe > co)) != 0) {
                         const int to = sees ? max(co, oe) : co;
@@ -268,8 +305,48 @@ attn_dkv_kernel(const AttnArgs g) {
                 }
                 AttnPair<SPLIT> wp[1][2], wd[1][2];
                 float ds[16];
+                if constexpr (ROWS) {
+                    const int lo = seen_from(q0), hi = seen_to(q0);
+                    const int64_t at_row = row0 + 32 * qb + 4 * (lane >> 5);
+                    float p[16];
+                    int most_o = kUnset, most = kUnset;  // of what the key is seen by
+                    uint32_t qx[4], ox[4];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        qx[r4] = attn_four_rows(g.q.row(head, at_row + 8 * r4));
+                        ox[r4] = attn_four_rows(g.dout.row(head, at_row + 8 * r4));
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = attn_row(r, lane);
+                        const int qr = attn_one_of(qx[r / 4], r % 4);
+                        const int dr = attn_one_of(ox[r / 4], r % 4);
+                        float x = ldexpf(s[r] * g.scale2, qr + ke - 2 * kAttnUnit);
+                        if constexpr (BIAS)
+                            x += far ? flat : near_at[8 * (r / 4) + r % 4];
+                        p[r] = attn_exp2(x - lse[row]);
+                        if constexpr (BIAS) p[r] *= lse[128 + row];
+                        ds[r] = p[r] * (ldexpf(dp[r], dr + ve - 2 * kAttnUnit) - delta[row]);
+                        const bool see = row >= lo && row < hi;
+                        p[r] = see ? p[r] : 0.0f;
+                        ds[r] = see ? ds[r] : 0.0f;
+                        if (p[r] != 0.0f) most_o = max(most_o, dr);
+                        if (ds[r] != 0.0f) most = max(most, attn_exponent(ds[r]) + qr);
+                    }
+                    most_o = max(max(most_o, __shfl_xor(most_o, 32)), co);
+                    scale_sums(dv, attn_pow2(co - most_o));
+                    co = most_o;
+                    raise_unit(most, cq, run, dk);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        p[r] = ldexpf(p[r], kAttnUnit + attn_one_of(ox[r / 4], r % 4) - co);
+                        ds[r] = ldexpf(ds[r], kAttnUnit + attn_one_of(qx[r / 4], r % 4) - cq);
+                    }
+                    wp[0][0] = attn_operand<SPLIT>(p);
+                    wp[0][1] = attn_operand<SPLIT>(p + 8);
+                }
+#pragma unroll
+                for (int half = 0; half < (ROWS ? 0 : 2); ++half) {
                     float p[8];
 #pragma unroll
                     for (int r4 = 0; r4 < 2; ++r4) {
@@ -302,8 +379,8 @@ attn_dkv_kernel(const AttnArgs g) {
                     }
                     wp[0][half] = attn_operand<SPLIT>(p);
                 }
-                run = fmaxf(run, largest(ds));
-                if (__builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
+                if constexpr (!ROWS) run = fmaxf(run, largest(ds));
+                if (!ROWS && __builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
                     run = fmaxf(run, __shfl_xor(run, 32));  // the key's other half
                     const bool out = ds_out(run);
                     const int u = static_cast<int>(unit);
@@ -334,7 +411,7 @@ attn_dkv_kernel(const AttnArgs g) {
             }
             __builtin_amdgcn_s_waitcnt(wait_vm(0));
             asm volatile("s_barrier" ::: "memory");
-            if (hr < rep) issue(next, hr, qt);
+            if (hr < rep) issue((AttnLds*)next, hr, qt);
             if (BIAS && i == 0) {  // a head's first stage
                 attn_bias_row(g.bias, head0 + h, bias_row);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -349,7 +426,7 @@ attn_dkv_kernel(const AttnArgs g) {
         if (left) stage(ring0, ring1);
     }
 
-    if (key >= seq.ek) return;
+    if (key >= seq.ek || (ROWS && nt == 0)) return;
     const float fk = ldexpf(g.scale, cq - 2 * kAttnUnit), fv = attn_pow2(co - 2 * kAttnUnit);
     const bool zero = key >= seq.nk || nt == 0;
     if (g.dkv_parts > 1 && key < seq.nk) {
@@ -449,12 +526,12 @@ attn_dq_kernel(const AttnArgs g) {
 
     if (t1 > 0) {
         const int64_t k_tile = seq.pk / 64;
-        auto issue = [&](unsigned char* to, int kt) __attribute__((always_inline)) {
+        auto issue = [&](AttnLds* to, int kt) __attribute__((always_inline)) {
             const int64_t at = (k_tile + kt) * kBytes;
             attn_stage<kBytes>(g.k.p + kvh * g.k.sh + at, to, wv, lane);
             attn_stage<kBytes>(g.v.p + kvh * g.v.sh + at, to + kBytes, wv, lane);
         };
-        issue(ring0, 0);
+        issue((AttnLds*)ring0, 0);
         const AttnReads<SPLIT, DB> rd(lane);
 
         const int q_row = seq.pq + min(wave0, (seq.nq + 63) / 64 * 64 - 32);
@@ -476,7 +553,7 @@ attn_dq_kernel(const AttnArgs g) {
         const float lse = mine ? g.lse[ri] : INFINITY;
         const float inv = BIAS && mine ? g.inv[ri] : 0.0f;
         const float delta = mine ? g.delta[ri] : 0.0f;
-        const int qe = attn_exp(g.q, head, q_row), oe = attn_exp(g.dout, head, q_row);
+        const int even_qe = attn_exp(g.q, head, q_row), even_oe = attn_exp(g.dout, head, q_row);
         const int de = attn_scalar(g.dexps + head * g.q.exps_sh + (q_row >> 6));
 
         int set_b = kUnset;  // the largest exponent, K's counted, that ck was looked at for
@@ -486,7 +563,10 @@ attn_dq_kernel(const AttnArgs g) {
             run *= f;
             ck = to;
         };
-        auto compute = [&](const unsigned char* buf, int key_tile) __attribute__((always_inline)) {
+        // ROWS: exponents row by row, as uneven tiles have them
+        auto compute = [&](auto rows, const unsigned char* buf, int key_tile)
+            __attribute__((always_inline)) {
+            constexpr bool ROWS = decltype(rows)::value;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const int key0 = key_tile + 32 * kb;
@@ -496,9 +576,11 @@ attn_dq_kernel(const AttnArgs g) {
                     key0 + 31 >= seq.nk || (g.causal && key0 + 31 > wave0 + shift);
                 const int ke = attn_exp(g.k, kvh, seq.pk + key0);
                 const int ve = attn_exp(g.v, kvh, seq.pk + key0);
-                const float c = ldexpf(g.scale2, qe + ke - 2 * kAttnUnit);
+                const int qe = ROWS ? *g.q.row(head, q_row + (lane & 31)) : even_qe;
+                const int oe = ROWS ? *g.dout.row(head, q_row + (lane & 31)) : even_oe;
+                const float c = ldexpf(g.scale2, min(qe + ke - 2 * kAttnUnit, 126));
                 const int b = ds_exponent(oe, ve, de, kLogDp);
-                if (ke + b > set_b) {
+                if (!ROWS && ke + b > set_b) {
                     const int to = max(ck, ke + b - kDsReach);
                     if (__builtin_amdgcn_ballot_w64(to != ck) != 0) move(to + (to != ck ? 14 : 0));
                     set_b = ke + b;
@@ -541,9 +623,29 @@ attn_dq_kernel(const AttnArgs g) {
                                                         (near ? away - 4 * (lane >> 5) : 27) - 27
                                                   : nullptr;
                 float ds[16];
+                uint32_t kx[4], vx[4];
+                if constexpr (ROWS) {
+                    const int64_t at = seq.pk + key0 + 4 * (lane >> 5);
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        kx[r4] = attn_four_rows(g.k.row(kvh, at + 8 * r4));
+                        vx[r4] = attn_four_rows(g.v.row(kvh, at + 8 * r4));
+                    }
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     float p;
+                    if constexpr (ROWS) {
+                        float x = ldexpf(s[r] * g.scale2,
+                                         qe + attn_one_of(kx[r / 4], r % 4) - 2 * kAttnUnit);
+                        if constexpr (BIAS)
+                            x += near ? near_at[27 - 8 * (r >> 2) - (r & 3)] : flat;
+                        p = attn_exp2(x - lse);
+                        if constexpr (BIAS) p *= inv;
+                        ds[r] = p * (ldexpf(dp[r], oe + attn_one_of(vx[r / 4], r % 4) -
+                                                       2 * kAttnUnit) - delta);
+                        continue;
+                    }
                     if constexpr (BIAS)
                         p = attn_exp2(__builtin_fmaf(s[r], c,
                                                      near ? near_at[27 - 8 * (r >> 2) - (r & 3)]
@@ -566,7 +668,7 @@ attn_dq_kernel(const AttnArgs g) {
                             for (int j = 0; j < 4; ++j) {
                                 const int k = 4 * (lane >> 5) + j;
                                 diag[((lane & 31) - k + 7) * kDiagRow + k] =
-                                    ldexpf(ds[4 * r4 + j], -x);
+                                    ROWS ? ds[4 * r4 + j] : ldexpf(ds[4 * r4 + j], -x);
                             }
                             wave_lds_fence();
                             const f32x4* const at =
@@ -585,13 +687,25 @@ attn_dq_kernel(const AttnArgs g) {
                         float y = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) y += ds[r];
-                        y = ldexpf(y, -x);
+                        if constexpr (!ROWS) y = ldexpf(y, -x);
                         if (away >= md) above += y;
                         else below += y;
                     }
                 }
-                run = fmaxf(run, largest(ds));
-                if (__builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
+                if constexpr (ROWS) {
+                    int most = kUnset;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (ds[r] != 0.0f)
+                            most = max(most, attn_exponent(ds[r]) + attn_one_of(kx[r / 4], r % 4));
+                    raise_unit(most, ck, run, dq);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        ds[r] = ldexpf(ds[r], kAttnUnit + attn_one_of(kx[r / 4], r % 4) - ck);
+                } else {
+                    run = fmaxf(run, largest(ds));
+                }
+                if (!ROWS && __builtin_amdgcn_ballot_w64(ds_out(run)) != 0) {
                     run = fmaxf(run, __shfl_xor(run, 32));  // the query's other half
                     const bool out = ds_out(run);
                     const int to = out ? ds_unit(run, ck, ke + b - kDsReach) : ck;
@@ -607,18 +721,31 @@ attn_dq_kernel(const AttnArgs g) {
                 attn_accumulate<SPLIT, DB, 1>(rd, buf, kb, w, dq);
             }
         };
-        auto stage = [&](const unsigned char* cur, unsigned char* next, int kt) __attribute__((always_inline)) {
+        auto stage = [&](auto rows, const unsigned char* cur, unsigned char* next, int kt)
+            __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(wait_vm(0));
             asm volatile("s_barrier" ::: "memory");
-            if (kt + 1 < t1) issue(next, kt + 1);
-            if (wave0 < seq.nq) compute(cur, kt * kAttnRows);
+            if (kt + 1 < t1) issue((AttnLds*)next, kt + 1);
+            if (wave0 < seq.nq) compute(rows, cur, kt * kAttnRows);
         };
-        int kt = 0;
-        for (; kt + 2 <= t1; kt += 2) {
-            stage(ring0, ring1, kt);
-            stage(ring1, ring0, kt + 1);
-        }
-        if (kt < t1) stage(ring0, ring1, kt);
+        auto all = [&](auto rows) __attribute__((always_inline)) {
+            int kt = 0;
+            for (; kt + 2 <= t1; kt += 2) {
+                stage(rows, ring0, ring1, kt);
+                stage(rows, ring1, ring0, kt + 1);
+            }
+            if (kt < t1) stage(rows, ring0, ring1, kt);
+        };
+        // of all the tiles that the workgroup meets
+        const int64_t q0 = (seq.pq + rows0) / 64, q1 = q0 + (min(seq.nq - rows0, 128) + 63) / 64;
+        if (attn_uneven(attn_flags(g.q, head, q0, q1, lane) |
+                        attn_flags(g.dout, head, q0, q1, lane) |
+                        attn_flags(g.k, kvh, k_tile, k_tile + t1, lane) |
+                        attn_flags(g.v, kvh, k_tile, k_tile + t1, lane) |
+                        attn_more_flags(g.k, kvh, k_tile, k_tile + t1, lane) |
+                        attn_more_flags(g.v, kvh, k_tile, k_tile + t1, lane)))
+            all(std::true_type{});
+        else all(std::false_type{});
     }
 
     if (q < seq.eq && g.dq.p != nullptr) {
@@ -747,9 +874,11 @@ int launch(const AttnArgs& g, const AttnPlan& kplan, int64_t q_entries, int64_t 
         a.plan = kplan;
         a.tiles = k_tiles;
         const dim3 grid(static_cast<unsigned>(k_entries * g.kv_heads * g.dkv_parts));
-        hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS>), grid, dim3(kAttnThreads),
-                           BIAS ? attn_bias_floats(g.bias.max_distance) * sizeof(float) : 0, st,
-                           a);
+        const size_t lds = BIAS ? attn_bias_floats(g.bias.max_distance) * sizeof(float) : 0;
+        hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS, false>), grid, dim3(kAttnThreads), lds,
+                           st, a);
+        hipLaunchKernelGGL((attn_dkv_kernel<SPLIT, DB, BIAS, true>), grid, dim3(kAttnThreads), lds,
+                           st, a);
         const int rc = check_launch("attention_backward: dk, dv");
         if (rc != SLK_OK) return rc;
         if (g.dkv_parts > 1) {

@@ -63,15 +63,15 @@ attn_forward_kernel(const AttnArgs g) {
     if (t0 < t1) {
         const char* const kp = g.k.p + kvh * g.k.sh + static_cast<int64_t>(seq.pk / 64) * kBytes;
         const char* const vp = g.v.p + kvh * g.v.sh + static_cast<int64_t>(seq.pk / 64) * kBytes;
-        auto issue = [&](unsigned char* to, int kt) __attribute__((always_inline)) {
+        auto issue = [&](AttnLds* to, int kt) __attribute__((always_inline)) {
             attn_stage<kBytes>(kp + static_cast<int64_t>(kt) * kBytes, to, wv, lane);
             attn_stage<kBytes>(vp + static_cast<int64_t>(kt) * kBytes, to + kBytes, wv, lane);
         };
-        issue(ring0, t0);
+        issue((AttnLds*)ring0, t0);
         const AttnReads<SPLIT, DB> rd(lane);
 
         const int q_row = seq.pq + min(wave0, (seq.nq + 63) / 64 * 64 - 32);
-        const int qe = attn_exp(g.q, head, q_row);
+        const int even_qe = attn_exp(g.q, head, q_row);
         AttnPair<SPLIT> qf[KS];
         {
             const unsigned char* at = reinterpret_cast<const unsigned char*>(
@@ -83,7 +83,10 @@ attn_forward_kernel(const AttnArgs g) {
         if constexpr (BIAS) attn_bias_row(g.bias, head, bias_row);
         const int md = BIAS ? g.bias.max_distance : 0;
 
-        auto compute = [&](const unsigned char* buf, int kt) __attribute__((always_inline)) {
+        // ROWS: exponents row by row, as uneven tiles have them
+        auto compute = [&](auto rows, const unsigned char* buf, int kt)
+            __attribute__((always_inline)) {
+            constexpr bool ROWS = decltype(rows)::value;
             const int key0 = kt * kAttnRows;
             // the wave's last query sees no key of this tile
             if (g.causal && key0 > wave0 + 31 + shift) return;
@@ -99,8 +102,22 @@ attn_forward_kernel(const AttnArgs g) {
                     s[i.value % 2] = attn_dot<SPLIT>(k, qf[i.value / 2], s[i.value % 2]);
                 });
             const int64_t et = kvh * g.k.exps_sh + tiles0 + kt;
+            const int qe = ROWS ? *g.q.row(head, q_row + (lane & 31)) : even_qe;
             const int ve = attn_scalar(g.v.exps + et), ke = attn_scalar(g.k.exps + et);
-            float c = ldexpf(g.scale2, qe + (ke >> 1) - 2 * kAttnUnit);
+            float c = 1.0f;
+            if constexpr (ROWS) {
+                const int8_t* const at = g.k.row(kvh, seq.pk + key0 + 4 * (lane >> 5));
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    const uint32_t four = attn_four_rows(at + 8 * (r / 4));
+                    s[r / 16][r % 16] =
+                        ldexpf(s[r / 16][r % 16] * g.scale2,
+                               qe + attn_one_of(four, r % 4) - 2 * kAttnUnit);
+                }
+            } else {
+                // not beyond float32: a row of zeros has scores of 0
+                c = ldexpf(g.scale2, min(qe + (ke >> 2) - 2 * kAttnUnit, 126));
+            }
             // the last key that this query sees, from the tile's first
             const int lim = (g.causal ? min(seq.nk - 1, q + shift) : seq.nk - 1) - key0;
             if constexpr (BIAS) {
@@ -135,16 +152,32 @@ attn_forward_kernel(const AttnArgs g) {
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(s[0][r], s[1][r]), top);
             top = fmaxf(top, __shfl_xor(top, 32)) * c;
-            // differences first: a bias of the lowest value would swallow what is added to it
-            const float over = static_cast<float>(max((ve >> 1) - ev, 0));
-            if (__builtin_amdgcn_ballot_w64(top - m + over > kGrowth) != 0) {
-                const float up = fmaxf(m, top);
+            // The largest weight times value, from the row's maximum: as a tile's exponent or
+            // row by row. Differences first: a bias of the lowest value would swallow what is
+            // added to it.
+            const int8_t* const v_rows = g.v.row(kvh, seq.pk + key0 + 4 * (lane >> 5));
+            const float up = fmaxf(m, top);
+            float most = top - up + static_cast<float>(ve >> 2), over;
+            if constexpr (ROWS) {
+                most = -INFINITY;
+                const float from = up == -INFINITY ? 0.0f : up;
+#pragma unroll
+                for (int r = 0; r < 32; ++r)
+                    most = fmaxf(most, s[r / 16][r % 16] - from +
+                                           static_cast<float>(attn_one_of(
+                                               attn_four_rows(v_rows + 8 * (r / 4)), r % 4)));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                over = up - m + fmaxf(most - static_cast<float>(ev), 0.0f);
+            } else {
+                over = top - m + static_cast<float>(max((ve >> 2) - ev, 0));
+            }
+            if (__builtin_amdgcn_ballot_w64(over > kGrowth) != 0) {
                 if (up > -INFINITY) {
                     // O shrinks with the weights: by whole powers of two its unit does. The
                     // fraction of a power of two is the same factor for the sum and for O.
                     const float grow = fminf(up - m, 1000.0f);
                     const int whole = static_cast<int>(grow);
-                    const int mine = (ve >> 1) + static_cast<int>(fmaxf(top - up, -1000.0f));
+                    const int mine = static_cast<int>(ceilf(fmaxf(most, -1000.0f)));
                     const int to = max(m > -INFINITY ? ev - whole : kUnset,
                                        top > -INFINITY ? mine : kUnset);
                     const float part = attn_exp2(static_cast<float>(whole) - grow);
@@ -159,7 +192,7 @@ attn_forward_kernel(const AttnArgs g) {
                 }
             }
             // weights times 2^(unit + d): values of a smaller exponent weigh less
-            const int d = max((ve >> 1) - ev, -60);
+            const int d = ROWS ? 0 : max((ve >> 2) - ev, -60);
             const float ref = m == -INFINITY ? 0.0f : m, unit = static_cast<float>(kWeightUnit + d);
             const float start = unit - ref;
             float sum = 0.0f;
@@ -169,6 +202,14 @@ attn_forward_kernel(const AttnArgs g) {
                 float p[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
+                    if constexpr (ROWS) {
+                        const float x = s[kb][r] - ref;
+                        sum += attn_exp2(x);
+                        const uint32_t four = attn_four_rows(v_rows + 32 * kb + 8 * (r / 4));
+                        p[r] = attn_exp2(x + static_cast<float>(attn_one_of(four, r % 4) - ev +
+                                                                kWeightUnit));
+                        continue;
+                    }
                     // a bias may be large enough to swallow the unit: it comes second
                     if constexpr (BIAS) p[r] = attn_exp2(__builtin_fmaf(s[kb][r], c, -ref) + unit);
                     else p[r] = attn_exp2(__builtin_fmaf(s[kb][r], c, start));
@@ -177,7 +218,7 @@ attn_forward_kernel(const AttnArgs g) {
                 w[kb][0] = attn_operand<SPLIT>(p);
                 w[kb][1] = attn_operand<SPLIT>(p + 8);
             }
-            l = __builtin_fmaf(sum, attn_pow2(-d), l);
+            l = __builtin_fmaf(sum, attn_pow2(ROWS ? kWeightUnit : -d), l);
             if (__builtin_expect((ve | ke) & 1, 0)) {  // rows that are not finite
                 const uint64_t bad = attn_scalar(g.v.bad + et) | attn_scalar(g.k.bad + et);
                 const uint64_t sees = lim >= 63 ? ~uint64_t{0}
@@ -187,19 +228,30 @@ attn_forward_kernel(const AttnArgs g) {
             }
             attn_accumulate<SPLIT, DB, 2>(rd, buf + kBytes, 0, w, o);
         };
-        auto stage = [&](const unsigned char* cur, unsigned char* next, int kt)
+        auto stage = [&](auto rows, const unsigned char* cur, unsigned char* next, int kt)
             __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(wait_vm(0));
             asm volatile("s_barrier" ::: "memory");
-            if (kt + 1 < t1) issue(next, kt + 1);
-            if (wave0 < seq.nq) compute(cur, kt);
+            if (kt + 1 < t1) issue((AttnLds*)next, kt + 1);
+            if (wave0 < seq.nq) compute(rows, cur, kt);
         };
-        int kt = t0;
-        for (; kt + 2 <= t1; kt += 2) {
-            stage(ring0, ring1, kt);
-            stage(ring1, ring0, kt + 1);
-        }
-        if (kt < t1) stage(ring0, ring1, kt);
+        auto all = [&](auto rows) __attribute__((always_inline)) {
+            int kt = t0;
+            for (; kt + 2 <= t1; kt += 2) {
+                stage(rows, ring0, ring1, kt);
+                stage(rows, ring1, ring0, kt + 1);
+            }
+            if (kt < t1) stage(rows, ring0, ring1, kt);
+        };
+        // of all the tiles that the workgroup meets
+        const int64_t q0 = (seq.pq + rows0) / kAttnRows, q1 = q0 + (min(seq.nq - rows0, 128) + 63) / 64;
+        if (attn_uneven(attn_flags(g.q, head, q0, q1, lane) |
+                        attn_flags(g.k, kvh, tiles0 + t0, tiles0 + t1, lane) |
+                        attn_flags(g.v, kvh, tiles0 + t0, tiles0 + t1, lane) |
+                        attn_more_flags(g.k, kvh, tiles0 + t0, tiles0 + t1, lane) |
+                        attn_more_flags(g.v, kvh, tiles0 + t0, tiles0 + t1, lane)))
+            all(std::true_type{});
+        else all(std::false_type{});
     }
 
     float sum = l + __shfl_xor(l, 32);

@@ -292,6 +292,22 @@ __device__ __forceinline__ int tile_exponent(uint32_t top) {
     return max(static_cast<int>(top >> 23) - 127, -100);
 }
 
+// Maximum over aligned groups of L lanes, in every lane.
+template <int L>
+__device__ __forceinline__ uint32_t lane_max(uint32_t m) {
+    auto dpp = [&](auto ctrl) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+            0, static_cast<int>(m), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    m = max(m, dpp(std::integral_constant<int, 0xb1>{}));                         // lanes 1, 0, 3, 2
+    m = max(m, dpp(std::integral_constant<int, 0x4e>{}));                         // 2, 3, 0, 1
+    if constexpr (L >= 8) m = max(m, dpp(std::integral_constant<int, 0x141>{}));  // half-row mirror
+    if constexpr (L >= 16) m = max(m, dpp(std::integral_constant<int, 0x140>{})); // row mirror
+    if constexpr (L >= 32) m = max(m, static_cast<uint32_t>(__shfl_xor(m, 16)));
+    if constexpr (L >= 64) m = max(m, static_cast<uint32_t>(__shfl_xor(m, 32)));
+    return m;
+}
+
 // Packs a tile of 64 rows of one head: blockIdx.x the tile, blockIdx.y the head of
 // an operand; one more y for the rows of biases, a head each. Of dO (with delta
 // given) also delta, from the same tile and O's. Rows of consecutive features go
@@ -307,7 +323,8 @@ __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& o
     using Regs = TileRegs<IO, DP, BY_ROWS>;
     __shared__ float turn[BY_ROWS ? kAttnRows : 1][BY_ROWS ? DP + 1 : 1];
     __shared__ float sums[DELTA && BY_ROWS ? 16 : 1][kAttnRows];
-    __shared__ uint32_t most[2][4], odd[2];  // odd: rows with a value that is not finite
+    __shared__ uint32_t most[4], odd[2];  // odd: rows with a value that is not finite
+    __shared__ uint32_t tops[BY_ROWS ? 4 : 1][kAttnRows];  // each row's largest finite magnitude
     const int t = threadIdx.x;
     const int64_t padded = static_cast<int64_t>(blockIdx.x) * kAttnRows;
     const int n = op.keys ? ro.seq.nk : ro.seq.nq, first = op.keys ? ro.seq.k0 : ro.seq.q0;
@@ -349,10 +366,13 @@ __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& o
 #pragma unroll
     for (int j = 0; j < Regs::kWide; ++j) d[j] = 0.0f;
     float rows_d[Regs::kPer];
-    uint32_t m = 0;  // the largest finite magnitude
+    uint32_t m[BY_ROWS ? 4 : 1];
+#pragma unroll
+    for (uint32_t& x : m) x = 0;
 #pragma unroll
     for (int k = 0; k < Regs::kPer; ++k) {
         rows_d[k] = 0.0f;
+        if constexpr (!BY_ROWS) m[0] = 0;
 #pragma unroll
         for (int j = 0; j < Regs::kWide; ++j) {
             int r, f;
@@ -364,28 +384,54 @@ __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& o
             }
             const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
             if (b < 0x7f800000u) {
-                m = max(m, b);
+                m[BY_ROWS ? j : 0] = max(m[BY_ROWS ? j : 0], b);
             } else {
                 v = 0.0f;
                 atomicOr(&odd[r >> 5], 1u << (r & 31));
             }
             if constexpr (BY_ROWS) turn[r][f] = v;
         }
+        if constexpr (!BY_ROWS) {
+            const uint32_t top = lane_max<DP / 8>(m[0]);
+            int r, f;
+            Regs::place(k, 0, r, f);
+            if (f == 0) tops[0][r] = top;
+        }
     }
-    const int e = tile_exponent(block_max(m, most[0]));
+    if constexpr (BY_ROWS) {
+        // sixteen threads share four rows: every sixteenth of a wave, in four waves
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[j] = max(m[j], static_cast<uint32_t>(__shfl_xor(m[j], 16)));
+            m[j] = max(m[j], static_cast<uint32_t>(__shfl_xor(m[j], 32)));
+            if ((t & 63) < 16) tops[t >> 6][4 * (t & 15) + j] = m[j];
+        }
+    }
+    __syncthreads();
+    // a lane a row, in every wave
+    const int lane = t & 63;
+    uint32_t top = tops[0][lane];
+    if constexpr (BY_ROWS) top = max(max(top, tops[1][lane]), max(tops[2][lane], tops[3][lane]));
+    const int e = tile_exponent(lane_max<64>(top));
+    const int own = tile_exponent(top);
+    const bool uneven = __builtin_amdgcn_ballot_w64(top != 0 && own < e - kAttnSpread) != 0;
+    const int row_e = uneven ? own : e;
     const uint64_t bad = static_cast<uint64_t>(odd[1]) << 32 | odd[0];
+    if (t < kAttnRows) op.row_exps[head * op.exps_sh * kAttnRows + padded + t] = row_e;
     if (t == 0) {
-        op.exps[head * op.exps_sh + padded / kAttnRows] = 2 * e + (bad != 0 ? 1 : 0);
+        op.exps[head * op.exps_sh + padded / kAttnRows] =
+            4 * e + (uneven ? 2 : 0) + (bad != 0 ? 1 : 0);
         op.bad[head * op.exps_sh + padded / kAttnRows] = bad;
     }
 
     // rows in pieces of eight features, permuted as they will lie in LDS
-    const float factor = ldexpf(1.0f, kAttnUnit - e);
+    const float even = ldexpf(1.0f, kAttnUnit - e);
     char* const to = op.dst + head * op.dst_sh +
                      static_cast<int64_t>(blockIdx.x) * ((SPLIT ? 2 : 1) * T::kPlane);
 #pragma unroll
     for (int k = 0; k < kAttnRows * T::kPieces / kAttnThreads; ++k) {
         const int i = kAttnThreads * k + t, r = i / T::kPieces, c = i % T::kPieces;
+        const float factor = uneven ? ldexpf(1.0f, kAttnUnit - __shfl(row_e, r)) : even;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -429,7 +475,8 @@ __device__ __forceinline__ void pack_tile(const AttnPack& a, const AttnPackOp& o
                 if (f == 0) put(r, y);
             }
         }
-        const int de = tile_exponent(block_max(largest, most[1]));
+        if (t == 0 && blockIdx.x == 0 && head == 0) *a.clear = 0;
+        const int de = tile_exponent(block_max(largest, most));
         if (t == 0) a.dexps[head * op.exps_sh + padded / kAttnRows] = de;
     }
 }

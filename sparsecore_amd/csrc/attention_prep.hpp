@@ -26,6 +26,7 @@ struct AttnPackOp {
     int64_t dst_sh;
     int32_t* exps;
     uint64_t* bad;
+    int8_t* row_exps;
     int64_t exps_sh, rows;
     int32_t heads, keys, vec;
 };
@@ -43,6 +44,7 @@ struct AttnPack {
     float* lse_out;  // lse, NaN where a row of dO is not finite
     int64_t delta_sh;
     int32_t* dexps;
+    int32_t* clear;  // with delta: set to 0
 };
 
 int attn_launch_plan(const AttnPlanArgs& a, hipStream_t st);

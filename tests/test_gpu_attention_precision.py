@@ -14,7 +14,7 @@ import pytest
 import torch
 
 import sparsecore_amd as slk
-from test_gpu_attention import BF16, F32, Ref, make
+from test_gpu_attention import BF16, F32, Ref, close, feature_major, make
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,112 @@ def test_values_of_different_sizes_behind_lowest_biases(dev, sizes, dtype):
     ref = Ref(torch.zeros_like(q), k, v, do, [(0, t, 0, t)], True, d ** -0.5)
     bias = torch.full((8, h), torch.finfo(F32).min, device=dev)
     rows_close("out", slk.attention(q, k, v, bias=bias, max_distance=20), ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [2.0 ** 30, 1e13, 1e30])
+@pytest.mark.parametrize("at", [0, 63, 90, 149])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("d,buckets", [(64, 0), (128, 16), (32, 0), (40, 8)])
+def test_one_row_much_larger_than_those_around_it(dev, d, buckets, which, at, size, dtype):
+    """What does not see the row, or is not seen by it, is as exact as without it; what does is
+    exact for its own size. (A large key or query: zeros but for a feature that all queries, or
+    keys, have a zero in, so that no score grows.)"""
+    t, h, g = 150, 2, 1
+    q, k, v, do = make((1, t), (1, t), h, g, d, dtype, dev)
+    q[..., 0], k[..., 0] = 0.0, 0.0
+    x = {"q": q, "k": k, "v": v, "dout": do}[which]
+    if which in "qk":
+        x[0, at], x[0, at, :, 0] = 0.0, size
+    else:
+        x[0, at] *= size
+    bias = torch.randn(buckets, h, device=dev).requires_grad_() if buckets else None
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5, bias, 20)
+    leaves = [y.requires_grad_() for y in (q, k, v)]
+    out = slk.attention(*leaves, bias=bias, max_distance=20)
+    grads = torch.autograd.grad(out, leaves + ([bias] if buckets else []), do)
+    for name, y in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        rows_close(name, y, ref, dtype)
+    if buckets:
+        close("dbias", grads[3], ref, dtype)
+    with torch.no_grad():
+        rows_close("out", slk.attention(q, k, v, bias=bias, max_distance=20), ref, dtype)
+
+
+def uneven(x, lo, hi, seed):
+    """Every row times a power of two of its own."""
+    gen = torch.Generator().manual_seed(seed)
+    e = torch.randint(lo, hi + 1, x.shape[:-2], generator=gen).double()
+    return (x.double().cpu() * (2.0 ** e)[..., None, None]).to(x.dtype).to(x.device)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h,g,d,buckets", [(4, 2, 64, 0), (4, 1, 128, 0), (2, 2, 32, 16),
+                                           (3, 3, 128, 16), (4, 2, 50, 0)])
+def test_rows_of_all_sizes_in_packed_sequences(dev, h, g, d, buckets, causal, cols, dtype):
+    lens = [1, 130, 0, 64, 65, 300]
+    n = sum(lens) + 3
+    q, k, v, do = make((n,), (n,), h, g, d, dtype, dev)
+    q, k = uneven(q, -30, 0, 1), uneven(k, -30, 0, 2)
+    v, do = uneven(v, -30, 30, 3), uneven(do, -30, 30, 4)
+    if cols:
+        q, k, v, do = (feature_major(x, (n,)) for x in (q, k, v, do))
+    bias = torch.randn(buckets, h, device=dev) if buckets else None
+    off = torch.tensor([0] + lens).cumsum(0)
+    seqs = [(int(a), m, int(a), m) for a, m in zip(off, lens)]
+    ref = Ref(q, k, v, do, seqs, causal, d ** -0.5, bias)
+    more = {"offsets": off.int().to(dev), "causal": causal, "bias": bias, "feature_major": cols}
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, **more)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        rows_close(name, x, ref, dtype)
+    with torch.no_grad():
+        rows_close("out", slk.attention(q, k, v, **more), ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("buckets", [0, 16])
+def test_rows_of_all_sizes_in_split_keys(dev, buckets, dtype):
+    b, t, s, h, d = 2, 70, 3001, 2, 64
+    q, k, v, do = make((b, t), (b, s), h, 1, d, dtype, dev)
+    k, v = uneven(k, -30, 0, 2), uneven(v, -30, 30, 3)
+    bias = torch.randn(buckets, h, device=dev) if buckets else None
+    ref = Ref(q, k, v, do, [(i * t, t, i * s, s) for i in range(b)], True, d ** -0.5, bias)
+    with torch.no_grad():
+        rows_close("out", slk.attention(q, k, v, bias=bias), ref, dtype)
+
+
+def test_uneven_and_even_calls_in_one_graph(dev):
+    """A captured step replayed with even rows, uneven ones and even ones again."""
+    t, h, d = 300, 2, 64
+    q, k, v, do = make((1, t), (1, t), h, 1, d, F32, dev)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def step(*x):
+        out = slk.attention(*x)
+        return [out.detach(), *torch.autograd.grad(out, x, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*leaves)
+    for i in range(4):
+        new = make((1, t), (1, t), h, 1, d, F32, dev, seed=i + 1)
+        with torch.no_grad():
+            for x, y in zip((q, k, v, do), new):
+                x.copy_(uneven(y, -30, 0, i) if i % 2 else y)
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = [x.clone() for x in got]
+        want = step(*(x.detach().clone().requires_grad_() for x in leaves))
+        assert all(torch.equal(a, b) for a, b in zip(seen, want)), i
+        ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5)
+        for name, x in zip(("out", "dq", "dk", "dv"), seen):
+            rows_close(name, x, ref, F32)
