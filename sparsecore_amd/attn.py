@@ -173,7 +173,7 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
             i serves the query heads i·H/G .. (i + 1)·H/G - 1.
         causal: a sequence's last query stands at its last key: of n queries and m keys,
             query i sees the keys up to i + m - n. Else every query sees every key.
-        scale: factor of the scores, not negative; default D ** -0.5.
+        scale: factor of the scores, 0 to 2e38; default D ** -0.5.
         offsets: (sequences + 1,) int32: packed sequence i is the rows offsets[i] to
             offsets[i + 1] of q, and of k and v unless k_offsets is given.
         lengths: (B,) int32: the first lengths[b] queries of entry b are live, and as many
@@ -198,8 +198,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     2^12 apart (then 1.5 to 1.7 times the time). float32 operands go in two parts: an element
     is off by at most 2^-22 of itself or 2^-27 of the largest of its row, about float32's own
     rounding. bfloat16 ones are exact down to 2^-19 of that. Between the products weights and
-    their gradients are rounded to 22 bits (bfloat16: 11) down to 2^-32 of the largest that
-    their row of results has. Softmax and sums are float32, in a fixed order: results
+    the scores' gradients are rounded to 22 bits (bfloat16: 11), or to 2^-32 of the largest
+    of their row of results where that is more (in dv to 2^-39 of 1). Softmax and sums are float32, in a fixed order: results
     repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
     packed (not the tensors themselves), and the output, which must not change in place
     before the backward, nor may offsets and lengths; of a bfloat16 output also what its

@@ -390,8 +390,9 @@ int check(const slk_attention* args, const char* who, bool backward) {
         return fail(SLK_EINVAL, w + ": heads must be a multiple of kv_heads, at most 16384, got " +
                                     std::to_string(a.heads) + " and " +
                                     std::to_string(a.kv_heads));
-    if (!(a.scale >= 0.0) || !(a.scale <= 3e38))
-        return fail(SLK_EINVAL, w + ": scale must be finite and not negative");
+    // times log2 e it is a float32
+    if (!(a.scale >= 0.0) || !(a.scale <= 2e38))
+        return fail(SLK_EINVAL, w + ": scale must be finite and not negative, at most 2e38");
     if (packed_rows(a) && (a.q_lengths != nullptr || a.k_lengths != nullptr))
         return fail(SLK_EINVAL, w + ": offsets or lengths, not both");
     if (!packed_rows(a) && a.k_offsets != nullptr)

@@ -44,3 +44,11 @@ def test_largest_sizes_are_counted():
     # two parts of 2 bytes an element
     assert lib.slk_attention_saved_bytes(ctypes.byref(a)) >= 4 * 128 * (16384 + 2) << 29
     assert lib.slk_attention_scratch_bytes(ctypes.byref(a), 1) >= 4 * 128 * 16384 << 29
+
+
+def test_scales_that_leave_float32_are_refused():
+    lib = _lib.load()
+    for scale in (3e38, 2.1e38, 1e300):
+        a = arguments(scale=scale)
+        assert lib.slk_attention_forward(ctypes.byref(a), None) == _lib.SLK_EINVAL
+        assert b"scale" in lib.slk_last_error()
