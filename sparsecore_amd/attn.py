@@ -199,8 +199,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
     is off by at most 2^-22 of itself or 2^-27 of the largest of its row, about float32's own
     rounding. bfloat16 ones are exact down to 2^-19 of that. Between the products weights and
     the scores' gradients are rounded to 22 bits (bfloat16: 11), or to 2^-32 of the largest
-    of their row of results where that is more (in dv to 2^-39 of 1). Softmax and sums are float32, in a fixed order: results
-    repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
+    of their row of results where that is more (in dv to 2^-39 of 1). Softmax and sums are
+    float32, in a fixed order: results repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,
     packed (not the tensors themselves), and the output, which must not change in place
     before the backward, nor may offsets and lengths; of a bfloat16 output also what its
     rounding took off, in two bytes an element.

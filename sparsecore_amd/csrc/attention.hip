@@ -148,7 +148,11 @@ Few few_of(const slk_attention& a) {
     return f;
 }
 
-// Parts of the keys in the tiled forward: where the query tiles leave CUs idle.
+// Parts of the keys in the tiled forward, where the query tiles leave CUs idle: two rounds
+// of workgroups, parts of 256 keys or more. 128 x 8192 keys, 8 heads of 128, bfloat16: 45 us,
+// unsplit 182; 1001 causal tokens, 12 heads of 64, float32: 37, unsplit 43, one round 40, parts
+// of 128 keys 34 (but 54 for the first), of 512 keys 43; 512 tokens, 8 heads of 64, bfloat16:
+// 23, unsplit 21, the join's price.
 int splits_of(const slk_attention& a, const Sizes& s) {
     if (a.keep) return 1;
     const int64_t groups = s.q_entries * a.heads;
@@ -196,8 +200,10 @@ Forward forward_of(const slk_attention& a, void* scratch) {
 
 // Parts of a group's query heads in the keys' gradients: where the keys' tiles
 // leave CUs idle, the heads go to workgroups of their own, whose sums are joined.
-// 8191 packed tokens, 16 heads over 4, 128 wide, bf16: two parts took 0.62 of one
-// part's time, the join counted, four 0.45 (106 us + 25 for the join).
+// Backward without dq, bfloat16, parts until there are four workgroups a CU: 8191 causal
+// tokens, 16 heads over 4 of 128: 1113 us, 2098 in one part, 1355 with two a CU, 1102 with
+// eight; 8 x 1024, 16 over 4 of 64: 139, 193, 145, 140; float32, 4 x 512, 16 over 2 of 64:
+// 80, 264, 81, 80. The join of 8191 packed tokens' parts, 4 heads of 128: 25 us.
 int dkv_parts(const slk_attention& a, const Sizes& s) {
     const int64_t rep = a.heads / a.kv_heads, groups = s.k_entries * a.kv_heads;
     int64_t parts = 1;

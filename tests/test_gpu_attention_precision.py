@@ -277,3 +277,25 @@ def test_uneven_and_even_calls_in_one_graph(dev):
         ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5)
         for name, x in zip(("out", "dq", "dk", "dv"), seen):
             rows_close(name, x, ref, F32)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("b,t,h,g,d,buckets", [(200, 4, 2, 1, 64, 0), (100, 9, 2, 2, 128, 0),
+                                               (100, 7, 2, 2, 32, 8), (3, 150, 4, 2, 64, 0),
+                                               (2, 300, 2, 1, 128, 16)])
+def test_bfloat16_is_rounded_to_11_bits_between_the_products(dev, b, t, h, g, d, buckets, causal):
+    """A result is rounded to bfloat16, half a step: 2^-8 of it. A weight, or dS, is rounded to
+    float16: 2^-11 of each term. O as it is read by the backward is off by 2^-8 of 2^-8 of it,
+    scores and sums by what float32 has (1e-5 of a term, see test_gpu_attention.py): 2^-14 of
+    each term covers both. (Weights or O in bfloat16 would be off by 2^-8 of the terms.)"""
+    q, k, v, do = make((b, t), (b, t), h, g, d, BF16, dev)
+    bias = torch.randn(buckets, h, device=dev) if buckets else None
+    ref = Ref(q, k, v, do, [(i * t, t, i * t, t) for i in range(b)], causal, d ** -0.5, bias)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves, causal=causal, bias=bias)
+    half = torch.finfo(BF16).eps / 2
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        want, mag = ref.val[name], ref.mag[name]
+        got = x.detach().double().cpu().reshape(want.shape)
+        off = (got - want).abs() - half * want.abs() - (2.0 ** -11 + 2.0 ** -14) * mag
+        assert float(off.max()) <= 0, (name, float(off.max()))
