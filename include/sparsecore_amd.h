@@ -935,9 +935,9 @@ typedef struct slk_attn_tensor {
  * A row with a value that is not finite makes NaN of the results that it has a
  * part in.
  * Products run on the float16 matrix instructions, 64 rows of a head scaled by a
- * power of two, or each row where they are more than 2^12 apart: float32 in two
- * parts an operand (an element off by 2^-22 of itself or 2^-27 of its row's
- * largest), bf16 exact down to 2^-19 of that; weights and scores' gradients in 22
+ * power of two, or each row where they are more than 2^14 apart: float32 in two
+ * parts an operand (an element off by 2^-22 of itself or 2^-25 of its row's
+ * largest), bf16 exact down to 2^-17 of that; weights and scores' gradients in 22
  * bits (bf16: 11) or to 2^-32 of the largest of their row of results (in dv to
  * 2^-39 of 1). Softmax statistics and sums are float32, in a
  * fixed order.

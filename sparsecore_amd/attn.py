@@ -195,9 +195,9 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
 
     Products run on the matrix cores' float16 instructions, each block of 64 rows of a head
     scaled by a power of two of its own, or each row where the block's rows are more than
-    2^12 apart (then 1.5 to 1.7 times the time). float32 operands go in two parts: an element
-    is off by at most 2^-22 of itself or 2^-27 of the largest of its row, about float32's own
-    rounding. bfloat16 ones are exact down to 2^-19 of that. Between the products weights and
+    2^14 apart (then 1.5 to 1.7 times the time). float32 operands go in two parts: an element
+    is off by at most 2^-22 of itself or 2^-25 of the largest of its row, about float32's own
+    rounding. bfloat16 ones are exact down to 2^-17 of that. Between the products weights and
     the scores' gradients are rounded to 22 bits (bfloat16: 11), or to 2^-32 of the largest
     of their row of results where that is more (in dv to 2^-39 of 1). Softmax and sums are
     float32, in a fixed order: results repeat bit for bit. A forward that a backward may follow keeps q, k and v once more,

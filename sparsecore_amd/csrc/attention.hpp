@@ -22,7 +22,7 @@
 // A tile with a row whose largest element is 2^-kAttnSpread or less of the tile's is
 // uneven: each of its rows has an exponent of its own, so that no row, least of all one
 // that others do not see, takes bits off another: an element is then off by 2^-22 of
-// itself or 2^-27 of its row's largest (bfloat16: exact down to 2^-19 of that). A
+// itself or 2^-25 of its row's largest (bfloat16: exact down to 2^-17 of that). A
 // workgroup that meets such a tile takes a second form of its loop, which applies
 // exponents row by row. 16384 tokens, 32 heads over 8 of 128, bfloat16, all tiles uneven:
 // forward 4.0 ms in place of 2.4, backward 12.6 in place of 8.3; the look at the tiles'
@@ -44,7 +44,7 @@ constexpr int kAttnTileRows = 128; // rows of a workgroup of the tiled kernels
 constexpr int kAttnThreads = 256;
 constexpr int kAttnMaxSplits = 128;  // parts of the keys
 constexpr int kAttnUnit = 14;     // a packed tile's largest element is in 2^[14, 15)
-constexpr int kAttnSpread = 12;   // of the exponents of an even tile's rows
+constexpr int kAttnSpread = 14;   // of the exponents of an even tile's rows
 constexpr int kUnset = -100000;   // the exponent of a row's unit before it has seen anything
 constexpr float kLog2e = 1.44269504088896340736f;
 

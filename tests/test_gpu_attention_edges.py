@@ -1,4 +1,4 @@
-"""attention at its edges: calls without queries, whose keys' and biases' gradients are zeros."""
+"""attention at its edges: calls without queries or without keys, and some of the gradients."""
 
 from __future__ import annotations
 
@@ -89,3 +89,48 @@ def test_no_queries_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all((x == 0).all() for x in got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mode", ["whole", "k_lengths", "packed"])
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_no_keys_in_any_layout(dev, mode, buckets, dtype):
+    leave_garbage(dev)
+    b, t, h, d = 3, 70, 2, 32
+    lead_q, lead_k = ((b * t,), (0,)) if mode == "packed" else ((b, t), (b, 0))
+    q = torch.randn(*lead_q, h, d, device=dev).to(dtype).requires_grad_()
+    k, v = (torch.randn(*lead_k, 1, d, device=dev).to(dtype).requires_grad_() for _ in range(2))
+    bias = torch.randn(buckets, h, device=dev, requires_grad=True) if buckets else None
+    zeros = torch.zeros(4, dtype=torch.int32, device=dev)
+    more = {"whole": {}, "k_lengths": {"k_lengths": zeros[:3]},
+            "packed": {"offsets": torch.tensor([3, t, t, 2 * t], dtype=torch.int32, device=dev),
+                       "k_offsets": zeros}}[mode]
+    out = slk.attention(q, k, v, bias=bias, max_distance=20, **more)
+    assert (out == 0).all()
+    leaves = [q, k, v] + ([bias] if buckets else [])
+    for x, y in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), leaves):
+        assert x.shape == y.shape and (x == 0).all()
+
+
+@pytest.mark.parametrize("uneven", [False, True])
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (3,), (1, 2), (0, 3)])
+def test_some_of_the_gradients(dev, wanted, uneven):
+    """Any of them alone has the bits that it has among all."""
+    t, h, d = 200, 4, 64
+    gen = torch.Generator().manual_seed(0)
+    q, k, v, bias = (torch.randn(*s, generator=gen) for s in ((1, t, h, d), (1, t, 2, d),
+                                                              (1, t, 2, d), (8, h)))
+    if uneven:
+        q[:, ::7] *= 2.0 ** -20
+        v[:, ::5] *= 2.0 ** 20
+    do = torch.randn(1, t, h, d, generator=gen).to(dev)
+    leaves = [x.to(dev) for x in (q, k, v, bias)]
+
+    def grads(of):
+        x = [y.clone().requires_grad_(i in of) for i, y in enumerate(leaves)]
+        out = slk.attention(*x[:3], bias=x[3], max_distance=20)
+        return torch.autograd.grad(out, [x[i] for i in of], do)
+
+    among_all = grads((0, 1, 2, 3))
+    for i, x in zip(wanted, grads(wanted)):
+        assert torch.equal(x, among_all[i]), i

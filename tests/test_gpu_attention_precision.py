@@ -299,3 +299,18 @@ def test_bfloat16_is_rounded_to_11_bits_between_the_products(dev, b, t, h, g, d,
         got = x.detach().double().cpu().reshape(want.shape)
         off = (got - want).abs() - half * want.abs() - (2.0 ** -11 + 2.0 ** -14) * mag
         assert float(off.max()) <= 0, (name, float(off.max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("least", [-10, -12, -14, -16])
+def test_rows_about_as_far_apart_as_one_power_of_two_serves(dev, least, dtype):
+    """On both sides of the spread from which rows have exponents of their own."""
+    t, h, d = 300, 2, 64
+    q, k, v, do = make((1, t), (1, t), h, 1, d, dtype, dev)
+    q, k = uneven(q, least, 0, 1), uneven(k, least, 0, 2)
+    v, do = uneven(v, least, 0, 3), uneven(do, least, 0, 4)
+    ref = Ref(q, k, v, do, [(0, t, 0, t)], True, d ** -0.5)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = slk.attention(*leaves)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do))):
+        rows_close(name, x, ref, dtype)
