@@ -245,6 +245,17 @@ attn_dkv_kernel(const AttnArgs g) {
             // the lane's key is seen by rows [from, to) of a block
             auto seen_from = [&](int q0) { return g.causal ? max(key - shift - q0, 0) : 0; };
             auto seen_to = [&](int q0) { return key < seq.nk ? min(seq.nq - q0, 32) : 0; };
+            // A row that sees one key alone, the sequence's first, has weight 1 there and dS 0,
+            // not what roundings leave of dP - delta (what is not finite stays so).
+            auto single_key = [&](int k) {
+                return seq.nk == 1 || (g.causal && k == 0);
+            };
+            auto only_key = [&](float* x, int r0, int q0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (seq.nk == 1 || (key == 0 && q0 + attn_row(r0 + i, lane) + shift == 0))
+                        x[i] *= 0.0f;
+            };
             auto move = [&](int to) __attribute__((always_inline)) {  // dK's unit
                 const float f = attn_pow2(cq - to);
                 scale_sums(dk, f);
@@ -331,8 +342,16 @@ attn_dkv_kernel(const AttnArgs g) {
                         p[r] = see ? p[r] : 0.0f;
                         ds[r] = see ? ds[r] : 0.0f;
                         if (p[r] != 0.0f) most_o = max(most_o, dr);
-                        if (ds[r] != 0.0f) most = max(most, attn_exponent(ds[r]) + qr);
                     }
+                    if (single_key(key0)) {
+                        only_key(ds, 0, q0);
+                        only_key(ds + 8, 8, q0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (ds[r] != 0.0f)
+                            most = max(most,
+                                       attn_exponent(ds[r]) + attn_one_of(qx[r / 4], r % 4));
                     most_o = max(max(most_o, __shfl_xor(most_o, 32)), co);
                     scale_sums(dv, attn_pow2(co - most_o));
                     co = most_o;
@@ -376,6 +395,7 @@ attn_dkv_kernel(const AttnArgs g) {
                             p[i] = see ? p[i] : 0.0f;
                             ds[8 * half + i] = see ? ds[8 * half + i] : 0.0f;
                         }
+                        if (single_key(key0)) only_key(ds + 8 * half, 8 * half, q0);
                     }
                     wp[0][half] = attn_operand<SPLIT>(p);
                 }
@@ -508,6 +528,9 @@ attn_dq_kernel(const AttnArgs g) {
     float* const far = lds_floats + 4 * kDiags * kDiagRow;  // [wave][below, above]
     float* const bias_row = far + 8;
     float* const bins = bias_row + attn_bias_floats(md);  // [wave][distance]
+    // Of a single key that a query sees the weight is 1 and dS 0, not what roundings leave of
+    // dP - delta (what is not finite stays so).
+    auto sees_one = [&]() { return seq.nk == 1 || (g.causal && q + shift == 0); };
     const int d_row = min(lane, kDiags - 1);
     float below = 0.0f, above = 0.0f;            // distances past the last bins
     if constexpr (BIAS) {
@@ -658,6 +681,10 @@ attn_dq_kernel(const AttnArgs g) {
                     for (int r = 0; r < 16; ++r)
                         ds[r] = attn_row(r, lane) <= lim ? ds[r] : 0.0f;
                 }
+                if (BIAS && key0 == 0 && sees_one()) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] *= 0.0f;
+                }
                 if constexpr (BIAS) {
                     if (near) {
                         // eight keys at a time: lane d sums the diagonal of distance
@@ -750,7 +777,9 @@ attn_dq_kernel(const AttnArgs g) {
 
     if (q < seq.eq && g.dq.p != nullptr) {
         const bool zero = q >= seq.nq || t1 == 0;
-        const float f = zero ? 1.0f : ldexpf(g.scale, ck - 2 * kAttnUnit);
+        const float f = zero         ? 1.0f
+                        : sees_one() ? 0.0f
+                                     : ldexpf(g.scale, ck - 2 * kAttnUnit);
         const int64_t at = sid * g.dq.sb + (seq.q0 + q) * g.dq.sr + head * g.dq.sh;
         const bool vec = g.dq.sd == 1 && g.vec_q;
 #pragma unroll

@@ -134,3 +134,42 @@ def test_some_of_the_gradients(dev, wanted, uneven):
     among_all = grads((0, 1, 2, 3))
     for i, x in zip(wanted, grads(wanted)):
         assert torch.equal(x, among_all[i]), i
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("mode,t,s", [("batch", 1, 1), ("batch", 70, 1), ("batch", 150, 150),
+                                      ("batch", 100, 40), ("packed", 35, 35), ("lengths", 9, 9)])
+@pytest.mark.parametrize("uneven", [False, True])
+def test_rows_that_see_a_single_key(dev, mode, t, s, causal, uneven, dtype):
+    """Their weight is 1 whatever the scores are: no gradient goes to the query, none through
+    it to the key or to the bias. Exactly none."""
+    gen = torch.Generator().manual_seed(0)
+    h, d, b = 2, 64, 1 if mode == "packed" else 3
+    lead_q, lead_k = ((t,), (s,)) if mode == "packed" else ((b, t), (b, s))
+    q, do = (torch.randn(*lead_q, h, d, generator=gen).to(dtype).to(dev) for _ in range(2))
+    k, v = (torch.randn(*lead_k, 1, d, generator=gen).to(dtype).to(dev) for _ in range(2))
+    if uneven:
+        v[..., 0, 0, :] *= 2.0 ** 30
+        do[..., -1, :, :] *= 2.0 ** -30
+    bias = torch.randn(8, h, generator=gen).to(dev)
+    more = {"packed": {"offsets": torch.arange(t + 1, dtype=torch.int32, device=dev)},
+            "lengths": {"k_lengths": torch.ones(b, dtype=torch.int32, device=dev),
+                        "lengths": torch.full((b,), t, dtype=torch.int32, device=dev)},
+            "batch": {}}[mode]
+    leaves = [x.requires_grad_() for x in (q, k, v, bias)]
+    out = slk.attention(q, k, v, bias=bias, causal=causal, max_distance=20, **more)
+    dq, dk, dv, dbias = torch.autograd.grad(out, leaves, do)
+    if mode == "packed" or mode == "lengths" or s == 1:
+        assert (dq == 0).all() and (dk == 0).all() and (dbias == 0).all()
+    elif causal:
+        first = max(0, t - s)  # the first query that sees a key
+        assert (dq[:, :first + 1] == 0).all() and not (dq[:, first + 1:] == 0).all()
+        # what that query leaves the first key: nothing but by its value
+        do2 = do.clone()
+        do2[:, first] *= 3.0
+        other = torch.autograd.grad(slk.attention(q, k, v, bias=bias, max_distance=20, **more),
+                                    leaves, do2)
+        assert torch.equal(dq, other[0]) and not torch.equal(dv, other[2])
+        torch.testing.assert_close(dk[:, 0], other[1][:, 0], rtol=2 ** -7, atol=1e-6)
+    assert not (dv == 0).all()
