@@ -931,7 +931,8 @@ typedef struct slk_attn_tensor {
  *              further ones. causal: all buckets are for d >= 0; else the first
  *              half is, and the second half for d < 0.
  * A query that sees no key, and a row of no sequence, has output 0 and gradient
- * 0. What is masked reaches nothing, whatever it holds.
+ * 0; one that sees a single key has gradient 0, and leaves it that of its value
+ * alone. What is masked reaches nothing, whatever it holds.
  * A row with a value that is not finite makes NaN of the results that it has a
  * part in.
  * Products run on the float16 matrix instructions, 64 rows of a head scaled by a

@@ -187,7 +187,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, offse
             are rows), as a SparseLinear takes it without a copy.
 
     Returns q's shape. A query that sees no key has output 0 and no gradient, and so has a
-    row that belongs to no sequence; what is masked reaches nothing, whatever it holds. A row
+    row that belongs to no sequence; of one that sees a single key only the value has a
+    gradient; what is masked reaches nothing, whatever it holds. A row
     of q, k, v or of the output's gradient with a value that is not finite makes NaN of the
     results that its row has a part in (for few queries without gradients, of what the value
     itself reaches). Offsets and lengths are read on the device: those out of range, or
